@@ -43,6 +43,20 @@ class dllm_config(C.Structure):
     ]
 
 
+class dllm_rope_config(C.Structure):
+    _fields_ = [
+        ("layout", C.c_int32), ("rotary_dim", C.c_int32), ("theta", C.c_double), ("scaling", C.c_int32),
+        ("factor", C.c_double), ("original_max_pos", C.c_int32), ("beta_fast", C.c_double), ("beta_slow", C.c_double),
+        ("attention_factor", C.c_double),
+    ]
+
+
+class dllm_pick(C.Structure):
+    _fields_ = [("n", C.c_int32)] + [(name, C.c_void_p) for name in (
+        "logits", "history", "history_offsets", "prompt_lens", "penalties", "bias_tokens", "bias_values",
+        "bias_offsets", "mask", "tree", "draft", "out", "tokens")]
+
+
 P = C.c_void_p
 I32P = C.POINTER(C.c_int32)
 F32P = C.POINTER(C.c_float)
@@ -124,6 +138,20 @@ SIGNATURES = {
     "dllm_pipeline_synchronize": (C.c_int, [P, C.c_int]),
     "dllm_pipeline_set_host_tokens": (C.c_int, [P, C.c_int]),
     "dllm_pipeline_run_micro": (C.c_int, [P, C.c_int, I32P, I32P]),
+    "dllm_create_i32": (C.c_int, [P, C.c_size_t, C.c_char_p, PP]),
+    "dllm_write_i32": (C.c_int, [P, P, I32P, C.c_size_t]),
+    "dllm_read_i32": (C.c_int, [P, P, I32P, C.c_size_t]),
+    "dllm_rope_plan_create": (C.c_int, [P, C.POINTER(dllm_rope_config), PP]),
+    "dllm_rope_plan_destroy": (None, [P]),
+    "dllm_rope_at": (C.c_int, [P, P, P, C.c_int, P, P, P, P]),
+    "dllm_tree_create": (C.c_int, [P, I32P, I32P, I32P, C.c_int, PP]),
+    "dllm_tree_destroy": (None, [P]),
+    "dllm_pick_tokens": (C.c_int, [P, C.POINTER(dllm_pick)]),
+    "dllm_stage_append_tree": (C.c_int, [P, C.c_int, P, P, P]),
+    "dllm_stage_tree_attention": (C.c_int, [P, C.c_int, P, P, P]),
+    "dllm_stage_commit_tree": (C.c_int, [P, P, I32P, I32P]),
+    "dllm_stage_forward_tree": (C.c_int, [P, P, P, P, P]),
+    "dllm_stage_kv_device_ptr": (P, [P, C.c_int]),
     "dllm_attention_noalloc": (C.c_int, [P, P, P, P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, P]),
     "dllm_attention_noalloc_status": (C.c_int, [P, C.c_int, I32P]),
 }

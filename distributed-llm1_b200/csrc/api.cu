@@ -23,6 +23,7 @@
 #include "kernels.cuh"
 #include "ops.cuh"
 #include "stage.cuh"
+#include "verify.cuh"
 
 using dllm::KvLayout;
 using dllm::LayerW;
@@ -46,7 +47,7 @@ struct dllm_buf {
   void* ptr = nullptr;
   size_t bytes = 0;
   size_t n = 0;    // elements
-  int dtype = 0;   // 0 fp32, 1 bf16
+  int dtype = 0;   // 0 fp32, 1 bf16, 2 int32
   int refs = 1;
   std::string label;
 };
@@ -75,6 +76,8 @@ struct dllm_ctx {
   int tc_min_rows = dllm::kTcMinRows;
   void* tc_scratch = nullptr;
   size_t tc_scratch_bytes = 0;
+  // partial results of split tree attention, sized for any call; allocated with the first tree
+  float* tree_part = nullptr;
   // freed buffers kept for reuse, by size in bytes
   std::multimap<size_t, void*> buf_cache;
   size_t buf_cache_bytes = 0;
@@ -124,6 +127,24 @@ struct dllm_stage {
   unsigned long long* trace = nullptr;
   int trace_cap = 0;
   int version = 0;  // bumped when weights or tracing change (captured graphs rebuild)
+};
+
+// A drafted tree per sequence: nodes in batch rows, parents before children.
+struct dllm_tree {
+  dllm_ctx* ctx = nullptr;
+  int n = 0, n_seqs = 0, max_m = 0;
+  std::vector<dllm::TreeSeq> seqs;
+  std::vector<int> parents, depth;  // [n], indices within the sequence
+  dllm_buf* dev = nullptr;          // TreeSeq[n_seqs], then ancestor masks u64[n]
+  const dllm::TreeSeq* seqs_dev() const { return (const dllm::TreeSeq*)dev->ptr; }
+  const unsigned long long* anc_dev() const { return (const unsigned long long*)(seqs_dev() + n_seqs); }
+};
+
+struct dllm_rope_plan {
+  dllm_ctx* ctx = nullptr;
+  int rotary = 0, interleaved = 0;
+  float factor = 1.f;
+  dllm_buf* turns = nullptr;  // double[rotary / 2] (held as int32 words)
 };
 
 struct dllm_leader {
@@ -245,6 +266,13 @@ int check_bf16(dllm_ctx* c, const dllm_buf* b, size_t need, const char* what) {
   return DLLM_OK;
 }
 
+int check_i32(dllm_ctx* c, const dllm_buf* b, size_t need, const char* what) {
+  if (!valid_buf(c, b)) return set_err(c, DLLM_EINVAL, "%s: null or foreign buffer", what);
+  if (b->dtype != 2) return set_err(c, DLLM_EINVAL, "%s: expected an i32 buffer", what);
+  if (b->n < need) return set_err(c, DLLM_EINVAL, "%s: buffer holds %zu integers, need %zu", what, b->n, need);
+  return DLLM_OK;
+}
+
 // Buffers of a ctx come from, and return to, a per-ctx cache of freed device
 // blocks keyed by size: the op outputs of a forward (one per op, as the reference
 // creates them, kernels.js:222-301) then cost no cudaMalloc/cudaFree (which can
@@ -269,7 +297,7 @@ int new_buf(dllm_ctx* c, size_t n, int dtype, const char* label, dllm_buf** out,
   b->device = c->device;
   b->n = n;
   b->dtype = dtype;
-  b->bytes = n * (dtype == 0 ? 4 : 2);
+  b->bytes = n * (dtype == 1 ? 2 : 4);
   b->label = label ? label : "";
   b->ptr = cache_take(c, b->bytes);
   if (!b->ptr) {
@@ -277,7 +305,7 @@ int new_buf(dllm_ctx* c, size_t n, int dtype, const char* label, dllm_buf** out,
     if (e != cudaSuccess) {
       cudaGetLastError();
       delete b;
-      return set_err(c, DLLM_ENOMEM, "cudaMalloc(%zu bytes, %s): %s", n * (dtype == 0 ? 4 : 2), label ? label : "",
+      return set_err(c, DLLM_ENOMEM, "cudaMalloc(%zu bytes, %s): %s", n * (dtype == 1 ? 2 : 4), label ? label : "",
                      cudaGetErrorString(e));
     }
   }
@@ -611,6 +639,76 @@ int ensure_wide(dllm_stage* s, int rows, bool logits) {
   return DLLM_OK;
 }
 
+// ---- drafted trees ------------------------------------------------------------------------
+// Calls that allocate or wait for the stream cannot be part of a captured graph.
+int refuse_capture(dllm_ctx* c, const char* what) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  CK(c, cudaStreamIsCapturing(c->stream, &st));
+  if (st != cudaStreamCaptureStatusNone)
+    return set_err(c, DLLM_EINVAL, "%s: not possible while the ctx stream is being captured", what);
+  return DLLM_OK;
+}
+
+// Uploads host bytes into a fresh buffer and waits for the copy, so that the buffer
+// may then be used on any stream.
+int upload(dllm_ctx* c, const void* src, size_t bytes, const char* label, dllm_buf** out) {
+  dllm_buf* b = nullptr;
+  if (int rc = new_buf(c, (bytes + 3) / 4, 2, label, &b, false)) return rc;
+  cudaError_t e = cudaMemcpyAsync(b->ptr, src, bytes, cudaMemcpyHostToDevice, c->stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
+  if (e != cudaSuccess) {
+    dllm_buf_free(b);
+    return set_err(c, DLLM_ECUDA, "%s upload: %s", label, cudaGetErrorString(e));
+  }
+  *out = b;
+  return DLLM_OK;
+}
+
+// The T0 of every sequence of a tree, with room for its nodes behind it.
+int tree_t0(dllm_stage* s, const dllm_tree* tree, const char* what, dllm::TreeT0* t0) {
+  dllm_ctx* c = s->ctx;
+  if (!tree || tree->ctx != c) return set_err(c, DLLM_EINVAL, "%s: null or foreign tree", what);
+  for (int i = 0; i < tree->n_seqs; ++i) {
+    const dllm::TreeSeq& q = tree->seqs[i];
+    if (q.seq >= s->max_seqs) return set_err(c, DLLM_EINVAL, "%s: invalid seq %d", what, q.seq);
+    if (s->T0[q.seq] + q.m > s->max_slots)
+      return set_err(c, DLLM_ERANGE, "%s: seq %d T0=%d + %d nodes > maxPos=%d", what, q.seq, s->T0[q.seq], q.m,
+                     s->max_slots);
+    t0->t0[i] = s->T0[q.seq];
+  }
+  return DLLM_OK;
+}
+
+int tree_layer(dllm_stage* s, int layer, const char* what) {
+  if (layer < s->start || layer >= s->end) return set_err(s->ctx, DLLM_EINVAL, "%s: layer %d not in stage", what, layer);
+  return DLLM_OK;
+}
+
+int tree_attention(dllm_stage* s, int layer, const dllm_tree* tree, const dllm::TreeT0& t0, const float* q, float* out) {
+  dllm_ctx* c = s->ctx;
+  const dllm_config& f = c->cfg;
+  dllm::TreeAttnArgs a{};
+  a.q = q;
+  a.out = out;
+  a.kc = layer_pool(s, s->kpool, layer);
+  a.vc = layer_pool(s, s->vpool, layer);
+  a.kv = stage_kv(s);
+  a.seqs = tree->seqs_dev();
+  a.anc = tree->anc_dev();
+  a.n_seqs = tree->n_seqs;
+  a.nq = f.num_q_heads;
+  a.kvh = f.num_kv_heads;
+  a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)f.head_dim));
+  a.part_o = c->tree_part;
+  a.part_ml = c->tree_part + dllm::tree_attn_part_rows(c->sms) * f.head_dim;
+  const dllm::TreeAttnShape shape{tree->seqs.data(), t0.t0, tree->n, tree->max_m};
+  int launches = 0;
+  const cudaError_t e = dllm::op_tree_attention(a, shape, f.kv_dtype, f.head_dim, c->sms, &launches, c->stream);
+  c->launches += launches;
+  if (e != cudaSuccess) return set_err(c, DLLM_ECUDA, "tree attention launch: %s", cudaGetErrorString(e));
+  return DLLM_OK;
+}
+
 // A wide pass of n rows (rd[t] = {seq, pos, slot}) over the stage's layers, one
 // kernel per op: RMSNorm + q|k|v projections on the tensor cores, bias + RoPE +
 // appendKv, attention over the paged cache, o_proj + residual, RMSNorm + gate|up,
@@ -618,7 +716,10 @@ int ensure_wide(dllm_stage* s, int rows, bool logits) {
 // tokens_in the rows start as token embeddings (pipeline.js:121-128); with
 // tokens_out each row ends with final norm + LM head + greedy argmax
 // (pipeline.js:141-174).
-int run_wide(dllm_stage* s, float* h, int n, const RowDesc* rd, const int32_t* tokens_in, int32_t* tokens_out) {
+// A tree pass (`tree`, n <= kTcMaxRows rows) attends with the tree's mask instead of
+// the rows' slots, and `logits` receives the LM head's rows.
+int run_wide(dllm_stage* s, float* h, int n, const RowDesc* rd, const int32_t* tokens_in, int32_t* tokens_out,
+             const dllm_tree* tree = nullptr, const dllm::TreeT0* t0 = nullptr, float* logits = nullptr) {
   dllm_ctx* c = s->ctx;
   const dllm_config& f = c->cfg;
   const int D = f.hidden_size, QD = f.num_q_heads * f.head_dim, KD = f.num_kv_heads * f.head_dim,
@@ -639,15 +740,23 @@ int run_wide(dllm_stage* s, float* h, int n, const RowDesc* rd, const int32_t* t
       if (int rc = tc_rows_multi(c, hh, m, D, qkv, 3, L.ln1)) return rc;
       CK(c, dllm::op_qkv_post(s->wq, s->wk, s->wv, L.bq, L.bk, L.bv, m, f.num_q_heads, f.num_kv_heads, f.head_dim,
                               c->freq, s->wrows, kv, L.kc, L.vc, f.kv_dtype, c->err_dev, c->stream));
-      const dllm::AttnArgs A{s->wq, s->watt, L.kc, L.vc, kv, s->wrows, m, f.num_q_heads, f.num_kv_heads, c->scale,
-                             s->wide_splits, s->wpart_o, s->wpart_ml, s->warrive, c->err_dev};
-      CK(c, dllm::op_attention_paged(A, f.kv_dtype, f.head_dim, c->sms, c->stream));
+      if (tree) {
+        if (int rc = tree_attention(s, s->start + l, tree, *t0, s->wq, s->watt)) return rc;
+      } else {
+        const dllm::AttnArgs A{s->wq, s->watt, L.kc, L.vc, kv, s->wrows, m, f.num_q_heads, f.num_kv_heads, c->scale,
+                               s->wide_splits, s->wpart_o, s->wpart_ml, s->warrive, c->err_dev};
+        CK(c, dllm::op_attention_paged(A, f.kv_dtype, f.head_dim, c->sms, c->stream));
+        c->launches += 1;
+      }
       if (int rc = tc_rows(c, s->watt, m, QD, L.wo, D, hh, 1, nullptr)) return rc;
       const dllm::TcTarget gu[2] = {{L.wg, I, s->wg, 0}, {L.wu, I, s->wu, 0}};
       if (int rc = tc_rows_multi(c, hh, m, D, gu, 2, L.ln2)) return rc;
       CK(c, dllm::op_silu_mul(s->wg, s->wu, s->wg, m * I, c->stream));
       if (int rc = tc_rows(c, s->wg, m, I, L.wd, D, hh, 1, nullptr)) return rc;
-      c->launches += 3;
+      c->launches += 2;
+    }
+    if (logits) {
+      if (int rc = tc_rows(c, hh, m, D, s->lm_head, f.vocab_size, logits, 0, s->norm)) return rc;
     }
     if (tokens_out) {
       if (int rc = tc_rows(c, hh, m, D, s->lm_head, f.vocab_size, s->wlogits, 0, s->norm)) return rc;
@@ -736,6 +845,7 @@ void ctx_free(dllm_ctx* c) {
   dev_free(c->attn.arrive);
   dev_free(c->attn_rows);
   dev_free(c->tc_scratch);
+  dev_free(c->tree_part);
   for (auto& kv : c->buf_cache) cudaFree(kv.second);
   c->buf_cache.clear();
   if (c->err_host) cudaFreeHost(c->err_host);
@@ -811,7 +921,8 @@ int dllm_init_kernels(int device, const dllm_config* cfg, dllm_ctx** out) {
   if (cudaGetDeviceProperties(&prop, device) != cudaSuccess) return fail(DLLM_ECUDA);
   if (prop.major < 10) return fail(DLLM_EDEVICE);  // built for sm_100a only
   c->sms = prop.multiProcessorCount;
-  if (dllm::configure_stage_kernels() != cudaSuccess || dllm::configure_op_kernels() != cudaSuccess) {
+  if (dllm::configure_stage_kernels() != cudaSuccess || dllm::configure_op_kernels() != cudaSuccess ||
+      dllm::configure_pick_kernels() != cudaSuccess || dllm::configure_tree_attn() != cudaSuccess) {
     cudaGetLastError();
     return fail(DLLM_ECUDA);
   }
@@ -913,6 +1024,33 @@ int dllm_create_bf16(dllm_ctx* c, size_t n, const char* label, dllm_buf** out) {
   if (n == 0) return set_err(c, DLLM_EINVAL, "create_bf16: invalid size %zu", n);
   if (int rc = use_device(c)) return rc;
   return new_buf(c, n, 1, label, out);
+}
+
+int dllm_create_i32(dllm_ctx* c, size_t n, const char* label, dllm_buf** out) {
+  if (!c || !out) return DLLM_EINVAL;
+  *out = nullptr;
+  if (n == 0) return set_err(c, DLLM_EINVAL, "createI32: invalid size %zu", n);
+  if (int rc = use_device(c)) return rc;
+  return new_buf(c, n, 2, label, out);
+}
+
+int dllm_write_i32(dllm_ctx* c, dllm_buf* b, const int32_t* src, size_t n) {
+  if (!c) return DLLM_EINVAL;
+  if (int rc = check_i32(c, b, n, "writeI32")) return rc;
+  if (!src && n) return set_err(c, DLLM_EINVAL, "writeI32: null source");
+  if (int rc = use_device(c)) return rc;
+  CK(c, cudaMemcpyAsync(b->ptr, src, n * 4, cudaMemcpyHostToDevice, c->stream));
+  return DLLM_OK;
+}
+
+int dllm_read_i32(dllm_ctx* c, const dllm_buf* b, int32_t* dst, size_t n) {
+  if (!c) return DLLM_EINVAL;
+  if (n == 0) return set_err(c, DLLM_EINVAL, "readI32: invalid size 0");
+  if (int rc = check_i32(c, b, n, "readI32")) return rc;
+  if (!dst) return set_err(c, DLLM_EINVAL, "readI32: null destination");
+  if (int rc = use_device(c)) return rc;
+  CK(c, cudaMemcpyAsync(dst, b->ptr, n * 4, cudaMemcpyDeviceToHost, c->stream));
+  return sync_check(c, kDefaultTimeoutMs);
 }
 
 int dllm_write_f32(dllm_ctx* c, dllm_buf* b, const float* src, size_t n) {
@@ -2099,6 +2237,360 @@ int dllm_pipeline_synchronize(dllm_pipeline* pl, int timeout_ms) {
   if (!pl) return DLLM_EINVAL;
   if (int rc = use_device(pl->ctx)) return rc;
   return sync_check(pl->ctx, timeout_ms);
+}
+
+// ---- verification of drafted tokens -----------------------------------------------------------
+int dllm_rope_plan_create(dllm_ctx* c, const dllm_rope_config* r, dllm_rope_plan** out) {
+  if (!c || !out) return DLLM_EINVAL;
+  *out = nullptr;
+  if (!r) return set_err(c, DLLM_EINVAL, "ropePlan: null configuration");
+  const int rd = r->rotary_dim;
+  if (rd < 2 || rd % 2 || rd > c->cfg.head_dim)
+    return set_err(c, DLLM_EINVAL, "ropePlan: rotary_dim=%d must be even, 2..%d", rd, c->cfg.head_dim);
+  if (r->layout != DLLM_ROPE_HALF && r->layout != DLLM_ROPE_INTERLEAVED)
+    return set_err(c, DLLM_EINVAL, "ropePlan: invalid layout %d", r->layout);
+  if (!(r->theta > 1.0) || !std::isfinite(r->theta)) return set_err(c, DLLM_EINVAL, "ropePlan: theta must exceed 1");
+  if (r->scaling < DLLM_ROPE_PLAIN || r->scaling > DLLM_ROPE_YARN)
+    return set_err(c, DLLM_EINVAL, "ropePlan: invalid scaling %d", r->scaling);
+  if (r->scaling != DLLM_ROPE_PLAIN && (!(r->factor >= 1.0) || !std::isfinite(r->factor)))
+    return set_err(c, DLLM_EINVAL, "ropePlan: factor must be at least 1");
+  if (r->scaling == DLLM_ROPE_NTK && rd < 4) return set_err(c, DLLM_EINVAL, "ropePlan: ntk needs rotary_dim >= 4");
+  if (r->scaling == DLLM_ROPE_YARN &&
+      (r->original_max_pos < 1 || !(r->beta_slow > 0.0) || !(r->beta_fast > r->beta_slow) || !std::isfinite(r->beta_fast)))
+    return set_err(c, DLLM_EINVAL, "ropePlan: yarn needs original_max_pos >= 1 and beta_fast > beta_slow > 0");
+  if (!(r->attention_factor >= 0.0) || !std::isfinite(r->attention_factor))
+    return set_err(c, DLLM_EINVAL, "ropePlan: attention_factor must be 0 (the scaling's own) or positive");
+  if (int rc = use_device(c)) return rc;
+  if (int rc = refuse_capture(c, "ropePlan")) return rc;
+  // inverse frequencies in 64 bits, divided by 2 pi: whole turns per position
+  const double kTwoPi = 6.283185307179586476925286766559;
+  double base = r->theta;
+  if (r->scaling == DLLM_ROPE_NTK) base *= std::pow(r->factor, (double)rd / (rd - 2));
+  double lo = 0, hi = 0;
+  if (r->scaling == DLLM_ROPE_YARN) {
+    // the pair that makes `beta` turns over the original context
+    auto pair = [&](double beta) {
+      return rd * std::log(r->original_max_pos / (beta * kTwoPi)) / (2 * std::log(base));
+    };
+    lo = std::max(std::floor(pair(r->beta_fast)), 0.0);
+    hi = std::min(std::ceil(pair(r->beta_slow)), (double)(rd - 1));
+  }
+  std::vector<double> turns(rd / 2);
+  for (int i = 0; i < rd / 2; ++i) {
+    double fr = std::pow(base, -2.0 * i / rd);
+    if (r->scaling == DLLM_ROPE_LINEAR) fr /= r->factor;
+    if (r->scaling == DLLM_ROPE_YARN) {
+      const double ramp = std::min(1.0, std::max(0.0, (i - lo) / (hi == lo ? 0.001 : hi - lo)));
+      fr = fr / r->factor * ramp + fr * (1.0 - ramp);
+    }
+    turns[i] = fr / kTwoPi;
+  }
+  auto* p = new dllm_rope_plan();
+  p->ctx = c;
+  p->rotary = rd;
+  p->interleaved = r->layout == DLLM_ROPE_INTERLEAVED;
+  p->factor = (float)(r->attention_factor > 0.0 ? r->attention_factor
+                      : r->scaling == DLLM_ROPE_YARN ? 0.1 * std::log(r->factor) + 1.0 : 1.0);
+  if (int rc = upload(c, turns.data(), turns.size() * sizeof(double), "rope plan", &p->turns)) {
+    delete p;
+    return rc;
+  }
+  *out = p;
+  return DLLM_OK;
+}
+
+void dllm_rope_plan_destroy(dllm_rope_plan* p) {
+  if (!p) return;
+  dllm_buf_free(p->turns);
+  delete p;
+}
+
+int dllm_rope_at(dllm_ctx* c, const dllm_rope_plan* p, const dllm_buf* positions, int n, dllm_buf* q, dllm_buf* k,
+                 dllm_buf* q_out, dllm_buf* k_out) {
+  if (!c) return DLLM_EINVAL;
+  if (!p || p->ctx != c) return set_err(c, DLLM_EINVAL, "ropeAt: null or foreign plan");
+  if (n <= 0) return set_err(c, DLLM_EINVAL, "ropeAt: invalid n=%d", n);
+  if (!q && !k) return set_err(c, DLLM_EINVAL, "ropeAt: neither q nor k given");
+  if ((!q && q_out) || (!k && k_out)) return set_err(c, DLLM_EINVAL, "ropeAt: an output without its input");
+  const dllm_config& f = c->cfg;
+  const size_t QD = (size_t)f.num_q_heads * f.head_dim, KD = (size_t)f.num_kv_heads * f.head_dim;
+  if (!q_out) q_out = q;
+  if (!k_out) k_out = k;
+  if (int rc = check_i32(c, positions, n, "ropeAt positions")) return rc;
+  if (q) {
+    if (int rc = check_f32(c, q, n * QD, "ropeAt q")) return rc;
+    if (int rc = check_f32(c, q_out, n * QD, "ropeAt qOut")) return rc;
+  }
+  if (k) {
+    if (int rc = check_f32(c, k, n * KD, "ropeAt k")) return rc;
+    if (int rc = check_f32(c, k_out, n * KD, "ropeAt kOut")) return rc;
+  }
+  if (q && k && (q_out == k_out || q_out == k || k_out == q))
+    return set_err(c, DLLM_EINVAL, "ropeAt: q and k must not share a buffer");
+  if (int rc = use_device(c)) return rc;
+  dllm::RopeAtArgs a{};
+  if (q) a.q = (const float*)q->ptr, a.q_out = (float*)q_out->ptr, a.q_heads = f.num_q_heads;
+  if (k) a.k = (const float*)k->ptr, a.k_out = (float*)k_out->ptr, a.k_heads = f.num_kv_heads;
+  a.pos = (const int32_t*)positions->ptr;
+  a.turns = (const double*)p->turns->ptr;
+  a.n = n;
+  a.hd = f.head_dim;
+  a.rotary = p->rotary;
+  a.interleaved = p->interleaved;
+  a.factor = p->factor;
+  CK(c, dllm::op_rope_at(a, c->stream));
+  c->launches += 1;
+  return DLLM_OK;
+}
+
+int dllm_tree_create(dllm_ctx* c, const int32_t* parents, const int32_t* counts, const int32_t* seqs, int n_seqs,
+                     dllm_tree** out) {
+  if (!c || !out) return DLLM_EINVAL;
+  *out = nullptr;
+  if (!parents || !counts || n_seqs < 1 || n_seqs > dllm::kTreeMaxSeqs)
+    return set_err(c, DLLM_EINVAL, "draftTree: need 1..%d sequences", dllm::kTreeMaxSeqs);
+  std::vector<dllm::TreeSeq> sq(n_seqs);
+  int n = 0, max_m = 0;
+  for (int i = 0; i < n_seqs; ++i) {
+    const int id = seqs ? seqs[i] : i;
+    if (counts[i] < 0 || counts[i] > dllm::kTreeMaxNodes)
+      return set_err(c, DLLM_EINVAL, "draftTree: %d nodes, at most %d per sequence", counts[i], dllm::kTreeMaxNodes);
+    if (id < 0) return set_err(c, DLLM_EINVAL, "draftTree: invalid seq %d", id);
+    for (int j = 0; j < i; ++j)
+      if (sq[j].seq == id) return set_err(c, DLLM_EINVAL, "draftTree: seq %d listed twice", id);
+    sq[i] = dllm::TreeSeq{id, n, counts[i], 0};
+    n += counts[i];
+    max_m = std::max(max_m, (int)counts[i]);
+  }
+  if (n < 1) return set_err(c, DLLM_EINVAL, "draftTree: no nodes");
+  std::vector<int> depth(n);
+  std::vector<unsigned char> bytes(n_seqs * sizeof(dllm::TreeSeq) + n * sizeof(unsigned long long));
+  memcpy(bytes.data(), sq.data(), n_seqs * sizeof(dllm::TreeSeq));
+  auto* anc = (unsigned long long*)(bytes.data() + n_seqs * sizeof(dllm::TreeSeq));
+  for (const auto& q : sq)
+    for (int i = 0; i < q.m; ++i) {
+      const int p = parents[q.row0 + i];
+      if (p < -1 || p >= i)
+        return set_err(c, DLLM_EINVAL, "draftTree: node %d has parent %d; parents come before their children", i, p);
+      anc[q.row0 + i] = (1ull << i) | (p < 0 ? 0ull : anc[q.row0 + p]);
+      depth[q.row0 + i] = p < 0 ? 0 : depth[q.row0 + p] + 1;
+    }
+  if (int rc = use_device(c)) return rc;
+  if (int rc = refuse_capture(c, "draftTree")) return rc;
+  if (!c->tree_part)
+    if (int rc = dev_alloc(c, &c->tree_part, dllm::tree_attn_part_rows(c->sms) * (c->cfg.head_dim + 2), "tree partials"))
+      return rc;
+  auto* t = new dllm_tree();
+  t->ctx = c;
+  t->n = n;
+  t->n_seqs = n_seqs;
+  t->max_m = max_m;
+  t->seqs = std::move(sq);
+  t->parents.assign(parents, parents + n);
+  t->depth = std::move(depth);
+  if (int rc = upload(c, bytes.data(), bytes.size(), "tree", &t->dev)) {
+    delete t;
+    return rc;
+  }
+  *out = t;
+  return DLLM_OK;
+}
+
+void dllm_tree_destroy(dllm_tree* t) {
+  if (!t) return;
+  dllm_buf_free(t->dev);
+  delete t;
+}
+
+int dllm_pick_tokens(dllm_ctx* c, const dllm_pick* p) {
+  if (!c) return DLLM_EINVAL;
+  if (!p) return set_err(c, DLLM_EINVAL, "pickTokens: null arguments");
+  const int n = p->n, V = c->cfg.vocab_size;
+  if (n <= 0) return set_err(c, DLLM_EINVAL, "pickTokens: invalid n=%d", n);
+  if ((p->tree != nullptr) != (p->draft != nullptr))
+    return set_err(c, DLLM_EINVAL, "pickTokens: a tree comes with its drafted tokens");
+  if (p->tree && (p->tree->ctx != c || p->tree->n != n))
+    return set_err(c, DLLM_EINVAL, "pickTokens: the tree is foreign or has not n=%d nodes", n);
+  const size_t b = p->tree ? p->tree->n_seqs : n;
+  if (int rc = check_f32(c, p->logits, (size_t)n * V, "pickTokens logits")) return rc;
+  if (int rc = check_i32(c, p->tokens, n, "pickTokens tokens")) return rc;
+  if (p->out)
+    if (int rc = check_f32(c, p->out, (size_t)n * V, "pickTokens out")) return rc;
+  if (p->draft)
+    if (int rc = check_i32(c, p->draft, n, "pickTokens draft")) return rc;
+  if (p->penalties) {
+    if (int rc = check_f32(c, p->penalties, 3 * b, "pickTokens penalties")) return rc;
+  } else if (p->history) {
+    return set_err(c, DLLM_EINVAL, "pickTokens: a history without penalties");
+  }
+  if (p->history) {
+    if (int rc = check_i32(c, p->history, 1, "pickTokens history")) return rc;
+    if (int rc = check_i32(c, p->history_offsets, b + 1, "pickTokens history offsets")) return rc;
+    if (p->history->n > 0x7fffffff) return set_err(c, DLLM_EINVAL, "pickTokens: history too long");
+    if (p->prompt_lens)
+      if (int rc = check_i32(c, p->prompt_lens, b, "pickTokens prompt lengths")) return rc;
+  } else if (p->history_offsets || p->prompt_lens) {
+    return set_err(c, DLLM_EINVAL, "pickTokens: history offsets or prompt lengths without a history");
+  }
+  if (p->bias_tokens) {
+    if (int rc = check_i32(c, p->bias_tokens, 1, "pickTokens bias tokens")) return rc;
+    if (int rc = check_f32(c, p->bias_values, p->bias_tokens->n, "pickTokens bias values")) return rc;
+    if (int rc = check_i32(c, p->bias_offsets, b + 1, "pickTokens bias offsets")) return rc;
+    if (p->bias_tokens->n > 0x7fffffff) return set_err(c, DLLM_EINVAL, "pickTokens: too many biases");
+  } else if (p->bias_values || p->bias_offsets) {
+    return set_err(c, DLLM_EINVAL, "pickTokens: bias values or offsets without their tokens");
+  }
+  if (p->mask)
+    if (int rc = check_i32(c, p->mask, (size_t)n * ((V + 31) / 32), "pickTokens mask")) return rc;
+  if (int rc = use_device(c)) return rc;
+  dllm::PickArgs a{};
+  a.logits = (const float*)p->logits->ptr;
+  a.out = p->out ? (float*)p->out->ptr : nullptr;
+  a.tokens = (int32_t*)p->tokens->ptr;
+  a.n = n;
+  a.vocab = V;
+  if (p->history) {
+    a.hist = (const int32_t*)p->history->ptr;
+    a.hist_off = (const int32_t*)p->history_offsets->ptr;
+    a.prompt = p->prompt_lens ? (const int32_t*)p->prompt_lens->ptr : nullptr;
+    a.hist_total = (int)p->history->n;
+  }
+  if (p->penalties) a.penalties = (const float*)p->penalties->ptr;
+  if (p->bias_tokens) {
+    a.bias_tok = (const int32_t*)p->bias_tokens->ptr;
+    a.bias_val = (const float*)p->bias_values->ptr;
+    a.bias_off = (const int32_t*)p->bias_offsets->ptr;
+    a.bias_total = (int)p->bias_tokens->n;
+  }
+  if (p->mask) a.mask = (const uint32_t*)p->mask->ptr;
+  a.n_seqs = (int)b;
+  a.max_m = 1;
+  if (p->tree) {
+    a.seqs = p->tree->seqs_dev();
+    a.anc = p->tree->anc_dev();
+    a.draft = (const int32_t*)p->draft->ptr;
+    a.max_m = p->tree->max_m;
+  }
+  CK(c, dllm::op_pick(a, c->sms, c->stream));
+  c->launches += 1;
+  return DLLM_OK;
+}
+
+int dllm_stage_append_tree(dllm_stage* s, int layer, const dllm_tree* tree, const dllm_buf* k, const dllm_buf* v) {
+  if (!s) return DLLM_EINVAL;
+  dllm_ctx* c = s->ctx;
+  const dllm_config& f = c->cfg;
+  dllm::TreeT0 t0;
+  if (int rc = tree_layer(s, layer, "append_tree")) return rc;
+  if (int rc = tree_t0(s, tree, "append_tree", &t0)) return rc;
+  const size_t KD = (size_t)f.num_kv_heads * f.head_dim;
+  if (int rc = check_f32(c, k, tree->n * KD, "append_tree k")) return rc;
+  if (int rc = check_f32(c, v, tree->n * KD, "append_tree v")) return rc;
+  if (int rc = use_device(c)) return rc;
+  CK(c, dllm::op_tree_append(tree->seqs_dev(), tree->n_seqs, tree->max_m, t0, stage_kv(s), (const float*)k->ptr,
+                             (const float*)v->ptr, layer_pool(s, s->kpool, layer), layer_pool(s, s->vpool, layer),
+                             f.kv_dtype, f.num_kv_heads, f.head_dim, c->err_dev, c->stream));
+  c->launches += 1;
+  return DLLM_OK;
+}
+
+int dllm_stage_tree_attention(dllm_stage* s, int layer, const dllm_tree* tree, const dllm_buf* q, dllm_buf* out) {
+  if (!s) return DLLM_EINVAL;
+  dllm_ctx* c = s->ctx;
+  const size_t QD = (size_t)c->cfg.num_q_heads * c->cfg.head_dim;
+  dllm::TreeT0 t0;
+  if (int rc = tree_layer(s, layer, "tree_attention")) return rc;
+  if (int rc = tree_t0(s, tree, "tree_attention", &t0)) return rc;
+  if (int rc = check_f32(c, q, tree->n * QD, "tree_attention q")) return rc;
+  if (int rc = check_f32(c, out, tree->n * QD, "tree_attention out")) return rc;
+  if (q == out) return set_err(c, DLLM_EINVAL, "tree_attention: out must not be q");
+  if (int rc = use_device(c)) return rc;
+  return tree_attention(s, layer, tree, t0, (const float*)q->ptr, (float*)out->ptr);
+}
+
+int dllm_stage_commit_tree(dllm_stage* s, const dllm_tree* tree, const int32_t* path, const int32_t* lens) {
+  if (!s) return DLLM_EINVAL;
+  dllm_ctx* c = s->ctx;
+  const dllm_config& f = c->cfg;
+  dllm::TreeT0 t0;
+  if (int rc = tree_t0(s, tree, "commit_tree", &t0)) return rc;
+  if (!path || !lens) return set_err(c, DLLM_EINVAL, "commit_tree: null path");
+  // every sequence's path: a root, then children in turn
+  const int32_t* p = path;
+  for (int i = 0; i < tree->n_seqs; ++i) {
+    const dllm::TreeSeq& q = tree->seqs[i];
+    if (lens[i] < 0 || lens[i] > q.m) return set_err(c, DLLM_EINVAL, "commit_tree: path of %d of %d nodes", lens[i], q.m);
+    for (int j = 0; j < lens[i]; ++j) {
+      if (p[j] < 0 || p[j] >= q.m || tree->parents[q.row0 + p[j]] != (j ? p[j - 1] : -1))
+        return set_err(c, DLLM_EINVAL, "commit_tree: node %d does not continue the path of seq %d", p[j], q.seq);
+    }
+    p += lens[i];
+  }
+  if (int rc = use_device(c)) return rc;
+  const KvLayout kv = stage_kv(s);
+  dllm::CommitArgs a;
+  a.n_seqs = 0;
+  auto flush = [&]() {
+    if (a.n_seqs == 0 || s->nl == 0) return cudaSuccess;
+    const cudaError_t e = dllm::op_tree_commit(a, kv, s->kpool, s->vpool, s->layer_elems, s->nl, f.kv_dtype,
+                                               f.num_kv_heads, f.head_dim, c->stream);
+    c->launches += 1;
+    a.n_seqs = 0;
+    return e;
+  };
+  p = path;
+  for (int i = 0; i < tree->n_seqs; ++i) {
+    int first = 0;
+    while (first < lens[i] && p[first] == first) ++first;  // these rows lie where they belong
+    if (first < lens[i]) {
+      const int k = a.n_seqs++;
+      a.seq[k] = tree->seqs[i].seq;
+      a.t0[k] = t0.t0[i];
+      a.first[k] = (uint8_t)first;
+      a.len[k] = (uint8_t)lens[i];
+      for (int j = 0; j < lens[i]; ++j) a.path[k][j] = (uint8_t)p[j];
+      if (a.n_seqs == dllm::kCommitSeqs) CK(c, flush());
+    }
+    p += lens[i];
+  }
+  CK(c, flush());
+  for (int i = 0; i < tree->n_seqs; ++i) s->T0[tree->seqs[i].seq] += lens[i];
+  return DLLM_OK;
+}
+
+int dllm_stage_forward_tree(dllm_stage* s, const dllm_tree* tree, dllm_buf* h, const dllm_buf* tokens, dllm_buf* logits) {
+  if (!s) return DLLM_EINVAL;
+  dllm_ctx* c = s->ctx;
+  const dllm_config& f = c->cfg;
+  dllm::TreeT0 t0;
+  if (int rc = tree_t0(s, tree, "forward_tree", &t0)) return rc;
+  if (tree->n > dllm::kTcMaxRows)
+    return set_err(c, DLLM_EINVAL, "forward_tree: %d nodes, at most %d in a pass", tree->n, dllm::kTcMaxRows);
+  if (c->tc_min_rows == 0) return set_err(c, DLLM_EINVAL, "forward_tree: needs the tensor-core projections, which are off");
+  if (int rc = check_f32(c, h, (size_t)tree->n * f.hidden_size, "forward_tree h")) return rc;
+  if (tokens)
+    if (int rc = check_i32(c, tokens, tree->n, "forward_tree tokens")) return rc;
+  if (logits)
+    if (int rc = check_f32(c, logits, (size_t)tree->n * f.vocab_size, "forward_tree logits")) return rc;
+  if (logits == h) return set_err(c, DLLM_EINVAL, "forward_tree: logits must not be h");
+  if (int rc = use_device(c)) return rc;
+  if (int rc = refuse_capture(c, "forward_tree")) return rc;
+  if (int rc = resolve(s)) return rc;
+  if (tokens && !s->embed) return set_err(c, DLLM_ENOTFOUND, "missing weight model.embed_tokens.weight");
+  if (logits)
+    if (int rc = need_head(s)) return rc;
+  std::vector<RowDesc> rd(tree->n);
+  for (int i = 0; i < tree->n_seqs; ++i) {
+    const dllm::TreeSeq& q = tree->seqs[i];
+    for (int j = 0; j < q.m; ++j)
+      rd[q.row0 + j] = RowDesc{q.seq, t0.t0[i] + tree->depth[q.row0 + j], t0.t0[i] + j, 0};
+  }
+  return run_wide(s, (float*)h->ptr, tree->n, rd.data(), tokens ? (const int32_t*)tokens->ptr : nullptr, nullptr, tree,
+                  &t0, logits ? (float*)logits->ptr : nullptr);
+}
+
+void* dllm_stage_kv_device_ptr(const dllm_stage* s, int which) {
+  return !s ? nullptr : which == 0 ? s->kpool : which == 1 ? s->vpool : nullptr;
 }
 
 }  // extern "C"

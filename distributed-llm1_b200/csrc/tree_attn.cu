@@ -1,0 +1,638 @@
+// tree_attn.cu — attention of a drafted tree over a stage's paged KV cache.
+//
+// Node i of a sequence with T0 cached slots sees the slots [0, T0) and slot T0 + j
+// for every node j on the path from the root to i, itself included:
+//   out_i = sum_j p_ij v_j,  p_ij = exp(q_i . k_j / sqrt(hd) - max_i) / sum_i
+// The G query heads of a KV head and the m nodes make m G rows that share one pass
+// over that head's K and V; the softmax runs online over blocks of slots, and a
+// sequence's slots are split over CTAs whose partial results a second kernel joins.
+//
+// Precision. q, p and the outputs are fp32 like every activation here, and the
+// products run on the tensor cores all the same: with a bf16 cache q and p are cut
+// into three bf16 terms (8 + 8 + 8 bits; the products with bf16 K and V are exact),
+// with an fp32 cache all four operands into two tf32 terms (11 + 11 bits, the low x
+// low product left out). The tensor core adds into its fp32 accumulator with
+// truncation, so long chains would drift towards zero by 2^-24 per step: the large
+// terms and the corrections have accumulators of their own, a block's p . V starts
+// from zero, and the sum over blocks is a rounded fp32 add in registers.
+//
+// Work split. A CTA has 8 warps and takes 16 WR rows of one (sequence, KV head): WR
+// warps side by side in rows, 8 / WR of them in slots, so that one node's G rows
+// still keep 8 warps busy. K and V blocks come through a cp.async ring, and slots
+// behind the sequence's last one are zero-filled, never read.
+#include <algorithm>
+
+#include "kernels.cuh"
+#include "verify.cuh"
+
+namespace dllm {
+namespace {
+
+constexpr int kTAThreads = 256;
+constexpr float kNegInf = -INFINITY;
+
+DLLM_DEV uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+DLLM_DEV void cp16_zfill(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+DLLM_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+DLLM_DEV void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+DLLM_DEV void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+DLLM_DEV void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+DLLM_DEV void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+DLLM_DEV void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+DLLM_DEV float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+DLLM_DEV uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// (x, y) -> three packed bf16 pairs whose sums are x and y to 2^-25 of them.
+DLLM_DEV void split3(float x, float y, uint32_t& h, uint32_t& m, uint32_t& l) {
+  h = pack_bf16(x, y);
+  x -= bf16_lo(h), y -= bf16_hi(h);
+  m = pack_bf16(x, y);
+  x -= bf16_lo(m), y -= bf16_hi(m);
+  l = pack_bf16(x, y);
+}
+// x = hi + lo, hi with 11 bits; lo is rounded to 11 bits by the conversion.
+DLLM_DEV void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = __float_as_uint(x) & 0xffffe000u;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+}
+DLLM_DEV bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
+
+// Tile shapes. SN: slots of a block that one warp takes; BN: slots of a block.
+// The ring depth is what fits beside the q tile in 227 KB.
+template <typename KT, int HD, int WR>
+struct TATile {
+  static constexpr bool kF32 = sizeof(KT) == 4;
+  static constexpr int WS = 8 / WR;                 // warps side by side in slots
+  static constexpr int SN = kF32 ? 8 * WR : (WR == 1 ? 16 : WR == 2 ? 32 : WR == 4 ? 32 : 64);
+  static constexpr int BN = SN * WS;                // 64, or 128 for few rows of a bf16 cache
+  static constexpr int RT = 16 * WR;                // rows of the tile
+  static constexpr int kRowBytes = HD * (int)sizeof(KT);
+  static constexpr int kChunks = kRowBytes / 16;    // 16-byte chunks per slot
+  static constexpr int kTileBytes = BN * kRowBytes; // one of K, V
+  static constexpr int kQBytes = RT * HD * (kF32 ? 4 : 6);
+  static constexpr int kMergeBytes = WS > 1 ? WS * RT * (HD + 2) * 4 : 0;
+  static constexpr int kRoom = 225 * 1024 - kQBytes;
+  static constexpr int kFit = kRoom / (2 * kTileBytes);
+  static constexpr int kStages = kFit > 4 ? 4 : kFit;
+  static_assert(kStages >= 2, "the K/V ring needs two stages");
+  static_assert(kMergeBytes <= kStages * 2 * kTileBytes, "the join of the slot groups reuses the ring");
+  static constexpr int kSmem = kQBytes + kStages * 2 * kTileBytes;
+};
+
+struct TAKernelArgs {
+  TreeAttnArgs a;
+  int bps;                       // blocks per split
+  int t0[kTreeMaxSeqs];
+  int part0[kTreeMaxSeqs];       // first partial row of a split sequence
+};
+
+// The number of splits of a sequence with `slots` slots; the same on host and device.
+__host__ __device__ inline int ta_splits(int slots, int bn, int bps) {
+  const int blocks = (slots + bn - 1) / bn;
+  return (blocks + bps - 1) / bps;
+}
+
+template <typename KT, int HD, int WR>
+__global__ void __launch_bounds__(kTAThreads, 1) tree_attn_kernel(const __grid_constant__ TAKernelArgs P) {
+  using T = TATile<KT, HD, WR>;
+  constexpr int SN = T::SN, BN = T::BN, WS = T::WS, RT = T::RT, NT = SN / 8, CH = T::kChunks, S = T::kStages;
+  constexpr bool F32 = T::kF32;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const TreeAttnArgs& a = P.a;
+  asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled; it waits for this grid's end
+  const TreeSeq sq = a.seqs[blockIdx.z];
+  const int G = a.nq / a.kvh;
+  const int head = blockIdx.y % a.kvh, tile = blockIdx.y / a.kvh;
+  const int R = sq.m * G, r0 = tile * RT;
+  const int T0 = P.t0[blockIdx.z], slots = T0 + sq.m;
+  const int nsplit = ta_splits(slots, BN, P.bps);
+  const int split = blockIdx.x;
+  if (r0 >= R || split >= nsplit) return;
+  const int nblk = (slots + BN - 1) / BN;
+  const int blk0 = split * P.bps, blk1 = min(nblk, blk0 + P.bps);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int wr = warp % WR, ws = warp / WR;
+  const int g = lane >> 2, t = lane & 3;
+  unsigned char* sQ = smem;
+  unsigned char* ring = smem + T::kQBytes;
+
+  // ---- K/V blocks through the ring. A thread copies one 16-byte chunk of every
+  // (256 / CH)-th slot; pages hold at least 32 slots, so a block has BN / 32 page
+  // lookups at most, made one block ahead of the copies that need them.
+  constexpr int kPass = kTAThreads / CH;  // slots per pass
+  constexpr int kPages = BN / 32;
+  const int cch = tid % CH, crow = tid / CH;
+  const KT* kc = static_cast<const KT*>(a.kc) + (size_t)head * a.kv.head_stride;
+  const KT* vc = static_cast<const KT*>(a.vc) + (size_t)head * a.kv.head_stride;
+  const int* table = a.kv.page_table + (size_t)sq.seq * a.kv.max_pages;
+  int page[kPages];
+  auto lookup = [&](int blk) {
+#pragma unroll
+    for (int i = 0; i < kPages; ++i) page[i] = __ldg(table + (min(blk * BN + 32 * i, slots - 1) >> a.kv.log2_page));
+  };
+  auto copy = [&](int blk, int stage) {
+    const uint32_t dk = smem_addr(ring + stage * 2 * T::kTileBytes), dv = dk + T::kTileBytes;
+#pragma unroll
+    for (int i = 0; i < BN / kPass; ++i) {
+      const int row = crow + i * kPass;
+      const int slot = blk * BN + row;
+      int pg = page[0];
+#pragma unroll
+      for (int u = 1; u < kPages; ++u) pg = row >= 32 * u ? page[u] : pg;
+      const long long off = (long long)pg * a.kv.page_stride +
+                            (long long)(slot & ((1 << a.kv.log2_page) - 1)) * a.kv.row_stride + cch * (16 / (int)sizeof(KT));
+      const uint32_t at = row * T::kRowBytes + ((cch ^ (row & 7)) << 4);
+      const bool real = slot < slots;
+      cp16_zfill(dk + at, real ? kc + off : kc, real);
+      cp16_zfill(dv + at, real ? vc + off : vc, real);
+    }
+  };
+  lookup(blk0);
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) {
+    if (blk0 + s < blk1) {
+      copy(blk0 + s, s);
+      lookup(blk0 + s + 1);
+    }
+    cp_commit();
+  }
+
+  // ---- the q tile, scaled by log2(e) / sqrt(hd) so that the softmax is in powers of two
+  for (int i = tid; i < RT * HD / 4; i += kTAThreads) {
+    const int row = i / (HD / 4), d = (i % (HD / 4)) * 4;
+    const int r = r0 + row;
+    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r < R) {
+      const int node = r / G;
+      f = *reinterpret_cast<const float4*>(a.q + ((size_t)(sq.row0 + node) * a.nq + head * G + (r - node * G)) * HD + d);
+      f.x *= a.scale_log2, f.y *= a.scale_log2, f.z *= a.scale_log2, f.w *= a.scale_log2;
+    }
+    if constexpr (F32) {
+      *reinterpret_cast<float4*>(sQ + row * HD * 4 + (((d >> 2) ^ (row & 7)) << 4)) = f;
+    } else {
+      uint32_t h[2], m[2], l[2];
+      split3(f.x, f.y, h[0], m[0], l[0]);
+      split3(f.z, f.w, h[1], m[1], l[1]);
+      unsigned char* p = sQ + row * HD * 2 + (((d >> 3) ^ (row & 7)) << 4) + (d & 4) * 2;
+      *reinterpret_cast<uint2*>(p) = make_uint2(h[0], h[1]);
+      *reinterpret_cast<uint2*>(p + RT * HD * 2) = make_uint2(m[0], m[1]);
+      *reinterpret_cast<uint2*>(p + 2 * RT * HD * 2) = make_uint2(l[0], l[1]);
+    }
+  }
+
+  // this thread's two rows of the tile and their ancestor masks
+  const int ra = wr * 16 + g, rb = ra + 8;
+  const unsigned long long anc_a = r0 + ra < R ? a.anc[sq.row0 + (r0 + ra) / G] : 0ull;
+  const unsigned long long anc_b = r0 + rb < R ? a.anc[sq.row0 + (r0 + rb) / G] : 0ull;
+
+  float o[HD / 8][4];
+#pragma unroll
+  for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+  float ma = kNegInf, mb = kNegInf, la = 0.f, lb = 0.f;
+
+  for (int blk = blk0; blk < blk1; ++blk) {
+    cp_wait<S - 2>();
+    __syncthreads();
+    {
+      const int next = blk + S - 1;
+      if (next < blk1) {
+        copy(next, (next - blk0) % S);
+        lookup(next + 1);
+      }
+      cp_commit();
+    }
+    unsigned char* sK = ring + ((blk - blk0) % S) * 2 * T::kTileBytes;
+    unsigned char* sV = sK + T::kTileBytes;
+    const int wslot = ws * SN;  // first slot of this warp within the block
+
+    // ---- scores
+    float sh[NT][4], ss[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sh[i][e] = ss[i][e] = 0.f;
+    if constexpr (F32) {
+#pragma unroll 4
+      for (int ks = 0; ks < HD / 8; ++ks) {
+        uint32_t qh[4], ql[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = wr * 16 + g + (e & 1) * 8, ch = ks * 2 + (e >> 1);
+          split_tf32(*reinterpret_cast<const float*>(sQ + row * HD * 4 + ((ch ^ (row & 7)) << 4) + t * 4), qh[e], ql[e]);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const int row = wslot + nt * 8 + g;
+          uint32_t kh[2], kl[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            split_tf32(*reinterpret_cast<const float*>(sK + row * T::kRowBytes + (((ks * 2 + e) ^ (row & 7)) << 4) + t * 4),
+                       kh[e], kl[e]);
+          mma_tf32(sh[nt], qh, kh[0], kh[1]);
+          mma_tf32(ss[nt], qh, kl[0], kl[1]);
+          mma_tf32(ss[nt], ql, kh[0], kh[1]);
+        }
+      }
+    } else {
+      const int arow = wr * 16 + (lane & 15);
+      const uint32_t qa = smem_addr(sQ) + arow * HD * 2;
+      const int krow = (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks) {
+        uint32_t qh[4], qm[4], ql[4];
+        const uint32_t at = qa + (((2 * ks + (lane >> 4)) ^ (arow & 7)) << 4);
+        ldsm4(qh, at);
+        ldsm4(qm, at + RT * HD * 2);
+        ldsm4(ql, at + 2 * RT * HD * 2);
+#pragma unroll
+        for (int np = 0; np < NT / 2; ++np) {
+          const int row = wslot + np * 16 + krow;
+          uint32_t k4[4];
+          ldsm4(k4, smem_addr(sK) + row * T::kRowBytes + (((2 * ks + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
+          mma_bf16(sh[2 * np], qh, k4[0], k4[1]);
+          mma_bf16(sh[2 * np + 1], qh, k4[2], k4[3]);
+          mma_bf16(ss[2 * np], qm, k4[0], k4[1]);
+          mma_bf16(ss[2 * np + 1], qm, k4[2], k4[3]);
+          mma_bf16(ss[2 * np], ql, k4[0], k4[1]);
+          mma_bf16(ss[2 * np + 1], ql, k4[2], k4[3]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sh[i][e] += ss[i][e];
+
+    // ---- mask: only blocks that reach behind the context have anything to hide
+    const bool drafted = (blk + 1) * BN > T0;
+    if (drafted) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int node = blk * BN + wslot + i * 8 + 2 * t + (e & 1) - T0;
+          const unsigned long long anc = e < 2 ? anc_a : anc_b;
+          if (node >= 0 && (node >= kTreeMaxNodes || !(anc >> node & 1))) sh[i][e] = kNegInf;
+        }
+    }
+
+    // ---- online softmax
+    float xa = kNegInf, xb = kNegInf;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      xa = fmaxf(xa, fmaxf(sh[i][0], sh[i][1]));
+      xb = fmaxf(xb, fmaxf(sh[i][2], sh[i][3]));
+    }
+#pragma unroll
+    for (int w = 1; w < 4; w <<= 1) {
+      xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, w));
+      xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, w));
+    }
+    xa = fmaxf(xa, ma), xb = fmaxf(xb, mb);
+    // rows that have seen nothing yet keep a maximum of -inf; their p are exp2(-inf - 0) = 0
+    const float ba = xa == kNegInf ? 0.f : xa, bb = xb == kNegInf ? 0.f : xb;
+    float fa = ex2(ma - ba), fb = ex2(mb - bb);
+    ma = xa, mb = xb;
+    float sa = 0.f, sb = 0.f;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      sh[i][0] = ex2(sh[i][0] - ba), sh[i][1] = ex2(sh[i][1] - ba);
+      sh[i][2] = ex2(sh[i][2] - bb), sh[i][3] = ex2(sh[i][3] - bb);
+      sa += sh[i][0] + sh[i][1];
+      sb += sh[i][2] + sh[i][3];
+    }
+    la = la * fa + sa, lb = lb * fb + sb;
+
+    // ---- a drafted row that some nodes do not see may hold infinities or NaN, and
+    // 0 * NaN would reach the nodes that must not see it: such values are taken out
+    // of the tile and added to the rows that do see them.
+    if (drafted) {
+      int bad = 0;
+      for (int i = tid; i < BN * HD; i += kTAThreads) {
+        const int row = i / HD, d = i % HD;
+        if (blk * BN + row < T0) continue;
+        const KT* p = reinterpret_cast<const KT*>(sV + row * T::kRowBytes +
+                                                  (((d * (int)sizeof(KT) >> 4) ^ (row & 7)) << 4) + (d * sizeof(KT) & 15));
+        float v;
+        if constexpr (F32) v = *p;
+        else v = bf16_to_f32(*p);
+        bad |= !finite(v);
+      }
+      if (__syncthreads_or(bad)) {
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) {
+          o[i][0] *= fa, o[i][1] *= fa, o[i][2] *= fb, o[i][3] *= fb;
+          for (int row = wslot; row < wslot + SN; ++row) {
+            const int node = blk * BN + row - T0;
+            if (node < 0 || node >= sq.m) continue;
+            const int d = i * 8 + 2 * t;
+            const KT* p = reinterpret_cast<const KT*>(
+                sV + row * T::kRowBytes + (((d * (int)sizeof(KT) >> 4) ^ (row & 7)) << 4) + (d * sizeof(KT) & 15));
+            float v0, v1;
+            if constexpr (F32) v0 = p[0], v1 = p[1];
+            else v0 = bf16_to_f32(p[0]), v1 = bf16_to_f32(p[1]);
+            if (anc_a >> node & 1) {
+              if (!finite(v0)) o[i][0] += v0;
+              if (!finite(v1)) o[i][1] += v1;
+            }
+            if (anc_b >> node & 1) {
+              if (!finite(v0)) o[i][2] += v0;
+              if (!finite(v1)) o[i][3] += v1;
+            }
+          }
+        }
+        fa = fb = 1.f;
+        __syncthreads();
+        for (int i = tid; i < BN * HD; i += kTAThreads) {
+          const int row = i / HD, d = i % HD;
+          if (blk * BN + row < T0) continue;
+          KT* p = reinterpret_cast<KT*>(sV + row * T::kRowBytes + (((d * (int)sizeof(KT) >> 4) ^ (row & 7)) << 4) +
+                                        (d * sizeof(KT) & 15));
+          float v;
+          if constexpr (F32) v = *p;
+          else v = bf16_to_f32(*p);
+          if (!finite(v)) *p = KT(0.f);
+        }
+        __syncthreads();
+      }
+    }
+
+    // ---- o = o * f + p . V, the block's product from a fresh accumulator
+    if constexpr (F32) {
+      uint32_t ph[NT][4], pl[NT][4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {  // slots 2t, 2t + 1 of a group take the places t, t + 4 of the product
+        split_tf32(sh[j][0], ph[j][0], pl[j][0]);
+        split_tf32(sh[j][2], ph[j][1], pl[j][1]);
+        split_tf32(sh[j][1], ph[j][2], pl[j][2]);
+        split_tf32(sh[j][3], ph[j][3], pl[j][3]);
+      }
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i) {
+        float ch[4] = {0.f, 0.f, 0.f, 0.f}, cs[4] = {0.f, 0.f, 0.f, 0.f};
+        const int d = i * 8 + g;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          uint32_t vh[2], vl[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int row = wslot + j * 8 + 2 * t + e;
+            split_tf32(*reinterpret_cast<const float*>(sV + row * T::kRowBytes + (((d >> 2) ^ (row & 7)) << 4) + (d & 3) * 4),
+                       vh[e], vl[e]);
+          }
+          mma_tf32(ch, ph[j], vh[0], vh[1]);
+          mma_tf32(cs, ph[j], vl[0], vl[1]);
+          mma_tf32(cs, pl[j], vh[0], vh[1]);
+        }
+        o[i][0] = fmaf(o[i][0], fa, ch[0] + cs[0]);
+        o[i][1] = fmaf(o[i][1], fa, ch[1] + cs[1]);
+        o[i][2] = fmaf(o[i][2], fb, ch[2] + cs[2]);
+        o[i][3] = fmaf(o[i][3], fb, ch[3] + cs[3]);
+      }
+    } else {
+      constexpr int NK = SN / 16;
+      uint32_t ph[NK][4], pm[NK][4], pl[NK][4];
+#pragma unroll
+      for (int j = 0; j < NK; ++j) {
+        split3(sh[2 * j][0], sh[2 * j][1], ph[j][0], pm[j][0], pl[j][0]);
+        split3(sh[2 * j][2], sh[2 * j][3], ph[j][1], pm[j][1], pl[j][1]);
+        split3(sh[2 * j + 1][0], sh[2 * j + 1][1], ph[j][2], pm[j][2], pl[j][2]);
+        split3(sh[2 * j + 1][2], sh[2 * j + 1][3], ph[j][3], pm[j][3], pl[j][3]);
+      }
+      const int vrow = (lane & 7) + (((lane >> 3) & 1) << 3);
+#pragma unroll
+      for (int np = 0; np < HD / 16; ++np) {
+        float ch[2][4], cs[2][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ch[0][e] = ch[1][e] = cs[0][e] = cs[1][e] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NK; ++j) {
+          const int row = wslot + j * 16 + vrow;
+          uint32_t v4[4];
+          ldsm4t(v4, smem_addr(sV) + row * T::kRowBytes + (((2 * np + (lane >> 4)) ^ (row & 7)) << 4));
+          mma_bf16(ch[0], ph[j], v4[0], v4[1]);
+          mma_bf16(ch[1], ph[j], v4[2], v4[3]);
+          mma_bf16(cs[0], pm[j], v4[0], v4[1]);
+          mma_bf16(cs[1], pm[j], v4[2], v4[3]);
+          mma_bf16(cs[0], pl[j], v4[0], v4[1]);
+          mma_bf16(cs[1], pl[j], v4[2], v4[3]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float(&oo)[4] = o[2 * np + u];
+          oo[0] = fmaf(oo[0], fa, ch[u][0] + cs[u][0]);
+          oo[1] = fmaf(oo[1], fa, ch[u][1] + cs[u][1]);
+          oo[2] = fmaf(oo[2], fb, ch[u][2] + cs[u][2]);
+          oo[3] = fmaf(oo[3], fb, ch[u][3] + cs[u][3]);
+        }
+      }
+    }
+  }
+  cp_wait<0>();
+#pragma unroll
+  for (int w = 1; w < 4; w <<= 1) {
+    la += __shfl_xor_sync(0xffffffffu, la, w);
+    lb += __shfl_xor_sync(0xffffffffu, lb, w);
+  }
+
+  // ---- results: normalised to out, or partials (o, m, l) of this split
+  auto row_out = [&](int row, float4 f, int d, float m, float l) {  // dims d..d+3 of tile row `row`
+    const int r = r0 + row;
+    if (r >= R) return;
+    const int node = r / G;
+    if (nsplit == 1) {
+      const float inv = 1.0f / l;
+      *reinterpret_cast<float4*>(a.out + ((size_t)(sq.row0 + node) * a.nq + head * G + (r - node * G)) * HD + d) =
+          make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
+    } else {
+      const size_t at = (size_t)P.part0[blockIdx.z] + ((size_t)split * sq.m + node) * a.nq + head * G + (r - node * G);
+      *reinterpret_cast<float4*>(a.part_o + at * HD + d) = f;
+      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
+    }
+  };
+  __syncthreads();  // the ring is free
+  // through shared memory: rows padded by 4 floats keep the quads' stores apart
+  constexpr int kPad = HD + 4;
+  float* sO = reinterpret_cast<float*>(ring);
+  float* sML = sO + WS * RT * kPad;
+  static_assert(WS * RT * (kPad + 2) * 4 <= S * 2 * T::kTileBytes, "the results pass through the ring");
+#pragma unroll
+  for (int i = 0; i < HD / 8; ++i) {
+    *reinterpret_cast<float2*>(sO + (ws * RT + ra) * kPad + i * 8 + 2 * t) = make_float2(o[i][0], o[i][1]);
+    *reinterpret_cast<float2*>(sO + (ws * RT + rb) * kPad + i * 8 + 2 * t) = make_float2(o[i][2], o[i][3]);
+  }
+  if (t == 0) {
+    sML[(ws * RT + ra) * 2] = ma, sML[(ws * RT + ra) * 2 + 1] = la;
+    sML[(ws * RT + rb) * 2] = mb, sML[(ws * RT + rb) * 2 + 1] = lb;
+  }
+  __syncthreads();
+  for (int i = tid; i < RT * HD / 4; i += kTAThreads) {
+    const int row = i / (HD / 4), d = (i % (HD / 4)) * 4;
+    float m = kNegInf, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < WS; ++w) m = fmaxf(m, sML[(w * RT + row) * 2]);
+    const float base = m == kNegInf ? 0.f : m;
+    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < WS; ++w) {
+      const float e = WS == 1 ? 1.f : ex2(sML[(w * RT + row) * 2] - base);
+      const float4 v = *reinterpret_cast<const float4*>(sO + (w * RT + row) * kPad + d);
+      f.x = fmaf(v.x, e, f.x), f.y = fmaf(v.y, e, f.y), f.z = fmaf(v.z, e, f.z), f.w = fmaf(v.w, e, f.w);
+      l = fmaf(sML[(w * RT + row) * 2 + 1], e, l);
+    }
+    row_out(row, f, d, m, l);
+  }
+}
+
+// Joins the splits of a sequence: one warp per (row, query head), splits in order.
+template <int HD>
+__global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ TAKernelArgs P, int bn) {
+  const TreeAttnArgs& a = P.a;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the splits' grid has ended and its stores are visible
+  const TreeSeq sq = a.seqs[blockIdx.y];
+  const int nsplit = ta_splits(P.t0[blockIdx.y] + sq.m, bn, P.bps);
+  const int item = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (nsplit <= 1 || item >= sq.m * a.nq) return;
+  constexpr int V = HD / 32;
+  const size_t step = (size_t)sq.m * a.nq, base = (size_t)P.part0[blockIdx.y] + item;
+  float m = kNegInf;
+  for (int s = lane; s < nsplit; s += 32) m = fmaxf(m, a.part_ml[(base + s * step) * 2]);
+  m = warp_max(m);
+  const float b = m == kNegInf ? 0.f : m;
+  float acc[V], l = 0.f;
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < nsplit; ++s) {
+    const size_t at = base + s * step;
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
+    const float w = ex2(ml.x - b);
+    l = fmaf(ml.y, w, l);
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = fmaf(a.part_o[at * HD + lane * V + e], w, acc[e]);
+  }
+  const float inv = 1.0f / l;
+  float* dst = a.out + ((size_t)sq.row0 * a.nq + item) * HD + lane * V;
+#pragma unroll
+  for (int e = 0; e < V; ++e) dst[e] = acc[e] * inv;
+}
+
+template <typename KT, int HD, int WR>
+cudaError_t configure_one() {
+  return cudaFuncSetAttribute(tree_attn_kernel<KT, HD, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              TATile<KT, HD, WR>::kSmem);
+}
+template <typename KT, int HD>
+cudaError_t configure_hd() {
+  cudaError_t e = configure_one<KT, HD, 1>();
+  if (e == cudaSuccess) e = configure_one<KT, HD, 2>();
+  if (e == cudaSuccess) e = configure_one<KT, HD, 4>();
+  if (e == cudaSuccess) e = configure_one<KT, HD, 8>();
+  return e;
+}
+
+template <typename KT, int HD, int WR>
+cudaError_t launch(const TreeAttnArgs& a, const TreeAttnShape& s, int sms, int* launches, cudaStream_t st) {
+  using T = TATile<KT, HD, WR>;
+  TAKernelArgs P;
+  P.a = a;
+  const int G = a.nq / a.kvh;
+  auto tiles = [&](int m) { return (m * G + T::RT - 1) / T::RT; };
+  // blocks per split: as many CTAs as SMs over all (sequence, KV head, row tile)
+  long long total = 0;
+  for (int i = 0; i < a.n_seqs; ++i)
+    total += (long long)((s.t0[i] + s.seqs[i].m + T::BN - 1) / T::BN) * a.kvh * tiles(s.seqs[i].m);
+  P.bps = (int)std::max<long long>(1, (total + sms - 1) / sms);
+  int splits = 1;
+  size_t part = 0;
+  for (int i = 0; i < a.n_seqs; ++i) {
+    P.t0[i] = s.t0[i];
+    const int m = s.seqs[i].m, ns = m ? ta_splits(s.t0[i] + m, T::BN, P.bps) : 1;
+    P.part0[i] = (int)part;
+    if (ns > 1) part += (size_t)ns * m * a.nq;
+    splits = std::max(splits, ns);
+  }
+  const dim3 grid(splits, a.kvh * tiles(s.max_m), a.n_seqs);
+  tree_attn_kernel<KT, HD, WR><<<grid, kTAThreads, T::kSmem, st>>>(P);
+  cudaError_t e = cudaGetLastError();
+  *launches += 1;
+  if (e != cudaSuccess || splits == 1) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((s.max_m * a.nq + 7) / 8, a.n_seqs);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  *launches += 1;
+  return cudaLaunchKernelEx(&cfg, tree_join_kernel<HD>, P, T::BN);
+}
+
+template <typename KT, int HD>
+cudaError_t launch_hd(const TreeAttnArgs& a, const TreeAttnShape& s, int sms, int* launches, cudaStream_t st) {
+  const int rows = s.max_m * (a.nq / a.kvh);  // rows of the largest sequence that share a KV head
+  if (rows <= 16) return launch<KT, HD, 1>(a, s, sms, launches, st);
+  if (rows <= 32) return launch<KT, HD, 2>(a, s, sms, launches, st);
+  if (rows <= 64) return launch<KT, HD, 4>(a, s, sms, launches, st);
+  return launch<KT, HD, 8>(a, s, sms, launches, st);
+}
+
+}  // namespace
+
+// Splits exist only while all CTAs fit the SMs once: with bps >= total / sms a
+// sequence of more than one split has at most 2 blocks / bps of them, so the split
+// sequences' CTAs are at most 2 sms, each with up to 128 rows.
+size_t tree_attn_part_rows(int sms) { return (size_t)2 * sms * 128; }
+
+cudaError_t configure_tree_attn() {
+  cudaError_t e = configure_hd<float, 64>();
+  if (e == cudaSuccess) e = configure_hd<float, 128>();
+  if (e == cudaSuccess) e = configure_hd<__nv_bfloat16, 64>();
+  if (e == cudaSuccess) e = configure_hd<__nv_bfloat16, 128>();
+  return e;
+}
+
+cudaError_t op_tree_attention(const TreeAttnArgs& a, const TreeAttnShape& s, int kv_dtype, int hd, int sms,
+                              int* launches, cudaStream_t st) {
+  if (kv_dtype == 0) return hd == 64 ? launch_hd<float, 64>(a, s, sms, launches, st)
+                                     : launch_hd<float, 128>(a, s, sms, launches, st);
+  return hd == 64 ? launch_hd<__nv_bfloat16, 64>(a, s, sms, launches, st)
+                  : launch_hd<__nv_bfloat16, 128>(a, s, sms, launches, st);
+}
+
+}  // namespace dllm

@@ -34,9 +34,101 @@ class GpuBuffer:
     def device_ptr(self) -> int:
         return int(self.ctx.lib.dllm_buf_device_ptr(self.handle) or 0)
 
+    @property
+    def __cuda_array_interface__(self) -> dict:
+        """The buffer's memory as a flat array (bf16 as int16 bits), e.g. for
+        torch.as_tensor(buf, device="cuda"). No stream is synchronised: order the
+        other library's work with the ctx stream (set_stream)."""
+        return {"shape": (self.n,), "typestr": {"f32": "<f4", "i32": "<i4", "bf16": "<i2"}[self.dtype],
+                "data": (self.device_ptr, False), "version": 3, "strides": None}
+
     def destroy(self):
         if self.handle:
             self.ctx.lib.dllm_buf_free(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+
+class RopePlan:
+    """Rotary frequencies of ropeAt on the device. Freed with the object."""
+
+    LAYOUTS = {"half": 0, "interleaved": 1}
+    SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+
+    def __init__(self, ctx: "KernelContext", layout: str, rotary_dim: int, theta: float, scaling: dict | None):
+        s = dict(scaling or {})
+        kind = s.pop("type", "none")
+        if layout not in self.LAYOUTS or kind not in self.SCALINGS:
+            raise _lib.DllmError(_lib.DLLM_EINVAL, f"ropePlan: unknown layout {layout!r} or scaling {kind!r}")
+        c = _lib.dllm_rope_config(self.LAYOUTS[layout], int(rotary_dim), float(theta), self.SCALINGS[kind],
+                                  float(s.pop("factor", 1.0)), int(s.pop("original_max_pos", 0)),
+                                  float(s.pop("beta_fast", 32.0)), float(s.pop("beta_slow", 1.0)),
+                                  float(s.pop("attention_factor", 0.0)))
+        if s:
+            raise _lib.DllmError(_lib.DLLM_EINVAL, f"ropePlan: unknown scaling keys {sorted(s)}")
+        self.ctx, self.handle = ctx, None
+        h = C.c_void_p()
+        ctx._check(ctx.lib.dllm_rope_plan_create(ctx.handle, C.byref(c), C.byref(h)), "ropePlan")
+        self.handle = h.value
+
+    def destroy(self):
+        if self.handle:
+            self.ctx.lib.dllm_rope_plan_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+
+class DraftTree:
+    """Drafted trees of one or more sequences (dllm_tree_create). Freed with the object."""
+
+    def __init__(self, ctx: "KernelContext", parents, counts=None, seqs=None):
+        self.ctx, self.handle = ctx, None
+        self.parents = np.array(parents, dtype=np.int32).reshape(-1)
+        self.counts = np.array([self.parents.size] if counts is None else counts, dtype=np.int32).reshape(-1)
+        self.seqs = np.array(range(self.counts.size) if seqs is None else seqs, dtype=np.int32).reshape(-1)
+        if self.seqs.size != self.counts.size or (self.counts < 0).any() or int(self.counts.sum()) != self.parents.size:
+            raise _lib.DllmError(_lib.DLLM_EINVAL, f"draftTree: {self.parents.size} parents for counts "
+                                                   f"{self.counts.tolist()} of sequences {self.seqs.tolist()}")
+        self.n = int(self.parents.size)
+        h = C.c_void_p()
+        ctx._check(ctx.lib.dllm_tree_create(ctx.handle, _lib.ptr(self.parents, C.c_int32),
+                                            _lib.ptr(self.counts, C.c_int32), _lib.ptr(self.seqs, C.c_int32),
+                                            self.counts.size, C.byref(h)), "draftTree")
+        self.handle = h.value
+
+    def accept(self, draft, picked) -> tuple[list, list]:
+        """Greedy verification: per sequence, the path of nodes whose tokens the picks
+        agree with and the new tokens. Node 0 is the sequence's last token; from it on,
+        the lowest child whose drafted token is the current node's pick continues the
+        path, and the last node's pick ends the new tokens."""
+        draft, picked = np.asarray(draft).reshape(-1), np.asarray(picked).reshape(-1)
+        if draft.size != self.n or picked.size != self.n:
+            raise _lib.DllmError(_lib.DLLM_EINVAL, f"accept: {draft.size} drafted, {picked.size} picked, {self.n} nodes")
+        paths, tokens, row0 = [], [], 0
+        for m in self.counts.tolist():
+            path, new = ([0], [int(picked[row0])]) if m else ([], [])
+            for j in range(1, m):
+                if self.parents[row0 + j] == path[-1] and draft[row0 + j] == new[-1]:
+                    path.append(j)
+                    new.append(int(picked[row0 + j]))
+            paths.append(path)
+            tokens.append(new)
+            row0 += m
+        return paths, tokens
+
+    def destroy(self):
+        if self.handle:
+            self.ctx.lib.dllm_tree_destroy(self.handle)
             self.handle = None
 
     def __del__(self):
@@ -75,9 +167,13 @@ class KernelContext:
 
     @staticmethod
     def _h(buf: GpuBuffer):
-        if not isinstance(buf, GpuBuffer) or not buf.handle:
+        if not isinstance(buf, (GpuBuffer, DraftTree, RopePlan)) or not buf.handle:
             raise ValueError("expected a live GpuBuffer")
         return buf.handle
+
+    @classmethod
+    def _opt(cls, buf):
+        return None if buf is None else cls._h(buf)
 
     def close(self):
         if getattr(self, "handle", None):
@@ -155,6 +251,20 @@ class KernelContext:
                                            label.encode()), "readF32")
         return out
 
+    def createI32(self, n: int, label: str = "") -> GpuBuffer:
+        out = C.c_void_p()
+        self._check(self.lib.dllm_create_i32(self.handle, max(0, int(n)), label.encode(), C.byref(out)), "createI32")
+        return GpuBuffer(self, out.value, int(n), "i32", label)
+
+    def writeI32(self, buf: GpuBuffer, values):
+        a = np.ascontiguousarray(values, dtype=np.int32).reshape(-1)
+        self._check(self.lib.dllm_write_i32(self.handle, self._h(buf), _lib.ptr(a, C.c_int32), a.size), "writeI32")
+
+    def readI32(self, buf: GpuBuffer, n: int | None = None) -> np.ndarray:
+        out = np.empty(buf.n if n is None else int(n), np.int32)
+        self._check(self.lib.dllm_read_i32(self.handle, self._h(buf), _lib.ptr(out, C.c_int32), out.size), "readI32")
+        return out
+
     # ---- ops (kernels.js:222-301)
     def matmul(self, xBuf, wBuf, n, din, dout) -> GpuBuffer:
         return self._out(self.lib.dllm_matmul, self._h(xBuf), self._h(wBuf), n, din, dout, n=n * dout,
@@ -192,6 +302,48 @@ class KernelContext:
         idx = C.c_int32()
         self._check(self.lib.dllm_argmax(self.handle, self._h(logitsBuf), n, C.byref(idx)), "argmax")
         return int(idx.value)
+
+    # ---- verification of drafted tokens (include/dllm.h; no counterpart in the reference)
+    def ropePlan(self, layout: str = "half", rotary_dim: int | None = None, theta: float | None = None,
+                 scaling: dict | None = None) -> RopePlan:
+        """Rotary frequencies for ropeAt. layout "half" (pairs i, i + rotary_dim / 2) or
+        "interleaved" (2i, 2i + 1); rotary_dim defaults to the head size, theta to the
+        config's. scaling: None, {"type": "linear" | "ntk", "factor": f} or {"type":
+        "yarn", "factor": f, "original_max_pos": n[, "beta_fast": 32, "beta_slow": 1]};
+        "attention_factor" overrides the factor on cos and sin."""
+        return RopePlan(self, layout, self.HD if rotary_dim is None else rotary_dim,
+                        self.cfg.rope_theta if theta is None else theta, scaling)
+
+    def ropeAt(self, plan: RopePlan, positions: GpuBuffer, n: int, qBuf: GpuBuffer | None = None,
+               kBuf: GpuBuffer | None = None, qOut: GpuBuffer | None = None, kOut: GpuBuffer | None = None):
+        """Row t of q [n, NQ*HD] and k [n, KVH*HD] at positions[t]; in place without outputs."""
+        h, o = self._h, self._opt
+        self._check(self.lib.dllm_rope_at(self.handle, h(plan), h(positions), n, o(qBuf), o(kBuf), o(qOut), o(kOut)),
+                    "ropeAt")
+        return qOut or qBuf, kOut or kBuf
+
+    def draftTree(self, parents, counts=None, seqs=None) -> DraftTree:
+        """Drafted trees of one or more cache sequences: counts[i] nodes for sequence
+        seqs[i] (default i), each node with the index of its parent in the sequence
+        (below its own), -1 for a root. counts defaults to one sequence."""
+        return DraftTree(self, parents, counts, seqs)
+
+    def pickTokens(self, logits: GpuBuffer, n: int, history=None, penalties: GpuBuffer | None = None, bias=None,
+                   mask: GpuBuffer | None = None, tree: DraftTree | None = None, draft: GpuBuffer | None = None,
+                   out: GpuBuffer | None = None, tokens: GpuBuffer | None = None) -> GpuBuffer:
+        """One token per row of logits [n, vocab] under penalties for repeated tokens,
+        biases and a grammar mask (dllm_pick_tokens); i32 [n], -1 where the mask allows
+        nothing. history: (tokens, offsets, prompt_lens or None); bias: (tokens, values,
+        offsets); `out` also receives the processed logits."""
+        if tokens is None:
+            tokens = self.createI32(n, "picked")
+        h, o = self._h, self._opt
+        ht, ho, hp = history if history is not None else (None, None, None)
+        bt, bv, bo = bias if bias is not None else (None, None, None)
+        a = _lib.dllm_pick(n, h(logits), o(ht), o(ho), o(hp), o(penalties), o(bt), o(bv), o(bo), o(mask), o(tree),
+                           o(draft), o(out), h(tokens))
+        self._check(self.lib.dllm_pick_tokens(self.handle, C.byref(a)), "pickTokens")
+        return tokens
 
     def __del__(self):
         try:

@@ -16,7 +16,7 @@ import numpy as np
 
 from . import _lib, frames
 from .constants import FRAME
-from .kernels import GpuBuffer, KernelContext
+from .kernels import DraftTree, GpuBuffer, KernelContext
 
 
 # ---- assignLayers (pipeline.js:6-23) ---------------------------------------------------
@@ -124,6 +124,22 @@ class _KvTensor:
         return out
 
 
+class _KvPool:
+    """A stage's whole K or V pool in device memory, shape [layers, max_seqs *
+    pages_per_seq, KVH, page, HD], for torch.as_tensor(pool, device="cuda") (bf16 as
+    int16 bits). Work on it is ordered with the stage's only on the ctx stream."""
+
+    def __init__(self, stage: "Stage", which: int):
+        f = stage.k.cfg
+        self.stage = stage  # keeps the memory alive
+        self.__cuda_array_interface__ = {
+            "shape": (stage.end - stage.start, f.max_seqs * stage.pages_per_seq(), f.num_kv_heads, f.kv_page_size,
+                      f.head_dim),
+            "typestr": "<i2" if f.kv_dtype == "bf16" else "<f4",
+            "data": (int(stage.lib.dllm_stage_kv_device_ptr(stage.handle, which) or 0), False),
+            "version": 3, "strides": None}
+
+
 class _KvLayer:
     def __init__(self, stage, layer):
         self.k = _KvTensor(stage, layer, 0)
@@ -213,6 +229,44 @@ class Stage:
         p = np.ascontiguousarray(pages, dtype=np.int32)
         self.k._check(self.lib.dllm_stage_set_page_table(self.handle, seq, _lib.ptr(p, C.c_int32), p.size),
                       "set_page_table")
+
+    # ---- drafted trees (include/dllm.h; no counterpart in the reference)
+    def kv_pool(self, which: str) -> _KvPool:
+        """The device memory of the "k" or "v" cache (see _KvPool)."""
+        return _KvPool(self, {"k": 0, "v": 1}[which])
+
+    def append_tree(self, L: int, tree: DraftTree, kBuf: GpuBuffer, vBuf: GpuBuffer):
+        """K/V rows of a tree's nodes -> slots T0 + node of their sequences (T0 unchanged)."""
+        h = self.k._h
+        self.k._check(self.lib.dllm_stage_append_tree(self.handle, L, h(tree), h(kBuf), h(vBuf)), "append_tree")
+
+    def tree_attention(self, L: int, tree: DraftTree, qBuf: GpuBuffer, out: GpuBuffer | None = None) -> GpuBuffer:
+        """Every node of a tree over its sequence's cached slots and its own ancestors."""
+        k = self.k
+        if out is None:
+            out = k.createF32(tree.n * k.NQ * k.HD, "tree_attn_out")
+        k._check(self.lib.dllm_stage_tree_attention(self.handle, L, k._h(tree), k._h(qBuf), k._h(out)), "tree_attention")
+        return out
+
+    def commit_tree(self, tree: DraftTree, paths):
+        """Keep one path of nodes per sequence (root first): its K/V rows move to slots
+        T0.. of every layer and T0 advances by its length."""
+        lens = np.array([len(p) for p in paths], dtype=np.int32)
+        if lens.size != tree.counts.size:
+            raise _lib.DllmError(_lib.DLLM_EINVAL, f"commit_tree: {lens.size} paths for {tree.counts.size} sequences")
+        flat = np.array([j for p in paths for j in p] or [0], dtype=np.int32)
+        self.k._check(self.lib.dllm_stage_commit_tree(self.handle, self.k._h(tree), _lib.ptr(flat, C.c_int32),
+                                                      _lib.ptr(lens, C.c_int32)), "commit_tree")
+
+    def forward_tree(self, tree: DraftTree, hBuf: GpuBuffer, tokens: GpuBuffer | None = None,
+                     logits: GpuBuffer | None = None) -> GpuBuffer:
+        """The stage's layers for a tree's rows (at most 128), h [n, D] in place; `tokens`
+        replaces h by their embeddings first, `logits` [n, vocab] receives the LM head's
+        rows. T0 stays until commit_tree."""
+        o = self.k._opt
+        self.k._check(self.lib.dllm_stage_forward_tree(self.handle, self.k._h(tree), self.k._h(hBuf), o(tokens),
+                                                       o(logits)), "forward_tree")
+        return hBuf
 
     def close(self):
         if self._owned and getattr(self, "handle", None):
@@ -381,6 +435,27 @@ class LeaderPipeline:
         out = np.empty(steps, np.int32)
         self.k._check(self.lib.dllm_leader_read_tokens(self.handle, _lib.ptr(out, C.c_int32), steps), "read_tokens")
         return [int(x) for x in out]
+
+    def verify_tree(self, tree: DraftTree, draft, **rules) -> list[list[int]]:
+        """One verification step of drafted trees (single node). draft: the nodes' tokens,
+        node 0 of a sequence its last token, not yet in the cache. All nodes go through
+        one pass, each gets a token (`rules`: the keyword arguments of pickTokens), and
+        the longest path that the picks agree with is kept in the cache. Returns the new
+        tokens of each sequence, at least one."""
+        if not self.singleNode:
+            raise _lib.DllmError(_lib.DLLM_EINVAL, "verify_tree: the leader's stage must own every layer (single node)")
+        k, cfg = self.k, self.k.cfg
+        draft = np.ascontiguousarray(draft, dtype=np.int32).reshape(-1)
+        if draft.size != tree.n or draft.size == 0 or draft.min() < 0 or draft.max() >= cfg.vocab_size:
+            raise _lib.DllmError(_lib.DLLM_EINVAL, f"verify_tree: need {tree.n} token ids in [0, {cfg.vocab_size})")
+        tok = k.createI32(tree.n, "draft")
+        k.writeI32(tok, draft)
+        h, logits = k.createF32(tree.n * k.D, "tree rows"), k.createF32(tree.n * cfg.vocab_size, "tree logits")
+        self.stage.forward_tree(tree, h, tok, logits)
+        picked = k.readI32(k.pickTokens(logits, tree.n, tree=tree, draft=tok, **rules))
+        paths, new = tree.accept(draft, picked)
+        self.stage.commit_tree(tree, paths)
+        return new
 
     def set_keep_logits(self, steps: int):
         self.k._check(self.lib.dllm_leader_set_keep_logits(self.handle, steps), "set_keep_logits")

@@ -121,6 +121,11 @@ int dllm_fill_normal_bf16(dllm_ctx* ctx, dllm_buf* buf, uint64_t seed, float std
 int dllm_fill_const_bf16(dllm_ctx* ctx, dllm_buf* buf, float value);
 int dllm_create_bf16(dllm_ctx* ctx, size_t n, const char* label, dllm_buf** out);
 
+/* Integer buffers: token ids, positions, offsets and mask words of the calls below. */
+int dllm_create_i32(dllm_ctx* ctx, size_t n, const char* label, dllm_buf** out);
+int dllm_write_i32(dllm_ctx* ctx, dllm_buf* buf, const int32_t* src, size_t n);
+int dllm_read_i32(dllm_ctx* ctx, const dllm_buf* buf, int32_t* dst, size_t n);
+
 /* ---- ops: one launcher per shader (kernels.js:222-301) --------------------- */
 /* ctx.matmul(x, w, n, din, dout) (kernels.js:222-231): out[t,j] = sum_k x[t,k]*W[j,k]. */
 int dllm_matmul(dllm_ctx* ctx, const dllm_buf* x, const dllm_buf* w, int n, int din, int dout, dllm_buf** out);
@@ -308,6 +313,101 @@ int dllm_attention_noalloc(const float* q, const float* kcache, const float* vca
  * code goes to *device_error (may be NULL). Allocates nothing. No counterpart in
  * the reference (readF32's bounded wait, kernels.js:201-207, is the model). */
 int dllm_attention_noalloc_status(void* cuda_stream, int timeout_ms, int* device_error);
+
+/* ---- verification of drafted tokens --------------------------------------------
+ * No counterpart in the reference, which decodes one token per pass. A draft
+ * proposes a tree of tokens per sequence; one pass scores all nodes, and the
+ * longest path that the model agrees with is kept:
+ *   dllm_tree_create         the trees' shape
+ *   dllm_rope_at             q and k at the nodes' positions, T0 + depth
+ *   dllm_stage_append_tree   K/V rows of the nodes, behind the cached context
+ *   dllm_stage_tree_attention  every node over the context and its own ancestors
+ *   dllm_pick_tokens         one token per node under penalties, biases and a mask
+ *   dllm_stage_commit_tree   keep a path's K/V rows, T0 += its length
+ * dllm_stage_forward_tree runs the first four (with the layers' projections) for
+ * every layer of a stage. All work is enqueued on the ctx stream, in order; scratch
+ * belongs to the ctx, so calls of one ctx, and graphs captured from them, must not
+ * overlap on the GPU. T0 values and paths become kernel arguments: a captured call
+ * replays with those of its capture. */
+
+typedef struct dllm_tree dllm_tree;
+typedef struct dllm_rope_plan dllm_rope_plan;
+
+enum { DLLM_ROPE_HALF = 0, DLLM_ROPE_INTERLEAVED = 1 };
+enum { DLLM_ROPE_PLAIN = 0, DLLM_ROPE_LINEAR = 1, DLLM_ROPE_NTK = 2, DLLM_ROPE_YARN = 3 };
+typedef struct dllm_rope_config {
+  int32_t layout;            /* pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) */
+  int32_t rotary_dim;        /* leading dims of a head that turn: even, 2..head_dim */
+  double theta;              /* inverse frequency i: theta^(-2i / rotary_dim) */
+  int32_t scaling;           /* PLAIN; LINEAR: frequencies / factor; NTK: theta * factor^(rd / (rd - 2));
+                                YARN: a ramp from plain (fast pairs) to linear (slow pairs) */
+  double factor;             /* >= 1 (not PLAIN) */
+  int32_t original_max_pos;  /* YARN: the context the frequencies were trained on */
+  double beta_fast, beta_slow; /* YARN: turns over that context between which the ramp runs (32, 1) */
+  double attention_factor;   /* scales cos and sin; 0: 0.1 ln(factor) + 1 for YARN, else 1 */
+} dllm_rope_config;
+int dllm_rope_plan_create(dllm_ctx* ctx, const dllm_rope_config* cfg, dllm_rope_plan** out);
+void dllm_rope_plan_destroy(dllm_rope_plan* plan);
+/* Row t of q [n, NQ*HD] and k [n, KVH*HD] (either may be NULL) at positions[t] (i32,
+ * any value); q_out / k_out NULL: in place. Angles are reduced in 64 bits, so
+ * positions far beyond 2^24 keep their precision (dllm_rope_q/k multiply in 32). */
+int dllm_rope_at(dllm_ctx* ctx, const dllm_rope_plan* plan, const dllm_buf* positions, int n, dllm_buf* q, dllm_buf* k,
+                 dllm_buf* q_out, dllm_buf* k_out);
+
+/* Trees of n_seqs sequences (1..128): counts[i] nodes (0..64) for cache sequence
+ * seqs[i] (NULL: i; distinct), their parents in turn: an index within the sequence
+ * below the node's own, or -1 for a root. Node j of a sequence is batch row (nodes
+ * of the sequences before) + j, and its K/V row goes to slot T0 + j. */
+int dllm_tree_create(dllm_ctx* ctx, const int32_t* parents, const int32_t* counts, const int32_t* seqs, int n_seqs,
+                     dllm_tree** out);
+void dllm_tree_destroy(dllm_tree* tree);
+
+/* Arguments of dllm_pick_tokens; optional buffers may be NULL. V = vocab_size; the
+ * sequences are the tree's, or without a tree the n rows themselves. */
+typedef struct dllm_pick {
+  int32_t n;
+  const dllm_buf* logits;          /* f32 [n, V] */
+  const dllm_buf* history;         /* i32: tokens of all sequences; ids outside [0, V) are ignored */
+  const dllm_buf* history_offsets; /* i32 [seqs + 1]: sequence s has [offsets[s], offsets[s + 1]) */
+  const dllm_buf* prompt_lens;     /* i32 [seqs]: leading tokens that were given, not generated; NULL: none */
+  const dllm_buf* penalties;       /* f32 [seqs, 3]: repetition, frequency, presence */
+  const dllm_buf* bias_tokens;     /* i32: entries of all sequences; of a token listed twice the last one counts */
+  const dllm_buf* bias_values;     /* f32 */
+  const dllm_buf* bias_offsets;    /* i32 [seqs + 1] */
+  const dllm_buf* mask;            /* i32 [n, ceil(V / 32)]: bit t % 32 of word t / 32 allows token t */
+  const dllm_tree* tree;           /* rows are the tree's nodes */
+  const dllm_buf* draft;           /* i32 [n], with a tree: the nodes' tokens */
+  dllm_buf* out;                   /* f32 [n, V]: the processed logits; may be `logits` */
+  dllm_buf* tokens;                /* i32 [n] */
+} dllm_pick;
+/* With c = occurrences of token t among the generated tokens of the row's history (a
+ * node's history ends with the drafted tokens from its root to itself):
+ *   y = x > 0 ? x / repetition : x * repetition   where t occurs in the history
+ *   y = y - frequency * c - presence              where c > 0
+ *   y += bias; y = -inf where the mask forbids t
+ * tokens[row] is the lowest allowed index with the largest y (NaN counts as -inf), or
+ * -1 where the mask allows nothing. Offsets outside their buffers are clamped. */
+int dllm_pick_tokens(dllm_ctx* ctx, const dllm_pick* args);
+
+/* K/V rows k, v [n, KVH*HD] fp32 -> slots T0 + node of each sequence; T0 unchanged. */
+int dllm_stage_append_tree(dllm_stage* st, int layer, const dllm_tree* tree, const dllm_buf* k, const dllm_buf* v);
+/* out[row] = attention of node `row` (q [n, NQ*HD], after RoPE) over its sequence's
+ * slots [0, T0) and the slots of its ancestors and itself. A non-finite value in a
+ * drafted K/V row reaches only the nodes that see the row. */
+int dllm_stage_tree_attention(dllm_stage* st, int layer, const dllm_tree* tree, const dllm_buf* q, dllm_buf* out);
+/* Keep one path per sequence: lens[i] node indices (a root, then a child each; 0: keep
+ * nothing), all sequences' in turn in `path`. Slot T0 + path[j] -> T0 + j in every
+ * layer of the stage; T0 += lens[i]. The slots behind hold leftovers. */
+int dllm_stage_commit_tree(dllm_stage* st, const dllm_tree* tree, const int32_t* path, const int32_t* lens);
+/* Every layer of the stage for the tree's rows (at most 128): h [n, D] in place; `tokens`
+ * (i32 [n], may be NULL) first replaces h by their embeddings; `logits` (f32 [n, V], may
+ * be NULL) receives final norm + LM head. K/V rows are appended, T0 is unchanged. */
+int dllm_stage_forward_tree(dllm_stage* st, const dllm_tree* tree, dllm_buf* h, const dllm_buf* tokens,
+                            dllm_buf* logits);
+/* The stage's K (which = 0) or V (1) pool on the device, [layers][max_seqs *
+ * pages_per_seq][KVH][page][HD] in the cache's type, for hosts that fill or inspect the
+ * cache with kernels of their own on the ctx stream. */
+void* dllm_stage_kv_device_ptr(const dllm_stage* st, int which);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,78 @@
+"""Host side of verifying drafted tokens: the greedy acceptance of a tree, and the
+calls that are refused before anything reaches a GPU."""
+import ctypes as C
+import importlib
+
+import numpy as np
+import pytest
+
+kernels = importlib.import_module("distributed-llm1_b200.kernels")
+
+
+def bare_tree(parents, counts):
+    t = object.__new__(kernels.DraftTree)
+    t.ctx, t.handle = None, None
+    t.parents, t.counts = np.array(parents, np.int32), np.array(counts, np.int32)
+    t.n = len(parents)
+    return t
+
+
+def test_accept_walks_the_picks():
+    #        0 -> 1, 2;  1 -> 3;  2 -> 4, 5;  5 -> 6
+    t = bare_tree([-1, 0, 0, 1, 2, 2, 5], [7])
+    draft = [10, 11, 12, 13, 14, 15, 16]
+    assert t.accept(draft, [12, 0, 15, 0, 0, 16, 99]) == ([[0, 2, 5, 6]], [[12, 15, 16, 99]])
+    assert t.accept(draft, [77, 0, 0, 0, 0, 0, 0]) == ([[0]], [[77]])
+    assert t.accept(draft, [11, 13, 0, 55, 0, 0, 0]) == ([[0, 1, 3]], [[11, 13, 55]])
+
+
+def test_accept_takes_the_lowest_of_equal_children_and_ignores_other_roots():
+    t = bare_tree([-1, 0, 0, 2, -1], [5])
+    assert t.accept([1, 5, 5, 6, 5], [5, 8, 6, 0, 0]) == ([[0, 1]], [[5, 8]])
+
+
+def test_accept_several_sequences_and_empty_ones():
+    t = bare_tree([-1, 0, -1], [2, 0, 1])
+    assert t.accept([4, 5, 9], [5, 6, 7]) == ([[0, 1], [], [0]], [[5, 6], [], [7]])
+    # nothing allowed (-1) ends a path
+    assert t.accept([4, 5, 9], [-1, 6, -1]) == ([[0], [], [0]], [[-1], [], [-1]])
+
+
+def test_accept_refuses_other_sizes(dllm):
+    t = bare_tree([-1, 0], [2])
+    with pytest.raises(dllm.DllmError):
+        t.accept([1], [1, 2])
+    with pytest.raises(dllm.DllmError):
+        t.accept([1, 2], [1, 2, 3])
+
+
+@pytest.mark.parametrize("parents,counts,seqs", [([-1, 0], [1], None), ([-1], [2], None), ([-1, 0], [3, -1], None),
+                                                 ([-1, -1], [1, 1], [0])])
+def test_tree_counts_are_checked(dllm, parents, counts, seqs):
+    with pytest.raises(dllm.DllmError):
+        kernels.DraftTree(None, parents, counts, seqs)
+
+
+def test_rope_plan_names_are_checked(dllm):
+    for kw in ({"layout": "spiral", "scaling": None}, {"layout": "half", "scaling": {"type": "cubic"}},
+               {"layout": "half", "scaling": {"type": "linear", "factor": 2.0, "speed": 3}}):
+        with pytest.raises(dllm.DllmError):
+            kernels.RopePlan(None, kw["layout"], 64, 1e4, kw["scaling"])
+
+
+def test_null_handles_are_refused(dllm):
+    lib = dllm.load_library()
+    out = C.c_void_p()
+    one = (C.c_int32 * 1)(0)
+    assert lib.dllm_tree_create(None, one, one, None, 1, C.byref(out)) == 1
+    assert lib.dllm_rope_plan_create(None, None, C.byref(out)) == 1
+    assert lib.dllm_rope_at(None, None, None, 1, None, None, None, None) == 1
+    assert lib.dllm_pick_tokens(None, None) == 1
+    assert lib.dllm_create_i32(None, 4, b"", C.byref(out)) == 1
+    for fn in (lib.dllm_stage_append_tree, lib.dllm_stage_tree_attention):
+        assert fn(None, 0, None, None, None) == 1
+    assert lib.dllm_stage_commit_tree(None, None, None, None) == 1
+    assert lib.dllm_stage_forward_tree(None, None, None, None, None) == 1
+    assert not lib.dllm_stage_kv_device_ptr(None, 0)
+    lib.dllm_tree_destroy(None)
+    lib.dllm_rope_plan_destroy(None)
