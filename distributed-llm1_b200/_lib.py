@@ -149,7 +149,7 @@ SIGNATURES = {
     "dllm_pick_tokens": (C.c_int, [P, C.POINTER(dllm_pick)]),
     "dllm_stage_append_tree": (C.c_int, [P, C.c_int, P, P, P]),
     "dllm_stage_tree_attention": (C.c_int, [P, C.c_int, P, P, P]),
-    "dllm_stage_commit_tree": (C.c_int, [P, P, I32P, I32P]),
+    "dllm_stage_commit_tree": (C.c_int, [P, P, P, P]),
     "dllm_stage_forward_tree": (C.c_int, [P, P, P, P, P]),
     "dllm_stage_kv_device_ptr": (P, [P, C.c_int]),
     "dllm_attention_noalloc": (C.c_int, [P, P, P, P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, P]),

@@ -78,6 +78,8 @@ struct dllm_ctx {
   size_t tc_scratch_bytes = 0;
   // partial results of split tree attention, sized for any call; allocated with the first tree
   float* tree_part = nullptr;
+  // token picks: per-row keys, then arrival counters (zero between calls)
+  unsigned long long* pick_best = nullptr;
   // freed buffers kept for reuse, by size in bytes
   std::multimap<size_t, void*> buf_cache;
   size_t buf_cache_bytes = 0;
@@ -846,6 +848,7 @@ void ctx_free(dllm_ctx* c) {
   dev_free(c->attn_rows);
   dev_free(c->tc_scratch);
   dev_free(c->tree_part);
+  dev_free(c->pick_best);
   for (auto& kv : c->buf_cache) cudaFree(kv.second);
   c->buf_cache.clear();
   if (c->err_host) cudaFreeHost(c->err_host);
@@ -934,6 +937,7 @@ int dllm_init_kernels(int device, const dllm_config* cfg, dllm_ctx** out) {
   if (cudaMallocHost(&c->best_host, sizeof(unsigned long long)) != cudaSuccess) return fail(DLLM_ENOMEM);
   if (dev_alloc(c, &c->err_dev, 1, "error flag")) return fail(DLLM_ENOMEM);
   if (dev_alloc(c, &c->best, 1, "argmax")) return fail(DLLM_ENOMEM);
+  if (dev_alloc(c, &c->pick_best, (size_t)dllm::kPickMaxRows * 3 / 2, "pick keys")) return fail(DLLM_ENOMEM);
   std::vector<float> fr;
   rope_table(f, &fr);
   if (dev_alloc(c, &c->freq, fr.size(), "rope table")) return fail(DLLM_ENOMEM);
@@ -2338,7 +2342,7 @@ int dllm_rope_at(dllm_ctx* c, const dllm_rope_plan* p, const dllm_buf* positions
   a.rotary = p->rotary;
   a.interleaved = p->interleaved;
   a.factor = p->factor;
-  CK(c, dllm::op_rope_at(a, c->stream));
+  CK(c, dllm::op_rope_at(a, c->sms, c->stream));
   c->launches += 1;
   return DLLM_OK;
 }
@@ -2406,7 +2410,8 @@ int dllm_pick_tokens(dllm_ctx* c, const dllm_pick* p) {
   if (!c) return DLLM_EINVAL;
   if (!p) return set_err(c, DLLM_EINVAL, "pickTokens: null arguments");
   const int n = p->n, V = c->cfg.vocab_size;
-  if (n <= 0) return set_err(c, DLLM_EINVAL, "pickTokens: invalid n=%d", n);
+  if (n <= 0 || n > dllm::kPickMaxRows)
+    return set_err(c, DLLM_EINVAL, "pickTokens: n=%d outside 1..%d", n, dllm::kPickMaxRows);
   if ((p->tree != nullptr) != (p->draft != nullptr))
     return set_err(c, DLLM_EINVAL, "pickTokens: a tree comes with its drafted tokens");
   if (p->tree && (p->tree->ctx != c || p->tree->n != n))
@@ -2465,6 +2470,8 @@ int dllm_pick_tokens(dllm_ctx* c, const dllm_pick* p) {
   if (p->mask) a.mask = (const uint32_t*)p->mask->ptr;
   a.n_seqs = (int)b;
   a.max_m = 1;
+  a.best = c->pick_best;
+  a.arrived = (unsigned int*)(c->pick_best + dllm::kPickMaxRows);
   if (p->tree) {
     a.seqs = p->tree->seqs_dev();
     a.anc = p->tree->anc_dev();

@@ -12,33 +12,28 @@
 // its sequence's tokens, then the drafted tokens on the path from the root to it.
 //
 // Bound by memory: the logits are read once (and written once); history, biases
-// and mask are small beside them. The vocabulary is cut into one slice per CTA of a
-// cluster. A CTA counts the history's tokens that fall into its slice in shared
-// memory (integer atomics, so their order does not matter), then streams its
-// slice of kRows rows that share that history; a tree's row adds its own path's
-// tokens before and takes them out after. The CTAs' best (value, index) keys meet in
-// the first CTA's shared memory: no global scratch, nothing to reset, one launch.
-#include <cooperative_groups.h>
+// and mask are small beside them. A CTA takes one slice of the vocabulary for one
+// row, or for several nodes of a tree: it counts the history's tokens that fall into
+// its slice in shared memory (integer atomics, so their order does not matter) and
+// streams its slice of those rows, a tree's node correcting the counts by the path
+// tokens it does not share with the node before. A thread keeps U 16-byte groups of
+// a row in registers and loads the next row's as it uses them up, the first row's
+// before the counting, so the logits stay in flight throughout. The slices' best
+// (value, index) keys meet in one 64-bit atomicMax per row (the largest key wins in
+// any order); the CTA that arrives last writes the token and clears the key.
+#include <algorithm>
+#include <climits>
 
 #include "verify.cuh"
-
-namespace cg = cooperative_groups;
 
 namespace dllm {
 namespace {
 
 constexpr int kPickThreads = 512;
 constexpr int kPickWarps = kPickThreads / 32;
-constexpr int kMaxCluster = 16;
-constexpr int kMaxChunk = 12288;  // tokens of a slice held in shared memory at a time
-constexpr int kMaxRowsPerCta = 8;
+constexpr int kMaxRowsPerCta = 16;
 
 constexpr uint32_t kGiven = 0x80000000u;  // the token occurs among the given (prompt) tokens
-
-struct PickSmem {
-  unsigned long long key[kMaxRowsPerCta][kMaxCluster];  // of the first CTA: every CTA's best
-  unsigned long long warp_key[kMaxRowsPerCta][kPickWarps];
-};
 
 // Best allowed token so far of one thread, which sees tokens in ascending order.
 struct Best {
@@ -54,8 +49,7 @@ struct Best {
 
 struct RowRules {
   float rep, freq, pres;
-  const uint32_t* mask;     // the row's words or null
-  const float* bias_val;    // of the row's sequence or null
+  const float* bias_val;  // the sequence's bias entries
 };
 
 // The rules above for one token. cnt: its count word; b: 1 + its entry in the bias
@@ -72,198 +66,224 @@ DLLM_DEV float apply(float x, uint32_t cnt, uint32_t b, const RowRules& r) {
 
 DLLM_DEV int clampi(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
 
-// Grid: clusters of `csize` CTAs; cluster = (sequence, group of `rows` rows).
-__global__ void __launch_bounds__(kPickThreads) pick_kernel(const PickArgs a, int rows, int groups, int slice, int chunk) {
-  extern __shared__ __align__(16) uint32_t dyn[];  // counts [chunk], then bias entries [chunk]
-  __shared__ PickSmem sm;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int csize = cluster.num_blocks(), rank = cluster.block_rank();
-  const int item = blockIdx.x / csize;
-  const int s = item / groups, group = item - s * groups;
-  // the sequence's rows that this cluster handles
+// One 16-byte group of a row: tokens [t, t + 4), some of which may lie outside the
+// vocabulary at a row's ends (rows whose length is no multiple of 4 start inside a
+// group). bits: which of the four are allowed tokens.
+struct Group {
+  float v[4];
+  uint32_t bits;
+};
+
+DLLM_DEV void load_group(Group& g, const float* x, const uint32_t* mask, int t, int vocab) {
+  if (t >= 0 && t + 3 < vocab) {
+    const float4 f = __ldcs(reinterpret_cast<const float4*>(x + t));
+    g.v[0] = f.x, g.v[1] = f.y, g.v[2] = f.z, g.v[3] = f.w;
+    g.bits = 0xfu;
+    if (mask) {
+      const int w = t >> 5, sh = t & 31;
+      g.bits = mask[w] >> sh;
+      if (sh > 28) g.bits |= mask[w + 1] << (32 - sh);
+    }
+  } else {
+    g.bits = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int tok = t + e;
+      g.v[e] = 0.f;
+      if (tok < 0 || tok >= vocab) continue;
+      g.v[e] = x[tok];
+      if (!mask || (mask[tok >> 5] >> (tok & 31) & 1)) g.bits |= 1u << e;
+    }
+  }
+}
+
+// The four count (or bias) words of a group: words [at, at + 4) of a shared array
+// whose groups are aligned for shift 0 and lie `shift` words earlier otherwise; two
+// aligned reads cover them.
+DLLM_DEV void four_words(uint32_t (&r)[4], const uint32_t* a, int i, int shift) {
+  const uint4 hi = *reinterpret_cast<const uint4*>(a + 4 * i + 4);
+  if (shift == 0) {
+    r[0] = hi.x, r[1] = hi.y, r[2] = hi.z, r[3] = hi.w;
+    return;
+  }
+  const uint4 lo = *reinterpret_cast<const uint4*>(a + 4 * i);
+  if (shift == 1)
+    r[0] = lo.w, r[1] = hi.x, r[2] = hi.y, r[3] = hi.z;
+  else if (shift == 2)
+    r[0] = lo.z, r[1] = lo.w, r[2] = hi.x, r[3] = hi.y;
+  else
+    r[0] = lo.y, r[1] = lo.z, r[2] = lo.w, r[3] = hi.x;
+}
+
+// Grid (slices, row groups of a sequence, sequences). U: groups per thread and row,
+// so a slice has 2048 U tokens.
+template <int U>
+__global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a, int rows) {
+  constexpr int kSlice = kPickThreads * 4 * U;
+  constexpr int kWords = kSlice + 4;  // a slice's tokens and the 4 before it (rows start up to 3 tokens early)
+  extern __shared__ __align__(16) uint32_t dyn[];  // counts, then bias entries
+  __shared__ unsigned long long warp_key[kMaxRowsPerCta][kPickWarps];
+  const int tid = threadIdx.x, s = blockIdx.z;
   const int m = a.seqs ? a.seqs[s].m : 1;
   const int row0 = a.seqs ? a.seqs[s].row0 : s;
-  const int r0 = group * rows, r1 = min(m, r0 + rows);
-  if (r0 >= r1) return;  // the whole cluster leaves
-  cluster.barrier_arrive();
-
-  const bool counting = a.penalties != nullptr;
-  uint32_t* cnt = dyn;
-  uint32_t* bia = counting ? dyn + chunk : dyn;
-  int h0 = 0, h1 = 0, given = 0;
-  if (counting && a.hist) {
-    h0 = clampi(a.hist_off[s], 0, a.hist_total);
-    h1 = clampi(a.hist_off[s + 1], h0, a.hist_total);
-    given = h0 + (a.prompt ? clampi(a.prompt[s], 0, h1 - h0) : 0);
-  }
-  int b0 = 0, b1 = 0;
-  if (a.bias_tok) {
-    b0 = clampi(a.bias_off[s], 0, a.bias_total);
-    b1 = clampi(a.bias_off[s + 1], b0, a.bias_total);
-  }
-  RowRules r;
-  r.rep = counting ? a.penalties[3 * s] : 1.f;
-  r.freq = counting ? a.penalties[3 * s + 1] : 0.f;
-  r.pres = counting ? a.penalties[3 * s + 2] : 0.f;
-  r.bias_val = a.bias_tok ? a.bias_val + b0 : nullptr;
+  const int r0 = blockIdx.y * rows, r1 = min(m, r0 + rows);
+  if (r0 >= r1) return;
+  const int c0 = blockIdx.x * kSlice;  // the slice: tokens [c0 - shift, c0 - shift + kSlice) of a row
   const int words = (a.vocab + 31) / 32;
-  const int v0 = rank * slice, v1 = min(a.vocab, v0 + slice);
+  // a row's first group starts `shift` tokens before its slice, where its address is 16-byte aligned
+  auto shift_of = [&](int row) { return (int)(((size_t)row * a.vocab) & 3); };
+  auto mask_of = [&](int row) { return a.mask ? a.mask + (size_t)row * words : nullptr; };
 
-  if (threadIdx.x < kMaxRowsPerCta * kPickWarps) sm.warp_key[threadIdx.x / kPickWarps][threadIdx.x % kPickWarps] = 0ull;
-  for (int c0 = v0; c0 < v1; c0 += chunk) {
-    const int n = min(chunk, v1 - c0);
-    __syncthreads();  // the previous chunk's counts are done with
-    if (counting || a.bias_tok) {
-      const int fill = (counting ? chunk : 0) + (a.bias_tok ? chunk : 0);
-      for (int i = threadIdx.x; i < fill / 4; i += kPickThreads) reinterpret_cast<uint4*>(dyn)[i] = make_uint4(0, 0, 0, 0);
-      __syncthreads();
-#pragma unroll 4
-      for (int i = h0 + threadIdx.x; i < h1; i += kPickThreads) {
-        const unsigned t = (unsigned)(a.hist[i] - c0);  // ids outside the vocabulary fall into no slice
-        if (t < (unsigned)n) {
-          if (i < given)
-            atomicOr(cnt + t, kGiven);
-          else
-            atomicAdd(cnt + t, 1u);
-        }
-      }
-      for (int i = b0 + threadIdx.x; i < b1; i += kPickThreads) {
-        const unsigned t = (unsigned)(a.bias_tok[i] - c0);
-        if (t < (unsigned)n) atomicMax(bia + t, (uint32_t)(i - b0 + 1));  // of a token listed twice the last entry
-      }
-      __syncthreads();
-    }
-#pragma unroll 1
-    for (int q = r0; q < r1; ++q) {
-      const int row = row0 + q;
-      if (counting && a.seqs) {  // the drafted tokens on the way to this node
-        const unsigned long long anc = a.anc[row];
-        if (threadIdx.x < m && (anc >> threadIdx.x & 1)) {
-          const unsigned t = (unsigned)(a.draft[row0 + threadIdx.x] - c0);
-          if (t < (unsigned)n) atomicAdd(cnt + t, 1u);
-        }
-        __syncthreads();
-      }
-      r.mask = a.mask ? a.mask + (size_t)row * words : nullptr;
-      const float* x = a.logits + (size_t)row * a.vocab + c0;
-      float* y = a.out ? a.out + (size_t)row * a.vocab + c0 : nullptr;
-      Best bst;
-      // 16-byte groups start where the row's address allows them
-      const int lead = min(n, (int)((4 - (((size_t)row * a.vocab + c0) & 3)) & 3));
-      const int body = (n - lead) / 4;
-      auto one = [&](int t) {
-        float v = apply(x[t], counting ? cnt[t] : 0, a.bias_tok ? bia[t] : 0, r);
-        const int tok = c0 + t;
-        if (r.mask && !(r.mask[tok >> 5] >> (tok & 31) & 1))
-          v = -INFINITY;
+  Group grp[U];
+  {
+    const int row = row0 + r0, sh = shift_of(row);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      load_group(grp[u], a.logits + (size_t)row * a.vocab, mask_of(row), c0 - sh + 4 * (tid + u * kPickThreads), a.vocab);
+  }
+
+  const bool counting = a.penalties != nullptr, biasing = a.bias_tok != nullptr;
+  uint32_t* cnt = dyn;
+  uint32_t* bia = counting ? dyn + kWords : dyn;
+  RowRules r{1.f, 1.f, 1.f, nullptr};
+  if (counting || biasing) {
+    for (int i = tid; i < (counting + biasing) * kWords / 4; i += kPickThreads)
+      reinterpret_cast<uint4*>(dyn)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+  }
+  if (counting) {
+    r.rep = a.penalties[3 * s], r.freq = a.penalties[3 * s + 1], r.pres = a.penalties[3 * s + 2];
+    if (a.hist) {
+      const int h0 = clampi(a.hist_off[s], 0, a.hist_total), h1 = clampi(a.hist_off[s + 1], h0, a.hist_total);
+      const int given = h0 + (a.prompt ? clampi(a.prompt[s], 0, h1 - h0) : 0);
+      auto see = [&](int i, int tok) {  // ids outside the vocabulary fall outside every slice's rows
+        const unsigned w = (unsigned)(tok - c0 + 4);
+        if (w >= (unsigned)kWords) return;
+        if (i < given)
+          atomicOr(cnt + w, kGiven);
         else
-          bst.see(v, tok);
-        if (y) y[t] = v;
+          atomicAdd(cnt + w, 1u);
       };
-      if (threadIdx.x < lead) one(threadIdx.x);
-      for (int i = threadIdx.x; i < body; i += kPickThreads) {
-        const int t = lead + 4 * i, tok = c0 + t;
-        float4 f = __ldcs(reinterpret_cast<const float4*>(x + t));
-        uint32_t k4[4] = {0, 0, 0, 0}, b4[4] = {0, 0, 0, 0};
-        if (counting) {
-          if (lead == 0) {
-            const uint4 u = *reinterpret_cast<const uint4*>(cnt + t);
-            k4[0] = u.x, k4[1] = u.y, k4[2] = u.z, k4[3] = u.w;
-          } else {
-            for (int e = 0; e < 4; ++e) k4[e] = cnt[t + e];
-          }
-        }
-        if (a.bias_tok) {
-          if (lead == 0) {
-            const uint4 u = *reinterpret_cast<const uint4*>(bia + t);
-            b4[0] = u.x, b4[1] = u.y, b4[2] = u.z, b4[3] = u.w;
-          } else {
-            for (int e = 0; e < 4; ++e) b4[e] = bia[t + e];
-          }
-        }
-        uint32_t bits = 0xfu;
-        if (r.mask) {
-          const int w = tok >> 5, sh = tok & 31;
-          bits = r.mask[w] >> sh;
-          if (sh > 28) bits |= r.mask[w + 1] << (32 - sh);  // the group's last token lies in the next word
-        }
-        float v[4] = {f.x, f.y, f.z, f.w};
+      constexpr int B = 8;  // loads in flight
+      for (int i = h0 + tid; i < h1; i += B * kPickThreads) {
+        int tok[B];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (k4[e] | b4[e]) v[e] = apply(v[e], k4[e], b4[e], r);
-          if (bits >> e & 1)
-            bst.see(v[e], tok + e);
-          else
-            v[e] = -INFINITY;
-        }
-        if (y) __stcs(reinterpret_cast<float4*>(y + t), make_float4(v[0], v[1], v[2], v[3]));
-      }
-      const int tail = lead + 4 * body;
-      if (threadIdx.x < n - tail) one(tail + threadIdx.x);
-      unsigned long long k = bst.t < 0 ? 0ull : argmax_key(bst.v, bst.t);
+        for (int e = 0; e < B; ++e) tok[e] = i + e * kPickThreads < h1 ? __ldg(a.hist + i + e * kPickThreads) : INT_MIN;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const unsigned long long other = __shfl_xor_sync(0xffffffffu, k, o);
-        if (other > k) k = other;
-      }
-      if ((threadIdx.x & 31) == 0 && k > sm.warp_key[q - r0][threadIdx.x >> 5]) sm.warp_key[q - r0][threadIdx.x >> 5] = k;
-      if (counting && a.seqs) {
-        __syncthreads();
-        const unsigned long long anc = a.anc[row];
-        if (threadIdx.x < m && (anc >> threadIdx.x & 1)) {
-          const unsigned t = (unsigned)(a.draft[row0 + threadIdx.x] - c0);
-          if (t < (unsigned)n) atomicSub(cnt + t, 1u);
-        }
-        __syncthreads();
+        for (int e = 0; e < B; ++e)
+          if (tok[e] >= 0) see(i + e * kPickThreads, tok[e]);
       }
     }
+  }
+  if (biasing) {
+    const int b0 = clampi(a.bias_off[s], 0, a.bias_total), b1 = clampi(a.bias_off[s + 1], b0, a.bias_total);
+    r.bias_val = a.bias_val + b0;
+    for (int i = b0 + tid; i < b1; i += kPickThreads) {
+      const int tok = a.bias_tok[i];
+      const unsigned w = (unsigned)(tok - c0 + 4);
+      if (tok >= 0 && w < (unsigned)kWords) atomicMax(bia + w, (uint32_t)(i - b0 + 1));  // a token's last entry counts
+    }
+  }
+
+  unsigned long long path = 0;  // nodes whose drafted tokens the counts hold
+#pragma unroll 1
+  for (int q = r0; q < r1; ++q) {
+    const int row = row0 + q;
+    if (counting && a.seqs) {
+      const unsigned long long anc = a.anc[row];
+      __syncthreads();  // the row before has been counted out
+      if (tid < m && ((anc ^ path) >> tid & 1)) {
+        const int tok = a.draft[row0 + tid];
+        const unsigned w = (unsigned)(tok - c0 + 4);
+        if (tok >= 0 && w < (unsigned)kWords) atomicAdd(cnt + w, (anc >> tid & 1) ? 1u : 0xffffffffu);
+      }
+      path = anc;
+    }
+    if (counting || biasing) __syncthreads();
+    const int sh = shift_of(row), next = row + 1, nsh = shift_of(next);
+    float* y = a.out ? a.out + (size_t)row * a.vocab : nullptr;
+    Best best;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = tid + u * kPickThreads, t = c0 - sh + 4 * i;
+      Group& g = grp[u];
+      if (counting || biasing) {
+        uint32_t k[4] = {0, 0, 0, 0}, b[4] = {0, 0, 0, 0};
+        if (counting) four_words(k, cnt, i, sh);
+        if (biasing) four_words(b, bia, i, sh);
+        if (k[0] | k[1] | k[2] | k[3] | b[0] | b[1] | b[2] | b[3]) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) g.v[e] = apply(g.v[e], k[e], b[e], r);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (g.bits >> e & 1)
+          best.see(g.v[e], t + e);
+        else
+          g.v[e] = -INFINITY;
+      }
+      if (y) {
+        if (t >= 0 && t + 3 < a.vocab) {
+          __stcs(reinterpret_cast<float4*>(y + t), make_float4(g.v[0], g.v[1], g.v[2], g.v[3]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (t + e >= 0 && t + e < a.vocab) y[t + e] = g.v[e];
+        }
+      }
+      if (q + 1 < r1)
+        load_group(g, a.logits + (size_t)next * a.vocab, mask_of(next), c0 - nsh + 4 * i, a.vocab);
+    }
+    unsigned long long key = best.t < 0 ? 0ull : argmax_key(best.v, best.t);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
+      if (other > key) key = other;
+    }
+    if ((tid & 31) == 0) warp_key[q - r0][tid >> 5] = key;
   }
   __syncthreads();
-  cluster.barrier_wait();  // every CTA of the cluster runs: its shared memory may be written
-  if (threadIdx.x < r1 - r0) {
-    unsigned long long k = 0;
-    for (int w = 0; w < kPickWarps; ++w) k = sm.warp_key[threadIdx.x][w] > k ? sm.warp_key[threadIdx.x][w] : k;
-    PickSmem* first = cluster.map_shared_rank(&sm, 0);
-    first->key[threadIdx.x][rank] = k;
+  if (tid < r1 - r0) {
+    unsigned long long key = 0;
+    for (int w = 0; w < kPickWarps; ++w) key = warp_key[tid][w] > key ? warp_key[tid][w] : key;
+    const int row = row0 + r0 + tid;
+    if (gridDim.x > 1) {
+      if (key) atomicMax(a.best + row, key);
+      __threadfence();
+      if (atomicInc(a.arrived + row, gridDim.x - 1) != gridDim.x - 1) return;  // wraps to 0 with the last arrival
+      __threadfence();
+      key = atomicExch(a.best + row, 0ull);
+    }
+    a.tokens[row] = key ? argmax_key_index(key) : -1;
   }
-  cluster.sync();
-  if (rank == 0 && threadIdx.x < r1 - r0) {
-    unsigned long long k = 0;
-    for (int w = 0; w < csize; ++w) k = sm.key[threadIdx.x][w] > k ? sm.key[threadIdx.x][w] : k;
-    a.tokens[row0 + r0 + threadIdx.x] = k ? argmax_key_index(k) : -1;
-  }
+}
+
+// Processes rows [0, n) of `a` in one launch (n <= kPickMaxRows).
+template <int U>
+cudaError_t launch_pick(const PickArgs& a, int rows, int groups, int slices, cudaStream_t st) {
+  const size_t smem = (size_t)(kPickThreads * 4 * U + 4) * 4 * ((a.penalties ? 1 : 0) + (a.bias_tok ? 1 : 0));
+  pick_kernel<U><<<dim3(slices, groups, a.n_seqs), kPickThreads, smem, st>>>(a, rows);
+  return cudaGetLastError();
 }
 
 }  // namespace
 
 cudaError_t configure_pick_kernels() {
-  cudaError_t e = cudaFuncSetAttribute(pick_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kMaxChunk * 4);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(pick_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  return e;
+  return cudaFuncSetAttribute(pick_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              2 * (kPickThreads * 16 + 4) * 4);
 }
 
 cudaError_t op_pick(const PickArgs& a, int sms, cudaStream_t st) {
-  const int csize = kMaxCluster;
-  // rows per CTA: sequences with many rows share the counting of their history
-  int rows = 1;
-  while (rows < kMaxRowsPerCta && rows < a.max_m && (long long)a.n * csize / rows > 2ll * sms) rows *= 2;
+  // Slices of 8192 tokens while they fill the SMs, else of 2048 (a single row over 75
+  // CTAs instead of 19). A slice is reached by rows that start up to 3 tokens early,
+  // hence vocab + 3. The nodes of a tree share a CTA as far as two CTAs per SM remain.
+  const int wide = (a.vocab + 3 + 8191) / 8192, narrow = (a.vocab + 3 + 2047) / 2048;
+  const long long ctas = (long long)a.n_seqs * a.max_m * wide;
+  const int rows = (int)std::min<long long>(std::min(a.max_m, kMaxRowsPerCta), std::max<long long>(1, (ctas + 2 * sms - 1) / (2 * sms)));
   const int groups = (a.max_m + rows - 1) / rows;
-  int slice = (a.vocab + csize - 1) / csize;
-  slice = (slice + 127) / 128 * 128;
-  const int chunk = slice < kMaxChunk ? slice : kMaxChunk;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)a.n_seqs * groups * csize);
-  cfg.blockDim = dim3(kPickThreads);
-  cfg.dynamicSmemBytes = (size_t)chunk * 4 * ((a.penalties ? 1 : 0) + (a.bias_tok ? 1 : 0));
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = csize;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, pick_kernel, a, rows, groups, slice, chunk);
+  if (ctas >= sms) return launch_pick<4>(a, rows, groups, wide, st);
+  return launch_pick<1>(a, rows, groups, narrow, st);
 }
 
 }  // namespace dllm

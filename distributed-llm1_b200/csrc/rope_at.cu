@@ -59,6 +59,21 @@ __global__ void __launch_bounds__(kRopeThreads) rope_at_kernel(const RopeAtArgs 
   // float offsets of the unit's two packs within a head
   const int o1 = turns ? (INTER ? unit * 2 * VEC : unit * VEC) : a.rotary + (unit - turning) * 2 * VEC;
   const int o2 = turns ? (INTER ? o1 + VEC : o1 + a.rotary / 2) : o1 + VEC;
+  // the first head's elements are on their way while the angles are computed
+  auto head_at = [&](int h, const float*& src, float*& dst) {
+    const bool is_q = h < a.q_heads;
+    const size_t at = is_q ? ((size_t)row * a.q_heads + h) * a.hd : ((size_t)row * a.k_heads + (h - a.q_heads)) * a.hd;
+    src = (is_q ? a.q : a.k) + at;
+    dst = (is_q ? a.q_out : a.k_out) + at;
+  };
+  const float* src;
+  float* dst;
+  int h = blockIdx.y * per + threadIdx.x / units;
+  Pack<VEC> x, y;
+  if (h < heads) {
+    head_at(h, src, dst);
+    x = ld_pack<VEC>(src + o1), y = ld_pack<VEC>(src + o2);
+  }
   float c[VEC], s[VEC];
   if (turns) {
     const double pos = (double)a.pos[row];
@@ -70,13 +85,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_at_kernel(const RopeAtArgs 
       c[i] *= a.factor;
     }
   }
-  for (int h = blockIdx.y * per + threadIdx.x / units; h < heads; h += per * gridDim.y) {
-    const bool is_q = h < a.q_heads;
-    const size_t at = is_q ? ((size_t)row * a.q_heads + h) * a.hd : ((size_t)row * a.k_heads + (h - a.q_heads)) * a.hd;
-    const float* src = (is_q ? a.q : a.k) + at;
-    float* dst = (is_q ? a.q_out : a.k_out) + at;
-    if (!turns && src == dst) continue;
-    Pack<VEC> x = ld_pack<VEC>(src + o1), y = ld_pack<VEC>(src + o2);
+  while (h < heads) {
     if (turns) {
       if constexpr (INTER && VEC == 4) {  // (x0 x1)(x2 x3) | (y0 y1)(y2 y3)
 #pragma unroll
@@ -96,16 +105,28 @@ __global__ void __launch_bounds__(kRopeThreads) rope_at_kernel(const RopeAtArgs 
         }
       }
     }
-    st_pack<VEC>(dst + o1, x);
-    st_pack<VEC>(dst + o2, y);
+    if (turns || src != dst) {
+      st_pack<VEC>(dst + o1, x);
+      st_pack<VEC>(dst + o2, y);
+    }
+    h += per * gridDim.y;
+    if (h < heads) {
+      head_at(h, src, dst);
+      x = ld_pack<VEC>(src + o1), y = ld_pack<VEC>(src + o2);
+    }
   }
 }
 
 }  // namespace
 
-cudaError_t op_rope_at(const RopeAtArgs& a, cudaStream_t st) {
+cudaError_t op_rope_at(const RopeAtArgs& a, int sms, cudaStream_t st) {
   const bool vec = a.rotary % 8 == 0;
-  const dim3 grid(a.n, 1);
+  // few rows: the heads of a row are spread over CTAs as well, which repeats the
+  // angles but leaves one load and store per thread (64 rows of 32 heads: 4.5 us in
+  // one CTA per row)
+  const int per = kRopeThreads / (a.hd / (vec ? 8 : 2));
+  const int chunks = (a.q_heads + a.k_heads + per - 1) / per;
+  const dim3 grid(a.n, (long long)a.n * chunks <= 8ll * sms ? chunks : 1);
   if (vec && a.interleaved)
     rope_at_kernel<4, true><<<grid, kRopeThreads, 0, st>>>(a);
   else if (vec)

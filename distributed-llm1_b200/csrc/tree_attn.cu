@@ -517,33 +517,85 @@ __global__ void __launch_bounds__(kTAThreads, 1) tree_attn_kernel(const __grid_c
   }
 }
 
-// Joins the splits of a sequence: one warp per (row, query head), splits in order.
-template <int HD>
+// Joins the splits of a sequence. W warps share one (row, query head): warp w folds the
+// splits w, w + W, ... in order, then the warps' results are folded in order, so the
+// sum does not depend on timing. Every split's maximum, sum and output are loaded
+// together: the chain is one load per kBatch splits.
+template <int HD, int W>
 __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ TAKernelArgs P, int bn) {
+  constexpr int V = HD / 32, kBatch = 4;
+  __shared__ float so[8][HD], sml[8][2];
   const TreeAttnArgs& a = P.a;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the splits' grid has ended and its stores are visible
   const TreeSeq sq = a.seqs[blockIdx.y];
   const int nsplit = ta_splits(P.t0[blockIdx.y] + sq.m, bn, P.bps);
-  const int item = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (nsplit <= 1 || item >= sq.m * a.nq) return;
-  constexpr int V = HD / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int item = blockIdx.x * (8 / W) + warp / W, w = warp % W;
+  const bool live = nsplit > 1 && item < sq.m * a.nq;
   const size_t step = (size_t)sq.m * a.nq, base = (size_t)P.part0[blockIdx.y] + item;
-  float m = kNegInf;
-  for (int s = lane; s < nsplit; s += 32) m = fmaxf(m, a.part_ml[(base + s * step) * 2]);
-  m = warp_max(m);
-  const float b = m == kNegInf ? 0.f : m;
-  float acc[V], l = 0.f;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the splits' grid has ended and its stores are visible
+  float m = kNegInf, l = 0.f, acc[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) acc[e] = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < nsplit; ++s) {
-    const size_t at = base + s * step;
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
-    const float w = ex2(ml.x - b);
-    l = fmaf(ml.y, w, l);
+  if (live) {
+    for (int s0 = w; s0 < nsplit; s0 += kBatch * W) {
+      float2 ml[kBatch];
+      float o[kBatch][V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] = fmaf(a.part_o[at * HD + lane * V + e], w, acc[e]);
+      for (int u = 0; u < kBatch; ++u) {
+        const int s = s0 + u * W;
+        ml[u] = make_float2(kNegInf, 0.f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[u][e] = 0.f;
+        if (s < nsplit) {
+          const size_t at = base + s * step;
+          ml[u] = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
+          if constexpr (V == 4) {
+            const float4 f = *reinterpret_cast<const float4*>(a.part_o + at * HD + lane * 4);
+            o[u][0] = f.x, o[u][1] = f.y, o[u][2] = f.z, o[u][3] = f.w;
+          } else {
+            const float2 f = *reinterpret_cast<const float2*>(a.part_o + at * HD + lane * 2);
+            o[u][0] = f.x, o[u][1] = f.y;
+          }
+        }
+      }
+      float x = m;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) x = fmaxf(x, ml[u].x);
+      const float b = x == kNegInf ? 0.f : x, f = ex2(m - b);
+      m = x, l *= f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] *= f;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const float wt = ex2(ml[u].x - b);
+        l = fmaf(ml[u].y, wt, l);
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] = fmaf(o[u][e], wt, acc[e]);
+      }
+    }
   }
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) so[warp][lane * V + e] = acc[e];
+    if (lane == 0) sml[warp][0] = m, sml[warp][1] = l;
+    __syncthreads();
+    if (w != 0) return;
+    float x = kNegInf;
+#pragma unroll
+    for (int u = 0; u < W; ++u) x = fmaxf(x, sml[warp + u][0]);
+    const float b = x == kNegInf ? 0.f : x;
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0.f;
+#pragma unroll
+    for (int u = 0; u < W; ++u) {
+      const float wt = ex2(sml[warp + u][0] - b);
+      l = fmaf(sml[warp + u][1], wt, l);
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] = fmaf(so[warp + u][lane * V + e], wt, acc[e]);
+    }
+  }
+  if (!live) return;
   const float inv = 1.0f / l;
   float* dst = a.out + ((size_t)sq.row0 * a.nq + item) * HD + lane * V;
 #pragma unroll
@@ -591,7 +643,9 @@ cudaError_t launch(const TreeAttnArgs& a, const TreeAttnShape& s, int sms, int* 
   *launches += 1;
   if (e != cudaSuccess || splits == 1) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((s.max_m * a.nq + 7) / 8, a.n_seqs);
+  const int items = s.max_m * a.nq;  // rows and query heads of a sequence
+  const bool many = splits > 8;
+  cfg.gridDim = dim3(many ? items : (items + 7) / 8, a.n_seqs);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -600,7 +654,7 @@ cudaError_t launch(const TreeAttnArgs& a, const TreeAttnShape& s, int sms, int* 
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   *launches += 1;
-  return cudaLaunchKernelEx(&cfg, tree_join_kernel<HD>, P, T::BN);
+  return cudaLaunchKernelEx(&cfg, many ? tree_join_kernel<HD, 8> : tree_join_kernel<HD, 1>, P, (int)T::BN);
 }
 
 template <typename KT, int HD>

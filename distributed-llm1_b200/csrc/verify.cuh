@@ -34,7 +34,7 @@ struct RopeAtArgs {
   int n, q_heads, k_heads, hd, rotary, interleaved;
   float factor;
 };
-cudaError_t op_rope_at(const RopeAtArgs& a, cudaStream_t st);
+cudaError_t op_rope_at(const RopeAtArgs& a, int sms, cudaStream_t st);
 
 // ---- pick.cu ----------------------------------------------------------------------
 struct PickArgs {
@@ -59,7 +59,11 @@ struct PickArgs {
   const unsigned long long* anc;  // [n] ancestors (self included) within the sequence
   const int32_t* draft;           // [n] drafted tokens
   int n_seqs, max_m;
+  // per row, zero before and after every call: the best key and the slices that have arrived
+  unsigned long long* best;
+  unsigned int* arrived;
 };
+constexpr int kPickMaxRows = kTreeMaxNodes * kTreeMaxSeqs;  // rows of one call (the capacity of best / arrived)
 cudaError_t configure_pick_kernels();
 cudaError_t op_pick(const PickArgs& a, int sms, cudaStream_t st);
 

@@ -158,7 +158,8 @@ class KernelContext:
 
     # ---- plumbing
     def _check(self, st: int, what: str = ""):
-        _lib.check(st, self.handle, what)
+        if st:
+            _lib.check(st, self.handle, what)
 
     def _out(self, fn, *args, n: int, label: str) -> GpuBuffer:
         out = C.c_void_p()

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from array import array
 
 import numpy as np
 
@@ -171,7 +172,7 @@ class Stage:
         self.k._check(self.lib.dllm_stage_set_t0(self.handle, 0, int(v)), "T0")
 
     def t0_of(self, seq: int) -> int:
-        return int(self.lib.dllm_stage_get_t0(self.handle, seq))
+        return self.lib.dllm_stage_get_t0(self.handle, seq)
 
     def set_t0(self, seq: int, v: int):
         self.k._check(self.lib.dllm_stage_set_t0(self.handle, seq, int(v)), "set_t0")
@@ -251,12 +252,12 @@ class Stage:
     def commit_tree(self, tree: DraftTree, paths):
         """Keep one path of nodes per sequence (root first): its K/V rows move to slots
         T0.. of every layer and T0 advances by its length."""
-        lens = np.array([len(p) for p in paths], dtype=np.int32)
-        if lens.size != tree.counts.size:
-            raise _lib.DllmError(_lib.DLLM_EINVAL, f"commit_tree: {lens.size} paths for {tree.counts.size} sequences")
-        flat = np.array([j for p in paths for j in p] or [0], dtype=np.int32)
-        self.k._check(self.lib.dllm_stage_commit_tree(self.handle, self.k._h(tree), _lib.ptr(flat, C.c_int32),
-                                                      _lib.ptr(lens, C.c_int32)), "commit_tree")
+        lens = array("i", map(len, paths))
+        if len(lens) != tree.counts.size:
+            raise _lib.DllmError(_lib.DLLM_EINVAL, f"commit_tree: {len(lens)} paths for {tree.counts.size} sequences")
+        flat = array("i", [j for p in paths for j in p] or [0])
+        self.k._check(self.lib.dllm_stage_commit_tree(self.handle, self.k._h(tree), flat.buffer_info()[0],
+                                                      lens.buffer_info()[0]), "commit_tree")
 
     def forward_tree(self, tree: DraftTree, hBuf: GpuBuffer, tokens: GpuBuffer | None = None,
                      logits: GpuBuffer | None = None) -> GpuBuffer:

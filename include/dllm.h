@@ -365,7 +365,7 @@ void dllm_tree_destroy(dllm_tree* tree);
 /* Arguments of dllm_pick_tokens; optional buffers may be NULL. V = vocab_size; the
  * sequences are the tree's, or without a tree the n rows themselves. */
 typedef struct dllm_pick {
-  int32_t n;
+  int32_t n;                       /* 1..8192 */
   const dllm_buf* logits;          /* f32 [n, V] */
   const dllm_buf* history;         /* i32: tokens of all sequences; ids outside [0, V) are ignored */
   const dllm_buf* history_offsets; /* i32 [seqs + 1]: sequence s has [offsets[s], offsets[s + 1]) */
