@@ -2410,6 +2410,7 @@ int dllm_pick_tokens(dllm_ctx* c, const dllm_pick* p) {
   if (!c) return DLLM_EINVAL;
   if (!p) return set_err(c, DLLM_EINVAL, "pickTokens: null arguments");
   const int n = p->n, V = c->cfg.vocab_size;
+  if (V > 1 << 30) return set_err(c, DLLM_EINVAL, "pickTokens: a vocabulary of %d", V);
   if (n <= 0 || n > dllm::kPickMaxRows)
     return set_err(c, DLLM_EINVAL, "pickTokens: n=%d outside 1..%d", n, dllm::kPickMaxRows);
   if ((p->tree != nullptr) != (p->draft != nullptr))

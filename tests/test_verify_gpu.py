@@ -540,19 +540,21 @@ def test_pick_rows(dllm, v, use):
 def test_pick_ties_nan_and_infinities(dllm):
     v = 1003
     ctx = make_ctx(dllm, vocab_size=v)
-    x = np.full((6, v), 1.0, np.float32)
+    x = np.full((8, v), 1.0, np.float32)
     x[1] = np.nan
     x[2] = -np.inf
     x[3, ::7], x[3, 500], x[3, 900] = np.nan, np.inf, np.inf
     x[4] = np.finfo(np.float32).min
     x[5, 11], x[5, 1002] = 2.0, 2.0
-    run_pick(ctx, x, range(6))
-    allowed = np.ones((6, v), bool)
+    x[6, :200], x[6, 200:] = np.nan, -7.0
+    x[7, :-1] = np.nan
+    run_pick(ctx, x, range(8))
+    allowed = np.ones((8, v), bool)
     allowed[:, :13] = False
-    run_pick(ctx, x, range(6), allowed=allowed)
-    hist = [[500, 3, 900, 900]] * 6
-    run_pick(ctx, x, range(6), hist=hist, prompt=[1] * 6, pen=[[2.0, 0.5, 0.25]] * 6, allowed=allowed,
-             bias=[[(900, float("-inf")), (20, float("nan"))]] * 6)
+    run_pick(ctx, x, range(8), allowed=allowed)
+    hist = [[500, 3, 900, 900, 2 ** 31 - 1, -2 ** 31]] * 8
+    run_pick(ctx, x, range(8), hist=hist, prompt=[1] * 8, pen=[[2.0, 0.5, 0.25]] * 8, allowed=allowed,
+             bias=[[(900, float("-inf")), (20, float("nan"))]] * 8)
     ctx.close()
 
 
