@@ -23,6 +23,7 @@
 #include "kernels.cuh"
 #include "ops.cuh"
 #include "stage.cuh"
+#include "tc.cuh"
 #include "verify.cuh"
 
 using dllm::KvLayout;
@@ -128,6 +129,9 @@ struct dllm_stage {
   // tracing: %globaltimer at kernel start and after every grid barrier (last launch)
   unsigned long long* trace = nullptr;
   int trace_cap = 0;
+  // tensor maps of the K and V pools as rows (layer, page, head, slot) of HD (bf16 caches)
+  CUtensorMap kv_map[2];
+  bool kv_mapped = false;
   int version = 0;  // bumped when weights or tracing change (captured graphs rebuild)
 };
 
@@ -701,6 +705,11 @@ int tree_attention(dllm_stage* s, int layer, const dllm_tree* tree, const dllm::
   a.nq = f.num_q_heads;
   a.kvh = f.num_kv_heads;
   a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)f.head_dim));
+  if (s->kv_mapped) {
+    a.tc_k = &s->kv_map[0];
+    a.tc_v = &s->kv_map[1];
+    a.tc_row0 = (int)((size_t)(layer - s->start) * s->layer_elems / f.head_dim);
+  }
   a.part_o = c->tree_part;
   a.part_ml = c->tree_part + dllm::tree_attn_part_rows(c->sms) * f.head_dim;
   const dllm::TreeAttnShape shape{tree->seqs.data(), t0.t0, tree->n, tree->max_m};
@@ -1351,6 +1360,12 @@ int dllm_stage_create(dllm_ctx* c, int start, int end, dllm_stage** out) {
   };
   if (!rc) rc = alloc_pool(&s->kpool);
   if (!rc) rc = alloc_pool(&s->vpool);
+  const size_t kv_rows = s->layer_elems * s->nl / f.head_dim;
+  if (!rc && f.kv_dtype == DLLM_KV_BF16 && kv_rows > 0 && kv_rows <= 0x7fffffff) {
+    const int box = std::min(s->page, 64);
+    s->kv_mapped = dllm::tc_encode_rows(&s->kv_map[0], s->kpool, f.head_dim, (int)kv_rows, box) &&
+                   dllm::tc_encode_rows(&s->kv_map[1], s->vpool, f.head_dim, (int)kv_rows, box);
+  }
   if (!rc) rc = dev_alloc(c, &s->page_table, (size_t)s->max_seqs * s->pages_per_seq, "page table");
   if (!rc) {
     std::vector<int> pt((size_t)s->max_seqs * s->pages_per_seq);

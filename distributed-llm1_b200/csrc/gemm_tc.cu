@@ -20,6 +20,7 @@
 
 #include "common.cuh"
 #include "gemm_tc.cuh"
+#include "tc.cuh"
 
 namespace dllm {
 namespace {
@@ -33,76 +34,6 @@ constexpr int kTcMaxTargets = 3;
 constexpr int kTcThreads = 128;
 constexpr int kABoxBytes = kBM * kBK * 2;              // 16 KB: one 128-row box
 constexpr int kATileBytes = kABoxBytes * kBoxes;        // 32 KB per stage
-constexpr long long kTcWaitCycles = 1ll << 32;        // ~2 s of SM cycles
-
-DLLM_DEV uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-DLLM_DEV void mbar_init(uint64_t* bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
-}
-DLLM_DEV void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-}
-// Bounded wait for completion of the phase with parity `parity`.
-DLLM_DEV bool mbar_wait(uint64_t* bar, uint32_t parity) {
-  const uint32_t a = smem_u32(bar);
-  const long long t0 = clock64();
-  for (;;) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(a), "r"(parity)
-        : "memory");
-    if (done) return true;
-    if (clock64() - t0 > kTcWaitCycles) return false;
-  }
-}
-
-// 2-D tiled TMA load of box (x = K offset, y = row offset) into shared memory,
-// completing on `bar` (no multicast: the tensor always lies in this GPU's memory).
-DLLM_DEV void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-          smem_u32(dst)),
-      "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
-      : "memory");
-}
-
-// Shared-memory matrix descriptor of a K-major tile written by TMA with the
-// 128-byte swizzle: rows of 128 bytes, 8-row groups 1024 bytes apart (stride
-// byte offset 1024 >> 4), leading byte offset unused (1), descriptor version 1,
-// layout type 2 (SWIZZLE_128B). The tile base must be 1024-byte aligned.
-DLLM_DEV uint64_t umma_desc_sw128(const void* tile) {
-  const uint64_t a = smem_u32(tile);
-  return ((a & 0x3FFFFull) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
-
-// D[tmem] (+)= A[128 x 16] * B[N x 16]^T, bf16 inputs, fp32 accumulate.
-DLLM_DEV void umma_bf16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
-}
-// Arrive on `bar` once every tcgen05.mma this thread issued so far has completed.
-DLLM_DEV void umma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
-}
-DLLM_DEV void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-DLLM_DEV void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// 8 consecutive fp32 accumulator columns of this thread's TMEM lane.
-DLLM_DEV void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(taddr));
-}
-DLLM_DEV void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // One output matrix of a launch: weight tiles [tile_begin, tile_begin + tiles) of
 // the grid belong to it. Several targets that share the activations (q|k|v,
@@ -361,19 +292,23 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
+}  // namespace
+
 // Row-major bf16 [outer][inner] as a 2-D tensor map with a (64 x box_rows) box and
 // the 128-byte swizzle; out-of-range boxes read zeros.
-bool encode_rows(CUtensorMap* m, const void* base, int inner, int outer, int box_rows) {
+bool tc_encode_rows(CUtensorMap* m, const void* base, int inner, int outer, int box_rows) {
   auto fn = encode_fn();
   if (!fn) return false;
   const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
   const cuuint64_t strides[1] = {(cuuint64_t)inner * 2};
-  const cuuint32_t box[2] = {(cuuint32_t)kBK, (cuuint32_t)box_rows};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
   const cuuint32_t es[2] = {1, 1};
   return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, es,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+
+namespace {
 
 int padded_rows(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
@@ -477,7 +412,7 @@ cudaError_t tc_matmul_multi(const float* x, int rows, int K, const TcTarget* t, 
   int tile = 0;
   size_t part_off = 0;
   for (int i = 0; i < n; ++i) {
-    if (!encode_rows(&tw[i], t[i].w, K, t[i].N, kBM)) return cudaErrorInvalidValue;
+    if (!tc_encode_rows(&tw[i], t[i].w, K, t[i].N, kBM)) return cudaErrorInvalidValue;
     a.t[i].N = t[i].N;
     a.t[i].tile_begin = tile;
     tile += (t[i].N + kBM - 1) / kBM;
@@ -493,7 +428,7 @@ cudaError_t tc_matmul_multi(const float* x, int rows, int K, const TcTarget* t, 
     }
   }
   for (int i = n; i < kTcMaxTargets; ++i) tw[i] = tw[0];  // unused parameters
-  if (!encode_rows(&tx, xb, K, 2 * p.rp, 2 * p.rp)) return cudaErrorInvalidValue;
+  if (!tc_encode_rows(&tx, xb, K, 2 * p.rp, 2 * p.rp)) return cudaErrorInvalidValue;
   const dim3 grid(p.n_tiles, p.splits);
   switch (p.rp) {
     case 16: e = launch_rp<16>(tw, tx, a, grid, p.smem, st); break;

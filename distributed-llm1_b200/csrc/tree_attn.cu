@@ -22,8 +22,7 @@
 // behind the sequence's last one are zero-filled, never read.
 #include <algorithm>
 
-#include "kernels.cuh"
-#include "verify.cuh"
+#include "tree_attn.cuh"
 
 namespace dllm {
 namespace {
@@ -62,35 +61,16 @@ DLLM_DEV void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint3
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-DLLM_DEV float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-DLLM_DEV uint32_t pack_bf16(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-// (x, y) -> three packed bf16 pairs whose sums are x and y to 2^-25 of them.
-DLLM_DEV void split3(float x, float y, uint32_t& h, uint32_t& m, uint32_t& l) {
-  h = pack_bf16(x, y);
-  x -= bf16_lo(h), y -= bf16_hi(h);
-  m = pack_bf16(x, y);
-  x -= bf16_lo(m), y -= bf16_hi(m);
-  l = pack_bf16(x, y);
-}
 // x = hi + lo, hi with 11 bits; lo is rounded to 11 bits by the conversion.
 DLLM_DEV void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
   hi = __float_as_uint(x) & 0xffffe000u;
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
 }
-DLLM_DEV bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
 
 // Tile shapes. SN: slots of a block that one warp takes; BN: slots of a block.
 // The ring depth is what fits beside the q tile in 227 KB.
 template <typename KT, int HD, int WR>
-struct TATile {
+struct MmaTile {
   static constexpr bool kF32 = sizeof(KT) == 4;
   static constexpr int WS = 8 / WR;                 // warps side by side in slots
   static constexpr int SN = kF32 ? 8 * WR : (WR == 1 ? 16 : WR == 2 ? 32 : WR == 4 ? 32 : 64);
@@ -109,22 +89,9 @@ struct TATile {
   static constexpr int kSmem = kQBytes + kStages * 2 * kTileBytes;
 };
 
-struct TAKernelArgs {
-  TreeAttnArgs a;
-  int bps;                       // blocks per split
-  int t0[kTreeMaxSeqs];
-  int part0[kTreeMaxSeqs];       // first partial row of a split sequence
-};
-
-// The number of splits of a sequence with `slots` slots; the same on host and device.
-__host__ __device__ inline int ta_splits(int slots, int bn, int bps) {
-  const int blocks = (slots + bn - 1) / bn;
-  return (blocks + bps - 1) / bps;
-}
-
 template <typename KT, int HD, int WR>
 __global__ void __launch_bounds__(kTAThreads, 1) tree_attn_kernel(const __grid_constant__ TAKernelArgs P) {
-  using T = TATile<KT, HD, WR>;
+  using T = MmaTile<KT, HD, WR>;
   constexpr int SN = T::SN, BN = T::BN, WS = T::WS, RT = T::RT, NT = SN / 8, CH = T::kChunks, S = T::kStages;
   constexpr bool F32 = T::kF32;
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -349,7 +316,7 @@ __global__ void __launch_bounds__(kTAThreads, 1) tree_attn_kernel(const __grid_c
         float v;
         if constexpr (F32) v = *p;
         else v = bf16_to_f32(*p);
-        bad |= !finite(v);
+        bad |= !is_finite(v);
       }
       if (__syncthreads_or(bad)) {
 #pragma unroll
@@ -365,12 +332,12 @@ __global__ void __launch_bounds__(kTAThreads, 1) tree_attn_kernel(const __grid_c
             if constexpr (F32) v0 = p[0], v1 = p[1];
             else v0 = bf16_to_f32(p[0]), v1 = bf16_to_f32(p[1]);
             if (anc_a >> node & 1) {
-              if (!finite(v0)) o[i][0] += v0;
-              if (!finite(v1)) o[i][1] += v1;
+              if (!is_finite(v0)) o[i][0] += v0;
+              if (!is_finite(v1)) o[i][1] += v1;
             }
             if (anc_b >> node & 1) {
-              if (!finite(v0)) o[i][2] += v0;
-              if (!finite(v1)) o[i][3] += v1;
+              if (!is_finite(v0)) o[i][2] += v0;
+              if (!is_finite(v1)) o[i][3] += v1;
             }
           }
         }
@@ -384,7 +351,7 @@ __global__ void __launch_bounds__(kTAThreads, 1) tree_attn_kernel(const __grid_c
           float v;
           if constexpr (F32) v = *p;
           else v = bf16_to_f32(*p);
-          if (!finite(v)) *p = KT(0.f);
+          if (!is_finite(v)) *p = KT(0.f);
         }
         __syncthreads();
       }
@@ -468,21 +435,7 @@ __global__ void __launch_bounds__(kTAThreads, 1) tree_attn_kernel(const __grid_c
     lb += __shfl_xor_sync(0xffffffffu, lb, w);
   }
 
-  // ---- results: normalised to out, or partials (o, m, l) of this split
-  auto row_out = [&](int row, float4 f, int d, float m, float l) {  // dims d..d+3 of tile row `row`
-    const int r = r0 + row;
-    if (r >= R) return;
-    const int node = r / G;
-    if (nsplit == 1) {
-      const float inv = 1.0f / l;
-      *reinterpret_cast<float4*>(a.out + ((size_t)(sq.row0 + node) * a.nq + head * G + (r - node * G)) * HD + d) =
-          make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
-    } else {
-      const size_t at = (size_t)P.part0[blockIdx.z] + ((size_t)split * sq.m + node) * a.nq + head * G + (r - node * G);
-      *reinterpret_cast<float4*>(a.part_o + at * HD + d) = f;
-      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
-    }
-  };
+  // ---- results
   __syncthreads();  // the ring is free
   // through shared memory: rows padded by 4 floats keep the quads' stores apart
   constexpr int kPad = HD + 4;
@@ -499,22 +452,7 @@ __global__ void __launch_bounds__(kTAThreads, 1) tree_attn_kernel(const __grid_c
     sML[(ws * RT + rb) * 2] = mb, sML[(ws * RT + rb) * 2 + 1] = lb;
   }
   __syncthreads();
-  for (int i = tid; i < RT * HD / 4; i += kTAThreads) {
-    const int row = i / (HD / 4), d = (i % (HD / 4)) * 4;
-    float m = kNegInf, l = 0.f;
-#pragma unroll
-    for (int w = 0; w < WS; ++w) m = fmaxf(m, sML[(w * RT + row) * 2]);
-    const float base = m == kNegInf ? 0.f : m;
-    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < WS; ++w) {
-      const float e = WS == 1 ? 1.f : ex2(sML[(w * RT + row) * 2] - base);
-      const float4 v = *reinterpret_cast<const float4*>(sO + (w * RT + row) * kPad + d);
-      f.x = fmaf(v.x, e, f.x), f.y = fmaf(v.y, e, f.y), f.z = fmaf(v.z, e, f.z), f.w = fmaf(v.w, e, f.w);
-      l = fmaf(sML[(w * RT + row) * 2 + 1], e, l);
-    }
-    row_out(row, f, d, m, l);
-  }
+  ta_finish<HD, WS, RT>(P, TATile{sq, G, head, r0, R, nsplit, split}, sO, sML, tid, kTAThreads);
 }
 
 // Joins the splits of a sequence. W warps share one (row, query head): warp w folds the
@@ -605,7 +543,7 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ 
 template <typename KT, int HD, int WR>
 cudaError_t configure_one() {
   return cudaFuncSetAttribute(tree_attn_kernel<KT, HD, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              TATile<KT, HD, WR>::kSmem);
+                              MmaTile<KT, HD, WR>::kSmem);
 }
 template <typename KT, int HD>
 cudaError_t configure_hd() {
@@ -616,35 +554,34 @@ cudaError_t configure_hd() {
   return e;
 }
 
-template <typename KT, int HD, int WR>
-cudaError_t launch(const TreeAttnArgs& a, const TreeAttnShape& s, int sms, int* launches, cudaStream_t st) {
-  using T = TATile<KT, HD, WR>;
+// Cuts the blocks of bn slots of all (sequence, KV head, tile of rt rows) into as many
+// CTAs as SMs, runs `main` over them, and joins the splits.
+template <int HD, typename Main>
+cudaError_t launch_split(const TreeAttnArgs& a, const TreeAttnShape& s, int rt, int bn, int sms, int* launches,
+                         cudaStream_t st, Main main) {
   TAKernelArgs P;
   P.a = a;
   const int G = a.nq / a.kvh;
-  auto tiles = [&](int m) { return (m * G + T::RT - 1) / T::RT; };
-  // blocks per split: as many CTAs as SMs over all (sequence, KV head, row tile)
+  auto tiles = [&](int m) { return (m * G + rt - 1) / rt; };
   long long total = 0;
   for (int i = 0; i < a.n_seqs; ++i)
-    total += (long long)((s.t0[i] + s.seqs[i].m + T::BN - 1) / T::BN) * a.kvh * tiles(s.seqs[i].m);
+    total += (long long)((s.t0[i] + s.seqs[i].m + bn - 1) / bn) * a.kvh * tiles(s.seqs[i].m);
   P.bps = (int)std::max<long long>(1, (total + sms - 1) / sms);
   int splits = 1;
   size_t part = 0;
   for (int i = 0; i < a.n_seqs; ++i) {
     P.t0[i] = s.t0[i];
-    const int m = s.seqs[i].m, ns = m ? ta_splits(s.t0[i] + m, T::BN, P.bps) : 1;
+    const int m = s.seqs[i].m, ns = m ? ta_splits(s.t0[i] + m, bn, P.bps) : 1;
     P.part0[i] = (int)part;
     if (ns > 1) part += (size_t)ns * m * a.nq;
     splits = std::max(splits, ns);
   }
-  const dim3 grid(splits, a.kvh * tiles(s.max_m), a.n_seqs);
-  tree_attn_kernel<KT, HD, WR><<<grid, kTAThreads, T::kSmem, st>>>(P);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e = main(P, dim3(splits, a.kvh * tiles(s.max_m), a.n_seqs));
   *launches += 1;
   if (e != cudaSuccess || splits == 1) return e;
-  cudaLaunchConfig_t cfg = {};
   const int items = s.max_m * a.nq;  // rows and query heads of a sequence
   const bool many = splits > 8;
+  cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(many ? items : (items + 7) / 8, a.n_seqs);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
@@ -654,13 +591,25 @@ cudaError_t launch(const TreeAttnArgs& a, const TreeAttnShape& s, int sms, int* 
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   *launches += 1;
-  return cudaLaunchKernelEx(&cfg, many ? tree_join_kernel<HD, 8> : tree_join_kernel<HD, 1>, P, (int)T::BN);
+  return cudaLaunchKernelEx(&cfg, many ? tree_join_kernel<HD, 8> : tree_join_kernel<HD, 1>, P, bn);
+}
+
+template <typename KT, int HD, int WR>
+cudaError_t launch(const TreeAttnArgs& a, const TreeAttnShape& s, int sms, int* launches, cudaStream_t st) {
+  using T = MmaTile<KT, HD, WR>;
+  return launch_split<HD>(a, s, T::RT, T::BN, sms, launches, st, [&](const TAKernelArgs& P, dim3 grid) {
+    tree_attn_kernel<KT, HD, WR><<<grid, kTAThreads, T::kSmem, st>>>(P);
+    return cudaGetLastError();
+  });
 }
 
 template <typename KT, int HD>
 cudaError_t launch_hd(const TreeAttnArgs& a, const TreeAttnShape& s, int sms, int* launches, cudaStream_t st) {
   const int rows = s.max_m * (a.nq / a.kvh);  // rows of the largest sequence that share a KV head
   if (rows <= 16) return launch<KT, HD, 1>(a, s, sms, launches, st);
+  if (sizeof(KT) == 2 && a.tc_k)
+    return launch_split<HD>(a, s, kTcRows, kTcBlock, sms, launches, st,
+                            [&](const TAKernelArgs& P, dim3 grid) { return launch_tree_attn_tc(P, HD, grid, st); });
   if (rows <= 32) return launch<KT, HD, 2>(a, s, sms, launches, st);
   if (rows <= 64) return launch<KT, HD, 4>(a, s, sms, launches, st);
   return launch<KT, HD, 8>(a, s, sms, launches, st);
@@ -678,6 +627,7 @@ cudaError_t configure_tree_attn() {
   if (e == cudaSuccess) e = configure_hd<float, 128>();
   if (e == cudaSuccess) e = configure_hd<__nv_bfloat16, 64>();
   if (e == cudaSuccess) e = configure_hd<__nv_bfloat16, 128>();
+  if (e == cudaSuccess) e = configure_tree_attn_tc();
   return e;
 }
 

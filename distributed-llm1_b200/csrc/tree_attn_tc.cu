@@ -1,0 +1,430 @@
+// tree_attn_tc.cu — tree attention over a bf16 cache on the tcgen05 tensor cores, for
+// trees whose rows (nodes x query heads of a KV head) are worth a 128-row tile.
+//
+// The mathematics and the precision are tree_attn.cu's: q and p are cut into three
+// bf16 terms, and each product runs smallest terms first into one fp32 accumulator, so
+// that only the last pass adds at full size (the tensor core truncates each addition);
+// a block's p . V starts from zero and is added to the running output in registers.
+//
+// One CTA, three warpgroups, one 128-row tile over its share of the 64-slot blocks:
+//   producer (1 thread)  TMA: K and V boxes of a block (128-byte swizzle) into rings
+//   MMA (1 thread)       S(n + 1) = q K^T of the next block, then O(n) = P(n) V
+//   two helper warps     the blocks that hold drafted rows: rows behind the last node are
+//                        zeroed and non-finite values taken out before the MMA reads V
+//   two softmax groups   128 threads, one row each; group w takes the blocks n % 2 = w
+//                        with a maximum, sum and output of its own: S from tensor memory,
+//                        online softmax, P back as three bf16 planes (the MMA's A operand
+//                        is read from tensor memory), then O(n) into its registers
+// so that the tensor core works on one block while the groups are in the softmax of the
+// two around it. The groups' results are joined like two splits.
+// Tensor memory (512 columns): S 2 x 64, P 2 x 96, O 128. V is read as it lies, slots x
+// dims: a descriptor with the dims as the contiguous ("MN") direction.
+// Bound: 6 x 2^20 multiply-adds per block at 4096 per cycle, 1536 cycles, against 64 slots x
+// 512 bytes from HBM at one SM's share of 44 GB/s, 0.74 us.
+#include "tc.cuh"
+#include "tree_attn.cuh"
+
+namespace dllm {
+namespace {
+
+constexpr int kTcAttnThreads = 384;
+constexpr int kStages = 3;
+constexpr int kErrWait = 5;  // the tensor-core wait code
+
+DLLM_DEV void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// A wait that ends early once another wait of the CTA has given up.
+DLLM_DEV bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort, int* err) {
+  const uint32_t a = smem_u32(bar);
+  const long long t0 = clock64();
+  for (;;) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(a), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if (*abort) return false;
+    if (clock64() - t0 > kTcWaitCycles) {
+      *abort = 1;
+      atomicExch(err, kErrWait);
+      return false;
+    }
+  }
+}
+
+// D[tmem] (+)= A[tmem, 128 x 16] * B[16 x N]: the A operand as packed bf16 pairs, 8 columns.
+DLLM_DEV void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+// Shared-memory descriptor of a tile whose contiguous direction is the MMA's N (dims): rows
+// of 64 dims (128 bytes, swizzled), one per K index (slot); 8-slot groups 1024 bytes
+// apart (stride offset), 64-dim boxes `box` bytes apart (leading offset).
+DLLM_DEV uint64_t umma_desc_mn_sw128(const void* tile, uint32_t box) {
+  const uint64_t a = smem_u32(tile);
+  return ((a & 0x3FFFFull) >> 4) | ((uint64_t)(box >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+
+#define R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+// 32 consecutive columns of this thread's lane.
+DLLM_DEV void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : R8(r, 0), R8(r, 8), R8(r, 16), R8(r, 24)
+      : "r"(addr));
+}
+DLLM_DEV void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::W8(r, 0), "r"(addr)
+               : "memory");
+}
+#undef R8
+#undef W8
+DLLM_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int HD>
+struct TcTile {
+  static constexpr int BOX = HD / 64;                      // 64-dim boxes
+  static constexpr int kQPlane = BOX * kTcRows * 128;      // bytes of one bf16 term of q
+  static constexpr int kBox = kTcBlock * 128;              // bytes of a 64 x 64 box
+  static constexpr int kKV = BOX * kBox;                   // bytes of a K or V block
+  static constexpr int kRing = 2 * kStages * kKV;
+  static constexpr int kOut = 2 * kTcRows * (HD + 6) * 4;  // both groups' results, over q and ring
+  static constexpr int kSmem = 1024 + 3 * kQPlane + kRing;
+  static_assert(kOut <= 3 * kQPlane + kRing, "results reuse the operands' memory");
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+  static constexpr uint32_t kP = 128, kO = 320;            // tensor-memory columns: S 0, 64; P; O
+};
+
+struct TcShared {
+  uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
+  uint64_t s_full[2], p_ready[2], o_full[2], o_free[2];  // per softmax group
+  uint64_t v_ok[2];                                      // the (at most two) blocks with drafted rows
+  uint32_t tmem;
+  int bad[2];
+  volatile int abort;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kTcAttnThreads, 1)
+    tree_attn_tc_kernel(const __grid_constant__ TAKernelArgs P, const __grid_constant__ CUtensorMap tmK,
+                        const __grid_constant__ CUtensorMap tmV) {
+  using T = TcTile<HD>;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ __align__(8) TcShared sh;
+  const TreeAttnArgs& a = P.a;
+  asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled; it waits for this grid's end
+  TATile k;
+  k.sq = a.seqs[blockIdx.z];
+  k.G = a.nq / a.kvh;
+  k.head = blockIdx.y % a.kvh;
+  k.r0 = (blockIdx.y / a.kvh) * kTcRows;
+  k.R = k.sq.m * k.G;
+  const int T0 = P.t0[blockIdx.z], slots = T0 + k.sq.m;
+  k.nsplit = ta_splits(slots, kTcBlock, P.bps);
+  k.split = blockIdx.x;
+  if (k.r0 >= k.R || k.split >= k.nsplit) return;
+  const int blk0 = k.split * P.bps;
+  const int nb = min((slots + kTcBlock - 1) / kTcBlock, blk0 + P.bps) - blk0;
+  const int draft0 = T0 / kTcBlock - blk0;  // the first block (of this CTA's) with drafted rows
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  unsigned char* sQ = base;
+  unsigned char* sK = base + 3 * T::kQPlane;
+  unsigned char* sV = sK + kStages * T::kKV;
+
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&sh.k_full[s], 1), mbar_init(&sh.k_empty[s], 1);
+      mbar_init(&sh.v_full[s], 1), mbar_init(&sh.v_empty[s], 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&sh.s_full[w], 1), mbar_init(&sh.p_ready[w], 128);
+      mbar_init(&sh.o_full[w], 1), mbar_init(&sh.o_free[w], 128);
+      mbar_init(&sh.v_ok[w], 64);
+      sh.bad[w] = 0;
+    }
+    sh.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  // q, scaled so that the softmax is in powers of two, as three bf16 planes of swizzled
+  // 64-dim boxes (what the K-major descriptor reads)
+  for (int i = tid; i < kTcRows * HD / 8; i += kTcAttnThreads) {
+    const int row = i / (HD / 8), d = (i % (HD / 8)) * 8, r = k.r0 + row;
+    uint4 h = make_uint4(0, 0, 0, 0), m = h, l = h;
+    if (r < k.R) {
+      const int node = r / k.G;
+      const float* q = a.q + ((size_t)(k.sq.row0 + node) * a.nq + k.head * k.G + (r - node * k.G)) * HD + d;
+      const float4 f = *reinterpret_cast<const float4*>(q), g = *reinterpret_cast<const float4*>(q + 4);
+      const float c = a.scale_log2;
+      split3(f.x * c, f.y * c, h.x, m.x, l.x);
+      split3(f.z * c, f.w * c, h.y, m.y, l.y);
+      split3(g.x * c, g.y * c, h.z, m.z, l.z);
+      split3(g.z * c, g.w * c, h.w, m.w, l.w);
+    }
+    unsigned char* at = sQ + (d / 64) * (kTcRows * 128) + row * 128 + ((((d % 64) >> 3) ^ (row & 7)) << 4);
+    *reinterpret_cast<uint4*>(at) = h;
+    *reinterpret_cast<uint4*>(at + T::kQPlane) = m;
+    *reinterpret_cast<uint4*>(at + 2 * T::kQPlane) = l;
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // q is read by the MMA
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 8 && lane == 0) {
+      // ---- producer. The pools are one tensor of rows (layer, page, head, slot); a page holds 32
+      // slots (two boxes of a block) or a multiple of 64 (one).
+      const int page = 1 << a.kv.log2_page, box = page < kTcBlock ? page : kTcBlock;
+      const int* table = a.kv.page_table + (size_t)k.sq.seq * a.kv.max_pages;
+      int k_sent = 0, v_sent = 0;
+      for (int n = 0; n < nb; ++n) {
+        const int s = n % kStages;
+        const uint32_t ph = (uint32_t)(n / kStages) & 1u;
+        int row[2];
+        for (int b = 0; b < kTcBlock / box; ++b) {
+          const int slot = min((blk0 + n) * kTcBlock + b * box, slots - 1) & ~(box - 1);  // behind the end: loaded again, unused
+          row[b] = a.tc_row0 + (table[slot >> a.kv.log2_page] * a.kvh + k.head) * page + (slot & (page - 1));
+        }
+        if (!wait_or_abort(&sh.k_empty[s], ph ^ 1u, &sh.abort, a.err)) break;
+        mbar_expect_tx(&sh.k_full[s], T::kKV);
+        for (int b = 0; b < kTcBlock / box; ++b)
+          for (int x = 0; x < T::BOX; ++x)
+            tma_load_2d(sK + s * T::kKV + x * T::kBox + b * box * 128, &tmK, x * 64, row[b], &sh.k_full[s]);
+        k_sent = n + 1;
+        if (!wait_or_abort(&sh.v_empty[s], ph ^ 1u, &sh.abort, a.err)) break;
+        mbar_expect_tx(&sh.v_full[s], T::kKV);
+        for (int b = 0; b < kTcBlock / box; ++b)
+          for (int x = 0; x < T::BOX; ++x)
+            tma_load_2d(sV + s * T::kKV + x * T::kBox + b * box * 128, &tmV, x * 64, row[b], &sh.v_full[s]);
+        v_sent = n + 1;
+      }
+      // whatever happened to the others, the copies under way land before the CTA ends
+      for (int j = max(0, k_sent - kStages); j < k_sent; ++j) mbar_wait(&sh.k_full[j % kStages], (uint32_t)(j / kStages) & 1u);
+      for (int j = max(0, v_sent - kStages); j < v_sent; ++j) mbar_wait(&sh.v_full[j % kStages], (uint32_t)(j / kStages) & 1u);
+    } else if (warp == 9 && lane == 0) {
+      // ---- MMA issuer
+      const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kTcRows >> 4) << 24);  // fp32 += bf16 x bf16
+      const uint32_t id_s = idesc | ((uint32_t)(kTcBlock >> 3) << 17);                  // N = 64 slots, K-major
+      const uint32_t id_o = idesc | ((uint32_t)(HD >> 3) << 17) | (1u << 16);           // N = hd, B with N contiguous
+      auto scores = [&](int n) {
+        const int s = n % kStages;
+        if (!wait_or_abort(&sh.k_full[s], (uint32_t)(n / kStages) & 1u, &sh.abort, a.err)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int p = 2; p >= 0; --p)
+#pragma unroll
+          for (int x = 0; x < T::BOX; ++x) {
+            const uint64_t ad = umma_desc_sw128(sQ + p * T::kQPlane + x * (kTcRows * 128));
+            const uint64_t bd = umma_desc_sw128(sK + s * T::kKV + x * T::kBox);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_bf16(tmem + (uint32_t)(n & 1) * 64, ad + 2ull * kk, bd + 2ull * kk, id_s, (uint32_t)(p != 2 || x || kk));
+          }
+        umma_commit(&sh.k_empty[s]);
+        umma_commit(&sh.s_full[n & 1]);
+        return true;
+      };
+      bool ok = scores(0);
+      for (int n = 0; ok && n < nb; ++n) {
+        if (n + 1 < nb) ok = scores(n + 1);
+        const int s = n % kStages, w = n & 1;
+        const uint32_t ph = (uint32_t)(n >> 1) & 1u;
+        if (ok && n > 0) ok = wait_or_abort(&sh.o_free[w ^ 1], (uint32_t)((n - 1) >> 1) & 1u, &sh.abort, a.err);
+        if (ok) ok = wait_or_abort(&sh.v_full[s], (uint32_t)(n / kStages) & 1u, &sh.abort, a.err);
+        if (ok && n >= draft0) ok = wait_or_abort(&sh.v_ok[n - draft0], 0u, &sh.abort, a.err);
+        if (ok) ok = wait_or_abort(&sh.p_ready[w], ph, &sh.abort, a.err);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int p = 2; p >= 0; --p) {
+          const uint32_t ap = tmem + T::kP + (uint32_t)w * 96 + (uint32_t)p * 32;
+          const uint64_t bd = umma_desc_mn_sw128(sV + s * T::kKV, T::kBox);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)  // 16 slots: 2048 bytes on
+            umma_bf16_ts(tmem + T::kO, ap + 8u * kk, bd + 128ull * kk, id_o, (uint32_t)(p != 2 || kk));
+        }
+        umma_commit(&sh.v_empty[s]);
+        umma_commit(&sh.o_full[w]);
+      }
+    } else if (warp >= 10) {
+      // ---- V rows of the blocks that reach behind the context: one thread per slot
+      const int row = tid - 320;
+      for (int n = max(0, draft0); n < nb; ++n) {
+        const int s = n % kStages, slot = (blk0 + n) * kTcBlock + row;
+        if (!wait_or_abort(&sh.v_full[s], (uint32_t)(n / kStages) & 1u, &sh.abort, a.err)) break;
+        if (slot >= T0) {
+#pragma unroll 1
+          for (int c = 0; c < HD / 8; ++c) {
+            uint4* at = reinterpret_cast<uint4*>(sV + s * T::kKV + (c / 8) * T::kBox + row * 128 + (((c & 7) ^ (row & 7)) << 4));
+            if (slot >= slots) {
+              *at = make_uint4(0, 0, 0, 0);
+              continue;
+            }
+            uint4 v = *at;
+            uint32_t hit = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t& u = e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w;
+              const uint32_t lo = (u & 0x7f80u) == 0x7f80u, hi = (u & 0x7f800000u) == 0x7f800000u;
+              if (lo) u &= 0xffff0000u;
+              if (hi) u &= 0x0000ffffu;
+              hit |= lo | hi;
+            }
+            if (hit) {
+              *at = v;
+              atomicOr(&sh.bad[n - draft0], 1);
+            }
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(&sh.v_ok[n - draft0]);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax: group w, one row per thread
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    const int w = warp >> 2, row = tid & 127, r = k.r0 + row;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const unsigned long long anc = r < k.R ? a.anc[k.sq.row0 + r / k.G] : 0ull;
+    float o[HD], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int d = 0; d < HD; ++d) o[d] = 0.f;
+    bool ok = true;
+    for (int n = w; ok && n < nb; n += 2) {
+      const uint32_t ph = (uint32_t)(n >> 1) & 1u;
+      const bool drafted = n >= draft0;
+      ok = wait_or_abort(&sh.s_full[w], ph, &sh.abort, a.err);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t u0[32], u1[32];
+      tmem_ld32(lanes + (uint32_t)w * 64, u0);
+      tmem_ld32(lanes + (uint32_t)w * 64 + 32, u1);
+      tmem_ld_wait();
+      unsigned long long see = ~0ull;  // which of the block's slots this row sees
+      if (drafted) {
+        const int node0 = (blk0 + n) * kTcBlock - T0;
+        see = node0 >= 0 ? (node0 < 64 ? anc >> node0 : 0ull) : (anc << -node0) | ((1ull << -node0) - 1);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          if (!(see >> c & 1)) u0[c] = __float_as_uint(-INFINITY);
+          if (!(see >> (c + 32) & 1)) u1[c] = __float_as_uint(-INFINITY);
+        }
+      }
+      float x0 = m, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 32; c += 2) {
+        x0 = fmaxf(x0, __uint_as_float(u0[c])), x1 = fmaxf(x1, __uint_as_float(u0[c + 1]));
+        x2 = fmaxf(x2, __uint_as_float(u1[c])), x3 = fmaxf(x3, __uint_as_float(u1[c + 1]));
+      }
+      const float x = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3));
+      const float b = x == -INFINITY ? 0.f : x;  // a row that has seen nothing: every p is 0
+      const float f = ex2(m - b);
+      m = x;
+      float s0 = 0.f, s1 = 0.f;
+      const uint32_t tp = lanes + T::kP + (uint32_t)w * 96;
+#pragma unroll
+      for (int c = 0; c < 64; c += 16) {  // 8 packed columns of each plane at a time
+        uint32_t ph8[8], pm8[8], pl8[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float p0 = ex2(__uint_as_float(c < 32 ? u0[(c + 2 * e) & 31] : u1[(c + 2 * e) & 31]) - b);
+          const float p1 = ex2(__uint_as_float(c < 32 ? u0[(c + 2 * e + 1) & 31] : u1[(c + 2 * e + 1) & 31]) - b);
+          s0 += p0, s1 += p1;
+          split3(p0, p1, ph8[e], pm8[e], pl8[e]);
+        }
+        tmem_st8(tp + (uint32_t)(c / 2), ph8);
+        tmem_st8(tp + 32u + (uint32_t)(c / 2), pm8);
+        tmem_st8(tp + 64u + (uint32_t)(c / 2), pl8);
+      }
+      l = fmaf(l, f, s0 + s1);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&sh.p_ready[w]);
+      ok = wait_or_abort(&sh.o_full[w], ph, &sh.abort, a.err);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll
+      for (int d = 0; d < HD; d += 32) {
+        tmem_ld32(lanes + T::kO + (uint32_t)d, u0);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[d + e] = fmaf(o[d + e], f, __uint_as_float(u0[e]));
+      }
+      tc_fence_before();
+      mbar_arrive(&sh.o_free[w]);
+      if (drafted) {
+        // values that were taken out of V, added where they are seen (the wait orders the flag)
+        if (!wait_or_abort(&sh.v_ok[n - draft0], 0u, &sh.abort, a.err)) break;
+        if (sh.bad[n - draft0]) {
+          for (int j = 0; j < kTcBlock; ++j) {
+            const int slot = (blk0 + n) * kTcBlock + j;
+            if (slot < T0 || slot >= slots || !(see >> j & 1)) continue;
+            const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.vc) + a.kv.offset(k.sq.seq, slot, k.head);
+#pragma unroll
+            for (int d = 0; d < HD; ++d) {
+              const float e = bf16_to_f32(v[d]);
+              if (!is_finite(e)) o[d] += e;
+            }
+          }
+        }
+      }
+    }
+    // every MMA has completed (this group waited for its last O, and so did the other)
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    float* sO = reinterpret_cast<float*>(base);
+    float* sML = sO + 2 * kTcRows * (HD + 4);
+    float* mine = sO + (w * kTcRows + row) * (HD + 4);
+#pragma unroll
+    for (int d = 0; d < HD; d += 4) *reinterpret_cast<float4*>(mine + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+    sML[(w * kTcRows + row) * 2] = m, sML[(w * kTcRows + row) * 2 + 1] = l;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (!sh.abort) ta_finish<HD, 2, kTcRows>(P, k, sO, sML, tid, 256);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
+}
+
+}  // namespace
+
+cudaError_t configure_tree_attn_tc() {
+  cudaError_t e = cudaFuncSetAttribute(tree_attn_tc_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcTile<64>::kSmem);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(tree_attn_tc_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcTile<128>::kSmem);
+  return e;
+}
+
+cudaError_t launch_tree_attn_tc(const TAKernelArgs& P, int hd, dim3 grid, cudaStream_t st) {
+  const CUtensorMap &mk = *static_cast<const CUtensorMap*>(P.a.tc_k), &mv = *static_cast<const CUtensorMap*>(P.a.tc_v);
+  if (hd == 64)
+    tree_attn_tc_kernel<64><<<grid, kTcAttnThreads, TcTile<64>::kSmem, st>>>(P, mk, mv);
+  else
+    tree_attn_tc_kernel<128><<<grid, kTcAttnThreads, TcTile<128>::kSmem, st>>>(P, mk, mv);
+  return cudaGetLastError();
+}
+
+}  // namespace dllm
