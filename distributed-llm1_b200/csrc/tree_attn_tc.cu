@@ -57,6 +57,34 @@ DLLM_DEV bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort,
   }
 }
 
+// The same for a whole warp that stays together; the result is the same in every lane.
+DLLM_DEV bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* err) {
+  const uint32_t a = smem_u32(bar);
+  const long long t0 = clock64();
+  for (;;) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(a), "r"(parity)
+        : "memory");
+    if (__all_sync(0xffffffffu, done)) return true;
+    if (__any_sync(0xffffffffu, *abort)) return false;
+    if (__any_sync(0xffffffffu, clock64() - t0 > kTcWaitCycles)) {
+      *abort = 1;
+      atomicExch(err, kErrWait);
+      return false;
+    }
+  }
+}
+DLLM_DEV uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
+}
+
 // D[tmem] (+)= A[tmem, 128 x 16] * B[16 x N]: the A operand as packed bf16 pairs, 8 columns.
 DLLM_DEV void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -137,7 +165,8 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
   const int nb = min((slots + kTcBlock - 1) / kTcBlock, blk0 + P.bps) - blk0;
   const int draft0 = T0 / kTcBlock - blk0;  // the first block (of this CTA's) with drafted rows
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // the warp's number as a value that is the same in all its lanes by construction
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* sQ = base;
   unsigned char* sK = base + 3 * T::kQPlane;
@@ -185,7 +214,7 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = sh.tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
@@ -219,50 +248,58 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
       // whatever happened to the others, the copies under way land before the CTA ends
       for (int j = max(0, k_sent - kStages); j < k_sent; ++j) mbar_wait(&sh.k_full[j % kStages], (uint32_t)(j / kStages) & 1u);
       for (int j = max(0, v_sent - kStages); j < v_sent; ++j) mbar_wait(&sh.v_full[j % kStages], (uint32_t)(j / kStages) & 1u);
-    } else if (warp == 9 && lane == 0) {
-      // ---- MMA issuer
+    } else if (warp == 9) {
+      // ---- MMA issuer. The whole warp runs the loop and one elected lane issues: the operands
+      // of tcgen05.mma live in uniform registers, and in a branch on the lane number
+      // every one of them was first moved there (130 to 230 cycles per MMA; 49 and 65 this way).
+      const uint32_t leader = elect_one();
       const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kTcRows >> 4) << 24);  // fp32 += bf16 x bf16
       const uint32_t id_s = idesc | ((uint32_t)(kTcBlock >> 3) << 17);                  // N = 64 slots, K-major
       const uint32_t id_o = idesc | ((uint32_t)(HD >> 3) << 17) | (1u << 16);           // N = hd, B with N contiguous
       auto scores = [&](int n) {
         const int s = n % kStages;
-        if (!wait_or_abort(&sh.k_full[s], (uint32_t)(n / kStages) & 1u, &sh.abort, a.err)) return false;
+        if (!warp_wait(&sh.k_full[s], (uint32_t)(n / kStages) & 1u, &sh.abort, a.err)) return false;
         tc_fence_after();
+        if (leader) {
 #pragma unroll
-        for (int p = 2; p >= 0; --p)
+          for (int p = 2; p >= 0; --p)
 #pragma unroll
-          for (int x = 0; x < T::BOX; ++x) {
-            const uint64_t ad = umma_desc_sw128(sQ + p * T::kQPlane + x * (kTcRows * 128));
-            const uint64_t bd = umma_desc_sw128(sK + s * T::kKV + x * T::kBox);
+            for (int x = 0; x < T::BOX; ++x) {
+              const uint64_t ad = umma_desc_sw128(sQ + p * T::kQPlane + x * (kTcRows * 128));
+              const uint64_t bd = umma_desc_sw128(sK + s * T::kKV + x * T::kBox);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              umma_bf16(tmem + (uint32_t)(n & 1) * 64, ad + 2ull * kk, bd + 2ull * kk, id_s, (uint32_t)(p != 2 || x || kk));
-          }
-        umma_commit(&sh.k_empty[s]);
-        umma_commit(&sh.s_full[n & 1]);
+              for (int kk = 0; kk < 4; ++kk)
+                umma_bf16(tmem + (uint32_t)(n & 1) * 64, ad + 2ull * kk, bd + 2ull * kk, id_s, (uint32_t)(p != 2 || x || kk));
+            }
+          umma_commit(&sh.k_empty[s]);
+          umma_commit(&sh.s_full[n & 1]);
+        }
+        __syncwarp();
         return true;
       };
       bool ok = scores(0);
       for (int n = 0; ok && n < nb; ++n) {
         if (n + 1 < nb) ok = scores(n + 1);
         const int s = n % kStages, w = n & 1;
-        const uint32_t ph = (uint32_t)(n >> 1) & 1u;
-        if (ok && n > 0) ok = wait_or_abort(&sh.o_free[w ^ 1], (uint32_t)((n - 1) >> 1) & 1u, &sh.abort, a.err);
-        if (ok) ok = wait_or_abort(&sh.v_full[s], (uint32_t)(n / kStages) & 1u, &sh.abort, a.err);
-        if (ok && n >= draft0) ok = wait_or_abort(&sh.v_ok[n - draft0], 0u, &sh.abort, a.err);
-        if (ok) ok = wait_or_abort(&sh.p_ready[w], ph, &sh.abort, a.err);
+        if (ok && n > 0) ok = warp_wait(&sh.o_free[w ^ 1], (uint32_t)((n - 1) >> 1) & 1u, &sh.abort, a.err);
+        if (ok) ok = warp_wait(&sh.v_full[s], (uint32_t)(n / kStages) & 1u, &sh.abort, a.err);
+        if (ok && n >= draft0) ok = warp_wait(&sh.v_ok[n - draft0], 0u, &sh.abort, a.err);
+        if (ok) ok = warp_wait(&sh.p_ready[w], (uint32_t)(n >> 1) & 1u, &sh.abort, a.err);
         if (!ok) break;
         tc_fence_after();
+        if (leader) {
 #pragma unroll
-        for (int p = 2; p >= 0; --p) {
-          const uint32_t ap = tmem + T::kP + (uint32_t)w * 96 + (uint32_t)p * 32;
-          const uint64_t bd = umma_desc_mn_sw128(sV + s * T::kKV, T::kBox);
+          for (int p = 2; p >= 0; --p) {
+            const uint32_t ap = tmem + T::kP + (uint32_t)w * 96 + (uint32_t)p * 32;
+            const uint64_t bd = umma_desc_mn_sw128(sV + s * T::kKV, T::kBox);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)  // 16 slots: 2048 bytes on
-            umma_bf16_ts(tmem + T::kO, ap + 8u * kk, bd + 128ull * kk, id_o, (uint32_t)(p != 2 || kk));
+            for (int kk = 0; kk < 4; ++kk)  // 16 slots: 2048 bytes on
+              umma_bf16_ts(tmem + T::kO, ap + 8u * kk, bd + 128ull * kk, id_o, (uint32_t)(p != 2 || kk));
+          }
+          umma_commit(&sh.v_empty[s]);
+          umma_commit(&sh.o_full[w]);
         }
-        umma_commit(&sh.v_empty[s]);
-        umma_commit(&sh.o_full[w]);
+        __syncwarp();
       }
     } else if (warp >= 10) {
       // ---- V rows of the blocks that reach behind the context: one thread per slot
