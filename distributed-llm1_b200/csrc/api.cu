@@ -699,7 +699,6 @@ int tree_attention(dllm_stage* s, int layer, const dllm_tree* tree, const dllm::
   a.kc = layer_pool(s, s->kpool, layer);
   a.vc = layer_pool(s, s->vpool, layer);
   a.kv = stage_kv(s);
-  a.seqs = tree->seqs_dev();
   a.anc = tree->anc_dev();
   a.n_seqs = tree->n_seqs;
   a.nq = f.num_q_heads;

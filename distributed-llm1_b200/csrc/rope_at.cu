@@ -9,10 +9,13 @@
 // sincospif in 32 bits. A 32-bit product would be off by pos * 2^-24 radians
 // (0.06 at position 10^6); this form stays within 2^-52 * turns of the angle.
 //
-// Bound by memory (8 bytes per element moved, ~1 flop per byte). A thread owns
-// kVec pairs of one head position and keeps their cos and sin in registers while
-// it walks the heads of the row, so the trigonometry is done once per row and not
-// once per head.
+// Bound by memory (8 bytes per element moved, ~1 flop per byte). A thread owns kVec pairs
+// of one head position and keeps their cos and sin in registers while it walks the heads
+// of a row, so the trigonometry is done once per row and not once per head. Short rows lie
+// side by side in a CTA (6000 rows of 1024 elements, 7.5 us of traffic: 18.6 us with one
+// CTA per row, 10.7 so). A CTA ends with its rows: one that stays and loads the next rows
+// ahead needs twice the registers and was slower (45.3 against 43.1 us for 8191 rows of
+// 4096, whose traffic takes 41.1).
 #include "verify.cuh"
 
 namespace dllm {
@@ -46,34 +49,36 @@ DLLM_DEV void st_pack(float* p, const Pack<VEC>& r) {
 
 // A head has hd / (2 VEC) units of VEC pairs: the first rotary / (2 VEC) turn, the
 // rest are copied (or left, in place). Four pairs at a time (16-byte accesses)
-// need rotary to be a multiple of 8; other sizes go pair by pair.
-template <int VEC, bool INTER>
-__global__ void __launch_bounds__(kRopeThreads) rope_at_kernel(const RopeAtArgs a) {
-  const int units = a.hd / (2 * VEC);
+// need rotary to be a multiple of 8; other sizes go pair by pair, with U heads in flight
+// per thread to keep as many bytes under way.
+template <int HD, int VEC, int U, bool INTER>
+__global__ void __launch_bounds__(kRopeThreads) rope_at_kernel(const RopeAtArgs a, int log2_side) {
+  constexpr int units = HD / (2 * VEC), slots = kRopeThreads / units;
   const int turning = a.rotary / (2 * VEC);
-  const int unit = threadIdx.x % units;
-  const int per = kRopeThreads / units;  // heads in flight
   const int heads = a.q_heads + a.k_heads;
-  const int row = blockIdx.x;
+  // a CTA's threads: rows, heads side by side (1 << log2_side, the rest in turn), units
+  const int unit = threadIdx.x % units, slot = threadIdx.x / units;
+  const int h_first = (blockIdx.y << log2_side) + (slot & ((1 << log2_side) - 1)), h_step = gridDim.y << log2_side;
+  const int row = blockIdx.x * (slots >> log2_side) + (slot >> log2_side);
   const bool turns = unit < turning;
   // float offsets of the unit's two packs within a head
   const int o1 = turns ? (INTER ? unit * 2 * VEC : unit * VEC) : a.rotary + (unit - turning) * 2 * VEC;
   const int o2 = turns ? (INTER ? o1 + VEC : o1 + a.rotary / 2) : o1 + VEC;
-  // the first head's elements are on their way while the angles are computed
-  auto head_at = [&](int h, const float*& src, float*& dst) {
-    const bool is_q = h < a.q_heads;
-    const size_t at = is_q ? ((size_t)row * a.q_heads + h) * a.hd : ((size_t)row * a.k_heads + (h - a.q_heads)) * a.hd;
-    src = (is_q ? a.q : a.k) + at;
-    dst = (is_q ? a.q_out : a.k_out) + at;
+  auto at = [&](int r, int h) {
+    return h < a.q_heads ? ((size_t)r * a.q_heads + h) * HD : ((size_t)r * a.k_heads + (h - a.q_heads)) * HD;
   };
-  const float* src;
-  float* dst;
-  int h = blockIdx.y * per + threadIdx.x / units;
-  Pack<VEC> x, y;
-  if (h < heads) {
-    head_at(h, src, dst);
-    x = ld_pack<VEC>(src + o1), y = ld_pack<VEC>(src + o2);
-  }
+  if (row >= a.n) return;
+  Pack<VEC> x[U], y[U];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u * h_step;
+      if (h >= heads) break;
+      const float* src = (h < a.q_heads ? a.q : a.k) + at(row, h);
+      x[u] = ld_pack<VEC>(src + o1), y[u] = ld_pack<VEC>(src + o2);
+    }
+  };
+  load(h_first);  // on the way while the angles are computed
   float c[VEC], s[VEC];
   if (turns) {
     const double pos = (double)a.pos[row];
@@ -85,57 +90,68 @@ __global__ void __launch_bounds__(kRopeThreads) rope_at_kernel(const RopeAtArgs 
       c[i] *= a.factor;
     }
   }
-  while (h < heads) {
-    if (turns) {
-      if constexpr (INTER && VEC == 4) {  // (x0 x1)(x2 x3) | (y0 y1)(y2 y3)
+  for (int h0 = h_first; h0 < heads; h0 += U * h_step) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float x1 = x.v[2 * i], x2 = x.v[2 * i + 1], y1 = y.v[2 * i], y2 = y.v[2 * i + 1];
-          x.v[2 * i] = fmaf(x1, c[i], -(x2 * s[i]));
-          x.v[2 * i + 1] = fmaf(x1, s[i], x2 * c[i]);
-          y.v[2 * i] = fmaf(y1, c[2 + i], -(y2 * s[2 + i]));
-          y.v[2 * i + 1] = fmaf(y1, s[2 + i], y2 * c[2 + i]);
-        }
-      } else {
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u * h_step;
+      if (h >= heads) break;
+      if (turns) {
+        if constexpr (INTER && VEC == 4) {  // (x0 x1)(x2 x3) | (y0 y1)(y2 y3)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float x1 = x.v[i], x2 = y.v[i];
-          x.v[i] = fmaf(x1, c[i], -(x2 * s[i]));
-          y.v[i] = fmaf(x1, s[i], x2 * c[i]);
+          for (int i = 0; i < 2; ++i) {
+            const float x1 = x[u].v[2 * i], x2 = x[u].v[2 * i + 1], y1 = y[u].v[2 * i], y2 = y[u].v[2 * i + 1];
+            x[u].v[2 * i] = fmaf(x1, c[i], -(x2 * s[i]));
+            x[u].v[2 * i + 1] = fmaf(x1, s[i], x2 * c[i]);
+            y[u].v[2 * i] = fmaf(y1, c[2 + i], -(y2 * s[2 + i]));
+            y[u].v[2 * i + 1] = fmaf(y1, s[2 + i], y2 * c[2 + i]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float x1 = x[u].v[i], x2 = y[u].v[i];
+            x[u].v[i] = fmaf(x1, c[i], -(x2 * s[i]));
+            y[u].v[i] = fmaf(x1, s[i], x2 * c[i]);
+          }
         }
       }
+      const size_t o = at(row, h);
+      float* dst = (h < a.q_heads ? a.q_out : a.k_out) + o;
+      if (turns || dst != (h < a.q_heads ? a.q : a.k) + o) {
+        st_pack<VEC>(dst + o1, x[u]);
+        st_pack<VEC>(dst + o2, y[u]);
+      }
     }
-    if (turns || src != dst) {
-      st_pack<VEC>(dst + o1, x);
-      st_pack<VEC>(dst + o2, y);
-    }
-    h += per * gridDim.y;
-    if (h < heads) {
-      head_at(h, src, dst);
-      x = ld_pack<VEC>(src + o1), y = ld_pack<VEC>(src + o2);
-    }
+    load(h0 + U * h_step);
   }
+}
+
+template <int HD, int VEC, int U, bool INTER>
+cudaError_t launch_rope(const RopeAtArgs& a, int sms, cudaStream_t st) {
+  constexpr int slots = kRopeThreads / (HD / (2 * VEC));
+  const int heads = a.q_heads + a.k_heads;
+  int log2_side = 0;
+  while ((1 << log2_side) < heads && (1 << log2_side) < slots) ++log2_side;
+  const int rows = slots >> log2_side, chunks = (heads + (1 << log2_side) - 1) >> log2_side;
+  const int ctas = (a.n + rows - 1) / rows;
+  // few rows: the heads of a row are spread over CTAs as well, which repeats the
+  // angles but leaves one load and store per thread (64 rows of 32 heads: 4.5 us in
+  // one CTA per row, 3.3 in two)
+  const dim3 grid(ctas, (long long)ctas * chunks <= 8ll * sms ? chunks : 1);
+  rope_at_kernel<HD, VEC, U, INTER><<<grid, kRopeThreads, 0, st>>>(a, log2_side);
+  return cudaGetLastError();
+}
+
+template <int HD>
+cudaError_t rope_hd(const RopeAtArgs& a, int sms, cudaStream_t st) {
+  if (a.rotary % 8 == 0)
+    return a.interleaved ? launch_rope<HD, 4, 1, true>(a, sms, st) : launch_rope<HD, 4, 1, false>(a, sms, st);
+  return a.interleaved ? launch_rope<HD, 1, 4, true>(a, sms, st) : launch_rope<HD, 1, 4, false>(a, sms, st);
 }
 
 }  // namespace
 
 cudaError_t op_rope_at(const RopeAtArgs& a, int sms, cudaStream_t st) {
-  const bool vec = a.rotary % 8 == 0;
-  // few rows: the heads of a row are spread over CTAs as well, which repeats the
-  // angles but leaves one load and store per thread (64 rows of 32 heads: 4.5 us in
-  // one CTA per row)
-  const int per = kRopeThreads / (a.hd / (vec ? 8 : 2));
-  const int chunks = (a.q_heads + a.k_heads + per - 1) / per;
-  const dim3 grid(a.n, (long long)a.n * chunks <= 8ll * sms ? chunks : 1);
-  if (vec && a.interleaved)
-    rope_at_kernel<4, true><<<grid, kRopeThreads, 0, st>>>(a);
-  else if (vec)
-    rope_at_kernel<4, false><<<grid, kRopeThreads, 0, st>>>(a);
-  else if (a.interleaved)
-    rope_at_kernel<1, true><<<grid, kRopeThreads, 0, st>>>(a);
-  else
-    rope_at_kernel<1, false><<<grid, kRopeThreads, 0, st>>>(a);
-  return cudaGetLastError();
+  return a.hd == 64 ? rope_hd<64>(a, sms, st) : rope_hd<128>(a, sms, st);
 }
 
 }  // namespace dllm

@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kTAThreads, 1) tree_attn_kernel(const __grid_c
   extern __shared__ __align__(1024) unsigned char smem[];
   const TreeAttnArgs& a = P.a;
   asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled; it waits for this grid's end
-  const TreeSeq sq = a.seqs[blockIdx.z];
+  const TreeSeq sq = ta_seq(P, blockIdx.z);
   const int G = a.nq / a.kvh;
   const int head = blockIdx.y % a.kvh, tile = blockIdx.y / a.kvh;
   const int R = sq.m * G, r0 = tile * RT;
@@ -464,7 +464,7 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ 
   constexpr int V = HD / 32, kBatch = 4;
   __shared__ float so[8][HD], sml[8][2];
   const TreeAttnArgs& a = P.a;
-  const TreeSeq sq = a.seqs[blockIdx.y];
+  const TreeSeq sq = ta_seq(P, blockIdx.y);
   const int nsplit = ta_splits(P.t0[blockIdx.y] + sq.m, bn, P.bps);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int item = blockIdx.x * (8 / W) + warp / W, w = warp % W;
@@ -554,8 +554,8 @@ cudaError_t configure_hd() {
   return e;
 }
 
-// Cuts the blocks of bn slots of all (sequence, KV head, tile of rt rows) into as many
-// CTAs as SMs, runs `main` over them, and joins the splits.
+// Cuts the blocks of bn slots of all (sequence, KV head, tile of rt rows) into at most as
+// many CTAs as SMs, runs `main` over them, and joins the splits.
 template <int HD, typename Main>
 cudaError_t launch_split(const TreeAttnArgs& a, const TreeAttnShape& s, int rt, int bn, int sms, int* launches,
                          cudaStream_t st, Main main) {
@@ -563,13 +563,28 @@ cudaError_t launch_split(const TreeAttnArgs& a, const TreeAttnShape& s, int rt, 
   P.a = a;
   const int G = a.nq / a.kvh;
   auto tiles = [&](int m) { return (m * G + rt - 1) / rt; };
-  long long total = 0;
-  for (int i = 0; i < a.n_seqs; ++i)
-    total += (long long)((s.t0[i] + s.seqs[i].m + bn - 1) / bn) * a.kvh * tiles(s.seqs[i].m);
+  auto blocks = [&](int i) { return s.seqs[i].m ? (s.t0[i] + s.seqs[i].m + bn - 1) / bn : 0; };
+  long long total = 0, items = 0;
+  for (int i = 0; i < a.n_seqs; ++i) {
+    const long long per = (long long)a.kvh * tiles(s.seqs[i].m);
+    total += blocks(i) * per;
+    items += per;
+  }
+  // blocks per split: the fewest with which all CTAs run at once (short last splits make
+  // that a little more than total / sms); with more items than SMs, about one SM's share
   P.bps = (int)std::max<long long>(1, (total + sms - 1) / sms);
+  for (int step = 0; items < sms && step < 256; ++step) {
+    long long ctas = 0;
+    for (int i = 0; i < a.n_seqs; ++i) ctas += (blocks(i) + P.bps - 1) / P.bps * (long long)a.kvh * tiles(s.seqs[i].m);
+    if (ctas <= sms) break;
+    P.bps += 1 + P.bps / 64;
+  }
   int splits = 1;
   size_t part = 0;
   for (int i = 0; i < a.n_seqs; ++i) {
+    P.seq[i] = s.seqs[i].seq;
+    P.row0[i] = s.seqs[i].row0;
+    P.m[i] = s.seqs[i].m;
     P.t0[i] = s.t0[i];
     const int m = s.seqs[i].m, ns = m ? ta_splits(s.t0[i] + m, bn, P.bps) : 1;
     P.part0[i] = (int)part;
@@ -579,10 +594,10 @@ cudaError_t launch_split(const TreeAttnArgs& a, const TreeAttnShape& s, int rt, 
   cudaError_t e = main(P, dim3(splits, a.kvh * tiles(s.max_m), a.n_seqs));
   *launches += 1;
   if (e != cudaSuccess || splits == 1) return e;
-  const int items = s.max_m * a.nq;  // rows and query heads of a sequence
+  const int rows = s.max_m * a.nq;  // rows and query heads of a sequence
   const bool many = splits > 8;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(many ? items : (items + 7) / 8, a.n_seqs);
+  cfg.gridDim = dim3(many ? rows : (rows + 7) / 8, a.n_seqs);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -617,9 +632,8 @@ cudaError_t launch_hd(const TreeAttnArgs& a, const TreeAttnShape& s, int sms, in
 
 }  // namespace
 
-// Splits exist only while all CTAs fit the SMs once: with bps >= total / sms a
-// sequence of more than one split has at most 2 blocks / bps of them, so the split
-// sequences' CTAs are at most 2 sms, each with up to 128 rows.
+// With bps >= total / sms a sequence of more than one split has at most 2 blocks / bps of
+// them, so the split sequences' CTAs are at most 2 sms, each with up to 128 rows.
 size_t tree_attn_part_rows(int sms) { return (size_t)2 * sms * 128; }
 
 cudaError_t configure_tree_attn() {

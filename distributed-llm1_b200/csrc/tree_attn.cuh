@@ -10,12 +10,19 @@
 
 namespace dllm {
 
+// Everything a CTA needs to know of its sequence travels as kernel arguments: a load
+// from memory before the first K/V address is known would cost every CTA its latency.
 struct TAKernelArgs {
   TreeAttnArgs a;
   int bps;                  // blocks per split
+  int seq[kTreeMaxSeqs];
+  int row0[kTreeMaxSeqs];
+  int m[kTreeMaxSeqs];
   int t0[kTreeMaxSeqs];
   int part0[kTreeMaxSeqs];  // first partial row of a split sequence
 };
+
+DLLM_DEV TreeSeq ta_seq(const TAKernelArgs& P, int i) { return TreeSeq{P.seq[i], P.row0[i], P.m[i], 0}; }
 
 // The number of splits of a sequence with `slots` slots; the same on host and device.
 __host__ __device__ inline int ta_splits(int slots, int bn, int bps) {

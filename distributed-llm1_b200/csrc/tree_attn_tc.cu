@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
   const TreeAttnArgs& a = P.a;
   asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled; it waits for this grid's end
   TATile k;
-  k.sq = a.seqs[blockIdx.z];
+  k.sq = ta_seq(P, blockIdx.z);
   k.G = a.nq / a.kvh;
   k.head = blockIdx.y % a.kvh;
   k.r0 = (blockIdx.y / a.kvh) * kTcRows;

@@ -95,7 +95,6 @@ struct TreeAttnArgs {
   const void* kc;  // the layer's pools
   const void* vc;
   KvLayout kv;
-  const TreeSeq* seqs;
   const unsigned long long* anc;
   int n_seqs, nq, kvh;
   float scale_log2;  // log2(e) / sqrt(hd)
@@ -106,10 +105,10 @@ struct TreeAttnArgs {
   float* part_o;   // [slots][hd] partial outputs of sequences that are split
   float* part_ml;  // [slots][2]
 };
-// Host-side counts of the call (the device reads the same from seqs).
+// The call's sequences, on the host.
 struct TreeAttnShape {
-  const TreeSeq* seqs;  // host
-  const int* t0;        // host, [n_seqs]
+  const TreeSeq* seqs;
+  const int* t0;  // [n_seqs]
   int n, max_m;
 };
 // Partial rows one call may write on `sms` SMs (the capacity of part_o / part_ml).
