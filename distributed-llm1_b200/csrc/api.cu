@@ -2446,7 +2446,7 @@ int dllm_pick_tokens(dllm_ctx* c, const dllm_pick* p) {
   if (p->history) {
     if (int rc = check_i32(c, p->history, 1, "pickTokens history")) return rc;
     if (int rc = check_i32(c, p->history_offsets, b + 1, "pickTokens history offsets")) return rc;
-    if (p->history->n > 0x7fffffff) return set_err(c, DLLM_EINVAL, "pickTokens: history too long");
+    if (p->history->n > 1u << 28) return set_err(c, DLLM_EINVAL, "pickTokens: history too long");
     if (p->prompt_lens)
       if (int rc = check_i32(c, p->prompt_lens, b, "pickTokens prompt lengths")) return rc;
   } else if (p->history_offsets || p->prompt_lens) {
@@ -2456,7 +2456,7 @@ int dllm_pick_tokens(dllm_ctx* c, const dllm_pick* p) {
     if (int rc = check_i32(c, p->bias_tokens, 1, "pickTokens bias tokens")) return rc;
     if (int rc = check_f32(c, p->bias_values, p->bias_tokens->n, "pickTokens bias values")) return rc;
     if (int rc = check_i32(c, p->bias_offsets, b + 1, "pickTokens bias offsets")) return rc;
-    if (p->bias_tokens->n > 0x7fffffff) return set_err(c, DLLM_EINVAL, "pickTokens: too many biases");
+    if (p->bias_tokens->n > 1u << 28) return set_err(c, DLLM_EINVAL, "pickTokens: too many biases");
   } else if (p->bias_values || p->bias_offsets) {
     return set_err(c, DLLM_EINVAL, "pickTokens: bias values or offsets without their tokens");
   }

@@ -16,19 +16,22 @@
 // sequence, that is one row, or all nodes of a tree, which share their history. The
 // slice is every K-th chunk of 128 tokens, not a contiguous range: text uses low token
 // ids far more often, and the CTA with the first tokens would hold half the history.
-// First the CTA counts the history's tokens that fall into its slice in shared memory
-// (integer atomics, so their order does not matter) and flags the tokens that any rule
-// touches, one bit each. From then on nothing is written that another warp reads: a warp
-// takes a row (or a part of one) through the slice's chunks, 4 tokens per lane. The
-// flagged tokens of a group are worked off one per lane and round, which keeps the
-// divisions to about two rounds where one token in ten is flagged instead of four. A
-// drafted token has the set of nodes that carry it, and its count for a node is the
-// size of that set among the node's ancestors. The slices' best (value, index) keys meet
-// in one 64-bit atomicMax per row (the largest key wins in any order); the CTA that
-// arrives last writes the tokens and clears the keys.
+// First the history's tokens are counted, every slice's in its CTA's shared memory:
+// the CTAs of a cluster share the reading and count into one another's memory (integer
+// atomics, so their order does not matter). From then on nothing is written that
+// another warp reads: a warp takes a row (or a part of one) through the slice's chunks,
+// 4 tokens per lane, and applies the rules where a count word says so. A drafted token
+// has the set of nodes that carry it, and its count for a node is the size of that set
+// among the node's ancestors. The slices' best (value, index) keys meet in one 64-bit
+// atomicMax per row (the largest key wins in any order); the CTA that arrives last
+// writes the tokens and clears the keys.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "verify.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace dllm {
 namespace {
@@ -39,31 +42,28 @@ constexpr int kChunk = 128;       // tokens one warp covers at a time, 4 per lan
 constexpr int kMaxChunks = 64;    // chunks per slice
 // Chunk c of a row has its tokens [128 c - shift, 128 c - shift + 128): a row whose
 // address is `shift` elements past a 16-byte boundary starts that much early. So a
-// chunk's words hold its 128 tokens behind a lead of 32, whose last 3 are the tokens
-// before it (they are counted in two chunks); with a lead of 32 the flags of a lane's
-// group lie in one word when shift is 0.
-constexpr int kLead = 32;
+// chunk's words hold its 128 tokens behind the 4 before them, the last 3 of which are
+// counted in two chunks.
+constexpr int kLead = 4;
 constexpr int kStride = kChunk + kLead;
-constexpr int kMaxFlags = kMaxChunks * kStride / 32;
+constexpr int kCluster = 8;       // CTAs that share the reading of a history
 constexpr int kBatch = 4;         // chunks whose loads are in flight together
 
 constexpr uint32_t kGiven = 0x80000000u;    // the token occurs among the given (prompt) tokens
 constexpr uint32_t kDrafted = 0x40000000u;  // the token is drafted somewhere in the tree
+constexpr uint32_t kBiased = 0x20000000u;   // the token has a bias
 
 struct RowRules {
   float rep, freq, pres;
   const float* bias_val;  // the sequence's bias entries
 };
 
-// The rules above for one token. cnt: its count word; b: 1 + its entry in the bias
-// list, or 0.
-DLLM_DEV float apply(float x, uint32_t cnt, uint32_t b, const RowRules& r) {
-  if (cnt) {
-    x = x > 0.f ? __fdiv_rn(x, r.rep) : __fmul_rn(x, r.rep);
-    const uint32_t c = cnt & ~kGiven;
-    if (c) x = __fsub_rn(__fsub_rn(x, __fmul_rn(r.freq, (float)c)), r.pres);
-  }
-  if (b) x = __fadd_rn(x, r.bias_val[b - 1]);
+// The rules above for one token. cnt: its count word without kDrafted.
+DLLM_DEV float apply(float x, uint32_t cnt, const uint32_t* bia, const RowRules& r) {
+  const uint32_t c = cnt & ~(kGiven | kBiased);
+  if (cnt & ~kBiased) x = x > 0.f ? __fdiv_rn(x, r.rep) : __fmul_rn(x, r.rep);
+  if (c) x = __fsub_rn(__fsub_rn(x, __fmul_rn(r.freq, (float)c)), r.pres);
+  if (cnt & kBiased) x = __fadd_rn(x, r.bias_val[*bia - 1]);
   return x;
 }
 
@@ -120,20 +120,38 @@ DLLM_DEV void store_group(float* y, const Group& g, int t, int vocab) {
 struct PickShared {
   unsigned long long key[kTreeMaxNodes];
   unsigned long long nodes[2 * kTreeMaxNodes];  // per entry of drafted: the nodes with that token
-  uint32_t flag[kMaxFlags + 1];                 // bit w: a rule touches the token of word w
   int32_t draft[kTreeMaxNodes];
   uint16_t drafted[2 * kTreeMaxNodes];          // words of drafted tokens
   int n_drafted;
   bool last;
 };
 
+// The four count words of a lane's group, which starts `sh` words before an aligned place:
+// two aligned reads cover them.
+template <bool ALIGNED>
+DLLM_DEV void four_words(uint32_t (&r)[4], const uint32_t* p, int sh) {
+  const uint4 hi = *reinterpret_cast<const uint4*>(p);
+  r[0] = hi.x, r[1] = hi.y, r[2] = hi.z, r[3] = hi.w;
+  if (ALIGNED || sh == 0) return;
+  const uint4 lo = *reinterpret_cast<const uint4*>(p - 4);
+  if (sh == 1)
+    r[3] = hi.z, r[2] = hi.y, r[1] = hi.x, r[0] = lo.w;
+  else if (sh == 2)
+    r[3] = hi.y, r[2] = hi.x, r[1] = lo.w, r[0] = lo.z;
+  else
+    r[3] = hi.x, r[2] = lo.w, r[1] = lo.z, r[0] = lo.y;
+}
+
 // Grid (K slices, sequences), K = 1 << log2k: slice s has the chunks c with c % K = s,
-// n_chunks of them at most. ALIGNED: the vocabulary is a multiple of 4, so every row is.
+// n_chunks of them at most. Clusters of neighbouring slices. ALIGNED: the vocabulary is a
+// multiple of 4, so every row starts at a 16-byte boundary.
 template <bool ALIGNED>
 __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a, int log2k, int n_chunks) {
   extern __shared__ __align__(16) uint32_t dyn[];  // counts, bias entries of the slice's words
   __shared__ PickShared sm;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  cg::cluster_group cluster = cg::this_cluster();
+  const unsigned csize = cluster.num_blocks(), crank = cluster.block_rank();
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int slice = blockIdx.x, s = blockIdx.y;
   const int m = a.seqs ? a.seqs[s].m : 1;
   const int row0 = a.seqs ? a.seqs[s].row0 : s;
@@ -146,16 +164,12 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a,
   // warps: `parts` of them share a row, n_rows rows are under way at once
   const int parts = m < kPickWarps ? kPickWarps / m : 1, n_rows = kPickWarps / parts;
   const int part = warp % parts, first_row = warp / parts;
-  // asks L2 for this warp's part of a row while something else is done
-  auto fetch = [&](int q) {
-    if (q >= m || first_row >= n_rows) return;
-    const float* x = a.logits + (size_t)(row0 + q) * a.vocab;
-    for (int lc = part; lc < n_chunks; lc += parts) {
+  // the first logits are on their way while the history is counted
+  if (first_row < min(n_rows, m))
+    for (int lc = part; lc < min(n_chunks, part + kBatch * parts); lc += parts) {
       const int t = token_of(lc);
-      if (t < a.vocab) asm volatile("prefetch.global.L2 [%0];" ::"l"(x + t));
+      if (t < a.vocab) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.logits + (size_t)(row0 + first_row) * a.vocab + t));
     }
-  };
-  fetch(first_row);
 
   const bool counting = a.penalties != nullptr, biasing = a.bias_tok != nullptr, ruled = counting || biasing;
   const bool pathed = counting && a.seqs;
@@ -168,15 +182,19 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a,
     for (int i = tid; i < 2 * n_words / 4; i += kPickThreads) reinterpret_cast<uint4*>(dyn)[i] = make_uint4(0, 0, 0, 0);
     if (pathed && tid < m) sm.draft[tid] = a.draft[row0 + tid];
   }
-  __syncthreads();
-  // calls f(word) for the words of a token within the slice: its own, and the one of the
-  // next chunk if rows can start early enough to have it there
-  auto words_of = [&](int tok, auto f) {
-    const unsigned c = (unsigned)tok / kChunk, in = tok & (kChunk - 1);
-    if (((c ^ slice) & kmask) == 0 && (unsigned)tok < (unsigned)a.vocab) f((c >> log2k) * kStride + kLead + in);
-    if (!ALIGNED && in >= kChunk - 3 && (((c + 1) ^ slice) & kmask) == 0 && (unsigned)tok < (unsigned)a.vocab &&
+  if (csize > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  // calls f(slice, word) for the words of a token within the `span` slices from `from` (a
+  // multiple of the power of two `span`): its own, and the one of the next chunk if rows
+  // can start early enough to have it there
+  auto words_of = [&](int tok, unsigned from, unsigned span, auto f) {
+    const unsigned c = (unsigned)tok / kChunk, in = tok & (kChunk - 1), near = kmask & ~(span - 1);
+    if (((c ^ from) & near) == 0 && (unsigned)tok < (unsigned)a.vocab) f(c & kmask, (int)((c >> log2k) * kStride + kLead + in));
+    if (!ALIGNED && in >= kChunk - 3 && (((c + 1) ^ from) & near) == 0 && (unsigned)tok < (unsigned)a.vocab &&
         (c + 1) >> log2k < (unsigned)n_chunks)
-      f(((c + 1) >> log2k) * kStride + kLead + in - kChunk);
+      f((c + 1) & kmask, (int)(((c + 1) >> log2k) * kStride + kLead + in - kChunk));
   };
   if (counting) {
     r.rep = a.penalties[3 * s], r.freq = a.penalties[3 * s + 1], r.pres = a.penalties[3 * s + 2];
@@ -184,29 +202,28 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a,
       const int h0 = clampi(a.hist_off[s], 0, a.hist_total), h1 = clampi(a.hist_off[s + 1], h0, a.hist_total);
       const int given = h0 + (a.prompt ? clampi(a.prompt[s], 0, h1 - h0) : 0);
       auto see = [&](int i, int tok) {
-        words_of(tok, [&](int w) {
+        words_of(tok, slice & ~(csize - 1), csize, [&](unsigned sl, int w) {
+          uint32_t* to = csize > 1 ? cluster.map_shared_rank(cnt, sl & (csize - 1)) : cnt;
           if (i < given)
-            atomicOr(cnt + w, kGiven);
+            atomicOr(to + w, kGiven);
           else
-            atomicAdd(cnt + w, 1u);
+            atomicAdd(to + w, 1u);
         });
       };
-      // Every CTA reads the whole history: each starts at a place of its own, so that they
-      // do not all ask the same L2 slice for the same line (18k cycles for 32000 tokens
-      // in step, 256 CTAs).
-      constexpr int B = 16;  // loads in flight
-      const int span = B * kPickThreads, turns = (h1 - h0 + span - 1) / span;
-      for (int n = 0, turn = turns ? slice % turns : 0; n < turns; ++n, turn = turn + 1 < turns ? turn + 1 : 0) {
-        const int i = h0 + turn * span + tid;
+      constexpr int B = 8;  // loads in flight
+      for (int i = h0 + (int)crank * kPickThreads + tid; i < h1; i += B * (int)csize * kPickThreads) {
         int tok[B];
 #pragma unroll
-        for (int e = 0; e < B; ++e) tok[e] = i + e * kPickThreads < h1 ? __ldg(a.hist + i + e * kPickThreads) : -1;
+        for (int e = 0; e < B; ++e) {
+          const int at = i + e * (int)csize * kPickThreads;
+          tok[e] = at < h1 ? __ldg(a.hist + at) : -1;
+        }
 #pragma unroll
-        for (int e = 0; e < B; ++e) see(i + e * kPickThreads, tok[e]);
+        for (int e = 0; e < B; ++e) see(i + e * (int)csize * kPickThreads, tok[e]);
       }
     }
     if (pathed && tid < m)
-      words_of(sm.draft[tid], [&](int w) {
+      words_of(sm.draft[tid], slice, 1, [&](unsigned, int w) {
         if (!(atomicOr(cnt + w, kDrafted) & kDrafted)) sm.drafted[atomicAdd(&sm.n_drafted, 1)] = (uint16_t)w;
       });
   }
@@ -214,15 +231,16 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a,
     const int b0 = clampi(a.bias_off[s], 0, a.bias_total), b1 = clampi(a.bias_off[s + 1], b0, a.bias_total);
     r.bias_val = a.bias_val + b0;
     for (int i = b0 + tid; i < b1; i += kPickThreads)
-      words_of(a.bias_tok[i], [&](int w) { atomicMax(bia + w, (uint32_t)(i - b0 + 1)); });  // the last entry counts
+      words_of(a.bias_tok[i], slice, 1, [&](unsigned, int w) {
+        atomicOr(cnt + w, kBiased);
+        atomicMax(bia + w, (uint32_t)(i - b0 + 1));  // of a token listed twice the last entry counts
+      });
   }
   if (ruled) {
-    __syncthreads();
-    for (int w = tid; w < n_words; w += kPickThreads) {  // whole warps: n_words is a multiple of 32
-      const uint32_t any = __ballot_sync(0xffffffffu, cnt[w] | bia[w]);
-      if (lane == 0) sm.flag[w >> 5] = any;
-    }
-    if (tid == 0) sm.flag[n_words / 32] = 0u;
+    if (csize > 1)
+      cluster.sync();
+    else
+      __syncthreads();
     if (tid < sm.n_drafted) {
       const int w = sm.drafted[tid], lc = w / kStride;
       const int tok = ((lc << log2k) + slice) * kChunk + (w - lc * kStride) - kLead;
@@ -230,7 +248,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a,
       for (int j = 0; j < m; ++j) nodes |= (unsigned long long)(sm.draft[j] == tok) << j;
       sm.nodes[tid] = nodes;
     }
-    __syncthreads();
+    if (pathed) __syncthreads();
   }
 
 #pragma unroll 1
@@ -240,7 +258,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a,
     float* y = a.out ? a.out + (size_t)row * a.vocab : nullptr;
     const uint32_t* mask = a.mask ? a.mask + (size_t)row * mask_words : nullptr;
     const unsigned long long anc = pathed ? a.anc[row] : 0ull;
-    float bv = -INFINITY;  // best of this lane: the first allowed token, then whatever is greater
+    float bv = -INFINITY;  // the greatest allowed logit of this lane, and its first token
     int bt = -1;
 #pragma unroll 1
     for (int lc0 = part; lc0 < n_chunks; lc0 += kBatch * parts) {
@@ -257,45 +275,43 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a,
         Group& g = grp[u];
         if (ruled) {
           const int w = lc * kStride + kLead - sh + 4 * lane;
-          uint32_t touched = sm.flag[w >> 5] >> (w & 31);
-          if (!ALIGNED) touched = __funnelshift_r(sm.flag[w >> 5], sm.flag[(w >> 5) + 1], w & 31);
-          touched &= g.bits;
-          while (touched) {  // one token per lane and round
-            const int e = __ffs(touched) - 1;
-            touched &= touched - 1;
-            uint32_t c = cnt[w + e];
-            if (c & kDrafted) {
+          uint32_t c[4];
+          four_words<ALIGNED>(c, cnt + w + sh, sh);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (!(g.bits >> e & 1)) c[e] = 0;
+            if (c[e] & kDrafted) {
               int d = 0;
               while (sm.drafted[d] != w + e) ++d;
-              c = (c & ~kDrafted) + (uint32_t)__popcll(anc & sm.nodes[d]);
+              c[e] = (c[e] & ~kDrafted) + (uint32_t)__popcll(anc & sm.nodes[d]);
             }
-            const float old = e == 0 ? g.v[0] : e == 1 ? g.v[1] : e == 2 ? g.v[2] : g.v[3];
-            const float z = apply(old, c, bia[w + e], r);
-            g.v[0] = e == 0 ? z : g.v[0];
-            g.v[1] = e == 1 ? z : g.v[1];
-            g.v[2] = e == 2 ? z : g.v[2];
-            g.v[3] = e == 3 ? z : g.v[3];
+            if (c[e]) g.v[e] = apply(g.v[e], c[e], bia + w + e, r);
           }
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (!(g.bits >> e & 1)) g.v[e] = -INFINITY;
         if (y) store_group<ALIGNED>(y, g, t, a.vocab);
-        const float most = fmaxf(fmaxf(g.v[0], g.v[1]), fmaxf(g.v[2], g.v[3]));  // NaN counts as -inf
-        if (most > bv || (bt < 0 && g.bits)) {
-#pragma unroll
-          for (int e = 3; e >= 0; --e)
-            if ((g.bits >> e & 1) && (g.v[e] == most || !(most > -INFINITY))) bt = t + e;
-          bv = most == most ? most : -INFINITY;
+        const float most = fmaxf(fmaxf(g.v[0], g.v[1]), fmaxf(g.v[2], g.v[3]));  // passes over NaN
+        if (most > bv) {
+          bv = most;
+          bt = t + (g.v[0] == most ? 0 : g.v[1] == most ? 1 : g.v[2] == most ? 2 : 3);
         }
       }
     }
-    unsigned long long key = bt < 0 ? 0ull : argmax_key(bv, bt);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
-      if (other > key) key = other;
+    // a lane without a logit above -inf (or only NaN): its first allowed token counts as -inf
+    if (bt < 0) {
+      for (int lc = part; lc < n_chunks && bt < 0; lc += parts) {
+        const int t = token_of(lc) - sh;
+        for (int e = 3; e >= 0; --e)
+          if (t + e >= 0 && t + e < a.vocab && (!mask || (mask[(t + e) >> 5] >> ((t + e) & 31) & 1))) bt = t + e;
+      }
     }
+    // the warp's best: the greatest value, then the lowest token (-0 + 0 = +0: zeros tie)
+    const uint32_t bits = __float_as_uint(__fadd_rn(bv, 0.f)), ord = bt < 0 ? 0u : (bits & 0x80000000u) ? ~bits : bits | 0x80000000u;
+    const uint32_t top = __reduce_max_sync(0xffffffffu, ord);
+    const uint32_t tok = __reduce_min_sync(0xffffffffu, ord == top && bt >= 0 ? (uint32_t)bt : 0xffffffffu);
+    const unsigned long long key = top ? ((unsigned long long)top << 32) | ~tok : 0ull;
     if (lane == 0 && key) atomicMax(&sm.key[q], key);
   }
   __syncthreads();
@@ -326,20 +342,28 @@ cudaError_t configure_pick_kernels() {
 
 cudaError_t op_pick(const PickArgs& a, int sms, cudaStream_t st) {
   // The fewest slices that fit a CTA (64 chunks), then twice as many as long as all CTAs
-  // still run at once, two per SM, and a slice keeps at least 4 chunks. A row that starts 3
-  // tokens early reaches vocab + 3.
+  // still run at once, two per SM, and a slice keeps at least 4 chunks and one for every
+  // warp. A row that starts 3 tokens early reaches vocab + 3.
   const long long chunks = ((long long)a.vocab + 3 + kChunk - 1) / kChunk;
   int log2k = 0;
   while ((chunks + (1ll << log2k) - 1) >> log2k > kMaxChunks) ++log2k;
-  while ((2ll << log2k) * a.n_seqs <= 2ll * sms && chunks >> (log2k + 1) >= 4) ++log2k;
+  while ((2ll << log2k) * a.n_seqs <= 2ll * sms && chunks >> (log2k + 1) >= 4 &&
+         (chunks >> (log2k + 1)) * a.max_m >= kPickWarps)
+    ++log2k;
   const int n_chunks = (int)((chunks + (1ll << log2k) - 1) >> log2k);
-  const size_t smem = a.penalties || a.bias_tok ? pick_smem(n_chunks) : 0;
-  const dim3 grid(1u << log2k, a.n_seqs);
-  if (a.vocab % 4 == 0)
-    pick_kernel<true><<<grid, kPickThreads, smem, st>>>(a, log2k, n_chunks);
-  else
-    pick_kernel<false><<<grid, kPickThreads, smem, st>>>(a, log2k, n_chunks);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(1u << log2k, a.n_seqs);
+  cfg.blockDim = dim3(kPickThreads);
+  cfg.dynamicSmemBytes = a.penalties || a.bias_tok ? pick_smem(n_chunks) : 0;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = a.hist ? std::min(kCluster, 1 << log2k) : 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, a.vocab % 4 == 0 ? pick_kernel<true> : pick_kernel<false>, a, log2k, n_chunks);
 }
 
 }  // namespace dllm

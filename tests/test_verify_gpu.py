@@ -548,6 +548,9 @@ def test_pick_ties_nan_and_infinities(dllm):
     x[5, 11], x[5, 1002] = 2.0, 2.0
     x[6, :200], x[6, 200:] = np.nan, -7.0
     x[7, :-1] = np.nan
+    z = np.full((2, v), -1.0, np.float32)  # zeros of both signs tie
+    z[0, 700], z[0, 5], z[1, 130], z[1, 131] = 0.0, -0.0, -0.0, 0.0
+    run_pick(ctx, z, range(2))
     run_pick(ctx, x, range(8))
     allowed = np.ones((8, v), bool)
     allowed[:, :13] = False
