@@ -97,14 +97,14 @@ __global__ void __launch_bounds__(kTAThreads, 1) tree_attn_kernel(const __grid_c
   extern __shared__ __align__(1024) unsigned char smem[];
   const TreeAttnArgs& a = P.a;
   asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled; it waits for this grid's end
-  const TreeSeq sq = ta_seq(P, blockIdx.z);
-  const int G = a.nq / a.kvh;
-  const int head = blockIdx.y % a.kvh, tile = blockIdx.y / a.kvh;
-  const int R = sq.m * G, r0 = tile * RT;
-  const int T0 = P.t0[blockIdx.z], slots = T0 + sq.m;
-  const int nsplit = ta_splits(slots, BN, P.bps);
-  const int split = blockIdx.x;
-  if (r0 >= R || split >= nsplit) return;
+  TATile k;
+  k.sq = ta_seq(P, blockIdx.z);
+  k.set_group(a.nq / a.kvh);
+  const int head = k.head = blockIdx.y % a.kvh, r0 = k.r0 = blockIdx.y / a.kvh * RT, R = k.R = k.sq.m * k.G;
+  const int T0 = P.t0[blockIdx.z], slots = T0 + k.sq.m, split = k.split = blockIdx.x;
+  k.nsplit = ta_splits(slots, BN, P.bps);
+  if (r0 >= R || split >= k.nsplit) return;
+  const TreeSeq& sq = k.sq;
   const int nblk = (slots + BN - 1) / BN;
   const int blk0 = split * P.bps, blk1 = min(nblk, blk0 + P.bps);
 
@@ -161,8 +161,8 @@ __global__ void __launch_bounds__(kTAThreads, 1) tree_attn_kernel(const __grid_c
     const int r = r0 + row;
     float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
     if (r < R) {
-      const int node = r / G;
-      f = *reinterpret_cast<const float4*>(a.q + ((size_t)(sq.row0 + node) * a.nq + head * G + (r - node * G)) * HD + d);
+      const int node = k.node_of(r);
+      f = *reinterpret_cast<const float4*>(a.q + ((size_t)(sq.row0 + node) * a.nq + head * k.G + (r - node * k.G)) * HD + d);
       f.x *= a.scale_log2, f.y *= a.scale_log2, f.z *= a.scale_log2, f.w *= a.scale_log2;
     }
     if constexpr (F32) {
@@ -180,8 +180,8 @@ __global__ void __launch_bounds__(kTAThreads, 1) tree_attn_kernel(const __grid_c
 
   // this thread's two rows of the tile and their ancestor masks
   const int ra = wr * 16 + g, rb = ra + 8;
-  const unsigned long long anc_a = r0 + ra < R ? a.anc[sq.row0 + (r0 + ra) / G] : 0ull;
-  const unsigned long long anc_b = r0 + rb < R ? a.anc[sq.row0 + (r0 + rb) / G] : 0ull;
+  const unsigned long long anc_a = r0 + ra < R ? a.anc[sq.row0 + k.node_of(r0 + ra)] : 0ull;
+  const unsigned long long anc_b = r0 + rb < R ? a.anc[sq.row0 + k.node_of(r0 + rb)] : 0ull;
 
   float o[HD / 8][4];
 #pragma unroll
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(kTAThreads, 1) tree_attn_kernel(const __grid_c
     sML[(ws * RT + rb) * 2] = mb, sML[(ws * RT + rb) * 2 + 1] = lb;
   }
   __syncthreads();
-  ta_finish<HD, WS, RT>(P, TATile{sq, G, head, r0, R, nsplit, split}, sO, sML, tid, kTAThreads);
+  ta_finish<HD, WS, RT, kTAThreads>(P, k, sO, sML, tid);
 }
 
 // Joins the splits of a sequence. W warps share one (row, query head): warp w folds the

@@ -53,18 +53,22 @@ DLLM_DEV bool is_finite(float v) { return fabsf(v) <= 3.402823466e38f; }
 // One row tile of a CTA: rows [r0, r0 + RT) of the m G rows that share a KV head.
 struct TATile {
   TreeSeq sq;
-  int G, head, r0, R, nsplit, split;
+  int G, inv_g, head, r0, R, nsplit, split;
+  DLLM_DEV void set_group(int g) { G = g, inv_g = (65536 + g - 1) / g; }
+  // row / G for rows below 2^13 (there are at most 64 nodes x 8 heads)
+  DLLM_DEV int node_of(int r) const { return r * inv_g >> 16; }
 };
 
 // The results of WS slot groups, each with RT rows of [HD + 4] outputs in sO and (max,
-// sum) in sML, to `out`, or to this split's partials.
-template <int HD, int WS, int RT>
-DLLM_DEV void ta_finish(const TAKernelArgs& P, const TATile& k, const float* sO, const float* sML, int tid, int threads) {
+// sum) in sML, to `out`, or to this split's partials. HD / 4 threads per row.
+template <int HD, int WS, int RT, int THREADS>
+DLLM_DEV void ta_finish(const TAKernelArgs& P, const TATile& k, const float* sO, const float* sML, int tid) {
   const TreeAttnArgs& a = P.a;
-  for (int i = tid; i < RT * HD / 4; i += threads) {
-    const int row = i / (HD / 4), d = (i % (HD / 4)) * 4;
-    const int r = k.r0 + row;
-    if (r >= k.R) continue;
+  constexpr int kLanes = HD / 4, kStep = THREADS / kLanes;
+  const int d = (tid % kLanes) * 4, rows = min(RT, k.R - k.r0);
+  const size_t split_base = (size_t)P.part0[blockIdx.z] + (size_t)k.split * k.sq.m * a.nq;
+#pragma unroll 4
+  for (int row = tid / kLanes; row < rows; row += kStep) {
     float m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int w = 0; w < WS; ++w) m = fmaxf(m, sML[(w * RT + row) * 2]);
@@ -77,15 +81,14 @@ DLLM_DEV void ta_finish(const TAKernelArgs& P, const TATile& k, const float* sO,
       f.x = fmaf(v.x, e, f.x), f.y = fmaf(v.y, e, f.y), f.z = fmaf(v.z, e, f.z), f.w = fmaf(v.w, e, f.w);
       l = fmaf(sML[(w * RT + row) * 2 + 1], e, l);
     }
-    const int node = r / k.G, hq = k.head * k.G + (r - node * k.G);
+    const int r = k.r0 + row, node = k.node_of(r), at = node * a.nq + k.head * k.G + (r - node * k.G);
     if (k.nsplit == 1) {
       const float inv = 1.0f / l;
-      *reinterpret_cast<float4*>(a.out + ((size_t)(k.sq.row0 + node) * a.nq + hq) * HD + d) =
+      *reinterpret_cast<float4*>(a.out + ((size_t)k.sq.row0 * a.nq + at) * HD + d) =
           make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
     } else {
-      const size_t at = (size_t)P.part0[blockIdx.z] + ((size_t)k.split * k.sq.m + node) * a.nq + hq;
-      *reinterpret_cast<float4*>(a.part_o + at * HD + d) = f;
-      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
+      *reinterpret_cast<float4*>(a.part_o + (split_base + at) * HD + d) = f;
+      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (split_base + at) * 2) = make_float2(m, l);
     }
   }
 }

@@ -6,21 +6,29 @@
 // that only the last pass adds at full size (the tensor core truncates each addition);
 // a block's p . V starts from zero and is added to the running output in registers.
 //
-// One CTA, three warpgroups, one 128-row tile over its share of the 64-slot blocks:
-//   producer (1 thread)  TMA: K and V boxes of a block (128-byte swizzle) into rings
-//   MMA (1 thread)       S(n + 1) = q K^T of the next block, then O(n) = P(n) V
-//   two helper warps     the blocks that hold drafted rows: rows behind the last node are
+// One CTA, three warpgroups, one 128-row tile over its share of the 64-slot blocks, which
+// it takes in pairs:
+//   producer (1 warp)    TMA: K of a pair, V of a block (128-byte swizzle) into rings
+//   MMA (1 warp)         S = q K^T of a pair (128 slots at once), O = P V of a block by halves
+//                        of 64 dims
+//   helper (1 warp)      the blocks that hold drafted rows: rows behind the last node are
 //                        zeroed and non-finite values taken out before the MMA reads V
-//   two softmax groups   128 threads, one row each; group w takes the blocks n % 2 = w
-//                        with a maximum, sum and output of its own: S from tensor memory,
-//                        online softmax, P back as three bf16 planes (the MMA's A operand
-//                        is read from tensor memory), then O(n) into its registers
-// so that the tensor core works on one block while the groups are in the softmax of the
-// two around it. The groups' results are joined like two splits.
-// Tensor memory (512 columns): S 2 x 64, P 2 x 96, O 128. V is read as it lies, slots x
-// dims: a descriptor with the dims as the contiguous ("MN") direction.
-// Bound: 6 x 2^20 multiply-adds per block at 4096 per cycle, 1536 cycles, against 64 slots x
-// 512 bytes from HBM at one SM's share of 44 GB/s, 0.74 us.
+//   two softmax groups   128 threads, one row each; group w takes the pair's block w with a
+//                        maximum, sum and output of its own: S from tensor memory, online
+//                        softmax, P back as three bf16 planes (the MMA's A operand is read
+//                        from tensor memory), then O into its registers
+// The groups' results are joined like two splits. Tensor memory (512 columns): S of two pairs
+// 2 x 128, P 2 x 96, O 64. The MMA warp runs the scores two pairs ahead, a quarter of a pair
+// after each half of O, so that O is read while the scores keep the tensor core busy and
+// the softmax of a block has a whole pair's time. V is read as it lies, slots x dims: a
+// descriptor with the dims as the contiguous ("MN") direction.
+// Bound: per pair 24 MMAs of 128 x 128 x 16 from shared memory (65 cycles) and 48 of 128 x 64
+// x 16 with A in tensor memory (33): 3150 cycles, 0.82 us per block of 64 slots, against 0.74
+// us for its 64 x 512 bytes at one SM's share of HBM. Measured 2150 cycles per block (64 nodes
+// x 7 heads at 32000 slots): the scores' MMAs read 126 of the 128 bytes that shared memory
+// gives per cycle, so every barrier and every tensor-memory store of the softmax waits behind
+// them, and a group's chain of softmax, P, O becomes the limit. (Scores block by block, 24
+// MMAs of N = 64, and O whole: 2565 cycles; a second issuing warp for O: 2240.)
 #include "tc.cuh"
 #include "tree_attn.cuh"
 
@@ -28,56 +36,40 @@ namespace dllm {
 namespace {
 
 constexpr int kTcAttnThreads = 384;
-constexpr int kStages = 3;
+constexpr int kKStages = 2;    // pairs
+constexpr int kVStages = 4;    // blocks
+constexpr int kPair = 2 * kTcBlock;
 constexpr int kErrWait = 5;  // the tensor-core wait code
 
 DLLM_DEV void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// A wait that ends early once another wait of the CTA has given up.
-DLLM_DEV bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort, int* err) {
-  const uint32_t a = smem_u32(bar);
-  const long long t0 = clock64();
-  for (;;) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(a), "r"(parity)
-        : "memory");
-    if (done) return true;
-    if (*abort) return false;
-    if (clock64() - t0 > kTcWaitCycles) {
-      *abort = 1;
-      atomicExch(err, kErrWait);
-      return false;
-    }
-  }
-}
-
-// The same for a whole warp that stays together; the result is the same in every lane.
-DLLM_DEV bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* err) {
-  const uint32_t a = smem_u32(bar);
-  const long long t0 = clock64();
-  for (;;) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(a), "r"(parity)
-        : "memory");
-    if (__all_sync(0xffffffffu, done)) return true;
-    if (__any_sync(0xffffffffu, *abort)) return false;
-    if (__any_sync(0xffffffffu, clock64() - t0 > kTcWaitCycles)) {
-      *abort = 1;
-      atomicExch(err, kErrWait);
-      return false;
-    }
-  }
+// Waits for a phase, at most about 2 s (200000 tries of up to 10 us each), and less once
+// another wait of the CTA has given up: then it returns false at once, and the CTA runs on
+// through its loops without waiting, computes nothing of use, reports the error and ends.
+// One asm block, so that the compiler sees no branch: a warp that issues MMAs has to stay
+// one piece (a loop with votes cost 200 cycles even where the phase had completed).
+DLLM_DEV bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n, gone;\n\t"
+      "mov.u32 n, 0;\n\t"
+      "mov.u32 %0, 1;\n\t"
+      "TRY:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 10000;\n\t"
+      "@p bra DONE;\n\t"
+      "ld.volatile.shared.u32 gone, [%3];\n\t"
+      "add.u32 n, n, 1;\n\t"
+      "setp.ne.u32 q, gone, 0;\n\t"
+      "setp.gt.or.u32 q, n, 200000, q;\n\t"
+      "@!q bra TRY;\n\t"
+      "mov.u32 %0, 0;\n\t"
+      "st.volatile.shared.u32 [%3], 1;\n\t"
+      "DONE:\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(smem_u32(const_cast<const int*>(abort)))
+      : "memory");
+  return ok;
 }
 DLLM_DEV uint32_t elect_one() {
   uint32_t r;
@@ -93,12 +85,12 @@ DLLM_DEV void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uin
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
       "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate));
 }
-// Shared-memory descriptor of a tile whose contiguous direction is the MMA's N (dims): rows
-// of 64 dims (128 bytes, swizzled), one per K index (slot); 8-slot groups 1024 bytes
-// apart (stride offset), 64-dim boxes `box` bytes apart (leading offset).
-DLLM_DEV uint64_t umma_desc_mn_sw128(const void* tile, uint32_t box) {
+// Shared-memory descriptor of a 16 x 64 operand whose contiguous direction is the MMA's N
+// (dims): rows of 64 dims (128 bytes, swizzled), one per K index (slot), 8-slot groups 1024
+// bytes apart (stride offset; one 64-dim box, so the leading offset is not used).
+DLLM_DEV uint64_t umma_desc_mn_sw128(const void* tile) {
   const uint64_t a = smem_u32(tile);
-  return ((a & 0x3FFFFull) >> 4) | ((uint64_t)(box >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+  return ((a & 0x3FFFFull) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 
 #define R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
@@ -123,20 +115,25 @@ template <int HD>
 struct TcTile {
   static constexpr int BOX = HD / 64;                      // 64-dim boxes
   static constexpr int kQPlane = BOX * kTcRows * 128;      // bytes of one bf16 term of q
-  static constexpr int kBox = kTcBlock * 128;              // bytes of a 64 x 64 box
-  static constexpr int kKV = BOX * kBox;                   // bytes of a K or V block
-  static constexpr int kRing = 2 * kStages * kKV;
-  static constexpr int kOut = 2 * kTcRows * (HD + 6) * 4;  // both groups' results, over q and ring
+  static constexpr int kKBox = kPair * 128;                // bytes of 128 slots x 64 dims
+  static constexpr int kVBox = kTcBlock * 128;             // bytes of 64 slots x 64 dims
+  static constexpr int kK = BOX * kKBox, kV = BOX * kVBox; // bytes of a pair's K, a block's V
+  static constexpr int kRing = kKStages * kK + kVStages * kV;
+  static constexpr int kOut = 2 * kTcRows * (HD + 6) * 4;  // both groups' results, over q and rings
   static constexpr int kSmem = 1024 + 3 * kQPlane + kRing;
   static_assert(kOut <= 3 * kQPlane + kRing, "results reuse the operands' memory");
-  static_assert(kSmem <= 227 * 1024, "shared memory");
-  static constexpr uint32_t kP = 128, kO = 320;            // tensor-memory columns: S 0, 64; P; O
+  static_assert(kSmem + 512 <= 227 * 1024, "shared memory");
+  static constexpr int kQMma = 3 * BOX * 4;                // MMAs of a pair's scores
+  static constexpr int kSteps = 2 * BOX;                   // halves of O per pair
+  static constexpr uint32_t kP = 256, kO = 448;            // tensor-memory columns: S 0, 128; P; O
 };
 
 struct TcShared {
-  uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-  uint64_t s_full[2], p_ready[2], o_full[2], o_free[2];  // per softmax group
-  uint64_t v_ok[2];                                      // the (at most two) blocks with drafted rows
+  uint64_t k_full[kKStages], k_empty[kKStages], v_full[kVStages], v_empty[kVStages];
+  uint64_t s_full[2], s_free[2];               // per S buffer
+  uint64_t p_ready[2], o_full[2], o_free[2];   // per softmax group
+  uint64_t v_ok[2];                            // the (at most two) blocks with drafted rows
+  uint64_t idle;                               // every MMA has completed
   uint32_t tmem;
   int bad[2];
   volatile int abort;
@@ -153,7 +150,7 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
   asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled; it waits for this grid's end
   TATile k;
   k.sq = ta_seq(P, blockIdx.z);
-  k.G = a.nq / a.kvh;
+  k.set_group(a.nq / a.kvh);
   k.head = blockIdx.y % a.kvh;
   k.r0 = (blockIdx.y / a.kvh) * kTcRows;
   k.R = k.sq.m * k.G;
@@ -163,6 +160,7 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
   if (k.r0 >= k.R || k.split >= k.nsplit) return;
   const int blk0 = k.split * P.bps;
   const int nb = min((slots + kTcBlock - 1) / kTcBlock, blk0 + P.bps) - blk0;
+  const int np = (nb + 1) / 2;              // pairs
   const int draft0 = T0 / kTcBlock - blk0;  // the first block (of this CTA's) with drafted rows
 
   // the warp's number as a value that is the same in all its lanes by construction
@@ -170,147 +168,199 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
   unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* sQ = base;
   unsigned char* sK = base + 3 * T::kQPlane;
-  unsigned char* sV = sK + kStages * T::kKV;
+  unsigned char* sV = sK + kKStages * T::kK;
 
   if (tid == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(&sh.k_full[s], 1), mbar_init(&sh.k_empty[s], 1);
-      mbar_init(&sh.v_full[s], 1), mbar_init(&sh.v_empty[s], 1);
-    }
+    for (int s = 0; s < kKStages; ++s) mbar_init(&sh.k_full[s], 1), mbar_init(&sh.k_empty[s], 1);
+    for (int s = 0; s < kVStages; ++s) mbar_init(&sh.v_full[s], 1), mbar_init(&sh.v_empty[s], 1);
     for (int w = 0; w < 2; ++w) {
-      mbar_init(&sh.s_full[w], 1), mbar_init(&sh.p_ready[w], 128);
-      mbar_init(&sh.o_full[w], 1), mbar_init(&sh.o_free[w], 128);
-      mbar_init(&sh.v_ok[w], 64);
+      mbar_init(&sh.s_full[w], 1), mbar_init(&sh.s_free[w], 256);
+      mbar_init(&sh.p_ready[w], 128), mbar_init(&sh.o_full[w], 1), mbar_init(&sh.o_free[w], 128);
+      mbar_init(&sh.v_ok[w], 32);
       sh.bad[w] = 0;
     }
+    mbar_init(&sh.idle, 1);
     sh.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  // the pool rows of a block's boxes (lane 0 of the producer); boxes behind the end are
+  // loaded again and not used
+  const int page = 1 << a.kv.log2_page, box = page < kTcBlock ? page : kTcBlock;
+  auto pool_row = [&](int n, int b) {
+    const int slot = min((blk0 + n) * kTcBlock + b * box, slots - 1) & ~(box - 1);
+    return a.tc_row0 + (a.kv.page_table[(size_t)k.sq.seq * a.kv.max_pages + (slot >> a.kv.log2_page)] * a.kvh + k.head) * page +
+           (slot & (page - 1));
+  };
   if (warp == 8) {
+    if (lane == 0) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&tmK) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&tmV) : "memory");
+    }
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512u));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  // q, scaled so that the softmax is in powers of two, as three bf16 planes of swizzled
-  // 64-dim boxes (what the K-major descriptor reads)
-  for (int i = tid; i < kTcRows * HD / 8; i += kTcAttnThreads) {
-    const int row = i / (HD / 8), d = (i % (HD / 8)) * 8, r = k.r0 + row;
-    uint4 h = make_uint4(0, 0, 0, 0), m = h, l = h;
-    if (r < k.R) {
-      const int node = r / k.G;
-      const float* q = a.q + ((size_t)(k.sq.row0 + node) * a.nq + k.head * k.G + (r - node * k.G)) * HD + d;
-      const float4 f = *reinterpret_cast<const float4*>(q), g = *reinterpret_cast<const float4*>(q + 4);
-      const float c = a.scale_log2;
-      split3(f.x * c, f.y * c, h.x, m.x, l.x);
-      split3(f.z * c, f.w * c, h.y, m.y, l.y);
-      split3(g.x * c, g.y * c, h.z, m.z, l.z);
-      split3(g.z * c, g.w * c, h.w, m.w, l.w);
-    }
-    unsigned char* at = sQ + (d / 64) * (kTcRows * 128) + row * 128 + ((((d % 64) >> 3) ^ (row & 7)) << 4);
-    *reinterpret_cast<uint4*>(at) = h;
-    *reinterpret_cast<uint4*>(at + T::kQPlane) = m;
-    *reinterpret_cast<uint4*>(at + 2 * T::kQPlane) = l;
-  }
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // q is read by the MMA
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
+  const unsigned long long anc = warp < 8 && k.r0 + (tid & 127) < k.R ? a.anc[k.sq.row0 + k.node_of(k.r0 + (tid & 127))] : 0ull;
+  if (warp != 8) {
+    // q, scaled so that the softmax is in powers of two, as three bf16 planes of swizzled
+    // 64-dim boxes (what the K-major descriptor reads), while the producer's first copies fly.
+    // Rows behind the last one stay as they are: a row of S, P and O comes from its row alone.
+    constexpr int kTasks = kTcRows * HD / 8, kWorkers = kTcAttnThreads - 32;
+    constexpr int kEach = (kTasks + kWorkers - 1) / kWorkers;
+    const int me = warp < 8 ? tid : tid - 32;
+    float4 f[kEach], g[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int i = me + e * kWorkers, row = i / (HD / 8), d = (i % (HD / 8)) * 8, r = k.r0 + row;
+      if (i < kTasks && r < k.R) {
+        const int node = k.node_of(r);
+        const float* q = a.q + ((size_t)(k.sq.row0 + node) * a.nq + k.head * k.G + (r - node * k.G)) * HD + d;
+        f[e] = *reinterpret_cast<const float4*>(q), g[e] = *reinterpret_cast<const float4*>(q + 4);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int i = me + e * kWorkers, row = i / (HD / 8), d = (i % (HD / 8)) * 8;
+      if (i >= kTasks || k.r0 + row >= k.R) break;
+      uint4 h, m, l;
+      const float c = a.scale_log2;
+      split3(f[e].x * c, f[e].y * c, h.x, m.x, l.x);
+      split3(f[e].z * c, f[e].w * c, h.y, m.y, l.y);
+      split3(g[e].x * c, g[e].y * c, h.z, m.z, l.z);
+      split3(g[e].z * c, g[e].w * c, h.w, m.w, l.w);
+      unsigned char* at = sQ + (d / 64) * (kTcRows * 128) + row * 128 + ((((d % 64) >> 3) ^ (row & 7)) << 4);
+      *reinterpret_cast<uint4*>(at) = h;
+      *reinterpret_cast<uint4*>(at + T::kQPlane) = m;
+      *reinterpret_cast<uint4*>(at + 2 * T::kQPlane) = l;
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // q is read by the MMA
+    asm volatile("bar.sync 2, %0;" ::"n"(kWorkers) : "memory");
+  }
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 8 && lane == 0) {
       // ---- producer. The pools are one tensor of rows (layer, page, head, slot); a page holds 32
       // slots (two boxes of a block) or a multiple of 64 (one).
-      const int page = 1 << a.kv.log2_page, box = page < kTcBlock ? page : kTcBlock;
-      const int* table = a.kv.page_table + (size_t)k.sq.seq * a.kv.max_pages;
       int k_sent = 0, v_sent = 0;
-      for (int n = 0; n < nb; ++n) {
-        const int s = n % kStages;
-        const uint32_t ph = (uint32_t)(n / kStages) & 1u;
-        int row[2];
-        for (int b = 0; b < kTcBlock / box; ++b) {
-          const int slot = min((blk0 + n) * kTcBlock + b * box, slots - 1) & ~(box - 1);  // behind the end: loaded again, unused
-          row[b] = a.tc_row0 + (table[slot >> a.kv.log2_page] * a.kvh + k.head) * page + (slot & (page - 1));
+      bool ok = true;  // nothing is loaded over memory that may still be read
+      // K runs a pair ahead of V
+      for (int j = 0; ok && j <= np; ++j) {
+        if (j < np) {
+          const int s = j % kKStages, blocks = min(2, nb - 2 * j);
+          ok = wait_phase(&sh.k_empty[s], ((uint32_t)(j / kKStages) & 1u) ^ 1u, &sh.abort);
+          if (!ok) break;
+          mbar_expect_tx(&sh.k_full[s], blocks * T::kV);
+          for (int h = 0; h < blocks; ++h)
+            for (int b = 0; b < kTcBlock / box; ++b) {
+              const int row = pool_row(2 * j + h, b);
+              for (int x = 0; x < T::BOX; ++x)
+                tma_load_2d(sK + s * T::kK + x * T::kKBox + (h * kTcBlock + b * box) * 128, &tmK, x * 64, row, &sh.k_full[s]);
+            }
+          k_sent = j + 1;
         }
-        if (!wait_or_abort(&sh.k_empty[s], ph ^ 1u, &sh.abort, a.err)) break;
-        mbar_expect_tx(&sh.k_full[s], T::kKV);
-        for (int b = 0; b < kTcBlock / box; ++b)
-          for (int x = 0; x < T::BOX; ++x)
-            tma_load_2d(sK + s * T::kKV + x * T::kBox + b * box * 128, &tmK, x * 64, row[b], &sh.k_full[s]);
-        k_sent = n + 1;
-        if (!wait_or_abort(&sh.v_empty[s], ph ^ 1u, &sh.abort, a.err)) break;
-        mbar_expect_tx(&sh.v_full[s], T::kKV);
-        for (int b = 0; b < kTcBlock / box; ++b)
-          for (int x = 0; x < T::BOX; ++x)
-            tma_load_2d(sV + s * T::kKV + x * T::kBox + b * box * 128, &tmV, x * 64, row[b], &sh.v_full[s]);
-        v_sent = n + 1;
+        for (int n = max(0, 2 * (j - 1)); ok && n < min(nb, 2 * j); ++n) {
+          const int s = n % kVStages;
+          ok = wait_phase(&sh.v_empty[s], ((uint32_t)(n / kVStages) & 1u) ^ 1u, &sh.abort);
+          if (!ok) break;
+          mbar_expect_tx(&sh.v_full[s], T::kV);
+          for (int b = 0; b < kTcBlock / box; ++b) {
+            const int row = pool_row(n, b);
+            for (int x = 0; x < T::BOX; ++x)
+              tma_load_2d(sV + s * T::kV + x * T::kVBox + b * box * 128, &tmV, x * 64, row, &sh.v_full[s]);
+          }
+          v_sent = n + 1;
+        }
       }
       // whatever happened to the others, the copies under way land before the CTA ends
-      for (int j = max(0, k_sent - kStages); j < k_sent; ++j) mbar_wait(&sh.k_full[j % kStages], (uint32_t)(j / kStages) & 1u);
-      for (int j = max(0, v_sent - kStages); j < v_sent; ++j) mbar_wait(&sh.v_full[j % kStages], (uint32_t)(j / kStages) & 1u);
+      for (int j = max(0, k_sent - kKStages); j < k_sent; ++j)
+        mbar_wait(&sh.k_full[j % kKStages], (uint32_t)(j / kKStages) & 1u);
+      for (int j = max(0, v_sent - kVStages); j < v_sent; ++j)
+        mbar_wait(&sh.v_full[j % kVStages], (uint32_t)(j / kVStages) & 1u);
     } else if (warp == 9) {
       // ---- MMA issuer. The whole warp runs the loop and one elected lane issues: the operands
       // of tcgen05.mma live in uniform registers, and in a branch on the lane number
-      // every one of them was first moved there (130 to 230 cycles per MMA; 49 and 65 this way).
+      // every one of them was first moved there (130 to 230 cycles per MMA; 33 to 65 this way).
       const uint32_t leader = elect_one();
       const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kTcRows >> 4) << 24);  // fp32 += bf16 x bf16
-      const uint32_t id_s = idesc | ((uint32_t)(kTcBlock >> 3) << 17);                  // N = 64 slots, K-major
-      const uint32_t id_o = idesc | ((uint32_t)(HD >> 3) << 17) | (1u << 16);           // N = hd, B with N contiguous
-      auto scores = [&](int n) {
-        const int s = n % kStages;
-        if (!warp_wait(&sh.k_full[s], (uint32_t)(n / kStages) & 1u, &sh.abort, a.err)) return false;
-        tc_fence_after();
-        if (leader) {
+      const uint32_t id_s = idesc | ((uint32_t)(kPair >> 3) << 17);            // N = 128 slots, K-major
+      const uint32_t id_o = idesc | ((uint32_t)(64 >> 3) << 17) | (1u << 16);  // N = 64 dims, B with N contiguous
+      // MMAs [from, to) of the scores of pair j, the lowest terms of q first
+      auto scores = [&](int j, int from, int to) {
+        const unsigned char* kb = sK + (j % kKStages) * T::kK;
 #pragma unroll
-          for (int p = 2; p >= 0; --p)
-#pragma unroll
-            for (int x = 0; x < T::BOX; ++x) {
-              const uint64_t ad = umma_desc_sw128(sQ + p * T::kQPlane + x * (kTcRows * 128));
-              const uint64_t bd = umma_desc_sw128(sK + s * T::kKV + x * T::kBox);
-#pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
-                umma_bf16(tmem + (uint32_t)(n & 1) * 64, ad + 2ull * kk, bd + 2ull * kk, id_s, (uint32_t)(p != 2 || x || kk));
-            }
-          umma_commit(&sh.k_empty[s]);
-          umma_commit(&sh.s_full[n & 1]);
+        for (int i = 0; i < T::kQMma; ++i) {
+          if (i < from || i >= to) continue;
+          const int p = 2 - i / (T::BOX * 4), x = i / 4 % T::BOX, kk = i % 4;
+          umma_bf16(tmem + (uint32_t)(j & 1) * kPair, umma_desc_sw128(sQ + p * T::kQPlane + x * (kTcRows * 128)) + 2ull * kk,
+                    umma_desc_sw128(kb + x * T::kKBox) + 2ull * kk, id_s, (uint32_t)(i != 0));
         }
-        __syncwarp();
-        return true;
+        if (to == T::kQMma) {
+          umma_commit(&sh.k_empty[j % kKStages]);
+          umma_commit(&sh.s_full[j & 1]);
+        }
       };
-      bool ok = scores(0);
-      for (int n = 0; ok && n < nb; ++n) {
-        if (n + 1 < nb) ok = scores(n + 1);
-        const int s = n % kStages, w = n & 1;
-        if (ok && n > 0) ok = warp_wait(&sh.o_free[w ^ 1], (uint32_t)((n - 1) >> 1) & 1u, &sh.abort, a.err);
-        if (ok) ok = warp_wait(&sh.v_full[s], (uint32_t)(n / kStages) & 1u, &sh.abort, a.err);
-        if (ok && n >= draft0) ok = warp_wait(&sh.v_ok[n - draft0], 0u, &sh.abort, a.err);
-        if (ok) ok = warp_wait(&sh.p_ready[w], (uint32_t)(n >> 1) & 1u, &sh.abort, a.err);
-        if (!ok) break;
+      for (int j = 0; j < min(2, np); ++j) {
+        wait_phase(&sh.k_full[j], 0u, &sh.abort);
         tc_fence_after();
-        if (leader) {
-#pragma unroll
-          for (int p = 2; p >= 0; --p) {
-            const uint32_t ap = tmem + T::kP + (uint32_t)w * 96 + (uint32_t)p * 32;
-            const uint64_t bd = umma_desc_mn_sw128(sV + s * T::kKV, T::kBox);
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)  // 16 slots: 2048 bytes on
-              umma_bf16_ts(tmem + T::kO, ap + 8u * kk, bd + 128ull * kk, id_o, (uint32_t)(p != 2 || kk));
-          }
-          umma_commit(&sh.v_empty[s]);
-          umma_commit(&sh.o_full[w]);
-        }
+        if (leader) scores(j, 0, T::kQMma);
         __syncwarp();
       }
-    } else if (warp >= 10) {
-      // ---- V rows of the blocks that reach behind the context: one thread per slot
-      const int row = tid - 320;
+      wait_phase(&sh.p_ready[0], 0u, &sh.abort);
+      for (int j = 0; j < np; ++j) {
+#pragma unroll
+        for (int i = 0; i < T::kSteps; ++i) {
+          const int w = i / T::BOX, h = i % T::BOX, n = 2 * j + w, s = n % kVStages;
+          if (n < nb) {
+            // O is free once its last half has been read
+            const int last = i == 0 ? T::kSteps - 1 : i - 1, lj = i == 0 ? j - 1 : j;
+            if (lj >= 0) wait_phase(&sh.o_free[last / T::BOX], (uint32_t)(lj * T::BOX + last % T::BOX) & 1u, &sh.abort);
+            tc_fence_after();
+            if (leader) {
+#pragma unroll
+              for (int p = 2; p >= 0; --p) {
+                const uint32_t ap = tmem + T::kP + (uint32_t)w * 96 + (uint32_t)p * 32;
+                const uint64_t bd = umma_desc_mn_sw128(sV + s * T::kV + h * T::kVBox);
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)  // 16 slots: 2048 bytes on
+                  umma_bf16_ts(tmem + T::kO, ap + 8u * kk, bd + 128ull * kk, id_o, (uint32_t)(p != 2 || kk));
+              }
+              if (h == T::BOX - 1) umma_commit(&sh.v_empty[s]);
+              umma_commit(&sh.o_full[w]);
+            }
+            __syncwarp();
+          }
+          // the next block's P (and V: the group has seen it), while the tensor core is busy
+          if (h == T::BOX - 1 && n + 1 < nb) wait_phase(&sh.p_ready[w ^ 1], (uint32_t)((n + 1) >> 1) & 1u, &sh.abort);
+          if (j + 2 < np) {
+            if (i == 0) {
+              wait_phase(&sh.k_full[j % kKStages], (uint32_t)((j + 2) / kKStages) & 1u, &sh.abort);
+              wait_phase(&sh.s_free[j & 1], (uint32_t)(j >> 1) & 1u, &sh.abort);
+            }
+            tc_fence_after();
+            if (leader) scores(j + 2, i * 6, i * 6 + 6);
+            __syncwarp();
+          }
+        }
+      }
+      // nothing of this warp's is under way when the tensor memory is freed
+      if (leader) umma_commit(&sh.idle);
+      __syncwarp();
+      mbar_wait(&sh.idle, 0u);
+    } else if (warp == 11) {
+      // ---- V rows of the blocks that reach behind the context
       for (int n = max(0, draft0); n < nb; ++n) {
-        const int s = n % kStages, slot = (blk0 + n) * kTcBlock + row;
-        if (!wait_or_abort(&sh.v_full[s], (uint32_t)(n / kStages) & 1u, &sh.abort, a.err)) break;
-        if (slot >= T0) {
+        const int s = n % kVStages;
+        if (!wait_phase(&sh.v_full[s], (uint32_t)(n / kVStages) & 1u, &sh.abort)) break;
+        for (int row = lane; row < kTcBlock; row += 32) {
+          const int slot = (blk0 + n) * kTcBlock + row;
+          if (slot < T0) continue;
 #pragma unroll 1
           for (int c = 0; c < HD / 8; ++c) {
-            uint4* at = reinterpret_cast<uint4*>(sV + s * T::kKV + (c / 8) * T::kBox + row * 128 + (((c & 7) ^ (row & 7)) << 4));
+            uint4* at = reinterpret_cast<uint4*>(sV + s * T::kV + (c / 8) * T::kVBox + row * 128 + (((c & 7) ^ (row & 7)) << 4));
             if (slot >= slots) {
               *at = make_uint4(0, 0, 0, 0);
               continue;
@@ -338,25 +388,23 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
     __syncwarp();
   } else {
     // ---- softmax: group w, one row per thread
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-    const int w = warp >> 2, row = tid & 127, r = k.r0 + row;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int w = warp >> 2, row = tid & 127;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const unsigned long long anc = r < k.R ? a.anc[k.sq.row0 + r / k.G] : 0ull;
     float o[HD], m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int d = 0; d < HD; ++d) o[d] = 0.f;
-    bool ok = true;
-    for (int n = w; ok && n < nb; n += 2) {
-      const uint32_t ph = (uint32_t)(n >> 1) & 1u;
+    for (int j = 0; 2 * j + w < nb; ++j) {
+      const int n = 2 * j + w;
       const bool drafted = n >= draft0;
-      ok = wait_or_abort(&sh.s_full[w], ph, &sh.abort, a.err);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
+      wait_phase(&sh.s_full[j & 1], (uint32_t)(j >> 1) & 1u, &sh.abort);
       tc_fence_after();
       uint32_t u0[32], u1[32];
-      tmem_ld32(lanes + (uint32_t)w * 64, u0);
-      tmem_ld32(lanes + (uint32_t)w * 64 + 32, u1);
+      tmem_ld32(lanes + (uint32_t)(j & 1) * kPair + (uint32_t)w * 64, u0);
+      tmem_ld32(lanes + (uint32_t)(j & 1) * kPair + (uint32_t)w * 64 + 32, u1);
       tmem_ld_wait();
+      tc_fence_before();
+      mbar_arrive(&sh.s_free[j & 1]);
       unsigned long long see = ~0ull;  // which of the block's slots this row sees
       if (drafted) {
         const int node0 = (blk0 + n) * kTcBlock - T0;
@@ -396,23 +444,26 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
       l = fmaf(l, f, s0 + s1);
       tmem_st_wait();
       tc_fence_before();
+      if (row == 0) wait_phase(&sh.v_full[n % kVStages], (uint32_t)(n / kVStages) & 1u, &sh.abort);
+      if (drafted) wait_phase(&sh.v_ok[n - draft0], 0u, &sh.abort);
       mbar_arrive(&sh.p_ready[w]);
-      ok = wait_or_abort(&sh.o_full[w], ph, &sh.abort, a.err);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc_fence_after();
 #pragma unroll
-      for (int d = 0; d < HD; d += 32) {
-        tmem_ld32(lanes + T::kO + (uint32_t)d, u0);
+      for (int h = 0; h < T::BOX; ++h) {
+        wait_phase(&sh.o_full[w], (uint32_t)(j * T::BOX + h) & 1u, &sh.abort);
+        tc_fence_after();
+        tmem_ld32(lanes + T::kO, u0);
+        tmem_ld32(lanes + T::kO + 32u, u1);
         tmem_ld_wait();
+        tc_fence_before();
+        mbar_arrive(&sh.o_free[w]);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[d + e] = fmaf(o[d + e], f, __uint_as_float(u0[e]));
+        for (int e = 0; e < 32; ++e) {
+          o[h * 64 + e] = fmaf(o[h * 64 + e], f, __uint_as_float(u0[e]));
+          o[h * 64 + 32 + e] = fmaf(o[h * 64 + 32 + e], f, __uint_as_float(u1[e]));
+        }
       }
-      tc_fence_before();
-      mbar_arrive(&sh.o_free[w]);
       if (drafted) {
-        // values that were taken out of V, added where they are seen (the wait orders the flag)
-        if (!wait_or_abort(&sh.v_ok[n - draft0], 0u, &sh.abort, a.err)) break;
+        // values that were taken out of V, added where they are seen
         if (sh.bad[n - draft0]) {
           for (int j = 0; j < kTcBlock; ++j) {
             const int slot = (blk0 + n) * kTcBlock + j;
@@ -436,10 +487,11 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
     for (int d = 0; d < HD; d += 4) *reinterpret_cast<float4*>(mine + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
     sML[(w * kTcRows + row) * 2] = m, sML[(w * kTcRows + row) * 2 + 1] = l;
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    if (!sh.abort) ta_finish<HD, 2, kTcRows>(P, k, sO, sML, tid, 256);
+    if (!sh.abort) ta_finish<HD, 2, kTcRows, 256>(P, k, sO, sML, tid);
   }
   tc_fence_before();
   __syncthreads();
+  if (tid == 0 && sh.abort) atomicExch(a.err, kErrWait);
   if (warp == 8) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
