@@ -165,18 +165,48 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a,
   // warps: `parts` of them share a row, n_rows rows are under way at once
   const int parts = m < kPickWarps ? kPickWarps / m : 1, n_rows = kPickWarps / parts;
   const int part = warp % parts, first_row = warp / parts;
-  // the first logits are on their way while the history is counted
-  if (first_row < min(n_rows, m))
-    for (int lc = part; lc < min(n_chunks, part + kBatch * parts); lc += parts) {
-      const int t = token_of(lc);
-      if (t < a.vocab) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.logits + (size_t)(row0 + first_row) * a.vocab + t));
+  // the loads of kBatch chunks of a row, from chunk lc0 on
+  Group grp[kBatch];
+  auto load_chunks = [&](int q, int lc0) {
+    const int row = row0 + q, sh = ALIGNED ? 0 : (int)(((size_t)row * a.vocab) & 3);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int lc = lc0 + u * parts;
+      if (lc < n_chunks)
+        load_group<ALIGNED>(grp[u], a.logits + (size_t)row * a.vocab, a.mask ? a.mask + (size_t)row * mask_words : nullptr,
+                            token_of(lc) - sh, a.vocab);
     }
+  };
+  if (first_row < min(n_rows, m)) load_chunks(first_row, part);  // on their way while the history is counted
 
   const bool counting = a.penalties != nullptr, biasing = a.bias_tok != nullptr, ruled = counting || biasing;
   const bool pathed = counting && a.seqs;
   uint32_t* cnt = dyn;
   uint32_t* bia = dyn + n_words;
   RowRules r{1.f, 1.f, 1.f, nullptr};
+  // what the counting needs first is loaded before the shared memory is cleared
+  constexpr int B = 8;  // history loads in flight per thread
+  const int h_step = (int)csize * kPickThreads;
+  int h0 = 0, h1 = 0, given = 0, b0 = 0, b1 = 0, tok[B];
+  if (counting) {
+    r.rep = a.penalties[3 * s], r.freq = a.penalties[3 * s + 1], r.pres = a.penalties[3 * s + 2];
+    if (a.hist) {
+      const int o0 = a.hist_off[s], o1 = a.hist_off[s + 1], pl = a.prompt ? a.prompt[s] : 0;
+      h0 = clampi(o0, 0, a.hist_total), h1 = clampi(o1, h0, a.hist_total), given = h0 + clampi(pl, 0, h1 - h0);
+    }
+  }
+  if (biasing) {
+    const int o0 = a.bias_off[s], o1 = a.bias_off[s + 1];
+    b0 = clampi(o0, 0, a.bias_total), b1 = clampi(o1, b0, a.bias_total);
+    r.bias_val = a.bias_val + b0;
+  }
+  auto load_history = [&](int i) {
+#pragma unroll
+    for (int e = 0; e < B; ++e) tok[e] = i + e * h_step < h1 ? __ldg(a.hist + i + e * h_step) : -1;
+  };
+  int h_at = h0 + (int)crank * kPickThreads + tid;
+  load_history(h_at);
+  const int b_tok = b0 + tid < b1 ? a.bias_tok[b0 + tid] : -1;
   if (tid < kTreeMaxNodes) sm.key[tid] = 0ull;
   if (tid == 0) sm.n_drafted = 0;
   if (ruled) {
@@ -198,45 +228,31 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a,
       f((c + 1) & kmask, (int)(((c + 1) >> log2k) * kStride + kLead + in - kChunk));
   };
   if (counting) {
-    r.rep = a.penalties[3 * s], r.freq = a.penalties[3 * s + 1], r.pres = a.penalties[3 * s + 2];
-    if (a.hist) {
-      const int h0 = clampi(a.hist_off[s], 0, a.hist_total), h1 = clampi(a.hist_off[s + 1], h0, a.hist_total);
-      const int given = h0 + (a.prompt ? clampi(a.prompt[s], 0, h1 - h0) : 0);
-      auto see = [&](int i, int tok) {
-        words_of(tok, slice & ~(csize - 1), csize, [&](unsigned sl, int w) {
+    while (h_at < h1) {
+#pragma unroll
+      for (int e = 0; e < B; ++e) {
+        if (tok[e] < 0) continue;
+        words_of(tok[e], slice & ~(csize - 1), csize, [&](unsigned sl, int w) {
           uint32_t* to = csize > 1 ? cluster.map_shared_rank(cnt, sl & (csize - 1)) : cnt;
-          if (i < given)
+          if (h_at + e * h_step < given)
             atomicOr(to + w, kGiven);
           else
             atomicAdd(to + w, 1u);
         });
-      };
-      constexpr int B = 8;  // loads in flight
-      for (int i = h0 + (int)crank * kPickThreads + tid; i < h1; i += B * (int)csize * kPickThreads) {
-        int tok[B];
-#pragma unroll
-        for (int e = 0; e < B; ++e) {
-          const int at = i + e * (int)csize * kPickThreads;
-          tok[e] = at < h1 ? __ldg(a.hist + at) : -1;
-        }
-#pragma unroll
-        for (int e = 0; e < B; ++e) see(i + e * (int)csize * kPickThreads, tok[e]);
       }
+      h_at += B * h_step;
+      load_history(h_at);
     }
     if (pathed && tid < m)
       words_of(sm.draft[tid], slice, 1, [&](unsigned, int w) {
         if (!(atomicOr(cnt + w, kDrafted) & kDrafted)) sm.drafted[atomicAdd(&sm.n_drafted, 1)] = (uint16_t)w;
       });
   }
-  if (biasing) {
-    const int b0 = clampi(a.bias_off[s], 0, a.bias_total), b1 = clampi(a.bias_off[s + 1], b0, a.bias_total);
-    r.bias_val = a.bias_val + b0;
-    for (int i = b0 + tid; i < b1; i += kPickThreads)
-      words_of(a.bias_tok[i], slice, 1, [&](unsigned, int w) {
-        atomicOr(cnt + w, kBiased);
-        atomicMax(bia + w, (uint32_t)(i - b0 + 1));  // of a token listed twice the last entry counts
-      });
-  }
+  for (int i = b0 + tid; i < b1; i += kPickThreads)
+    words_of(i == b0 + tid ? b_tok : a.bias_tok[i], slice, 1, [&](unsigned, int w) {
+      atomicOr(cnt + w, kBiased);
+      atomicMax(bia + w, (uint32_t)(i - b0 + 1));  // of a token listed twice the last entry counts
+    });
   if (ruled) {
     if (csize > 1)
       cluster.sync();
@@ -255,7 +271,6 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a,
 #pragma unroll 1
   for (int q = first_row; q < m && first_row < n_rows; q += n_rows) {
     const int row = row0 + q, sh = ALIGNED ? 0 : (int)(((size_t)row * a.vocab) & 3);
-    const float* x = a.logits + (size_t)row * a.vocab;
     float* y = a.out ? a.out + (size_t)row * a.vocab : nullptr;
     const uint32_t* mask = a.mask ? a.mask + (size_t)row * mask_words : nullptr;
     const unsigned long long anc = pathed ? a.anc[row] : 0ull;
@@ -263,12 +278,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a,
     int bt = -1;
 #pragma unroll 1
     for (int lc0 = part; lc0 < n_chunks; lc0 += kBatch * parts) {
-      Group grp[kBatch];
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const int lc = lc0 + u * parts;
-        if (lc < n_chunks) load_group<ALIGNED>(grp[u], x, mask, token_of(lc) - sh, a.vocab);
-      }
+      if (lc0 != part || q != first_row) load_chunks(q, lc0);
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         const int lc = lc0 + u * parts, t = token_of(lc) - sh;
