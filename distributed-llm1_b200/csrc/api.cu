@@ -129,7 +129,7 @@ struct dllm_stage {
   // tracing: %globaltimer at kernel start and after every grid barrier (last launch)
   unsigned long long* trace = nullptr;
   int trace_cap = 0;
-  // tensor maps of the K and V pools as rows (layer, page, head, slot) of HD (bf16 caches)
+  // tensor maps of the K and V pools as rows (layer, page, head, slot) of HD
   CUtensorMap kv_map[2];
   bool kv_mapped = false;
   int version = 0;  // bumped when weights or tracing change (captured graphs rebuild)
@@ -1360,10 +1360,14 @@ int dllm_stage_create(dllm_ctx* c, int start, int end, dllm_stage** out) {
   if (!rc) rc = alloc_pool(&s->kpool);
   if (!rc) rc = alloc_pool(&s->vpool);
   const size_t kv_rows = s->layer_elems * s->nl / f.head_dim;
-  if (!rc && f.kv_dtype == DLLM_KV_BF16 && kv_rows > 0 && kv_rows <= 0x7fffffff) {
-    const int box = std::min(s->page, 64);
-    s->kv_mapped = dllm::tc_encode_rows(&s->kv_map[0], s->kpool, f.head_dim, (int)kv_rows, box) &&
-                   dllm::tc_encode_rows(&s->kv_map[1], s->vpool, f.head_dim, (int)kv_rows, box);
+  if (!rc && kv_rows > 0 && kv_rows <= 0x7fffffff) {
+    s->kv_mapped = true;
+    for (int i = 0; i < 2; ++i) {
+      const void* pool = i ? s->vpool : s->kpool;
+      s->kv_mapped = s->kv_mapped && (f.kv_dtype == DLLM_KV_BF16
+                                          ? dllm::tc_encode_rows(&s->kv_map[i], pool, f.head_dim, (int)kv_rows, std::min(s->page, 64))
+                                          : dllm::tc_encode_rows_f32(&s->kv_map[i], pool, f.head_dim, (int)kv_rows, 32));
+    }
   }
   if (!rc) rc = dev_alloc(c, &s->page_table, (size_t)s->max_seqs * s->pages_per_seq, "page table");
   if (!rc) {

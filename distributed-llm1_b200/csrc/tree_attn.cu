@@ -622,9 +622,10 @@ template <typename KT, int HD>
 cudaError_t launch_hd(const TreeAttnArgs& a, const TreeAttnShape& s, int sms, int* launches, cudaStream_t st) {
   const int rows = s.max_m * (a.nq / a.kvh);  // rows of the largest sequence that share a KV head
   if (rows <= 16) return launch<KT, HD, 1>(a, s, sms, launches, st);
-  if (sizeof(KT) == 2 && a.tc_k)
-    return launch_split<HD>(a, s, kTcRows, kTcBlock, sms, launches, st,
-                            [&](const TAKernelArgs& P, dim3 grid) { return launch_tree_attn_tc(P, HD, grid, st); });
+  if (a.tc_k)
+    return launch_split<HD>(a, s, kTcRows, kTcBlock, sms, launches, st, [&](const TAKernelArgs& P, dim3 grid) {
+      return sizeof(KT) == 2 ? launch_tree_attn_tc(P, HD, grid, st) : launch_tree_attn_tc32(P, HD, grid, st);
+    });
   if (rows <= 32) return launch<KT, HD, 2>(a, s, sms, launches, st);
   if (rows <= 64) return launch<KT, HD, 4>(a, s, sms, launches, st);
   return launch<KT, HD, 8>(a, s, sms, launches, st);
@@ -642,6 +643,7 @@ cudaError_t configure_tree_attn() {
   if (e == cudaSuccess) e = configure_hd<__nv_bfloat16, 64>();
   if (e == cudaSuccess) e = configure_hd<__nv_bfloat16, 128>();
   if (e == cudaSuccess) e = configure_tree_attn_tc();
+  if (e == cudaSuccess) e = configure_tree_attn_tc32();
   return e;
 }
 

@@ -93,10 +93,12 @@ DLLM_DEV void ta_finish(const TAKernelArgs& P, const TATile& k, const float* sO,
   }
 }
 
-// tree_attn_tc.cu
+// tree_attn_tc.cu (bf16 caches), tree_attn_tc32.cu (fp32 caches)
 constexpr int kTcBlock = 64;   // slots per block
 constexpr int kTcRows = 128;   // rows per tile
 cudaError_t configure_tree_attn_tc();
 cudaError_t launch_tree_attn_tc(const TAKernelArgs& P, int hd, dim3 grid, cudaStream_t st);
+cudaError_t configure_tree_attn_tc32();
+cudaError_t launch_tree_attn_tc32(const TAKernelArgs& P, int hd, dim3 grid, cudaStream_t st);
 
 }  // namespace dllm

@@ -29,8 +29,7 @@
 // gives per cycle, so every barrier and every tensor-memory store of the softmax waits behind
 // them, and a group's chain of softmax, P, O becomes the limit. (Scores block by block, 24
 // MMAs of N = 64, and O whole: 2565 cycles; a second issuing warp for O: 2240.)
-#include "tc.cuh"
-#include "tree_attn.cuh"
+#include "tree_attn_tc.cuh"
 
 namespace dllm {
 namespace {
@@ -39,78 +38,6 @@ constexpr int kTcAttnThreads = 384;
 constexpr int kKStages = 2;    // pairs
 constexpr int kVStages = 4;    // blocks
 constexpr int kPair = 2 * kTcBlock;
-constexpr int kErrWait = 5;  // the tensor-core wait code
-
-DLLM_DEV void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-// Waits for a phase, at most about 2 s (200000 tries of up to 10 us each), and less once
-// another wait of the CTA has given up: then it returns false at once, and the CTA runs on
-// through its loops without waiting, computes nothing of use, reports the error and ends.
-// One asm block, so that the compiler sees no branch: a warp that issues MMAs has to stay
-// one piece (a loop with votes cost 200 cycles even where the phase had completed).
-DLLM_DEV bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t.reg .u32 n, gone;\n\t"
-      "mov.u32 n, 0;\n\t"
-      "mov.u32 %0, 1;\n\t"
-      "TRY:\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 10000;\n\t"
-      "@p bra DONE;\n\t"
-      "ld.volatile.shared.u32 gone, [%3];\n\t"
-      "add.u32 n, n, 1;\n\t"
-      "setp.ne.u32 q, gone, 0;\n\t"
-      "setp.gt.or.u32 q, n, 200000, q;\n\t"
-      "@!q bra TRY;\n\t"
-      "mov.u32 %0, 0;\n\t"
-      "st.volatile.shared.u32 [%3], 1;\n\t"
-      "DONE:\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity), "r"(smem_u32(const_cast<const int*>(abort)))
-      : "memory");
-  return ok;
-}
-DLLM_DEV uint32_t elect_one() {
-  uint32_t r;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
-  return r;
-}
-
-// D[tmem] (+)= A[tmem, 128 x 16] * B[16 x N]: the A operand as packed bf16 pairs, 8 columns.
-DLLM_DEV void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate));
-}
-// Shared-memory descriptor of a 16 x 64 operand whose contiguous direction is the MMA's N
-// (dims): rows of 64 dims (128 bytes, swizzled), one per K index (slot), 8-slot groups 1024
-// bytes apart (stride offset; one 64-dim box, so the leading offset is not used).
-DLLM_DEV uint64_t umma_desc_mn_sw128(const void* tile) {
-  const uint64_t a = smem_u32(tile);
-  return ((a & 0x3FFFFull) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
-
-#define R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
-#define W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
-// 32 consecutive columns of this thread's lane.
-DLLM_DEV void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : R8(r, 0), R8(r, 8), R8(r, 16), R8(r, 24)
-      : "r"(addr));
-}
-DLLM_DEV void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::W8(r, 0), "r"(addr)
-               : "memory");
-}
-#undef R8
-#undef W8
-DLLM_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
 template <int HD>
 struct TcTile {
   static constexpr int BOX = HD / 64;                      // 64-dim boxes
@@ -208,34 +135,8 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
     // q, scaled so that the softmax is in powers of two, as three bf16 planes of swizzled
     // 64-dim boxes (what the K-major descriptor reads), while the producer's first copies fly.
     // Rows behind the last one stay as they are: a row of S, P and O comes from its row alone.
-    constexpr int kTasks = kTcRows * HD / 8, kWorkers = kTcAttnThreads - 32;
-    constexpr int kEach = (kTasks + kWorkers - 1) / kWorkers;
-    const int me = warp < 8 ? tid : tid - 32;
-    float4 f[kEach], g[kEach];
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const int i = me + e * kWorkers, row = i / (HD / 8), d = (i % (HD / 8)) * 8, r = k.r0 + row;
-      if (i < kTasks && r < k.R) {
-        const int node = k.node_of(r);
-        const float* q = a.q + ((size_t)(k.sq.row0 + node) * a.nq + k.head * k.G + (r - node * k.G)) * HD + d;
-        f[e] = *reinterpret_cast<const float4*>(q), g[e] = *reinterpret_cast<const float4*>(q + 4);
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const int i = me + e * kWorkers, row = i / (HD / 8), d = (i % (HD / 8)) * 8;
-      if (i >= kTasks || k.r0 + row >= k.R) break;
-      uint4 h, m, l;
-      const float c = a.scale_log2;
-      split3(f[e].x * c, f[e].y * c, h.x, m.x, l.x);
-      split3(f[e].z * c, f[e].w * c, h.y, m.y, l.y);
-      split3(g[e].x * c, g[e].y * c, h.z, m.z, l.z);
-      split3(g[e].z * c, g[e].w * c, h.w, m.w, l.w);
-      unsigned char* at = sQ + (d / 64) * (kTcRows * 128) + row * 128 + ((((d % 64) >> 3) ^ (row & 7)) << 4);
-      *reinterpret_cast<uint4*>(at) = h;
-      *reinterpret_cast<uint4*>(at + T::kQPlane) = m;
-      *reinterpret_cast<uint4*>(at + 2 * T::kQPlane) = l;
-    }
+    constexpr int kWorkers = kTcAttnThreads - 32;
+    ta_load_q<HD, kWorkers>(P, k, sQ, warp < 8 ? tid : tid - 32);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // q is read by the MMA
     asm volatile("bar.sync 2, %0;" ::"n"(kWorkers) : "memory");
   }
@@ -309,7 +210,12 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
         if (leader) scores(j, 0, T::kQMma);
         __syncwarp();
       }
-      wait_phase(&sh.p_ready[0], 0u, &sh.abort);
+      auto operands = [&](int n) {
+        wait_phase(&sh.v_full[n % kVStages], (uint32_t)(n / kVStages) & 1u, &sh.abort);
+        if (n >= draft0) wait_phase(&sh.v_ok[n - draft0], 0u, &sh.abort);
+        wait_phase(&sh.p_ready[n & 1], (uint32_t)(n >> 1) & 1u, &sh.abort);
+      };
+      operands(0);
       for (int j = 0; j < np; ++j) {
 #pragma unroll
         for (int i = 0; i < T::kSteps; ++i) {
@@ -323,7 +229,7 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
 #pragma unroll
               for (int p = 2; p >= 0; --p) {
                 const uint32_t ap = tmem + T::kP + (uint32_t)w * 96 + (uint32_t)p * 32;
-                const uint64_t bd = umma_desc_mn_sw128(sV + s * T::kV + h * T::kVBox);
+                const uint64_t bd = umma_desc_mn_sw128(sV + s * T::kV + h * T::kVBox, T::kVBox);
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk)  // 16 slots: 2048 bytes on
                   umma_bf16_ts(tmem + T::kO, ap + 8u * kk, bd + 128ull * kk, id_o, (uint32_t)(p != 2 || kk));
@@ -333,8 +239,8 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
             }
             __syncwarp();
           }
-          // the next block's P (and V: the group has seen it), while the tensor core is busy
-          if (h == T::BOX - 1 && n + 1 < nb) wait_phase(&sh.p_ready[w ^ 1], (uint32_t)((n + 1) >> 1) & 1u, &sh.abort);
+          // the next block's V and P, while the tensor core is busy
+          if (h == T::BOX - 1 && n + 1 < nb) operands(n + 1);
           if (j + 2 < np) {
             if (i == 0) {
               wait_phase(&sh.k_full[j % kKStages], (uint32_t)((j + 2) / kKStages) & 1u, &sh.abort);
@@ -405,47 +311,10 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
       tmem_ld_wait();
       tc_fence_before();
       mbar_arrive(&sh.s_free[j & 1]);
-      unsigned long long see = ~0ull;  // which of the block's slots this row sees
-      if (drafted) {
-        const int node0 = (blk0 + n) * kTcBlock - T0;
-        see = node0 >= 0 ? (node0 < 64 ? anc >> node0 : 0ull) : (anc << -node0) | ((1ull << -node0) - 1);
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          if (!(see >> c & 1)) u0[c] = __float_as_uint(-INFINITY);
-          if (!(see >> (c + 32) & 1)) u1[c] = __float_as_uint(-INFINITY);
-        }
-      }
-      float x0 = m, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < 32; c += 2) {
-        x0 = fmaxf(x0, __uint_as_float(u0[c])), x1 = fmaxf(x1, __uint_as_float(u0[c + 1]));
-        x2 = fmaxf(x2, __uint_as_float(u1[c])), x3 = fmaxf(x3, __uint_as_float(u1[c + 1]));
-      }
-      const float x = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3));
-      const float b = x == -INFINITY ? 0.f : x;  // a row that has seen nothing: every p is 0
-      const float f = ex2(m - b);
-      m = x;
-      float s0 = 0.f, s1 = 0.f;
-      const uint32_t tp = lanes + T::kP + (uint32_t)w * 96;
-#pragma unroll
-      for (int c = 0; c < 64; c += 16) {  // 8 packed columns of each plane at a time
-        uint32_t ph8[8], pm8[8], pl8[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float p0 = ex2(__uint_as_float(c < 32 ? u0[(c + 2 * e) & 31] : u1[(c + 2 * e) & 31]) - b);
-          const float p1 = ex2(__uint_as_float(c < 32 ? u0[(c + 2 * e + 1) & 31] : u1[(c + 2 * e + 1) & 31]) - b);
-          s0 += p0, s1 += p1;
-          split3(p0, p1, ph8[e], pm8[e], pl8[e]);
-        }
-        tmem_st8(tp + (uint32_t)(c / 2), ph8);
-        tmem_st8(tp + 32u + (uint32_t)(c / 2), pm8);
-        tmem_st8(tp + 64u + (uint32_t)(c / 2), pl8);
-      }
-      l = fmaf(l, f, s0 + s1);
+      const unsigned long long see = drafted ? ta_sees(anc, (blk0 + n) * kTcBlock - T0) : ~0ull;
+      const float f = ta_softmax_block(u0, u1, drafted, see, m, l, lanes + T::kP + (uint32_t)w * 96);
       tmem_st_wait();
       tc_fence_before();
-      if (row == 0) wait_phase(&sh.v_full[n % kVStages], (uint32_t)(n / kVStages) & 1u, &sh.abort);
-      if (drafted) wait_phase(&sh.v_ok[n - draft0], 0u, &sh.abort);
       mbar_arrive(&sh.p_ready[w]);
 #pragma unroll
       for (int h = 0; h < T::BOX; ++h) {
@@ -464,18 +333,8 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
       }
       if (drafted) {
         // values that were taken out of V, added where they are seen
-        if (sh.bad[n - draft0]) {
-          for (int j = 0; j < kTcBlock; ++j) {
-            const int slot = (blk0 + n) * kTcBlock + j;
-            if (slot < T0 || slot >= slots || !(see >> j & 1)) continue;
-            const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.vc) + a.kv.offset(k.sq.seq, slot, k.head);
-#pragma unroll
-            for (int d = 0; d < HD; ++d) {
-              const float e = bf16_to_f32(v[d]);
-              if (!is_finite(e)) o[d] += e;
-            }
-          }
-        }
+        wait_phase(&sh.v_ok[n - draft0], 0u, &sh.abort);
+        if (sh.bad[n - draft0]) ta_add_nonfinite<__nv_bfloat16, HD>(P, k, o, see, (blk0 + n) * kTcBlock, T0);
       }
     }
     // every MMA has completed (this group waited for its last O, and so did the other)
