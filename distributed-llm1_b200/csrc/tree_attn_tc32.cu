@@ -15,8 +15,13 @@
 // The planes of K and of V are single: K(n + 1) is converted while O(n - 1) runs, V(n)
 // while S(n + 1) runs. Tensor memory: S 2 x 64, P 2 x 96, O 128 columns.
 // Bound: per block 48 MMAs of 128 x 64 x 16 (49 cycles) and 24 of 128 x 128 x 16 (65): 3900
-// cycles, 2.0 us, against 1.5 us for 64 slots x 1024 bytes at one SM's share of HBM. The
-// mma.sync kernel with tf32 terms takes 8.5 us per block for 64 rows.
+// cycles, 2.0 us, against 1.5 us for 64 slots x 1024 bytes at one SM's share of HBM. Measured
+// 6500 cycles per block: the MMAs, the converters and the copies share 128 bytes of shared
+// memory per cycle, and V(n) waits for O(n - 1) before it is converted. The upper terms of q
+// in tensor memory with two sets of K planes made a block shorter (6000 cycles) but cost as
+// much at the start; several loads per converter thread in flight only held the MMAs up
+// (64 nodes x 7 heads at 32000 slots: 221 us one at a time, 241 two). The mma.sync kernel with
+// tf32 terms takes 16000 cycles per block for 64 rows.
 #include "tree_attn_tc.cuh"
 
 namespace dllm {
@@ -153,7 +158,7 @@ __global__ void __launch_bounds__(kTc32Threads, 1)
   };
 
   if (warp >= 8 && warp < 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 8 && lane == 0) {
       // ---- producer. The pools are one tensor of rows (layer, page, head, slot); a page holds at
       // least 32 slots, so a half lies in one page. Halves behind the end are loaded again.
@@ -227,7 +232,7 @@ __global__ void __launch_bounds__(kTc32Threads, 1)
     __syncwarp();
   } else if (warp >= 12) {
     // ---- converters
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     const int me = tid - 384;
     tiles([&](bool is_v, int n, int h, int i) {
       if (!wait_phase(&sh.in_full[i & 1], (uint32_t)(i >> 1) & 1u, &sh.abort)) return false;
@@ -237,10 +242,16 @@ __global__ void __launch_bounds__(kTc32Threads, 1)
       unsigned char* out = is_v ? sV : sK;
       const int slot0 = (blk0 + n) * kTcBlock + h * kHalf;
       const bool edge = is_v && slot0 + kHalf > T0;  // rows that some nodes do not see
-#pragma unroll 2
+#pragma unroll 1
       for (int j = me; j < kHalf * HD / 8; j += 128) {
         const int s = j / (HD / 8), c = j % (HD / 8), row = h * kHalf + s;
-        float4 f = *reinterpret_cast<const float4*>(in + j * 32), g = *reinterpret_cast<const float4*>(in + j * 32 + 16);
+        // lanes 4-7 of each eight read their second half first: the eight cover every bank
+        const int swap = (me & 4) << 2;
+        float4 f = *reinterpret_cast<const float4*>(in + j * 32 + swap), g = *reinterpret_cast<const float4*>(in + j * 32 + (swap ^ 16));
+        if (swap) {
+          const float4 z = f;
+          f = g, g = z;
+        }
         if (edge && slot0 + s >= T0) {
           if (slot0 + s >= slots) {
             f = g = make_float4(0.f, 0.f, 0.f, 0.f);
