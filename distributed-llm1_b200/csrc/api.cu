@@ -131,7 +131,7 @@ struct dllm_stage {
   int trace_cap = 0;
   // tensor maps of the K and V pools as rows (layer, page, head, slot) of HD
   CUtensorMap kv_map[2];
-  bool kv_mapped = false;
+  bool kv_mapped = false;  // the driver has encoded them
   int version = 0;  // bumped when weights or tracing change (captured graphs rebuild)
 };
 
@@ -704,11 +704,10 @@ int tree_attention(dllm_stage* s, int layer, const dllm_tree* tree, const dllm::
   a.nq = f.num_q_heads;
   a.kvh = f.num_kv_heads;
   a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)f.head_dim));
-  if (s->kv_mapped) {
-    a.tc_k = &s->kv_map[0];
-    a.tc_v = &s->kv_map[1];
-    a.tc_row0 = (int)((size_t)(layer - s->start) * s->layer_elems / f.head_dim);
-  }
+  if (!s->kv_mapped) return set_err(c, DLLM_ECUDA, "tree attention: the driver has no tensor map of the KV cache");
+  a.tc_k = &s->kv_map[0];
+  a.tc_v = &s->kv_map[1];
+  a.tc_row0 = (int)((size_t)(layer - s->start) * s->layer_elems / f.head_dim);
   a.part_o = c->tree_part;
   a.part_ml = c->tree_part + dllm::tree_attn_part_rows(c->sms) * f.head_dim;
   const dllm::TreeAttnShape shape{tree->seqs.data(), t0.t0, tree->n, tree->max_m};

@@ -73,8 +73,8 @@ template <typename KT, int HD, int WR>
 struct MmaTile {
   static constexpr bool kF32 = sizeof(KT) == 4;
   static constexpr int WS = 8 / WR;                 // warps side by side in slots
-  static constexpr int SN = kF32 ? 8 * WR : (WR == 1 ? 16 : WR == 2 ? 32 : WR == 4 ? 32 : 64);
-  static constexpr int BN = SN * WS;                // 64, or 128 for few rows of a bf16 cache
+  static constexpr int SN = kF32 ? 8 * WR : WR == 1 ? 16 : 32;
+  static constexpr int BN = SN * WS;                // 64, or 128 for up to 32 rows of a bf16 cache
   static constexpr int RT = 16 * WR;                // rows of the tile
   static constexpr int kRowBytes = HD * (int)sizeof(KT);
   static constexpr int kChunks = kRowBytes / 16;    // 16-byte chunks per slot
@@ -545,12 +545,13 @@ cudaError_t configure_one() {
   return cudaFuncSetAttribute(tree_attn_kernel<KT, HD, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                               MmaTile<KT, HD, WR>::kSmem);
 }
-template <typename KT, int HD>
+template <int HD>
 cudaError_t configure_hd() {
-  cudaError_t e = configure_one<KT, HD, 1>();
-  if (e == cudaSuccess) e = configure_one<KT, HD, 2>();
-  if (e == cudaSuccess) e = configure_one<KT, HD, 4>();
-  if (e == cudaSuccess) e = configure_one<KT, HD, 8>();
+  cudaError_t e = configure_one<float, HD, 1>();
+  if (e == cudaSuccess) e = configure_one<float, HD, 2>();
+  if (e == cudaSuccess) e = configure_one<__nv_bfloat16, HD, 1>();
+  if (e == cudaSuccess) e = configure_one<__nv_bfloat16, HD, 2>();
+  if (e == cudaSuccess) e = configure_one<__nv_bfloat16, HD, 4>();
   return e;
 }
 
@@ -618,17 +619,24 @@ cudaError_t launch(const TreeAttnArgs& a, const TreeAttnShape& s, int sms, int* 
   });
 }
 
+// Few rows take the mma.sync tiles of 16 and 32 rows: their CTAs start faster, and up to
+// there they keep up with HBM (7B heads, us with mma.sync / tcgen05: 3 nodes at 2000 slots
+// 12.6 / 16.7, at 16000 20.7 / 24.1). 64 rows only pay on a bf16 cache while no SM has more than
+// two blocks (8 nodes at 2000 slots 14.5 / 18.6, at 16000 30.9 / 24.8; fp32 18.6 / 16.6 and 55.9 /
+// 41.1). The rest runs on tcgen05.
 template <typename KT, int HD>
 cudaError_t launch_hd(const TreeAttnArgs& a, const TreeAttnShape& s, int sms, int* launches, cudaStream_t st) {
   const int rows = s.max_m * (a.nq / a.kvh);  // rows of the largest sequence that share a KV head
   if (rows <= 16) return launch<KT, HD, 1>(a, s, sms, launches, st);
-  if (a.tc_k)
-    return launch_split<HD>(a, s, kTcRows, kTcBlock, sms, launches, st, [&](const TAKernelArgs& P, dim3 grid) {
-      return sizeof(KT) == 2 ? launch_tree_attn_tc(P, HD, grid, st) : launch_tree_attn_tc32(P, HD, grid, st);
-    });
   if (rows <= 32) return launch<KT, HD, 2>(a, s, sms, launches, st);
-  if (rows <= 64) return launch<KT, HD, 4>(a, s, sms, launches, st);
-  return launch<KT, HD, 8>(a, s, sms, launches, st);
+  if constexpr (sizeof(KT) == 2) {
+    long long blocks = 0;
+    for (int i = 0; i < a.n_seqs; ++i) blocks += (long long)((s.t0[i] + s.seqs[i].m + kTcBlock - 1) / kTcBlock) * a.kvh;
+    if (rows <= 64 && blocks <= 2ll * sms) return launch<KT, HD, 4>(a, s, sms, launches, st);
+  }
+  return launch_split<HD>(a, s, kTcRows, kTcBlock, sms, launches, st, [&](const TAKernelArgs& P, dim3 grid) {
+    return sizeof(KT) == 2 ? launch_tree_attn_tc(P, HD, grid, st) : launch_tree_attn_tc32(P, HD, grid, st);
+  });
 }
 
 }  // namespace
@@ -638,10 +646,8 @@ cudaError_t launch_hd(const TreeAttnArgs& a, const TreeAttnShape& s, int sms, in
 size_t tree_attn_part_rows(int sms) { return (size_t)2 * sms * 128; }
 
 cudaError_t configure_tree_attn() {
-  cudaError_t e = configure_hd<float, 64>();
-  if (e == cudaSuccess) e = configure_hd<float, 128>();
-  if (e == cudaSuccess) e = configure_hd<__nv_bfloat16, 64>();
-  if (e == cudaSuccess) e = configure_hd<__nv_bfloat16, 128>();
+  cudaError_t e = configure_hd<64>();
+  if (e == cudaSuccess) e = configure_hd<128>();
   if (e == cudaSuccess) e = configure_tree_attn_tc();
   if (e == cudaSuccess) e = configure_tree_attn_tc32();
   return e;

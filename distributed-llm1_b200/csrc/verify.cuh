@@ -99,8 +99,8 @@ struct TreeAttnArgs {
   int n_seqs, nq, kvh;
   float scale_log2;  // log2(e) / sqrt(hd)
   int* err;
-  const void* tc_k;  // host: tensor maps (CUtensorMap) of the whole K and V pools as rows of hd;
-  const void* tc_v;  // null: no tcgen05 path
+  const void* tc_k;  // host: tensor maps (CUtensorMap) of the whole K and V pools as rows of hd
+  const void* tc_v;
   int tc_row0;       // the layer's first row
   float* part_o;   // [slots][hd] partial outputs of sequences that are split
   float* part_ml;  // [slots][2]
