@@ -710,6 +710,7 @@ int tree_attention(dllm_stage* s, int layer, const dllm_tree* tree, const dllm::
   a.tc_row0 = (int)((size_t)(layer - s->start) * s->layer_elems / f.head_dim);
   a.part_o = c->tree_part;
   a.part_ml = c->tree_part + dllm::tree_attn_part_rows(c->sms) * f.head_dim;
+  a.err = c->err_dev;
   const dllm::TreeAttnShape shape{tree->seqs.data(), t0.t0, tree->n, tree->max_m};
   int launches = 0;
   const cudaError_t e = dllm::op_tree_attention(a, shape, f.kv_dtype, f.head_dim, c->sms, &launches, c->stream);

@@ -655,6 +655,8 @@ cudaError_t configure_tree_attn() {
 
 cudaError_t op_tree_attention(const TreeAttnArgs& a, const TreeAttnShape& s, int kv_dtype, int hd, int sms,
                               int* launches, cudaStream_t st) {
+  // what the kernels use without asking; err only after a wait that gave up
+  if (!a.tc_k || !a.tc_v || !a.part_o || !a.part_ml || !a.err) return cudaErrorInvalidValue;
   if (kv_dtype == 0) return hd == 64 ? launch_hd<float, 64>(a, s, sms, launches, st)
                                      : launch_hd<float, 128>(a, s, sms, launches, st);
   return hd == 64 ? launch_hd<__nv_bfloat16, 64>(a, s, sms, launches, st)
