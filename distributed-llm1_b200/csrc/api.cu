@@ -2466,6 +2466,13 @@ int dllm_pick_tokens(dllm_ctx* c, const dllm_pick* p) {
   }
   if (p->mask)
     if (int rc = check_i32(c, p->mask, (size_t)n * ((V + 31) / 32), "pickTokens mask")) return rc;
+  // a row's results are stored while other rows still read theirs (a sequence's own draft
+  // has been read by then)
+  for (const dllm_buf* in : {p->history, p->history_offsets, p->prompt_lens, p->bias_tokens, p->bias_offsets, p->mask})
+    if (in == p->tokens)
+      return set_err(c, DLLM_EINVAL, "pickTokens: tokens must not be the history, offsets, biases or mask");
+  if (p->out && (p->out == p->penalties || p->out == p->bias_values))
+    return set_err(c, DLLM_EINVAL, "pickTokens: out must not be the penalties or bias values");
   if (int rc = use_device(c)) return rc;
   dllm::PickArgs a{};
   a.logits = (const float*)p->logits->ptr;

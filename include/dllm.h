@@ -378,7 +378,7 @@ typedef struct dllm_pick {
   const dllm_tree* tree;           /* rows are the tree's nodes */
   const dllm_buf* draft;           /* i32 [n], with a tree: the nodes' tokens */
   dllm_buf* out;                   /* f32 [n, V]: the processed logits; may be `logits` */
-  dllm_buf* tokens;                /* i32 [n] */
+  dllm_buf* tokens;                /* i32 [n]; may be `draft`, no other input */
 } dllm_pick;
 /* With c = occurrences of token t among the generated tokens of the row's history (a
  * node's history ends with the drafted tokens from its root to itself):

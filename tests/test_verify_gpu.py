@@ -639,8 +639,37 @@ def test_pick_refusals(dllm):
             ctx.pickTokens(*args, **kw)
     with pytest.raises(E):
         ctx.createI32(0)
+    # an output that other rows still read as their input
+    mask, wide = ctx.createI32(2 * 4), ctx.createF32(200)
+    offs = i32(ctx, [0, 0, 0, 0, 0])
+    for kw in (dict(history=(h, offs, pl), penalties=pen, tokens=h), dict(history=(h, offs, pl), penalties=pen, tokens=offs),
+               dict(history=(h, offs, pl), penalties=pen, tokens=pl), dict(bias=(h, vals, offs), tokens=h),
+               dict(bias=(h, vals, offs), tokens=offs), dict(mask=mask, tokens=mask), dict(penalties=wide, out=wide),
+               dict(bias=(h, wide, offs), out=wide)):
+        with pytest.raises(E):
+            ctx.pickTokens(x, 2, **kw)
     ctx.close()
     other.close()
+
+
+def test_pick_over_its_inputs(dllm):
+    """The tokens may replace the drafted ones, and the processed logits the logits."""
+    ctx = make_ctx(dllm, vocab_size=10007)
+    rng = np.random.default_rng(8)
+    n, V = 21, 10007
+    parents = [bushy(rng, 13), chain(7), [-1]]
+    tree = ctx.draftTree([p for t in parents for p in t], [13, 7, 1])
+    x, said = rng.standard_normal((n, V)).astype(np.float32), rng.integers(0, V, n)
+    pen = f32(ctx, [[1.3, 0.2, 0.1]] * 3)
+    out = ctx.createF32(n * V)
+    want = ctx.readI32(ctx.pickTokens(f32(ctx, x), n, penalties=pen, tree=tree, draft=i32(ctx, said), out=out))
+    processed = ctx.readF32(out, out.n)
+    for _ in range(3):
+        both, over = i32(ctx, said), f32(ctx, x)
+        ctx.pickTokens(over, n, penalties=pen, tree=tree, draft=both, tokens=both, out=over)
+        assert np.array_equal(ctx.readI32(both), want)
+        assert np.array_equal(ctx.readF32(over, over.n), processed)
+    ctx.close()
 
 
 # ---- streams and graphs ---------------------------------------------------------------------------------
