@@ -2560,6 +2560,8 @@ int dllm_stage_commit_tree(dllm_stage* s, const dllm_tree* tree, const int32_t* 
     p += lens[i];
   }
   if (int rc = use_device(c)) return rc;
+  // T0 would move at the capture, the rows with every replay
+  if (int rc = refuse_capture(c, "commit_tree")) return rc;
   const KvLayout kv = stage_kv(s);
   dllm::CommitArgs a;
   a.n_seqs = 0;

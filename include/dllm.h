@@ -327,8 +327,10 @@ int dllm_attention_noalloc_status(void* cuda_stream, int timeout_ms, int* device
  * dllm_stage_forward_tree runs the first four (with the layers' projections) for
  * every layer of a stage. All work is enqueued on the ctx stream, in order; scratch
  * belongs to the ctx, so calls of one ctx, and graphs captured from them, must not
- * overlap on the GPU. T0 values and paths become kernel arguments: a captured call
- * replays with those of its capture. */
+ * overlap on the GPU. T0 values become kernel arguments: a captured call replays with
+ * those of its capture, and refers to the buffers, trees and plans it was given. Not to
+ * be captured: dllm_tree_create, dllm_rope_plan_create, dllm_stage_commit_tree and
+ * dllm_stage_forward_tree. */
 
 typedef struct dllm_tree dllm_tree;
 typedef struct dllm_rope_plan dllm_rope_plan;
@@ -393,7 +395,8 @@ int dllm_pick_tokens(dllm_ctx* ctx, const dllm_pick* args);
 int dllm_stage_append_tree(dllm_stage* st, int layer, const dllm_tree* tree, const dllm_buf* k, const dllm_buf* v);
 /* out[row] = attention of node `row` (q [n, NQ*HD], after RoPE) over its sequence's
  * slots [0, T0) and the slots of its ancestors and itself. A non-finite value in a
- * drafted K/V row reaches only the nodes that see the row. */
+ * drafted K/V row reaches only the nodes that see the row; there, an infinity may come
+ * out as NaN. */
 int dllm_stage_tree_attention(dllm_stage* st, int layer, const dllm_tree* tree, const dllm_buf* q, dllm_buf* out);
 /* Keep one path per sequence: lens[i] node indices (a root, then a child each; 0: keep
  * nothing), all sequences' in turn in `path`. Slot T0 + path[j] -> T0 + j in every

@@ -713,8 +713,10 @@ def test_on_a_side_stream_and_in_a_captured_graph(dllm):
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g, stream=s):
         step()
-        with pytest.raises(dllm.DllmError):
-            ctx.draftTree([-1])
+        for call in (lambda: ctx.draftTree([-1]), lambda: ctx.ropePlan(), lambda: stage.commit_tree(tree, [[0], []])):
+            with pytest.raises(dllm.DllmError):
+                call()
+    assert [stage.t0_of(0), stage.t0_of(1)] == [900, 40]
     for seed, want in zip((5, 6, 5), wants + wants[:1]):
         fill(seed)
         with torch.cuda.stream(s):
