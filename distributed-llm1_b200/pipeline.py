@@ -252,6 +252,7 @@ class Stage:
     def commit_tree(self, tree: DraftTree, paths):
         """Keep one path of nodes per sequence (root first): its K/V rows move to slots
         T0.. of every layer and T0 advances by its length."""
+        paths = [list(p) for p in paths]  # read twice
         lens = array("i", map(len, paths))
         if len(lens) != tree.counts.size:
             raise _lib.DllmError(_lib.DLLM_EINVAL, f"commit_tree: {len(lens)} paths for {tree.counts.size} sequences")

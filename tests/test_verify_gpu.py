@@ -378,6 +378,13 @@ def test_append_tree(dllm, kv):
     P.close()
 
 
+def test_commit_tree_takes_iterators(dllm):
+    P = Paged(dllm, 4, 2, 64, "f32", [5, 9], [[-1, 0, 0], [-1, 0]])
+    P.stage.commit_tree(P.tree, (iter(p) for p in ([0, 2], [0])))
+    assert [P.stage.t0_of(s) for s in (0, 1)] == [7, 10]
+    P.close()
+
+
 @pytest.mark.parametrize("kv", ["bf16", "f32"])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_commit_tree(dllm, kv, hd):
