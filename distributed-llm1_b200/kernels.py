@@ -39,6 +39,8 @@ class GpuBuffer:
         """The buffer's memory as a flat array (bf16 as int16 bits), e.g. for
         torch.as_tensor(buf, device="cuda"). No stream is synchronised: order the
         other library's work with the ctx stream (set_stream)."""
+        if not self.handle:
+            raise ValueError(f"buffer {self.label!r} has been destroyed")
         return {"shape": (self.n,), "typestr": {"f32": "<f4", "i32": "<i4", "bf16": "<i2"}[self.dtype],
                 "data": (self.device_ptr, False), "version": 3, "strides": None}
 

@@ -132,6 +132,8 @@ class _KvPool:
 
     def __init__(self, stage: "Stage", which: int):
         f = stage.k.cfg
+        if not stage.handle:
+            raise ValueError("the stage has been closed")
         self.stage = stage  # keeps the memory alive
         self.__cuda_array_interface__ = {
             "shape": (stage.end - stage.start, f.max_seqs * stage.pages_per_seq(), f.num_kv_heads, f.kv_page_size,

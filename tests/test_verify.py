@@ -76,3 +76,9 @@ def test_null_handles_are_refused(dllm):
     assert not lib.dllm_stage_kv_device_ptr(None, 0)
     lib.dllm_tree_destroy(None)
     lib.dllm_rope_plan_destroy(None)
+
+
+def test_memory_of_freed_buffers_is_refused():
+    b = kernels.GpuBuffer(None, None, 4, "f32", "gone")
+    with pytest.raises(ValueError):
+        b.__cuda_array_interface__
