@@ -254,11 +254,14 @@ class Stage:
     def commit_tree(self, tree: DraftTree, paths):
         """Keep one path of nodes per sequence (root first): its K/V rows move to slots
         T0.. of every layer and T0 advances by its length."""
-        paths = [list(p) for p in paths]  # read twice
-        lens = array("i", map(len, paths))
+        flat, lens = [], []
+        for p in paths:
+            before = len(flat)
+            flat += p
+            lens.append(len(flat) - before)
+        flat, lens = array("i", flat or (0,)), array("i", lens)
         if len(lens) != tree.counts.size:
             raise _lib.DllmError(_lib.DLLM_EINVAL, f"commit_tree: {len(lens)} paths for {tree.counts.size} sequences")
-        flat = array("i", [j for p in paths for j in p] or [0])
         self.k._check(self.lib.dllm_stage_commit_tree(self.handle, self.k._h(tree), flat.buffer_info()[0],
                                                       lens.buffer_info()[0]), "commit_tree")
 
