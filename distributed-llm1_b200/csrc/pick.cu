@@ -39,7 +39,8 @@ namespace {
 constexpr int kPickThreads = 512;
 constexpr int kPickWarps = kPickThreads / 32;
 constexpr int kChunk = 128;       // tokens one warp covers at a time, 4 per lane
-constexpr int kMaxChunks = 64;    // chunks per slice
+constexpr int kMaxChunks = 192;   // chunks per slice: two CTAs per SM have room for their count words, or for
+                                  // half as many and the bias words
 // Chunk c of a row has its tokens [128 c - shift, 128 c - shift + 128): a row whose
 // address is `shift` elements past a 16-byte boundary starts that much early. So a
 // chunk's words hold its 128 tokens behind the 4 before them, the last 3 of which are
@@ -148,7 +149,7 @@ DLLM_DEV void four_words(uint32_t (&r)[4], const uint32_t* p, int sh) {
 // multiple of 4, so every row starts at a 16-byte boundary.
 template <bool ALIGNED>
 __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a, int log2k, int n_chunks) {
-  extern __shared__ __align__(16) uint32_t dyn[];  // counts, bias entries of the slice's words
+  extern __shared__ __align__(16) uint32_t dyn[];  // counts, and bias entries if there are any, of the slice's words
   __shared__ PickShared sm;
   cg::cluster_group cluster = cg::this_cluster();
   const unsigned csize = cluster.num_blocks(), crank = cluster.block_rank();
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a,
   if (tid < kTreeMaxNodes) sm.key[tid] = 0ull;
   if (tid == 0) sm.n_drafted = 0;
   if (ruled) {
-    for (int i = tid; i < 2 * n_words / 4; i += kPickThreads) reinterpret_cast<uint4*>(dyn)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < (biasing ? 2 : 1) * n_words / 4; i += kPickThreads) reinterpret_cast<uint4*>(dyn)[i] = make_uint4(0, 0, 0, 0);
     if (pathed && tid < m) sm.draft[tid] = a.draft[row0 + tid];
   }
   if (csize > 1)
@@ -339,8 +340,7 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a,
   if (tid < m) a.tokens[row0 + tid] = sm.key[tid] ? argmax_key_index(sm.key[tid]) : -1;
 }
 
-// counts and bias entries of a slice's words
-constexpr size_t pick_smem(int n_chunks) { return (size_t)n_chunks * kStride * 8; }
+constexpr size_t pick_smem(int n_chunks) { return (size_t)n_chunks * kStride * 4; }  // one set of words
 
 }  // namespace
 
@@ -352,12 +352,13 @@ cudaError_t configure_pick_kernels() {
 }
 
 cudaError_t op_pick(const PickArgs& a, int sms, cudaStream_t st) {
-  // The fewest slices that fit a CTA (64 chunks), then twice as many as long as all CTAs
-  // still run at once, two per SM, and a slice keeps at least 4 chunks and one for every
-  // warp. A row that starts 3 tokens early reaches vocab + 3.
+  // The fewest slices whose count words fit a CTA (one without rules, which has none), then
+  // twice as many as long as all CTAs still run at once, two per SM, and a slice keeps at
+  // least 4 chunks and one for every warp. A row that starts 3 tokens early reaches vocab + 3.
   const long long chunks = ((long long)a.vocab + 3 + kChunk - 1) / kChunk;
   int log2k = 0;
-  while ((chunks + (1ll << log2k) - 1) >> log2k > kMaxChunks) ++log2k;
+  const int sets = (a.penalties || a.bias_tok ? 1 : 0) + (a.bias_tok ? 1 : 0);
+  while ((chunks + (1ll << log2k) - 1) * sets >> log2k > kMaxChunks) ++log2k;
   while ((2ll << log2k) * a.n_seqs <= 2ll * sms && chunks >> (log2k + 1) >= 4 &&
          (chunks >> (log2k + 1)) * a.max_m >= kPickWarps)
     ++log2k;
@@ -365,7 +366,7 @@ cudaError_t op_pick(const PickArgs& a, int sms, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(1u << log2k, a.n_seqs);
   cfg.blockDim = dim3(kPickThreads);
-  cfg.dynamicSmemBytes = a.penalties || a.bias_tok ? pick_smem(n_chunks) : 0;
+  cfg.dynamicSmemBytes = sets * pick_smem(n_chunks);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
