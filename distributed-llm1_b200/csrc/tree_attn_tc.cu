@@ -59,7 +59,7 @@ struct TcShared {
   uint64_t k_full[kKStages], k_empty[kKStages], v_full[kVStages], v_empty[kVStages];
   uint64_t s_full[2], s_free[2];               // per S buffer
   uint64_t p_ready[2], o_full[2], o_free[2];   // per softmax group
-  uint64_t v_ok[2];                            // the (at most two) blocks with drafted rows
+  uint64_t v_here[2], v_ok[2];                 // the (at most two) blocks with drafted rows
   uint64_t idle;                               // every MMA has completed
   uint32_t tmem;
   int bad[2];
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
     for (int w = 0; w < 2; ++w) {
       mbar_init(&sh.s_full[w], 1), mbar_init(&sh.s_free[w], 256);
       mbar_init(&sh.p_ready[w], 128), mbar_init(&sh.o_full[w], 1), mbar_init(&sh.o_free[w], 128);
-      mbar_init(&sh.v_ok[w], 32);
+      mbar_init(&sh.v_here[w], 32), mbar_init(&sh.v_ok[w], 32);
       sh.bad[w] = 0;
     }
     mbar_init(&sh.idle, 1);
@@ -212,7 +212,10 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
       }
       auto operands = [&](int n) {
         wait_phase(&sh.v_full[n % kVStages], (uint32_t)(n / kVStages) & 1u, &sh.abort);
-        if (n >= draft0) wait_phase(&sh.v_ok[n - draft0], 0u, &sh.abort);
+        if (n >= draft0) {
+          mbar_arrive(&sh.v_here[n - draft0]);
+          wait_phase(&sh.v_ok[n - draft0], 0u, &sh.abort);
+        }
         wait_phase(&sh.p_ready[n & 1], (uint32_t)(n >> 1) & 1u, &sh.abort);
       };
       operands(0);
@@ -257,9 +260,12 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
       __syncwarp();
       mbar_wait(&sh.idle, 0u);
     } else if (warp == 11) {
-      // ---- V rows of the blocks that reach behind the context
+      // ---- V rows of the blocks that reach behind the context. The MMA warp, which has seen
+      // every block before, says when one is there: a parity alone would also match an
+      // earlier turn of the ring. (The wait on v_full then orders the copy before the reads.)
       for (int n = max(0, draft0); n < nb; ++n) {
         const int s = n % kVStages;
+        if (!wait_phase(&sh.v_here[n - draft0], 0u, &sh.abort)) break;
         if (!wait_phase(&sh.v_full[s], (uint32_t)(n / kVStages) & 1u, &sh.abort)) break;
         for (int row = lane; row < kTcBlock; row += 32) {
           const int slot = (blk0 + n) * kTcBlock + row;

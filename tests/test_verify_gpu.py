@@ -295,6 +295,40 @@ def test_tree_attention_batch(dllm, kv, page):
     P.close()
 
 
+@pytest.mark.parametrize("kv", ["bf16", "f32"])
+@pytest.mark.parametrize("hd,nq,lens,m", [(128, 12, [8051, 6039], 55), (128, 12, [8051] * 3, 23),
+                                          (64, 16, [7990, 8001, 5000, 6666], 40), (128, 16, [2001] * 16, 9)])
+def test_tree_attention_many_blocks_per_split(dllm, kv, hd, nq, lens, m):
+    """The drafted rows come after many turns of the K/V rings and end inside a block."""
+    rng = np.random.default_rng(m)
+    P = Paged(dllm, nq, 2, hd, kv, lens, [bushy(rng, m) for _ in lens])
+    check_attention(P)
+    P.close()
+
+
+@pytest.mark.parametrize("kv", ["bf16", "f32"])
+def test_tree_attention_leftovers_after_many_blocks(dllm, kv):
+    """NaN behind the last node, and in a drafted row that only itself sees, far into a split."""
+    lens, m = [8051, 6039], 55
+    trees = [[-1] + [0] * (m - 1)] * 2
+    P = Paged(dllm, 12, 2, 128, kv, lens, trees, max_pos=8192)
+    n = 2 * m
+    q = f32(P.ctx, np.random.default_rng(3).standard_normal((n, 12 * 128)))
+    want = P.ctx.readF32(P.stage.tree_attention(0, P.tree, q), n * 12 * 128).reshape(n, -1)
+    assert np.isfinite(want).all()
+    for s, t0 in enumerate(lens):
+        for slot in [*range(t0 + m, 8192), t0 + 20]:
+            for pool in P.pool:
+                pool[:, int(P.table[s][slot // 64]), :, slot % 64] = float("nan")
+    torch_().cuda.synchronize()
+    got = P.ctx.readF32(P.stage.tree_attention(0, P.tree, q), n * 12 * 128).reshape(n, -1)
+    seers = [20, m + 20]
+    assert np.isnan(got[seers]).all()
+    rest = np.delete(np.arange(n), seers)
+    assert np.array_equal(got[rest], want[rest])
+    P.close()
+
+
 def test_tree_attention_many_sequences(dllm):
     rng = np.random.default_rng(8)
     lens = [int(x) for x in rng.integers(0, 90, 128)]
