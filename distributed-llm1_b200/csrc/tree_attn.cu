@@ -620,10 +620,11 @@ cudaError_t launch(const TreeAttnArgs& a, const TreeAttnShape& s, int sms, int* 
 }
 
 // Few rows take the mma.sync tiles of 16 and 32 rows: their CTAs start faster, and up to
-// there they keep up with HBM (7B heads, us with mma.sync / tcgen05: 3 nodes at 2000 slots
-// 12.6 / 16.7, at 16000 20.7 / 24.1). 64 rows only pay on a bf16 cache while no SM has more than
-// two blocks (8 nodes at 2000 slots 14.5 / 18.6, at 16000 30.9 / 24.8; fp32 18.6 / 16.6 and 55.9 /
-// 41.1). The rest runs on tcgen05.
+// there they keep up with HBM (28 query heads on 4 KV heads of 128, us with mma.sync /
+// tcgen05: 3 nodes at 2000 slots 12.6 / 16.7, at 16000 20.7 / 24.1). Tiles of 64 rows pay on
+// a bf16 cache while no SM has more than two blocks (9 nodes at 2000 slots 14.5 / 18.6, 16
+// nodes there 16.9 / 20.7, at 3500 22.5 / 18.7; 32 nodes at 300 slots 14.7 / 18.6; on an
+// fp32 cache 8 nodes at 2000 slots 18.6 / 16.6). The rest runs on tcgen05.
 template <typename KT, int HD>
 cudaError_t launch_hd(const TreeAttnArgs& a, const TreeAttnShape& s, int sms, int* launches, cudaStream_t st) {
   const int rows = s.max_m * (a.nq / a.kvh);  // rows of the largest sequence that share a KV head
@@ -632,7 +633,7 @@ cudaError_t launch_hd(const TreeAttnArgs& a, const TreeAttnShape& s, int sms, in
   if constexpr (sizeof(KT) == 2) {
     long long blocks = 0;
     for (int i = 0; i < a.n_seqs; ++i) blocks += (long long)((s.t0[i] + s.seqs[i].m + kTcBlock - 1) / kTcBlock) * a.kvh;
-    if (rows <= 64 && blocks <= 2ll * sms) return launch<KT, HD, 4>(a, s, sms, launches, st);
+    if ((rows + 63) / 64 * blocks <= 2ll * sms) return launch<KT, HD, 4>(a, s, sms, launches, st);
   }
   return launch_split<HD>(a, s, kTcRows, kTcBlock, sms, launches, st, [&](const TAKernelArgs& P, dim3 grid) {
     return sizeof(KT) == 2 ? launch_tree_attn_tc(P, HD, grid, st) : launch_tree_attn_tc32(P, HD, grid, st);
