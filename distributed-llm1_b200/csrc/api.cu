@@ -945,7 +945,10 @@ int dllm_init_kernels(int device, const dllm_config* cfg, dllm_ctx** out) {
   if (cudaMallocHost(&c->best_host, sizeof(unsigned long long)) != cudaSuccess) return fail(DLLM_ENOMEM);
   if (dev_alloc(c, &c->err_dev, 1, "error flag")) return fail(DLLM_ENOMEM);
   if (dev_alloc(c, &c->best, 1, "argmax")) return fail(DLLM_ENOMEM);
-  if (dev_alloc(c, &c->pick_best, (size_t)dllm::kPickMaxRows * 3 / 2, "pick keys")) return fail(DLLM_ENOMEM);
+  // 4 MB, an allocation of its own: among the small ones it would move the stage's grid
+  // barrier to another place in L2 (0.8 % of a decode token)
+  static_assert(dllm::kPickMaxRows * 3 / 2 <= 1 << 19, "keys and arrival counters");
+  if (dev_alloc(c, &c->pick_best, (size_t)1 << 19, "pick keys")) return fail(DLLM_ENOMEM);
   std::vector<float> fr;
   rope_table(f, &fr);
   if (dev_alloc(c, &c->freq, fr.size(), "rope table")) return fail(DLLM_ENOMEM);
