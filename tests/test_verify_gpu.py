@@ -649,6 +649,26 @@ def test_pick_many_rows_and_a_vocabulary_beyond_one_chunk(dllm):
     ctx.close()
 
 
+@pytest.mark.parametrize("v", [152064, 151937])
+@pytest.mark.parametrize("use", ["plain", "penalties", "bias"])
+def test_pick_slices_of_many_rows(dllm, v, use):
+    """Enough rows that a slice is as large as its shared memory allows (or, without rules,
+    the whole vocabulary)."""
+    ctx = make_ctx(dllm, vocab_size=v)
+    rng = np.random.default_rng(v)
+    n = 300 if use == "plain" else 40
+    x = rng.standard_normal((n, v), np.float32)
+    kw = {}
+    if use != "plain":
+        kw["pen"] = [[1.2, 0.1, 0.3]] * n
+        kw["hist"] = [list(map(int, rng.integers(0, v, 200))) + [v - 1, 0] for _ in range(n)]
+        kw["prompt"] = [60] * n
+    if use == "bias":
+        kw["bias"] = [[(int(t), 2.0) for t in rng.integers(0, v, 20)] + [(v - 1, 1.0)] for _ in range(n)]
+    run_pick(ctx, x, range(n), **kw)
+    ctx.close()
+
+
 def test_pick_clamps_offsets_outside_the_buffers(dllm):
     """Offsets come from the device: wild ones are clamped, never followed."""
     ctx = make_ctx(dllm, vocab_size=100)
