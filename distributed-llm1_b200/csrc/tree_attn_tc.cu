@@ -260,12 +260,12 @@ __global__ void __launch_bounds__(kTcAttnThreads, 1)
       __syncwarp();
       mbar_wait(&sh.idle, 0u);
     } else if (warp == 11) {
-      // ---- V rows of the blocks that reach behind the context. The MMA warp, which has seen
-      // every block before, says when one is there: a parity alone would also match an
-      // earlier turn of the ring. (The wait on v_full then orders the copy before the reads.)
+      // ---- V rows of the blocks that reach behind the context. After the ring's first turn the
+      // MMA warp, which has seen every block before, says when one is there: a parity alone
+      // would also match an earlier turn. (The wait on v_full orders the copy before the reads.)
       for (int n = max(0, draft0); n < nb; ++n) {
         const int s = n % kVStages;
-        if (!wait_phase(&sh.v_here[n - draft0], 0u, &sh.abort)) break;
+        if (n >= kVStages && !wait_phase(&sh.v_here[n - draft0], 0u, &sh.abort)) break;
         if (!wait_phase(&sh.v_full[s], (uint32_t)(n / kVStages) & 1u, &sh.abort)) break;
         for (int row = lane; row < kTcBlock; row += 32) {
           const int slot = (blk0 + n) * kTcBlock + row;
