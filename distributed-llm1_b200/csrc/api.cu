@@ -2569,10 +2569,12 @@ int dllm_stage_commit_tree(dllm_stage* s, const dllm_tree* tree, const int32_t* 
   dllm::CommitArgs a;
   a.n_seqs = 0;
   auto flush = [&]() {
-    if (a.n_seqs == 0 || s->nl == 0) return cudaSuccess;
-    const cudaError_t e = dllm::op_tree_commit(a, kv, s->kpool, s->vpool, s->layer_elems, s->nl, f.kv_dtype,
-                                               f.num_kv_heads, f.head_dim, c->stream);
-    c->launches += 1;
+    cudaError_t e = cudaSuccess;
+    if (a.n_seqs > 0 && s->nl > 0) {  // a stage may have no layers, and nothing to move
+      e = dllm::op_tree_commit(a, kv, s->kpool, s->vpool, s->layer_elems, s->nl, f.kv_dtype, f.num_kv_heads, f.head_dim,
+                               c->stream);
+      c->launches += 1;
+    }
     a.n_seqs = 0;
     return e;
   };

@@ -446,6 +446,21 @@ def test_commit_tree(dllm, kv, hd):
     P.close()
 
 
+def test_commit_tree_on_a_stage_without_layers(dllm):
+    """Nothing to move, but more sequences whose rows would have to than one launch takes: T0 moves on."""
+    n = 128
+    ctx = make_ctx(dllm, max_seqs=n, max_pos=64)
+    stage = dllm.Stage(ctx, 0, 0)
+    tree = ctx.draftTree([-1, 0, 0] * n, [3] * n)
+    before = ctx.launch_count
+    stage.commit_tree(tree, [[0, 2]] * n)
+    ctx.synchronize()
+    assert ctx.launch_count == before
+    assert [stage.t0_of(s) for s in range(n)] == [2] * n
+    stage.close()
+    ctx.close()
+
+
 def test_tree_refusals(dllm):
     ctx, other = make_ctx(dllm, max_seqs=2, max_pos=100), make_ctx(dllm)
     stage = dllm.Stage(ctx, 0, 1)
