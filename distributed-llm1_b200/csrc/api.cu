@@ -40,9 +40,14 @@ constexpr int kMaxSplitsAlloc = dllm::kAttnMaxSplits;  // attention splits per (
 #endif
 constexpr int kPrefetchBytes = DLLM_PREFETCH_BYTES;  // per-CTA L2 prefetch budget between phases
 
+// Buffers, trees and rope plans are opaque pointers to their callers: the first word tells
+// which of them a pointer is, so that one in the place of another is refused.
+enum Kind : uint32_t { kBuf = 0x64627566, kTree = 0x64747265, kRopePlan = 0x64726f70 };
+
 }  // namespace
 
 struct dllm_buf {
+  const Kind kind = kBuf;
   dllm_ctx* ctx = nullptr;
   int device = 0;  // kept so the buffer can be freed after its ctx is destroyed
   void* ptr = nullptr;
@@ -137,6 +142,7 @@ struct dllm_stage {
 
 // A drafted tree per sequence: nodes in batch rows, parents before children.
 struct dllm_tree {
+  const Kind kind = kTree;
   dllm_ctx* ctx = nullptr;
   int n = 0, n_seqs = 0, max_m = 0;
   std::vector<dllm::TreeSeq> seqs;
@@ -147,6 +153,7 @@ struct dllm_tree {
 };
 
 struct dllm_rope_plan {
+  const Kind kind = kRopePlan;
   dllm_ctx* ctx = nullptr;
   int rotary = 0, interleaved = 0;
   float factor = 1.f;
@@ -257,7 +264,8 @@ int sync_check(dllm_ctx* c, int timeout_ms) {
   return DLLM_OK;
 }
 
-bool valid_buf(const dllm_ctx* c, const dllm_buf* b) { return b && b->ctx == c && b->ptr; }
+bool valid_buf(const dllm_ctx* c, const dllm_buf* b) { return b && b->kind == kBuf && b->ctx == c && b->ptr; }
+bool valid_tree(const dllm_ctx* c, const dllm_tree* t) { return t && t->kind == kTree && t->ctx == c; }
 
 int check_f32(dllm_ctx* c, const dllm_buf* b, size_t need, const char* what) {
   if (!valid_buf(c, b)) return set_err(c, DLLM_EINVAL, "%s: null or foreign buffer", what);
@@ -673,7 +681,7 @@ int upload(dllm_ctx* c, const void* src, size_t bytes, const char* label, dllm_b
 // The T0 of every sequence of a tree, with room for its nodes behind it.
 int tree_t0(dllm_stage* s, const dllm_tree* tree, const char* what, dllm::TreeT0* t0) {
   dllm_ctx* c = s->ctx;
-  if (!tree || tree->ctx != c) return set_err(c, DLLM_EINVAL, "%s: null or foreign tree", what);
+  if (!valid_tree(c, tree)) return set_err(c, DLLM_EINVAL, "%s: null or foreign tree", what);
   for (int i = 0; i < tree->n_seqs; ++i) {
     const dllm::TreeSeq& q = tree->seqs[i];
     if (q.seq >= s->max_seqs) return set_err(c, DLLM_EINVAL, "%s: invalid seq %d", what, q.seq);
@@ -1100,7 +1108,7 @@ int dllm_read_bf16(dllm_ctx* c, const dllm_buf* b, uint16_t* dst, size_t n) {
 }
 
 void dllm_buf_free(dllm_buf* b) {
-  if (!b) return;
+  if (!b || b->kind != kBuf) return;
   if (--b->refs > 0) return;
   dllm_ctx* c = b->ctx;
   if (b->ptr) {
@@ -1116,8 +1124,8 @@ void dllm_buf_free(dllm_buf* b) {
   ctx_release(c);
 }
 
-size_t dllm_buf_bytes(const dllm_buf* b) { return b ? b->bytes : 0; }
-void* dllm_buf_device_ptr(const dllm_buf* b) { return b ? b->ptr : nullptr; }
+size_t dllm_buf_bytes(const dllm_buf* b) { return b && b->kind == kBuf ? b->bytes : 0; }
+void* dllm_buf_device_ptr(const dllm_buf* b) { return b && b->kind == kBuf ? b->ptr : nullptr; }
 
 int dllm_fill_normal_bf16(dllm_ctx* c, dllm_buf* b, uint64_t seed, float std) {
   if (!c) return DLLM_EINVAL;
@@ -2325,7 +2333,7 @@ int dllm_rope_plan_create(dllm_ctx* c, const dllm_rope_config* r, dllm_rope_plan
 }
 
 void dllm_rope_plan_destroy(dllm_rope_plan* p) {
-  if (!p) return;
+  if (!p || p->kind != kRopePlan) return;
   dllm_buf_free(p->turns);
   delete p;
 }
@@ -2333,7 +2341,7 @@ void dllm_rope_plan_destroy(dllm_rope_plan* p) {
 int dllm_rope_at(dllm_ctx* c, const dllm_rope_plan* p, const dllm_buf* positions, int n, dllm_buf* q, dllm_buf* k,
                  dllm_buf* q_out, dllm_buf* k_out) {
   if (!c) return DLLM_EINVAL;
-  if (!p || p->ctx != c) return set_err(c, DLLM_EINVAL, "ropeAt: null or foreign plan");
+  if (!p || p->kind != kRopePlan || p->ctx != c) return set_err(c, DLLM_EINVAL, "ropeAt: null or foreign plan");
   if (n <= 0) return set_err(c, DLLM_EINVAL, "ropeAt: invalid n=%d", n);
   if (!q && !k) return set_err(c, DLLM_EINVAL, "ropeAt: neither q nor k given");
   if ((!q && q_out) || (!k && k_out)) return set_err(c, DLLM_EINVAL, "ropeAt: an output without its input");
@@ -2422,7 +2430,7 @@ int dllm_tree_create(dllm_ctx* c, const int32_t* parents, const int32_t* counts,
 }
 
 void dllm_tree_destroy(dllm_tree* t) {
-  if (!t) return;
+  if (!t || t->kind != kTree) return;
   dllm_buf_free(t->dev);
   delete t;
 }
@@ -2436,7 +2444,7 @@ int dllm_pick_tokens(dllm_ctx* c, const dllm_pick* p) {
     return set_err(c, DLLM_EINVAL, "pickTokens: n=%d outside 1..%d", n, dllm::kPickMaxRows);
   if ((p->tree != nullptr) != (p->draft != nullptr))
     return set_err(c, DLLM_EINVAL, "pickTokens: a tree comes with its drafted tokens");
-  if (p->tree && (p->tree->ctx != c || p->tree->n != n))
+  if (p->tree && (!valid_tree(c, p->tree) || p->tree->n != n))
     return set_err(c, DLLM_EINVAL, "pickTokens: the tree is foreign or has not n=%d nodes", n);
   const size_t b = p->tree ? p->tree->n_seqs : n;
   if (int rc = check_f32(c, p->logits, (size_t)n * V, "pickTokens logits")) return rc;

@@ -169,14 +169,15 @@ class KernelContext:
         return GpuBuffer(self, out.value, n, "f32", label)
 
     @staticmethod
-    def _h(buf: GpuBuffer):
-        if not isinstance(buf, (GpuBuffer, DraftTree, RopePlan)) or not buf.handle:
-            raise ValueError("expected a live GpuBuffer")
-        return buf.handle
+    def _h(obj, kind=GpuBuffer):
+        """The handle of a live object of one kind: the library takes plain pointers."""
+        if not isinstance(obj, kind) or not obj.handle:
+            raise ValueError(f"expected a live {kind.__name__}")
+        return obj.handle
 
     @classmethod
-    def _opt(cls, buf):
-        return None if buf is None else cls._h(buf)
+    def _opt(cls, obj, kind=GpuBuffer):
+        return None if obj is None else cls._h(obj, kind)
 
     def close(self):
         if getattr(self, "handle", None):
@@ -321,8 +322,8 @@ class KernelContext:
                kBuf: GpuBuffer | None = None, qOut: GpuBuffer | None = None, kOut: GpuBuffer | None = None):
         """Row t of q [n, NQ*HD] and k [n, KVH*HD] at positions[t]; in place without outputs."""
         h, o = self._h, self._opt
-        self._check(self.lib.dllm_rope_at(self.handle, h(plan), h(positions), n, o(qBuf), o(kBuf), o(qOut), o(kOut)),
-                    "ropeAt")
+        self._check(self.lib.dllm_rope_at(self.handle, h(plan, RopePlan), h(positions), n, o(qBuf), o(kBuf), o(qOut),
+                                          o(kOut)), "ropeAt")
         return qOut or qBuf, kOut or kBuf
 
     def draftTree(self, parents, counts=None, seqs=None) -> DraftTree:
@@ -343,8 +344,8 @@ class KernelContext:
         h, o = self._h, self._opt
         ht, ho, hp = history if history is not None else (None, None, None)
         bt, bv, bo = bias if bias is not None else (None, None, None)
-        a = _lib.dllm_pick(n, h(logits), o(ht), o(ho), o(hp), o(penalties), o(bt), o(bv), o(bo), o(mask), o(tree),
-                           o(draft), o(out), h(tokens))
+        a = _lib.dllm_pick(n, h(logits), o(ht), o(ho), o(hp), o(penalties), o(bt), o(bv), o(bo), o(mask),
+                           o(tree, DraftTree), o(draft), o(out), h(tokens))
         self._check(self.lib.dllm_pick_tokens(self.handle, C.byref(a)), "pickTokens")
         return tokens
 

@@ -241,19 +241,21 @@ class Stage:
     def append_tree(self, L: int, tree: DraftTree, kBuf: GpuBuffer, vBuf: GpuBuffer):
         """K/V rows of a tree's nodes -> slots T0 + node of their sequences (T0 unchanged)."""
         h = self.k._h
-        self.k._check(self.lib.dllm_stage_append_tree(self.handle, L, h(tree), h(kBuf), h(vBuf)), "append_tree")
+        self.k._check(self.lib.dllm_stage_append_tree(self.handle, L, h(tree, DraftTree), h(kBuf), h(vBuf)), "append_tree")
 
     def tree_attention(self, L: int, tree: DraftTree, qBuf: GpuBuffer, out: GpuBuffer | None = None) -> GpuBuffer:
         """Every node of a tree over its sequence's cached slots and its own ancestors."""
         k = self.k
+        t, q = k._h(tree, DraftTree), k._h(qBuf)
         if out is None:
             out = k.createF32(tree.n * k.NQ * k.HD, "tree_attn_out")
-        k._check(self.lib.dllm_stage_tree_attention(self.handle, L, k._h(tree), k._h(qBuf), k._h(out)), "tree_attention")
+        k._check(self.lib.dllm_stage_tree_attention(self.handle, L, t, q, k._h(out)), "tree_attention")
         return out
 
     def commit_tree(self, tree: DraftTree, paths):
         """Keep one path of nodes per sequence (root first): its K/V rows move to slots
         T0.. of every layer and T0 advances by its length."""
+        t = self.k._h(tree, DraftTree)
         flat, lens = [], []
         for p in paths:
             before = len(flat)
@@ -262,17 +264,17 @@ class Stage:
         flat, lens = array("i", flat or (0,)), array("i", lens)
         if len(lens) != tree.counts.size:
             raise _lib.DllmError(_lib.DLLM_EINVAL, f"commit_tree: {len(lens)} paths for {tree.counts.size} sequences")
-        self.k._check(self.lib.dllm_stage_commit_tree(self.handle, self.k._h(tree), flat.buffer_info()[0],
-                                                      lens.buffer_info()[0]), "commit_tree")
+        self.k._check(self.lib.dllm_stage_commit_tree(self.handle, t, flat.buffer_info()[0], lens.buffer_info()[0]),
+                      "commit_tree")
 
     def forward_tree(self, tree: DraftTree, hBuf: GpuBuffer, tokens: GpuBuffer | None = None,
                      logits: GpuBuffer | None = None) -> GpuBuffer:
         """The stage's layers for a tree's rows (at most 128), h [n, D] in place; `tokens`
         replaces h by their embeddings first, `logits` [n, vocab] receives the LM head's
         rows. T0 stays until commit_tree."""
-        o = self.k._opt
-        self.k._check(self.lib.dllm_stage_forward_tree(self.handle, self.k._h(tree), self.k._h(hBuf), o(tokens),
-                                                       o(logits)), "forward_tree")
+        h, o = self.k._h, self.k._opt
+        self.k._check(self.lib.dllm_stage_forward_tree(self.handle, h(tree, DraftTree), h(hBuf), o(tokens), o(logits)),
+                      "forward_tree")
         return hBuf
 
     def close(self):
@@ -452,6 +454,7 @@ class LeaderPipeline:
         if not self.singleNode:
             raise _lib.DllmError(_lib.DLLM_EINVAL, "verify_tree: the leader's stage must own every layer (single node)")
         k, cfg = self.k, self.k.cfg
+        k._h(tree, DraftTree)
         draft = np.ascontiguousarray(draft, dtype=np.int32).reshape(-1)
         if draft.size != tree.n or draft.size == 0 or draft.min() < 0 or draft.max() >= cfg.vocab_size:
             raise _lib.DllmError(_lib.DLLM_EINVAL, f"verify_tree: need {tree.n} token ids in [0, {cfg.vocab_size})")

@@ -82,3 +82,55 @@ def test_memory_of_freed_buffers_is_refused():
     b = kernels.GpuBuffer(None, None, 4, "f32", "gone")
     with pytest.raises(ValueError):
         b.__cuda_array_interface__
+
+
+class NoLibrary:
+    """Stands in for the library where no call may reach it."""
+
+    def __getattr__(self, name):
+        def call(*args):
+            raise AssertionError(f"{name} was called")
+        return call
+
+
+def test_objects_of_another_kind_are_refused(dllm):
+    """The library takes plain pointers: a buffer, a tree and a plan must not pass for one another."""
+    ctx = object.__new__(kernels.KernelContext)
+    ctx.lib, ctx.handle, ctx.cfg = NoLibrary(), None, dllm.CFG
+    ctx.NQ, ctx.KVH, ctx.HD, ctx.D = 2, 2, 64, 8
+    stage = object.__new__(dllm.Stage)
+    stage.k, stage.lib, stage.handle, stage._owned = ctx, ctx.lib, 8, False
+    stage.W = importlib.import_module("distributed-llm1_b200.pipeline")._StageWeights(stage)
+    leader = object.__new__(dllm.LeaderPipeline)
+    leader.k, leader.lib, leader.stage, leader.singleNode, leader.handle = ctx, ctx.lib, stage, True, None
+    buf = kernels.GpuBuffer(ctx, 16, 2, "f32")
+    tree = bare_tree([-1, 0], [2])
+    plan = object.__new__(kernels.RopePlan)
+    tree.handle, plan.handle, plan.ctx = 32, 48, ctx
+    try:
+        for wrong in (tree, plan, None, "buffer"):
+            for call in (lambda: ctx.add(wrong, buf, 2), lambda: ctx.readF32(wrong, 2), lambda: ctx.readI32(wrong, 2),
+                         lambda: ctx.ropeAt(plan, wrong, 2, buf), lambda: ctx.pickTokens(wrong, 2, tokens=buf),
+                         lambda: stage.append_tree(0, tree, wrong, buf), lambda: stage.append_tree(0, tree, buf, wrong),
+                         lambda: stage.tree_attention(0, tree, wrong, buf), lambda: stage.forward_tree(tree, wrong),
+                         lambda: stage.W.__setitem__("model.norm.weight", wrong), lambda: leader.setLeaderWeights(tree)):
+                with pytest.raises(ValueError):
+                    call()
+        for wrong in (tree, plan):
+            for call in (lambda: ctx.ropeAt(plan, buf, 2, wrong), lambda: ctx.ropeAt(plan, buf, 2, buf, qOut=wrong),
+                         lambda: stage.tree_attention(0, tree, buf, wrong), lambda: stage.forward_tree(tree, buf, wrong),
+                         lambda: ctx.pickTokens(buf, 2, tokens=wrong), lambda: ctx.pickTokens(buf, 2, mask=wrong, tokens=buf)):
+                with pytest.raises(ValueError):
+                    call()
+        for wrong in (buf, plan):
+            for call in (lambda: stage.append_tree(0, wrong, buf, buf), lambda: stage.tree_attention(0, wrong, buf, buf),
+                         lambda: stage.tree_attention(0, wrong, buf), lambda: stage.commit_tree(wrong, [[0]]),
+                         lambda: stage.forward_tree(wrong, buf), lambda: leader.verify_tree(wrong, [1, 2]),
+                         lambda: ctx.pickTokens(buf, 2, tree=wrong, draft=buf, tokens=buf)):
+                with pytest.raises(ValueError):
+                    call()
+        for wrong in (buf, tree):
+            with pytest.raises(ValueError):
+                ctx.ropeAt(wrong, buf, 2, buf)
+    finally:  # the handles are made up
+        buf.handle = tree.handle = plan.handle = stage.handle = None

@@ -501,6 +501,39 @@ def test_tree_refusals(dllm):
     other.close()
 
 
+def test_handles_of_another_kind_are_refused(dllm):
+    """The C calls themselves, as a host without the Python checks makes them."""
+    ctx = make_ctx(dllm)
+    stage = dllm.Stage(ctx, 0, 1)
+    lib = ctx.lib
+    tree, plan = ctx.draftTree([-1, 0, 0]), ctx.ropePlan()
+    b, pos = ctx.createF32(3 * 256), ctx.createI32(3)
+    launches = ctx.launch_count
+    for wrong in (tree.handle, plan.handle):
+        assert lib.dllm_stage_set_weight(stage.handle, b"model.norm.weight", wrong) == 1
+        assert lib.dllm_rope_at(ctx.handle, plan.handle, wrong, 3, b.handle, None, None, None) == 1
+        assert lib.dllm_rope_at(ctx.handle, plan.handle, pos.handle, 3, wrong, None, None, None) == 1
+        assert lib.dllm_stage_tree_attention(stage.handle, 0, tree.handle, wrong, b.handle) == 1
+        assert lib.dllm_buf_bytes(wrong) == 0 and not lib.dllm_buf_device_ptr(wrong)
+        lib.dllm_buf_free(wrong)
+    for wrong in (b.handle, plan.handle):
+        assert lib.dllm_stage_append_tree(stage.handle, 0, wrong, b.handle, b.handle) == 1
+        assert lib.dllm_stage_tree_attention(stage.handle, 0, wrong, b.handle, b.handle) == 1
+        assert lib.dllm_stage_forward_tree(stage.handle, wrong, b.handle, None, None) == 1
+        lib.dllm_tree_destroy(wrong)
+    for wrong in (b.handle, tree.handle):
+        assert lib.dllm_rope_at(ctx.handle, wrong, pos.handle, 3, b.handle, None, None, None) == 1
+        lib.dllm_rope_plan_destroy(wrong)
+    assert ctx.launch_count == launches
+    # all of them are as alive as before
+    ctx.writeI32(pos, [0, 1, 1])
+    ctx.ropeAt(plan, pos, 3, b)
+    out = stage.tree_attention(0, tree, b)
+    assert np.array_equal(ctx.readF32(out, out.n), np.zeros(out.n, np.float32))
+    stage.close()
+    ctx.close()
+
+
 # ---- token picks -----------------------------------------------------------------------------------
 def pick_reference(x, seq_of, hist, prompt, pen, bias, allowed, said):
     """The rules, each step rounded to fp32, and the picks. hist[s], bias[s]: lists; said[row]:
