@@ -22,12 +22,14 @@
 // another warp reads: a warp takes a row (or a part of one) through the slice's chunks,
 // 4 tokens per lane, and applies the rules where a count word says so. A drafted token
 // has the set of nodes that carry it, and its count for a node is the size of that set
-// among the node's ancestors. The slices' best (value, index) keys meet in one 64-bit
-// atomicMax per row (the largest key wins in any order); the CTA that arrives last
-// writes the tokens and clears the keys.
+// among the node's ancestors, less the nodes that a prompt longer than the history
+// reaches. The slices' best (value, index) keys meet in one 64-bit atomicMax per row
+// (the largest key wins in any order); the CTA that arrives last writes the tokens and
+// clears the keys.
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "verify.cuh"
 
@@ -122,6 +124,7 @@ DLLM_DEV void store_group(float* y, const Group& g, int t, int vocab) {
 struct PickShared {
   unsigned long long key[kTreeMaxNodes];
   unsigned long long nodes[2 * kTreeMaxNodes];  // per entry of drafted: the nodes with that token
+  unsigned long long given;                     // nodes whose tokens still belong to the prompt
   int32_t draft[kTreeMaxNodes];
   uint16_t drafted[2 * kTreeMaxNodes];          // words of drafted tokens
   int n_drafted;
@@ -147,7 +150,8 @@ DLLM_DEV void four_words(uint32_t (&r)[4], const uint32_t* p, int sh) {
 // Grid (K slices, sequences), K = 1 << log2k: slice s has the chunks c with c % K = s,
 // n_chunks of them at most. Clusters of neighbouring slices. ALIGNED: the vocabulary is a
 // multiple of 4, so every row starts at a 16-byte boundary.
-template <bool ALIGNED>
+// PROMPTED: a tree with prompt lengths.
+template <bool ALIGNED, bool PROMPTED>
 __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a, int log2k, int n_chunks) {
   extern __shared__ __align__(16) uint32_t dyn[];  // counts, and bias entries if there are any, of the slice's words
   __shared__ PickShared sm;
@@ -188,12 +192,13 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a,
   // what the counting needs first is loaded before the shared memory is cleared
   constexpr int B = 8;  // history loads in flight per thread
   const int h_step = (int)csize * kPickThreads;
-  int h0 = 0, h1 = 0, given = 0, b0 = 0, b1 = 0, tok[B];
+  int h0 = 0, h1 = 0, given = 0, levels = 0, b0 = 0, b1 = 0, tok[B];
   if (counting) {
     r.rep = a.penalties[3 * s], r.freq = a.penalties[3 * s + 1], r.pres = a.penalties[3 * s + 2];
     if (a.hist) {
       const int o0 = a.hist_off[s], o1 = a.hist_off[s + 1], pl = a.prompt ? a.prompt[s] : 0;
       h0 = clampi(o0, 0, a.hist_total), h1 = clampi(o1, h0, a.hist_total), given = h0 + clampi(pl, 0, h1 - h0);
+      if (PROMPTED && pl > h1 - h0) levels = pl - (h1 - h0);  // of the tree, which the prompt reaches into
     }
   }
   if (biasing) {
@@ -209,7 +214,10 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a,
   load_history(h_at);
   const int b_tok = b0 + tid < b1 ? a.bias_tok[b0 + tid] : -1;
   if (tid < kTreeMaxNodes) sm.key[tid] = 0ull;
-  if (tid == 0) sm.n_drafted = 0;
+  if (tid == 0) {
+    sm.n_drafted = 0;
+    if (PROMPTED) sm.given = 0ull;
+  }
   if (ruled) {
     for (int i = tid; i < (biasing ? 2 : 1) * n_words / 4; i += kPickThreads) reinterpret_cast<uint4*>(dyn)[i] = make_uint4(0, 0, 0, 0);
     if (pathed && tid < m) sm.draft[tid] = a.draft[row0 + tid];
@@ -244,10 +252,12 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a,
       h_at += B * h_step;
       load_history(h_at);
     }
-    if (pathed && tid < m)
+    if (pathed && tid < m) {
       words_of(sm.draft[tid], slice, 1, [&](unsigned, int w) {
         if (!(atomicOr(cnt + w, kDrafted) & kDrafted)) sm.drafted[atomicAdd(&sm.n_drafted, 1)] = (uint16_t)w;
       });
+      if (PROMPTED && levels && __popcll(a.anc[row0 + tid]) <= levels) atomicOr(&sm.given, 1ull << tid);
+    }
   }
   for (int i = b0 + tid; i < b1; i += kPickThreads)
     words_of(i == b0 + tid ? b_tok : a.bias_tok[i], slice, 1, [&](unsigned, int w) {
@@ -269,63 +279,75 @@ __global__ void __launch_bounds__(kPickThreads, 2) pick_kernel(const PickArgs a,
     if (pathed) __syncthreads();
   }
 
+  // A prompt that reaches into the tree is rare: its rule has a copy of the loop of its own
+  // (in the one loop it cost 64 nodes of 152064 tokens 5 %), in trees with prompt lengths only
+  // (16 rows of 50257 took 12.3 us with the copy, 12.0 without).
+  auto rows = [&](auto with_given) {
+    constexpr bool GIVEN = decltype(with_given)::value;
 #pragma unroll 1
-  for (int q = first_row; q < m && first_row < n_rows; q += n_rows) {
-    const int row = row0 + q, sh = ALIGNED ? 0 : (int)(((size_t)row * a.vocab) & 3);
-    float* y = a.out ? a.out + (size_t)row * a.vocab : nullptr;
-    const uint32_t* mask = a.mask ? a.mask + (size_t)row * mask_words : nullptr;
-    const unsigned long long anc = pathed ? a.anc[row] : 0ull;
-    float bv = -INFINITY;  // the greatest allowed logit of this lane, and its first token
-    int bt = -1;
+    for (int q = first_row; q < m && first_row < n_rows; q += n_rows) {
+      const int row = row0 + q, sh = ALIGNED ? 0 : (int)(((size_t)row * a.vocab) & 3);
+      float* y = a.out ? a.out + (size_t)row * a.vocab : nullptr;
+      const uint32_t* mask = a.mask ? a.mask + (size_t)row * mask_words : nullptr;
+      const unsigned long long anc = pathed ? a.anc[row] : 0ull;
+      float bv = -INFINITY;  // the greatest allowed logit of this lane, and its first token
+      int bt = -1;
 #pragma unroll 1
-    for (int lc0 = part; lc0 < n_chunks; lc0 += kBatch * parts) {
-      if (lc0 != part || q != first_row) load_chunks(q, lc0);
+      for (int lc0 = part; lc0 < n_chunks; lc0 += kBatch * parts) {
+        if (lc0 != part || q != first_row) load_chunks(q, lc0);
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const int lc = lc0 + u * parts, t = token_of(lc) - sh;
-        if (lc >= n_chunks) break;
-        Group& g = grp[u];
-        if (ruled) {
-          const int w = lc * kStride + kLead - sh + 4 * lane;
-          uint32_t c[4];
-          four_words<ALIGNED>(c, cnt + w + sh, sh);
+        for (int u = 0; u < kBatch; ++u) {
+          const int lc = lc0 + u * parts, t = token_of(lc) - sh;
+          if (lc >= n_chunks) break;
+          Group& g = grp[u];
+          if (ruled) {
+            const int w = lc * kStride + kLead - sh + 4 * lane;
+            uint32_t c[4];
+            four_words<ALIGNED>(c, cnt + w + sh, sh);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (!(g.bits >> e & 1)) c[e] = 0;
-            if (c[e] & kDrafted) {
-              int d = 0;
-              while (sm.drafted[d] != w + e) ++d;
-              c[e] = (c[e] & ~kDrafted) + (uint32_t)__popcll(anc & sm.nodes[d]);
+            for (int e = 0; e < 4; ++e) {
+              if (!(g.bits >> e & 1)) c[e] = 0;
+              if (c[e] & kDrafted) {
+                int d = 0;
+                while (sm.drafted[d] != w + e) ++d;
+                const unsigned long long on = anc & sm.nodes[d];
+                c[e] = (c[e] & ~kDrafted) + (uint32_t)__popcll(GIVEN ? on & ~sm.given : on);
+                if (GIVEN && (on & sm.given)) c[e] |= kGiven;
+              }
+              if (c[e]) g.v[e] = apply(g.v[e], c[e], bia + w + e, r);
             }
-            if (c[e]) g.v[e] = apply(g.v[e], c[e], bia + w + e, r);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!(g.bits >> e & 1)) g.v[e] = -INFINITY;
+          if (y) store_group<ALIGNED>(y, g, t, a.vocab);
+          const float most = fmaxf(fmaxf(g.v[0], g.v[1]), fmaxf(g.v[2], g.v[3]));  // passes over NaN
+          if (most > bv) {
+            bv = most;
+            bt = t + (g.v[0] == most ? 0 : g.v[1] == most ? 1 : g.v[2] == most ? 2 : 3);
           }
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (!(g.bits >> e & 1)) g.v[e] = -INFINITY;
-        if (y) store_group<ALIGNED>(y, g, t, a.vocab);
-        const float most = fmaxf(fmaxf(g.v[0], g.v[1]), fmaxf(g.v[2], g.v[3]));  // passes over NaN
-        if (most > bv) {
-          bv = most;
-          bt = t + (g.v[0] == most ? 0 : g.v[1] == most ? 1 : g.v[2] == most ? 2 : 3);
+      }
+      // a lane without a logit above -inf (or only NaN): its first allowed token counts as -inf
+      if (bt < 0) {
+        for (int lc = part; lc < n_chunks && bt < 0; lc += parts) {
+          const int t = token_of(lc) - sh;
+          for (int e = 3; e >= 0; --e)
+            if (t + e >= 0 && t + e < a.vocab && (!mask || (mask[(t + e) >> 5] >> ((t + e) & 31) & 1))) bt = t + e;
         }
       }
+      // the warp's best: the greatest value, then the lowest token (-0 + 0 = +0: zeros tie)
+      const uint32_t bits = __float_as_uint(__fadd_rn(bv, 0.f)), ord = bt < 0 ? 0u : (bits & 0x80000000u) ? ~bits : bits | 0x80000000u;
+      const uint32_t top = __reduce_max_sync(0xffffffffu, ord);
+      const uint32_t tok = __reduce_min_sync(0xffffffffu, ord == top && bt >= 0 ? (uint32_t)bt : 0xffffffffu);
+      const unsigned long long key = top ? ((unsigned long long)top << 32) | ~tok : 0ull;
+      if (lane == 0 && key) atomicMax(&sm.key[q], key);
     }
-    // a lane without a logit above -inf (or only NaN): its first allowed token counts as -inf
-    if (bt < 0) {
-      for (int lc = part; lc < n_chunks && bt < 0; lc += parts) {
-        const int t = token_of(lc) - sh;
-        for (int e = 3; e >= 0; --e)
-          if (t + e >= 0 && t + e < a.vocab && (!mask || (mask[(t + e) >> 5] >> ((t + e) & 31) & 1))) bt = t + e;
-      }
-    }
-    // the warp's best: the greatest value, then the lowest token (-0 + 0 = +0: zeros tie)
-    const uint32_t bits = __float_as_uint(__fadd_rn(bv, 0.f)), ord = bt < 0 ? 0u : (bits & 0x80000000u) ? ~bits : bits | 0x80000000u;
-    const uint32_t top = __reduce_max_sync(0xffffffffu, ord);
-    const uint32_t tok = __reduce_min_sync(0xffffffffu, ord == top && bt >= 0 ? (uint32_t)bt : 0xffffffffu);
-    const unsigned long long key = top ? ((unsigned long long)top << 32) | ~tok : 0ull;
-    if (lane == 0 && key) atomicMax(&sm.key[q], key);
-  }
+  };
+  if (PROMPTED && pathed && sm.given)
+    rows(std::bool_constant<PROMPTED>());
+  else
+    rows(std::false_type());
   __syncthreads();
   if (gridDim.x > 1) {
     if (tid < m && sm.key[tid]) atomicMax(a.best + row0 + tid, sm.key[tid]);
@@ -346,9 +368,11 @@ constexpr size_t pick_smem(int n_chunks) { return (size_t)n_chunks * kStride * 4
 
 cudaError_t configure_pick_kernels() {
   const int smem = (int)pick_smem(kMaxChunks);
-  cudaError_t e = cudaFuncSetAttribute(pick_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(pick_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  return e;
+  for (auto* kernel : {pick_kernel<true, true>, pick_kernel<true, false>, pick_kernel<false, true>, pick_kernel<false, false>}) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 cudaError_t op_pick(const PickArgs& a, int sms, cudaStream_t st) {
@@ -378,7 +402,11 @@ cudaError_t op_pick(const PickArgs& a, int sms, cudaStream_t st) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, a.vocab % 4 == 0 ? pick_kernel<true> : pick_kernel<false>, a, log2k, n_chunks);
+  const bool prompted = a.seqs && a.prompt;
+  return cudaLaunchKernelEx(&cfg,
+                            a.vocab % 4 == 0 ? (prompted ? pick_kernel<true, true> : pick_kernel<true, false>)
+                                             : (prompted ? pick_kernel<false, true> : pick_kernel<false, false>),
+                            a, log2k, n_chunks);
 }
 
 }  // namespace dllm

@@ -42,7 +42,8 @@ struct PickArgs {
   float* out;           // [n][vocab] or null
   int32_t* tokens;      // [n]
   int n, vocab;
-  // token history of sequence s: tokens [hist_off[s], hist_off[s + 1]), the first prompt[s] of them given
+  // token history of sequence s: tokens [hist_off[s], hist_off[s + 1]), then a node's path; the first
+  // prompt[s] of them given
   const int32_t* hist;
   const int32_t* hist_off;
   const int32_t* prompt;

@@ -337,8 +337,9 @@ class KernelContext:
                    out: GpuBuffer | None = None, tokens: GpuBuffer | None = None) -> GpuBuffer:
         """One token per row of logits [n, vocab] under penalties for repeated tokens,
         biases and a grammar mask (dllm_pick_tokens); i32 [n], -1 where the mask allows
-        nothing. history: (tokens, offsets, prompt_lens or None); bias: (tokens, values,
-        offsets); `out` also receives the processed logits."""
+        nothing. history: (tokens, offsets, prompt_lens or None), with a tree the tokens
+        before each root, and prompt_lens may reach into the nodes' paths; bias: (tokens,
+        values, offsets); `out` also receives the processed logits."""
         if tokens is None:
             tokens = self.createI32(n, "picked")
         h, o = self._h, self._opt

@@ -448,7 +448,9 @@ class LeaderPipeline:
     def verify_tree(self, tree: DraftTree, draft, **rules) -> list[list[int]]:
         """One verification step of drafted trees (single node). draft: the nodes' tokens,
         node 0 of a sequence its last token, not yet in the cache. All nodes go through
-        one pass, each gets a token (`rules`: the keyword arguments of pickTokens), and
+        one pass, each gets a token (`rules`: the keyword arguments of pickTokens; a
+        history holds the tokens before node 0, and prompt_lens count node 0 where it is
+        the prompt's last token), and
         the longest path that the picks agree with is kept in the cache. Returns the new
         tokens of each sequence, at least one."""
         if not self.singleNode:

@@ -371,7 +371,8 @@ typedef struct dllm_pick {
   const dllm_buf* logits;          /* f32 [n, V] */
   const dllm_buf* history;         /* i32: tokens of all sequences; ids outside [0, V) are ignored */
   const dllm_buf* history_offsets; /* i32 [seqs + 1]: sequence s has [offsets[s], offsets[s + 1]) */
-  const dllm_buf* prompt_lens;     /* i32 [seqs]: leading tokens that were given, not generated; NULL: none */
+  const dllm_buf* prompt_lens;     /* i32 [seqs]: leading tokens that were given, not generated; NULL: none. Beyond
+                                      the history they are the first tokens of a node's path */
   const dllm_buf* penalties;       /* f32 [seqs, 3]: repetition, frequency, presence */
   const dllm_buf* bias_tokens;     /* i32: entries of all sequences; of a token listed twice the last one counts */
   const dllm_buf* bias_values;     /* f32 */
@@ -383,7 +384,8 @@ typedef struct dllm_pick {
   dllm_buf* tokens;                /* i32 [n]; may be `draft`, no other input */
 } dllm_pick;
 /* With c = occurrences of token t among the generated tokens of the row's history (a
- * node's history ends with the drafted tokens from its root to itself):
+ * node's history ends with the drafted tokens from its root to itself, so a root that
+ * is the sequence's last token is not in `history` itself):
  *   y = x > 0 ? x / repetition : x * repetition   where t occurs in the history
  *   y = y - frequency * c - presence              where c > 0
  *   y += bias; y = -inf where the mask forbids t

@@ -675,6 +675,40 @@ def test_pick_tree(dllm, v):
     ctx.close()
 
 
+@pytest.mark.parametrize("v", [1000, 4099, 50257])
+def test_pick_tree_whose_prompt_reaches_into_the_paths(dllm, v):
+    """prompt_lens counts over the history and the path: every node equals a row of its own
+    that has both as its history."""
+    ctx = make_ctx(dllm, vocab_size=v)
+    rng = np.random.default_rng(v)
+    trees = [bushy(rng, 20), chain(64), [-1, 0, 0], bushy(rng, 11, roots=3), [-1, 0], chain(5)]
+    hist = [list(map(int, rng.integers(0, 20, k))) for k in (30, 4, 0, 9, 7, 6)]
+    prompt = [31, 40, 2, 11, 2 ** 31 - 1, 6]  # nodes of depth 0; 36 levels; two; two; all; none
+    n = sum(map(len, trees))
+    seq_of = [s for s, t in enumerate(trees) for _ in t]
+    draft = rng.integers(0, 20, n)  # a path meets a token given and generated
+    whole, row0 = [], 0
+    for s, t in enumerate(trees):
+        for see in ancestors(t):
+            whole.append(hist[s] + [int(draft[row0 + j]) for j in np.flatnonzero(see)])
+        row0 += len(t)
+    x = (rng.standard_normal((n, v)) * 3).astype(np.float32)
+    pen = np.array([[1.3, 0.2, 0.1], [0.8, 0.5, 0.0], [1.1, 0.0, 0.7], [1.2, -0.3, 0.4], [1.5, 0.6, 0.2], [1.3, 0.2, 0.1]])
+
+    def pick(tokens, prompts, penalties, **kw):
+        offsets = np.concatenate([[0], np.cumsum([len(t) for t in tokens])])
+        out = ctx.createF32(x.size)
+        got = ctx.pickTokens(f32(ctx, x), n, out=out, penalties=f32(ctx, penalties),
+                             history=(i32(ctx, sum(tokens, [])), i32(ctx, offsets), i32(ctx, prompts)), **kw)
+        return ctx.readI32(got), ctx.readF32(out, out.n)
+
+    tree = ctx.draftTree([p for t in trees for p in t], [len(t) for t in trees])
+    got = pick(hist, prompt, pen, tree=tree, draft=i32(ctx, draft))
+    want = pick(whole, [prompt[s] for s in seq_of], pen[seq_of])
+    assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+    ctx.close()
+
+
 def test_pick_many_rows_and_a_vocabulary_beyond_one_chunk(dllm):
     """64 nodes share a history; 400003 tokens need several passes per slice."""
     ctx = make_ctx(dllm, vocab_size=400003, hidden_size=8)
@@ -919,3 +953,46 @@ def test_verify_tree_under_rules_and_batches(dllm, weights_cache):
         ld.verify_tree(tree, [1, 2, 3, 4, 5])
     ld.close()
     ctx.close()
+
+
+def test_verify_tree_under_penalties_picks_what_single_steps_pick(dllm, weights_cache):
+    """A prompt, then drafted steps with a history: the tokens are those of one pick per token
+    over the whole text. The first step's root is the prompt's last token, which was given: a
+    bias makes it the pick unless it counted as generated."""
+    cfg = oracle_cfg("tiny")
+    W = get_weights(weights_cache, "tiny", cfg)
+    prompt = [int(t) for t in synth.prompt_tokens(cfg, 9, seed=5)]
+    rep, freq, pres = 1.25, 0.4, 0.3
+    ctx, ld = build_leader(dllm, cfg, W, "f32")
+    pen = f32(ctx, [[rep, freq, pres]])
+    text, bias = list(prompt), None
+    row = ld.forward(ld.embedTokens(prompt), len(prompt), 0)
+    while len(text) < len(prompt) + 12:
+        x = ld.sampleLast(row, return_logits=True)[1]
+        if bias is None:
+            y = x.astype(np.float64)
+            seen = sorted(set(prompt))
+            y[seen] = np.where(y[seen] > 0, y[seen] / rep, y[seen] * rep)
+            lead = np.delete(y, prompt[-1]).max() - y[prompt[-1]]
+            bias = (i32(ctx, [prompt[-1]]), f32(ctx, [lead + (freq + pres) / 2]), i32(ctx, [0, 1]))
+        text.append(int(ctx.readI32(ctx.pickTokens(
+            f32(ctx, x), 1, history=(i32(ctx, text), i32(ctx, [0, len(text)]), i32(ctx, [len(prompt)])), penalties=pen,
+            bias=bias))[0]))
+        row = ld.forward(ld.embedTokens(text[-1:]), 1, len(text) - 1)
+    assert text[len(prompt)] == prompt[-1]
+    ctx2, ld2 = build_leader(dllm, cfg, W, "f32")
+    pen2, bias2 = f32(ctx2, [[rep, freq, pres]]), (i32(ctx2, [prompt[-1]]), f32(ctx2, ctx.readF32(bias[1], 1)), i32(ctx2, [0, 1]))
+    ld2.forward(ld2.embedTokens(prompt[:-1]), len(prompt) - 1, 0)
+    got = list(prompt)
+    while len(got) < len(text):
+        true = (text[len(got):len(got) + 3] + [1, 2, 3])[:3]
+        tree = ctx2.draftTree([-1, 0, 0, 2, 3])
+        new = ld2.verify_tree(tree, [got[-1], (true[0] + 1) % cfg.vocab_size] + true, penalties=pen2, bias=bias2,
+                              history=(i32(ctx2, got[:-1]), i32(ctx2, [0, len(got) - 1]), i32(ctx2, [len(prompt)])))
+        assert len(new) == 1 and len(new[0]) >= min(4, len(text) - len(got))
+        got += new[0]
+    assert got[:len(text)] == text
+    for x in (ld, ld2):
+        x.close()
+    ctx.close()
+    ctx2.close()
