@@ -10,8 +10,11 @@
 // Precision. q, p and the outputs are fp32 like every activation here, and the
 // products run on the tensor cores all the same: with a bf16 cache q and p are cut
 // into three bf16 terms (8 + 8 + 8 bits; the products with bf16 K and V are exact),
-// with an fp32 cache all four operands into two tf32 terms (11 + 11 bits, the low x
-// low product left out). The tensor core adds into its fp32 accumulator with
+// with an fp32 cache all four operands into two tf32 terms. q, K and V are cut (a
+// rounded high term could overflow), so that a low term is up to 2^-10 of its operand
+// and has its sign: the scores take all four products, since without low x low each
+// would be short by up to 2^-20 of itself. p, at most 1, is rounded: p_low v_low has
+// either sign, stays below 2^-21 of the product and is left out. The tensor core adds into its fp32 accumulator with
 // truncation, so long chains would drift towards zero by 2^-24 per step: the large
 // terms and the corrections have accumulators of their own, a block's p . V starts
 // from zero, and the sum over blocks is a rounded fp32 add in registers.
@@ -61,9 +64,14 @@ DLLM_DEV void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint3
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x = hi + lo, hi with 11 bits; lo is rounded to 11 bits by the conversion.
+// x = hi + lo, hi with 11 bits, cut; lo, the other 13, is rounded to 11 (2^-22 of x).
 DLLM_DEV void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
   hi = __float_as_uint(x) & 0xffffe000u;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+}
+// The same with hi rounded to nearest; not for values next to the largest number.
+DLLM_DEV void split_tf32_near(float x, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
 }
 
@@ -212,7 +220,15 @@ __global__ void __launch_bounds__(kTAThreads, 1) tree_attn_kernel(const __grid_c
 #pragma unroll
       for (int e = 0; e < 4; ++e) sh[i][e] = ss[i][e] = 0.f;
     if constexpr (F32) {
-#pragma unroll 4
+      // a chain of accumulators per product: one that takes several is waited for (16
+      // sequences x 2 nodes x 12 heads at 4000 slots 45 us with two chains for three
+      // products and loops of four, 41 so with four products)
+      float s1[NT][4], s2[NT][4];
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s1[i][e] = s2[i][e] = 0.f;
+#pragma unroll
       for (int ks = 0; ks < HD / 8; ++ks) {
         uint32_t qh[4], ql[4];
 #pragma unroll
@@ -228,11 +244,16 @@ __global__ void __launch_bounds__(kTAThreads, 1) tree_attn_kernel(const __grid_c
           for (int e = 0; e < 2; ++e)
             split_tf32(*reinterpret_cast<const float*>(sK + row * T::kRowBytes + (((ks * 2 + e) ^ (row & 7)) << 4) + t * 4),
                        kh[e], kl[e]);
+          mma_tf32(ss[nt], ql, kl[0], kl[1]);
           mma_tf32(sh[nt], qh, kh[0], kh[1]);
-          mma_tf32(ss[nt], qh, kl[0], kl[1]);
-          mma_tf32(ss[nt], ql, kh[0], kh[1]);
+          mma_tf32(s1[nt], qh, kl[0], kl[1]);
+          mma_tf32(s2[nt], ql, kh[0], kh[1]);
         }
       }
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ss[i][e] += s1[i][e] + s2[i][e];
     } else {
       const int arow = wr * 16 + (lane & 15);
       const uint32_t qa = smem_addr(sQ) + arow * HD * 2;
@@ -362,10 +383,10 @@ __global__ void __launch_bounds__(kTAThreads, 1) tree_attn_kernel(const __grid_c
       uint32_t ph[NT][4], pl[NT][4];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {  // slots 2t, 2t + 1 of a group take the places t, t + 4 of the product
-        split_tf32(sh[j][0], ph[j][0], pl[j][0]);
-        split_tf32(sh[j][2], ph[j][1], pl[j][1]);
-        split_tf32(sh[j][1], ph[j][2], pl[j][2]);
-        split_tf32(sh[j][3], ph[j][3], pl[j][3]);
+        split_tf32_near(sh[j][0], ph[j][0], pl[j][0]);
+        split_tf32_near(sh[j][2], ph[j][1], pl[j][1]);
+        split_tf32_near(sh[j][1], ph[j][2], pl[j][2]);
+        split_tf32_near(sh[j][3], ph[j][3], pl[j][3]);
       }
 #pragma unroll
       for (int i = 0; i < HD / 8; ++i) {

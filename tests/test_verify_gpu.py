@@ -346,6 +346,50 @@ def test_tree_attention_sharp_rows(dllm):
     P.close()
 
 
+def low_bits(x, bits=13):
+    return int(np.float32(x).view(np.uint32)) & ((1 << bits) - 1)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nq,m", [(2, 1), (16, 3)])  # tiles of 16 and of 32 rows
+def test_tree_attention_keeps_the_low_bits_of_q_and_k(dllm, hd, nq, m):
+    """An fp32 cache, two slots of equal weight per node: k and, scaled, q hold a leading one
+    and ones in their last 13 bits, which the tf32 tiles take as a second term. A node's own k
+    is the next number, whose second term is zero.
+
+    With z the score in powers of two (about 2^11), the scores differ by z 2^-23. Of what the
+    products lose, everything that is in proportion to k cancels between the slots (the cut of
+    q, the rounding of q's scale). What is left: the second term of k, 13 ones, is rounded to
+    11 bits, one step of 2^-23; both scores are summed from two accumulators, 2^-24 each. The
+    difference is off by d = z 2^-22 at most, the weights 1 / (1 + 2^-difference) by
+    d ln2 / 4, and V = 1, -1 counts that twice. p and the sum are off by the exponential's
+    2^-21 and roundings below it: 2^-19 covers them. Left out, the product of the two second
+    terms would shift one score by z 2^-20, four times d."""
+    P = Paged(dllm, nq, 2, hd, "f32", [1], [[-1] * m])
+    scale = np.float32(math.log2(math.e) / math.sqrt(hd))
+    target = np.float32(64 * (1 + 2.0 ** -10 - 2.0 ** -23))
+    near = (np.float32(target / scale).view(np.int32) + np.arange(-4, 5, dtype=np.int32)).view(np.float32)
+    q0 = max((c for c in near if c * scale <= target), key=lambda c: c * scale)
+    assert low_bits(q0 * scale) >= 0x1ffc and q0 * scale <= target
+    k0 = np.float32(32 * (1 + 2.0 ** -10 - 2.0 ** -23))
+    k1 = np.float32(32 * (1 + 2.0 ** -10))
+    assert low_bits(k0) == 0x1fff and low_bits(k1) == 0
+    for pool in P.pool:
+        pool.zero_()
+    page = int(P.table[0][0])
+    P.pool[0][0, page, :, 0, 0], P.pool[0][0, page, :, 1:1 + m, 0] = float(k0), float(k1)
+    P.pool[1][0, page, :, 0], P.pool[1][0, page, :, 1:1 + m] = 1.0, -1.0
+    torch_().cuda.synchronize()
+    q = np.zeros((m, nq, hd), np.float32)
+    q[:, :, 0] = q0
+    z = [float(q0) * float(k) / math.sqrt(hd) * math.log2(math.e) for k in (k0, k1)]
+    want = 2.0 / (1.0 + 2.0 ** (z[1] - z[0])) - 1.0
+    out = P.stage.tree_attention(0, P.tree, f32(P.ctx, q))
+    err = np.abs(P.ctx.readF32(out, out.n).astype(np.float64) - want).max()
+    assert err <= z[0] * 2.0 ** -22 * math.log(2) / 2 + 2.0 ** -19, (err, z[0] * 2.0 ** -20 * math.log(2) / 2)
+    P.close()
+
+
 @pytest.mark.parametrize("kv", ["bf16", "f32"])
 @pytest.mark.parametrize("nq", [2, 16])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
