@@ -2313,7 +2313,8 @@ int dllm_rope_plan_create(dllm_ctx* c, const dllm_rope_config* r, dllm_rope_plan
     double fr = std::pow(base, -2.0 * i / rd);
     if (r->scaling == DLLM_ROPE_LINEAR) fr /= r->factor;
     if (r->scaling == DLLM_ROPE_YARN) {
-      const double ramp = std::min(1.0, std::max(0.0, (i - lo) / (hi == lo ? 0.001 : hi - lo)));
+      // every pair beyond the ramp (hi < 0), or every pair before it (lo > rd - 1)
+      const double ramp = hi < lo ? i > hi : std::min(1.0, std::max(0.0, (i - lo) / (hi == lo ? 0.001 : hi - lo)));
       fr = fr / r->factor * ramp + fr * (1.0 - ramp);
     }
     turns[i] = fr / kTwoPi;

@@ -110,6 +110,28 @@ def test_rope_at(dllm, layout, hd, rd, scaling):
     ctx.close()
 
 
+@pytest.mark.parametrize("theta,original,turns", [(1e6, 4, "few"), (1e4, 1, "few"), (100.0, 2 ** 31 - 1, "many"),
+                                                  (1.5, 100000, "many")])
+def test_rope_at_yarn_without_a_ramp(dllm, theta, original, turns):
+    """Contexts in which every pair makes less than one turn (all of them are slow: divided by
+    the factor), or every pair more than 32 (all fast: as they are)."""
+    ctx = make_ctx(dllm, 4, 2, 64)
+    plan = ctx.ropePlan(theta=theta, scaling={"type": "yarn", "factor": 4.0, "original_max_pos": original})
+    f = theta ** (-np.arange(32, dtype=np.float64) / 32)
+    of = original * f / (2 * math.pi)
+    assert (of < 1).all() if turns == "few" else (of > 32).all()
+    rng = np.random.default_rng(1)
+    pos = rng.integers(0, 1 << 20, 5)
+    q = rng.standard_normal((5, 4, 64), np.float32)
+    b = f32(ctx, q)
+    ctx.ropeAt(plan, i32(ctx, pos), 5, b)
+    factor = 0.1 * math.log(4.0) + 1
+    want, mag = rope64(q, pos, 64, "half", f / 4.0 if turns == "few" else f, factor)
+    # as in test_rope_at
+    assert (np.abs(ctx.readF32(b, b.n).reshape(q.shape) - want) <= 9 * EPS * factor * mag).all()
+    ctx.close()
+
+
 def test_rope_at_one_of_q_and_k_and_far_positions(dllm):
     ctx = make_ctx(dllm, 4, 1, 128)
     plan = ctx.ropePlan(theta=1e4)
