@@ -68,6 +68,7 @@ PP = C.POINTER(C.c_void_p)
 SIGNATURES = {
     "dllm_version": (C.c_char_p, []),
     "dllm_status_string": (C.c_char_p, [C.c_int]),
+    "dllm_device_error_string": (C.c_char_p, [C.c_int]),
     "dllm_config_default": (None, [C.POINTER(dllm_config)]),
     "dllm_init_kernels": (C.c_int, [C.c_int, C.POINTER(dllm_config), PP]),
     "dllm_ctx_destroy": (None, [P]),

@@ -232,6 +232,20 @@ void dev_free(void* p) {
   if (p) cudaFree(p);
 }
 
+// What kernels leave in the error flag.
+struct DeviceError {
+  int code, status;
+  const char* text;
+};
+constexpr DeviceError kDeviceErrors[] = {
+    {dllm::kErrBarrier, DLLM_ETIMEOUT, "device grid barrier timed out"},
+    {dllm::kErrKvRange, DLLM_ERANGE, "KV slot out of range (T0 + n > max_pos)"},
+    {dllm::kErrToken, DLLM_EINVAL, "token id out of vocabulary range"},
+    {dllm::kErrTcWait, DLLM_ETIMEOUT, "tensor-core matmul: a pipeline wait timed out"},
+    {dllm::kErrPeerWait, DLLM_ETIMEOUT, "pipeline hop: the previous stage's rows did not arrive in time"},
+    {dllm::kErrTreeWait, DLLM_ETIMEOUT, "tree attention: a pipeline wait timed out"},
+};
+
 // Bounded wait for the ctx stream, then the device error flag. Mirrors the
 // 15 s timeout race of readF32 (kernels.js:201-207).
 int sync_check(dllm_ctx* c, int timeout_ms) {
@@ -253,12 +267,8 @@ int sync_check(dllm_ctx* c, int timeout_ms) {
   if (code != 0) {
     cudaMemsetAsync(c->err_dev, 0, sizeof(int), c->stream);
     cudaStreamSynchronize(c->stream);
-    if (code == dllm::kErrKvRange) return set_err(c, DLLM_ERANGE, "KV slot out of range (T0 + n > max_pos)");
-    if (code == dllm::kErrBarrier) return set_err(c, DLLM_ETIMEOUT, "device grid barrier timed out");
-    if (code == dllm::kErrToken) return set_err(c, DLLM_EINVAL, "token id out of vocabulary range");
-    if (code == dllm::kErrPeerWait)
-      return set_err(c, DLLM_ETIMEOUT, "pipeline hop: the previous stage's rows did not arrive in time");
-    if (code == dllm::kErrTcWait) return set_err(c, DLLM_ETIMEOUT, "tensor-core matmul: a pipeline wait timed out");
+    for (const DeviceError& d : kDeviceErrors)
+      if (d.code == code) return set_err(c, d.status, "%s", d.text);
     return set_err(c, DLLM_EDEVICE, "device error code %d", code);
   }
   return DLLM_OK;
@@ -892,6 +902,12 @@ const char* dllm_status_string(int s) {
     case DLLM_EDEVICE: return "device error";
     default: return "unknown status";
   }
+}
+
+const char* dllm_device_error_string(int code) {
+  for (const DeviceError& d : kDeviceErrors)
+    if (d.code == code) return d.text;
+  return code == 0 ? "ok" : "unknown device error";
 }
 
 void dllm_config_default(dllm_config* f) {

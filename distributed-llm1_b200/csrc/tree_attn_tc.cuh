@@ -7,8 +7,6 @@
 
 namespace dllm {
 
-constexpr int kErrWait = 5;  // the tensor-core wait code
-
 // q rows of the tile, scaled so that the softmax is in powers of two, as three bf16 planes
 // (highest terms first) of swizzled 64-dim boxes, what the K-major descriptor reads.
 // WORKERS threads, `me` the caller's number. Rows behind the last one stay as they are: a row

@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kTc32Threads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (tid == 0 && sh.abort) atomicExch(a.err, kErrWait);
+  if (tid == 0 && sh.abort) atomicExch(a.err, kErrTreeWait);
   if (warp == 8) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));

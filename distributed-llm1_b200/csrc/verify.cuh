@@ -14,6 +14,7 @@ namespace dllm {
 
 constexpr int kTreeMaxNodes = 64;  // nodes per sequence: one bit each of an ancestor mask
 constexpr int kTreeMaxSeqs = 128;  // sequences per tree: their T0s travel as kernel arguments
+constexpr int kErrTreeWait = 7;    // a tcgen05 attention kernel gave up waiting on an mbarrier
 
 // One sequence of a drafted tree: its nodes are rows [row0, row0 + m) of the batch.
 struct TreeSeq {

@@ -76,6 +76,8 @@ typedef struct dllm_leader dllm_leader;
 /* ---- library / context ----------------------------------------------------- */
 const char* dllm_version(void);
 const char* dllm_status_string(int status);
+/* Text of a code that a kernel left in an error flag (dllm_attention_noalloc_status). */
+const char* dllm_device_error_string(int code);
 /* Fills the Qwen2.5-1.5B defaults of constants.js:10-23 (max_pos 4096, fp32 KV). */
 void dllm_config_default(dllm_config* cfg);
 

@@ -2,6 +2,8 @@
 calls that are refused before anything reaches a GPU."""
 import ctypes as C
 import importlib
+import os
+import re
 
 import numpy as np
 import pytest
@@ -76,6 +78,21 @@ def test_null_handles_are_refused(dllm):
     assert not lib.dllm_stage_kv_device_ptr(None, 0)
     lib.dllm_tree_destroy(None)
     lib.dllm_rope_plan_destroy(None)
+
+
+def test_a_wait_that_ran_out_is_told_where_it_ran_out(dllm):
+    """Every kind of device error has a text of its own: the matmul's and the attention's waits too."""
+    lib = dllm.load_library()
+    csrc = os.path.join(os.path.dirname(dllm.LIB_PATH), "csrc")
+    codes = {}
+    for name in os.listdir(csrc):
+        for const, value in re.findall(r"constexpr int (kErr\w+) = (\d+);", open(os.path.join(csrc, name)).read()):
+            codes[const] = int(value)
+    assert len(codes) >= 6 and len(set(codes.values())) == len(codes), codes
+    texts = {const: lib.dllm_device_error_string(value).decode() for const, value in codes.items()}
+    assert len(set(texts.values())) == len(codes) and lib.dllm_device_error_string(99).decode() not in texts.values()
+    assert "matmul" in texts["kErrTcWait"]
+    assert "attention" in texts["kErrTreeWait"]
 
 
 def test_memory_of_freed_buffers_is_refused():
