@@ -653,7 +653,8 @@ cudaError_t launch_hd(const TreeAttnArgs& a, const TreeAttnShape& s, int sms, in
   if (rows <= 32) return launch<KT, HD, 2>(a, s, sms, launches, st);
   if constexpr (sizeof(KT) == 2) {
     long long blocks = 0;
-    for (int i = 0; i < a.n_seqs; ++i) blocks += (long long)((s.t0[i] + s.seqs[i].m + kTcBlock - 1) / kTcBlock) * a.kvh;
+    for (int i = 0; i < a.n_seqs; ++i)
+      if (s.seqs[i].m) blocks += (long long)((s.t0[i] + s.seqs[i].m + kTcBlock - 1) / kTcBlock) * a.kvh;
     if ((rows + 63) / 64 * blocks <= 2ll * sms) return launch<KT, HD, 4>(a, s, sms, launches, st);
   }
   return launch_split<HD>(a, s, kTcRows, kTcBlock, sms, launches, st, [&](const TAKernelArgs& P, dim3 grid) {

@@ -318,6 +318,19 @@ def test_tree_attention_batch(dllm, kv, page):
 
 
 @pytest.mark.parametrize("kv", ["bf16", "f32"])
+def test_tree_attention_idle_sequences_change_nothing(dllm, kv):
+    """A long sequence without nodes has no work, and does not move the others to another kernel."""
+    tree = bushy(np.random.default_rng(4), 9)
+    P = Paged(dllm, 8, 1, 64, kv, [2000, 9000], [tree, []])
+    q = f32(P.ctx, np.random.default_rng(5).standard_normal(9 * 8 * 64))
+    out = P.stage.tree_attention(0, P.tree, q)
+    alone = P.stage.tree_attention(0, P.ctx.draftTree(tree), q)
+    assert np.array_equal(P.ctx.readF32(out, out.n), P.ctx.readF32(alone, alone.n))
+    check_attention(P)
+    P.close()
+
+
+@pytest.mark.parametrize("kv", ["bf16", "f32"])
 @pytest.mark.parametrize("hd,nq,lens,m", [(128, 12, [8051, 6039], 55), (128, 12, [8051] * 3, 23),
                                           (64, 16, [7990, 8001, 5000, 6666], 40), (128, 16, [2001] * 16, 9)])
 def test_tree_attention_many_blocks_per_split(dllm, kv, hd, nq, lens, m):
