@@ -1078,6 +1078,7 @@ int dllm_write_i32(dllm_ctx* c, dllm_buf* b, const int32_t* src, size_t n) {
   if (int rc = check_i32(c, b, n, "writeI32")) return rc;
   if (!src && n) return set_err(c, DLLM_EINVAL, "writeI32: null source");
   if (int rc = use_device(c)) return rc;
+  if (int rc = refuse_capture(c, "writeI32")) return rc;  // a replay would read src again
   CK(c, cudaMemcpyAsync(b->ptr, src, n * 4, cudaMemcpyHostToDevice, c->stream));
   return DLLM_OK;
 }
@@ -1088,6 +1089,7 @@ int dllm_read_i32(dllm_ctx* c, const dllm_buf* b, int32_t* dst, size_t n) {
   if (int rc = check_i32(c, b, n, "readI32")) return rc;
   if (!dst) return set_err(c, DLLM_EINVAL, "readI32: null destination");
   if (int rc = use_device(c)) return rc;
+  if (int rc = refuse_capture(c, "readI32")) return rc;  // a replay would write dst again
   CK(c, cudaMemcpyAsync(dst, b->ptr, n * 4, cudaMemcpyDeviceToHost, c->stream));
   return sync_check(c, kDefaultTimeoutMs);
 }
@@ -1107,6 +1109,7 @@ int dllm_read_f32(dllm_ctx* c, const dllm_buf* b, float* dst, size_t n, const ch
   if (int rc = check_f32(c, b, n, "readF32")) return rc;
   if (!dst) return set_err(c, DLLM_EINVAL, "readF32: null destination");
   if (int rc = use_device(c)) return rc;
+  if (int rc = refuse_capture(c, "readF32")) return rc;  // its wait would fail, its copy stay in the graph
   CK(c, cudaMemcpyAsync(dst, b->ptr, n * 4, cudaMemcpyDeviceToHost, c->stream));
   int rc = sync_check(c, kDefaultTimeoutMs);
   if (rc == DLLM_ETIMEOUT)

@@ -330,9 +330,11 @@ int dllm_attention_noalloc_status(void* cuda_stream, int timeout_ms, int* device
  * every layer of a stage. All work is enqueued on the ctx stream, in order; scratch
  * belongs to the ctx, so calls of one ctx, and graphs captured from them, must not
  * overlap on the GPU. T0 values become kernel arguments: a captured call replays with
- * those of its capture, and refers to the buffers, trees and plans it was given. Not to
- * be captured: dllm_tree_create, dllm_rope_plan_create, dllm_stage_commit_tree and
- * dllm_stage_forward_tree. */
+ * those of its capture, and refers to the buffers, trees and plans it was given. Refused
+ * while the ctx stream is captured: dllm_tree_create, dllm_rope_plan_create,
+ * dllm_stage_commit_tree, dllm_stage_forward_tree, dllm_write_i32, dllm_read_i32 and
+ * dllm_read_f32. A captured dllm_write_f32 reads its source with every replay, and
+ * buffers are to be made before a capture. */
 
 typedef struct dllm_tree dllm_tree;
 typedef struct dllm_rope_plan dllm_rope_plan;

@@ -949,6 +949,33 @@ def test_on_a_side_stream_and_in_a_captured_graph(dllm):
     P.close()
 
 
+def test_host_copies_are_refused_in_a_capture(dllm):
+    """A graph would keep the host's address: replays would read and write memory that the host
+    has long given to something else. The capture itself stays good."""
+    torch = torch_()
+    ctx = make_ctx(dllm)
+    s = torch.cuda.Stream()
+    ctx.synchronize()
+    ctx.set_stream(s.cuda_stream)
+    ints, logits, toks = i32(ctx, [1, 2, 3]), f32(ctx, np.zeros(4096)), ctx.createI32(1)
+    x = np.zeros(4096, np.float32)
+    x[77] = 1.0
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        ctx.pickTokens(logits, 1, tokens=toks)
+        for call in (lambda: ctx.writeI32(ints, [4, 5, 6]), lambda: ctx.readI32(ints), lambda: ctx.readF32(logits, 4)):
+            with pytest.raises(dllm.DllmError, match="captured"):
+                call()
+    ctx.writeF32(logits, x)
+    with torch.cuda.stream(s):
+        g.replay()
+    assert list(ctx.readI32(toks)) == [77]
+    assert list(ctx.readI32(ints)) == [1, 2, 3]
+    del g
+    ctx.close()
+
+
 def test_two_runs_give_the_same_bits(dllm):
     P = Paged(dllm, 14, 2, 64, "f32", [3000], [bushy(np.random.default_rng(1), 40)])
     q = f32(P.ctx, np.random.default_rng(2).standard_normal(40 * 14 * 64))
