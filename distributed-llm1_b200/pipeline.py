@@ -464,7 +464,7 @@ class LeaderPipeline:
         k.writeI32(tok, draft)
         h, logits = k.createF32(tree.n * k.D, "tree rows"), k.createF32(tree.n * cfg.vocab_size, "tree logits")
         self.stage.forward_tree(tree, h, tok, logits)
-        picked = k.readI32(k.pickTokens(logits, tree.n, tree=tree, draft=tok, **rules))
+        picked = k.readI32(k.pickTokens(logits, tree.n, tree=tree, draft=tok, **rules), tree.n)
         paths, new = tree.accept(draft, picked)
         self.stage.commit_tree(tree, paths)
         return new

@@ -1102,3 +1102,18 @@ def test_verify_tree_under_penalties_picks_what_single_steps_pick(dllm, weights_
         x.close()
     ctx.close()
     ctx2.close()
+
+
+def test_verify_tree_into_buffers_of_the_caller(dllm, weights_cache):
+    """`tokens` and `out` of pickTokens may be larger than the tree."""
+    cfg = oracle_cfg("tiny")
+    ctx, ld = build_leader(dllm, cfg, get_weights(weights_cache, "tiny", cfg), "f32")
+    tree, draft = ctx.draftTree([-1, 0, 1]), [3, 4, 5]
+    want = ld.verify_tree(tree, draft)
+    ld.stage.reset()
+    toks, out = ctx.createI32(7), ctx.createF32(5 * cfg.vocab_size)
+    assert ld.verify_tree(tree, draft, tokens=toks, out=out) == want
+    assert ld.stage.T0 == len(want[0])
+    assert list(ctx.readI32(toks)[3:]) == [0] * 4
+    ld.close()
+    ctx.close()
