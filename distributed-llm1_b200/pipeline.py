@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import weakref
 from array import array
 
 import numpy as np
@@ -134,7 +135,7 @@ class _KvPool:
         f = stage.k.cfg
         if not stage.handle:
             raise ValueError("the stage has been closed")
-        self.stage = stage  # keeps the memory alive
+        self.stage, self.owner = stage, stage._owner()  # keep the memory alive
         self.__cuda_array_interface__ = {
             "shape": (stage.end - stage.start, f.max_seqs * stage.pages_per_seq(), f.num_kv_heads, f.kv_page_size,
                       f.head_dim),
@@ -152,8 +153,9 @@ class _KvLayer:
 class Stage:
     """Runs a contiguous block of decoder layers, resumable with its own KV cache."""
 
-    def __init__(self, kctx: KernelContext, start: int, end: int, _handle: int | None = None):
+    def __init__(self, kctx: KernelContext, start: int, end: int, _handle: int | None = None, _owner=lambda: None):
         self.k = kctx
+        self._owner = _owner  # the leader whose stage this is, if it is one: it holds the cache
         self.lib = kctx.lib
         self.start, self.end = start, end
         self._owned = _handle is None
@@ -324,7 +326,8 @@ class LeaderPipeline:
         h = C.c_void_p()
         kctx._check(self.lib.dllm_leader_create(kctx.handle, myRange[0], myRange[1], C.byref(h)), "LeaderPipeline")
         self.handle = h.value
-        self.stage = Stage(kctx, myRange[0], myRange[1], _handle=self.lib.dllm_leader_stage(self.handle))
+        self.stage = Stage(kctx, myRange[0], myRange[1], _handle=self.lib.dllm_leader_stage(self.handle),
+                           _owner=weakref.ref(self))
         self.stages = stages or [{"id": self.myId, "start": myRange[0], "end": myRange[1]}]
         self.stagesTail = [s for s in self.stages if s["id"] != self.myId]
         self.singleNode = len(self.stagesTail) == 0 and myRange[1] >= kctx.cfg.num_layers

@@ -1,6 +1,7 @@
 """Host side of verifying drafted tokens: the greedy acceptance of a tree, and the
 calls that are refused before anything reaches a GPU."""
 import ctypes as C
+import gc
 import importlib
 import os
 import re
@@ -151,3 +152,40 @@ def test_objects_of_another_kind_are_refused(dllm):
                 ctx.ropeAt(wrong, buf, 2, buf)
     finally:  # the handles are made up
         buf.handle = tree.handle = plan.handle = stage.handle = None
+
+
+class LeaderLibrary:
+    """A library whose leader lives at made-up addresses."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append(name)
+            if name.endswith("_create"):
+                args[-1]._obj.value = 16
+            return {"dllm_leader_stage": 32, "dllm_stage_kv_device_ptr": 4096, "dllm_stage_pages_per_seq": 2}.get(name, 0)
+        return call
+
+
+def test_a_pool_keeps_the_leader_of_its_stage(dllm):
+    """A leader frees its stage's cache when it goes; a pool in use must not lose it."""
+    ctx = object.__new__(kernels.KernelContext)
+    ctx.lib, ctx.handle, ctx.cfg = LeaderLibrary(), None, dllm.CFG
+    leader = dllm.LeaderPipeline(ctx, (0, 1))
+    pool = leader.stage.kv_pool("k")
+    assert pool.__cuda_array_interface__["data"][0] == 4096
+    del leader
+    gc.collect()
+    assert "dllm_leader_destroy" not in ctx.lib.calls
+    del pool
+    gc.collect()
+    assert ctx.lib.calls.count("dllm_leader_destroy") == 1
+    # without a pool nothing holds a leader
+    leader = dllm.LeaderPipeline(ctx, (0, 1))
+    stage = leader.stage
+    del leader
+    assert ctx.lib.calls.count("dllm_leader_destroy") == 2 and stage.handle is None
+    with pytest.raises(ValueError):
+        stage.kv_pool("v")
