@@ -425,6 +425,54 @@ def test_tree_attention_keeps_the_low_bits_of_q_and_k(dllm, hd, nq, m):
     P.close()
 
 
+@pytest.mark.parametrize("kv,operand", [("bf16", "q"), ("f32", "q"), ("f32", "k")])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nq,m,t0", [(2, 1, 1), (16, 3, 1), (16, 5, 1), (16, 16, 1), (16, 16, 4800)])  # every kernel
+def test_tree_attention_operands_keep_their_last_bits(dllm, kv, operand, hd, nq, m, t0):
+    """One context slot and a node's own slot of nearly equal scores z of about 2^11 (in powers
+    of two); all others have a score of 0 and no weight. One operand of the first score is
+    1 + 2^-9 and ones in its last 5 bits, its counterpart 1 + 2^-9: an operand that is held in
+    19 bits, or in two bf16 terms, shifts the first score by z 2^-18.
+
+    A score may lose: the rounding of q's scale, z 2^-24; the last bits of q and k, z 2^-22 each
+    where two tf32 terms hold them; the sum of its parts in fp32, rounded or cut, z 2^-24 twice:
+    10 z 2^-24, and the two scores' difference twice that. V = 1, -1 makes it half that times
+    ln2 in the output; 2^-19 covers the exponential and the quotient."""
+    trees = [[-1] * m]
+    P = Paged(dllm, nq, 2, hd, kv, [t0], trees)
+    scale = np.float32(math.log2(math.e) / math.sqrt(hd))
+
+    def unscaled(x):  # the float whose scaled value comes nearest to x
+        c = (np.float32(x / scale).view(np.int32) + np.arange(-4, 5, dtype=np.int32)).view(np.float32)
+        return min(c, key=lambda y: abs(float(y * scale) - float(x)))
+
+    full, short = (np.float32(1 + 2.0 ** -9 + last) for last in (2.0 ** -18 - 2.0 ** -23, 0.0))
+    assert low_bits(full, 14) == 0x1f and low_bits(short, 14) == 0
+    if operand == "q":  # q in two dims, each slot has one of them
+        q01, k0, k1 = (unscaled(64 * full), unscaled(64 * short)), (32.0, 0.0), (0.0, 32.0)
+        assert low_bits(q01[0] * scale, 5) >= 0x1d
+    else:
+        q01, k0, k1 = (unscaled(np.float32(64)), np.float32(0)), (float(32 * full), 0.0), (float(32 * short), 0.0)
+    for pool in P.pool:
+        pool.zero_()
+    slot = lambda j: (int(P.table[0][j // 64]), j % 64)  # noqa: E731
+    for j, k, v in [(0, k0, 1.0)] + [(t0 + i, k1, -1.0) for i in range(m)]:
+        page, row = slot(j)
+        P.pool[0][0, page, :, row, 0], P.pool[0][0, page, :, row, 1] = k
+        P.pool[1][0, page, :, row] = v
+    torch_().cuda.synchronize()
+    q = np.zeros((m, nq, hd), np.float32)
+    q[:, :, 0], q[:, :, 1] = q01
+    z = [(float(q01[0]) * k[0] + float(q01[1]) * k[1]) / math.sqrt(hd) * math.log2(math.e) for k in (k0, k1)]
+    want = 2.0 / (1.0 + 2.0 ** (z[1] - z[0])) - 1.0
+    out = P.stage.tree_attention(0, P.tree, f32(P.ctx, q))
+    err = np.abs(P.ctx.readF32(out, out.n).astype(np.float64) - want).max()
+    bound = z[0] * 20 * 2.0 ** -24 * math.log(2) / 2 + 2.0 ** -19
+    assert bound < 0.5 * z[0] * 2.0 ** -18 * math.log(2) / 2  # a lost term is well outside
+    assert err <= bound, (err, bound)
+    P.close()
+
+
 @pytest.mark.parametrize("kv", ["bf16", "f32"])
 @pytest.mark.parametrize("nq", [2, 16])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
