@@ -394,9 +394,10 @@ cudaError_t op_pick(const PickArgs& a, int sms, cudaStream_t st) {
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  // A cluster costs two cluster barriers (about 2 us): worth it from about 8000 tokens per
-  // history (one row over 1500 tokens 6.2 us without, 8.8 with; 64 nodes over 32000
-  // 45 without, 39 with).
+  // A cluster costs two cluster barriers: worth it from about 8000 tokens per history
+  // (launches back to back: one row over 1500 tokens takes 2.6 us more with them; 64 nodes
+  // over 32000 take 39 us, 45 without). The histories' lengths are on the device: the rule
+  // takes the buffer's.
   attr[0].val.clusterDim.x = a.hist_total / a.n_seqs >= kSharedHistory ? std::min(kCluster, 1 << log2k) : 1;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;

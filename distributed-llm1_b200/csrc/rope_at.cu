@@ -6,8 +6,10 @@
 // pass. A pair is (i, i + rotary / 2) in the half layout and (2i, 2i + 1) in the
 // interleaved one. The angle is reduced in 64 bits: pos * inv_freq / 2 pi is taken
 // in turns, whole turns are dropped, and only the remaining half turn goes to
-// sincospif in 32 bits. A 32-bit product would be off by pos * 2^-24 radians
-// (0.06 at position 10^6); this form stays within 2^-52 * turns of the angle.
+// sincospif in 32 bits. A 32-bit product would be off by pos * 2^-24 radians (0.06 at
+// position 10^6). Here the angle is off by two parts: the frequency and its product with
+// the position are rounded to 64 bits, about 2^-52 of the whole turns, and what is left of
+// a turn to 32, at most pi 2^-25 radians at any position.
 //
 // Bound by memory (8 bytes per element moved, ~1 flop per byte). A thread owns kVec pairs
 // of one head position and keeps their cos and sin in registers while it walks the heads

@@ -24,11 +24,17 @@
 // descriptor with the dims as the contiguous ("MN") direction.
 // Bound: per pair 24 MMAs of 128 x 128 x 16 from shared memory (65 cycles) and 48 of 128 x 64
 // x 16 with A in tensor memory (33): 3150 cycles, 0.82 us per block of 64 slots, against 0.74
-// us for its 64 x 512 bytes at one SM's share of HBM. Measured 2150 cycles per block (64 nodes
-// x 7 heads at 32000 slots): the scores' MMAs read 126 of the 128 bytes that shared memory
-// gives per cycle, so every barrier and every tensor-memory store of the softmax waits behind
-// them, and a group's chain of softmax, P, O becomes the limit. (Scores block by block, 24
-// MMAs of N = 64, and O whole: 2565 cycles; a second issuing warp for O: 2240.)
+// us for its 64 x 512 bytes at one SM's share of HBM. Measured with clock stamps, 64 nodes x
+// 7 heads at 32000 slots, 56 blocks per CTA, cold cache: 2370 cycles per block between the
+// first S and the last O (1575 of MMAs), 10 500 cycles until the first S (1900 of them to set
+// up barriers and tensor memory, the rest the first copies and the cut of q) and 10 000 from
+// the last O to the end: 87, 7 and 6 % of the kernel. In the loop the scores' MMAs read 126
+// of the 128 bytes that shared memory gives per cycle, so every barrier and every
+// tensor-memory store of the softmax waits behind them, and a group's chain of softmax, P, O
+// becomes the limit. (Scores block by block, 24 MMAs of N = 64, and O whole: a fifth more per
+// block; a second issuing warp for O: 4 %.) With two blocks per CTA (13 nodes x 6 heads at 8191 slots)
+// start, loop and end take 10 400, 9700 and 9300 cycles. The softmax threads spill 64 bytes
+// at HD = 128.
 #include "tree_attn_tc.cuh"
 
 namespace dllm {

@@ -16,12 +16,14 @@
 // while S(n + 1) runs. Tensor memory: S 2 x 64, P 2 x 96, O 128 columns.
 // Bound: per block 48 MMAs of 128 x 64 x 16 (49 cycles) and 24 of 128 x 128 x 16 (65): 3900
 // cycles, 2.0 us, against 1.5 us for 64 slots x 1024 bytes at one SM's share of HBM. Measured
-// 6500 cycles per block: the MMAs, the converters and the copies share 128 bytes of shared
-// memory per cycle, and V(n) waits for O(n - 1) before it is converted. The upper terms of q
-// in tensor memory with two sets of K planes made a block shorter (6000 cycles) but cost as
-// much at the start; several loads per converter thread in flight only held the MMAs up
+// with clock stamps, 8 sequences x 7 nodes x 6 heads, six blocks per CTA, cold cache: 6050 cycles
+// per block between the first S and the last O, 10 400 until the first S and 8700 from the last O
+// to the end (66, 19 and 15 % of the kernel). In the loop the MMAs, the converters and the copies
+// share 128 bytes of shared memory per cycle, and V(n) waits for O(n - 1) before it is
+// converted. The upper terms of q in tensor memory with two sets of K planes made a block 8 %
+// shorter but cost as much at the start; several loads per converter thread in flight only held the MMAs up
 // (64 nodes x 7 heads at 32000 slots: 221 us one at a time, 241 two). The mma.sync kernel with
-// tf32 terms takes 16000 cycles per block for 64 rows.
+// tf32 terms takes 16000 cycles per block for 64 rows. 112 bytes are spilled at HD = 128.
 #include "tree_attn_tc.cuh"
 
 namespace dllm {

@@ -454,8 +454,9 @@ class LeaderPipeline:
         one pass, each gets a token (`rules`: the keyword arguments of pickTokens; a
         history holds the tokens before node 0, and prompt_lens count node 0 where it is
         the prompt's last token), and
-        the longest path that the picks agree with is kept in the cache. Returns the new
-        tokens of each sequence, at least one."""
+        the path that the picks agree with (DraftTree.accept) is kept in the cache. Returns
+        the new tokens of each sequence, one more than its path has nodes below node 0 (none
+        for a sequence without nodes); the last is -1 where the mask allows nothing."""
         if not self.singleNode:
             raise _lib.DllmError(_lib.DLLM_EINVAL, "verify_tree: the leader's stage must own every layer (single node)")
         k, cfg = self.k, self.k.cfg

@@ -318,16 +318,18 @@ int dllm_attention_noalloc_status(void* cuda_stream, int timeout_ms, int* device
 
 /* ---- verification of drafted tokens --------------------------------------------
  * No counterpart in the reference, which decodes one token per pass. A draft
- * proposes a tree of tokens per sequence; one pass scores all nodes, and the
- * longest path that the model agrees with is kept:
+ * proposes a tree of tokens per sequence; one pass scores all nodes, and a path
+ * that the model agrees with is kept:
  *   dllm_tree_create         the trees' shape
  *   dllm_rope_at             q and k at the nodes' positions, T0 + depth
  *   dllm_stage_append_tree   K/V rows of the nodes, behind the cached context
  *   dllm_stage_tree_attention  every node over the context and its own ancestors
  *   dllm_pick_tokens         one token per node under penalties, biases and a mask
  *   dllm_stage_commit_tree   keep a path's K/V rows, T0 += its length
- * dllm_stage_forward_tree runs the first four (with the layers' projections) for
- * every layer of a stage. All work is enqueued on the ctx stream, in order; scratch
+ * dllm_stage_forward_tree is the whole pass for a stage's layers: projections, the
+ * config's rotary positions (as in dllm_stage_forward: whole heads, half layout, no
+ * scaling), the nodes' K/V rows and their attention. The parts serve hosts with layers
+ * of their own, dllm_rope_at those with other rotary positions. All work is enqueued on the ctx stream, in order; scratch
  * belongs to the ctx, so calls of one ctx, and graphs captured from them, must not
  * overlap on the GPU. T0 values become kernel arguments: a captured call replays with
  * those of its capture, and refers to the buffers, trees and plans it was given. Refused
