@@ -90,14 +90,24 @@ class RopePlan:
             pass
 
 
+def int32s(values, what: str) -> np.ndarray:
+    """Integers as a flat int32 array; numbers that do not fit, or are no integers, are refused."""
+    a = np.asarray(values).reshape(-1)
+    b = a.astype(np.int32) if a.dtype.kind in "iu" or not a.size else None
+    if b is None or (a != b).any():
+        raise _lib.DllmError(_lib.DLLM_EINVAL, f"{what}: need 32-bit integers")
+    return b
+
+
 class DraftTree:
     """Drafted trees of one or more sequences (dllm_tree_create). Freed with the object."""
 
     def __init__(self, ctx: "KernelContext", parents, counts=None, seqs=None):
         self.ctx, self.handle = ctx, None
-        self.parents = np.array(parents, dtype=np.int32).reshape(-1)
-        self.counts = np.array([self.parents.size] if counts is None else counts, dtype=np.int32).reshape(-1)
-        self.seqs = np.array(range(self.counts.size) if seqs is None else seqs, dtype=np.int32).reshape(-1)
+        self.parents = int32s(parents, "draftTree parents")
+        n = self.parents.size
+        self.counts = np.array([n], np.int32) if counts is None else int32s(counts, "draftTree counts")
+        self.seqs = np.arange(self.counts.size, dtype=np.int32) if seqs is None else int32s(seqs, "draftTree seqs")
         if self.seqs.size != self.counts.size or (self.counts < 0).any() or int(self.counts.sum()) != self.parents.size:
             raise _lib.DllmError(_lib.DLLM_EINVAL, f"draftTree: {self.parents.size} parents for counts "
                                                    f"{self.counts.tolist()} of sequences {self.seqs.tolist()}")

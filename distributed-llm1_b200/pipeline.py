@@ -18,7 +18,7 @@ import numpy as np
 
 from . import _lib, frames
 from .constants import FRAME
-from .kernels import DraftTree, GpuBuffer, KernelContext
+from .kernels import DraftTree, GpuBuffer, KernelContext, int32s
 
 
 # ---- assignLayers (pipeline.js:6-23) ---------------------------------------------------
@@ -461,7 +461,7 @@ class LeaderPipeline:
             raise _lib.DllmError(_lib.DLLM_EINVAL, "verify_tree: the leader's stage must own every layer (single node)")
         k, cfg = self.k, self.k.cfg
         k._h(tree, DraftTree)
-        draft = np.ascontiguousarray(draft, dtype=np.int32).reshape(-1)
+        draft = int32s(draft, "verify_tree")
         if draft.size != tree.n or draft.size == 0 or draft.min() < 0 or draft.max() >= cfg.vocab_size:
             raise _lib.DllmError(_lib.DLLM_EINVAL, f"verify_tree: need {tree.n} token ids in [0, {cfg.vocab_size})")
         tok = k.createI32(tree.n, "draft")

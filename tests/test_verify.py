@@ -56,6 +56,26 @@ def test_tree_counts_are_checked(dllm, parents, counts, seqs):
         kernels.DraftTree(None, parents, counts, seqs)
 
 
+@pytest.mark.parametrize("bad", [2 ** 32, -2 ** 32 - 1, 2 ** 31])
+def test_numbers_beyond_32_bits_are_refused(dllm, bad):
+    """An int64 array must not turn into other parents, counts, sequences or tokens."""
+    for args in (([-1, bad], None, None), ([-1], [bad + 1], None), ([-1], [1], [bad])):
+        with pytest.raises(dllm.DllmError):
+            kernels.DraftTree(None, *(a if a is None else np.array(a, np.int64) for a in args))
+    ctx = object.__new__(kernels.KernelContext)
+    ctx.lib, ctx.handle, ctx.cfg = NoLibrary(), None, dllm.CFG
+    leader = object.__new__(dllm.LeaderPipeline)
+    leader.k, leader.lib, leader.singleNode, leader.handle = ctx, ctx.lib, True, None
+    tree = bare_tree([-1, 0], [2])
+    tree.handle = 8
+    try:
+        for draft in (np.array([1, bad], np.int64), np.array([1.0, 2.5])):
+            with pytest.raises(dllm.DllmError):
+                leader.verify_tree(tree, draft)
+    finally:  # the handle is made up
+        tree.handle = None
+
+
 def test_rope_plan_names_are_checked(dllm):
     for kw in ({"layout": "spiral", "scaling": None}, {"layout": "half", "scaling": {"type": "cubic"}},
                {"layout": "half", "scaling": {"type": "linear", "factor": 2.0, "speed": 3}}):
