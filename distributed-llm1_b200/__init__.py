@@ -9,8 +9,8 @@ package is the host-side mirror of the reference's JavaScript interface.
 """
 from . import _lib, constants, frames, net, tokenizer, weights
 from .constants import CFG, FRAME, PRESETS, ModelConfig
-from .kernels import DraftTree, GpuBuffer, KernelContext, RopePlan, initKernels, init_kernels
-from .pipeline import LeaderPipeline, LocalTransport, Stage, assignLayers, assign_layers, handle_stage_frame, plan_stages
+from .kernels import DraftTree, GpuBuffer, KernelContext, RopePlan, RowBatch, initKernels, init_kernels
+from .pipeline import Cache4, LeaderPipeline, LocalTransport, Stage, assignLayers, assign_layers, handle_stage_frame, plan_stages
 from .weights import bf16BitsToF32, bf16BytesToF32Bits, load_checkpoint, reinterpretBits, tensorsForLayers
 from ._lib import DllmError, KvOverflowError
 from .net import FrameServer, TcpTransport, serve_stage

@@ -153,6 +153,22 @@ SIGNATURES = {
     "dllm_stage_commit_tree": (C.c_int, [P, P, P, P]),
     "dllm_stage_forward_tree": (C.c_int, [P, P, P, P, P]),
     "dllm_stage_kv_device_ptr": (P, [P, C.c_int]),
+    "dllm_norm_rope_at": (C.c_int, [P, P, P, C.c_int, P, P, P, P, P, P]),
+    "dllm_rows_create": (C.c_int, [P, I32P, I32P, C.c_int, PP]),
+    "dllm_rows_destroy": (None, [P]),
+    "dllm_stage_append_rows": (C.c_int, [P, C.c_int, P, P, P]),
+    "dllm_stage_window_attention": (C.c_int, [P, C.c_int, P, P, P, C.c_int, C.c_int]),
+    "dllm_kv4_create": (C.c_int, [P, C.c_int, C.c_int, PP]),
+    "dllm_kv4_destroy": (None, [P]),
+    "dllm_kv4_reset": (C.c_int, [P]),
+    "dllm_kv4_get_t0": (C.c_int, [P, C.c_int]),
+    "dllm_kv4_set_t0": (C.c_int, [P, C.c_int, C.c_int]),
+    "dllm_kv4_pages_per_seq": (C.c_int, [P]),
+    "dllm_kv4_set_page_table": (C.c_int, [P, C.c_int, I32P, C.c_int]),
+    "dllm_kv4_bytes": (C.c_size_t, [P]),
+    "dllm_kv4_append": (C.c_int, [P, C.c_int, P, P, P]),
+    "dllm_kv4_read_rows": (C.c_int, [P, C.c_int, P, P, P]),
+    "dllm_kv4_attention": (C.c_int, [P, C.c_int, P, P, P, C.c_int, C.c_int]),
     "dllm_attention_noalloc": (C.c_int, [P, P, P, P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, P]),
     "dllm_attention_noalloc_status": (C.c_int, [P, C.c_int, I32P]),
 }

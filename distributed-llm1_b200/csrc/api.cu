@@ -22,6 +22,7 @@
 #include "gemm_tc.cuh"
 #include "kernels.cuh"
 #include "ops.cuh"
+#include "rows_attn.cuh"
 #include "stage.cuh"
 #include "tc.cuh"
 #include "verify.cuh"
@@ -40,9 +41,12 @@ constexpr int kMaxSplitsAlloc = dllm::kAttnMaxSplits;  // attention splits per (
 #endif
 constexpr int kPrefetchBytes = DLLM_PREFETCH_BYTES;  // per-CTA L2 prefetch budget between phases
 
-// Buffers, trees and rope plans are opaque pointers to their callers: the first word tells
+constexpr int kMostRows = 1 << 20;  // of a row batch
+
+// Buffers, trees, rope plans and the like are opaque pointers to their callers: the first word tells
 // which of them a pointer is, so that one in the place of another is refused.
-enum Kind : uint32_t { kBuf = 0x64627566, kTree = 0x64747265, kRopePlan = 0x64726f70 };
+enum Kind : uint32_t { kBuf = 0x64627566, kTree = 0x64747265, kRopePlan = 0x64726f70, kRows = 0x64726f77,
+                      kCache4 = 0x646b7634 };
 
 }  // namespace
 
@@ -84,6 +88,8 @@ struct dllm_ctx {
   size_t tc_scratch_bytes = 0;
   // partial results of split tree attention, sized for any call; allocated with the first tree
   float* tree_part = nullptr;
+  // partial results of split attention of rows, sized for any call; allocated with the first batch
+  float* rows_part = nullptr;
   // token picks: per-row keys, then arrival counters (zero between calls)
   unsigned long long* pick_best = nullptr;
   // freed buffers kept for reuse, by size in bytes
@@ -150,6 +156,28 @@ struct dllm_tree {
   dllm_buf* dev = nullptr;          // TreeSeq[n_seqs], then ancestor masks u64[n]
   const dllm::TreeSeq* seqs_dev() const { return (const dllm::TreeSeq*)dev->ptr; }
   const unsigned long long* anc_dev() const { return (const unsigned long long*)(seqs_dev() + n_seqs); }
+};
+
+// Rows of a batch: counts[i] of sequence seqs[i], one after the other.
+struct dllm_rows {
+  const Kind kind = kRows;
+  dllm_ctx* ctx = nullptr;
+  int n = 0;
+  std::vector<int> seqs, counts;
+};
+
+// A paged cache in 4 bits. Row (layer, page, head, slot) has HD / 2 bytes of codes and HD / 32
+// (scale, minimum) pairs, each in an array of its own.
+struct dllm_kv4 {
+  const Kind kind = kCache4;
+  dllm_ctx* ctx = nullptr;
+  int start = 0, end = 0;
+  int log2_page = 6, pages_per_seq = 0, max_seqs = 1, max_slots = 0;
+  size_t layer_rows = 0;
+  unsigned char* codes[2] = {nullptr, nullptr};  // K, V
+  uint32_t* pairs[2] = {nullptr, nullptr};
+  int* page_table = nullptr;
+  std::vector<int> T0;
 };
 
 struct dllm_rope_plan {
@@ -244,6 +272,7 @@ constexpr DeviceError kDeviceErrors[] = {
     {dllm::kErrTcWait, DLLM_ETIMEOUT, "tensor-core matmul: a pipeline wait timed out"},
     {dllm::kErrPeerWait, DLLM_ETIMEOUT, "pipeline hop: the previous stage's rows did not arrive in time"},
     {dllm::kErrTreeWait, DLLM_ETIMEOUT, "tree attention: a pipeline wait timed out"},
+    {dllm::kErrRowsWait, DLLM_ETIMEOUT, "attention of rows: a pipeline wait timed out"},
 };
 
 // Bounded wait for the ctx stream, then the device error flag. Mirrors the
@@ -737,6 +766,126 @@ int tree_attention(dllm_stage* s, int layer, const dllm_tree* tree, const dllm::
   return DLLM_OK;
 }
 
+// The arguments that dllm_rope_at and dllm_norm_rope_at share, checked.
+int rope_args(dllm_ctx* c, const char* what, const dllm_rope_plan* p, const dllm_buf* positions, int n, dllm_buf* q,
+              dllm_buf* k, dllm_buf* q_out, dllm_buf* k_out, dllm::RopeAtArgs* out) {
+  if (!p || p->kind != kRopePlan || p->ctx != c) return set_err(c, DLLM_EINVAL, "%s: null or foreign plan", what);
+  if (n <= 0) return set_err(c, DLLM_EINVAL, "%s: invalid n=%d", what, n);
+  if (!q && !k) return set_err(c, DLLM_EINVAL, "%s: neither q nor k given", what);
+  if ((!q && q_out) || (!k && k_out)) return set_err(c, DLLM_EINVAL, "%s: an output without its input", what);
+  const dllm_config& f = c->cfg;
+  const size_t QD = (size_t)f.num_q_heads * f.head_dim, KD = (size_t)f.num_kv_heads * f.head_dim;
+  if (!q_out) q_out = q;
+  if (!k_out) k_out = k;
+  if (int rc = check_i32(c, positions, n, (std::string(what) + " positions").c_str())) return rc;
+  if (q) {
+    if (int rc = check_f32(c, q, n * QD, (std::string(what) + " q").c_str())) return rc;
+    if (int rc = check_f32(c, q_out, n * QD, (std::string(what) + " qOut").c_str())) return rc;
+  }
+  if (k) {
+    if (int rc = check_f32(c, k, n * KD, (std::string(what) + " k").c_str())) return rc;
+    if (int rc = check_f32(c, k_out, n * KD, (std::string(what) + " kOut").c_str())) return rc;
+  }
+  if (q && k && (q_out == k_out || q_out == k || k_out == q))
+    return set_err(c, DLLM_EINVAL, "%s: q and k must not share a buffer", what);
+  *out = dllm::RopeAtArgs{};
+  dllm::RopeAtArgs& a = *out;
+  if (q) a.q = (const float*)q->ptr, a.q_out = (float*)q_out->ptr, a.q_heads = f.num_q_heads;
+  if (k) a.k = (const float*)k->ptr, a.k_out = (float*)k_out->ptr, a.k_heads = f.num_kv_heads;
+  a.pos = (const int32_t*)positions->ptr;
+  a.turns = (const double*)p->turns->ptr;
+  a.n = n;
+  a.hd = f.head_dim;
+  a.rotary = p->rotary;
+  a.interleaved = p->interleaved;
+  a.factor = p->factor;
+  return DLLM_OK;
+}
+
+// The pages of one sequence into its line of a page table.
+int set_pages(dllm_ctx* c, int* page_table, int max_seqs, int pages_per_seq, int seq, const int32_t* pages, int n_pages) {
+  if (!pages || n_pages != pages_per_seq)
+    return set_err(c, DLLM_EINVAL, "set_page_table: need exactly %d pages", pages_per_seq);
+  const int total = max_seqs * pages_per_seq;
+  std::vector<char> seen(total, 0);
+  for (int i = 0; i < n_pages; ++i) {
+    if (pages[i] < 0 || pages[i] >= total || seen[pages[i]])
+      return set_err(c, DLLM_EINVAL, "set_page_table: page %d invalid or repeated", pages[i]);
+    seen[pages[i]] = 1;
+  }
+  if (int rc = use_device(c)) return rc;
+  if (int rc = refuse_capture(c, "set_page_table")) return rc;
+  CK(c, cudaMemcpyAsync(page_table + (size_t)seq * pages_per_seq, pages, (size_t)n_pages * 4, cudaMemcpyHostToDevice,
+                        c->stream));
+  CK(c, cudaStreamSynchronize(c->stream));
+  return DLLM_OK;
+}
+
+// ---- batches of rows ------------------------------------------------------------------------
+// The places of a batch's rows in a cache whose sequences have T0 slots, with room behind.
+int rows_batch(dllm_ctx* c, const dllm_rows* rows, const std::vector<int>& T0, int max_slots, const char* what,
+               dllm::RowsBatch* b) {
+  if (!rows || rows->kind != kRows || rows->ctx != c) return set_err(c, DLLM_EINVAL, "%s: null or foreign row batch", what);
+  b->n_seqs = 0;
+  int row0 = 0;
+  for (size_t i = 0; i < rows->seqs.size(); ++i) {
+    const int id = rows->seqs[i], m = rows->counts[i];
+    if (id >= (int)T0.size()) return set_err(c, DLLM_EINVAL, "%s: invalid seq %d", what, id);
+    if ((long long)T0[id] + m > max_slots)
+      return set_err(c, DLLM_ERANGE, "%s: seq %d T0=%d + %d rows > maxPos=%d", what, id, T0[id], m, max_slots);
+    if (m == 0) continue;
+    const int k = b->n_seqs++;
+    b->seq[k] = id, b->row0[k] = row0, b->m[k] = m, b->t0[k] = T0[id];
+    row0 += m;
+  }
+  return DLLM_OK;
+}
+
+dllm::RowPages stage_pages(const dllm_stage* s) {
+  return dllm::RowPages{s->page_table, s->log2_page, s->pages_per_seq, s->ctx->cfg.num_kv_heads};
+}
+dllm::RowPages kv4_pages(const dllm_kv4* v) {
+  return dllm::RowPages{v->page_table, v->log2_page, v->pages_per_seq, v->ctx->cfg.num_kv_heads};
+}
+bool valid_kv4(const dllm_kv4* v) { return v && v->kind == kCache4; }
+void* kv4_codes(const dllm_kv4* v, int which, int layer) {
+  return v->codes[which] + (size_t)(layer - v->start) * v->layer_rows * (v->ctx->cfg.head_dim / 2);
+}
+uint32_t* kv4_pairs(const dllm_kv4* v, int which, int layer) {
+  return v->pairs[which] + (size_t)(layer - v->start) * v->layer_rows * (v->ctx->cfg.head_dim / dllm::kGroup4);
+}
+
+// Attention of a batch's rows: `a` holds the cache, the rest is filled in here.
+int rows_attention(dllm_ctx* c, const char* what, dllm::RowsAttnArgs& a, const dllm::RowsBatch& b, int n, int kind,
+                   const dllm_buf* q, dllm_buf* out, int window, int sinks) {
+  const dllm_config& f = c->cfg;
+  const size_t QD = (size_t)f.num_q_heads * f.head_dim;
+  if (window < 0 || sinks < 0) return set_err(c, DLLM_EINVAL, "%s: window=%d, sinks=%d", what, window, sinks);
+  if (int rc = check_f32(c, q, n * QD, what)) return rc;
+  if (int rc = check_f32(c, out, n * QD, what)) return rc;
+  if (q == out) return set_err(c, DLLM_EINVAL, "%s: out must not be q", what);
+  if (int rc = use_device(c)) return rc;
+  a.q = (const float*)q->ptr;
+  a.out = (float*)out->ptr;
+  a.nq = f.num_q_heads;
+  a.window = window ? window : 0x7fffffff;
+  a.sinks = sinks;
+  a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)f.head_dim));
+  a.err = c->err_dev;
+  a.part_o = c->rows_part;
+  a.part_ml = c->rows_part + dllm::rows_attn_part_rows(c->sms) * f.head_dim;
+  int launches = 0;
+  const cudaError_t e = dllm::op_rows_attention(a, b, kind, f.head_dim, c->sms, &launches, c->stream);
+  c->launches += launches;
+  if (e != cudaSuccess) return set_err(c, DLLM_ECUDA, "%s launch: %s", what, cudaGetErrorString(e));
+  return DLLM_OK;
+}
+
+int kv4_layer(dllm_kv4* v, int layer, const char* what) {
+  if (layer < v->start || layer >= v->end) return set_err(v->ctx, DLLM_EINVAL, "%s: layer %d not in the cache", what, layer);
+  return DLLM_OK;
+}
+
 // A wide pass of n rows (rd[t] = {seq, pos, slot}) over the stage's layers, one
 // kernel per op: RMSNorm + q|k|v projections on the tensor cores, bias + RoPE +
 // appendKv, attention over the paged cache, o_proj + residual, RMSNorm + gate|up,
@@ -874,6 +1023,7 @@ void ctx_free(dllm_ctx* c) {
   dev_free(c->attn_rows);
   dev_free(c->tc_scratch);
   dev_free(c->tree_part);
+  dev_free(c->rows_part);
   dev_free(c->pick_best);
   for (auto& kv : c->buf_cache) cudaFree(kv.second);
   c->buf_cache.clear();
@@ -957,7 +1107,8 @@ int dllm_init_kernels(int device, const dllm_config* cfg, dllm_ctx** out) {
   if (prop.major < 10) return fail(DLLM_EDEVICE);  // built for sm_100a only
   c->sms = prop.multiProcessorCount;
   if (dllm::configure_stage_kernels() != cudaSuccess || dllm::configure_op_kernels() != cudaSuccess ||
-      dllm::configure_pick_kernels() != cudaSuccess || dllm::configure_tree_attn() != cudaSuccess) {
+      dllm::configure_pick_kernels() != cudaSuccess || dllm::configure_tree_attn() != cudaSuccess ||
+      dllm::configure_rows_attn() != cudaSuccess) {
     cudaGetLastError();
     return fail(DLLM_ECUDA);
   }
@@ -1631,20 +1782,7 @@ int dllm_stage_set_page_table(dllm_stage* s, int seq, const int32_t* pages, int 
   if (!s) return DLLM_EINVAL;
   dllm_ctx* c = s->ctx;
   if (seq < 0 || seq >= s->max_seqs) return set_err(c, DLLM_EINVAL, "set_page_table: invalid seq %d", seq);
-  if (!pages || n_pages != s->pages_per_seq)
-    return set_err(c, DLLM_EINVAL, "set_page_table: need exactly %d pages", s->pages_per_seq);
-  const int total = s->max_seqs * s->pages_per_seq;
-  std::vector<char> seen(total, 0);
-  for (int i = 0; i < n_pages; ++i) {
-    if (pages[i] < 0 || pages[i] >= total || seen[pages[i]])
-      return set_err(c, DLLM_EINVAL, "set_page_table: page %d invalid or repeated", pages[i]);
-    seen[pages[i]] = 1;
-  }
-  if (int rc = use_device(c)) return rc;
-  CK(c, cudaMemcpyAsync(s->page_table + (size_t)seq * s->pages_per_seq, pages, (size_t)n_pages * 4,
-                        cudaMemcpyHostToDevice, c->stream));
-  CK(c, cudaStreamSynchronize(c->stream));
-  return DLLM_OK;
+  return set_pages(c, s->page_table, s->max_seqs, s->pages_per_seq, seq, pages, n_pages);
 }
 
 int dllm_stage_pages_per_seq(const dllm_stage* s) { return s ? s->pages_per_seq : -1; }
@@ -2361,36 +2499,9 @@ void dllm_rope_plan_destroy(dllm_rope_plan* p) {
 int dllm_rope_at(dllm_ctx* c, const dllm_rope_plan* p, const dllm_buf* positions, int n, dllm_buf* q, dllm_buf* k,
                  dllm_buf* q_out, dllm_buf* k_out) {
   if (!c) return DLLM_EINVAL;
-  if (!p || p->kind != kRopePlan || p->ctx != c) return set_err(c, DLLM_EINVAL, "ropeAt: null or foreign plan");
-  if (n <= 0) return set_err(c, DLLM_EINVAL, "ropeAt: invalid n=%d", n);
-  if (!q && !k) return set_err(c, DLLM_EINVAL, "ropeAt: neither q nor k given");
-  if ((!q && q_out) || (!k && k_out)) return set_err(c, DLLM_EINVAL, "ropeAt: an output without its input");
-  const dllm_config& f = c->cfg;
-  const size_t QD = (size_t)f.num_q_heads * f.head_dim, KD = (size_t)f.num_kv_heads * f.head_dim;
-  if (!q_out) q_out = q;
-  if (!k_out) k_out = k;
-  if (int rc = check_i32(c, positions, n, "ropeAt positions")) return rc;
-  if (q) {
-    if (int rc = check_f32(c, q, n * QD, "ropeAt q")) return rc;
-    if (int rc = check_f32(c, q_out, n * QD, "ropeAt qOut")) return rc;
-  }
-  if (k) {
-    if (int rc = check_f32(c, k, n * KD, "ropeAt k")) return rc;
-    if (int rc = check_f32(c, k_out, n * KD, "ropeAt kOut")) return rc;
-  }
-  if (q && k && (q_out == k_out || q_out == k || k_out == q))
-    return set_err(c, DLLM_EINVAL, "ropeAt: q and k must not share a buffer");
-  if (int rc = use_device(c)) return rc;
   dllm::RopeAtArgs a{};
-  if (q) a.q = (const float*)q->ptr, a.q_out = (float*)q_out->ptr, a.q_heads = f.num_q_heads;
-  if (k) a.k = (const float*)k->ptr, a.k_out = (float*)k_out->ptr, a.k_heads = f.num_kv_heads;
-  a.pos = (const int32_t*)positions->ptr;
-  a.turns = (const double*)p->turns->ptr;
-  a.n = n;
-  a.hd = f.head_dim;
-  a.rotary = p->rotary;
-  a.interleaved = p->interleaved;
-  a.factor = p->factor;
+  if (int rc = rope_args(c, "ropeAt", p, positions, n, q, k, q_out, k_out, &a)) return rc;
+  if (int rc = use_device(c)) return rc;
   CK(c, dllm::op_rope_at(a, c->sms, c->stream));
   c->launches += 1;
   return DLLM_OK;
@@ -2659,6 +2770,245 @@ int dllm_stage_forward_tree(dllm_stage* s, const dllm_tree* tree, dllm_buf* h, c
 
 void* dllm_stage_kv_device_ptr(const dllm_stage* s, int which) {
   return !s ? nullptr : which == 0 ? s->kpool : which == 1 ? s->vpool : nullptr;
+}
+
+// ---- long conversations -------------------------------------------------------------------------
+int dllm_norm_rope_at(dllm_ctx* c, const dllm_rope_plan* p, const dllm_buf* positions, int n, dllm_buf* q, dllm_buf* k,
+                      const dllm_buf* q_norm, const dllm_buf* k_norm, dllm_buf* q_out, dllm_buf* k_out) {
+  if (!c) return DLLM_EINVAL;
+  dllm::NormRopeArgs a{};
+  if (int rc = rope_args(c, "normRopeAt", p, positions, n, q, k, q_out, k_out, &a.rope)) return rc;
+  if (!q != !q_norm || !k != !k_norm) return set_err(c, DLLM_EINVAL, "normRopeAt: q and k come each with its norm");
+  if (q)
+    if (int rc = check_bf16(c, q_norm, c->cfg.head_dim, "normRopeAt qNorm")) return rc;
+  if (k)
+    if (int rc = check_bf16(c, k_norm, c->cfg.head_dim, "normRopeAt kNorm")) return rc;
+  if (int rc = use_device(c)) return rc;
+  if (q) a.q_norm = (const __nv_bfloat16*)q_norm->ptr;
+  if (k) a.k_norm = (const __nv_bfloat16*)k_norm->ptr;
+  a.eps = c->cfg.rms_norm_eps;
+  CK(c, dllm::op_norm_rope(a, c->sms, c->stream));
+  c->launches += 1;
+  return DLLM_OK;
+}
+
+int dllm_rows_create(dllm_ctx* c, const int32_t* counts, const int32_t* seqs, int n_seqs, dllm_rows** out) {
+  if (!c || !out) return DLLM_EINVAL;
+  *out = nullptr;
+  if (!counts || n_seqs < 1 || n_seqs > dllm::kRowsMaxSeqs)
+    return set_err(c, DLLM_EINVAL, "rowBatch: need 1..%d sequences", dllm::kRowsMaxSeqs);
+  long long n = 0;
+  for (int i = 0; i < n_seqs; ++i) {
+    const int id = seqs ? seqs[i] : i;
+    if (counts[i] < 0 || counts[i] > c->cfg.max_pos)
+      return set_err(c, DLLM_EINVAL, "rowBatch: %d rows of a sequence, need 0..%d", counts[i], c->cfg.max_pos);
+    if (id < 0) return set_err(c, DLLM_EINVAL, "rowBatch: invalid seq %d", id);
+    for (int j = 0; j < i; ++j)
+      if ((seqs ? seqs[j] : j) == id) return set_err(c, DLLM_EINVAL, "rowBatch: seq %d listed twice", id);
+    n += counts[i];
+  }
+  if (n < 1 || n > kMostRows) return set_err(c, DLLM_EINVAL, "rowBatch: %lld rows, need 1..%d", n, kMostRows);
+  if (int rc = use_device(c)) return rc;
+  if (int rc = refuse_capture(c, "rowBatch")) return rc;
+  if (!c->rows_part) {
+    if (int rc = dev_alloc(c, &c->rows_part, dllm::rows_attn_part_rows(c->sms) * (c->cfg.head_dim + 2), "row partials"))
+      return rc;
+    CK(c, cudaStreamSynchronize(c->stream));  // the stream may be another one by the first call
+  }
+  auto* r = new dllm_rows();
+  r->ctx = c;
+  r->n = (int)n;
+  for (int i = 0; i < n_seqs; ++i) r->seqs.push_back(seqs ? seqs[i] : i);
+  r->counts.assign(counts, counts + n_seqs);
+  ctx_retain(c);
+  *out = r;
+  return DLLM_OK;
+}
+
+void dllm_rows_destroy(dllm_rows* r) {
+  if (!r || r->kind != kRows) return;
+  ctx_release(r->ctx);
+  delete r;
+}
+
+int dllm_stage_append_rows(dllm_stage* s, int layer, const dllm_rows* rows, const dllm_buf* k, const dllm_buf* v) {
+  if (!s) return DLLM_EINVAL;
+  dllm_ctx* c = s->ctx;
+  const dllm_config& f = c->cfg;
+  dllm::RowsBatch b;
+  if (int rc = tree_layer(s, layer, "append_rows")) return rc;
+  if (int rc = rows_batch(c, rows, s->T0, s->max_slots, "append_rows", &b)) return rc;
+  const size_t KD = (size_t)f.num_kv_heads * f.head_dim;
+  if (int rc = check_f32(c, k, rows->n * KD, "append_rows k")) return rc;
+  if (int rc = check_f32(c, v, rows->n * KD, "append_rows v")) return rc;
+  if (int rc = use_device(c)) return rc;
+  CK(c, dllm::op_rows_append(b, rows->n, stage_pages(s), f.kv_dtype == DLLM_KV_F32 ? dllm::kKvF32 : dllm::kKvBf16, f.head_dim,
+                             (const float*)k->ptr, (const float*)v->ptr, layer_pool(s, s->kpool, layer),
+                             layer_pool(s, s->vpool, layer), nullptr, nullptr, c->stream));
+  c->launches += 1;
+  return DLLM_OK;
+}
+
+int dllm_stage_window_attention(dllm_stage* s, int layer, const dllm_rows* rows, const dllm_buf* q, dllm_buf* out,
+                                int window, int sinks) {
+  if (!s) return DLLM_EINVAL;
+  dllm_ctx* c = s->ctx;
+  dllm::RowsBatch b;
+  if (int rc = tree_layer(s, layer, "window_attention")) return rc;
+  if (int rc = rows_batch(c, rows, s->T0, s->max_slots, "window_attention", &b)) return rc;
+  dllm::RowsAttnArgs a{};
+  a.kc = layer_pool(s, s->kpool, layer);
+  a.vc = layer_pool(s, s->vpool, layer);
+  a.pages = stage_pages(s);
+  if (!s->kv_mapped) return set_err(c, DLLM_ECUDA, "window_attention: the driver has no tensor map of the KV cache");
+  a.tc_k = &s->kv_map[0];
+  a.tc_v = &s->kv_map[1];
+  a.tc_row0 = (int)((size_t)(layer - s->start) * s->layer_elems / c->cfg.head_dim);
+  return rows_attention(c, "window_attention", a, b, rows->n, c->cfg.kv_dtype == DLLM_KV_F32 ? dllm::kKvF32 : dllm::kKvBf16, q,
+                        out, window, sinks);
+}
+
+int dllm_kv4_create(dllm_ctx* c, int start, int end, dllm_kv4** out) {
+  if (!c || !out) return DLLM_EINVAL;
+  *out = nullptr;
+  const dllm_config& f = c->cfg;
+  if (start < 0 || end < start || end > f.num_layers)
+    return set_err(c, DLLM_EINVAL, "Cache4: invalid layer range [%d,%d) of %d", start, end, f.num_layers);
+  if (int rc = use_device(c)) return rc;
+  if (int rc = refuse_capture(c, "Cache4")) return rc;
+  auto* v = new dllm_kv4();
+  v->ctx = c;
+  ctx_retain(c);
+  v->start = start, v->end = end;
+  v->log2_page = ilog2(f.kv_page_size);
+  v->pages_per_seq = (f.max_pos + f.kv_page_size - 1) / f.kv_page_size;
+  v->max_seqs = f.max_seqs, v->max_slots = f.max_pos;
+  const size_t pages = (size_t)v->max_seqs * v->pages_per_seq;
+  v->layer_rows = pages * f.num_kv_heads * f.kv_page_size;
+  v->T0.assign(v->max_seqs, 0);
+  const size_t rows = v->layer_rows * (end - start);
+  int rc = pages > 0x7fffffff ? set_err(c, DLLM_EINVAL, "Cache4: %zu pages", pages) : DLLM_OK;
+  for (int i = 0; i < 2; ++i) {
+    if (!rc) rc = dev_alloc(c, &v->codes[i], rows * (f.head_dim / 2), "4-bit cache");
+    if (!rc) rc = dev_alloc(c, &v->pairs[i], rows * (f.head_dim / dllm::kGroup4), "4-bit cache scales");
+  }
+  if (!rc) rc = dev_alloc(c, &v->page_table, pages, "page table");
+  if (!rc) {
+    std::vector<int> pt(pages);
+    for (size_t i = 0; i < pages; ++i) pt[i] = (int)i;  // sequence-major identity map
+    cudaError_t e = cudaMemcpyAsync(v->page_table, pt.data(), pages * 4, cudaMemcpyHostToDevice, c->stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
+    if (e != cudaSuccess) rc = set_err(c, DLLM_ECUDA, "page table upload: %s", cudaGetErrorString(e));
+  }
+  if (rc) {
+    dllm_kv4_destroy(v);
+    return rc;
+  }
+  *out = v;
+  return DLLM_OK;
+}
+
+void dllm_kv4_destroy(dllm_kv4* v) {
+  if (!valid_kv4(v)) return;
+  dllm_ctx* c = v->ctx;
+  cudaSetDevice(c->device);
+  cudaStreamSynchronize(c->stream);
+  for (int i = 0; i < 2; ++i) {
+    dev_free(v->codes[i]);
+    dev_free(v->pairs[i]);
+  }
+  dev_free(v->page_table);
+  delete v;
+  ctx_release(c);
+}
+
+int dllm_kv4_reset(dllm_kv4* v) {
+  if (!valid_kv4(v)) return DLLM_EINVAL;
+  for (auto& t : v->T0) t = 0;
+  return DLLM_OK;
+}
+
+int dllm_kv4_get_t0(const dllm_kv4* v, int seq) {
+  return !valid_kv4(v) || seq < 0 || seq >= v->max_seqs ? -1 : v->T0[seq];
+}
+
+int dllm_kv4_set_t0(dllm_kv4* v, int seq, int t0) {
+  if (!valid_kv4(v)) return DLLM_EINVAL;
+  if (seq < 0 || seq >= v->max_seqs) return set_err(v->ctx, DLLM_EINVAL, "set_t0: invalid seq %d", seq);
+  if (t0 < 0 || t0 > v->max_slots) return set_err(v->ctx, DLLM_ERANGE, "set_t0: T0=%d outside [0,%d]", t0, v->max_slots);
+  v->T0[seq] = t0;
+  return DLLM_OK;
+}
+
+int dllm_kv4_pages_per_seq(const dllm_kv4* v) { return valid_kv4(v) ? v->pages_per_seq : -1; }
+
+int dllm_kv4_set_page_table(dllm_kv4* v, int seq, const int32_t* pages, int n_pages) {
+  if (!valid_kv4(v)) return DLLM_EINVAL;
+  dllm_ctx* c = v->ctx;
+  if (seq < 0 || seq >= v->max_seqs) return set_err(c, DLLM_EINVAL, "set_page_table: invalid seq %d", seq);
+  return set_pages(c, v->page_table, v->max_seqs, v->pages_per_seq, seq, pages, n_pages);
+}
+
+size_t dllm_kv4_bytes(const dllm_kv4* v) {
+  if (!valid_kv4(v)) return 0;
+  const int hd = v->ctx->cfg.head_dim;
+  return 2 * v->layer_rows * (v->end - v->start) * (hd / 2 + hd / dllm::kGroup4 * 4);
+}
+
+int dllm_kv4_append(dllm_kv4* v, int layer, const dllm_rows* rows, const dllm_buf* k, const dllm_buf* w) {
+  if (!valid_kv4(v)) return DLLM_EINVAL;
+  dllm_ctx* c = v->ctx;
+  const dllm_config& f = c->cfg;
+  dllm::RowsBatch b;
+  if (int rc = kv4_layer(v, layer, "append")) return rc;
+  if (int rc = rows_batch(c, rows, v->T0, v->max_slots, "append", &b)) return rc;
+  const size_t KD = (size_t)f.num_kv_heads * f.head_dim;
+  if (int rc = check_f32(c, k, rows->n * KD, "append k")) return rc;
+  if (int rc = check_f32(c, w, rows->n * KD, "append v")) return rc;
+  if (int rc = use_device(c)) return rc;
+  CK(c, dllm::op_rows_append(b, rows->n, kv4_pages(v), dllm::kKv4, f.head_dim, (const float*)k->ptr, (const float*)w->ptr,
+                             kv4_codes(v, 0, layer), kv4_codes(v, 1, layer), kv4_pairs(v, 0, layer), kv4_pairs(v, 1, layer),
+                             c->stream));
+  c->launches += 1;
+  return DLLM_OK;
+}
+
+int dllm_kv4_read_rows(dllm_kv4* v, int layer, const dllm_rows* rows, dllm_buf* k, dllm_buf* w) {
+  if (!valid_kv4(v)) return DLLM_EINVAL;
+  dllm_ctx* c = v->ctx;
+  const dllm_config& f = c->cfg;
+  dllm::RowsBatch b;
+  if (int rc = kv4_layer(v, layer, "read_rows")) return rc;
+  if (int rc = rows_batch(c, rows, v->T0, v->max_slots, "read_rows", &b)) return rc;
+  const size_t KD = (size_t)f.num_kv_heads * f.head_dim;
+  if (!k && !w) return set_err(c, DLLM_EINVAL, "read_rows: neither k nor v given");
+  if (k)
+    if (int rc = check_f32(c, k, rows->n * KD, "read_rows k")) return rc;
+  if (w)
+    if (int rc = check_f32(c, w, rows->n * KD, "read_rows v")) return rc;
+  if (k == w) return set_err(c, DLLM_EINVAL, "read_rows: k and v must not share a buffer");
+  if (int rc = use_device(c)) return rc;
+  CK(c, dllm::op_rows_read4(b, rows->n, kv4_pages(v), f.head_dim, kv4_codes(v, 0, layer), kv4_codes(v, 1, layer),
+                            kv4_pairs(v, 0, layer), kv4_pairs(v, 1, layer), k ? (float*)k->ptr : nullptr,
+                            w ? (float*)w->ptr : nullptr, c->stream));
+  c->launches += 1;
+  return DLLM_OK;
+}
+
+int dllm_kv4_attention(dllm_kv4* v, int layer, const dllm_rows* rows, const dllm_buf* q, dllm_buf* out, int window,
+                       int sinks) {
+  if (!valid_kv4(v)) return DLLM_EINVAL;
+  dllm_ctx* c = v->ctx;
+  dllm::RowsBatch b;
+  if (int rc = kv4_layer(v, layer, "attention")) return rc;
+  if (int rc = rows_batch(c, rows, v->T0, v->max_slots, "attention", &b)) return rc;
+  dllm::RowsAttnArgs a{};
+  a.kc = kv4_codes(v, 0, layer);
+  a.vc = kv4_codes(v, 1, layer);
+  a.ks = kv4_pairs(v, 0, layer);
+  a.vs = kv4_pairs(v, 1, layer);
+  a.pages = kv4_pages(v);
+  return rows_attention(c, "attention", a, b, rows->n, dllm::kKv4, q, out, window, sinks);
 }
 
 }  // extern "C"

@@ -49,6 +49,28 @@ DLLM_DEV void st_pack(float* p, const Pack<VEC>& r) {
     *p = r.v[0];
 }
 
+// Turns the VEC pairs of a unit.
+template <int VEC, bool INTER>
+DLLM_DEV void turn(Pack<VEC>& x, Pack<VEC>& y, const float (&c)[VEC], const float (&s)[VEC]) {
+  if constexpr (INTER && VEC == 4) {  // (x0 x1)(x2 x3) | (y0 y1)(y2 y3)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float x1 = x.v[2 * i], x2 = x.v[2 * i + 1], y1 = y.v[2 * i], y2 = y.v[2 * i + 1];
+      x.v[2 * i] = fmaf(x1, c[i], -(x2 * s[i]));
+      x.v[2 * i + 1] = fmaf(x1, s[i], x2 * c[i]);
+      y.v[2 * i] = fmaf(y1, c[2 + i], -(y2 * s[2 + i]));
+      y.v[2 * i + 1] = fmaf(y1, s[2 + i], y2 * c[2 + i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float x1 = x.v[i], x2 = y.v[i];
+      x.v[i] = fmaf(x1, c[i], -(x2 * s[i]));
+      y.v[i] = fmaf(x1, s[i], x2 * c[i]);
+    }
+  }
+}
+
 // A head has hd / (2 VEC) units of VEC pairs: the first rotary / (2 VEC) turn, the
 // rest are copied (or left, in place). Four pairs at a time (16-byte accesses)
 // need rotary to be a multiple of 8; other sizes go pair by pair, with U heads in flight
@@ -97,25 +119,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_at_kernel(const RopeAtArgs 
     for (int u = 0; u < U; ++u) {
       const int h = h0 + u * h_step;
       if (h >= heads) break;
-      if (turns) {
-        if constexpr (INTER && VEC == 4) {  // (x0 x1)(x2 x3) | (y0 y1)(y2 y3)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float x1 = x[u].v[2 * i], x2 = x[u].v[2 * i + 1], y1 = y[u].v[2 * i], y2 = y[u].v[2 * i + 1];
-            x[u].v[2 * i] = fmaf(x1, c[i], -(x2 * s[i]));
-            x[u].v[2 * i + 1] = fmaf(x1, s[i], x2 * c[i]);
-            y[u].v[2 * i] = fmaf(y1, c[2 + i], -(y2 * s[2 + i]));
-            y[u].v[2 * i + 1] = fmaf(y1, s[2 + i], y2 * c[2 + i]);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float x1 = x[u].v[i], x2 = y[u].v[i];
-            x[u].v[i] = fmaf(x1, c[i], -(x2 * s[i]));
-            y[u].v[i] = fmaf(x1, s[i], x2 * c[i]);
-          }
-        }
-      }
+      if (turns) turn<VEC, INTER>(x[u], y[u], c, s);
       const size_t o = at(row, h);
       float* dst = (h < a.q_heads ? a.q_out : a.k_out) + o;
       if (turns || dst != (h < a.q_heads ? a.q : a.k) + o) {
@@ -150,10 +154,109 @@ cudaError_t rope_hd(const RopeAtArgs& a, int sms, cudaStream_t st) {
   return a.interleaved ? launch_rope<HD, 1, 4, true>(a, sms, st) : launch_rope<HD, 1, 4, false>(a, sms, st);
 }
 
+// ---- norms of the heads, then the rotation ---------------------------------------------------
+// y = x * rsqrt(mean(x^2) + eps) * w for each head, then the rotation above, in one pass: a
+// head's HD / 8 threads (a warp, where pairs go one by one) hold it in registers, add their
+// squares in fp32 by shuffles, and turn it. Bound by memory like the rotation alone: the norm
+// adds 4 flops per element and one chain of shuffles, and saves a whole pass over q and k.
+template <int HD, int VEC, bool INTER>
+__global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const NormRopeArgs n, int log2_side) {
+  constexpr int units = HD / (2 * VEC), lanes = units < 32 ? units : 32, U = units / lanes, slots = kRopeThreads / lanes;
+  const RopeAtArgs& a = n.rope;
+  const int turning = a.rotary / (2 * VEC), heads = a.q_heads + a.k_heads;
+  const int lane = threadIdx.x % lanes, slot = threadIdx.x / lanes;
+  const int h_first = (blockIdx.y << log2_side) + (slot & ((1 << log2_side) - 1)), h_step = gridDim.y << log2_side;
+  const int row = blockIdx.x * (slots >> log2_side) + (slot >> log2_side);
+  if (row >= a.n) return;  // a head's threads leave together
+  const unsigned group = (lanes == 32 ? 0xffffffffu : (1u << (lanes & 31)) - 1) << (threadIdx.x % 32 - lane);
+  // float offsets of this thread's packs within a head
+  int o1[U], o2[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int unit = lane + u * lanes;
+    const bool turns = unit < turning;
+    o1[u] = turns ? (INTER ? unit * 2 * VEC : unit * VEC) : a.rotary + (unit - turning) * 2 * VEC;
+    o2[u] = turns ? (INTER ? o1[u] + VEC : o1[u] + a.rotary / 2) : o1[u] + VEC;
+  }
+  auto at = [&](int h) {
+    return h < a.q_heads ? ((size_t)row * a.q_heads + h) * HD : ((size_t)row * a.k_heads + (h - a.q_heads)) * HD;
+  };
+  Pack<VEC> x[U], y[U];
+  auto load = [&](int h) {
+    if (h >= heads) return;
+    const float* src = (h < a.q_heads ? a.q : a.k) + at(h);
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = ld_pack<VEC>(src + o1[u]), y[u] = ld_pack<VEC>(src + o2[u]);
+  };
+  load(h_first);  // on the way while the angles are computed
+  float c[U][VEC], s[U][VEC];
+  const double pos = (double)a.pos[row];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (lane + u * lanes >= turning) continue;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const double t = pos * a.turns[(lane + u * lanes) * VEC + i];
+      sincospif(2.0f * (float)(t - rint(t)), &s[u][i], &c[u][i]);
+      s[u][i] *= a.factor;
+      c[u][i] *= a.factor;
+    }
+  }
+  for (int h = h_first; h < heads; h += h_step) {
+    const __nv_bfloat16* w = h < a.q_heads ? n.q_norm : n.k_norm;  // 2 HD bytes, from L1
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) sum = fmaf(x[u].v[i], x[u].v[i], fmaf(y[u].v[i], y[u].v[i], sum));
+#pragma unroll
+    for (int d = lanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(group, sum, d);
+    const float r = rsqrtf(fmaf(sum, 1.f / HD, n.eps));
+    float* dst = (h < a.q_heads ? a.q_out : a.k_out) + at(h);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        x[u].v[i] *= r * bf16_to_f32(w[o1[u] + i]);
+        y[u].v[i] *= r * bf16_to_f32(w[o2[u] + i]);
+      }
+      if (lane + u * lanes < turning) turn<VEC, INTER>(x[u], y[u], c[u], s[u]);
+      st_pack<VEC>(dst + o1[u], x[u]);
+      st_pack<VEC>(dst + o2[u], y[u]);
+    }
+    load(h + h_step);
+  }
+}
+
+template <int HD, int VEC, bool INTER>
+cudaError_t launch_norm_rope(const NormRopeArgs& n, int sms, cudaStream_t st) {
+  constexpr int units = HD / (2 * VEC), slots = kRopeThreads / (units < 32 ? units : 32);
+  const RopeAtArgs& a = n.rope;
+  const int heads = a.q_heads + a.k_heads;
+  int log2_side = 0;
+  while ((1 << log2_side) < heads && (1 << log2_side) < slots) ++log2_side;
+  const int rows = slots >> log2_side, chunks = (heads + (1 << log2_side) - 1) >> log2_side;
+  const int ctas = (a.n + rows - 1) / rows;
+  const dim3 grid(ctas, (long long)ctas * chunks <= 8ll * sms ? chunks : 1);  // as above
+  norm_rope_kernel<HD, VEC, INTER><<<grid, kRopeThreads, 0, st>>>(n, log2_side);
+  return cudaGetLastError();
+}
+
+template <int HD>
+cudaError_t norm_rope_hd(const NormRopeArgs& n, int sms, cudaStream_t st) {
+  if (n.rope.rotary % 8 == 0)
+    return n.rope.interleaved ? launch_norm_rope<HD, 4, true>(n, sms, st) : launch_norm_rope<HD, 4, false>(n, sms, st);
+  return n.rope.interleaved ? launch_norm_rope<HD, 1, true>(n, sms, st) : launch_norm_rope<HD, 1, false>(n, sms, st);
+}
+
 }  // namespace
 
 cudaError_t op_rope_at(const RopeAtArgs& a, int sms, cudaStream_t st) {
   return a.hd == 64 ? rope_hd<64>(a, sms, st) : rope_hd<128>(a, sms, st);
+}
+
+cudaError_t op_norm_rope(const NormRopeArgs& n, int sms, cudaStream_t st) {
+  return n.rope.hd == 64 ? norm_rope_hd<64>(n, sms, st) : norm_rope_hd<128>(n, sms, st);
 }
 
 }  // namespace dllm

@@ -1,0 +1,922 @@
+// rows_attn.cu — attention of a batch of rows over a paged cache, few rows per sequence.
+//
+// A row at cache slot p sees the slots s <= p with s > p - window or s < sinks:
+//   out = sum_s p_s v_s,  p_s = exp(q . k_s / sqrt(hd) - max) / sum
+// The m rows of a sequence and the G query heads of a KV head make m G rows that share one
+// pass over that head's K and V; the softmax runs online over blocks of slots, blocks that
+// no row of the tile sees are not read, and the blocks of a tile are split over CTAs whose
+// partial results a second kernel joins.
+//
+// Precision. q, p and the outputs are fp32. bf16 and fp32 caches: q and p are cut into three
+// bf16 or two tf32 terms (tree_attn.cu has the reasons). 4-bit rows, value = middle + scale *
+// (code - 8) with middle = minimum + 8 scale:
+//   q . k = sum over groups of 32 dims of scale * (q . (code - 8)) + middle * (sum of q)
+//   o     = sum over slots of (p scale) (code - 8), + sum over slots of p middle
+// (With the minima and the codes themselves both sums are far larger than what they add up to:
+// over 8000 slots the outputs were off by 8e-6, and are by 7e-7.) Codes are exact in any 16-bit type, and the other operand runs as two fp16 terms (22 bits)
+// of fp32 values brought into fp16's range by a power of two: a row of q by one next to its
+// largest element, p scale by one next to the block's largest scale. A pair of codes becomes
+// fp16 as (nibbles | bits of 1024) - 1032. (The nibbles alone, read as fp16, are code * 2^-24,
+// but the tensor core aligns such subnormal products by their exponents, 10 bits above their
+// leading ones, and the sums lose as many: 4e-6 over 9 slots.) p meets the middles in bf16
+// terms, three of p and two of them.
+//
+// Work split. A CTA has 8 warps and takes 16 WR rows of one (sequence, KV head): WR warps
+// side by side in rows, 8 / WR of them in slots, each with a maximum, sum and output of its
+// own, joined at the end. K and V blocks come through a cp.async ring; slots behind the
+// tile's last row are zero-filled, never read.
+#include "rows_attn.cuh"
+
+#include <algorithm>
+#include <climits>
+#include <vector>
+
+#include "mma_sync.cuh"
+
+namespace dllm {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr float kNegInf = -INFINITY;
+
+DLLM_DEV void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+DLLM_DEV uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+DLLM_DEV void unpack_f16(uint32_t u, float& lo, float& hi) {
+  asm("{\n\t.reg .f16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}"
+      : "=f"(lo), "=f"(hi)
+      : "r"(u));
+}
+// (x, y) -> two packed fp16 pairs whose sums are x and y to 2^-22 of them, or to 2^-25.
+DLLM_DEV void split2_f16(float x, float y, uint32_t& h, uint32_t& l) {
+  h = pack_f16(x, y);
+  float a, b;
+  unpack_f16(h, a, b);
+  l = pack_f16(x - a, y - b);
+}
+// Nibbles 0 and 4 of u, less 8, as packed fp16.
+DLLM_DEV uint32_t codes_f16(uint32_t u) {
+  uint32_t r;
+  asm("{\n\t.reg .b32 t;\n\tlop3.b32 t, %1, 0x000f000f, 0x64006400, 0xea;\n\tsub.rn.f16x2 %0, t, %2;\n\t}"
+      : "=r"(r)
+      : "r"(u), "r"(0x64086408u));
+  return r;
+}
+DLLM_DEV float power_of_two(int biased) { return __uint_as_float((uint32_t)biased << 23); }
+DLLM_DEV void cp8_zfill(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(real ? 8 : 0) : "memory");
+}
+
+// Tile shapes. SN: slots of a block that one warp takes; BN: slots of a block. The ring
+// depth is what fits beside the q tile in 227 KB, four at most.
+template <int KIND, int HD, int WR>
+struct Tile {
+  static constexpr bool kF32 = KIND == kKvF32, kQ4 = KIND == kKv4;
+  static constexpr int WS = 8 / WR;
+  static constexpr int SN = kF32 ? 8 * WR : WR == 1 ? 16 : 32;
+  static constexpr int BN = SN * WS;
+  static constexpr int RT = 16 * WR;
+  static constexpr int kRowBytes = KvRow<KIND, HD>::kBytes;
+  static constexpr int kPairBytes = KvRow<KIND, HD>::kPairs * 4;
+  static constexpr int kChunks = kRowBytes / 16;
+  static constexpr int kRows = BN * kRowBytes, kTileBytes = kRows + BN * kPairBytes;  // one of K, V
+  static constexpr int kQBytes = kQ4 ? 0 : RT * HD * (kF32 ? 4 : 6);  // 4-bit rows: q lives in registers
+  static constexpr int kPad = HD + 4;
+  static constexpr int kMergeBytes = WS * RT * (kPad + 2) * 4;
+  static constexpr int kFit = (225 * 1024 - kQBytes) / (2 * kTileBytes);
+  static constexpr int kStages = kFit > 4 ? 4 : kFit;
+  static constexpr int kRing = kStages * 2 * kTileBytes;
+  static constexpr int kSmem = kQBytes + (kRing > kMergeBytes ? kRing : kMergeBytes);
+  static_assert(kStages >= 2 && kSmem <= 227 * 1024, "shared memory");
+  static_assert(BN % 32 == 0, "a page lookup serves 32 slots");
+};
+
+// Where 16-byte chunk c of a 4-bit K or V row lies: K is read by 8 slots at once (a word of one
+// chunk each), V by 4, both without bank conflicts.
+template <int HD, bool V>
+DLLM_DEV uint32_t at4(int row, int c) {
+  if constexpr (HD == 128)
+    return row * 64 + ((V ? c ^ (row >> 1 & 1) : c ^ (row >> 1 & 3)) << 4);
+  else
+    return row * 32 + ((V ? c : c ^ (row >> 2 & 1)) << 4);
+}
+
+template <int KIND, int HD, int WR>
+__global__ void __launch_bounds__(kThreads, 1) rows_attn_kernel(const __grid_constant__ RowsKernelArgs P) {
+  using T = Tile<KIND, HD, WR>;
+  constexpr int SN = T::SN, BN = T::BN, WS = T::WS, RT = T::RT, NT = SN / 8, CH = T::kChunks, S = T::kStages;
+  constexpr bool F32 = T::kF32, Q4 = T::kQ4;
+  constexpr int NG = HD / kGroup4;  // 4-bit rows: groups
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const RowsAttnArgs& a = P.a;
+  asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled; it waits for this grid's end
+  const RowsTile k(P, blockIdx.x, RT, BN);
+  if (k.split >= k.nsplit) return;
+  const int window = a.window, sinks = a.sinks, end = k.v.p1 + 1;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int wr = warp % WR, ws = warp / WR;
+  const int g = lane >> 2, t = lane & 3;
+  unsigned char* sQ = smem;
+  unsigned char* ring = smem + T::kQBytes;
+
+  // ---- K/V blocks through the ring. Pages hold at least 32 slots, so a block has BN / 32
+  // page lookups at most, made one block ahead of the copies that need them.
+  constexpr int kPages = BN / 32;
+  int page[kPages];
+  const int* table = a.pages.table + (size_t)k.seq * a.pages.max_pages;
+  const int log2_page = a.pages.log2_page, in_page = (1 << log2_page) - 1;
+  auto lookup = [&](int b) {
+    const int s0 = k.v.slot0(b, BN);
+#pragma unroll
+    for (int i = 0; i < kPages; ++i) page[i] = __ldg(table + (min(s0 + 32 * i, end - 1) >> log2_page));
+  };
+  auto row_of = [&](int s0, int row) {
+    int pg = page[0];
+#pragma unroll
+    for (int u = 1; u < kPages; ++u) pg = row >= 32 * u ? page[u] : pg;
+    return (((size_t)pg * a.pages.kvh + k.head) << log2_page) + ((s0 + row) & in_page);
+  };
+  auto copy = [&](int b, int stage) {
+    const int s0 = k.v.slot0(b, BN);
+    const uint32_t dk = smem_addr(ring + stage * 2 * T::kTileBytes), dv = dk + T::kTileBytes;
+    const unsigned char *kc = static_cast<const unsigned char*>(a.kc), *vc = static_cast<const unsigned char*>(a.vc);
+    constexpr int kPass = kThreads / CH;  // slots per pass
+    const int c = tid % CH;
+#pragma unroll
+    for (int i = 0; i < (BN + kPass - 1) / kPass; ++i) {
+      const int row = tid / CH + i * kPass;
+      if (BN % kPass && row >= BN) break;
+      const size_t off = row_of(s0, row) * T::kRowBytes + c * 16;
+      const bool real = s0 + row < end;
+      uint32_t ak, av;
+      if constexpr (Q4) ak = at4<HD, false>(row, c), av = at4<HD, true>(row, c);
+      else ak = av = row * T::kRowBytes + ((c ^ (row & 7)) << 4);
+      cp16_zfill(dk + ak, real ? kc + off : kc, real);
+      cp16_zfill(dv + av, real ? vc + off : vc, real);
+    }
+    if constexpr (Q4) {
+      static_assert(2 * BN <= kThreads, "a thread copies the pairs of one row");
+      const int row = tid % BN;
+      if (tid < 2 * BN) {
+        const bool real = s0 + row < end;
+        const uint32_t* src = (tid < BN ? a.ks : a.vs);
+        const uint32_t dst = (tid < BN ? dk : dv) + T::kRows + row * T::kPairBytes;
+        if (real) src += row_of(s0, row) * NG;
+        if constexpr (HD == 128) cp16_zfill(dst, src, real);
+        else cp8_zfill(dst, src, real);
+      }
+    }
+  };
+  lookup(k.b0);
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) {
+    if (k.b0 + s < k.b1) {
+      copy(k.b0 + s, s);
+      lookup(min(k.b0 + s + 1, k.b1 - 1));
+    }
+    cp_commit();
+  }
+
+  // this thread's two rows of the tile
+  const int ra = wr * 16 + g, rb = ra + 8;
+  const int pa = k.slot_of(k.r0 + ra), pb = k.slot_of(k.r0 + rb);
+
+  // ---- the q tile, scaled by log2(e) / sqrt(hd) so that the softmax is in powers of two
+  uint32_t qf[Q4 ? HD / 16 : 1][2][4];        // 4-bit rows: A fragments of two fp16 terms
+  float qsum_a[Q4 ? NG : 1], qsum_b[Q4 ? NG : 1], back_a = 1.f, back_b = 1.f;
+  if constexpr (Q4) {
+    // lane t of a row holds dims 8t .. 8t + 7 of every group: a u32 of codes
+    float xa[NG][8], xb[NG][8], ma = 0.f, mb = 0.f;
+    const float* qa = a.q + ((size_t)k.row0 * a.nq + (pa < 0 ? 0 : k.place(k.r0 + ra, a.nq))) * HD + t * 8;
+    const float* qb = a.q + ((size_t)k.row0 * a.nq + (pb < 0 ? 0 : k.place(k.r0 + rb, a.nq))) * HD + t * 8;
+#pragma unroll
+    for (int i = 0; i < NG; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 fa = pa < 0 ? z : *reinterpret_cast<const float4*>(qa + i * kGroup4 + e);
+        const float4 fb = pb < 0 ? z : *reinterpret_cast<const float4*>(qb + i * kGroup4 + e);
+        xa[i][e] = fa.x, xa[i][e + 1] = fa.y, xa[i][e + 2] = fa.z, xa[i][e + 3] = fa.w;
+        xb[i][e] = fb.x, xb[i][e + 1] = fb.y, xb[i][e + 2] = fb.z, xb[i][e + 3] = fb.w;
+      }
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      qsum_a[i] = qsum_b[i] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        xa[i][e] *= a.scale_log2, xb[i][e] *= a.scale_log2;
+        ma = fmaxf(ma, fabsf(xa[i][e])), mb = fmaxf(mb, fabsf(xb[i][e]));
+        qsum_a[i] += xa[i][e], qsum_b[i] += xb[i][e];
+      }
+    }
+#pragma unroll
+    for (int w = 1; w < 4; w <<= 1) {
+      ma = fmaxf(ma, __shfl_xor_sync(0xffffffffu, ma, w));
+      mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, w));
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        qsum_a[i] += __shfl_xor_sync(0xffffffffu, qsum_a[i], w);
+        qsum_b[i] += __shfl_xor_sync(0xffffffffu, qsum_b[i], w);
+      }
+    }
+    // 2^e next to the largest element: the row divided by it lies in [-2, 2]. The exponent is
+    // kept where 2^e and its inverse are normal numbers.
+    auto power = [](float m) { return min(max((int)(__float_as_uint(m) >> 23) & 0xff, 1), 253); };
+    const int ea = power(ma), eb = power(mb);
+    const float ia = power_of_two(254 - ea), ib = power_of_two(254 - eb);
+    back_a = power_of_two(ea), back_b = power_of_two(eb);
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) {
+      const int i = ks / 2, d = (ks & 1) * 2;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {  // dims d + u and d + u + 4: the two halves of a nibble pair
+        split2_f16(xa[i][d + u] * ia, xa[i][d + u + 4] * ia, qf[ks][0][2 * u], qf[ks][1][2 * u]);
+        split2_f16(xb[i][d + u] * ib, xb[i][d + u + 4] * ib, qf[ks][0][2 * u + 1], qf[ks][1][2 * u + 1]);
+      }
+    }
+  } else {
+    for (int i = tid; i < RT * HD / 4; i += kThreads) {
+      const int row = i / (HD / 4), d = (i % (HD / 4)) * 4;
+      const int r = k.r0 + row;
+      float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < k.R) {
+        f = *reinterpret_cast<const float4*>(a.q + ((size_t)k.row0 * a.nq + k.place(r, a.nq)) * HD + d);
+        f.x *= a.scale_log2, f.y *= a.scale_log2, f.z *= a.scale_log2, f.w *= a.scale_log2;
+      }
+      if constexpr (F32) {
+        *reinterpret_cast<float4*>(sQ + row * HD * 4 + (((d >> 2) ^ (row & 7)) << 4)) = f;
+      } else {
+        uint32_t h[2], m[2], l[2];
+        split3(f.x, f.y, h[0], m[0], l[0]);
+        split3(f.z, f.w, h[1], m[1], l[1]);
+        unsigned char* p = sQ + row * HD * 2 + (((d >> 3) ^ (row & 7)) << 4) + (d & 4) * 2;
+        *reinterpret_cast<uint2*>(p) = make_uint2(h[0], h[1]);
+        *reinterpret_cast<uint2*>(p + RT * HD * 2) = make_uint2(m[0], m[1]);
+        *reinterpret_cast<uint2*>(p + 2 * RT * HD * 2) = make_uint2(l[0], l[1]);
+      }
+    }
+  }
+
+  // 4-bit rows: o of a group is in units of `unit` (a power of two, the same in the whole warp),
+  // and om is the middles' share, by group
+  float o[HD / 8][4], om[4] = {0.f, 0.f, 0.f, 0.f}, unit[Q4 ? NG : 1];
+#pragma unroll
+  for (int i = 0; i < (Q4 ? NG : 1); ++i) unit[i] = 0.f;
+#pragma unroll
+  for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+  float ma = kNegInf, mb = kNegInf, la = 0.f, lb = 0.f;
+
+  // slot (within the block) of column c of this warp's score tile i. 4-bit rows: columns 2t and
+  // 2t + 1 are slots t and t + 4, so that a lane's four slots of 16 are the ones whose V rows
+  // it unpacks.
+  const int wslot = ws * SN;
+  auto slot_at = [&](int i, int e) {
+    return Q4 ? wslot + i * 8 + t + (e & 1) * 4 : wslot + i * 8 + 2 * t + (e & 1);
+  };
+
+  for (int b = k.b0; b < k.b1; ++b) {
+    cp_wait<S - 2>();
+    __syncthreads();
+    {
+      const int next = b + S - 1;
+      if (next < k.b1) {
+        copy(next, (next - k.b0) % S);
+        lookup(min(next + 1, k.b1 - 1));
+      }
+      cp_commit();
+    }
+    unsigned char* sK = ring + ((b - k.b0) % S) * 2 * T::kTileBytes;
+    unsigned char* sV = sK + T::kTileBytes;
+    const int s0 = k.v.slot0(b, BN);
+
+    // ---- scores
+    float sh[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sh[i][e] = 0.f;
+    if constexpr (Q4) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        uint32_t pr[2][NG];  // the pairs of this lane's two slots
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const unsigned char* p = sK + T::kRows + slot_at(i, e) * T::kPairBytes;
+          if constexpr (NG == 4) *reinterpret_cast<uint4*>(pr[e]) = *reinterpret_cast<const uint4*>(p);
+          else *reinterpret_cast<uint2*>(pr[e]) = *reinterpret_cast<const uint2*>(p);
+        }
+        const int row = wslot + i * 8 + (g >> 1) + (g & 1) * 4;  // the slot of column g
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          const uint32_t w = *reinterpret_cast<const uint32_t*>(sK + at4<HD, false>(row, gr) + t * 4);
+          float c[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint32_t n0 = codes_f16(w), n1 = codes_f16(w >> 4), n2 = codes_f16(w >> 8), n3 = codes_f16(w >> 12);
+          mma_f16(c, qf[2 * gr][1], n0, n1);
+          mma_f16(c, qf[2 * gr + 1][1], n2, n3);
+          mma_f16(c, qf[2 * gr][0], n0, n1);
+          mma_f16(c, qf[2 * gr + 1][0], n2, n3);
+          // c is (q . (code - 8)) / back
+          const float sc0 = bf16_lo(pr[0][gr]), sc1 = bf16_lo(pr[1][gr]);
+          const float mn0 = fmaf(8.f, sc0, bf16_hi(pr[0][gr])), mn1 = fmaf(8.f, sc1, bf16_hi(pr[1][gr]));
+          sh[i][0] = fmaf(c[0] * back_a, sc0, fmaf(qsum_a[gr], mn0, sh[i][0]));
+          sh[i][1] = fmaf(c[1] * back_a, sc1, fmaf(qsum_a[gr], mn1, sh[i][1]));
+          sh[i][2] = fmaf(c[2] * back_b, sc0, fmaf(qsum_b[gr], mn0, sh[i][2]));
+          sh[i][3] = fmaf(c[3] * back_b, sc1, fmaf(qsum_b[gr], mn1, sh[i][3]));
+        }
+      }
+    } else if constexpr (F32) {
+      float s0_[NT][4], s1[NT][4], s2[NT][4];  // an accumulator chain per product
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s0_[i][e] = s1[i][e] = s2[i][e] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < HD / 8; ++ks) {
+        uint32_t qh[4], ql[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = wr * 16 + g + (e & 1) * 8, ch = ks * 2 + (e >> 1);
+          split_tf32(*reinterpret_cast<const float*>(sQ + row * HD * 4 + ((ch ^ (row & 7)) << 4) + t * 4), qh[e], ql[e]);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const int row = wslot + nt * 8 + g;
+          uint32_t kh[2], kl[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            split_tf32(*reinterpret_cast<const float*>(sK + row * T::kRowBytes + (((ks * 2 + e) ^ (row & 7)) << 4) + t * 4),
+                       kh[e], kl[e]);
+          mma_tf32(s0_[nt], ql, kl[0], kl[1]);
+          mma_tf32(sh[nt], qh, kh[0], kh[1]);
+          mma_tf32(s1[nt], qh, kl[0], kl[1]);
+          mma_tf32(s2[nt], ql, kh[0], kh[1]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sh[i][e] += s0_[i][e] + (s1[i][e] + s2[i][e]);
+    } else {
+      float ss[NT][4];
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ss[i][e] = 0.f;
+      const int arow = wr * 16 + (lane & 15);
+      const uint32_t qa = smem_addr(sQ) + arow * HD * 2;
+      const int krow = (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks) {
+        uint32_t qh[4], qm[4], ql[4];
+        const uint32_t at = qa + (((2 * ks + (lane >> 4)) ^ (arow & 7)) << 4);
+        ldsm4(qh, at);
+        ldsm4(qm, at + RT * HD * 2);
+        ldsm4(ql, at + 2 * RT * HD * 2);
+#pragma unroll
+        for (int np = 0; np < NT / 2; ++np) {
+          const int row = wslot + np * 16 + krow;
+          uint32_t k4[4];
+          ldsm4(k4, smem_addr(sK) + row * T::kRowBytes + (((2 * ks + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
+          mma_bf16(sh[2 * np], qh, k4[0], k4[1]);
+          mma_bf16(sh[2 * np + 1], qh, k4[2], k4[3]);
+          mma_bf16(ss[2 * np], qm, k4[0], k4[1]);
+          mma_bf16(ss[2 * np + 1], qm, k4[2], k4[3]);
+          mma_bf16(ss[2 * np], ql, k4[0], k4[1]);
+          mma_bf16(ss[2 * np + 1], ql, k4[2], k4[3]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sh[i][e] += ss[i][e];
+    }
+
+    // ---- mask: only blocks that some row sees a part of have anything to hide
+    const bool edge = k.v.edge(s0, BN, window, sinks);
+    if (edge) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!rows_sees(e < 2 ? pa : pb, s0 + slot_at(i, e), window, sinks)) sh[i][e] = kNegInf;
+    }
+
+    // ---- online softmax
+    float xa = kNegInf, xb = kNegInf;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      xa = fmaxf(xa, fmaxf(sh[i][0], sh[i][1]));
+      xb = fmaxf(xb, fmaxf(sh[i][2], sh[i][3]));
+    }
+#pragma unroll
+    for (int w = 1; w < 4; w <<= 1) {
+      xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, w));
+      xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, w));
+    }
+    xa = fmaxf(xa, ma), xb = fmaxf(xb, mb);
+    // rows that have seen nothing yet keep a maximum of -inf; their p are exp2(-inf - 0) = 0
+    const float ba = xa == kNegInf ? 0.f : xa, bb = xb == kNegInf ? 0.f : xb;
+    float fa = ex2(ma - ba), fb = ex2(mb - bb);
+    ma = xa, mb = xb;
+    float sa = 0.f, sb = 0.f;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      sh[i][0] = ex2(sh[i][0] - ba), sh[i][1] = ex2(sh[i][1] - ba);
+      sh[i][2] = ex2(sh[i][2] - bb), sh[i][3] = ex2(sh[i][3] - bb);
+      sa += sh[i][0] + sh[i][1];
+      sb += sh[i][2] + sh[i][3];
+    }
+    la = la * fa + sa, lb = lb * fb + sb;
+
+    // ---- o = o * f + p . V, the block's product from a fresh accumulator
+    if constexpr (Q4) {
+      constexpr int NK = SN / 16;
+      const unsigned char* pairs = sV + T::kRows;
+      float cm[4] = {0.f, 0.f, 0.f, 0.f};
+      uint32_t nan_bits[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int j = 0; j < NK; ++j) {
+        // the middles: column g of the product is group g; this lane's slots are t, t + 4, t + 8, t + 12
+        const int row = wslot + j * 16 + t;
+        uint32_t h[4], m[4], l[4];
+        float mid[4];
+        split3(sh[2 * j][0], sh[2 * j][1], h[0], m[0], l[0]), split3(sh[2 * j][2], sh[2 * j][3], h[1], m[1], l[1]);
+        split3(sh[2 * j + 1][0], sh[2 * j + 1][1], h[2], m[2], l[2]);
+        split3(sh[2 * j + 1][2], sh[2 * j + 1][3], h[3], m[3], l[3]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t pr = *reinterpret_cast<const uint32_t*>(pairs + (row + 4 * e) * T::kPairBytes + (g & (NG - 1)) * 4);
+          mid[e] = fmaf(8.f, bf16_lo(pr), bf16_hi(pr));
+        }
+        if (edge) {
+          // A group that was appended with a NaN or an infinity in it has a NaN for its minimum. Where
+          // the row is hidden, 0 x NaN must not reach the output: the NaN is taken out, and counted for
+          // the rows that see it.
+          bool bad = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) bad |= mid[e] != mid[e];
+          if (__any_sync(0xffffffffu, bad)) {
+            uint32_t seen[4], nan[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              nan[e] = mid[e] != mid[e] ? 0x3f80u : 0u;
+              if (nan[e]) mid[e] = 0.f;
+              const int p = e & 1 ? pb : pa, at = s0 + row + (e >> 1) * 8;
+              seen[e] = (rows_sees(p, at, window, sinks) ? 0x3f80u : 0u) |
+                        (rows_sees(p, at + 4, window, sinks) ? 0x3f800000u : 0u);
+            }
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_bf16(c, seen, nan[0] | nan[1] << 16, nan[2] | nan[3] << 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (c[e] > 0.f) nan_bits[e] = 0x7fc00000u;
+          }
+        }
+        const uint32_t b0 = pack_bf16(mid[0], mid[1]), b1 = pack_bf16(mid[2], mid[3]);
+        const uint32_t d0 = pack_bf16(mid[0] - bf16_lo(b0), mid[1] - bf16_hi(b0));
+        const uint32_t d1 = pack_bf16(mid[2] - bf16_lo(b1), mid[3] - bf16_hi(b1));
+        mma_bf16(cm, l, b0, b1);
+        mma_bf16(cm, m, d0, d1);
+        mma_bf16(cm, h, d0, d1);
+        mma_bf16(cm, m, b0, b1);
+        mma_bf16(cm, h, b0, b1);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) om[e] = nan_bits[e] ? __uint_as_float(nan_bits[e]) : fmaf(om[e], e < 2 ? fa : fb, cm[e]);
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr) {
+        // Column c of tile i of a group is its dim 8 (c & 3) + 4 (c >> 2) + i: lane (g, t) holds the
+        // four nibbles of column g in one half of a word, of two slots side by side in a register.
+        float c[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[i][e] = 0.f;
+        float sc[NK][4], most = 0.f;
+#pragma unroll
+        for (int j = 0; j < NK; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sc[j][e] = bf16_lo(*reinterpret_cast<const uint32_t*>(pairs + (wslot + j * 16 + t + 4 * e) * T::kPairBytes + gr * 4));
+            most = fmaxf(most, sc[j][e]);
+          }
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        // scale * up lies below 2^15; the exponent moves in steps of 8, so that it hardly ever does.
+        // (A scale is below 2^109, so both factors are normal numbers.)
+        const int ex = max((int)(__float_as_uint(most) >> 23) | 7, 15);
+        const float up = power_of_two(268 - ex), back = power_of_two(ex - 14);
+#pragma unroll
+        for (int j = 0; j < NK; ++j) {
+          const int row = wslot + j * 16 + t;
+          uint32_t w[4], h[4], l[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sc[j][e] *= up;
+            w[e] = *reinterpret_cast<const uint16_t*>(sV + at4<HD, true>(row + 4 * e, gr) + (g & 3) * 4 + (g >> 2) * 2);
+          }
+          split2_f16(sh[2 * j][0] * sc[j][0], sh[2 * j][1] * sc[j][1], h[0], l[0]);
+          split2_f16(sh[2 * j][2] * sc[j][0], sh[2 * j][3] * sc[j][1], h[1], l[1]);
+          split2_f16(sh[2 * j + 1][0] * sc[j][2], sh[2 * j + 1][1] * sc[j][3], h[2], l[2]);
+          split2_f16(sh[2 * j + 1][2] * sc[j][2], sh[2 * j + 1][3] * sc[j][3], h[3], l[3]);
+          const uint32_t w0 = w[0] | w[1] << 16, w1 = w[2] | w[3] << 16;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t b0 = codes_f16(w0 >> (4 * i)), b1 = codes_f16(w1 >> (4 * i));
+            mma_f16(c[i], l, b0, b1);
+            mma_f16(c[i], h, b0, b1);
+          }
+        }
+        float ga = fa, gb = fb;
+        if (back != unit[gr]) {
+          const float now = fmaxf(back, unit[gr]), lift = unit[gr] / now, drop = back / now;
+          ga *= lift, gb *= lift;
+          unit[gr] = now;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[i][e] *= drop;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[gr * 4 + i][e] = fmaf(o[gr * 4 + i][e], e < 2 ? ga : gb, c[i][e]);
+      }
+    } else {
+      // A row of V that some rows do not see may hold infinities or NaN, and 0 x NaN would reach
+      // the rows that must not see it: such values are taken out of the tile and added to the
+      // rows that do see them.
+      if (edge) {
+        auto value = [&](int row, int d) -> float {
+          const unsigned char* p = sV + row * T::kRowBytes + (((d * (F32 ? 4 : 2) >> 4) ^ (row & 7)) << 4) + (d * (F32 ? 4 : 2) & 15);
+          if constexpr (F32) return *reinterpret_cast<const float*>(p);
+          else return bf16_to_f32(*reinterpret_cast<const __nv_bfloat16*>(p));
+        };
+        int bad = 0;
+        for (int i = tid; i < BN * HD; i += kThreads) bad |= !is_finite(value(i / HD, i % HD));
+        if (__syncthreads_or(bad)) {
+#pragma unroll
+          for (int i = 0; i < HD / 8; ++i) {
+            o[i][0] *= fa, o[i][1] *= fa, o[i][2] *= fb, o[i][3] *= fb;
+            for (int row = wslot; row < wslot + SN; ++row) {
+              const float v0 = value(row, i * 8 + 2 * t), v1 = value(row, i * 8 + 2 * t + 1);
+              if (is_finite(v0) && is_finite(v1)) continue;
+              if (rows_sees(pa, s0 + row, window, sinks)) {
+                if (!is_finite(v0)) o[i][0] += v0;
+                if (!is_finite(v1)) o[i][1] += v1;
+              }
+              if (rows_sees(pb, s0 + row, window, sinks)) {
+                if (!is_finite(v0)) o[i][2] += v0;
+                if (!is_finite(v1)) o[i][3] += v1;
+              }
+            }
+          }
+          fa = fb = 1.f;
+          __syncthreads();
+          for (int i = tid; i < BN * HD; i += kThreads) {
+            const int row = i / HD, d = i % HD;
+            if (is_finite(value(row, d))) continue;
+            unsigned char* p = sV + row * T::kRowBytes + (((d * (F32 ? 4 : 2) >> 4) ^ (row & 7)) << 4) + (d * (F32 ? 4 : 2) & 15);
+            if constexpr (F32) *reinterpret_cast<float*>(p) = 0.f;
+            else *reinterpret_cast<uint16_t*>(p) = 0;
+          }
+          __syncthreads();
+        }
+      }
+      if constexpr (F32) {
+        uint32_t ph[NT][4], pl[NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {  // slots 2t, 2t + 1 of a group take the places t, t + 4 of the product
+          split_tf32_near(sh[j][0], ph[j][0], pl[j][0]);
+          split_tf32_near(sh[j][2], ph[j][1], pl[j][1]);
+          split_tf32_near(sh[j][1], ph[j][2], pl[j][2]);
+          split_tf32_near(sh[j][3], ph[j][3], pl[j][3]);
+        }
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) {
+          float ch[4] = {0.f, 0.f, 0.f, 0.f}, cs[4] = {0.f, 0.f, 0.f, 0.f};
+          const int d = i * 8 + g;
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            uint32_t vh[2], vl[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int row = wslot + j * 8 + 2 * t + e;
+              split_tf32(*reinterpret_cast<const float*>(sV + row * T::kRowBytes + (((d >> 2) ^ (row & 7)) << 4) + (d & 3) * 4),
+                         vh[e], vl[e]);
+            }
+            mma_tf32(ch, ph[j], vh[0], vh[1]);
+            mma_tf32(cs, ph[j], vl[0], vl[1]);
+            mma_tf32(cs, pl[j], vh[0], vh[1]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][e] = fmaf(o[i][e], e < 2 ? fa : fb, ch[e] + cs[e]);
+        }
+      } else {
+        constexpr int NK = SN / 16;
+        uint32_t ph[NK][4], pm[NK][4], pl[NK][4];
+#pragma unroll
+        for (int j = 0; j < NK; ++j) {
+          split3(sh[2 * j][0], sh[2 * j][1], ph[j][0], pm[j][0], pl[j][0]);
+          split3(sh[2 * j][2], sh[2 * j][3], ph[j][1], pm[j][1], pl[j][1]);
+          split3(sh[2 * j + 1][0], sh[2 * j + 1][1], ph[j][2], pm[j][2], pl[j][2]);
+          split3(sh[2 * j + 1][2], sh[2 * j + 1][3], ph[j][3], pm[j][3], pl[j][3]);
+        }
+        const int vrow = (lane & 7) + (((lane >> 3) & 1) << 3);
+#pragma unroll
+        for (int np = 0; np < HD / 16; ++np) {
+          float ch[2][4], cs[2][4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ch[0][e] = ch[1][e] = cs[0][e] = cs[1][e] = 0.f;
+#pragma unroll
+          for (int j = 0; j < NK; ++j) {
+            const int row = wslot + j * 16 + vrow;
+            uint32_t v4[4];
+            ldsm4t(v4, smem_addr(sV) + row * T::kRowBytes + (((2 * np + (lane >> 4)) ^ (row & 7)) << 4));
+            mma_bf16(ch[0], ph[j], v4[0], v4[1]);
+            mma_bf16(ch[1], ph[j], v4[2], v4[3]);
+            mma_bf16(cs[0], pm[j], v4[0], v4[1]);
+            mma_bf16(cs[1], pm[j], v4[2], v4[3]);
+            mma_bf16(cs[0], pl[j], v4[0], v4[1]);
+            mma_bf16(cs[1], pl[j], v4[2], v4[3]);
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[2 * np + u][e] = fmaf(o[2 * np + u][e], e < 2 ? fa : fb, ch[u][e] + cs[u][e]);
+        }
+      }
+    }
+  }
+  cp_wait<0>();
+#pragma unroll
+  for (int w = 1; w < 4; w <<= 1) {
+    la += __shfl_xor_sync(0xffffffffu, la, w);
+    lb += __shfl_xor_sync(0xffffffffu, lb, w);
+  }
+
+  // ---- results, through shared memory: the slot groups are joined, and rows leave whole
+  __syncthreads();  // the ring is free
+  constexpr int kPad = T::kPad;
+  float* sO = reinterpret_cast<float*>(ring);
+  float* sML = sO + WS * RT * kPad;
+#pragma unroll
+  for (int i = 0; i < HD / 8; ++i) {
+    float* oa = sO + (ws * RT + ra) * kPad;
+    float* ob = sO + (ws * RT + rb) * kPad;
+    if constexpr (Q4) {
+      const int gr = i / 4, d = gr * kGroup4 + (t & 1) * 16 + (t >> 1) * 4 + i % 4, from = (lane & ~3) | gr >> 1;
+      const float m0 = __shfl_sync(0xffffffffu, om[gr & 1], from), m1 = __shfl_sync(0xffffffffu, om[2 + (gr & 1)], from);
+      oa[d] = fmaf(o[i][0], unit[gr], m0), oa[d + 8] = fmaf(o[i][1], unit[gr], m0);
+      ob[d] = fmaf(o[i][2], unit[gr], m1), ob[d + 8] = fmaf(o[i][3], unit[gr], m1);
+    } else {
+      *reinterpret_cast<float2*>(oa + i * 8 + 2 * t) = make_float2(o[i][0], o[i][1]);
+      *reinterpret_cast<float2*>(ob + i * 8 + 2 * t) = make_float2(o[i][2], o[i][3]);
+    }
+  }
+  if (t == 0) {
+    sML[(ws * RT + ra) * 2] = ma, sML[(ws * RT + ra) * 2 + 1] = la;
+    sML[(ws * RT + rb) * 2] = mb, sML[(ws * RT + rb) * 2 + 1] = lb;
+  }
+  __syncthreads();
+  rows_finish<HD, WS, RT, kThreads>(P, k, sO, sML, tid);
+}
+
+// Joins the splits of a sequence. W warps share one (row, query head): warp w folds the
+// splits w, w + W, ... in order, then the warps' results are folded in order, so the sum does
+// not depend on timing. Every split's maximum, sum and output are loaded together: the chain
+// is one load per kBatch splits.
+template <int HD, int W>
+__global__ void __launch_bounds__(kThreads) rows_join_kernel(const __grid_constant__ RowsKernelArgs P, int rt, int bn) {
+  constexpr int V = HD / 32, kBatch = 4;
+  __shared__ float so[8][HD], sml[8][2];
+  const RowsAttnArgs& a = P.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = warp % W;
+  const int item = blockIdx.x * (8 / W) + warp / W;
+  int i = 0, at = 0, nsplit = 1;
+  if (item < P.join0[P.n_seqs]) {
+    i = rows_find(P.join0, P.n_seqs, item);
+    at = item - P.join0[i];
+    // the tile of this row, and its blocks, as the main kernel had them
+    const int G = a.nq / a.pages.kvh, j = at / a.nq, head = at % a.nq;
+    const int r0 = (j * G + head % G) / rt * rt, last = min(r0 + rt, P.m[i] * G) - 1;
+    nsplit = (RowsView(P.t0[i] + r0 / G, P.t0[i] + last / G, a.window, a.sinks, bn).nb + P.bps - 1) / P.bps;
+  }
+  const bool live = nsplit > 1;
+  const size_t step = (size_t)P.m[i] * a.nq, base = (size_t)P.part0[i] + at;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the splits' grid has ended and its stores are visible
+  float m = kNegInf, l = 0.f, acc[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] = 0.f;
+  if (live) {
+    for (int s0 = w; s0 < nsplit; s0 += kBatch * W) {
+      float2 ml[kBatch];
+      float o[kBatch][V];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int s = s0 + u * W;
+        ml[u] = make_float2(kNegInf, 0.f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[u][e] = 0.f;
+        if (s < nsplit) {
+          const size_t p = base + s * step;
+          ml[u] = *reinterpret_cast<const float2*>(a.part_ml + p * 2);
+          if constexpr (V == 4) {
+            const float4 f = *reinterpret_cast<const float4*>(a.part_o + p * HD + lane * 4);
+            o[u][0] = f.x, o[u][1] = f.y, o[u][2] = f.z, o[u][3] = f.w;
+          } else {
+            const float2 f = *reinterpret_cast<const float2*>(a.part_o + p * HD + lane * 2);
+            o[u][0] = f.x, o[u][1] = f.y;
+          }
+        }
+      }
+      float x = m;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) x = fmaxf(x, ml[u].x);
+      const float b = x == kNegInf ? 0.f : x, f = ex2(m - b);
+      m = x, l *= f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] *= f;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const float wt = ex2(ml[u].x - b);
+        l = fmaf(ml[u].y, wt, l);
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] = fmaf(o[u][e], wt, acc[e]);
+      }
+    }
+  }
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) so[warp][lane * V + e] = acc[e];
+    if (lane == 0) sml[warp][0] = m, sml[warp][1] = l;
+    __syncthreads();
+    if (w != 0) return;
+    float x = kNegInf;
+#pragma unroll
+    for (int u = 0; u < W; ++u) x = fmaxf(x, sml[warp + u][0]);
+    const float b = x == kNegInf ? 0.f : x;
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0.f;
+#pragma unroll
+    for (int u = 0; u < W; ++u) {
+      const float wt = ex2(sml[warp + u][0] - b);
+      l = fmaf(sml[warp + u][1], wt, l);
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] = fmaf(so[warp + u][lane * V + e], wt, acc[e]);
+    }
+  }
+  if (!live) return;
+  const float inv = 1.0f / l;
+  float* dst = a.out + ((size_t)P.row0[i] * a.nq + at) * HD + lane * V;
+#pragma unroll
+  for (int e = 0; e < V; ++e) dst[e] = acc[e] * inv;
+}
+
+template <int KIND, int HD, int WR>
+cudaError_t configure_one() {
+  return cudaFuncSetAttribute(rows_attn_kernel<KIND, HD, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              Tile<KIND, HD, WR>::kSmem);
+}
+template <int HD>
+cudaError_t configure_hd() {
+  cudaError_t e = configure_one<kKvF32, HD, 1>();
+  if (e == cudaSuccess) e = configure_one<kKvF32, HD, 2>();
+  if (e == cudaSuccess) e = configure_one<kKvBf16, HD, 1>();
+  if (e == cudaSuccess) e = configure_one<kKvBf16, HD, 2>();
+  if (e == cudaSuccess) e = configure_one<kKvBf16, HD, 4>();
+  if (e == cudaSuccess) e = configure_one<kKv4, HD, 1>();
+  if (e == cudaSuccess) e = configure_one<kKv4, HD, 2>();
+  if (e == cudaSuccess) e = configure_one<kKv4, HD, 4>();
+  return e;
+}
+
+// Cuts the blocks of bn slots of all (sequence, KV head, tile of rt rows) into CTAs, runs
+// `main` over them, and joins the splits.
+template <int HD, typename Main>
+cudaError_t launch_split(const RowsAttnArgs& a, const RowsBatch& s, int rt, int bn, int sms, int* launches,
+                         cudaStream_t st, Main main) {
+  RowsKernelArgs P;
+  P.a = a;
+  P.n_seqs = s.n_seqs;
+  const int kvh = a.pages.kvh, G = a.nq / kvh;
+  std::vector<int> blocks;  // of every tile, sequence by sequence
+  int first[kRowsMaxSeqs + 1];
+  long long total = 0;
+  for (int i = 0; i < s.n_seqs; ++i) {
+    first[i] = (int)blocks.size();
+    const int R = s.m[i] * G;
+    for (int r0 = 0; r0 < R; r0 += rt) {
+      const int last = std::min(r0 + rt, R) - 1;
+      blocks.push_back(RowsView(s.t0[i] + r0 / G, s.t0[i] + last / G, a.window, a.sinks, bn).nb);
+      total += (long long)blocks.back() * kvh;
+    }
+  }
+  first[s.n_seqs] = (int)blocks.size();
+  const long long items = (long long)blocks.size() * kvh;
+  // blocks per split: the fewest with which all CTAs run at once (short last splits make
+  // that a little more than total / sms); with more items than SMs, about one SM's share.
+  // Partial results have to fit their buffer.
+  P.bps = (int)std::max<long long>(1, (total + sms - 1) / sms);
+  for (;;) {
+    long long ctas = 0, part = 0;
+    for (int i = 0; i < s.n_seqs; ++i) {
+      int most = 1;
+      for (int t = first[i]; t < first[i + 1]; ++t) {
+        const int ns = (blocks[t] + P.bps - 1) / P.bps;
+        ctas += (long long)ns * kvh;
+        most = std::max(most, ns);
+      }
+      if (most > 1) part += (long long)most * s.m[i] * a.nq;
+    }
+    if ((ctas <= sms || items >= sms) && part <= (long long)rows_attn_part_rows(sms)) break;
+    P.bps += 1 + P.bps / 64;
+  }
+  int splits = 1, part = 0, item = 0, join = 0;
+  for (int i = 0; i < s.n_seqs; ++i) {
+    P.seq[i] = s.seq[i], P.row0[i] = s.row0[i], P.m[i] = s.m[i], P.t0[i] = s.t0[i];
+    int most = 1;
+    for (int t = first[i]; t < first[i + 1]; ++t) most = std::max(most, (blocks[t] + P.bps - 1) / P.bps);
+    P.splits[i] = most;
+    P.item0[i] = item;
+    P.part0[i] = part;
+    P.join0[i] = join;
+    item += (first[i + 1] - first[i]) * kvh * most;
+    if (most > 1) part += most * s.m[i] * a.nq, join += s.m[i] * a.nq;
+    splits = std::max(splits, most);
+  }
+  P.item0[s.n_seqs] = item;
+  P.join0[s.n_seqs] = join;
+  cudaError_t e = main(P, item);
+  *launches += 1;
+  if (e != cudaSuccess || splits == 1) return e;
+  const bool many = splits > 8;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(many ? join : (join + 7) / 8);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  *launches += 1;
+  return cudaLaunchKernelEx(&cfg, many ? rows_join_kernel<HD, 8> : rows_join_kernel<HD, 1>, P, rt, bn);
+}
+
+template <int KIND, int HD, int WR>
+cudaError_t launch(const RowsAttnArgs& a, const RowsBatch& s, int sms, int* launches, cudaStream_t st) {
+  using T = Tile<KIND, HD, WR>;
+  return launch_split<HD>(a, s, T::RT, T::BN, sms, launches, st, [&](const RowsKernelArgs& P, int ctas) {
+    rows_attn_kernel<KIND, HD, WR><<<ctas, kThreads, T::kSmem, st>>>(P);
+    return cudaGetLastError();
+  });
+}
+
+template <int KIND, int HD>
+cudaError_t launch_kind(const RowsAttnArgs& a, const RowsBatch& b, int sms, int* launches, cudaStream_t st) {
+  int rows = 0;  // of the largest sequence that share a KV head
+  for (int i = 0; i < b.n_seqs; ++i) rows = std::max(rows, b.m[i] * (a.nq / a.pages.kvh));
+  if (rows == 0) return cudaSuccess;
+  if (rows <= 16) return launch<KIND, HD, 1>(a, b, sms, launches, st);
+  if constexpr (KIND != kKvF32)
+    if (rows > 32) return launch<KIND, HD, 4>(a, b, sms, launches, st);
+  return launch<KIND, HD, 2>(a, b, sms, launches, st);
+}
+
+}  // namespace
+
+size_t rows_attn_part_rows(int sms) { return (size_t)2 * sms * 256; }
+
+cudaError_t configure_rows_attn() {
+  cudaError_t e = configure_hd<64>();
+  if (e == cudaSuccess) e = configure_hd<128>();
+  return e;
+}
+
+cudaError_t op_rows_attention(const RowsAttnArgs& a, const RowsBatch& b, int kind, int hd, int sms, int* launches,
+                              cudaStream_t st) {
+  if (!a.part_o || !a.part_ml || !a.err) return cudaErrorInvalidValue;
+  switch (kind) {
+    case kKvF32:
+      return hd == 64 ? launch_kind<kKvF32, 64>(a, b, sms, launches, st) : launch_kind<kKvF32, 128>(a, b, sms, launches, st);
+    case kKvBf16:
+      return hd == 64 ? launch_kind<kKvBf16, 64>(a, b, sms, launches, st) : launch_kind<kKvBf16, 128>(a, b, sms, launches, st);
+    default:
+      return hd == 64 ? launch_kind<kKv4, 64>(a, b, sms, launches, st) : launch_kind<kKv4, 128>(a, b, sms, launches, st);
+  }
+}
+
+}  // namespace dllm

@@ -6,6 +6,7 @@
 #include <cuda.h>
 
 #include "kernels.cuh"
+#include "mma_sync.cuh"
 #include "verify.cuh"
 
 namespace dllm {
@@ -29,26 +30,6 @@ __host__ __device__ inline int ta_splits(int slots, int bn, int bps) {
   const int blocks = (slots + bn - 1) / bn;
   return (blocks + bps - 1) / bps;
 }
-
-DLLM_DEV float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-DLLM_DEV uint32_t pack_bf16(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-// (x, y) -> three packed bf16 pairs whose sums are x and y to 2^-25 of them.
-DLLM_DEV void split3(float x, float y, uint32_t& h, uint32_t& m, uint32_t& l) {
-  h = pack_bf16(x, y);
-  x -= bf16_lo(h), y -= bf16_hi(h);
-  m = pack_bf16(x, y);
-  x -= bf16_lo(m), y -= bf16_hi(m);
-  l = pack_bf16(x, y);
-}
-DLLM_DEV bool is_finite(float v) { return fabsf(v) <= 3.402823466e38f; }
 
 // One row tile of a CTA: rows [r0, r0 + RT) of the m G rows that share a KV head.
 struct TATile {

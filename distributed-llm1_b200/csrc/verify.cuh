@@ -36,6 +36,13 @@ struct RopeAtArgs {
   float factor;
 };
 cudaError_t op_rope_at(const RopeAtArgs& a, int sms, cudaStream_t st);
+struct NormRopeArgs {
+  RopeAtArgs rope;
+  const __nv_bfloat16* q_norm;  // [hd]
+  const __nv_bfloat16* k_norm;
+  float eps;
+};
+cudaError_t op_norm_rope(const NormRopeArgs& n, int sms, cudaStream_t st);
 
 // ---- pick.cu ----------------------------------------------------------------------
 struct PickArgs {

@@ -150,6 +150,34 @@ class DraftTree:
             pass
 
 
+class RowBatch:
+    """How many rows each sequence of a batch has (dllm_rows_create). Freed with the object."""
+
+    def __init__(self, ctx: "KernelContext", counts, seqs=None):
+        self.ctx, self.handle = ctx, None
+        self.counts = int32s(counts, "rowBatch counts")
+        self.seqs = np.arange(self.counts.size, dtype=np.int32) if seqs is None else int32s(seqs, "rowBatch seqs")
+        if self.seqs.size != self.counts.size or (self.counts < 0).any():
+            raise _lib.DllmError(_lib.DLLM_EINVAL, f"rowBatch: counts {self.counts.tolist()} of sequences "
+                                                   f"{self.seqs.tolist()}")
+        self.n = int(self.counts.sum(dtype=np.int64))
+        h = C.c_void_p()
+        ctx._check(ctx.lib.dllm_rows_create(ctx.handle, _lib.ptr(self.counts, C.c_int32), _lib.ptr(self.seqs, C.c_int32),
+                                            self.counts.size, C.byref(h)), "rowBatch")
+        self.handle = h.value
+
+    def destroy(self):
+        if self.handle:
+            self.ctx.lib.dllm_rows_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+
 class KernelContext:
     def __init__(self, device: int = 0, cfg: ModelConfig | None = None):
         self.lib = _lib.load()
@@ -335,6 +363,21 @@ class KernelContext:
         self._check(self.lib.dllm_rope_at(self.handle, h(plan, RopePlan), h(positions), n, o(qBuf), o(kBuf), o(qOut),
                                           o(kOut)), "ropeAt")
         return qOut or qBuf, kOut or kBuf
+
+    def normRopeAt(self, plan: RopePlan, positions: GpuBuffer, n: int, qBuf: GpuBuffer | None = None,
+                   kBuf: GpuBuffer | None = None, qNorm: GpuBuffer | None = None, kNorm: GpuBuffer | None = None,
+                   qOut: GpuBuffer | None = None, kOut: GpuBuffer | None = None):
+        """Each head of q [n, NQ*HD] and k [n, KVH*HD] divided by its root mean square and scaled
+        by its norm (bf16 [HD]), then turned as by ropeAt; in place without outputs."""
+        h, o = self._h, self._opt
+        self._check(self.lib.dllm_norm_rope_at(self.handle, h(plan, RopePlan), h(positions), n, o(qBuf), o(kBuf), o(qNorm),
+                                               o(kNorm), o(qOut), o(kOut)), "normRopeAt")
+        return qOut or qBuf, kOut or kBuf
+
+    def rowBatch(self, counts, seqs=None) -> RowBatch:
+        """Rows of one or more cache sequences: counts[i] rows (a chunk of a prompt, one new
+        token, none) of sequence seqs[i] (default i), one after the other."""
+        return RowBatch(self, counts, seqs)
 
     def draftTree(self, parents, counts=None, seqs=None) -> DraftTree:
         """Drafted trees of one or more cache sequences: counts[i] nodes for sequence

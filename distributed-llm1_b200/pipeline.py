@@ -18,7 +18,7 @@ import numpy as np
 
 from . import _lib, frames
 from .constants import FRAME
-from .kernels import DraftTree, GpuBuffer, KernelContext, int32s
+from .kernels import DraftTree, GpuBuffer, KernelContext, RowBatch, int32s
 
 
 # ---- assignLayers (pipeline.js:6-23) ---------------------------------------------------
@@ -279,10 +279,102 @@ class Stage:
                       "forward_tree")
         return hBuf
 
+    # ---- batches of rows (include/dllm.h; no counterpart in the reference)
+    def append_rows(self, L: int, rows: RowBatch, kBuf: GpuBuffer, vBuf: GpuBuffer):
+        """K/V rows of a batch -> slots T0 + j of their sequences (T0 unchanged)."""
+        h = self.k._h
+        self.k._check(self.lib.dllm_stage_append_rows(self.handle, L, h(rows, RowBatch), h(kBuf), h(vBuf)), "append_rows")
+
+    def window_attention(self, L: int, rows: RowBatch, qBuf: GpuBuffer, out: GpuBuffer | None = None, window: int = 0,
+                         sinks: int = 0) -> GpuBuffer:
+        """Every row of a batch, at slot p = T0 + j, over its sequence's slots s <= p with
+        s > p - window or s < sinks (window 0: all). The rows' own K/V come before, by append_rows."""
+        return _rows_attention(self.lib.dllm_stage_window_attention, self, L, rows, qBuf, out, window, sinks, "window_attention")
+
     def close(self):
         if self._owned and getattr(self, "handle", None):
             self.lib.dllm_stage_destroy(self.handle)
         self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _rows_attention(fn, cache, L, rows, qBuf, out, window, sinks, what) -> GpuBuffer:
+    k = cache.k
+    r, q = k._h(rows, RowBatch), k._h(qBuf)
+    if out is None:
+        out = k.createF32(rows.n * k.NQ * k.HD, what + " out")
+    window, sinks = (int(x) for x in int32s([window, sinks], what))
+    k._check(fn(cache.handle, L, r, q, k._h(out), window, sinks), what)
+    return out
+
+
+class Cache4:
+    """K and V of layers [start, end) in 4 bits (dllm_kv4_create): max_seqs sequences of max_pos
+    slots in pages, each with its T0, as a Stage holds them in bf16 or fp32."""
+
+    def __init__(self, kctx: KernelContext, start: int, end: int):
+        self.k, self.lib, self.start, self.end, self.handle = kctx, kctx.lib, start, end, None
+        h = C.c_void_p()
+        kctx._check(self.lib.dllm_kv4_create(kctx.handle, start, end, C.byref(h)), "Cache4")
+        self.handle = h.value
+
+    @property
+    def T0(self) -> int:
+        return self.t0_of(0)
+
+    @T0.setter
+    def T0(self, v: int):
+        self.set_t0(0, v)
+
+    def t0_of(self, seq: int) -> int:
+        return self.lib.dllm_kv4_get_t0(self.handle, seq)
+
+    def set_t0(self, seq: int, v: int):
+        self.k._check(self.lib.dllm_kv4_set_t0(self.handle, seq, int(v)), "set_t0")
+
+    def reset(self):
+        self.k._check(self.lib.dllm_kv4_reset(self.handle), "reset")
+
+    @property
+    def size(self) -> int:
+        """Bytes on the device."""
+        return int(self.lib.dllm_kv4_bytes(self.handle))
+
+    def pages_per_seq(self) -> int:
+        return int(self.lib.dllm_kv4_pages_per_seq(self.handle))
+
+    def set_page_table(self, seq: int, pages):
+        p = int32s(pages, "set_page_table")
+        self.k._check(self.lib.dllm_kv4_set_page_table(self.handle, seq, _lib.ptr(p, C.c_int32), p.size), "set_page_table")
+
+    def append(self, L: int, rows: RowBatch, kBuf: GpuBuffer, vBuf: GpuBuffer):
+        """K/V rows of a batch -> slots T0 + j of their sequences, rounded to 4 bits (T0 unchanged)."""
+        h = self.k._h
+        self.k._check(self.lib.dllm_kv4_append(self.handle, L, h(rows, RowBatch), h(kBuf), h(vBuf)), "append")
+
+    def read_rows(self, L: int, rows: RowBatch, kOut: GpuBuffer | None = None, vOut: GpuBuffer | None = None):
+        """The values that the slots T0 + j of a batch stand for, fp32 [n, KVH*HD]."""
+        k = self.k
+        r, n = k._h(rows, RowBatch), rows.n * k.KVH * k.HD
+        if kOut is None and vOut is None:
+            kOut, vOut = k.createF32(n, "k rows"), k.createF32(n, "v rows")
+        k._check(self.lib.dllm_kv4_read_rows(self.handle, L, r, k._opt(kOut), k._opt(vOut)), "read_rows")
+        return kOut, vOut
+
+    def attention(self, L: int, rows: RowBatch, qBuf: GpuBuffer, out: GpuBuffer | None = None, window: int = 0,
+                  sinks: int = 0) -> GpuBuffer:
+        """Stage.window_attention over this cache."""
+        return _rows_attention(self.lib.dllm_kv4_attention, self, L, rows, qBuf, out, window, sinks, "attention")
+
+    def close(self):
+        if getattr(self, "handle", None):
+            self.lib.dllm_kv4_destroy(self.handle)
+            self.handle = None
 
     def __del__(self):
         try:

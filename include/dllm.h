@@ -420,6 +420,64 @@ int dllm_stage_forward_tree(dllm_stage* st, const dllm_tree* tree, dllm_buf* h, 
  * cache with kernels of their own on the ctx stream. */
 void* dllm_stage_kv_device_ptr(const dllm_stage* st, int which);
 
+/* ---- long conversations -----------------------------------------------------------
+ * No counterpart in the reference. For hosts with layers of their own: norms of the query
+ * and key heads, K/V rows of a batch, attention under a sliding window and first tokens
+ * that stay visible ("sinks"), and a cache that holds K and V in 4 bits.
+ * A batch of rows (dllm_rows) says how many rows each of its sequences has: one new token,
+ * a chunk of a prompt, or none. Row j of a sequence is cache slot T0 + j. As with drafted
+ * trees, work is enqueued on the ctx stream in order, scratch belongs to the ctx (calls of
+ * one ctx, and graphs captured from them, must not overlap on the GPU), and T0 values are
+ * those of the call: a captured call replays with them, and refers to the buffers it was
+ * given. dllm_rows_create, dllm_kv4_create, dllm_kv4_set_page_table are refused while the
+ * ctx stream is captured. */
+
+/* For every head of q [n, NQ*HD] and k [n, KVH*HD] (either may be NULL, with its norm):
+ * y = x / sqrt(mean(x^2) + rms_norm_eps) * norm, norm a bf16 weight [HD]; then the plan's
+ * rotation at positions[t], as in dllm_rope_at. q_out / k_out NULL: in place. */
+int dllm_norm_rope_at(dllm_ctx* ctx, const dllm_rope_plan* plan, const dllm_buf* positions, int n, dllm_buf* q, dllm_buf* k,
+                      const dllm_buf* q_norm, const dllm_buf* k_norm, dllm_buf* q_out, dllm_buf* k_out);
+
+/* counts[i] rows (0..max_pos) for cache sequence seqs[i] (NULL: i; distinct), 1..128
+ * sequences and 1..1048576 rows in all. */
+typedef struct dllm_rows dllm_rows;
+int dllm_rows_create(dllm_ctx* ctx, const int32_t* counts, const int32_t* seqs, int n_seqs, dllm_rows** out);
+void dllm_rows_destroy(dllm_rows* rows);
+
+/* K/V rows k, v [n, KVH*HD] fp32 -> slots T0 + j of each sequence; T0 unchanged. */
+int dllm_stage_append_rows(dllm_stage* st, int layer, const dllm_rows* rows, const dllm_buf* k, const dllm_buf* v);
+/* out[row] = attention of the row at slot p = T0 + j (q [n, NQ*HD], after RoPE) over its
+ * sequence's slots s <= p with s > p - window or s < sinks; window 0: all of them. The rows'
+ * own K/V are in the cache before. A non-finite K/V value reaches only the rows that see it
+ * (there an infinity may come out as NaN). */
+int dllm_stage_window_attention(dllm_stage* st, int layer, const dllm_rows* rows, const dllm_buf* q, dllm_buf* out,
+                                int window, int sinks);
+
+/* A cache of layers [start, end) in 4 bits: max_seqs sequences of max_pos slots in pages of
+ * kv_page_size, as a stage has them, and T0 per sequence. Each 32 dims of a K or V row
+ * share a minimum m and a scale s in bf16 (5 bits per value in all): a value is m + c s,
+ *   m = the smallest of the 32 rounded down, s = fp32((largest - m) / 15) rounded up,
+ *   c = (x - m) / s to the nearest of 0..15 (ties to even)
+ * so that it is off by s / 2 at most. 32 values with a NaN, an infinity or a range of 2^112
+ * and more among them all read NaN. */
+typedef struct dllm_kv4 dllm_kv4;
+int dllm_kv4_create(dllm_ctx* ctx, int start, int end, dllm_kv4** out);
+void dllm_kv4_destroy(dllm_kv4* kv);
+int dllm_kv4_reset(dllm_kv4* kv);
+int dllm_kv4_get_t0(const dllm_kv4* kv, int seq);
+int dllm_kv4_set_t0(dllm_kv4* kv, int seq, int t0);
+int dllm_kv4_pages_per_seq(const dllm_kv4* kv);
+int dllm_kv4_set_page_table(dllm_kv4* kv, int seq, const int32_t* pages, int n_pages);
+/* Device memory of the cache (codes, scales and minima). */
+size_t dllm_kv4_bytes(const dllm_kv4* kv);
+/* K/V rows k, v [n, KVH*HD] fp32 -> slots T0 + j of each sequence; T0 unchanged. */
+int dllm_kv4_append(dllm_kv4* kv, int layer, const dllm_rows* rows, const dllm_buf* k, const dllm_buf* v);
+/* The values that slots T0 + j stand for, fp32 [n, KVH*HD]; either output may be NULL. */
+int dllm_kv4_read_rows(dllm_kv4* kv, int layer, const dllm_rows* rows, dllm_buf* k, dllm_buf* v);
+/* dllm_stage_window_attention over this cache's values. */
+int dllm_kv4_attention(dllm_kv4* kv, int layer, const dllm_rows* rows, const dllm_buf* q, dllm_buf* out, int window,
+                       int sinks);
+
 #ifdef __cplusplus
 }
 #endif

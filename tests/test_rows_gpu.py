@@ -1,0 +1,583 @@
+"""The operators of long conversations, each against its definition in 64 bits: norms of the
+query and key heads with their rotation, K/V rows of a batch, a cache in 4 bits, and
+attention under a window and first tokens that stay visible; then all of them together as a
+host's own layer runs them.
+
+EPS below is half a step of fp32, 2^-24."""
+import math
+
+import numpy as np
+import pytest
+
+from test_verify_gpu import EPS, f32, frequencies, i32, make_ctx, rope64, torch_
+
+pytestmark = pytest.mark.gpu
+
+
+def bf16(ctx, a):
+    return ctx.loadWeightBf16((np.ascontiguousarray(a, np.float32).view(np.uint32) >> 16).astype(np.uint16))
+
+
+def cut(a):
+    """fp32 values cut to bf16, as fp32."""
+    return (np.ascontiguousarray(a, np.float32).view(np.uint32) & np.uint32(0xFFFF0000)).view(np.float32)
+
+
+# ---- norms of the heads with the rotation -------------------------------------------------------
+def norm64(x, w, eps):
+    x = x.astype(np.float64)
+    return x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * w.astype(np.float64)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("hd,rd", [(64, 64), (64, 2), (64, 22), (64, 56), (128, 128), (128, 96), (128, 34), (128, 126)])
+def test_norm_rope_at(dllm, layout, hd, rd):
+    nq, kvh = 6, 2
+    ctx = make_ctx(dllm, nq, kvh, hd)
+    plan = ctx.ropePlan(layout=layout, rotary_dim=rd, theta=1e6)
+    f, factor = frequencies(rd, 1e6, None)
+    rng = np.random.default_rng(rd)
+    qn, kn = (cut(1 + 0.3 * rng.standard_normal(hd)) for _ in range(2))
+    for n in (1, 3, 37, 700):
+        pos = rng.integers(0, 1 << 24, n)
+        # rows of very different sizes, one of them next to eps, and a head of zeros
+        size = np.float32(10.0) ** rng.integers(-4, 5, (n, 1, 1)).astype(np.float32)
+        q, k = (rng.standard_normal((n, h, hd), np.float32) * size for h in (nq, kvh))
+        k[0, 0] = 0
+        qb, kb, pb, qw, kw = f32(ctx, q), f32(ctx, k), i32(ctx, pos), bf16(ctx, qn), bf16(ctx, kn)
+        qo, ko = ctx.createF32(q.size), ctx.createF32(k.size)
+        ctx.normRopeAt(plan, pb, n, qb, kb, qw, kw, qo, ko)
+        outs = [ctx.readF32(b, b.n) for b in (qo, ko)]
+        assert np.array_equal(ctx.readF32(qb, qb.n), q.reshape(-1))  # inputs untouched
+        ctx.normRopeAt(plan, pb, n, qb, kb, qw, kw)  # in place
+        inplace = [ctx.readF32(b, b.n) for b in (qb, kb)]
+        for x, w, o, ip in ((q, qn, outs[0], inplace[0]), (k, kn, outs[1], inplace[1])):
+            y = norm64(x, w, 1e-6)
+            want, mag = rope64(y, pos, rd, layout, f, factor)
+            # a sum of squares in at most 8 + 5 rounded steps, halved by the root, the mean: 8 eps; the
+            # root's reciprocal 4; three rounded products 3: 15 eps of y. The rotation: 9 eps (|y1| + |y2|).
+            bound = 24 * EPS * np.maximum(mag, np.abs(y))
+            err = np.abs(o.reshape(x.shape) - want)
+            assert (err <= bound).all(), (n, float((err / np.maximum(bound, 1e-30)).max()))
+            assert np.array_equal(o, ip)
+    ctx.close()
+
+
+def test_norm_rope_at_one_of_q_and_k(dllm):
+    ctx = make_ctx(dllm, 4, 2, 64)
+    plan, rng = ctx.ropePlan(), np.random.default_rng(0)
+    q, k = rng.standard_normal((5, 4, 64)).astype(np.float32), rng.standard_normal((5, 2, 64)).astype(np.float32)
+    pos, w = i32(ctx, [5, 0, 2 ** 31 - 1, -7, 9]), bf16(ctx, np.ones(64))
+    both = [ctx.createF32(q.size), ctx.createF32(k.size)]
+    ctx.normRopeAt(plan, pos, 5, f32(ctx, q), f32(ctx, k), w, w, *both)
+    qb, kb = f32(ctx, q), f32(ctx, k)
+    ctx.normRopeAt(plan, pos, 5, qBuf=qb, qNorm=w)
+    ctx.normRopeAt(plan, pos, 5, kBuf=kb, kNorm=w)
+    for one, b in zip((qb, kb), both):
+        assert np.array_equal(ctx.readF32(one, one.n), ctx.readF32(b, b.n))
+    # rows behind the n given stay as they are
+    qb = f32(ctx, q)
+    ctx.normRopeAt(plan, pos, 3, qBuf=qb, qNorm=w)
+    assert np.array_equal(ctx.readF32(qb, qb.n)[3 * 256:], q.reshape(-1)[3 * 256:])
+
+
+def test_norm_rope_at_refusals(dllm):
+    ctx = make_ctx(dllm, 4, 2, 64)
+    plan, pos = ctx.ropePlan(), i32(ctx, [0, 1])
+    q, k, w = ctx.createF32(2 * 256), ctx.createF32(2 * 128), bf16(ctx, np.ones(64))
+    short, other = bf16(ctx, np.ones(63)), make_ctx(dllm, 4, 2, 64)
+    for args, kw in (((plan, pos, 0, q, k, w, w), {}), ((plan, pos, 3, q, k, w, w), {}), ((plan, pos, 2, q, k, w, None), {}),
+                     ((plan, pos, 2, q, None, w, w), {}), ((plan, pos, 2), {}), ((plan, pos, 2, q, k, short, w), {}),
+                     ((plan, pos, 2, q, k, q, w), {}), ((plan, pos, 2, q, q, w, w), {}), ((plan, pos, 2, k, k, w, w), {}),
+                     ((plan, pos, 2, q, None, w, None), {"kOut": k}), ((plan, q, 2, q, k, w, w), {}),
+                     ((plan, pos, 2, q, k, w, w), {"qOut": k}), ((other.ropePlan(), pos, 2, q, k, w, w), {})):
+        with pytest.raises(dllm.DllmError):
+            ctx.normRopeAt(*args, **kw)
+
+
+# ---- caches and their rows --------------------------------------------------------------------
+def codes64(x):
+    """The values that 4-bit rows stand for, by the definition, 64 bits: [..., hd] fp32 in."""
+    z = np.ascontiguousarray(x, np.float32).reshape(*x.shape[:-1], x.shape[-1] // 32, 32)
+
+    def down(a):  # to bf16: 8 significant bits, or multiples of the smallest number, 2^-133
+        ex = np.maximum(np.frexp(a.astype(np.float64))[1] - 8, -133)
+        return np.ldexp(np.floor(np.ldexp(a.astype(np.float64), -ex)), ex)
+    low = down(z.min(-1, keepdims=True)).astype(np.float32)
+    span = (z.max(-1, keepdims=True) - low).astype(np.float32)
+    scale = -down(-(span.astype(np.float64) / 15).astype(np.float32))
+    c = np.rint((z - low).astype(np.float64) / np.where(scale > 0, scale, 1)).clip(0, 15)
+    return (low + c * scale).reshape(x.shape), np.broadcast_to(scale, z.shape).reshape(x.shape)
+
+
+class Rows:
+    """A paged cache ("f32", "bf16" or "4") filled through the operators under shuffled pages,
+    and its values in 64 bits on the GPU, [sequence][which] -> [slots, KVH, HD]."""
+
+    def __init__(self, dllm, nq, kvh, hd, kind, lens, counts, page=64, seqs=None, seed=0, layers=1, max_pos=None, edit=None):
+        torch = torch_()
+        self.lens, self.counts, self.kind, self.hd, self.nq, self.kvh = lens, counts, kind, hd, nq, kvh
+        self.seqs = seqs or list(range(len(lens)))
+        max_pos = max_pos or max(t + c for t, c in zip(lens, counts))
+        self.ctx = make_ctx(dllm, nq, kvh, hd, kv_dtype="f32" if kind == "f32" else "bf16", kv_page_size=page,
+                            max_pos=max_pos, max_seqs=max(self.seqs) + 1, num_layers=layers)
+        self.cache = dllm.Cache4(self.ctx, 0, layers) if kind == "4" else dllm.Stage(self.ctx, 0, layers)
+        self.layer = layers - 1
+        rng = np.random.default_rng(seed)
+        per = self.cache.pages_per_seq()
+        table = rng.permutation((max(self.seqs) + 1) * per).reshape(-1, per)
+        for s in range(max(self.seqs) + 1):
+            self.cache.set_page_table(s, table[s])
+        # slots behind the batch hold other data (NaN in the pages' own memory, where it can be reached)
+        if kind != "4":
+            for which in ("k", "v"):
+                torch.as_tensor(self.cache.kv_pool(which), device="cuda").fill_(-1 if kind == "bf16" else float("nan"))
+            torch.cuda.synchronize()
+        self.values, bufs = [], []
+        for t, c in zip(lens, counts):
+            kv = [rng.standard_normal((t + c, kvh, hd)).astype(np.float32) + rng.standard_normal((kvh, hd)).astype(np.float32)
+                  for _ in range(2)]
+            if edit:
+                edit(len(bufs), kv)
+            bufs.append(kv)
+            self.values.append([torch.from_numpy(self.held(x)).cuda() for x in kv])
+        at = [i for i, (t, c) in enumerate(zip(lens, counts)) if t + c]
+        rows = self.ctx.rowBatch([lens[i] + counts[i] for i in at], [self.seqs[i] for i in at])
+        self.append(rows, *(f32(self.ctx, np.concatenate([bufs[i][w] for i in at])) for w in (0, 1)))
+        for s, t in zip(self.seqs, lens):
+            self.cache.set_t0(s, t)
+        self.rows = self.ctx.rowBatch(counts, self.seqs)
+
+    def held(self, x):
+        if self.kind == "4":
+            return codes64(x)[0]
+        if self.kind == "bf16":
+            return torch_().from_numpy(x).bfloat16().double().numpy()
+        return x.astype(np.float64)
+
+    def append(self, rows, k, v):
+        (self.cache.append if self.kind == "4" else self.cache.append_rows)(self.layer, rows, k, v)
+
+    def attend(self, q, window=0, sinks=0, rows=None, out=None):
+        fn = self.cache.attention if self.kind == "4" else self.cache.window_attention
+        return fn(self.layer, rows or self.rows, q, out, window=window, sinks=sinks)
+
+    def close(self):
+        self.cache.close()
+        self.ctx.close()
+
+
+def attend64(R, q, window, sinks):
+    """The definition, with per row the largest visible |v| and the largest visible sum of |q_i k_i|
+    in powers of two (what the error bound is made of), each [n, NQ, ...]."""
+    torch = torch_()
+    G, outs, vmax, amax, row = R.nq // R.kvh, [], [], [], 0
+    for (k, v), t0, m in zip(R.values, R.lens, R.counts):
+        if not m:
+            continue
+        qq = torch.from_numpy(q[row:row + m]).cuda().double()
+        row += m
+        slot, at = torch.arange(t0, t0 + m, device="cuda")[:, None], torch.arange(t0 + m, device="cuda")[None]
+        see = at <= slot
+        if window:
+            see &= (at > slot - window) | (at < sinks)
+        for h0 in range(0, R.kvh):
+            kk, vv = torch.nan_to_num(k[:, h0]), torch.nan_to_num(v[:, h0])
+            z = torch.einsum("mgd,td->mgt", qq[:, h0 * G:(h0 + 1) * G], kk) / math.sqrt(R.hd)
+            p = torch.softmax(torch.where(see[:, None], z, -math.inf), -1)
+            outs.append(torch.einsum("mgt,td->mgd", p, vv))
+            a = torch.einsum("mgd,td->mgt", qq[:, h0 * G:(h0 + 1) * G].abs(), kk.abs())
+            amax.append(torch.where(see[:, None], a, 0).amax(-1) * (math.log2(math.e) / math.sqrt(R.hd)))
+            vm = torch.where(see[..., None], vv.abs()[None], 0).amax((1, 2)) if m * vv.numel() < 1e8 else vv.abs().max().expand(m)
+            vmax.append(vm[:, None].expand(m, G))
+    group = lambda xs: np.concatenate([np.concatenate([x.cpu().numpy() for x in xs[i:i + R.kvh]], 1)  # noqa: E731
+                                       for i in range(0, len(xs), R.kvh)])
+    return group(outs), group(vmax), group(amax)
+
+
+def attention_bound(R, vmax, amax):
+    """A score sums hd products in at most hd / 8 + 6 truncated steps of 2^-23 of the sum of
+    magnitudes (operands cut to 22 bits or more count as two of the six; 4-bit rows add codes and
+    minima, each at most three times the value they make up): e. Every p is off by e ln 2 and the
+    exponential's 2^-21 relative, which counts twice (numerator and sum); a block's product adds up
+    to 20 truncated steps of 2^-23, the blocks one rounding each, the join and the quotient a few."""
+    e = (R.hd / 8 + 6) * 2.0 ** -23 * amax * (3 if R.kind == "4" else 1)
+    slots = max(t + c for t, c in zip(R.lens, R.counts))
+    return (vmax * (2 * (0.7 * e + 2.0 ** -21) + (28 + slots / 64) * 2.0 ** -23 * (3 if R.kind == "4" else 1)))[:, :, None]
+
+
+def check_attention(R, window=0, sinks=0, seed=1, scale=1.5):
+    n = sum(R.counts)
+    q = np.random.default_rng(seed).standard_normal((n, R.nq, R.hd)).astype(np.float32) * np.float32(scale)
+    out = R.attend(f32(R.ctx, q), window, sinks)
+    got = R.ctx.readF32(out, out.n).reshape(n, R.nq, R.hd)
+    want, vmax, amax = attend64(R, q, window, sinks)
+    err, bound = np.abs(got - want), attention_bound(R, vmax, amax)
+    assert np.isfinite(got).all()
+    assert (err <= bound).all(), f"worst {float((err / bound).max())} of the bound, {float(err.max())}"
+    # on average the errors are far inside the worst case; fp32 level
+    assert np.linalg.norm(got - want) <= 4e-6 * np.linalg.norm(want)
+    return got
+
+
+KINDS = ["bf16", "f32", "4"]
+HEAD_SHAPES = [(4, 2, 64), (7, 1, 64), (8, 1, 128), (6, 2, 128), (3, 3, 128)]
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("page", [32, 64, 256])
+def test_cache4_rows(dllm, hd, page):
+    """The values are the definition's, bit for bit, and each is within half a scale of its own."""
+    rng = np.random.default_rng(hd)
+    ctx = make_ctx(dllm, 6, 3, hd, max_pos=600, max_seqs=4, num_layers=2, kv_page_size=page)
+    cache = dllm.Cache4(ctx, 0, 2)
+    per = cache.pages_per_seq()
+    table = rng.permutation(4 * per).reshape(4, per)
+    for s in range(4):
+        cache.set_page_table(s, table[s])
+        cache.set_t0(s, [0, 59, 31, 300][s])
+    assert cache.size == 2 * 2 * 4 * per * page * 3 * hd * 5 // 8
+    rows = ctx.rowBatch([3, 0, 130, 1], [2, 0, 3, 1])
+    n = rows.n
+    kv = []
+    for w in range(2):
+        x = rng.standard_normal((n, 3, hd)).astype(np.float32) * np.float32(10.0) ** rng.integers(-6, 7, (n, 3, 1)).astype(np.float32)
+        x[0, 0, :32] = 0  # a group of zeros, of one value, of negative values, of bf16 values, with an offset
+        x[1, 0, :32] = np.float32(1 / 3)
+        x[2, 0, :32] = -np.abs(x[2, 0, :32])
+        x[3, 1, :32] = cut(x[3, 1, :32])
+        x[4, 1] += np.float32(1000)
+        x[5, 2, :32] = np.arange(32) % 16  # codes with nothing to round
+        x[6, 2, :32] = np.float32(1e-41) * np.arange(32)  # subnormal
+        kv.append(x)
+    other = [f32(ctx, np.full((n, 3, hd), 7)) for _ in range(2)]
+    cache.append(0, rows, *other)
+    cache.append(1, rows, *(f32(ctx, x) for x in kv))
+    for got, x in zip(cache.read_rows(1, rows), kv):
+        got = ctx.readF32(got, got.n).reshape(x.shape)
+        want, scale = codes64(x)
+        assert np.array_equal(got, want.astype(np.float32))
+        assert (np.abs(got.astype(np.float64) - x) <= scale / 2 * (1 + 2.0 ** -20) + np.abs(x) * 2.0 ** -22).all()
+    for got in cache.read_rows(0, rows):
+        assert (ctx.readF32(got, got.n) == 7).all()
+    # one of the two only; rows behind the batch stay as they are
+    only = f32(ctx, np.full((n + 2) * 3 * hd, 5))
+    cache.read_rows(1, rows, vOut=only)
+    got = ctx.readF32(only, only.n).reshape(n + 2, 3, hd)
+    assert np.array_equal(got[:n], codes64(kv[1])[0].astype(np.float32)) and (got[n:] == 5).all()
+    ctx.close()
+
+
+def test_cache4_without_a_number(dllm):
+    """NaN, infinities and ranges of 2^112 make NaN of their 32 values, and of no others."""
+    ctx = make_ctx(dllm, 2, 1, 128, max_pos=64)
+    cache, rows = dllm.Cache4(ctx, 0, 1), ctx.rowBatch([5])
+    x = np.random.default_rng(0).standard_normal((5, 128)).astype(np.float32)
+    for i, v in enumerate([np.nan, np.inf, -np.inf]):
+        x[i, 40] = v
+    x[3, 3], x[3, 4] = 3e38, -3e38
+    x[4] = np.float32(2.0 ** 111) * np.sign(x[4]) * np.float32(0.5)  # a range just inside
+    k = f32(ctx, x)
+    cache.append(0, rows, k, k)
+    got = ctx.readF32(cache.read_rows(0, rows)[0], 640).reshape(5, 4, 32)
+    bad = np.zeros((5, 4), bool)
+    bad[:3, 1] = bad[3, 0] = True
+    assert np.isnan(got[bad]).all()
+    assert np.array_equal(got[~bad], codes64(x)[0].reshape(5, 4, 32)[~bad].astype(np.float32))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("page", [32, 128])
+def test_stage_append_rows(dllm, kind, page):
+    R = Rows(dllm, 4, 2, 64, kind, [100, 0, 7], [0, 33, 1], page=page, seqs=[2, 0, 1], layers=2)
+    for s, want, n in zip(R.seqs, R.values, (100, 33, 8)):
+        for which, w in (("k", 0), ("v", 1)):
+            got = getattr(R.cache.kv[1], which).read(0, n, s)
+            assert np.array_equal(got, want[w].reshape(n, -1).cpu().numpy())
+    assert R.cache.t0_of(2) == 100 and R.cache.t0_of(0) == 0
+    R.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("nq,kvh,hd", HEAD_SHAPES)
+@pytest.mark.parametrize("m", [1, 2, 5, 9, 40, 130])
+@pytest.mark.parametrize("t0", [0, 1, 63, 333])
+def test_window_attention_small(dllm, kind, nq, kvh, hd, m, t0):
+    R = Rows(dllm, nq, kvh, hd, kind, [t0], [m])
+    for window, sinks in ((0, 0), (1, 0), (1, 3), (37, 0), (100, 4), (64, 64), (200, 130), (10000, 7), (0, 9)):
+        check_attention(R, window, sinks)
+    R.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("t0,m,page,window,sinks", [(4095, 1, 64, 0, 0), (5000, 3, 32, 4096, 4), (3001, 300, 128, 1000, 5),
+                                                    (9999, 2, 64, 8192, 1), (2500, 513, 64, 0, 0), (0, 1025, 64, 0, 0),
+                                                    (20000, 1, 64, 128, 64)])
+def test_window_attention_long(dllm, kind, t0, m, page, window, sinks):
+    R = Rows(dllm, 14, 2, 64 if m % 2 else 128, kind, [t0], [m], page=page)
+    check_attention(R, window, sinks)
+    R.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("page", [32, 64, 256])
+def test_window_attention_batch(dllm, kind, page):
+    """Decode steps, chunks and a sequence without rows in one batch, in another order than the
+    cache's."""
+    lens, counts = [700, 0, 33, 2100, 64, 5], [1, 300, 0, 1, 77, 30]
+    R = Rows(dllm, 12, 2, 128, kind, lens, counts, page=page, max_pos=2300, seqs=[3, 0, 5, 1, 7, 2])
+    for window, sinks in ((0, 0), (256, 4), (50, 70)):
+        check_attention(R, window, sinks)
+    R.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_window_attention_many_sequences(dllm, kind):
+    lens = [(37 * i) % 900 for i in range(128)]
+    R = Rows(dllm, 4, 1, 64, kind, lens, [1 + (i % 29 == 3) * 70 for i in range(128)])
+    check_attention(R)
+    check_attention(R, 128, 2)
+    R.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m", [1, 4, 200])
+def test_window_attention_sharp_rows(dllm, kind, m):
+    """Scores in the hundreds: one slot takes almost all, and maxima move late."""
+    R = Rows(dllm, 8, 2, 128, kind, [1500], [m])
+    check_attention(R, scale=40.0)
+    check_attention(R, 600, 3, scale=40.0)
+    R.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m", [1, 6, 150])
+@pytest.mark.parametrize("size", [2.0 ** -90, 2.0 ** 60])
+def test_window_attention_small_and_large_values(dllm, kind, m, size):
+    """V of any size and K of sizes that go with q: nothing is lost to a type's range. (q and K
+    together make scores of ordinary size.)"""
+    def edit(_, kv):
+        kv[0] /= np.float32(size)
+        kv[1] *= np.float32(size)
+        kv[1][::3] *= np.float32(2.0 ** -20)  # and rows of very unequal sizes
+    R = Rows(dllm, 6, 2, 64, kind, [300], [m], edit=edit)
+    check_attention(R, 0, 0, scale=1.5 * size)
+    check_attention(R, 90, 3, scale=1.5 * size)
+    R.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m", [1, 8, 90, 300])
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+def test_hidden_rows_do_not_leak(dllm, kind, m, value):
+    """Non-finite K and V rows: those no row sees change nothing; those that some rows see make
+    these rows non-finite, in the dims concerned, and no others."""
+    t0, window, sinks = 200, 70, 6
+    hidden, seen = (6, 9, 64, 129), ((t0 + m - 1,) if m > 1 else ())
+
+    def edit(_, kv):
+        for s in hidden:
+            kv[0][s] = kv[1][s] = value
+        for s in seen:
+            kv[1][s, :, 5] = value
+    R = Rows(dllm, 8, 2, 64, kind, [t0], [m], edit=edit)
+    n = m
+    q = np.random.default_rng(3).standard_normal((n, 8, 64)).astype(np.float32)
+    out = R.attend(f32(R.ctx, q), window, sinks)
+    got = R.ctx.readF32(out, out.n).reshape(n, 8, 64)
+    want, vmax, amax = attend64(R, q, window, sinks)
+    bad = np.zeros((n, 8, 64), bool)
+    if seen:  # 4 bits: the whole group of 32
+        bad[-1, :, 0:32 if R.kind == "4" else 6] = True
+        if R.kind != "4":
+            bad[-1, :, :5] = False
+    assert (~np.isfinite(got[bad])).all()
+    assert np.isfinite(got[~bad]).all()
+    err, bound = np.abs(got - want), np.broadcast_to(attention_bound(R, vmax, amax), got.shape)
+    assert (err[~bad] <= bound[~bad]).all()
+    R.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_rows_one_by_one_and_in_chunks(dllm, kind):
+    """A prompt in one chunk, in chunks of 17, and token by token sees the same; and what lies
+    behind the rows of a call is not written."""
+    t = 90
+    R = Rows(dllm, 4, 2, 64, kind, [0], [t])
+    q = np.random.default_rng(2).standard_normal((t, 256)).astype(np.float32)
+    whole = R.attend(f32(R.ctx, q), 33, 2)
+    whole = R.ctx.readF32(whole, whole.n).reshape(t, 256)
+    for step in (17, 1):
+        for a in range(0, t, step):
+            e = min(t, a + step)
+            R.cache.set_t0(0, a)
+            buf = f32(R.ctx, np.full((e - a + 1) * 256, 9))
+            R.attend(f32(R.ctx, q[a:e]), 33, 2, rows=R.ctx.rowBatch([e - a]), out=buf)
+            got = R.ctx.readF32(buf, buf.n).reshape(-1, 256)
+            assert (got[-1] == 9).all()
+            # two results within the bound of the definition; 4e-6 of their size on average
+            assert np.linalg.norm(got[:-1] - whole[a:e]) <= 8e-6 * np.linalg.norm(whole[a:e])
+    R.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_two_runs_give_the_same_bits(dllm, kind):
+    R = Rows(dllm, 12, 2, 128, kind, [3000, 40], [1, 200])
+    q = f32(R.ctx, np.random.default_rng(0).standard_normal(201 * 12 * 128))
+    a, b = R.attend(q), R.attend(q)
+    assert np.array_equal(R.ctx.readF32(a, a.n), R.ctx.readF32(b, b.n))
+    R.close()
+
+
+# ---- refusals -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["bf16", "4"])
+def test_rows_refusals(dllm, kind):
+    R = Rows(dllm, 4, 2, 64, kind, [10, 5], [2, 1], max_pos=40)
+    ctx, rows = R.ctx, R.rows
+    for counts, seqs in (([], None), ([0, 0], None), ([-1], None), ([41], None), ([1, 1], [0, 0]), ([1], [-1]),
+                         ([1] * 129, None), ([1, 1], [0])):
+        with pytest.raises(dllm.DllmError):
+            ctx.rowBatch(counts, seqs)
+    q, k = ctx.createF32(3 * 256), ctx.createF32(3 * 128)
+    fine = lambda **kw: R.attend(q, **kw)  # noqa: E731
+    fine()
+    for bad in (lambda: fine(window=-1), lambda: fine(sinks=-1), lambda: fine(window=2 ** 31), lambda: fine(out=q),
+                lambda: R.attend(k), lambda: fine(out=k), lambda: fine(rows=ctx.rowBatch([1], [2])),
+                lambda: R.append(rows, q, ctx.createF32(3 * 128 - 1)), lambda: R.append(ctx.rowBatch([1], [9]), k, k)):
+        with pytest.raises(dllm.DllmError):
+            bad()
+    with pytest.raises(ValueError):
+        R.attend(q, rows=k)
+    with pytest.raises(ValueError):
+        R.append(rows, k, rows)
+    R.cache.set_t0(0, 39)  # no room for two rows
+    for bad in (lambda: fine(), lambda: R.append(rows, k, k)):
+        with pytest.raises(dllm.KvOverflowError):
+            bad()
+    R.cache.set_t0(0, 38)
+    fine()
+    fine(window=2 ** 31 - 1, sinks=2 ** 31 - 1)
+    R.layer = 1
+    for bad in (lambda: fine(), lambda: R.append(rows, k, k)):
+        with pytest.raises(dllm.DllmError):
+            bad()
+    other = make_ctx(dllm, 4, 2, 64, max_pos=40)
+    R.layer = 0
+    with pytest.raises(dllm.DllmError):
+        fine(rows=other.rowBatch([1, 1]))
+    R.close()
+
+
+def test_cache4_refusals(dllm):
+    ctx = make_ctx(dllm, 4, 2, 64, max_pos=100, max_seqs=2)
+    for a, b in ((-1, 1), (1, 0), (0, 3)):
+        with pytest.raises(dllm.DllmError):
+            dllm.Cache4(ctx, a, b)
+    cache, rows = dllm.Cache4(ctx, 1, 2), ctx.rowBatch([2])
+    k = ctx.createF32(2 * 128)
+    for bad in (lambda: cache.append(0, rows, k, k), lambda: cache.read_rows(1, rows, k, k),
+                lambda: cache.read_rows(1, rows, ctx.createF32(255)), lambda: cache.set_t0(2, 0), lambda: cache.set_t0(0, 101),
+                lambda: cache.set_t0(0, -1), lambda: cache.set_page_table(0, [0]), lambda: cache.set_page_table(0, [0, 0]),
+                lambda: cache.set_page_table(0, [0, 4]), lambda: cache.set_page_table(2, [0, 1]),
+                lambda: cache.set_page_table(0, [0, 2 ** 32 + 1])):
+        with pytest.raises((dllm.DllmError, IndexError)):
+            bad()
+    assert cache.t0_of(2) == -1 and cache.pages_per_seq() == 2
+    cache.set_t0(1, 5)
+    cache.reset()
+    assert cache.t0_of(1) == 0
+    cache.close()
+    with pytest.raises(dllm.DllmError):
+        cache.append(1, rows, k, k)
+    assert cache.t0_of(0) == -1 and cache.size == 0
+
+
+# ---- streams, graphs, and all of them together --------------------------------------------------------
+@pytest.mark.parametrize("kind", KINDS)
+def test_rows_on_a_side_stream_and_in_a_captured_graph(dllm, kind):
+    """A decode step of a host's own layer (norm + rotation, append, attention) captured once and
+    replayed with other inputs gives what the calls give."""
+    torch = torch_()
+    R = Rows(dllm, 8, 2, 128, kind, [500, 30], [1, 1], max_pos=600)
+    ctx = R.ctx
+    rng = np.random.default_rng(0)
+    make = lambda w: rng.standard_normal(2 * w * 128).astype(np.float32)  # noqa: E731
+    steps = [[make(8), make(2), make(2)] for _ in range(3)]
+    plan, pos, w = ctx.ropePlan(), i32(ctx, [500, 30]), bf16(ctx, np.ones(128))
+    q, k, v, out = ctx.createF32(2 * 1024), ctx.createF32(2 * 256), ctx.createF32(2 * 256), ctx.createF32(2 * 1024)
+    qt, kt = ctx.createF32(2 * 1024), ctx.createF32(2 * 256)
+
+    def step():
+        ctx.normRopeAt(plan, pos, 2, q, k, w, w, qt, kt)
+        R.append(R.rows, kt, v)
+        R.attend(qt, 300, 4, out=out)
+    want = []
+    for s in steps:
+        for b, x in zip((q, k, v), s):
+            ctx.writeF32(b, x)
+        step()
+        want.append(ctx.readF32(out, out.n))
+    ctx.synchronize()
+    stream = torch.cuda.Stream()
+    ctx.set_stream(stream.cuda_stream)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        step()
+        for refused in (lambda: ctx.rowBatch([1]), lambda: dllm.Cache4(ctx, 0, 1), lambda: R.cache.set_page_table(0, range(R.cache.pages_per_seq()))):
+            with pytest.raises(dllm.DllmError):
+                refused()
+    for s, x in zip(steps, want):
+        for b, a in zip((q, k, v), s):
+            ctx.writeF32(b, a)
+        with torch.cuda.stream(stream):
+            g.replay()
+        assert np.array_equal(ctx.readF32(out, out.n), x)
+    ctx.set_stream(None)
+    del g
+    R.close()
+
+
+def test_a_conversation(dllm):
+    """A host's own layer through a conversation: a prompt in two chunks beside another sequence's
+    decode steps, then decode steps, with windows and sinks, over the cache in 4 bits and over a
+    stage's: every step is the definition's on what the caches hold."""
+    nq, kvh, hd, window, sinks = 6, 2, 64, 40, 3
+    rng = np.random.default_rng(5)
+    ctx = make_ctx(dllm, nq, kvh, hd, max_pos=256, max_seqs=2, kv_dtype="f32")
+    stage, cache = dllm.Stage(ctx, 0, 1), dllm.Cache4(ctx, 0, 1)
+    plan = ctx.ropePlan(rotary_dim=48)
+    f, factor = frequencies(48, ctx.cfg.rope_theta, None)
+    qn, kn = (cut(1 + 0.2 * rng.standard_normal(hd)) for _ in range(2))
+    qw, kw = bf16(ctx, qn), bf16(ctx, kn)
+    held = [[np.zeros((0, kvh, hd)) for _ in range(2)] for _ in range(2)]  # fp32 K, V of each sequence
+    for counts in ([60, 0], [41, 5], [1, 1], [1, 1], [0, 1]):
+        rows, n = ctx.rowBatch(counts), sum(counts)
+        assert [stage.t0_of(s) for s in (0, 1)] == [len(h[0]) for h in held] == [cache.t0_of(s) for s in (0, 1)]
+        pos = np.concatenate([np.arange(len(held[s][0]), len(held[s][0]) + counts[s]) for s in (0, 1)])
+        q, k, v = (rng.standard_normal((n, h, hd)).astype(np.float32) for h in (nq, kvh, kvh))
+        qb, kb, vb = f32(ctx, q), f32(ctx, k), f32(ctx, v)
+        ctx.normRopeAt(plan, i32(ctx, pos), n, qb, kb, qw, kw)
+        qt = ctx.readF32(qb, qb.n).reshape(q.shape)
+        kt = ctx.readF32(kb, kb.n).reshape(k.shape)
+        for x, w, got in ((q, qn, qt), (k, kn, kt)):
+            y, mag = rope64(norm64(x, w, 1e-6), pos, 48, "half", f, factor)
+            assert np.abs(got - y).max() <= 24 * EPS * max(mag.max(), np.abs(y).max())
+        stage.append_rows(0, rows, kb, vb)
+        cache.append(0, rows, kb, vb)
+        at = 0
+        for s in (0, 1):
+            held[s] = [np.concatenate([h, x[at:at + counts[s]]]) for h, x in zip(held[s], (kt, v))]
+            at += counts[s]
+        for kind, out in (("f32", stage.window_attention(0, rows, qb, window=window, sinks=sinks)),
+                          ("4", cache.attention(0, rows, qb, window=window, sinks=sinks))):
+            R = object.__new__(Rows)
+            R.kind, R.nq, R.kvh, R.hd = kind, nq, kvh, hd
+            R.counts, R.lens = counts, [len(h[0]) - c for h, c in zip(held, counts)]
+            R.values = [[torch_().from_numpy(Rows.held(R, x.astype(np.float32))).cuda() for x in h] for h in held]
+            want, vmax, amax = attend64(R, qt, window, sinks)
+            got = ctx.readF32(out, out.n).reshape(want.shape)
+            assert (np.abs(got - want) <= attention_bound(R, vmax, amax)).all()
+        for s in (0, 1):
+            stage.set_t0(s, len(held[s][0]))
+            cache.set_t0(s, len(held[s][0]))
+    ctx.close()
