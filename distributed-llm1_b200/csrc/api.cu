@@ -90,6 +90,10 @@ struct dllm_ctx {
   float* tree_part = nullptr;
   // partial results of split attention of rows, sized for any call; allocated with the first batch
   float* rows_part = nullptr;
+  // fp16 K and V blocks of long chunks. Grown by replacement: captured graphs may still refer to the
+  // earlier ones, which stay until the ctx goes.
+  std::vector<void*> rows_planes;
+  size_t rows_planes_bytes = 0;
   // token picks: per-row keys, then arrival counters (zero between calls)
   unsigned long long* pick_best = nullptr;
   // freed buffers kept for reuse, by size in bytes
@@ -874,6 +878,21 @@ int rows_attention(dllm_ctx* c, const char* what, dllm::RowsAttnArgs& a, const d
   a.err = c->err_dev;
   a.part_o = c->rows_part;
   a.part_ml = c->rows_part + dllm::rows_attn_part_rows(c->sms) * f.head_dim;
+  const size_t need = dllm::rows_attn_planes_bytes(a, b, kind, f.head_dim);
+  if (need > c->rows_planes_bytes) {
+    if (int rc = refuse_capture(c, "attention of a longer chunk than any call before")) return rc;
+    const size_t bytes = std::max(need, std::min(2 * c->rows_planes_bytes, (size_t)1 << 30));
+    void* p = nullptr;
+    const cudaError_t e = cudaMalloc(&p, bytes);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return set_err(c, DLLM_ENOMEM, "%s: scratch of %zu bytes: %s", what, bytes, cudaGetErrorString(e));
+    }
+    c->rows_planes.push_back(p);
+    c->rows_planes_bytes = bytes;
+  }
+  a.planes = c->rows_planes.empty() ? nullptr : c->rows_planes.back();
+  a.planes_bytes = c->rows_planes_bytes;
   int launches = 0;
   const cudaError_t e = dllm::op_rows_attention(a, b, kind, f.head_dim, c->sms, &launches, c->stream);
   c->launches += launches;
@@ -1024,6 +1043,7 @@ void ctx_free(dllm_ctx* c) {
   dev_free(c->tc_scratch);
   dev_free(c->tree_part);
   dev_free(c->rows_part);
+  for (void* p : c->rows_planes) dev_free(p);
   dev_free(c->pick_best);
   for (auto& kv : c->buf_cache) cudaFree(kv.second);
   c->buf_cache.clear();
@@ -2860,10 +2880,6 @@ int dllm_stage_window_attention(dllm_stage* s, int layer, const dllm_rows* rows,
   a.kc = layer_pool(s, s->kpool, layer);
   a.vc = layer_pool(s, s->vpool, layer);
   a.pages = stage_pages(s);
-  if (!s->kv_mapped) return set_err(c, DLLM_ECUDA, "window_attention: the driver has no tensor map of the KV cache");
-  a.tc_k = &s->kv_map[0];
-  a.tc_v = &s->kv_map[1];
-  a.tc_row0 = (int)((size_t)(layer - s->start) * s->layer_elems / c->cfg.head_dim);
   return rows_attention(c, "window_attention", a, b, rows->n, c->cfg.kv_dtype == DLLM_KV_F32 ? dllm::kKvF32 : dllm::kKvBf16, q,
                         out, window, sinks);
 }

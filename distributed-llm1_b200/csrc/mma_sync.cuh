@@ -68,5 +68,23 @@ DLLM_DEV void split3(float x, float y, uint32_t& h, uint32_t& m, uint32_t& l) {
   l = pack_bf16(x, y);
 }
 DLLM_DEV bool is_finite(float v) { return fabsf(v) <= 3.402823466e38f; }
+DLLM_DEV uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+DLLM_DEV void unpack_f16(uint32_t u, float& lo, float& hi) {
+  asm("{\n\t.reg .f16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}"
+      : "=f"(lo), "=f"(hi)
+      : "r"(u));
+}
+// (x, y) -> two packed fp16 pairs whose sums are x and y to 2^-22 of them, or to 2^-25.
+DLLM_DEV void split2_f16(float x, float y, uint32_t& h, uint32_t& l) {
+  h = pack_f16(x, y);
+  float a, b;
+  unpack_f16(h, a, b);
+  l = pack_f16(x - a, y - b);
+}
+DLLM_DEV float power_of_two(int biased) { return __uint_as_float((uint32_t)biased << 23); }
 
 }  // namespace dllm

@@ -32,6 +32,7 @@
 #include <vector>
 
 #include "mma_sync.cuh"
+#include "rows_attn_tc.cuh"
 
 namespace dllm {
 namespace {
@@ -45,23 +46,6 @@ DLLM_DEV void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-DLLM_DEV uint32_t pack_f16(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-DLLM_DEV void unpack_f16(uint32_t u, float& lo, float& hi) {
-  asm("{\n\t.reg .f16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}"
-      : "=f"(lo), "=f"(hi)
-      : "r"(u));
-}
-// (x, y) -> two packed fp16 pairs whose sums are x and y to 2^-22 of them, or to 2^-25.
-DLLM_DEV void split2_f16(float x, float y, uint32_t& h, uint32_t& l) {
-  h = pack_f16(x, y);
-  float a, b;
-  unpack_f16(h, a, b);
-  l = pack_f16(x - a, y - b);
-}
 // Nibbles 0 and 4 of u, less 8, as packed fp16.
 DLLM_DEV uint32_t codes_f16(uint32_t u) {
   uint32_t r;
@@ -70,7 +54,6 @@ DLLM_DEV uint32_t codes_f16(uint32_t u) {
       : "r"(u), "r"(0x64086408u));
   return r;
 }
-DLLM_DEV float power_of_two(int biased) { return __uint_as_float((uint32_t)biased << 23); }
 DLLM_DEV void cp8_zfill(uint32_t dst, const void* src, bool real) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(real ? 8 : 0) : "memory");
 }
@@ -844,7 +827,7 @@ cudaError_t launch_split(const RowsAttnArgs& a, const RowsBatch& s, int rt, int 
     if ((ctas <= sms || items >= sms) && part <= (long long)rows_attn_part_rows(sms)) break;
     P.bps += 1 + P.bps / 64;
   }
-  int splits = 1, part = 0, item = 0, join = 0;
+  int splits = 1, part = 0, item = 0, join = 0, units = 0;
   for (int i = 0; i < s.n_seqs; ++i) {
     P.seq[i] = s.seq[i], P.row0[i] = s.row0[i], P.m[i] = s.m[i], P.t0[i] = s.t0[i];
     int most = 1;
@@ -853,13 +836,16 @@ cudaError_t launch_split(const RowsAttnArgs& a, const RowsBatch& s, int rt, int 
     P.item0[i] = item;
     P.part0[i] = part;
     P.join0[i] = join;
+    P.unit0[i] = units;
+    units += kvh * RowsView(s.t0[i], s.t0[i] + s.m[i] - 1, a.window, a.sinks, bn).nb;
     item += (first[i + 1] - first[i]) * kvh * most;
     if (most > 1) part += most * s.m[i] * a.nq, join += s.m[i] * a.nq;
     splits = std::max(splits, most);
   }
   P.item0[s.n_seqs] = item;
   P.join0[s.n_seqs] = join;
-  cudaError_t e = main(P, item);
+  P.unit0[s.n_seqs] = units;
+  cudaError_t e = main(P, item, units);
   *launches += 1;
   if (e != cudaSuccess || splits == 1) return e;
   const bool many = splits > 8;
@@ -879,30 +865,91 @@ cudaError_t launch_split(const RowsAttnArgs& a, const RowsBatch& s, int rt, int 
 template <int KIND, int HD, int WR>
 cudaError_t launch(const RowsAttnArgs& a, const RowsBatch& s, int sms, int* launches, cudaStream_t st) {
   using T = Tile<KIND, HD, WR>;
-  return launch_split<HD>(a, s, T::RT, T::BN, sms, launches, st, [&](const RowsKernelArgs& P, int ctas) {
+  return launch_split<HD>(a, s, T::RT, T::BN, sms, launches, st, [&](const RowsKernelArgs& P, int ctas, int) {
     rows_attn_kernel<KIND, HD, WR><<<ctas, kThreads, T::kSmem, st>>>(P);
     return cudaGetLastError();
   });
 }
 
+// Rows of a sequence that share a KV head, from which on it is a long chunk.
+constexpr int kLongRows = 65;
+bool is_long(const RowsAttnArgs& a, int m) { return m * (a.nq / a.pages.kvh) >= kLongRows; }
+
+// Scratch of one sequence's fp16 blocks: the blocks and their factors.
+size_t planes_units(const RowsAttnArgs& a, const RowsBatch& b, int i, int kind) {
+  return (size_t)a.pages.kvh * RowsView(b.t0[i], b.t0[i] + b.m[i] - 1, a.window, a.sinks, tc_block(kind)).nb;
+}
+constexpr size_t unit_bytes(int hd) { return (size_t)2 * 128 * 2 * hd + 16; }
+
+void add(RowsBatch& to, const RowsBatch& b, int i) {
+  const int k = to.n_seqs++;
+  to.seq[k] = b.seq[i], to.row0[k] = b.row0[i], to.m[k] = b.m[i], to.t0[k] = b.t0[i];
+}
+
 template <int KIND, int HD>
-cudaError_t launch_kind(const RowsAttnArgs& a, const RowsBatch& b, int sms, int* launches, cudaStream_t st) {
+cudaError_t launch_short(const RowsAttnArgs& a, const RowsBatch& b, int sms, int* launches, cudaStream_t st) {
   int rows = 0;  // of the largest sequence that share a KV head
   for (int i = 0; i < b.n_seqs; ++i) rows = std::max(rows, b.m[i] * (a.nq / a.pages.kvh));
-  if (rows == 0) return cudaSuccess;
   if (rows <= 16) return launch<KIND, HD, 1>(a, b, sms, launches, st);
   if constexpr (KIND != kKvF32)
     if (rows > 32) return launch<KIND, HD, 4>(a, b, sms, launches, st);
   return launch<KIND, HD, 2>(a, b, sms, launches, st);
 }
 
+template <int KIND, int HD>
+cudaError_t launch_long(RowsAttnArgs a, const RowsBatch& b, size_t units, int sms, int* launches, cudaStream_t st) {
+  a.info = static_cast<char*>(a.planes) + units * (unit_bytes(HD) - 16);
+  return launch_split<HD>(a, b, kTcTileRows, tc_block(KIND), sms, launches, st, [&](const RowsKernelArgs& P, int ctas, int n) {
+    *launches += 1;
+    return launch_rows_tc(P, KIND, HD, ctas, n, st);
+  });
+}
+
+// Sequences with few rows in one launch, those with many in another, or in several where their
+// fp16 blocks do not fit the scratch together.
+template <int KIND, int HD>
+cudaError_t launch_kind(const RowsAttnArgs& a, const RowsBatch& b, int sms, int* launches, cudaStream_t st) {
+  RowsBatch few;
+  few.n_seqs = 0;
+  for (int i = 0; i < b.n_seqs; ++i)
+    if (!is_long(a, b.m[i])) add(few, b, i);
+  cudaError_t e = few.n_seqs ? launch_short<KIND, HD>(a, few, sms, launches, st) : cudaSuccess;
+  RowsBatch many;
+  many.n_seqs = 0;
+  size_t units = 0;
+  for (int i = 0; e == cudaSuccess && i < b.n_seqs; ++i) {
+    if (!is_long(a, b.m[i])) continue;
+    const size_t u = planes_units(a, b, i, KIND);
+    if (u * unit_bytes(HD) > a.planes_bytes) return cudaErrorInvalidValue;
+    if ((units + u) * unit_bytes(HD) > a.planes_bytes) {
+      e = launch_long<KIND, HD>(a, many, units, sms, launches, st);
+      many.n_seqs = 0, units = 0;
+    }
+    add(many, b, i);
+    units += u;
+  }
+  if (e == cudaSuccess && many.n_seqs) e = launch_long<KIND, HD>(a, many, units, sms, launches, st);
+  return e;
+}
+
 }  // namespace
 
 size_t rows_attn_part_rows(int sms) { return (size_t)2 * sms * 256; }
 
+size_t rows_attn_planes_bytes(const RowsAttnArgs& a, const RowsBatch& b, int kind, int hd) {
+  size_t all = 0, most = 0;
+  for (int i = 0; i < b.n_seqs; ++i) {
+    if (!is_long(a, b.m[i])) continue;
+    const size_t n = planes_units(a, b, i, kind) * unit_bytes(hd);
+    all += n, most = std::max(most, n);
+  }
+  return std::max(most, std::min(all, (size_t)1 << 30));
+}
+
 cudaError_t configure_rows_attn() {
   cudaError_t e = configure_hd<64>();
   if (e == cudaSuccess) e = configure_hd<128>();
+  if (e == cudaSuccess) e = configure_rows_attn_tc();
   return e;
 }
 

@@ -56,12 +56,16 @@ struct RowsAttnArgs {
   int window, sinks;         // row at slot p sees s <= p where s > p - window or s < sinks
   float scale_log2;          // log2(e) / sqrt(hd)
   int* err;
-  const void *tc_k, *tc_v;   // host: tensor maps (CUtensorMap) of a bf16 cache's pools as rows of hd
-  int tc_row0;               // the layer's first row in them
+  void* planes;              // scratch for the K and V blocks of long chunks in fp16 (rows_attn_tc.cu)
+  size_t planes_bytes;
+  void* info;                // in it: the blocks' factors (set by op_rows_attention)
   float* part_o;             // [rows][hd] partial outputs of sequences that are split
   float* part_ml;            // [rows][2]
 };
 size_t rows_attn_part_rows(int sms);  // capacity of part_o / part_ml
+// The scratch a call wants: all its long chunks at once, but no more than 1 GB unless one
+// sequence needs it (the others take turns then).
+size_t rows_attn_planes_bytes(const RowsAttnArgs& a, const RowsBatch& b, int kind, int hd);
 cudaError_t configure_rows_attn();
 cudaError_t op_rows_attention(const RowsAttnArgs& a, const RowsBatch& b, int kind, int hd, int sms, int* launches,
                               cudaStream_t st);
@@ -104,6 +108,7 @@ struct RowsKernelArgs {
   int item0[kRowsMaxSeqs + 1];   // CTAs: tiles (the last first), KV heads, splits
   int splits[kRowsMaxSeqs];      // of the sequence's tile that has most
   int part0[kRowsMaxSeqs];       // first partial row of a split sequence
+  int unit0[kRowsMaxSeqs + 1];   // long chunks: (KV head, block) pairs before the sequence's
   int join0[kRowsMaxSeqs + 1];   // joined (row, query head) pairs, 0 for sequences that are not split
 };
 static_assert(sizeof(RowsKernelArgs) <= 8192, "kernel arguments");

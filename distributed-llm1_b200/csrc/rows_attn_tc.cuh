@@ -1,0 +1,33 @@
+// rows_attn_tc.cuh — the tile shapes of rows_attn_tc.cu, for the host that cuts a batch into
+// tiles, and its launchers.
+#pragma once
+
+#include "rows_attn.cuh"
+
+namespace dllm {
+
+constexpr int kTcThreads = 384;
+constexpr int kTcTileRows = 256;  // rows of a CTA
+constexpr int kTcRing = 6;        // tiles of the ring at most
+
+template <int KIND, int HD>
+struct TcTile {
+  static constexpr int kPlanes = KIND == kKvBf16 ? 1 : 2;
+  static constexpr int BN = 128 / kPlanes;               // slots of a block
+  static constexpr int BOX = HD / 64;                    // 64-dim boxes
+  static constexpr int kBox = 128 * 128;                 // bytes of 128 rows of a box
+  static constexpr int kTile = BOX * kBox;               // of a K or V block, and of one term of 128 rows of q
+  static constexpr int kRing = HD == 64 ? 6 : 3;         // K and V blocks under way
+  static constexpr int kOut = kTcTileRows * (HD + 6) * 4;  // the results, over q and the ring
+  static constexpr int kSmem = 1024 + (4 + kRing) * kTile;
+  static_assert(kOut <= (4 + kRing) * kTile, "results reuse the operands' memory");
+  static_assert(kSmem + 2048 <= 227 * 1024, "shared memory");
+};
+inline int tc_block(int kind) { return kind == kKvBf16 ? 128 : 64; }
+
+cudaError_t configure_rows_attn_tc();
+// `units`: (KV head, block) pairs of all sequences, 2 x 256 x head-size bytes each in a.planes
+// and 16 in a.info.
+cudaError_t launch_rows_tc(const RowsKernelArgs& P, int kind, int hd, int ctas, int units, cudaStream_t st);
+
+}  // namespace dllm

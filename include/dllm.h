@@ -430,7 +430,9 @@ void* dllm_stage_kv_device_ptr(const dllm_stage* st, int which);
  * one ctx, and graphs captured from them, must not overlap on the GPU), and T0 values are
  * those of the call: a captured call replays with them, and refers to the buffers it was
  * given. dllm_rows_create, dllm_kv4_create, dllm_kv4_set_page_table are refused while the
- * ctx stream is captured. */
+ * ctx stream is captured, and so is attention of a long chunk that needs more scratch than
+ * any call before: make the call once outside. (Scratch is 2 bytes per K or V value that long
+ * chunks see in a bf16 cache, 4 in the others, up to 1 GB or one sequence's share.) */
 
 /* For every head of q [n, NQ*HD] and k [n, KVH*HD] (either may be NULL, with its norm):
  * y = x / sqrt(mean(x^2) + rms_norm_eps) * norm, norm a bf16 weight [HD]; then the plan's
