@@ -16,8 +16,8 @@
 //   MMA (1 warp)        S = q K^T per tile and block, O = P V
 //   two softmax groups  128 threads each, one row per thread: S from tensor memory, online
 //                       softmax, P back over S as two fp16 terms, then O into registers
-// q and p run as two fp16 terms too (22 bits; each row of q by its own power of two, p as
-// 2^15 p), so a product takes two MMAs where K and V are one plane, three where they are two:
+// q and p run as two fp16 terms too (22 bits; each row of q by its own power of two, p between
+// 2^8 and 2^15 at its largest), so a product takes two MMAs where K and V are one plane, three where they are two:
 // the low terms first, so that only the last ones add at full size (the tensor core
 // truncates each addition); a block's P V starts from zero and the blocks are added in fp32
 // registers. With two planes S takes q_high (K_high | K_low) as one MMA of N = 128, and
@@ -116,24 +116,44 @@ __global__ void __launch_bounds__(kPlaneThreads) rows_planes_kernel(const __grid
 
 // ---- the main kernel ---------------------------------------------------------------------------
 struct TcShared {
-  uint64_t full[kTcRing], empty[kTcRing];
-  uint64_t s_full[2], p_ready[2], o_full[2];
+  uint64_t empty[kTcRing];
+  // What the MMA warp waits for, one barrier at a time: the first tile's P and V, its O and the next
+  // K (both in turn, so that the producer may run ahead), the second tile's P, its O.
+  uint64_t pv_ready[kTcTurns], ok_ready[kTcTurns], p1_ready, o1_done;
+  uint64_t s_full[2], o_full[2];  // the softmax groups' side
   uint64_t idle;
   uint32_t tmem;
   volatile int abort;
   float back[kTcTileRows];  // what a row of q was divided by, times 2^14
 };
+static_assert(sizeof(TcShared) <= 2048, "operands start 2048 bytes into shared memory");
 
-// 32 columns of this thread's lane to tensor memory.
-DLLM_DEV void tmem_st32(uint32_t addr, const uint32_t (&h)[16], const uint32_t (&l)[16]) {
+// 16 columns of this thread's lane from tensor memory, and 8 + 8 to it.
+DLLM_DEV void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(h[0]),
-      "r"(h[1]), "r"(h[2]), "r"(h[3]), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]), "r"(h[8]), "r"(h[9]), "r"(h[10]),
-      "r"(h[11]), "r"(h[12]), "r"(h[13]), "r"(h[14]), "r"(h[15]), "r"(l[0]), "r"(l[1]), "r"(l[2]), "r"(l[3]), "r"(l[4]),
-      "r"(l[5]), "r"(l[6]), "r"(l[7]), "r"(l[8]), "r"(l[9]), "r"(l[10]), "r"(l[11]), "r"(l[12]), "r"(l[13]), "r"(l[14]),
-      "r"(l[15]), "r"(addr)
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+DLLM_DEV void tmem_st16(uint32_t addr, const uint32_t (&h)[8], const uint32_t (&l)[8]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(h[0]),
+      "r"(h[1]), "r"(h[2]), "r"(h[3]), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]), "r"(l[0]), "r"(l[1]), "r"(l[2]), "r"(l[3]),
+      "r"(l[4]), "r"(l[5]), "r"(l[6]), "r"(l[7]), "r"(addr)
       : "memory");
+}
+DLLM_DEV float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Two values of p, below 2^16, as two fp16 terms each: the high one cut to 11 bits (its cut is
+// exact in fp16; below 2^-14 it rounds, by 2^-25 at most), the low one rounded.
+DLLM_DEV void split_p(float x, float y, uint32_t& h, uint32_t& l) {
+  const float a = __uint_as_float(__float_as_uint(x) & 0xffffe000u), b = __uint_as_float(__float_as_uint(y) & 0xffffe000u);
+  h = pack_f16(a, b);
+  l = pack_f16(x - a, y - b);
 }
 DLLM_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
@@ -141,11 +161,34 @@ DLLM_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* ba
                : "memory");
 }
 
+// The MMA's shared-memory descriptors (tc.cuh) as two words: the upper one is the same for all
+// operands here, and the lower one moves by constants. Built anew as 64-bit values, an MMA took 95
+// cycles to issue and 65 to run.
+constexpr uint32_t kDescHigh = 64u | 1u << 14 | 2u << 29;
+DLLM_DEV uint32_t desc_low(const void* tile, uint32_t leading) { return (smem_u32(tile) & 0x3FFFFu) >> 4 | leading << 16; }
+DLLM_DEV void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 x, {%1, %5};\n\t"
+      "mov.b64 y, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh));
+}
+DLLM_DEV void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 y, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh));
+}
+
 template <int KIND, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_constant__ RowsKernelArgs P) {
   using T = TcTile<KIND, HD>;
   constexpr int BN = T::BN, BOX = T::BOX;
-  extern __shared__ unsigned char smem_raw[];
+  extern __shared__ __align__(1024) unsigned char base[];
   __shared__ __align__(8) TcShared sh;
   const RowsAttnArgs& a = P.a;
   asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled; it waits for this grid's end
@@ -156,7 +199,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
 
   // the warp's number as a value that is the same in all its lanes by construction
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-  unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* sQ = base;  // [tile][term][box][128 rows][128 bytes]
   unsigned char* ring = base + 4 * T::kTile;
 
@@ -169,13 +211,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
   };
 
   if (tid == 0) {
-    for (int s = 0; s < T::kRing; ++s) mbar_init(&sh.full[s], 1), mbar_init(&sh.empty[s], 1);
-    for (int w = 0; w < 2; ++w) mbar_init(&sh.s_full[w], 1), mbar_init(&sh.p_ready[w], 128), mbar_init(&sh.o_full[w], 1);
+    for (int s = 0; s < T::kRing; ++s) mbar_init(&sh.empty[s], 1);
+    for (int i = 0; i < T::kTurns; ++i) mbar_init(&sh.pv_ready[i], 128 + 1), mbar_init(&sh.ok_ready[i], 1 + 1);
+    for (int w = 0; w < 2; ++w) mbar_init(&sh.s_full[w], 1), mbar_init(&sh.o_full[w], 1);
+    mbar_init(&sh.p1_ready, 128), mbar_init(&sh.o1_done, 1);
     mbar_init(&sh.idle, 1);
+    mbar_arrive(&sh.ok_ready[0]);  // the first scores wait for no O
     sh.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) {
+  if (warp == kTcSoftWarps) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512u));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -184,88 +229,97 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
 
-  if (warp >= 8) {
+  if (warp >= kTcSoftWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == 8 && lane == 0) {
-      // ---- producer: tile t is K of block t / 2 (even) or V
+    if (warp == kTcSoftWarps && lane == 0) {
+      // ---- producer: tile t is K of block t / 2 (even) or V. It reports to the barriers that the
+      // first tile's MMAs wait for: ok_ready of the block (K), pv_ready (V). A barrier's earlier turn, 2
+      // kTurns >= kRing tiles before, has ended: the stage's earlier tile came later, and is used up.
       int sent = 0;
       const unsigned char* planes = static_cast<const unsigned char*>(a.planes);
+      auto bar = [&](int t) { return t & 1 ? &sh.pv_ready[t / 2 % T::kTurns] : &sh.ok_ready[t / 2 % T::kTurns]; };
       for (int t = 0; t < 2 * nb; ++t) {
         const int s = t % T::kRing;
         if (!wait_phase(&sh.empty[s], ((uint32_t)(t / T::kRing) & 1u) ^ 1u, &sh.abort)) break;  // nothing is loaded over memory that may still be read
-        mbar_expect_tx(&sh.full[s], T::kTile);
+        mbar_expect_tx(bar(t), T::kTile);
         bulk_load(ring + s * T::kTile, planes + ((size_t)unit_of(k.v.slot0(k.b0 + t / 2, BN)) * 2 + (t & 1)) * T::kTile, T::kTile,
-                  &sh.full[s]);
+                  bar(t));
         sent = t + 1;
       }
-      // whatever happened to the others, the copies under way land before the CTA ends
-      for (int t = max(0, sent - T::kRing); t < sent; ++t) mbar_wait(&sh.full[t % T::kRing], (uint32_t)(t / T::kRing) & 1u);
-    } else if (warp == 9) {
-      // ---- MMA issuer. The whole warp runs the loop and one elected lane issues, so that the
-      // operands stay in uniform registers.
-      asm volatile("bar.sync 2, 288;" ::: "memory");  // q is there
+    } else if (warp == kTcSoftWarps + 1) {
+      // ---- MMA issuer. The whole warp runs the loop and one elected lane issues, so that the operands
+      // stay in uniform registers. Little more than one MMA queues up behind the running one, and a wait
+      // costs 100 to 200 cycles while shared memory serves the operands, even where nothing is left to wait
+      // for: so there is one for each of the four products of a block, and no more. (A warp per tile
+      // was slower: both tiles' MMAs then ran, and both softmaxes waited, at the same time.)
+      asm volatile("bar.sync 2, %0;" ::"n"(kTcSoft + 32) : "memory");  // q is there
       const uint32_t leader = elect_one();
       const uint32_t idesc = (1u << 4) | ((uint32_t)(128 >> 4) << 24);                // fp32 += fp16 x fp16, M = 128
       const uint32_t id_s = idesc | ((uint32_t)(128 >> 3) << 17);                     // N = 128 rows of K, K-major
       const uint32_t id_half = idesc | ((uint32_t)(64 >> 3) << 17);                   // the first 64 of them
       const uint32_t id_o = idesc | ((uint32_t)(HD >> 3) << 17) | (1u << 16);         // N = dims, B with N contiguous
-      auto full = [&](int t) {
-        wait_phase(&sh.full[t % T::kRing], (uint32_t)(t / T::kRing) & 1u, &sh.abort);
-        tc_fence_after();
-      };
+      constexpr uint32_t kTile16 = T::kTile >> 4, kBox16 = T::kBox >> 4;
+      const uint32_t q_low = desc_low(sQ, 1u), k_low = desc_low(ring, 1u), v_low = desc_low(ring, T::kBox >> 4);
       auto scores = [&](int w, int n) {
+        tc_fence_after();
         if (leader) {
-          const unsigned char* kb = ring + (2 * n % T::kRing) * T::kTile;
-          const unsigned char* qb = sQ + w * 2 * T::kTile;
-          const uint32_t d = tmem + (uint32_t)w * 128;
+          const int s = 2 * n % T::kRing;
+          const uint32_t d = tmem + (uint32_t)w * 128, q = q_low + (uint32_t)w * (2 * kTile16), kb = k_low + (uint32_t)s * kTile16;
           // the low term of q first; with two planes of K it comes second, into their half
 #pragma unroll
-          for (int term = 0; term < 2; ++term)
+          for (int term = 0; term < 2; ++term) {
+            const uint32_t qt = q + (T::kPlanes == 1 ? 1 - term : term) * kTile16;
 #pragma unroll
             for (int x = 0; x < BOX; ++x)
 #pragma unroll
               for (int kk = 0; kk < 4; ++kk) {
-                const uint64_t bd = umma_desc_sw128(kb + x * T::kBox) + 2ull * kk;
-                const int plane = T::kPlanes == 1 ? 1 - term : term;
-                const uint64_t ad = umma_desc_sw128(qb + plane * T::kTile + x * T::kBox) + 2ull * kk;
-                if (T::kPlanes == 2 && term == 1) umma_bf16(d + 64, ad, bd, id_half, 1u);
-                else umma_bf16(d, ad, bd, id_s, (uint32_t)(term || x || kk));
+                const uint32_t at = x * kBox16 + 2 * kk;
+                if (T::kPlanes == 2 && term == 1) mma_ss(d + 64, qt + at, kb + at, id_half, 1u);
+                else mma_ss(d, qt + at, kb + at, id_s, (uint32_t)(term || x || kk));
               }
-          if (w == tiles - 1) umma_commit(&sh.empty[2 * n % T::kRing]);
+          }
           umma_commit(&sh.s_full[w]);
+          if (w == tiles - 1) umma_commit(&sh.empty[s]);
         }
         __syncwarp();
       };
-      full(0);
+      auto output = [&](int w, int n) {
+        tc_fence_after();
+        if (leader) {
+          const int s = (2 * n + 1) % T::kRing;
+          const uint32_t p = tmem + (uint32_t)w * 128, d = p + 256u, vb = v_low + (uint32_t)s * kTile16;
+          // products (term of p, plane of V), the smallest first
+#pragma unroll
+          for (int i = 0; i < T::kPlanes + 1; ++i) {
+            const int low = i == 0, plane = T::kPlanes == 2 && i == 1;
+#pragma unroll
+            for (int ks = 0; ks < BN / 16; ++ks)  // 16 slots: 2048 bytes on
+              mma_ts(d, p + 16u * ks + 8u * low, vb + (plane * (BN * 128) + ks * 2048) / 16, id_o, (uint32_t)(i || ks));
+          }
+          umma_commit(w ? &sh.o1_done : &sh.ok_ready[(n + 1) % T::kTurns]);
+          umma_commit(&sh.o_full[w]);
+          if (w == tiles - 1) umma_commit(&sh.empty[s]);
+        }
+        __syncwarp();
+      };
+      auto turn = [&](int n) { return (uint32_t)(n / T::kTurns) & 1u; };
+      wait_phase(&sh.ok_ready[0], 0u, &sh.abort);
       for (int w = 0; w < tiles; ++w) scores(w, 0);
       for (int n = 0; n < nb; ++n) {
-        for (int w = 0; w < tiles; ++w) {
-          if (w == 0) full(2 * n + 1);
-          wait_phase(&sh.p_ready[w], (uint32_t)n & 1u, &sh.abort);  // (P is there, and O of the block before has been read)
-          tc_fence_after();
-          if (leader) {
-            const int s = (2 * n + 1) % T::kRing;
-            const unsigned char* vb = ring + s * T::kTile;
-            const uint32_t p = tmem + (uint32_t)w * 128, d = tmem + 256u + (uint32_t)w * 128;
-            // products (term of p, plane of V), the smallest first
-#pragma unroll
-            for (int i = 0; i < T::kPlanes + 1; ++i) {
-              const int low = i == 0, plane = T::kPlanes == 2 && i == 1;
-              const uint64_t bd = umma_desc_mn_sw128(vb + plane * (BN * 128), T::kBox);
-#pragma unroll
-              for (int ks = 0; ks < BN / 16; ++ks)  // 16 slots: 2048 bytes on
-                umma_bf16_ts(d, p + 32u * (ks / 2) + 8u * (ks % 2) + 16u * low, bd + 128ull * ks, id_o, (uint32_t)(i || ks));
-            }
-            if (w == tiles - 1) umma_commit(&sh.empty[s]);
-            umma_commit(&sh.o_full[w]);
-          }
-          __syncwarp();
-          if (n + 1 < nb) {
-            if (w == 0) full(2 * n + 2);
-            // the next scores replace P
-            wait_phase(&sh.o_full[w], (uint32_t)n & 1u, &sh.abort);
-            tc_fence_after();
-            scores(w, n + 1);
+        const bool more = n + 1 < nb;
+        // P is there (and so O of the block before has been read), and V; the next scores replace P
+        wait_phase(&sh.pv_ready[n % T::kTurns], turn(n), &sh.abort);
+        output(0, n);
+        if (more) {
+          wait_phase(&sh.ok_ready[(n + 1) % T::kTurns], turn(n + 1), &sh.abort);
+          scores(0, n + 1);
+        }
+        if (tiles == 2) {
+          wait_phase(&sh.p1_ready, (uint32_t)n & 1u, &sh.abort);
+          output(1, n);
+          if (more) {
+            wait_phase(&sh.o1_done, (uint32_t)n & 1u, &sh.abort);
+            scores(1, n + 1);
           }
         }
       }
@@ -280,7 +334,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
     // next to its largest element, as two fp16 terms. Rows behind the last one are zero.
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     {
-      constexpr int C = HD / 8, kPass = 256 / C, kBatch = 4;  // C threads per row
+      constexpr int C = HD / 8, kPass = kTcSoft / C, kBatch = 8;  // C threads per row
       const int c = tid % C;
 #pragma unroll 1
       for (int r1 = tid / C; r1 < kTcTileRows; r1 += kPass * kBatch) {
@@ -312,10 +366,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // q is read by the MMA
-      asm volatile("bar.sync 2, 288;" ::: "memory");
+      asm volatile("bar.sync 2, %0;" ::"n"(kTcSoft + 32) : "memory");
     }
     // ---- softmax: group w, one row per thread
-    const int w = warp >> 2, r = k.r0 + tid, slot = k.slot_of(r);
+    const int w = warp >> 2, slot = k.slot_of(k.r0 + tid);
     const uint32_t lanes = tmem + (uint32_t)w * 128 + ((uint32_t)((warp & 3) * 32) << 16);
     float o[HD], m = -INFINITY, l = 0.f, unit = 0.f;
 #pragma unroll
@@ -334,93 +388,156 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
           s0 = k.v.slot0(k.b0 + n + 1, BN);
           next = __ldg(reinterpret_cast<const float4*>(info + 2 * (size_t)unit_of(s0)));
         }
-        const float f = back * now.x;
+        const float f = fmaxf(back * now.x, 1.175494351e-38f);  // (-inf times 0 would be NaN)
         const bool edge = s_now + BN - 1 > p0 || (s_now <= p1 - a.window && s_now + BN > a.sinks);
-        // column c is visible where c <= last and (c >= first or c < sink)
+        // column c of the block is visible where c <= last and (c >= first or c < sink)
         const int last = slot - s_now, first = last >= a.window ? last - a.window + 1 : 0, sink = a.sinks - s_now;
         wait_phase(&sh.s_full[w], (uint32_t)n & 1u, &sh.abort);
         tc_fence_after();
-        // 32 scores from column c on, hidden ones at -inf
-        auto load = [&](int c, uint32_t(&u)[32]) {
-          tmem_ld32(lanes + (uint32_t)c, u);
-          if constexpr (T::kPlanes == 2) {
-            uint32_t z[32];
-            tmem_ld32(lanes + 64u + (uint32_t)c, z);
-            tmem_ld_wait();
+        // ---- the largest score; hidden ones are at -inf here and below
+        uint32_t ua[32], ub[32];
+        float x = -INFINITY, x1 = x, x2 = x, x3 = x;
+        auto most = [&](const uint32_t(&u)[32]) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(__uint_as_float(u[e]) + __uint_as_float(z[e]));
-          } else {
-            tmem_ld_wait();
-          }
-          if (edge) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!(c + e <= last && (c + e >= first || c + e < sink))) u[e] = 0xff800000u;
+          for (int e = 0; e < 32; e += 8) {
+            x = max3(x, __uint_as_float(u[e]), __uint_as_float(u[e + 1])), x1 = max3(x1, __uint_as_float(u[e + 2]), __uint_as_float(u[e + 3]));
+            x2 = max3(x2, __uint_as_float(u[e + 4]), __uint_as_float(u[e + 5])), x3 = max3(x3, __uint_as_float(u[e + 6]), __uint_as_float(u[e + 7]));
           }
         };
-        float x0 = -INFINITY, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
+        // bit e: column c + e is visible (no branches: they would part the rows of a warp)
+        auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
+        auto visible = [&](int c) { return below(last - c + 1) & (~below(first - c) | below(sink - c)); };
+        if (__builtin_expect(edge, 0)) {
+#pragma unroll 1
+          for (int c = 0; c < BN; c += 16) {
+            uint32_t u[16], z[16];
+            tmem_ld16(lanes + (uint32_t)c, u);
+            if constexpr (T::kPlanes == 2) tmem_ld16(lanes + (uint32_t)(64 + c), z);
+            const uint32_t see = visible(c);
+            tmem_ld_wait();
 #pragma unroll
-        for (int c = 0; c < BN; c += 32) {
-          uint32_t u[32];
-          load(c, u);
+            for (int e = 0; e < 16; ++e) {
+              float y = __uint_as_float(u[e]);
+              if constexpr (T::kPlanes == 2) y += __uint_as_float(z[e]);
+              x = fmaxf(x, see >> e & 1 ? y : -INFINITY);
+            }
+          }
+        } else if constexpr (T::kPlanes == 2) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            x0 = fmaxf(x0, __uint_as_float(u[e])), x1 = fmaxf(x1, __uint_as_float(u[e + 1]));
-            x2 = fmaxf(x2, __uint_as_float(u[e + 2])), x3 = fmaxf(x3, __uint_as_float(u[e + 3]));
+          for (int c = 0; c < BN; c += 32) {
+            tmem_ld32(lanes + (uint32_t)c, ua);
+            tmem_ld32(lanes + (uint32_t)(64 + c), ub);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) ua[e] = __float_as_uint(__uint_as_float(ua[e]) + __uint_as_float(ub[e]));
+            most(ua);
+          }
+        } else {
+          tmem_ld32(lanes, ua);
+#pragma unroll
+          for (int c = 0; c < BN; c += 64) {
+            tmem_ld_wait();
+            tmem_ld32(lanes + (uint32_t)(c + 32), ub);
+            most(ua);
+            tmem_ld_wait();
+            if (c + 64 < BN) tmem_ld32(lanes + (uint32_t)(c + 64), ua);
+            most(ub);
           }
         }
-        const float x = fmaxf(m, fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * f);
-        const float b = x == -INFINITY ? 0.f : x;  // a row that has seen nothing: every p is 0
-        float g = ex2(m - b);
-        const float shift = 15.f - b;
-        m = x;
-        float sum0 = 0.f, sum1 = 0.f;
+        x = fmaxf(max3(x, x1, x2), x3) * f;
+        // p is 2^(x - m + 8) with scores x up to m + 7: m is the row's maximum at a time, and moves (with
+        // l and o) only when a score exceeds that.
+        if (__any_sync(0xffffffffu, x > m + 7.f)) {
+          const float to = fmaxf(m, x), g = to == -INFINITY ? 1.f : ex2(m - to);
+          m = to, l *= g;
 #pragma unroll
-        for (int c = 0; c < BN; c += 32) {
-          uint32_t u[32], ph[16], pl[16];
-          load(c, u);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float q0 = ex2(fmaf(__uint_as_float(u[2 * e]), f, shift)), q1 = ex2(fmaf(__uint_as_float(u[2 * e + 1]), f, shift));
-            sum0 += q0, sum1 += q1;
-            split2_f16(q0, q1, ph[e], pl[e]);
-          }
-          tmem_st32(lanes + (uint32_t)c, ph, pl);
+          for (int d = 0; d < HD; ++d) o[d] *= g;
         }
-        l = fmaf(l, g, sum0 + sum1);
+        const float shift = 8.f - (m == -INFINITY ? 0.f : m);
+        // ---- p over the scores, 32 columns of tensor memory at a time (32 scores, or 16 and their
+        // second parts): while the exponentials of some are under way, the next ones land. A loop, not
+        // unrolled: the code of both groups has to stay in the instruction cache. (And no decision inside:
+        // with a vote per 16 columns they took 3700 cycles per 128 columns, two warps on a scheduler, and
+        // take 2800, 2050 of which are the exponentials.)
+        float sum = 0.f;
+        auto fetch = [&](int i) {
+          uint32_t(&u0)[16] = reinterpret_cast<uint32_t(&)[16]>(ua[0]);
+          uint32_t(&u1)[16] = reinterpret_cast<uint32_t(&)[16]>(ua[16]);
+          if constexpr (T::kPlanes == 1) tmem_ld16(lanes + (uint32_t)(32 * i), u0), tmem_ld16(lanes + (uint32_t)(32 * i + 16), u1);
+          else tmem_ld16(lanes + (uint32_t)(16 * i), u0), tmem_ld16(lanes + (uint32_t)(64 + 16 * i), u1);
+        };
+        constexpr int kStep = 32 / T::kPlanes;
+        fetch(0);
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          float y[kStep];
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < kStep; ++e) {
+            y[e] = fmaf(__uint_as_float(ua[e]), f, shift);
+            if constexpr (T::kPlanes == 2) y[e] = fmaf(__uint_as_float(ua[16 + e]), f, y[e]);
+          }
+          if (i < 3) fetch(i + 1);
+          if (__builtin_expect(edge, 0)) {
+            const uint32_t see = visible(i * kStep);
+#pragma unroll
+            for (int e = 0; e < kStep; ++e) y[e] = see >> e & 1 ? y[e] : -INFINITY;
+          }
+#pragma unroll
+          for (int c = 0; c < kStep; c += 16) {
+            uint32_t ph[8], pl[8];
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float q0 = ex2(y[c + 2 * e]), q1 = ex2(y[c + 2 * e + 1]);
+              s[e % 2 * 2] += q0, s[e % 2 * 2 + 1] += q1;
+              split_p(q0, q1, ph[e], pl[e]);
+            }
+            tmem_st16(lanes + (uint32_t)(i * kStep + c), ph, pl);
+            sum += (s[0] + s[1]) + (s[2] + s[3]);
+          }
+        }
+        l += sum;
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&sh.p_ready[w]);
+        mbar_arrive(w ? &sh.p1_ready : &sh.pv_ready[n % T::kTurns]);
         // o is in units of `unit`, a power of two that only grows
-        float drop = 1.f;
+        float lift = 1.f, drop = 1.f;
         if (now.z != unit) {
           const float to = fmaxf(now.z, unit);
-          g *= unit / to, drop = now.z / to, unit = to;
+          lift = unit / to, drop = now.z / to, unit = to;
         }
         wait_phase(&sh.o_full[w], (uint32_t)n & 1u, &sh.abort);
         tc_fence_after();
+        const uint32_t from = lanes + 256u;
+        auto take = [&](int d, uint32_t(&v)[32]) {
+          if (__builtin_expect(drop != 1.f, 0)) {
 #pragma unroll
-        for (int d = 0; d < HD; d += 32) {
-          uint32_t u[32];
-          tmem_ld32(lanes + 256u + (uint32_t)d, u);
-          tmem_ld_wait();
-          if (drop != 1.f) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(__uint_as_float(u[e]) * drop);
+            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * drop);
           }
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[d + e] = fmaf(o[d + e], g, __uint_as_float(u[e]));
+          for (int e = 0; e < 32; ++e) o[d + e] = fmaf(o[d + e], lift, __uint_as_float(v[e]));
+        };
+        tmem_ld32(from, ua);
+#pragma unroll
+        for (int d = 0; d < HD; d += 64) {
+          tmem_ld_wait();
+          tmem_ld32(from + (uint32_t)(d + 32), ub);
+          take(d, ua);
+          tmem_ld_wait();
+          if (d + 64 < HD) tmem_ld32(from + (uint32_t)(d + 64), ua);
+          take(d + 32, ub);
         }
         tc_fence_before();
         if (now.w != 0.f) {
 #pragma unroll 1
           for (int c = 0; c < BN; ++c) {
             if (!(c <= last && (c >= first || c < sink))) continue;
-            const size_t row = a.pages.row(k.seq, s_now + c, k.head);
+            const size_t at = a.pages.row(k.seq, s_now + c, k.head);
 #pragma unroll
             for (int d = 0; d < HD; d += 8) {
               float v[8];
-              load8<KIND, HD>(a.vc, a.vs, row, d / 8, v);
+              load8<KIND, HD>(a.vc, a.vs, at, d / 8, v);
 #pragma unroll
               for (int e = 0; e < 8; ++e)
                 if (!is_finite(v[e])) o[d + e] += v[e];
@@ -430,7 +547,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
       }
     }
     // every MMA has completed (each group waited for its last O): the operands' memory is free
-    asm volatile("bar.sync 1, 256;" ::: "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(kTcSoft) : "memory");
     float* sO = reinterpret_cast<float*>(base);
     float* sML = sO + kTcTileRows * (HD + 4);
     float* mine = sO + tid * (HD + 4);
@@ -438,13 +555,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
     for (int d = 0; d < HD; d += 4)
       *reinterpret_cast<float4*>(mine + d) = make_float4(o[d] * unit, o[d + 1] * unit, o[d + 2] * unit, o[d + 3] * unit);
     sML[tid * 2] = m, sML[tid * 2 + 1] = l;
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    if (!sh.abort) rows_finish<HD, 1, kTcTileRows, 256>(P, k, sO, sML, tid);
+    asm volatile("bar.sync 1, %0;" ::"n"(kTcSoft) : "memory");
+    if (!sh.abort) rows_finish<HD, 1, kTcTileRows, kTcSoft>(P, k, sO, sML, tid);
   }
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && sh.abort) atomicExch(a.err, kErrRowsWait);
-  if (warp == 8) {
+  if (warp == kTcSoftWarps) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
   }

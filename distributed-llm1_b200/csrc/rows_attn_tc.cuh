@@ -6,9 +6,10 @@
 
 namespace dllm {
 
-constexpr int kTcThreads = 384;
+constexpr int kTcSoftWarps = 8, kTcSoft = 32 * kTcSoftWarps;  // the softmax's share
+constexpr int kTcThreads = kTcSoft + 128;
 constexpr int kTcTileRows = 256;  // rows of a CTA
-constexpr int kTcRing = 6;        // tiles of the ring at most
+constexpr int kTcRing = 6, kTcTurns = 3;  // tiles of the ring at most, and half as many
 
 template <int KIND, int HD>
 struct TcTile {
@@ -18,8 +19,9 @@ struct TcTile {
   static constexpr int kBox = 128 * 128;                 // bytes of 128 rows of a box
   static constexpr int kTile = BOX * kBox;               // of a K or V block, and of one term of 128 rows of q
   static constexpr int kRing = HD == 64 ? 6 : 3;         // K and V blocks under way
+  static constexpr int kTurns = (kRing + 1) / 2;
   static constexpr int kOut = kTcTileRows * (HD + 6) * 4;  // the results, over q and the ring
-  static constexpr int kSmem = 1024 + (4 + kRing) * kTile;
+  static constexpr int kSmem = (4 + kRing) * kTile;
   static_assert(kOut <= (4 + kRing) * kTile, "results reuse the operands' memory");
   static_assert(kSmem + 2048 <= 227 * 1024, "shared memory");
 };
