@@ -827,7 +827,7 @@ cudaError_t launch_split(const RowsAttnArgs& a, const RowsBatch& s, int rt, int 
     if ((ctas <= sms || items >= sms) && part <= (long long)rows_attn_part_rows(sms)) break;
     P.bps += 1 + P.bps / 64;
   }
-  int splits = 1, part = 0, item = 0, join = 0, units = 0;
+  int splits = 1, part = 0, item = 0, join = 0;
   for (int i = 0; i < s.n_seqs; ++i) {
     P.seq[i] = s.seq[i], P.row0[i] = s.row0[i], P.m[i] = s.m[i], P.t0[i] = s.t0[i];
     int most = 1;
@@ -836,16 +836,13 @@ cudaError_t launch_split(const RowsAttnArgs& a, const RowsBatch& s, int rt, int 
     P.item0[i] = item;
     P.part0[i] = part;
     P.join0[i] = join;
-    P.unit0[i] = units;
-    units += kvh * RowsView(s.t0[i], s.t0[i] + s.m[i] - 1, a.window, a.sinks, bn).nb;
     item += (first[i + 1] - first[i]) * kvh * most;
     if (most > 1) part += most * s.m[i] * a.nq, join += s.m[i] * a.nq;
     splits = std::max(splits, most);
   }
   P.item0[s.n_seqs] = item;
   P.join0[s.n_seqs] = join;
-  P.unit0[s.n_seqs] = units;
-  cudaError_t e = main(P, item, units);
+  cudaError_t e = main(P, item);
   *launches += 1;
   if (e != cudaSuccess || splits == 1) return e;
   const bool many = splits > 8;
@@ -865,7 +862,7 @@ cudaError_t launch_split(const RowsAttnArgs& a, const RowsBatch& s, int rt, int 
 template <int KIND, int HD, int WR>
 cudaError_t launch(const RowsAttnArgs& a, const RowsBatch& s, int sms, int* launches, cudaStream_t st) {
   using T = Tile<KIND, HD, WR>;
-  return launch_split<HD>(a, s, T::RT, T::BN, sms, launches, st, [&](const RowsKernelArgs& P, int ctas, int) {
+  return launch_split<HD>(a, s, T::RT, T::BN, sms, launches, st, [&](const RowsKernelArgs& P, int ctas) {
     rows_attn_kernel<KIND, HD, WR><<<ctas, kThreads, T::kSmem, st>>>(P);
     return cudaGetLastError();
   });
@@ -896,15 +893,6 @@ cudaError_t launch_short(const RowsAttnArgs& a, const RowsBatch& b, int sms, int
   return launch<KIND, HD, 2>(a, b, sms, launches, st);
 }
 
-template <int KIND, int HD>
-cudaError_t launch_long(RowsAttnArgs a, const RowsBatch& b, size_t units, int sms, int* launches, cudaStream_t st) {
-  a.info = static_cast<char*>(a.planes) + units * (unit_bytes(HD) - 16);
-  return launch_split<HD>(a, b, kTcTileRows, tc_block(KIND), sms, launches, st, [&](const RowsKernelArgs& P, int ctas, int n) {
-    *launches += 1;
-    return launch_rows_tc(P, KIND, HD, ctas, n, st);
-  });
-}
-
 // Sequences with few rows in one launch, those with many in another, or in several where their
 // fp16 blocks do not fit the scratch together.
 template <int KIND, int HD>
@@ -922,13 +910,13 @@ cudaError_t launch_kind(const RowsAttnArgs& a, const RowsBatch& b, int sms, int*
     const size_t u = planes_units(a, b, i, KIND);
     if (u * unit_bytes(HD) > a.planes_bytes) return cudaErrorInvalidValue;
     if ((units + u) * unit_bytes(HD) > a.planes_bytes) {
-      e = launch_long<KIND, HD>(a, many, units, sms, launches, st);
+      e = launch_rows_tc(a, many, KIND, HD, sms, launches, st);
       many.n_seqs = 0, units = 0;
     }
     add(many, b, i);
     units += u;
   }
-  if (e == cudaSuccess && many.n_seqs) e = launch_long<KIND, HD>(a, many, units, sms, launches, st);
+  if (e == cudaSuccess && many.n_seqs) e = launch_rows_tc(a, many, KIND, HD, sms, launches, st);
   return e;
 }
 

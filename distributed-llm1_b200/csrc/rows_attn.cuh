@@ -108,7 +108,6 @@ struct RowsKernelArgs {
   int item0[kRowsMaxSeqs + 1];   // CTAs: tiles (the last first), KV heads, splits
   int splits[kRowsMaxSeqs];      // of the sequence's tile that has most
   int part0[kRowsMaxSeqs];       // first partial row of a split sequence
-  int unit0[kRowsMaxSeqs + 1];   // long chunks: (KV head, block) pairs before the sequence's
   int join0[kRowsMaxSeqs + 1];   // joined (row, query head) pairs, 0 for sequences that are not split
 };
 static_assert(sizeof(RowsKernelArgs) <= 8192, "kernel arguments");

@@ -10,9 +10,10 @@
 // 128 rows (128 slots, or 64 slots and their second terms) in swizzled boxes of 64 dims, so
 // the main kernel fetches it with one bulk copy and knows no page table.
 //
-// rows_tc_kernel: one CTA per 256 rows (query head and token) that share a KV head, two
-// tiles of 128, over all their blocks or a share of them:
-//   producer (1 warp)   bulk copies of K(0), V(0), K(1), V(1) ... into a ring
+// rows_tc_kernel: one CTA per SM takes an equal share of all blocks, a segment after the other:
+// 256 rows (query head and token) that share a KV head, two tiles of 128, over all their blocks
+// or some. (A CTA per 256 rows left a quarter of the SMs idle with 224 of them.)
+//   producer (1 warp)   bulk copies of K(0), V(0), K(1), V(1) ... into a ring, across segments
 //   MMA (1 warp)        S = q K^T per tile and block, O = P V
 //   two softmax groups  128 threads each, one row per thread: S from tensor memory, online
 //                       softmax, P back over S as two fp16 terms, then O into registers
@@ -24,6 +25,7 @@
 // q_low K_high goes to the K_low half; the softmax adds the halves.
 // Tensor memory: S and P of both tiles 2 x 128 columns, O 2 x 128.
 #include <algorithm>
+#include <vector>
 
 #include "rows_attn_tc.cuh"
 #include "tc.cuh"
@@ -54,7 +56,7 @@ DLLM_DEV void load8(const void* rows, const uint32_t* pairs, size_t row, int c, 
 
 // Grid: (KV head, block, K or V) of every sequence in turn.
 template <int KIND, int HD>
-__global__ void __launch_bounds__(kPlaneThreads) rows_planes_kernel(const __grid_constant__ RowsKernelArgs P) {
+__global__ void __launch_bounds__(kPlaneThreads) rows_planes_kernel(const __grid_constant__ RowsTcArgs P) {
   using T = TcTile<KIND, HD>;
   constexpr int C = HD / 8, kEach = T::BN * C / kPlaneThreads;
   __shared__ float smax[kPlaneThreads / 32];
@@ -120,6 +122,7 @@ struct TcShared {
   // What the MMA warp waits for, one barrier at a time: the first tile's P and V, its O and the next
   // K (both in turn, so that the producer may run ahead), the second tile's P, its O.
   uint64_t pv_ready[kTcTurns], ok_ready[kTcTurns], p1_ready, o1_done;
+  uint64_t q_ready[2];
   uint64_t s_full[2], o_full[2];  // the softmax groups' side
   uint64_t idle;
   uint32_t tmem;
@@ -184,30 +187,40 @@ DLLM_DEV void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_
       "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh));
 }
 
+// One CTA's segments: calls f(tile, its first block, the block behind its last one, whether it is
+// the CTA's first).
+template <int BN, typename F>
+DLLM_DEV void rows_segments(const RowsTcArgs& P, F f) {
+  int tile = P.begin_tile[blockIdx.x], b0 = P.begin_block[blockIdx.x];
+  int left = min(P.share, P.total - (int)blockIdx.x * P.share);
+  for (bool first = true; left > 0; first = false) {
+    const RowsTcTile k(P, tile, BN);
+    const int b1 = min(k.v.nb, b0 + left);
+    f(k, b0, b1, first);
+    left -= b1 - b0;
+    ++tile, b0 = 0;
+  }
+}
+
 template <int KIND, int HD>
-__global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_constant__ RowsKernelArgs P) {
+__global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_constant__ RowsTcArgs P) {
   using T = TcTile<KIND, HD>;
   constexpr int BN = T::BN, BOX = T::BOX;
   extern __shared__ __align__(1024) unsigned char base[];
   __shared__ __align__(8) TcShared sh;
   const RowsAttnArgs& a = P.a;
   asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled; it waits for this grid's end
-  const RowsTile k(P, blockIdx.x, kTcTileRows, BN);
-  if (k.split >= k.nsplit) return;
-  const int nb = k.b1 - k.b0;
-  const int tiles = k.R - k.r0 > 128 ? 2 : 1;
 
   // the warp's number as a value that is the same in all its lanes by construction
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   unsigned char* sQ = base;  // [tile][term][box][128 rows][128 bytes]
   unsigned char* ring = base + 4 * T::kTile;
 
-  // number of a block among the sequence's (KV head, block) pairs
-  const RowsView all(k.t0, k.t0 + k.m - 1, a.window, a.sinks, BN);
-  const int unit0 = P.unit0[k.i] + k.head * all.nb;
-  auto unit_of = [&](int s0) {
+  // number of the block that starts at slot s0 among all (KV head, block) pairs
+  auto unit_of = [&](const RowsTcTile& k, int s0) {
+    const RowsView all(k.t0, k.t0 + k.m - 1, a.window, a.sinks, BN);
     const int blk = s0 / BN;
-    return unit0 + (blk >= all.first ? blk - all.first + all.nsink : blk);
+    return P.unit0[k.i] + k.head * all.nb + (blk >= all.first ? blk - all.first + all.nsink : blk);
   };
 
   if (tid == 0) {
@@ -215,6 +228,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
     for (int i = 0; i < T::kTurns; ++i) mbar_init(&sh.pv_ready[i], 128 + 1), mbar_init(&sh.ok_ready[i], 1 + 1);
     for (int w = 0; w < 2; ++w) mbar_init(&sh.s_full[w], 1), mbar_init(&sh.o_full[w], 1);
     mbar_init(&sh.p1_ready, 128), mbar_init(&sh.o1_done, 1);
+    for (int w = 0; w < 2; ++w) mbar_init(&sh.q_ready[w], 128);
     mbar_init(&sh.idle, 1);
     mbar_arrive(&sh.ok_ready[0]);  // the first scores wait for no O
     sh.abort = 0;
@@ -238,21 +252,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
       int sent = 0;
       const unsigned char* planes = static_cast<const unsigned char*>(a.planes);
       auto bar = [&](int t) { return t & 1 ? &sh.pv_ready[t / 2 % T::kTurns] : &sh.ok_ready[t / 2 % T::kTurns]; };
-      for (int t = 0; t < 2 * nb; ++t) {
-        const int s = t % T::kRing;
-        if (!wait_phase(&sh.empty[s], ((uint32_t)(t / T::kRing) & 1u) ^ 1u, &sh.abort)) break;  // nothing is loaded over memory that may still be read
-        mbar_expect_tx(bar(t), T::kTile);
-        bulk_load(ring + s * T::kTile, planes + ((size_t)unit_of(k.v.slot0(k.b0 + t / 2, BN)) * 2 + (t & 1)) * T::kTile, T::kTile,
-                  bar(t));
-        sent = t + 1;
-      }
+      rows_segments<BN>(P, [&](const RowsTcTile& k, int b0, int b1, bool) {
+        for (int b = 2 * b0; b < 2 * b1; ++b) {
+          const int t = sent, s = t % T::kRing;
+          // nothing is loaded over memory that may still be read
+          if (!wait_phase(&sh.empty[s], ((uint32_t)(t / T::kRing) & 1u) ^ 1u, &sh.abort)) return;
+          mbar_expect_tx(bar(t), T::kTile);
+          bulk_load(ring + s * T::kTile, planes + ((size_t)unit_of(k, k.v.slot0(b / 2, BN)) * 2 + (b & 1)) * T::kTile, T::kTile, bar(t));
+          sent = t + 1;
+        }
+      });
+      // whatever happened to the others, the copies under way land before the CTA ends
+      for (int t = max(0, sent - T::kRing); t < sent; ++t) mbar_wait(bar(t), (uint32_t)(t / 2 / T::kTurns) & 1u);
     } else if (warp == kTcSoftWarps + 1) {
       // ---- MMA issuer. The whole warp runs the loop and one elected lane issues, so that the operands
       // stay in uniform registers. Little more than one MMA queues up behind the running one, and a wait
       // costs 100 to 200 cycles while shared memory serves the operands, even where nothing is left to wait
       // for: so there is one for each of the four products of a block, and no more. (A warp per tile
       // was slower: both tiles' MMAs then ran, and both softmaxes waited, at the same time.)
-      asm volatile("bar.sync 2, %0;" ::"n"(kTcSoft + 32) : "memory");  // q is there
       const uint32_t leader = elect_one();
       const uint32_t idesc = (1u << 4) | ((uint32_t)(128 >> 4) << 24);                // fp32 += fp16 x fp16, M = 128
       const uint32_t id_s = idesc | ((uint32_t)(128 >> 3) << 17);                     // N = 128 rows of K, K-major
@@ -260,6 +277,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
       const uint32_t id_o = idesc | ((uint32_t)(HD >> 3) << 17) | (1u << 16);         // N = dims, B with N contiguous
       constexpr uint32_t kTile16 = T::kTile >> 4, kBox16 = T::kBox >> 4;
       const uint32_t q_low = desc_low(sQ, 1u), k_low = desc_low(ring, 1u), v_low = desc_low(ring, T::kBox >> 4);
+      int tiles = 0;
       auto scores = [&](int w, int n) {
         tc_fence_after();
         if (leader) {
@@ -303,26 +321,36 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
         __syncwarp();
       };
       auto turn = [&](int n) { return (uint32_t)(n / T::kTurns) & 1u; };
-      wait_phase(&sh.ok_ready[0], 0u, &sh.abort);
-      for (int w = 0; w < tiles; ++w) scores(w, 0);
-      for (int n = 0; n < nb; ++n) {
-        const bool more = n + 1 < nb;
-        // P is there (and so O of the block before has been read), and V; the next scores replace P
-        wait_phase(&sh.pv_ready[n % T::kTurns], turn(n), &sh.abort);
-        output(0, n);
-        if (more) {
-          wait_phase(&sh.ok_ready[(n + 1) % T::kTurns], turn(n + 1), &sh.abort);
-          scores(0, n + 1);
+      // blocks of the CTA so far, those with a second tile, and segments of each tile
+      int n = 0, n1 = 0;
+      uint32_t segments[2] = {0u, 0u};
+      rows_segments<BN>(P, [&](const RowsTcTile& k, int b0, int b1, bool) {
+        tiles = k.R - k.r0 > 128 ? 2 : 1;
+        wait_phase(&sh.ok_ready[n % T::kTurns], turn(n), &sh.abort);
+        for (int w = 0; w < tiles; ++w) {
+          wait_phase(&sh.q_ready[w], segments[w]++ & 1u, &sh.abort);  // (and the output before has been read)
+          scores(w, n);
         }
-        if (tiles == 2) {
-          wait_phase(&sh.p1_ready, (uint32_t)n & 1u, &sh.abort);
-          output(1, n);
+        for (int b = b0; b < b1; ++b, ++n) {
+          const bool more = b + 1 < b1;
+          // P is there (and so O of the block before has been read), and V; the next scores replace P
+          wait_phase(&sh.pv_ready[n % T::kTurns], turn(n), &sh.abort);
+          output(0, n);
           if (more) {
-            wait_phase(&sh.o1_done, (uint32_t)n & 1u, &sh.abort);
-            scores(1, n + 1);
+            wait_phase(&sh.ok_ready[(n + 1) % T::kTurns], turn(n + 1), &sh.abort);
+            scores(0, n + 1);
+          }
+          if (tiles == 2) {
+            wait_phase(&sh.p1_ready, (uint32_t)n1 & 1u, &sh.abort);
+            output(1, n);
+            if (more) {
+              wait_phase(&sh.o1_done, (uint32_t)n1 & 1u, &sh.abort);
+              scores(1, n + 1);
+            }
+            ++n1;
           }
         }
-      }
+      });
       // nothing of this warp's is under way when the tensor memory is freed
       if (leader) umma_commit(&sh.idle);
       __syncwarp();
@@ -330,69 +358,76 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
     }
     __syncwarp();
   } else {
-    // ---- q: rows scaled so that the softmax is in powers of two, each divided by a power of two
-    // next to its largest element, as two fp16 terms. Rows behind the last one are zero.
+    // ---- softmax: group w, one row of its tile per thread
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    {
-      constexpr int C = HD / 8, kPass = kTcSoft / C, kBatch = 8;  // C threads per row
-      const int c = tid % C;
-#pragma unroll 1
-      for (int r1 = tid / C; r1 < kTcTileRows; r1 += kPass * kBatch) {
-        float x[kBatch][8];
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          const int r = k.r0 + r1 + u * kPass;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[u][e] = 0.f;
-          if (r < k.R) load8<kKvF32, HD>(a.q, nullptr, (size_t)k.row0 * a.nq + k.place(r, a.nq), c, x[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          const int row = r1 + u * kPass;
-          float m = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[u][e] *= a.scale_log2, m = fmaxf(m, fabsf(x[u][e]));
-#pragma unroll
-          for (int d = C / 2; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-          const int ex = min(max((int)(__float_as_uint(m) >> 23), 15), 254);
-          const float up = power_of_two(268 - ex);
-          uint32_t h[4], l[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) split2_f16(x[u][2 * e] * up, x[u][2 * e + 1] * up, h[e], l[e]);
-          unsigned char* p = sQ + (row / 128) * 2 * T::kTile + (c / 8) * T::kBox + (row % 128) * 128 + (((c & 7) ^ (row & 7)) << 4);
-          *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
-          *reinterpret_cast<uint4*>(p + T::kTile) = make_uint4(l[0], l[1], l[2], l[3]);
-          if (c == 0) sh.back[row] = power_of_two(ex - 14);
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // q is read by the MMA
-      asm volatile("bar.sync 2, %0;" ::"n"(kTcSoft + 32) : "memory");
-    }
-    // ---- softmax: group w, one row per thread
-    const int w = warp >> 2, slot = k.slot_of(k.r0 + tid);
+    const int w = warp >> 2, me = tid & 127;
     const uint32_t lanes = tmem + (uint32_t)w * 128 + ((uint32_t)((warp & 3) * 32) << 16);
-    float o[HD], m = -INFINITY, l = 0.f, unit = 0.f;
+    unsigned char* tile = sQ + w * 2 * T::kTile;
+    int done = 0, all = 0;  // blocks of this tile's, and of the CTA
+    rows_segments<BN>(P, [&](const RowsTcTile& k, int b0, int b1, bool first_segment) {
+      const int nb = b1 - b0, r0 = k.r0 + w * 128, all0 = all;
+      all += nb;
+      if (r0 >= k.R) return;
+      // ---- q: rows scaled so that the softmax is in powers of two, each divided by a power of two
+      // next to its largest element, as two fp16 terms. Rows behind the last one are zero.
+      {
+        constexpr int C = HD / 8, kPass = 128 / C, kBatch = 8;  // C threads per row
+        const int c = me % C;
+#pragma unroll 1
+        for (int r1 = me / C; r1 < 128; r1 += kPass * kBatch) {
+          float x[kBatch][8];
 #pragma unroll
-    for (int d = 0; d < HD; ++d) o[d] = 0.f;
-    if (w < tiles) {
-      const float back = sh.back[tid];
+          for (int u = 0; u < kBatch; ++u) {
+            const int r = r0 + r1 + u * kPass;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[u][e] = 0.f;
+            if (r < k.R) load8<kKvF32, HD>(a.q, nullptr, (size_t)k.row0 * a.nq + k.place(r, a.nq), c, x[u]);
+          }
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            const int row = r1 + u * kPass;
+            float m = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[u][e] *= a.scale_log2, m = fmaxf(m, fabsf(x[u][e]));
+#pragma unroll
+            for (int d = C / 2; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+            const int ex = min(max((int)(__float_as_uint(m) >> 23), 15), 254);
+            const float up = power_of_two(268 - ex);
+            uint32_t h[4], l[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) split2_f16(x[u][2 * e] * up, x[u][2 * e + 1] * up, h[e], l[e]);
+            unsigned char* p = tile + (c / 8) * T::kBox + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+            *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(p + T::kTile) = make_uint4(l[0], l[1], l[2], l[3]);
+            if (c == 0) sh.back[w * 128 + row] = power_of_two(ex - 14);
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // q is read by the MMA
+        mbar_arrive(&sh.q_ready[w]);
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory");  // `back` is there
+      }
+      const int slot = k.slot_of(r0 + me);
+      float o[HD], m = -INFINITY, l = 0.f, unit = 0.f;
+#pragma unroll
+      for (int d = 0; d < HD; ++d) o[d] = 0.f;
+      const float back = sh.back[w * 128 + me];
       // the rows of this tile see slots up to p0 at least, and from p1 - window on
-      const int p0 = k.t0 + (k.r0 + w * 128) / k.G, p1 = k.t0 + (min(k.r0 + w * 128 + 128, k.R) - 1) / k.G;
+      const int p0 = k.t0 + r0 / k.G, p1 = k.t0 + (min(r0 + 128, k.R) - 1) / k.G;
       const float2* info = static_cast<const float2*>(a.info);
-      int s0 = k.v.slot0(k.b0, BN);
-      float4 next = __ldg(reinterpret_cast<const float4*>(info + 2 * (size_t)unit_of(s0)));
-      for (int n = 0; n < nb; ++n) {
+      int s0 = k.v.slot0(b0, BN);
+      float4 next = __ldg(reinterpret_cast<const float4*>(info + 2 * (size_t)unit_of(k, s0)));
+      for (int n = 0; n < nb; ++n, ++done) {
         const float4 now = next;  // factor of K, -, factor of V, whether V had other than numbers
         const int s_now = s0;
         if (n + 1 < nb) {
-          s0 = k.v.slot0(k.b0 + n + 1, BN);
-          next = __ldg(reinterpret_cast<const float4*>(info + 2 * (size_t)unit_of(s0)));
+          s0 = k.v.slot0(b0 + n + 1, BN);
+          next = __ldg(reinterpret_cast<const float4*>(info + 2 * (size_t)unit_of(k, s0)));
         }
         const float f = fmaxf(back * now.x, 1.175494351e-38f);  // (-inf times 0 would be NaN)
         const bool edge = s_now + BN - 1 > p0 || (s_now <= p1 - a.window && s_now + BN > a.sinks);
         // column c of the block is visible where c <= last and (c >= first or c < sink)
         const int last = slot - s_now, first = last >= a.window ? last - a.window + 1 : 0, sink = a.sinks - s_now;
-        wait_phase(&sh.s_full[w], (uint32_t)n & 1u, &sh.abort);
+        wait_phase(&sh.s_full[w], (uint32_t)done & 1u, &sh.abort);
         tc_fence_after();
         // ---- the largest score; hidden ones are at -inf here and below
         uint32_t ua[32], ub[32];
@@ -500,14 +535,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
         l += sum;
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(w ? &sh.p1_ready : &sh.pv_ready[n % T::kTurns]);
+        mbar_arrive(w ? &sh.p1_ready : &sh.pv_ready[(all0 + n) % T::kTurns]);
         // o is in units of `unit`, a power of two that only grows
         float lift = 1.f, drop = 1.f;
         if (now.z != unit) {
           const float to = fmaxf(now.z, unit);
           lift = unit / to, drop = now.z / to, unit = to;
         }
-        wait_phase(&sh.o_full[w], (uint32_t)n & 1u, &sh.abort);
+        wait_phase(&sh.o_full[w], (uint32_t)done & 1u, &sh.abort);
         tc_fence_after();
         const uint32_t from = lanes + 256u;
         auto take = [&](int d, uint32_t(&v)[32]) {
@@ -545,18 +580,30 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
           }
         }
       }
-    }
-    // every MMA has completed (each group waited for its last O): the operands' memory is free
-    asm volatile("bar.sync 1, %0;" ::"n"(kTcSoft) : "memory");
-    float* sO = reinterpret_cast<float*>(base);
-    float* sML = sO + kTcTileRows * (HD + 4);
-    float* mine = sO + tid * (HD + 4);
+      // ---- results. Every MMA of this tile has completed (the group waited for its last O), so they pass
+      // through q's memory, and rows leave whole.
+      const bool whole = b0 == 0 && b1 == k.v.nb;
+      const size_t part = ((size_t)blockIdx.x * 2 + !first_segment) * kTcTileRows + w * 128;
+      const float scale = whole ? unit / l : unit;
+      if (!whole && r0 + me < k.R) *reinterpret_cast<float2*>(a.part_ml + (part + me) * 2) = make_float2(m, l);
+      constexpr int C4 = HD / 4;
+      float4* stage = reinterpret_cast<float4*>(tile);
 #pragma unroll
-    for (int d = 0; d < HD; d += 4)
-      *reinterpret_cast<float4*>(mine + d) = make_float4(o[d] * unit, o[d + 1] * unit, o[d + 2] * unit, o[d + 3] * unit);
-    sML[tid * 2] = m, sML[tid * 2 + 1] = l;
-    asm volatile("bar.sync 1, %0;" ::"n"(kTcSoft) : "memory");
-    if (!sh.abort) rows_finish<HD, 1, kTcTileRows, kTcSoft>(P, k, sO, sML, tid);
+      for (int c = 0; c < C4; ++c)
+        stage[me * C4 + (c ^ (me & (C4 - 1)))] =
+            make_float4(o[4 * c] * scale, o[4 * c + 1] * scale, o[4 * c + 2] * scale, o[4 * c + 3] * scale);
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory");
+      if (!sh.abort) {
+        const int c = me % C4, rows = min(128, k.R - r0);
+#pragma unroll 4
+        for (int row = me / C4; row < rows; row += 128 / C4) {
+          const float4 v = stage[row * C4 + (c ^ (row & (C4 - 1)))];
+          float* to = whole ? a.out + ((size_t)k.row0 * a.nq + k.place(r0 + row, a.nq)) * HD : a.part_o + (part + row) * HD;
+          reinterpret_cast<float4*>(to)[c] = v;
+        }
+      }
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory");  // the next q may come
+    });
   }
   tc_fence_before();
   __syncthreads();
@@ -567,11 +614,118 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
   }
 }
 
+// Joins the segments of a tile: a warp per row.
+template <int HD>
+__global__ void __launch_bounds__(256) rows_tc_join_kernel(const __grid_constant__ RowsTcArgs P, int bn) {
+  constexpr int V = HD / 32, kBatch = 4;
+  const RowsAttnArgs& a = P.a;
+  const int s = blockIdx.x / (kTcTileRows / 8), row = blockIdx.x % (kTcTileRows / 8) * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
+  const RowsTcTile k(P, P.split_tile[s], bn);
+  const int c0 = P.split_cta[s], n = P.split_n[s];
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the segments' grid has ended and its stores are visible
+  if (k.r0 + row >= k.R) return;
+  // the tile is the first segment of every CTA but the first one, and of that one if it began there
+  const bool later = P.begin_tile[c0] != P.split_tile[s];
+  float m = -INFINITY, l = 0.f, acc[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] = 0.f;
+  for (int c = 0; c < n; c += kBatch) {
+    float2 ml[kBatch];
+    float o[kBatch][V];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      ml[u] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) o[u][e] = 0.f;
+      if (c + u < n) {
+        const size_t p = ((size_t)(c0 + c + u) * 2 + (c + u == 0 && later)) * kTcTileRows + row;
+        ml[u] = *reinterpret_cast<const float2*>(a.part_ml + p * 2);
+        if constexpr (V == 4) {
+          const float4 f = *reinterpret_cast<const float4*>(a.part_o + p * HD + lane * 4);
+          o[u][0] = f.x, o[u][1] = f.y, o[u][2] = f.z, o[u][3] = f.w;
+        } else {
+          const float2 f = *reinterpret_cast<const float2*>(a.part_o + p * HD + lane * 2);
+          o[u][0] = f.x, o[u][1] = f.y;
+        }
+      }
+    }
+    float x = m;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) x = fmaxf(x, ml[u].x);
+    const float b = x == -INFINITY ? 0.f : x, f = ex2(m - b);
+    m = x, l *= f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] *= f;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const float wt = ex2(ml[u].x - b);
+      l = fmaf(ml[u].y, wt, l);
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] = fmaf(o[u][e], wt, acc[e]);
+    }
+  }
+  const float inv = 1.f / l;
+  float* dst = a.out + ((size_t)k.row0 * a.nq + k.place(k.r0 + row, a.nq)) * HD + lane * V;
+#pragma unroll
+  for (int e = 0; e < V; ++e) dst[e] = acc[e] * inv;
+}
+
+// Shares below this many blocks are not worth a CTA of their own (its start, a partial result and
+// the join take about as long as two blocks).
+constexpr int kTcLeastShare = 2;
+
 template <int KIND, int HD>
-cudaError_t launch(const RowsKernelArgs& P, int ctas, int units, cudaStream_t st) {
+cudaError_t launch(const RowsAttnArgs& a, const RowsBatch& b, int sms, int* launches, cudaStream_t st) {
+  using T = TcTile<KIND, HD>;
+  RowsTcArgs P;
+  P.a = a;
+  P.n_seqs = b.n_seqs;
+  const int kvh = a.pages.kvh, G = a.nq / kvh;
+  std::vector<int> blocks;  // of every tile
+  int units = 0;
+  P.total = 0;
+  for (int i = 0; i < b.n_seqs; ++i) {
+    P.seq[i] = b.seq[i], P.row0[i] = b.row0[i], P.m[i] = b.m[i], P.t0[i] = b.t0[i];
+    P.tile0[i] = (int)blocks.size();
+    P.unit0[i] = units;
+    units += kvh * RowsView(b.t0[i], b.t0[i] + b.m[i] - 1, a.window, a.sinks, T::BN).nb;
+    const int tiles = RowsTcTile::tiles_of(b.m[i], G);
+    for (int h = 0; h < kvh; ++h)
+      for (int t = 0; t < tiles; ++t) {
+        const int r0 = t * kTcTileRows, last = std::min(r0 + kTcTileRows, b.m[i] * G) - 1;
+        blocks.push_back(RowsView(b.t0[i] + r0 / G, b.t0[i] + last / G, a.window, a.sinks, T::BN).nb);
+        P.total += blocks.back();
+      }
+  }
+  P.tile0[b.n_seqs] = (int)blocks.size();
+  P.unit0[b.n_seqs] = units;
+  P.a.info = static_cast<char*>(a.planes) + (size_t)units * 2 * T::kTile;
+  const int most = std::min(sms, kTcMaxCtas);
+  P.share = std::max((P.total + most - 1) / most, kTcLeastShare);
+  const int ctas = (P.total + P.share - 1) / P.share;
+  int splits = 0, at = 0;
+  for (int t = 0, c = 0; t < (int)blocks.size(); ++t) {
+    const int end = at + blocks[t], first = at / P.share, last = (end - 1) / P.share;
+    for (; c < ctas && c * P.share < end; ++c) P.begin_tile[c] = t, P.begin_block[c] = c * P.share - at;
+    if (first != last) P.split_tile[splits] = t, P.split_cta[splits] = first, P.split_n[splits] = last - first + 1, ++splits;
+    at = end;
+  }
   rows_planes_kernel<KIND, HD><<<2 * units, kPlaneThreads, 0, st>>>(P);
-  rows_tc_kernel<KIND, HD><<<ctas, kTcThreads, TcTile<KIND, HD>::kSmem, st>>>(P);
-  return cudaGetLastError();
+  rows_tc_kernel<KIND, HD><<<ctas, kTcThreads, T::kSmem, st>>>(P);
+  *launches += 2;
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || splits == 0) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(splits * (kTcTileRows / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  *launches += 1;
+  return cudaLaunchKernelEx(&cfg, rows_tc_join_kernel<HD>, P, T::BN);
 }
 
 template <int KIND, int HD>
@@ -591,11 +745,12 @@ cudaError_t configure_rows_attn_tc() {
   return e;
 }
 
-cudaError_t launch_rows_tc(const RowsKernelArgs& P, int kind, int hd, int ctas, int units, cudaStream_t st) {
+cudaError_t launch_rows_tc(const RowsAttnArgs& a, const RowsBatch& b, int kind, int hd, int sms, int* launches,
+                           cudaStream_t st) {
   switch (kind) {
-    case kKvF32: return hd == 64 ? launch<kKvF32, 64>(P, ctas, units, st) : launch<kKvF32, 128>(P, ctas, units, st);
-    case kKvBf16: return hd == 64 ? launch<kKvBf16, 64>(P, ctas, units, st) : launch<kKvBf16, 128>(P, ctas, units, st);
-    default: return hd == 64 ? launch<kKv4, 64>(P, ctas, units, st) : launch<kKv4, 128>(P, ctas, units, st);
+    case kKvF32: return hd == 64 ? launch<kKvF32, 64>(a, b, sms, launches, st) : launch<kKvF32, 128>(a, b, sms, launches, st);
+    case kKvBf16: return hd == 64 ? launch<kKvBf16, 64>(a, b, sms, launches, st) : launch<kKvBf16, 128>(a, b, sms, launches, st);
+    default: return hd == 64 ? launch<kKv4, 64>(a, b, sms, launches, st) : launch<kKv4, 128>(a, b, sms, launches, st);
   }
 }
 
