@@ -71,6 +71,7 @@ struct Tile {
   static constexpr int kPairBytes = KvRow<KIND, HD>::kPairs * 4;
   static constexpr int kChunks = kRowBytes / 16;
   static constexpr int kRows = BN * kRowBytes, kTileBytes = kRows + BN * kPairBytes;  // one of K, V
+  static constexpr int kCtas = 1;  // per SM
   static constexpr int kQBytes = kQ4 ? 0 : RT * HD * (kF32 ? 4 : 6);  // 4-bit rows: q lives in registers
   static constexpr int kPad = HD + 4;
   static constexpr int kMergeBytes = WS * RT * (kPad + 2) * 4;
@@ -93,7 +94,7 @@ DLLM_DEV uint32_t at4(int row, int c) {
 }
 
 template <int KIND, int HD, int WR>
-__global__ void __launch_bounds__(kThreads, 1) rows_attn_kernel(const __grid_constant__ RowsKernelArgs P) {
+__global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn_kernel(const __grid_constant__ RowsKernelArgs P) {
   using T = Tile<KIND, HD, WR>;
   constexpr int SN = T::SN, BN = T::BN, WS = T::WS, RT = T::RT, NT = SN / 8, CH = T::kChunks, S = T::kStages;
   constexpr bool F32 = T::kF32, Q4 = T::kQ4;
@@ -101,15 +102,14 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attn_kernel(const __grid_con
   extern __shared__ __align__(1024) unsigned char smem[];
   const RowsAttnArgs& a = P.a;
   asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled; it waits for this grid's end
-  const RowsTile k(P, blockIdx.x, RT, BN);
-  if (k.split >= k.nsplit) return;
-  const int window = a.window, sinks = a.sinks, end = k.v.p1 + 1;
-
+  const int window = a.window, sinks = a.sinks;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int wr = warp % WR, ws = warp / WR;
   const int g = lane >> 2, t = lane & 3;
   unsigned char* sQ = smem;
   unsigned char* ring = smem + T::kQBytes;
+  rows_segments(P, RT, BN, [&](const RowsTile& k, int b0, int b1, bool first_segment) {
+  const int end = k.v.p1 + 1;
 
   // ---- K/V blocks through the ring. Pages hold at least 32 slots, so a block has BN / 32
   // page lookups at most, made one block ahead of the copies that need them.
@@ -159,12 +159,12 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attn_kernel(const __grid_con
       }
     }
   };
-  lookup(k.b0);
+  lookup(b0);
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) {
-    if (k.b0 + s < k.b1) {
-      copy(k.b0 + s, s);
-      lookup(min(k.b0 + s + 1, k.b1 - 1));
+    if (b0 + s < b1) {
+      copy(b0 + s, s);
+      lookup(min(b0 + s + 1, b1 - 1));
     }
     cp_commit();
   }
@@ -268,18 +268,18 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attn_kernel(const __grid_con
     return Q4 ? wslot + i * 8 + t + (e & 1) * 4 : wslot + i * 8 + 2 * t + (e & 1);
   };
 
-  for (int b = k.b0; b < k.b1; ++b) {
+  for (int b = b0; b < b1; ++b) {
     cp_wait<S - 2>();
     __syncthreads();
     {
       const int next = b + S - 1;
-      if (next < k.b1) {
-        copy(next, (next - k.b0) % S);
-        lookup(min(next + 1, k.b1 - 1));
+      if (next < b1) {
+        copy(next, (next - b0) % S);
+        lookup(min(next + 1, b1 - 1));
       }
       cp_commit();
     }
-    unsigned char* sK = ring + ((b - k.b0) % S) * 2 * T::kTileBytes;
+    unsigned char* sK = ring + ((b - b0) % S) * 2 * T::kTileBytes;
     unsigned char* sV = sK + T::kTileBytes;
     const int s0 = k.v.slot0(b, BN);
 
@@ -673,32 +673,27 @@ __global__ void __launch_bounds__(kThreads, 1) rows_attn_kernel(const __grid_con
     sML[(ws * RT + rb) * 2] = mb, sML[(ws * RT + rb) * 2 + 1] = lb;
   }
   __syncthreads();
-  rows_finish<HD, WS, RT, kThreads>(P, k, sO, sML, tid);
+  rows_finish<HD, WS, RT, kThreads>(a, k, b0 == 0 && b1 == k.v.nb, ((size_t)blockIdx.x * 2 + !first_segment) * RT, sO, sML, tid);
+  __syncthreads();  // the next segment may use the memory
+  });
 }
 
-// Joins the splits of a sequence. W warps share one (row, query head): warp w folds the
-// splits w, w + W, ... in order, then the warps' results are folded in order, so the sum does
-// not depend on timing. Every split's maximum, sum and output are loaded together: the chain
-// is one load per kBatch splits.
+// Joins a tile's segments. W warps share one row: warp w folds the segments w, w + W, ... in order,
+// then the warps' results are folded in order, so the sum does not depend on timing. Every
+// segment's maximum, sum and output are loaded together: the chain is one load per kBatch segments.
 template <int HD, int W>
 __global__ void __launch_bounds__(kThreads) rows_join_kernel(const __grid_constant__ RowsKernelArgs P, int rt, int bn) {
-  constexpr int V = HD / 32, kBatch = 4;
+  constexpr int V = HD / 32, kBatch = 4, kRows = 8 / W;
   __shared__ float so[8][HD], sml[8][2];
   const RowsAttnArgs& a = P.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = warp % W;
-  const int item = blockIdx.x * (8 / W) + warp / W;
-  int i = 0, at = 0, nsplit = 1;
-  if (item < P.join0[P.n_seqs]) {
-    i = rows_find(P.join0, P.n_seqs, item);
-    at = item - P.join0[i];
-    // the tile of this row, and its blocks, as the main kernel had them
-    const int G = a.nq / a.pages.kvh, j = at / a.nq, head = at % a.nq;
-    const int r0 = (j * G + head % G) / rt * rt, last = min(r0 + rt, P.m[i] * G) - 1;
-    nsplit = (RowsView(P.t0[i] + r0 / G, P.t0[i] + last / G, a.window, a.sinks, bn).nb + P.bps - 1) / P.bps;
-  }
-  const bool live = nsplit > 1;
-  const size_t step = (size_t)P.m[i] * a.nq, base = (size_t)P.part0[i] + at;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the splits' grid has ended and its stores are visible
+  const int per = rt / kRows, split = blockIdx.x / per, row = blockIdx.x % per * kRows + warp / W;
+  const RowsTile k(P, P.split_tile[split], rt, bn);
+  const int c0 = P.split_cta[split], nsplit = P.split_n[split];
+  const bool live = k.r0 + row < k.R;
+  // the tile is the first segment of every CTA but the first one, and of that one if it began there
+  const bool later = P.begin_tile[c0] != P.split_tile[split];
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the segments' grid has ended and its stores are visible
   float m = kNegInf, l = 0.f, acc[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) acc[e] = 0.f;
@@ -713,7 +708,7 @@ __global__ void __launch_bounds__(kThreads) rows_join_kernel(const __grid_consta
 #pragma unroll
         for (int e = 0; e < V; ++e) o[u][e] = 0.f;
         if (s < nsplit) {
-          const size_t p = base + s * step;
+          const size_t p = ((size_t)(c0 + s) * 2 + (s == 0 && later)) * rt + row;
           ml[u] = *reinterpret_cast<const float2*>(a.part_ml + p * 2);
           if constexpr (V == 4) {
             const float4 f = *reinterpret_cast<const float4*>(a.part_o + p * HD + lane * 4);
@@ -763,7 +758,7 @@ __global__ void __launch_bounds__(kThreads) rows_join_kernel(const __grid_consta
   }
   if (!live) return;
   const float inv = 1.0f / l;
-  float* dst = a.out + ((size_t)P.row0[i] * a.nq + at) * HD + lane * V;
+  float* dst = a.out + ((size_t)k.row0 * a.nq + k.place(k.r0 + row, a.nq)) * HD + lane * V;
 #pragma unroll
   for (int e = 0; e < V; ++e) dst[e] = acc[e] * inv;
 }
@@ -786,86 +781,15 @@ cudaError_t configure_hd() {
   return e;
 }
 
-// Cuts the blocks of bn slots of all (sequence, KV head, tile of rt rows) into CTAs, runs
-// `main` over them, and joins the splits.
-template <int HD, typename Main>
-cudaError_t launch_split(const RowsAttnArgs& a, const RowsBatch& s, int rt, int bn, int sms, int* launches,
-                         cudaStream_t st, Main main) {
-  RowsKernelArgs P;
-  P.a = a;
-  P.n_seqs = s.n_seqs;
-  const int kvh = a.pages.kvh, G = a.nq / kvh;
-  std::vector<int> blocks;  // of every tile, sequence by sequence
-  int first[kRowsMaxSeqs + 1];
-  long long total = 0;
-  for (int i = 0; i < s.n_seqs; ++i) {
-    first[i] = (int)blocks.size();
-    const int R = s.m[i] * G;
-    for (int r0 = 0; r0 < R; r0 += rt) {
-      const int last = std::min(r0 + rt, R) - 1;
-      blocks.push_back(RowsView(s.t0[i] + r0 / G, s.t0[i] + last / G, a.window, a.sinks, bn).nb);
-      total += (long long)blocks.back() * kvh;
-    }
-  }
-  first[s.n_seqs] = (int)blocks.size();
-  const long long items = (long long)blocks.size() * kvh;
-  // blocks per split: the fewest with which all CTAs run at once (short last splits make
-  // that a little more than total / sms); with more items than SMs, about one SM's share.
-  // Partial results have to fit their buffer.
-  P.bps = (int)std::max<long long>(1, (total + sms - 1) / sms);
-  for (;;) {
-    long long ctas = 0, part = 0;
-    for (int i = 0; i < s.n_seqs; ++i) {
-      int most = 1;
-      for (int t = first[i]; t < first[i + 1]; ++t) {
-        const int ns = (blocks[t] + P.bps - 1) / P.bps;
-        ctas += (long long)ns * kvh;
-        most = std::max(most, ns);
-      }
-      if (most > 1) part += (long long)most * s.m[i] * a.nq;
-    }
-    if ((ctas <= sms || items >= sms) && part <= (long long)rows_attn_part_rows(sms)) break;
-    P.bps += 1 + P.bps / 64;
-  }
-  int splits = 1, part = 0, item = 0, join = 0;
-  for (int i = 0; i < s.n_seqs; ++i) {
-    P.seq[i] = s.seq[i], P.row0[i] = s.row0[i], P.m[i] = s.m[i], P.t0[i] = s.t0[i];
-    int most = 1;
-    for (int t = first[i]; t < first[i + 1]; ++t) most = std::max(most, (blocks[t] + P.bps - 1) / P.bps);
-    P.splits[i] = most;
-    P.item0[i] = item;
-    P.part0[i] = part;
-    P.join0[i] = join;
-    item += (first[i + 1] - first[i]) * kvh * most;
-    if (most > 1) part += most * s.m[i] * a.nq, join += s.m[i] * a.nq;
-    splits = std::max(splits, most);
-  }
-  P.item0[s.n_seqs] = item;
-  P.join0[s.n_seqs] = join;
-  cudaError_t e = main(P, item);
-  *launches += 1;
-  if (e != cudaSuccess || splits == 1) return e;
-  const bool many = splits > 8;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(many ? join : (join + 7) / 8);
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  *launches += 1;
-  return cudaLaunchKernelEx(&cfg, many ? rows_join_kernel<HD, 8> : rows_join_kernel<HD, 1>, P, rt, bn);
-}
-
 template <int KIND, int HD, int WR>
-cudaError_t launch(const RowsAttnArgs& a, const RowsBatch& s, int sms, int* launches, cudaStream_t st) {
+cudaError_t launch(const RowsAttnArgs& a, const RowsBatch& b, int sms, int* launches, cudaStream_t st) {
   using T = Tile<KIND, HD, WR>;
-  return launch_split<HD>(a, s, T::RT, T::BN, sms, launches, st, [&](const RowsKernelArgs& P, int ctas) {
-    rows_attn_kernel<KIND, HD, WR><<<ctas, kThreads, T::kSmem, st>>>(P);
-    return cudaGetLastError();
-  });
+  RowsKernelArgs P;
+  const RowsPlan plan = rows_plan(a, b, T::RT, T::BN, sms * T::kCtas, 1, 2, &P);
+  rows_attn_kernel<KIND, HD, WR><<<plan.ctas, kThreads, T::kSmem, st>>>(P);
+  *launches += 1;
+  const cudaError_t e = cudaGetLastError();
+  return e != cudaSuccess ? e : rows_join(P, plan, T::RT, T::BN, HD, launches, st);
 }
 
 // Rows of a sequence that share a KV head, from which on it is a long chunk.
@@ -922,6 +846,82 @@ cudaError_t launch_kind(const RowsAttnArgs& a, const RowsBatch& b, int sms, int*
 
 }  // namespace
 
+RowsPlan rows_plan(const RowsAttnArgs& a, const RowsBatch& b, int rt, int bn, int max_ctas, int least, int start,
+                   RowsKernelArgs* P) {
+  RowsPlan plan{0, 0, 0, 0};
+  P->a = a;
+  P->n_seqs = b.n_seqs;
+  const int kvh = a.pages.kvh, G = a.nq / kvh;
+  std::vector<int> blocks;  // of every tile
+  int total = 0;
+  for (int i = 0; i < b.n_seqs; ++i) {
+    P->seq[i] = b.seq[i], P->row0[i] = b.row0[i], P->m[i] = b.m[i], P->t0[i] = b.t0[i];
+    P->tile0[i] = (int)blocks.size();
+    P->unit0[i] = plan.units;
+    plan.units += kvh * RowsView(b.t0[i], b.t0[i] + b.m[i] - 1, a.window, a.sinks, bn).nb;
+    const int first = (int)blocks.size(), R = b.m[i] * G;
+    for (int r0 = 0; r0 < R; r0 += rt)
+      blocks.push_back(RowsView(b.t0[i] + r0 / G, b.t0[i] + (std::min(r0 + rt, R) - 1) / G, a.window, a.sinks, bn).nb);
+    const int tiles = (int)blocks.size() - first;
+    for (int h = 1; h < kvh; ++h)
+      for (int t = 0; t < tiles; ++t) blocks.push_back(blocks[first + t]);
+    for (size_t t = first; t < blocks.size(); ++t) total += blocks[t];
+  }
+  const int tiles = (int)blocks.size();
+  P->tile0[b.n_seqs] = tiles;
+  P->unit0[b.n_seqs] = plan.units;
+  max_ctas = std::min(max_ctas, kRowsMaxCtas);
+  const int share = std::max((total + max_ctas - 1) / max_ctas, least);
+  // the smallest shares with which every tile's blocks are split on their own
+  int own = share;
+  for (; tiles <= max_ctas && own <= share + start; ++own) {
+    int ctas = 0;
+    for (int t = 0; t < tiles; ++t) ctas += (blocks[t] + own - 1) / own;
+    if (ctas <= max_ctas) break;
+  }
+  const bool apart = tiles <= max_ctas && own <= share + start;
+  int c = 0, left = 0;  // CTAs so far, and what the latest of them may still take
+  for (int t = 0; t < tiles; ++t) {
+    const int n = (blocks[t] + own - 1) / own;  // apart: the tile's CTAs, as equal as can be
+    int first = -1;
+    for (int at = 0, k = 0; at < blocks[t]; ++k) {
+      if (apart || left == 0) {
+        P->begin_tile[c] = t, P->begin_block[c] = at, P->count[c] = 0;
+        left = apart ? blocks[t] * (k + 1) / n - at : share;
+        ++c;
+      }
+      const int take = std::min(left, blocks[t] - at);
+      P->count[c - 1] += take, left -= take, at += take;
+      if (first < 0) first = c - 1;
+    }
+    if (c - 1 > first) {
+      P->split_tile[plan.splits] = t, P->split_cta[plan.splits] = first, P->split_n[plan.splits] = c - first;
+      ++plan.splits;
+      plan.most_n = std::max(plan.most_n, c - first);
+    }
+  }
+  plan.ctas = c;
+  return plan;
+}
+
+cudaError_t rows_join(const RowsKernelArgs& P, const RowsPlan& plan, int rt, int bn, int hd, int* launches, cudaStream_t st) {
+  if (plan.splits == 0) return cudaSuccess;
+  const bool many = plan.most_n > 8;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(plan.splits * (many ? rt : rt / 8));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  *launches += 1;
+  if (hd == 64) return cudaLaunchKernelEx(&cfg, many ? rows_join_kernel<64, 8> : rows_join_kernel<64, 1>, P, rt, bn);
+  return cudaLaunchKernelEx(&cfg, many ? rows_join_kernel<128, 8> : rows_join_kernel<128, 1>, P, rt, bn);
+}
+
+// Two partial tiles per CTA: 2 sms of 256 rows, or 4 sms of 64.
 size_t rows_attn_part_rows(int sms) { return (size_t)2 * sms * 256; }
 
 size_t rows_attn_planes_bytes(const RowsAttnArgs& a, const RowsBatch& b, int kind, int hd) {

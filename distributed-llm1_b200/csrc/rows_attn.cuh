@@ -98,19 +98,22 @@ struct RowsView {
 };
 DLLM_DEV bool rows_sees(int p, int s, int window, int sinks) { return s <= p && (s > p - window || s < sinks); }
 
-// One kernel's share of a batch: its sequences, cut into CTAs. Item i of the grid belongs to
-// the sequence whose [item0, item0 of the next) holds it.
+// All tiles of rt rows of a batch (sequence by sequence, KV head by KV head), and their blocks one
+// after the other, cut into a share per CTA: CTA c takes count[c] blocks from block begin_block[c]
+// of tile begin_tile[c] on. A tile in one CTA's share is written out; of the others each CTA leaves
+// partial results, at most two of rt rows (its first segment's, and its last one's), which are
+// joined.
+constexpr int kRowsMaxCtas = 320;
 struct RowsKernelArgs {
   RowsAttnArgs a;
   int n_seqs;
-  int bps;  // blocks per split
   int seq[kRowsMaxSeqs], row0[kRowsMaxSeqs], m[kRowsMaxSeqs], t0[kRowsMaxSeqs];
-  int item0[kRowsMaxSeqs + 1];   // CTAs: tiles (the last first), KV heads, splits
-  int splits[kRowsMaxSeqs];      // of the sequence's tile that has most
-  int part0[kRowsMaxSeqs];       // first partial row of a split sequence
-  int join0[kRowsMaxSeqs + 1];   // joined (row, query head) pairs, 0 for sequences that are not split
+  int tile0[kRowsMaxSeqs + 1];  // tiles before the sequence
+  int unit0[kRowsMaxSeqs + 1];  // (KV head, block) pairs before the sequence (rows_attn_tc.cu)
+  int begin_tile[kRowsMaxCtas], begin_block[kRowsMaxCtas], count[kRowsMaxCtas];
+  int split_tile[kRowsMaxCtas], split_cta[kRowsMaxCtas], split_n[kRowsMaxCtas];  // joined tiles, their first CTA, CTAs
 };
-static_assert(sizeof(RowsKernelArgs) <= 8192, "kernel arguments");
+static_assert(sizeof(RowsKernelArgs) <= 16384, "kernel arguments");
 
 DLLM_DEV int rows_find(const int* first, int n, int item) {
   int lo = 0, hi = n;  // first[lo] <= item < first[hi]
@@ -122,25 +125,21 @@ DLLM_DEV int rows_find(const int* first, int n, int item) {
   return lo;
 }
 
-// A CTA's work: rows [r0, r0 + rt) of the m G rows of a sequence that share a KV head (row r
-// is query head r % G of batch row r / G), over the blocks [b0, b1) of their view.
+// One tile: rows [r0, r0 + rt) of the R = m G rows of a sequence that share a KV head (row r is query
+// head r % G of batch row r / G).
 struct RowsTile {
-  int i, seq, row0, m, t0, head, G, r0, R, split, nsplit, b0, b1;
+  int i, seq, row0, m, t0, head, G, r0, R;
   RowsView v;
-  DLLM_DEV RowsTile(const RowsKernelArgs& P, int item, int rt, int bn) : v(0, 0, 1, 0, 1) {
-    i = rows_find(P.item0, P.n_seqs, item);
+  __host__ __device__ static int tiles_of(int m, int G, int rt) { return (m * G + rt - 1) / rt; }
+  DLLM_DEV RowsTile(const RowsKernelArgs& P, int tile, int rt, int bn) : v(0, 0, 1, 0, 1) {
+    i = rows_find(P.tile0, P.n_seqs, tile);
     seq = P.seq[i], row0 = P.row0[i], m = P.m[i], t0 = P.t0[i];
-    const int kvh = P.a.pages.kvh;
-    G = P.a.nq / kvh, R = m * G;
-    const int at = item - P.item0[i], s = P.splits[i], tiles = (R + rt - 1) / rt;
-    split = at % s;
-    head = at / s % kvh;
-    r0 = (tiles - 1 - at / s / kvh) * rt;
+    G = P.a.nq / P.a.pages.kvh, R = m * G;
+    const int tiles = tiles_of(m, G, rt), at = tile - P.tile0[i];
+    head = at / tiles;
+    r0 = at % tiles * rt;
     const int last = (r0 + rt < R ? r0 + rt : R) - 1;
     v = RowsView(t0 + r0 / G, t0 + last / G, P.a.window, P.a.sinks, bn);
-    nsplit = (v.nb + P.bps - 1) / P.bps;
-    b0 = split * P.bps;
-    b1 = b0 + P.bps < v.nb ? b0 + P.bps : v.nb;
   }
   // cache slot of row r, or -1 behind the last row
   DLLM_DEV int slot_of(int r) const { return r < R ? t0 + r / G : -1; }
@@ -148,14 +147,39 @@ struct RowsTile {
   DLLM_DEV int place(int r, int nq) const { return r / G * nq + head * G + r % G; }
 };
 
+// One CTA's segments: calls f(tile, its first block, the block behind its last one, whether it is
+// the CTA's first).
+template <typename F>
+DLLM_DEV void rows_segments(const RowsKernelArgs& P, int rt, int bn, F f) {
+  int tile = P.begin_tile[blockIdx.x], b0 = P.begin_block[blockIdx.x];
+  int left = P.count[blockIdx.x];
+  for (bool first = true; left > 0; first = false) {
+    const RowsTile k(P, tile, rt, bn);
+    const int b1 = min(k.v.nb, b0 + left);
+    f(k, b0, b1, first);
+    left -= b1 - b0;
+    ++tile, b0 = 0;
+  }
+}
+
+// Cuts a batch into shares for at most max_ctas CTAs, none of less than `least` blocks unless there
+// are fewer: equal shares of all blocks, or, where that is no slower, shares that end with their
+// tiles (a CTA's second segment costs it a start, about as long as `start` blocks).
+struct RowsPlan {
+  int ctas, splits, most_n, units;  // CTAs, joined tiles, the most segments of one, (KV head, block) pairs
+};
+RowsPlan rows_plan(const RowsAttnArgs& a, const RowsBatch& b, int rt, int bn, int max_ctas, int least, int start, RowsKernelArgs* P);
+// Joins the split tiles' segments.
+cudaError_t rows_join(const RowsKernelArgs& P, const RowsPlan& plan, int rt, int bn, int hd, int* launches, cudaStream_t st);
+
 // The results of WS slot groups, each with RT rows of [HD + 4] outputs in sO and (max, sum) in
-// sML, to `out`, or to this split's partials. HD / 4 threads per row.
+// sML, to `out`, or where `whole` is false to the partial rows from `part` on. HD / 4 threads per
+// row.
 template <int HD, int WS, int RT, int THREADS>
-DLLM_DEV void rows_finish(const RowsKernelArgs& P, const RowsTile& k, const float* sO, const float* sML, int tid) {
-  const RowsAttnArgs& a = P.a;
+DLLM_DEV void rows_finish(const RowsAttnArgs& a, const RowsTile& k, bool whole, size_t part, const float* sO, const float* sML,
+                          int tid) {
   constexpr int kLanes = HD / 4, kStep = THREADS / kLanes;
   const int d = (tid % kLanes) * 4, rows = min(RT, k.R - k.r0);
-  const size_t split_base = (size_t)P.part0[k.i] + (size_t)k.split * k.m * a.nq;
 #pragma unroll 4
   for (int row = tid / kLanes; row < rows; row += kStep) {
     float m = -INFINITY, l = 0.f;
@@ -170,14 +194,13 @@ DLLM_DEV void rows_finish(const RowsKernelArgs& P, const RowsTile& k, const floa
       f.x = fmaf(v.x, e, f.x), f.y = fmaf(v.y, e, f.y), f.z = fmaf(v.z, e, f.z), f.w = fmaf(v.w, e, f.w);
       l = fmaf(sML[(w * RT + row) * 2 + 1], e, l);
     }
-    const int at = k.place(k.r0 + row, a.nq);
-    if (k.nsplit == 1) {
+    if (whole) {
       const float inv = 1.0f / l;
-      *reinterpret_cast<float4*>(a.out + ((size_t)k.row0 * a.nq + at) * HD + d) =
+      *reinterpret_cast<float4*>(a.out + ((size_t)k.row0 * a.nq + k.place(k.r0 + row, a.nq)) * HD + d) =
           make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
     } else {
-      *reinterpret_cast<float4*>(a.part_o + (split_base + at) * HD + d) = f;
-      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (split_base + at) * 2) = make_float2(m, l);
+      *reinterpret_cast<float4*>(a.part_o + (part + row) * HD + d) = f;
+      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (part + row) * 2) = make_float2(m, l);
     }
   }
 }

@@ -24,9 +24,6 @@
 // registers. With two planes S takes q_high (K_high | K_low) as one MMA of N = 128, and
 // q_low K_high goes to the K_low half; the softmax adds the halves.
 // Tensor memory: S and P of both tiles 2 x 128 columns, O 2 x 128.
-#include <algorithm>
-#include <vector>
-
 #include "rows_attn_tc.cuh"
 #include "tc.cuh"
 
@@ -56,7 +53,7 @@ DLLM_DEV void load8(const void* rows, const uint32_t* pairs, size_t row, int c, 
 
 // Grid: (KV head, block, K or V) of every sequence in turn.
 template <int KIND, int HD>
-__global__ void __launch_bounds__(kPlaneThreads) rows_planes_kernel(const __grid_constant__ RowsTcArgs P) {
+__global__ void __launch_bounds__(kPlaneThreads) rows_planes_kernel(const __grid_constant__ RowsKernelArgs P) {
   using T = TcTile<KIND, HD>;
   constexpr int C = HD / 8, kEach = T::BN * C / kPlaneThreads;
   __shared__ float smax[kPlaneThreads / 32];
@@ -187,23 +184,8 @@ DLLM_DEV void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_
       "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh));
 }
 
-// One CTA's segments: calls f(tile, its first block, the block behind its last one, whether it is
-// the CTA's first).
-template <int BN, typename F>
-DLLM_DEV void rows_segments(const RowsTcArgs& P, F f) {
-  int tile = P.begin_tile[blockIdx.x], b0 = P.begin_block[blockIdx.x];
-  int left = min(P.share, P.total - (int)blockIdx.x * P.share);
-  for (bool first = true; left > 0; first = false) {
-    const RowsTcTile k(P, tile, BN);
-    const int b1 = min(k.v.nb, b0 + left);
-    f(k, b0, b1, first);
-    left -= b1 - b0;
-    ++tile, b0 = 0;
-  }
-}
-
 template <int KIND, int HD>
-__global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_constant__ RowsTcArgs P) {
+__global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_constant__ RowsKernelArgs P) {
   using T = TcTile<KIND, HD>;
   constexpr int BN = T::BN, BOX = T::BOX;
   extern __shared__ __align__(1024) unsigned char base[];
@@ -217,7 +199,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
   unsigned char* ring = base + 4 * T::kTile;
 
   // number of the block that starts at slot s0 among all (KV head, block) pairs
-  auto unit_of = [&](const RowsTcTile& k, int s0) {
+  auto unit_of = [&](const RowsTile& k, int s0) {
     const RowsView all(k.t0, k.t0 + k.m - 1, a.window, a.sinks, BN);
     const int blk = s0 / BN;
     return P.unit0[k.i] + k.head * all.nb + (blk >= all.first ? blk - all.first + all.nsink : blk);
@@ -252,7 +234,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
       int sent = 0;
       const unsigned char* planes = static_cast<const unsigned char*>(a.planes);
       auto bar = [&](int t) { return t & 1 ? &sh.pv_ready[t / 2 % T::kTurns] : &sh.ok_ready[t / 2 % T::kTurns]; };
-      rows_segments<BN>(P, [&](const RowsTcTile& k, int b0, int b1, bool) {
+      rows_segments(P, kTcTileRows, BN, [&](const RowsTile& k, int b0, int b1, bool) {
         for (int b = 2 * b0; b < 2 * b1; ++b) {
           const int t = sent, s = t % T::kRing;
           // nothing is loaded over memory that may still be read
@@ -324,7 +306,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
       // blocks of the CTA so far, those with a second tile, and segments of each tile
       int n = 0, n1 = 0;
       uint32_t segments[2] = {0u, 0u};
-      rows_segments<BN>(P, [&](const RowsTcTile& k, int b0, int b1, bool) {
+      rows_segments(P, kTcTileRows, BN, [&](const RowsTile& k, int b0, int b1, bool) {
         tiles = k.R - k.r0 > 128 ? 2 : 1;
         wait_phase(&sh.ok_ready[n % T::kTurns], turn(n), &sh.abort);
         for (int w = 0; w < tiles; ++w) {
@@ -364,7 +346,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
     const uint32_t lanes = tmem + (uint32_t)w * 128 + ((uint32_t)((warp & 3) * 32) << 16);
     unsigned char* tile = sQ + w * 2 * T::kTile;
     int done = 0, all = 0;  // blocks of this tile's, and of the CTA
-    rows_segments<BN>(P, [&](const RowsTcTile& k, int b0, int b1, bool first_segment) {
+    rows_segments(P, kTcTileRows, BN, [&](const RowsTile& k, int b0, int b1, bool first_segment) {
       const int nb = b1 - b0, r0 = k.r0 + w * 128, all0 = all;
       all += nb;
       if (r0 >= k.R) return;
@@ -614,62 +596,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
   }
 }
 
-// Joins the segments of a tile: a warp per row.
-template <int HD>
-__global__ void __launch_bounds__(256) rows_tc_join_kernel(const __grid_constant__ RowsTcArgs P, int bn) {
-  constexpr int V = HD / 32, kBatch = 4;
-  const RowsAttnArgs& a = P.a;
-  const int s = blockIdx.x / (kTcTileRows / 8), row = blockIdx.x % (kTcTileRows / 8) * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
-  const RowsTcTile k(P, P.split_tile[s], bn);
-  const int c0 = P.split_cta[s], n = P.split_n[s];
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the segments' grid has ended and its stores are visible
-  if (k.r0 + row >= k.R) return;
-  // the tile is the first segment of every CTA but the first one, and of that one if it began there
-  const bool later = P.begin_tile[c0] != P.split_tile[s];
-  float m = -INFINITY, l = 0.f, acc[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) acc[e] = 0.f;
-  for (int c = 0; c < n; c += kBatch) {
-    float2 ml[kBatch];
-    float o[kBatch][V];
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      ml[u] = make_float2(-INFINITY, 0.f);
-#pragma unroll
-      for (int e = 0; e < V; ++e) o[u][e] = 0.f;
-      if (c + u < n) {
-        const size_t p = ((size_t)(c0 + c + u) * 2 + (c + u == 0 && later)) * kTcTileRows + row;
-        ml[u] = *reinterpret_cast<const float2*>(a.part_ml + p * 2);
-        if constexpr (V == 4) {
-          const float4 f = *reinterpret_cast<const float4*>(a.part_o + p * HD + lane * 4);
-          o[u][0] = f.x, o[u][1] = f.y, o[u][2] = f.z, o[u][3] = f.w;
-        } else {
-          const float2 f = *reinterpret_cast<const float2*>(a.part_o + p * HD + lane * 2);
-          o[u][0] = f.x, o[u][1] = f.y;
-        }
-      }
-    }
-    float x = m;
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) x = fmaxf(x, ml[u].x);
-    const float b = x == -INFINITY ? 0.f : x, f = ex2(m - b);
-    m = x, l *= f;
-#pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] *= f;
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const float wt = ex2(ml[u].x - b);
-      l = fmaf(ml[u].y, wt, l);
-#pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] = fmaf(o[u][e], wt, acc[e]);
-    }
-  }
-  const float inv = 1.f / l;
-  float* dst = a.out + ((size_t)k.row0 * a.nq + k.place(k.r0 + row, a.nq)) * HD + lane * V;
-#pragma unroll
-  for (int e = 0; e < V; ++e) dst[e] = acc[e] * inv;
-}
-
 // Shares below this many blocks are not worth a CTA of their own (its start, a partial result and
 // the join take about as long as two blocks).
 constexpr int kTcLeastShare = 2;
@@ -677,55 +603,14 @@ constexpr int kTcLeastShare = 2;
 template <int KIND, int HD>
 cudaError_t launch(const RowsAttnArgs& a, const RowsBatch& b, int sms, int* launches, cudaStream_t st) {
   using T = TcTile<KIND, HD>;
-  RowsTcArgs P;
-  P.a = a;
-  P.n_seqs = b.n_seqs;
-  const int kvh = a.pages.kvh, G = a.nq / kvh;
-  std::vector<int> blocks;  // of every tile
-  int units = 0;
-  P.total = 0;
-  for (int i = 0; i < b.n_seqs; ++i) {
-    P.seq[i] = b.seq[i], P.row0[i] = b.row0[i], P.m[i] = b.m[i], P.t0[i] = b.t0[i];
-    P.tile0[i] = (int)blocks.size();
-    P.unit0[i] = units;
-    units += kvh * RowsView(b.t0[i], b.t0[i] + b.m[i] - 1, a.window, a.sinks, T::BN).nb;
-    const int tiles = RowsTcTile::tiles_of(b.m[i], G);
-    for (int h = 0; h < kvh; ++h)
-      for (int t = 0; t < tiles; ++t) {
-        const int r0 = t * kTcTileRows, last = std::min(r0 + kTcTileRows, b.m[i] * G) - 1;
-        blocks.push_back(RowsView(b.t0[i] + r0 / G, b.t0[i] + last / G, a.window, a.sinks, T::BN).nb);
-        P.total += blocks.back();
-      }
-  }
-  P.tile0[b.n_seqs] = (int)blocks.size();
-  P.unit0[b.n_seqs] = units;
-  P.a.info = static_cast<char*>(a.planes) + (size_t)units * 2 * T::kTile;
-  const int most = std::min(sms, kTcMaxCtas);
-  P.share = std::max((P.total + most - 1) / most, kTcLeastShare);
-  const int ctas = (P.total + P.share - 1) / P.share;
-  int splits = 0, at = 0;
-  for (int t = 0, c = 0; t < (int)blocks.size(); ++t) {
-    const int end = at + blocks[t], first = at / P.share, last = (end - 1) / P.share;
-    for (; c < ctas && c * P.share < end; ++c) P.begin_tile[c] = t, P.begin_block[c] = c * P.share - at;
-    if (first != last) P.split_tile[splits] = t, P.split_cta[splits] = first, P.split_n[splits] = last - first + 1, ++splits;
-    at = end;
-  }
-  rows_planes_kernel<KIND, HD><<<2 * units, kPlaneThreads, 0, st>>>(P);
-  rows_tc_kernel<KIND, HD><<<ctas, kTcThreads, T::kSmem, st>>>(P);
+  RowsKernelArgs P;
+  const RowsPlan plan = rows_plan(a, b, kTcTileRows, T::BN, sms, kTcLeastShare, 2, &P);
+  P.a.info = static_cast<char*>(a.planes) + (size_t)plan.units * 2 * T::kTile;
+  rows_planes_kernel<KIND, HD><<<2 * plan.units, kPlaneThreads, 0, st>>>(P);
+  rows_tc_kernel<KIND, HD><<<plan.ctas, kTcThreads, T::kSmem, st>>>(P);
   *launches += 2;
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || splits == 0) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(splits * (kTcTileRows / 8));
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  *launches += 1;
-  return cudaLaunchKernelEx(&cfg, rows_tc_join_kernel<HD>, P, T::BN);
+  const cudaError_t e = cudaGetLastError();
+  return e != cudaSuccess ? e : rows_join(P, plan, kTcTileRows, T::BN, HD, launches, st);
 }
 
 template <int KIND, int HD>
