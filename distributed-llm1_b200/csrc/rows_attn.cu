@@ -25,6 +25,11 @@
 // side by side in rows, 8 / WR of them in slots, each with a maximum, sum and output of its
 // own, joined at the end. K and V blocks come through a cp.async ring; slots behind the
 // tile's last row are zero-filled, never read.
+//
+// Up to 8 rows (WR = 0: decode steps) the products' 16 rows would be half empty. There o is
+// computed transposed, V^T (p^T): the 8 rows are the products' narrow side, what a thread holds of
+// row g of the scores is what the second operand wants, and scaling, cutting and accumulating p
+// and o take half the instructions and registers, so that two CTAs share an SM.
 #include "rows_attn.cuh"
 
 #include <algorithm>
@@ -62,24 +67,25 @@ DLLM_DEV void cp8_zfill(uint32_t dst, const void* src, bool real) {
 // depth is what fits beside the q tile in 227 KB, four at most.
 template <int KIND, int HD, int WR>
 struct Tile {
-  static constexpr bool kF32 = KIND == kKvF32, kQ4 = KIND == kKv4;
-  static constexpr int WS = 8 / WR;
-  static constexpr int SN = kF32 ? 8 * WR : WR == 1 ? 16 : 32;
+  static constexpr bool kF32 = KIND == kKvF32, kQ4 = KIND == kKv4, kNarrow = WR == 0;
+  static constexpr int WS = kNarrow ? 8 : 8 / WR;
+  static constexpr int SN = kF32 ? (kNarrow ? 8 : 8 * WR) : WR == 1 || (kNarrow && !kQ4) ? 16 : 32;
   static constexpr int BN = SN * WS;
-  static constexpr int RT = 16 * WR;
+  static constexpr int RT = kNarrow ? 8 : 16 * WR;
   static constexpr int kRowBytes = KvRow<KIND, HD>::kBytes;
   static constexpr int kPairBytes = KvRow<KIND, HD>::kPairs * 4;
   static constexpr int kChunks = kRowBytes / 16;
   static constexpr int kRows = BN * kRowBytes, kTileBytes = kRows + BN * kPairBytes;  // one of K, V
-  static constexpr int kCtas = 1;  // per SM
-  static constexpr int kQBytes = kQ4 ? 0 : RT * HD * (kF32 ? 4 : 6);  // 4-bit rows: q lives in registers
+  static constexpr int kCtas = kNarrow && kQ4 ? 2 : 1;  // per SM
+  static constexpr int kQRows = kNarrow ? 16 : RT;
+  static constexpr int kQBytes = kQ4 ? (kNarrow ? HD * 32 : 0) : kQRows * HD * (kF32 ? 4 : 6);  // (wide 4-bit tiles: registers)
   static constexpr int kPad = HD + 4;
   static constexpr int kMergeBytes = WS * RT * (kPad + 2) * 4;
-  static constexpr int kFit = (225 * 1024 - kQBytes) / (2 * kTileBytes);
+  static constexpr int kFit = ((kCtas == 2 ? 112 : 225) * 1024 - kQBytes) / (2 * kTileBytes);
   static constexpr int kStages = kFit > 4 ? 4 : kFit;
   static constexpr int kRing = kStages * 2 * kTileBytes;
   static constexpr int kSmem = kQBytes + (kRing > kMergeBytes ? kRing : kMergeBytes);
-  static_assert(kStages >= 2 && kSmem <= 227 * 1024, "shared memory");
+  static_assert(kStages >= 2 && kCtas * (kSmem + 1024) <= 228 * 1024, "shared memory");
   static_assert(BN % 32 == 0, "a page lookup serves 32 slots");
 };
 
@@ -97,14 +103,14 @@ template <int KIND, int HD, int WR>
 __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn_kernel(const __grid_constant__ RowsKernelArgs P) {
   using T = Tile<KIND, HD, WR>;
   constexpr int SN = T::SN, BN = T::BN, WS = T::WS, RT = T::RT, NT = SN / 8, CH = T::kChunks, S = T::kStages;
-  constexpr bool F32 = T::kF32, Q4 = T::kQ4;
+  constexpr bool F32 = T::kF32, Q4 = T::kQ4, N8 = T::kNarrow;
   constexpr int NG = HD / kGroup4;  // 4-bit rows: groups
   extern __shared__ __align__(1024) unsigned char smem[];
   const RowsAttnArgs& a = P.a;
   asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled; it waits for this grid's end
   const int window = a.window, sinks = a.sinks;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int wr = warp % WR, ws = warp / WR;
+  const int wr = N8 ? 0 : warp % (N8 ? 1 : WR), ws = N8 ? warp : warp / (N8 ? 1 : WR);
   const int g = lane >> 2, t = lane & 3;
   unsigned char* sQ = smem;
   unsigned char* ring = smem + T::kQBytes;
@@ -147,12 +153,13 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
       cp16_zfill(dv + av, real ? vc + off : vc, real);
     }
     if constexpr (Q4) {
-      static_assert(2 * BN <= kThreads, "a thread copies the pairs of one row");
-      const int row = tid % BN;
-      if (tid < 2 * BN) {
+#pragma unroll
+      for (int i = 0; i < (2 * BN + kThreads - 1) / kThreads; ++i) {
+        const int at = tid + i * kThreads, row = at % BN;
+        if (2 * BN % kThreads && at >= 2 * BN) break;
         const bool real = s0 + row < end;
-        const uint32_t* src = (tid < BN ? a.ks : a.vs);
-        const uint32_t dst = (tid < BN ? dk : dv) + T::kRows + row * T::kPairBytes;
+        const uint32_t* src = at < BN ? a.ks : a.vs;
+        const uint32_t dst = (at < BN ? dk : dv) + T::kRows + row * T::kPairBytes;
         if (real) src += row_of(s0, row) * NG;
         if constexpr (HD == 128) cp16_zfill(dst, src, real);
         else cp8_zfill(dst, src, real);
@@ -171,10 +178,11 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
 
   // this thread's two rows of the tile
   const int ra = wr * 16 + g, rb = ra + 8;
-  const int pa = k.slot_of(k.r0 + ra), pb = k.slot_of(k.r0 + rb);
+  const int pa = k.slot_of(k.r0 + ra), pb = N8 ? -1 : k.slot_of(k.r0 + rb);
 
   // ---- the q tile, scaled by log2(e) / sqrt(hd) so that the softmax is in powers of two
-  uint32_t qf[Q4 ? HD / 16 : 1][2][4];        // 4-bit rows: A fragments of two fp16 terms
+  uint32_t qf[Q4 && !N8 ? HD / 16 : 1][2][4];  // 4-bit rows: A fragments of two fp16 terms
+  uint2* qs = reinterpret_cast<uint2*>(sQ) + lane;  // of a narrow tile (rows 8 to 15 are zero): [k step][term][lane]
   float qsum_a[Q4 ? NG : 1], qsum_b[Q4 ? NG : 1], back_a = 1.f, back_b = 1.f;
   if constexpr (Q4) {
     // lane t of a row holds dims 8t .. 8t + 7 of every group: a u32 of codes
@@ -218,20 +226,32 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
     const float ia = power_of_two(254 - ea), ib = power_of_two(254 - eb);
     back_a = power_of_two(ea), back_b = power_of_two(eb);
 #pragma unroll
+    for (int i = 0; i < NG; ++i) qsum_a[i] *= ia, qsum_b[i] *= ib;
+#pragma unroll
     for (int ks = 0; ks < HD / 16; ++ks) {
       const int i = ks / 2, d = (ks & 1) * 2;
+      uint32_t f[2][4];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {  // dims d + u and d + u + 4: the two halves of a nibble pair
-        split2_f16(xa[i][d + u] * ia, xa[i][d + u + 4] * ia, qf[ks][0][2 * u], qf[ks][1][2 * u]);
-        split2_f16(xb[i][d + u] * ib, xb[i][d + u + 4] * ib, qf[ks][0][2 * u + 1], qf[ks][1][2 * u + 1]);
+        split2_f16(xa[i][d + u] * ia, xa[i][d + u + 4] * ia, f[0][2 * u], f[1][2 * u]);
+        split2_f16(xb[i][d + u] * ib, xb[i][d + u + 4] * ib, f[0][2 * u + 1], f[1][2 * u + 1]);
+      }
+#pragma unroll
+      for (int term = 0; term < 2; ++term) {
+        if constexpr (N8) {
+          if (warp == ks % 8) qs[(ks * 2 + term) * 32] = make_uint2(f[term][0], f[term][2]);  // (all warps have it)
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) qf[ks][term][e] = f[term][e];
+        }
       }
     }
   } else {
-    for (int i = tid; i < RT * HD / 4; i += kThreads) {
+    for (int i = tid; i < T::kQRows * HD / 4; i += kThreads) {
       const int row = i / (HD / 4), d = (i % (HD / 4)) * 4;
       const int r = k.r0 + row;
       float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r < k.R) {
+      if (row < RT && r < k.R) {
         f = *reinterpret_cast<const float4*>(a.q + ((size_t)k.row0 * a.nq + k.place(r, a.nq)) * HD + d);
         f.x *= a.scale_log2, f.y *= a.scale_log2, f.z *= a.scale_log2, f.w *= a.scale_log2;
       }
@@ -243,22 +263,28 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
         split3(f.z, f.w, h[1], m[1], l[1]);
         unsigned char* p = sQ + row * HD * 2 + (((d >> 3) ^ (row & 7)) << 4) + (d & 4) * 2;
         *reinterpret_cast<uint2*>(p) = make_uint2(h[0], h[1]);
-        *reinterpret_cast<uint2*>(p + RT * HD * 2) = make_uint2(m[0], m[1]);
-        *reinterpret_cast<uint2*>(p + 2 * RT * HD * 2) = make_uint2(l[0], l[1]);
+        *reinterpret_cast<uint2*>(p + T::kQRows * HD * 2) = make_uint2(m[0], m[1]);
+        *reinterpret_cast<uint2*>(p + 2 * T::kQRows * HD * 2) = make_uint2(l[0], l[1]);
       }
     }
   }
 
   // 4-bit rows: o of a group is in units of `unit` (a power of two, the same in the whole warp),
   // and om is the middles' share, by group
-  float o[HD / 8][4], om[4] = {0.f, 0.f, 0.f, 0.f}, unit[Q4 ? NG : 1];
+  constexpr int NO = N8 ? HD / 16 : HD / 8;
+  float o[NO][4], om[4] = {0.f, 0.f, 0.f, 0.f}, unit[Q4 ? NG : 1];
 #pragma unroll
   for (int i = 0; i < (Q4 ? NG : 1); ++i) unit[i] = 0.f;
 #pragma unroll
-  for (int i = 0; i < HD / 8; ++i)
+  for (int i = 0; i < NO; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
   float ma = kNegInf, mb = kNegInf, la = 0.f, lb = 0.f;
+
+  // the dim and the row of o[i][e] (4-bit rows have an order of their own)
+  const int pc = N8 ? k.slot_of(k.r0 + 2 * t) : pa, pd = N8 ? k.slot_of(k.r0 + 2 * t + 1) : pb;
+  auto dim_at = [&](int i, int e) { return N8 ? i * 16 + g + (e >> 1) * 8 : i * 8 + 2 * t + (e & 1); };
+  auto second = [&](int e) { return N8 ? e & 1 : e >> 1; };  // of the thread's two rows
 
   // slot (within the block) of column c of this warp's score tile i. 4-bit rows: columns 2t and
   // 2t + 1 are slots t and t + 4, so that a lane's four slots of 16 are the ones whose V rows
@@ -291,33 +317,43 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
       for (int e = 0; e < 4; ++e) sh[i][e] = 0.f;
     if constexpr (Q4) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        uint32_t pr[2][NG];  // the pairs of this lane's two slots
+      for (int gr = 0; gr < NG; ++gr) {
+        uint32_t q[2][2][4];  // [k step][term]
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const unsigned char* p = sK + T::kRows + slot_at(i, e) * T::kPairBytes;
-          if constexpr (NG == 4) *reinterpret_cast<uint4*>(pr[e]) = *reinterpret_cast<const uint4*>(p);
-          else *reinterpret_cast<uint2*>(pr[e]) = *reinterpret_cast<const uint2*>(p);
+        for (int u = 0; u < 4; ++u) {
+          if constexpr (N8) {
+            const uint2 f = qs[(gr * 4 + u) * 32];
+            q[u / 2][u % 2][0] = f.x, q[u / 2][u % 2][1] = 0u, q[u / 2][u % 2][2] = f.y, q[u / 2][u % 2][3] = 0u;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[u / 2][u % 2][e] = qf[gr * 2 + u / 2][u % 2][e];
+          }
         }
-        const int row = wslot + i * 8 + (g >> 1) + (g & 1) * 4;  // the slot of column g
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
+        for (int i = 0; i < NT; ++i) {
+          const int row = wslot + i * 8 + (g >> 1) + (g & 1) * 4;  // the slot of column g
           const uint32_t w = *reinterpret_cast<const uint32_t*>(sK + at4<HD, false>(row, gr) + t * 4);
+          const uint32_t p0 = *reinterpret_cast<const uint32_t*>(sK + T::kRows + slot_at(i, 0) * T::kPairBytes + gr * 4);
+          const uint32_t p1 = *reinterpret_cast<const uint32_t*>(sK + T::kRows + slot_at(i, 1) * T::kPairBytes + gr * 4);
           float c[4] = {0.f, 0.f, 0.f, 0.f};
           const uint32_t n0 = codes_f16(w), n1 = codes_f16(w >> 4), n2 = codes_f16(w >> 8), n3 = codes_f16(w >> 12);
-          mma_f16(c, qf[2 * gr][1], n0, n1);
-          mma_f16(c, qf[2 * gr + 1][1], n2, n3);
-          mma_f16(c, qf[2 * gr][0], n0, n1);
-          mma_f16(c, qf[2 * gr + 1][0], n2, n3);
-          // c is (q . (code - 8)) / back
-          const float sc0 = bf16_lo(pr[0][gr]), sc1 = bf16_lo(pr[1][gr]);
-          const float mn0 = fmaf(8.f, sc0, bf16_hi(pr[0][gr])), mn1 = fmaf(8.f, sc1, bf16_hi(pr[1][gr]));
-          sh[i][0] = fmaf(c[0] * back_a, sc0, fmaf(qsum_a[gr], mn0, sh[i][0]));
-          sh[i][1] = fmaf(c[1] * back_a, sc1, fmaf(qsum_a[gr], mn1, sh[i][1]));
-          sh[i][2] = fmaf(c[2] * back_b, sc0, fmaf(qsum_b[gr], mn0, sh[i][2]));
-          sh[i][3] = fmaf(c[3] * back_b, sc1, fmaf(qsum_b[gr], mn1, sh[i][3]));
+          mma_f16(c, q[0][1], n0, n1);
+          mma_f16(c, q[1][1], n2, n3);
+          mma_f16(c, q[0][0], n0, n1);
+          mma_f16(c, q[1][0], n2, n3);
+          // c is (q . (code - 8)) / back, and the sums of q are divided alike
+          const float sc0 = bf16_lo(p0), sc1 = bf16_lo(p1);
+          const float mn0 = fmaf(8.f, sc0, bf16_hi(p0)), mn1 = fmaf(8.f, sc1, bf16_hi(p1));
+          sh[i][0] = fmaf(c[0], sc0, fmaf(qsum_a[gr], mn0, sh[i][0]));
+          sh[i][1] = fmaf(c[1], sc1, fmaf(qsum_a[gr], mn1, sh[i][1]));
+          if constexpr (!N8) {
+            sh[i][2] = fmaf(c[2], sc0, fmaf(qsum_b[gr], mn0, sh[i][2]));
+            sh[i][3] = fmaf(c[3], sc1, fmaf(qsum_b[gr], mn1, sh[i][3]));
+          }
         }
       }
+#pragma unroll
+      for (int i = 0; i < NT; ++i) sh[i][0] *= back_a, sh[i][1] *= back_a, sh[i][2] *= back_b, sh[i][3] *= back_b;
     } else if constexpr (F32) {
       float s0_[NT][4], s1[NT][4], s2[NT][4];  // an accumulator chain per product
 #pragma unroll
@@ -330,7 +366,8 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int row = wr * 16 + g + (e & 1) * 8, ch = ks * 2 + (e >> 1);
-          split_tf32(*reinterpret_cast<const float*>(sQ + row * HD * 4 + ((ch ^ (row & 7)) << 4) + t * 4), qh[e], ql[e]);
+          if (N8 && (e & 1)) qh[e] = ql[e] = 0u;
+          else split_tf32(*reinterpret_cast<const float*>(sQ + row * HD * 4 + ((ch ^ (row & 7)) << 4) + t * 4), qh[e], ql[e]);
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -364,8 +401,8 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
         uint32_t qh[4], qm[4], ql[4];
         const uint32_t at = qa + (((2 * ks + (lane >> 4)) ^ (arow & 7)) << 4);
         ldsm4(qh, at);
-        ldsm4(qm, at + RT * HD * 2);
-        ldsm4(ql, at + 2 * RT * HD * 2);
+        ldsm4(qm, at + T::kQRows * HD * 2);
+        ldsm4(ql, at + 2 * T::kQRows * HD * 2);
 #pragma unroll
         for (int np = 0; np < NT / 2; ++np) {
           const int row = wslot + np * 16 + krow;
@@ -400,27 +437,32 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       xa = fmaxf(xa, fmaxf(sh[i][0], sh[i][1]));
-      xb = fmaxf(xb, fmaxf(sh[i][2], sh[i][3]));
+      if (!N8) xb = fmaxf(xb, fmaxf(sh[i][2], sh[i][3]));
     }
 #pragma unroll
     for (int w = 1; w < 4; w <<= 1) {
       xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, w));
-      xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, w));
+      if (!N8) xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, w));
     }
     xa = fmaxf(xa, ma), xb = fmaxf(xb, mb);
     // rows that have seen nothing yet keep a maximum of -inf; their p are exp2(-inf - 0) = 0
     const float ba = xa == kNegInf ? 0.f : xa, bb = xb == kNegInf ? 0.f : xb;
-    float fa = ex2(ma - ba), fb = ex2(mb - bb);
+    float fa = ex2(ma - ba), fb = N8 ? 1.f : ex2(mb - bb);
     ma = xa, mb = xb;
     float sa = 0.f, sb = 0.f;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       sh[i][0] = ex2(sh[i][0] - ba), sh[i][1] = ex2(sh[i][1] - ba);
-      sh[i][2] = ex2(sh[i][2] - bb), sh[i][3] = ex2(sh[i][3] - bb);
       sa += sh[i][0] + sh[i][1];
+      if (N8) continue;
+      sh[i][2] = ex2(sh[i][2] - bb), sh[i][3] = ex2(sh[i][3] - bb);
       sb += sh[i][2] + sh[i][3];
     }
     la = la * fa + sa, lb = lb * fb + sb;
+    if constexpr (N8) {  // from row g to the rows of o, 2t and 2t + 1
+      fb = __shfl_sync(0xffffffffu, fa, 8 * t + 4);
+      fa = __shfl_sync(0xffffffffu, fa, 8 * t);
+    }
 
     // ---- o = o * f + p . V, the block's product from a fresh accumulator
     if constexpr (Q4) {
@@ -430,13 +472,14 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
       uint32_t nan_bits[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
       for (int j = 0; j < NK; ++j) {
-        // the middles: column g of the product is group g; this lane's slots are t, t + 4, t + 8, t + 12
+        // the middles: column g of the product (narrow: row g) is group g; this lane's slots are t, t + 4,
+        // t + 8, t + 12
         const int row = wslot + j * 16 + t;
         uint32_t h[4], m[4], l[4];
         float mid[4];
-        split3(sh[2 * j][0], sh[2 * j][1], h[0], m[0], l[0]), split3(sh[2 * j][2], sh[2 * j][3], h[1], m[1], l[1]);
-        split3(sh[2 * j + 1][0], sh[2 * j + 1][1], h[2], m[2], l[2]);
-        split3(sh[2 * j + 1][2], sh[2 * j + 1][3], h[3], m[3], l[3]);
+        split3(sh[2 * j][0], sh[2 * j][1], h[0], m[0], l[0]), split3(sh[2 * j + 1][0], sh[2 * j + 1][1], h[2], m[2], l[2]);
+        if constexpr (!N8)
+          split3(sh[2 * j][2], sh[2 * j][3], h[1], m[1], l[1]), split3(sh[2 * j + 1][2], sh[2 * j + 1][3], h[3], m[3], l[3]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t pr = *reinterpret_cast<const uint32_t*>(pairs + (row + 4 * e) * T::kPairBytes + (g & (NG - 1)) * 4);
@@ -460,7 +503,12 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
                         (rows_sees(p, at + 4, window, sinks) ? 0x3f800000u : 0u);
             }
             float c[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_bf16(c, seen, nan[0] | nan[1] << 16, nan[2] | nan[3] << 16);
+            if constexpr (N8) {
+              const uint32_t n4[4] = {nan[0] | nan[1] << 16, 0u, nan[2] | nan[3] << 16, 0u};
+              mma_bf16(c, n4, seen[0], seen[2]);
+            } else {
+              mma_bf16(c, seen, nan[0] | nan[1] << 16, nan[2] | nan[3] << 16);
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               if (c[e] > 0.f) nan_bits[e] = 0x7fc00000u;
@@ -469,21 +517,33 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
         const uint32_t b0 = pack_bf16(mid[0], mid[1]), b1 = pack_bf16(mid[2], mid[3]);
         const uint32_t d0 = pack_bf16(mid[0] - bf16_lo(b0), mid[1] - bf16_hi(b0));
         const uint32_t d1 = pack_bf16(mid[2] - bf16_lo(b1), mid[3] - bf16_hi(b1));
-        mma_bf16(cm, l, b0, b1);
-        mma_bf16(cm, m, d0, d1);
-        mma_bf16(cm, h, d0, d1);
-        mma_bf16(cm, m, b0, b1);
-        mma_bf16(cm, h, b0, b1);
+        if constexpr (N8) {
+          const uint32_t bb4[4] = {b0, 0u, b1, 0u}, dd4[4] = {d0, 0u, d1, 0u};
+          mma_bf16(cm, bb4, l[0], l[2]);
+          mma_bf16(cm, dd4, m[0], m[2]);
+          mma_bf16(cm, dd4, h[0], h[2]);
+          mma_bf16(cm, bb4, m[0], m[2]);
+          mma_bf16(cm, bb4, h[0], h[2]);
+        } else {
+          mma_bf16(cm, l, b0, b1);
+          mma_bf16(cm, m, d0, d1);
+          mma_bf16(cm, h, d0, d1);
+          mma_bf16(cm, m, b0, b1);
+          mma_bf16(cm, h, b0, b1);
+        }
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) om[e] = nan_bits[e] ? __uint_as_float(nan_bits[e]) : fmaf(om[e], e < 2 ? fa : fb, cm[e]);
+      for (int e = 0; e < 4; ++e)
+        om[e] = nan_bits[e] ? __uint_as_float(nan_bits[e]) : fmaf(om[e], second(e) ? fb : fa, cm[e]);
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
         // Column c of tile i of a group is its dim 8 (c & 3) + 4 (c >> 2) + i: lane (g, t) holds the
-        // four nibbles of column g in one half of a word, of two slots side by side in a register.
-        float c[4][4];
+        // four nibbles of column g in one half of a word, of two slots side by side in a register. (Narrow:
+        // tiles i and i + 1 are the halves of a product's 16 rows.)
+        constexpr int NC = N8 ? 2 : 4;
+        float c[NC][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < NC; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) c[i][e] = 0.f;
         float sc[NK][4], most = 0.f;
@@ -510,15 +570,23 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
             w[e] = *reinterpret_cast<const uint16_t*>(sV + at4<HD, true>(row + 4 * e, gr) + (g & 3) * 4 + (g >> 2) * 2);
           }
           split2_f16(sh[2 * j][0] * sc[j][0], sh[2 * j][1] * sc[j][1], h[0], l[0]);
-          split2_f16(sh[2 * j][2] * sc[j][0], sh[2 * j][3] * sc[j][1], h[1], l[1]);
           split2_f16(sh[2 * j + 1][0] * sc[j][2], sh[2 * j + 1][1] * sc[j][3], h[2], l[2]);
-          split2_f16(sh[2 * j + 1][2] * sc[j][2], sh[2 * j + 1][3] * sc[j][3], h[3], l[3]);
+          if constexpr (!N8) {
+            split2_f16(sh[2 * j][2] * sc[j][0], sh[2 * j][3] * sc[j][1], h[1], l[1]);
+            split2_f16(sh[2 * j + 1][2] * sc[j][2], sh[2 * j + 1][3] * sc[j][3], h[3], l[3]);
+          }
           const uint32_t w0 = w[0] | w[1] << 16, w1 = w[2] | w[3] << 16;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t b0 = codes_f16(w0 >> (4 * i)), b1 = codes_f16(w1 >> (4 * i));
-            mma_f16(c[i], l, b0, b1);
-            mma_f16(c[i], h, b0, b1);
+          for (int i = 0; i < NC; ++i) {
+            if constexpr (N8) {
+              const uint32_t v[4] = {codes_f16(w0 >> (8 * i)), codes_f16(w0 >> (8 * i + 4)), codes_f16(w1 >> (8 * i)), codes_f16(w1 >> (8 * i + 4))};
+              mma_f16(c[i], v, l[0], l[2]);
+              mma_f16(c[i], v, h[0], h[2]);
+            } else {
+              const uint32_t b0 = codes_f16(w0 >> (4 * i)), b1 = codes_f16(w1 >> (4 * i));
+              mma_f16(c[i], l, b0, b1);
+              mma_f16(c[i], h, b0, b1);
+            }
           }
         }
         float ga = fa, gb = fb;
@@ -527,14 +595,14 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
           ga *= lift, gb *= lift;
           unit[gr] = now;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < NC; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) c[i][e] *= drop;
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < NC; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[gr * 4 + i][e] = fmaf(o[gr * 4 + i][e], e < 2 ? ga : gb, c[i][e]);
+          for (int e = 0; e < 4; ++e) o[gr * NC + i][e] = fmaf(o[gr * NC + i][e], second(e) ? gb : ga, c[i][e]);
       }
     } else {
       // A row of V that some rows do not see may hold infinities or NaN, and 0 x NaN would reach
@@ -550,20 +618,18 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
         for (int i = tid; i < BN * HD; i += kThreads) bad |= !is_finite(value(i / HD, i % HD));
         if (__syncthreads_or(bad)) {
 #pragma unroll
-          for (int i = 0; i < HD / 8; ++i) {
-            o[i][0] *= fa, o[i][1] *= fa, o[i][2] *= fb, o[i][3] *= fb;
-            for (int row = wslot; row < wslot + SN; ++row) {
-              const float v0 = value(row, i * 8 + 2 * t), v1 = value(row, i * 8 + 2 * t + 1);
-              if (is_finite(v0) && is_finite(v1)) continue;
-              if (rows_sees(pa, s0 + row, window, sinks)) {
-                if (!is_finite(v0)) o[i][0] += v0;
-                if (!is_finite(v1)) o[i][1] += v1;
+          for (int i = 0; i < NO; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][e] *= second(e) ? fb : fa;
+          for (int row = wslot; row < wslot + SN; ++row) {
+            const bool first = rows_sees(pc, s0 + row, window, sinks), other = rows_sees(pd, s0 + row, window, sinks);
+#pragma unroll
+            for (int i = 0; i < NO; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float v = value(row, dim_at(i, e));
+                if (!is_finite(v) && (second(e) ? other : first)) o[i][e] += v;
               }
-              if (rows_sees(pb, s0 + row, window, sinks)) {
-                if (!is_finite(v0)) o[i][2] += v0;
-                if (!is_finite(v1)) o[i][3] += v1;
-              }
-            }
           }
           fa = fb = 1.f;
           __syncthreads();
@@ -577,7 +643,54 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
           __syncthreads();
         }
       }
-      if constexpr (F32) {
+      if constexpr (F32 && N8) {
+        uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j)  // slots 2t, 2t + 1 of a group take the places t, t + 4 of the product
+          split_tf32_near(sh[j][0], ph[j][0], pl[j][0]), split_tf32_near(sh[j][1], ph[j][1], pl[j][1]);
+#pragma unroll
+        for (int i = 0; i < NO; ++i) {
+          float ch[4] = {0.f, 0.f, 0.f, 0.f}, cs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            uint32_t vh[4], vl[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int row = wslot + j * 8 + 2 * t + (e >> 1), d = i * 16 + g + (e & 1) * 8;
+              split_tf32(*reinterpret_cast<const float*>(sV + row * T::kRowBytes + (((d >> 2) ^ (row & 7)) << 4) + (d & 3) * 4),
+                         vh[e], vl[e]);
+            }
+            mma_tf32(ch, vh, ph[j][0], ph[j][1]);
+            mma_tf32(cs, vl, ph[j][0], ph[j][1]);
+            mma_tf32(cs, vh, pl[j][0], pl[j][1]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][e] = fmaf(o[i][e], e & 1 ? fb : fa, ch[e] + cs[e]);
+        }
+      } else if constexpr (N8) {
+        constexpr int NK = SN / 16;
+        uint32_t ph[NK][2], pm[NK][2], pl[NK][2];
+#pragma unroll
+        for (int j = 0; j < NK; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) split3(sh[2 * j + e][0], sh[2 * j + e][1], ph[j][e], pm[j][e], pl[j][e]);
+        const int vrow = (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+        for (int i = 0; i < NO; ++i) {
+          float ch[4] = {0.f, 0.f, 0.f, 0.f}, cs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < NK; ++j) {
+            const int row = wslot + j * 16 + vrow;
+            uint32_t v4[4];
+            ldsm4t(v4, smem_addr(sV) + row * T::kRowBytes + (((2 * i + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
+            mma_bf16(ch, v4, ph[j][0], ph[j][1]);
+            mma_bf16(cs, v4, pm[j][0], pm[j][1]);
+            mma_bf16(cs, v4, pl[j][0], pl[j][1]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][e] = fmaf(o[i][e], e & 1 ? fb : fa, ch[e] + cs[e]);
+        }
+      } else if constexpr (F32) {
         uint32_t ph[NT][4], pl[NT][4];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {  // slots 2t, 2t + 1 of a group take the places t, t + 4 of the product
@@ -654,23 +767,45 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
   constexpr int kPad = T::kPad;
   float* sO = reinterpret_cast<float*>(ring);
   float* sML = sO + WS * RT * kPad;
-#pragma unroll
-  for (int i = 0; i < HD / 8; ++i) {
-    float* oa = sO + (ws * RT + ra) * kPad;
-    float* ob = sO + (ws * RT + rb) * kPad;
+  if constexpr (N8) {
+    float* oc = sO + (ws * RT + 2 * t) * kPad;
+    float* od = oc + kPad;
     if constexpr (Q4) {
-      const int gr = i / 4, d = gr * kGroup4 + (t & 1) * 16 + (t >> 1) * 4 + i % 4, from = (lane & ~3) | gr >> 1;
-      const float m0 = __shfl_sync(0xffffffffu, om[gr & 1], from), m1 = __shfl_sync(0xffffffffu, om[2 + (gr & 1)], from);
-      oa[d] = fmaf(o[i][0], unit[gr], m0), oa[d + 8] = fmaf(o[i][1], unit[gr], m0);
-      ob[d] = fmaf(o[i][2], unit[gr], m1), ob[d + 8] = fmaf(o[i][3], unit[gr], m1);
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr) {
+        const float m0 = __shfl_sync(0xffffffffu, om[0], gr * 4 + t), m1 = __shfl_sync(0xffffffffu, om[1], gr * 4 + t);
+        const int d = gr * kGroup4 + 8 * (g & 3) + 4 * (g >> 2);
+        const float(&x)[4] = o[gr * 2];
+        const float(&y)[4] = o[gr * 2 + 1];
+        const float u = unit[gr];
+        *reinterpret_cast<float4*>(oc + d) = make_float4(fmaf(x[0], u, m0), fmaf(x[2], u, m0), fmaf(y[0], u, m0), fmaf(y[2], u, m0));
+        *reinterpret_cast<float4*>(od + d) = make_float4(fmaf(x[1], u, m1), fmaf(x[3], u, m1), fmaf(y[1], u, m1), fmaf(y[3], u, m1));
+      }
     } else {
-      *reinterpret_cast<float2*>(oa + i * 8 + 2 * t) = make_float2(o[i][0], o[i][1]);
-      *reinterpret_cast<float2*>(ob + i * 8 + 2 * t) = make_float2(o[i][2], o[i][3]);
+#pragma unroll
+      for (int i = 0; i < NO; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) (e & 1 ? od : oc)[dim_at(i, e)] = o[i][e];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NO; ++i) {
+      float* oa = sO + (ws * RT + ra) * kPad;
+      float* ob = sO + (ws * RT + rb) * kPad;
+      if constexpr (Q4) {
+        const int gr = i / 4, d = gr * kGroup4 + (t & 1) * 16 + (t >> 1) * 4 + i % 4, from = (lane & ~3) | gr >> 1;
+        const float m0 = __shfl_sync(0xffffffffu, om[gr & 1], from), m1 = __shfl_sync(0xffffffffu, om[2 + (gr & 1)], from);
+        oa[d] = fmaf(o[i][0], unit[gr], m0), oa[d + 8] = fmaf(o[i][1], unit[gr], m0);
+        ob[d] = fmaf(o[i][2], unit[gr], m1), ob[d + 8] = fmaf(o[i][3], unit[gr], m1);
+      } else {
+        *reinterpret_cast<float2*>(oa + i * 8 + 2 * t) = make_float2(o[i][0], o[i][1]);
+        *reinterpret_cast<float2*>(ob + i * 8 + 2 * t) = make_float2(o[i][2], o[i][3]);
+      }
     }
   }
   if (t == 0) {
     sML[(ws * RT + ra) * 2] = ma, sML[(ws * RT + ra) * 2 + 1] = la;
-    sML[(ws * RT + rb) * 2] = mb, sML[(ws * RT + rb) * 2 + 1] = lb;
+    if (!N8) sML[(ws * RT + rb) * 2] = mb, sML[(ws * RT + rb) * 2 + 1] = lb;
   }
   __syncthreads();
   rows_finish<HD, WS, RT, kThreads>(a, k, b0 == 0 && b1 == k.v.nb, ((size_t)blockIdx.x * 2 + !first_segment) * RT, sO, sML, tid);
@@ -770,11 +905,14 @@ cudaError_t configure_one() {
 }
 template <int HD>
 cudaError_t configure_hd() {
-  cudaError_t e = configure_one<kKvF32, HD, 1>();
+  cudaError_t e = configure_one<kKvF32, HD, 0>();
+  if (e == cudaSuccess) e = configure_one<kKvF32, HD, 1>();
   if (e == cudaSuccess) e = configure_one<kKvF32, HD, 2>();
+  if (e == cudaSuccess) e = configure_one<kKvBf16, HD, 0>();
   if (e == cudaSuccess) e = configure_one<kKvBf16, HD, 1>();
   if (e == cudaSuccess) e = configure_one<kKvBf16, HD, 2>();
   if (e == cudaSuccess) e = configure_one<kKvBf16, HD, 4>();
+  if (e == cudaSuccess) e = configure_one<kKv4, HD, 0>();
   if (e == cudaSuccess) e = configure_one<kKv4, HD, 1>();
   if (e == cudaSuccess) e = configure_one<kKv4, HD, 2>();
   if (e == cudaSuccess) e = configure_one<kKv4, HD, 4>();
@@ -811,6 +949,7 @@ template <int KIND, int HD>
 cudaError_t launch_short(const RowsAttnArgs& a, const RowsBatch& b, int sms, int* launches, cudaStream_t st) {
   int rows = 0;  // of the largest sequence that share a KV head
   for (int i = 0; i < b.n_seqs; ++i) rows = std::max(rows, b.m[i] * (a.nq / a.pages.kvh));
+  if (rows <= 8) return launch<KIND, HD, 0>(a, b, sms, launches, st);
   if (rows <= 16) return launch<KIND, HD, 1>(a, b, sms, launches, st);
   if constexpr (KIND != kKvF32)
     if (rows > 32) return launch<KIND, HD, 4>(a, b, sms, launches, st);
