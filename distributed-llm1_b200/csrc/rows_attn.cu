@@ -118,15 +118,18 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
   const int end = k.v.p1 + 1;
 
   // ---- K/V blocks through the ring. Pages hold at least 32 slots, so a block has BN / 32
-  // page lookups at most, made one block ahead of the copies that need them.
-  constexpr int kPages = BN / 32;
-  int page[kPages];
+  // page lookups at most, made one block ahead of the copies that need them. A narrow tile's
+  // warps copy the slots that they work on themselves: one page each, and no barriers.
   const int* table = a.pages.table + (size_t)k.seq * a.pages.max_pages;
   const int log2_page = a.pages.log2_page, in_page = (1 << log2_page) - 1;
+  const int wslot = ws * SN;  // first slot of this warp within a block
+  const unsigned char *kc = static_cast<const unsigned char*>(a.kc), *vc = static_cast<const unsigned char*>(a.vc);
+  constexpr int kPages = N8 ? 1 : BN / 32;
+  int page[kPages];
   auto lookup = [&](int b) {
     const int s0 = k.v.slot0(b, BN);
 #pragma unroll
-    for (int i = 0; i < kPages; ++i) page[i] = __ldg(table + (min(s0 + 32 * i, end - 1) >> log2_page));
+    for (int i = 0; i < kPages; ++i) page[i] = __ldg(table + (min(s0 + (N8 ? wslot : 32 * i), end - 1) >> log2_page));
   };
   auto row_of = [&](int s0, int row) {
     int pg = page[0];
@@ -134,35 +137,63 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
     for (int u = 1; u < kPages; ++u) pg = row >= 32 * u ? page[u] : pg;
     return (((size_t)pg * a.pages.kvh + k.head) << log2_page) + ((s0 + row) & in_page);
   };
+  auto at_k = [](int row, int c) -> uint32_t {
+    if constexpr (Q4) return at4<HD, false>(row, c);
+    else return row * T::kRowBytes + ((c ^ (row & 7)) << 4);
+  };
+  auto at_v = [](int row, int c) -> uint32_t {
+    if constexpr (Q4) return at4<HD, true>(row, c);
+    else return row * T::kRowBytes + ((c ^ (row & 7)) << 4);
+  };
   auto copy = [&](int b, int stage) {
     const int s0 = k.v.slot0(b, BN);
     const uint32_t dk = smem_addr(ring + stage * 2 * T::kTileBytes), dv = dk + T::kTileBytes;
-    const unsigned char *kc = static_cast<const unsigned char*>(a.kc), *vc = static_cast<const unsigned char*>(a.vc);
-    constexpr int kPass = kThreads / CH;  // slots per pass
-    const int c = tid % CH;
+    if constexpr (N8) {
+      constexpr int kPass = 32 / CH > 0 ? 32 / CH : 1;  // slots per pass
+      const size_t row0 = row_of(s0, wslot);
+      const int c = lane % CH, left = end - (s0 + wslot);
 #pragma unroll
-    for (int i = 0; i < (BN + kPass - 1) / kPass; ++i) {
-      const int row = tid / CH + i * kPass;
-      if (BN % kPass && row >= BN) break;
-      const size_t off = row_of(s0, row) * T::kRowBytes + c * 16;
-      const bool real = s0 + row < end;
-      uint32_t ak, av;
-      if constexpr (Q4) ak = at4<HD, false>(row, c), av = at4<HD, true>(row, c);
-      else ak = av = row * T::kRowBytes + ((c ^ (row & 7)) << 4);
-      cp16_zfill(dk + ak, real ? kc + off : kc, real);
-      cp16_zfill(dv + av, real ? vc + off : vc, real);
-    }
-    if constexpr (Q4) {
+      for (int i = 0; i < SN / kPass; ++i) {
+        const int row = lane / CH + i * kPass;
+        const size_t off = (row0 + row) * T::kRowBytes + c * 16;
+        const bool real = row < left;
+        cp16_zfill(dk + at_k(wslot + row, c), real ? kc + off : kc, real);
+        cp16_zfill(dv + at_v(wslot + row, c), real ? vc + off : vc, real);
+      }
+      if constexpr (Q4) {
+        static_assert(SN == 32, "a lane copies the pairs of one slot");
+        const size_t off = (row0 + lane) * NG;
+        const bool real = lane < left;
+        const uint32_t at = T::kRows + (wslot + lane) * T::kPairBytes;
+        if constexpr (HD == 128)
+          cp16_zfill(dk + at, real ? a.ks + off : a.ks, real), cp16_zfill(dv + at, real ? a.vs + off : a.vs, real);
+        else
+          cp8_zfill(dk + at, real ? a.ks + off : a.ks, real), cp8_zfill(dv + at, real ? a.vs + off : a.vs, real);
+      }
+    } else {
+      constexpr int kPass = kThreads / CH;  // slots per pass
+      const int c = tid % CH;
 #pragma unroll
-      for (int i = 0; i < (2 * BN + kThreads - 1) / kThreads; ++i) {
-        const int at = tid + i * kThreads, row = at % BN;
-        if (2 * BN % kThreads && at >= 2 * BN) break;
+      for (int i = 0; i < (BN + kPass - 1) / kPass; ++i) {
+        const int row = tid / CH + i * kPass;
+        if (BN % kPass && row >= BN) break;
+        const size_t off = row_of(s0, row) * T::kRowBytes + c * 16;
         const bool real = s0 + row < end;
-        const uint32_t* src = at < BN ? a.ks : a.vs;
-        const uint32_t dst = (at < BN ? dk : dv) + T::kRows + row * T::kPairBytes;
-        if (real) src += row_of(s0, row) * NG;
-        if constexpr (HD == 128) cp16_zfill(dst, src, real);
-        else cp8_zfill(dst, src, real);
+        cp16_zfill(dk + at_k(row, c), real ? kc + off : kc, real);
+        cp16_zfill(dv + at_v(row, c), real ? vc + off : vc, real);
+      }
+      if constexpr (Q4) {
+#pragma unroll
+        for (int i = 0; i < (2 * BN + kThreads - 1) / kThreads; ++i) {
+          const int at = tid + i * kThreads, row = at % BN;
+          if (2 * BN % kThreads && at >= 2 * BN) break;
+          const bool real = s0 + row < end;
+          const uint32_t* src = at < BN ? a.ks : a.vs;
+          const uint32_t dst = (at < BN ? dk : dv) + T::kRows + row * T::kPairBytes;
+          if (real) src += row_of(s0, row) * NG;
+          if constexpr (HD == 128) cp16_zfill(dst, src, real);
+          else cp8_zfill(dst, src, real);
+        }
       }
     }
   };
@@ -289,14 +320,15 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
   // slot (within the block) of column c of this warp's score tile i. 4-bit rows: columns 2t and
   // 2t + 1 are slots t and t + 4, so that a lane's four slots of 16 are the ones whose V rows
   // it unpacks.
-  const int wslot = ws * SN;
   auto slot_at = [&](int i, int e) {
     return Q4 ? wslot + i * 8 + t + (e & 1) * 4 : wslot + i * 8 + 2 * t + (e & 1);
   };
 
+  if (N8) __syncthreads();  // q is there
   for (int b = b0; b < b1; ++b) {
     cp_wait<S - 2>();
-    __syncthreads();
+    if (N8) __syncwarp();
+    else __syncthreads();
     {
       const int next = b + S - 1;
       if (next < b1) {
@@ -614,9 +646,11 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
           if constexpr (F32) return *reinterpret_cast<const float*>(p);
           else return bf16_to_f32(*reinterpret_cast<const __nv_bfloat16*>(p));
         };
+        // (a narrow tile's warps look at their own slots)
+        const int from = N8 ? wslot * HD + lane : tid, to = N8 ? (wslot + SN) * HD : BN * HD, step = N8 ? 32 : kThreads;
         int bad = 0;
-        for (int i = tid; i < BN * HD; i += kThreads) bad |= !is_finite(value(i / HD, i % HD));
-        if (__syncthreads_or(bad)) {
+        for (int i = from; i < to; i += step) bad |= !is_finite(value(i / HD, i % HD));
+        if (N8 ? __any_sync(0xffffffffu, bad) : __syncthreads_or(bad)) {
 #pragma unroll
           for (int i = 0; i < NO; ++i)
 #pragma unroll
@@ -632,15 +666,17 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
               }
           }
           fa = fb = 1.f;
-          __syncthreads();
-          for (int i = tid; i < BN * HD; i += kThreads) {
+          if (N8) __syncwarp();
+          else __syncthreads();
+          for (int i = from; i < to; i += step) {
             const int row = i / HD, d = i % HD;
             if (is_finite(value(row, d))) continue;
             unsigned char* p = sV + row * T::kRowBytes + (((d * (F32 ? 4 : 2) >> 4) ^ (row & 7)) << 4) + (d * (F32 ? 4 : 2) & 15);
             if constexpr (F32) *reinterpret_cast<float*>(p) = 0.f;
             else *reinterpret_cast<uint16_t*>(p) = 0;
           }
-          __syncthreads();
+          if (N8) __syncwarp();
+          else __syncthreads();
         }
       }
       if constexpr (F32 && N8) {
