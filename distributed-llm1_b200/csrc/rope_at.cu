@@ -49,6 +49,18 @@ DLLM_DEV void st_pack(float* p, const Pack<VEC>& r) {
     *p = r.v[0];
 }
 
+template <int VEC>
+DLLM_DEV Pack<VEC> ld_pack(const __nv_bfloat16* p) {
+  Pack<VEC> r;
+  if constexpr (VEC == 4) {
+    const uint2 f = *reinterpret_cast<const uint2*>(p);
+    r.v[0] = bf16_lo(f.x), r.v[1] = bf16_hi(f.x), r.v[2] = bf16_lo(f.y), r.v[3] = bf16_hi(f.y);
+  } else {
+    r.v[0] = bf16_to_f32(*p);
+  }
+  return r;
+}
+
 // Turns the VEC pairs of a unit.
 template <int VEC, bool INTER>
 DLLM_DEV void turn(Pack<VEC>& x, Pack<VEC>& y, const float (&c)[VEC], const float (&s)[VEC]) {
@@ -159,9 +171,15 @@ cudaError_t rope_hd(const RopeAtArgs& a, int sms, cudaStream_t st) {
 // head's HD / 8 threads (a warp, where pairs go one by one) hold it in registers, add their
 // squares in fp32 by shuffles, and turn it. Bound by memory like the rotation alone: the norm
 // adds 4 flops per element and one chain of shuffles, and saves a whole pass over q and k.
+// 6007 rows of 32 heads of 128: 37 us, 197 MB at 5.3 TB/s (a copy moves 6.6). The next head's
+// loads ahead of this one's sum, or the heads of a row over several CTAs, were slower (41, 43):
+// more registers and angles taken twice. The weights are loaded before the sum, so that one row
+// waits for memory once (7.1 -> 6.3 us; CTAs of 256 threads then cost long batches 2 us).
+constexpr int kNormRopeThreads = 128;
+
 template <int HD, int VEC, bool INTER>
-__global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const NormRopeArgs n, int log2_side) {
-  constexpr int units = HD / (2 * VEC), lanes = units < 32 ? units : 32, U = units / lanes, slots = kRopeThreads / lanes;
+__global__ void __launch_bounds__(kNormRopeThreads) norm_rope_kernel(const NormRopeArgs n, int log2_side) {
+  constexpr int units = HD / (2 * VEC), lanes = units < 32 ? units : 32, U = units / lanes, slots = kNormRopeThreads / lanes;
   const RopeAtArgs& a = n.rope;
   const int turning = a.rotary / (2 * VEC), heads = a.q_heads + a.k_heads;
   const int lane = threadIdx.x % lanes, slot = threadIdx.x / lanes;
@@ -203,7 +221,10 @@ __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const NormRopeA
     }
   }
   for (int h = h_first; h < heads; h += h_step) {
-    const __nv_bfloat16* w = h < a.q_heads ? n.q_norm : n.k_norm;  // 2 HD bytes, from L1
+    const __nv_bfloat16* w = h < a.q_heads ? n.q_norm : n.k_norm;  // from L1 but for the first head
+    Pack<VEC> wx[U], wy[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) wx[u] = ld_pack<VEC>(w + o1[u]), wy[u] = ld_pack<VEC>(w + o2[u]);
     float sum = 0.f;
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -217,8 +238,8 @@ __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const NormRopeA
     for (int u = 0; u < U; ++u) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        x[u].v[i] *= r * bf16_to_f32(w[o1[u] + i]);
-        y[u].v[i] *= r * bf16_to_f32(w[o2[u] + i]);
+        x[u].v[i] *= r * wx[u].v[i];
+        y[u].v[i] *= r * wy[u].v[i];
       }
       if (lane + u * lanes < turning) turn<VEC, INTER>(x[u], y[u], c[u], s[u]);
       st_pack<VEC>(dst + o1[u], x[u]);
@@ -230,7 +251,7 @@ __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const NormRopeA
 
 template <int HD, int VEC, bool INTER>
 cudaError_t launch_norm_rope(const NormRopeArgs& n, int sms, cudaStream_t st) {
-  constexpr int units = HD / (2 * VEC), slots = kRopeThreads / (units < 32 ? units : 32);
+  constexpr int units = HD / (2 * VEC), slots = kNormRopeThreads / (units < 32 ? units : 32);
   const RopeAtArgs& a = n.rope;
   const int heads = a.q_heads + a.k_heads;
   int log2_side = 0;
@@ -238,7 +259,7 @@ cudaError_t launch_norm_rope(const NormRopeArgs& n, int sms, cudaStream_t st) {
   const int rows = slots >> log2_side, chunks = (heads + (1 << log2_side) - 1) >> log2_side;
   const int ctas = (a.n + rows - 1) / rows;
   const dim3 grid(ctas, (long long)ctas * chunks <= 8ll * sms ? chunks : 1);  // as above
-  norm_rope_kernel<HD, VEC, INTER><<<grid, kRopeThreads, 0, st>>>(n, log2_side);
+  norm_rope_kernel<HD, VEC, INTER><<<grid, kNormRopeThreads, 0, st>>>(n, log2_side);
   return cudaGetLastError();
 }
 
