@@ -849,89 +849,102 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
   });
 }
 
-// Joins a tile's segments. W warps share one row: warp w folds the segments w, w + W, ... in order,
+// Joins a tile's segments. W warps share a row: warp w folds the segments w, w + W, ... in order,
 // then the warps' results are folded in order, so the sum does not depend on timing. Every
 // segment's maximum, sum and output are loaded together: the chain is one load per kBatch segments.
-template <int HD, int W>
+// A warp takes J rows at once: the 36600 rows of two segments that a chunk of 2048 leaves are one
+// wave of CTAs with four of them, four waves with one (3 us longer).
+template <int HD, int W, int J>
 __global__ void __launch_bounds__(kThreads) rows_join_kernel(const __grid_constant__ RowsKernelArgs P, int rt, int bn) {
-  constexpr int V = HD / 32, kBatch = 4, kRows = 8 / W;
+  constexpr int V = HD / 32, kBatch = J == 1 ? 4 : 2, kRows = 8 / W * J;
+  static_assert(J == 1 || W == 1, "shared rows come one at a time");
   __shared__ float so[8][HD], sml[8][2];
   const RowsAttnArgs& a = P.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = warp % W;
-  const int per = rt / kRows, split = blockIdx.x / per, row = blockIdx.x % per * kRows + warp / W;
+  const int per = rt / kRows, split = blockIdx.x / per, row0 = blockIdx.x % per * kRows + warp / W * J;
   const RowsTile k(P, P.split_tile[split], rt, bn);
   const int c0 = P.split_cta[split], nsplit = P.split_n[split];
-  const bool live = k.r0 + row < k.R;
+  const int live = k.R - k.r0 - row0;  // rows from row0 on
   // the tile is the first segment of every CTA but the first one, and of that one if it began there
   const bool later = P.begin_tile[c0] != P.split_tile[split];
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the segments' grid has ended and its stores are visible
-  float m = kNegInf, l = 0.f, acc[V];
+  float m[J], l[J], acc[J][V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) acc[e] = 0.f;
-  if (live) {
-    for (int s0 = w; s0 < nsplit; s0 += kBatch * W) {
-      float2 ml[kBatch];
-      float o[kBatch][V];
+  for (int j = 0; j < J; ++j) {
+    m[j] = kNegInf, l[j] = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[j][e] = 0.f;
+  }
+  for (int s0 = w; s0 < nsplit; s0 += kBatch * W) {
+    float2 ml[J][kBatch];
+    float o[J][kBatch][V];
+#pragma unroll
+    for (int j = 0; j < J; ++j)
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         const int s = s0 + u * W;
-        ml[u] = make_float2(kNegInf, 0.f);
+        ml[j][u] = make_float2(kNegInf, 0.f);
 #pragma unroll
-        for (int e = 0; e < V; ++e) o[u][e] = 0.f;
-        if (s < nsplit) {
-          const size_t p = ((size_t)(c0 + s) * 2 + (s == 0 && later)) * rt + row;
-          ml[u] = *reinterpret_cast<const float2*>(a.part_ml + p * 2);
+        for (int e = 0; e < V; ++e) o[j][u][e] = 0.f;
+        if (s < nsplit && j < live) {
+          const size_t p = ((size_t)(c0 + s) * 2 + (s == 0 && later)) * rt + row0 + j;
+          ml[j][u] = *reinterpret_cast<const float2*>(a.part_ml + p * 2);
           if constexpr (V == 4) {
             const float4 f = *reinterpret_cast<const float4*>(a.part_o + p * HD + lane * 4);
-            o[u][0] = f.x, o[u][1] = f.y, o[u][2] = f.z, o[u][3] = f.w;
+            o[j][u][0] = f.x, o[j][u][1] = f.y, o[j][u][2] = f.z, o[j][u][3] = f.w;
           } else {
             const float2 f = *reinterpret_cast<const float2*>(a.part_o + p * HD + lane * 2);
-            o[u][0] = f.x, o[u][1] = f.y;
+            o[j][u][0] = f.x, o[j][u][1] = f.y;
           }
         }
       }
-      float x = m;
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) x = fmaxf(x, ml[u].x);
-      const float b = x == kNegInf ? 0.f : x, f = ex2(m - b);
-      m = x, l *= f;
+    for (int j = 0; j < J; ++j) {
+      float x = m[j];
 #pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] *= f;
+      for (int u = 0; u < kBatch; ++u) x = fmaxf(x, ml[j][u].x);
+      const float b = x == kNegInf ? 0.f : x, f = ex2(m[j] - b);
+      m[j] = x, l[j] *= f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[j][e] *= f;
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
-        const float wt = ex2(ml[u].x - b);
-        l = fmaf(ml[u].y, wt, l);
+        const float wt = ex2(ml[j][u].x - b);
+        l[j] = fmaf(ml[j][u].y, wt, l[j]);
 #pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] = fmaf(o[u][e], wt, acc[e]);
+        for (int e = 0; e < V; ++e) acc[j][e] = fmaf(o[j][u][e], wt, acc[j][e]);
       }
     }
   }
   if constexpr (W > 1) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) so[warp][lane * V + e] = acc[e];
-    if (lane == 0) sml[warp][0] = m, sml[warp][1] = l;
+    for (int e = 0; e < V; ++e) so[warp][lane * V + e] = acc[0][e];
+    if (lane == 0) sml[warp][0] = m[0], sml[warp][1] = l[0];
     __syncthreads();
     if (w != 0) return;
     float x = kNegInf;
 #pragma unroll
     for (int u = 0; u < W; ++u) x = fmaxf(x, sml[warp + u][0]);
     const float b = x == kNegInf ? 0.f : x;
-    l = 0.f;
+    l[0] = 0.f;
 #pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] = 0.f;
+    for (int e = 0; e < V; ++e) acc[0][e] = 0.f;
 #pragma unroll
     for (int u = 0; u < W; ++u) {
       const float wt = ex2(sml[warp + u][0] - b);
-      l = fmaf(sml[warp + u][1], wt, l);
+      l[0] = fmaf(sml[warp + u][1], wt, l[0]);
 #pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] = fmaf(so[warp + u][lane * V + e], wt, acc[e]);
+      for (int e = 0; e < V; ++e) acc[0][e] = fmaf(so[warp + u][lane * V + e], wt, acc[0][e]);
     }
   }
-  if (!live) return;
-  const float inv = 1.0f / l;
-  float* dst = a.out + ((size_t)k.row0 * a.nq + k.place(k.r0 + row, a.nq)) * HD + lane * V;
 #pragma unroll
-  for (int e = 0; e < V; ++e) dst[e] = acc[e] * inv;
+  for (int j = 0; j < J; ++j) {
+    if (j >= live) return;
+    const float inv = 1.0f / l[j];
+    float* dst = a.out + ((size_t)k.row0 * a.nq + k.place(k.r0 + row0 + j, a.nq)) * HD + lane * V;
+    if constexpr (V == 4) *reinterpret_cast<float4*>(dst) = make_float4(acc[j][0] * inv, acc[j][1] * inv, acc[j][2] * inv, acc[j][3] * inv);
+    else *reinterpret_cast<float2*>(dst) = make_float2(acc[j][0] * inv, acc[j][1] * inv);
+  }
 }
 
 template <int KIND, int HD, int WR>
@@ -1028,7 +1041,7 @@ RowsPlan rows_plan(const RowsAttnArgs& a, const RowsBatch& b, int rt, int bn, in
   P->n_seqs = b.n_seqs;
   const int kvh = a.pages.kvh, G = a.nq / kvh;
   std::vector<int> blocks;  // of every tile
-  int total = 0;
+  long long total = 0;
   for (int i = 0; i < b.n_seqs; ++i) {
     P->seq[i] = b.seq[i], P->row0[i] = b.row0[i], P->m[i] = b.m[i], P->t0[i] = b.t0[i];
     P->tile0[i] = (int)blocks.size();
@@ -1046,7 +1059,7 @@ RowsPlan rows_plan(const RowsAttnArgs& a, const RowsBatch& b, int rt, int bn, in
   P->tile0[b.n_seqs] = tiles;
   P->unit0[b.n_seqs] = plan.units;
   max_ctas = std::min(max_ctas, kRowsMaxCtas);
-  const int share = std::max((total + max_ctas - 1) / max_ctas, least);
+  const int share = std::max((int)((total + max_ctas - 1) / max_ctas), least);
   // the smallest shares with which every tile's blocks are split on their own
   int own = share;
   for (; tiles <= max_ctas && own <= share + start; ++own) {
@@ -1079,11 +1092,10 @@ RowsPlan rows_plan(const RowsAttnArgs& a, const RowsBatch& b, int rt, int bn, in
   return plan;
 }
 
-cudaError_t rows_join(const RowsKernelArgs& P, const RowsPlan& plan, int rt, int bn, int hd, int* launches, cudaStream_t st) {
-  if (plan.splits == 0) return cudaSuccess;
-  const bool many = plan.most_n > 8;
+template <int HD, int W, int J>
+cudaError_t launch_join(const RowsKernelArgs& P, int splits, int rt, int bn, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(plan.splits * (many ? rt : rt / 8));
+  cfg.gridDim = dim3(splits * (rt / (8 / W * J)));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -1091,9 +1103,18 @@ cudaError_t rows_join(const RowsKernelArgs& P, const RowsPlan& plan, int rt, int
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, rows_join_kernel<HD, W, J>, P, rt, bn);
+}
+template <int HD>
+cudaError_t join_hd(const RowsKernelArgs& P, const RowsPlan& plan, int rt, int bn, cudaStream_t st) {
+  if (plan.most_n > 8) return launch_join<HD, 8, 1>(P, plan.splits, rt, bn, st);
+  return rt % 32 ? launch_join<HD, 1, 1>(P, plan.splits, rt, bn, st) : launch_join<HD, 1, 4>(P, plan.splits, rt, bn, st);
+}
+
+cudaError_t rows_join(const RowsKernelArgs& P, const RowsPlan& plan, int rt, int bn, int hd, int* launches, cudaStream_t st) {
+  if (plan.splits == 0) return cudaSuccess;
   *launches += 1;
-  if (hd == 64) return cudaLaunchKernelEx(&cfg, many ? rows_join_kernel<64, 8> : rows_join_kernel<64, 1>, P, rt, bn);
-  return cudaLaunchKernelEx(&cfg, many ? rows_join_kernel<128, 8> : rows_join_kernel<128, 1>, P, rt, bn);
+  return hd == 64 ? join_hd<64>(P, plan, rt, bn, st) : join_hd<128>(P, plan, rt, bn, st);
 }
 
 // Two partial tiles per CTA: 2 sms of 256 rows, or 4 sms of 64.

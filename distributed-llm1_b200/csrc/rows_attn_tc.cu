@@ -24,6 +24,8 @@
 // registers. With two planes S takes q_high (K_high | K_low) as one MMA of N = 128, and
 // q_low K_high goes to the K_low half; the softmax adds the halves.
 // Tensor memory: S and P of both tiles 2 x 128 columns, O 2 x 128.
+// The main kernel starts while the planes are written (its CTAs set up and bring q), and waits for
+// that grid's end before it reads them (a prompt of 1501 rows: 47 -> 43 us with its launches).
 #include "rows_attn_tc.cuh"
 #include "tc.cuh"
 
@@ -59,6 +61,7 @@ __global__ void __launch_bounds__(kPlaneThreads) rows_planes_kernel(const __grid
   __shared__ float smax[kPlaneThreads / 32];
   __shared__ int sbad;
   const RowsAttnArgs& a = P.a;
+  asm volatile("griddepcontrol.launch_dependents;");  // the main kernel may start; it waits for this grid's end
   const int which = blockIdx.x & 1, at = blockIdx.x >> 1, i = rows_find(P.unit0, P.n_seqs, at);
   const RowsView v(P.t0[i], P.t0[i] + P.m[i] - 1, a.window, a.sinks, T::BN);
   const int head = (at - P.unit0[i]) / v.nb, s0 = v.slot0((at - P.unit0[i]) % v.nb, T::BN), end = v.p1 + 1;
@@ -162,8 +165,8 @@ DLLM_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* ba
 }
 
 // The MMA's shared-memory descriptors (tc.cuh) as two words: the upper one is the same for all
-// operands here, and the lower one moves by constants. Built anew as 64-bit values, an MMA took 95
-// cycles to issue and 65 to run.
+// operands here, and the lower one moves by constants (2% of a long chunk's time against 64-bit
+// values built anew).
 constexpr uint32_t kDescHigh = 64u | 1u << 14 | 2u << 29;
 DLLM_DEV uint32_t desc_low(const void* tile, uint32_t leading) { return (smem_u32(tile) & 0x3FFFFu) >> 4 | leading << 16; }
 DLLM_DEV void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
@@ -228,6 +231,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
   if (warp >= kTcSoftWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == kTcSoftWarps && lane == 0) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");  // the blocks are there
       // ---- producer: tile t is K of block t / 2 (even) or V. It reports to the barriers that the
       // first tile's MMAs wait for: ok_ready of the block (K), pv_ready (V). A barrier's earlier turn, 2
       // kTurns >= kRing tiles before, has ended: the stage's earlier tile came later, and is used up.
@@ -388,6 +392,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
         mbar_arrive(&sh.q_ready[w]);
         asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory");  // `back` is there
       }
+      asm volatile("griddepcontrol.wait;" ::: "memory");  // the blocks' factors are there
       const int slot = k.slot_of(r0 + me);
       float o[HD], m = -INFINITY, l = 0.f, unit = 0.f;
 #pragma unroll
@@ -397,13 +402,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
       const int p0 = k.t0 + r0 / k.G, p1 = k.t0 + (min(r0 + 128, k.R) - 1) / k.G;
       const float2* info = static_cast<const float2*>(a.info);
       int s0 = k.v.slot0(b0, BN);
-      float4 next = __ldg(reinterpret_cast<const float4*>(info + 2 * (size_t)unit_of(k, s0)));
+      float4 next = *reinterpret_cast<const float4*>(info + 2 * (size_t)unit_of(k, s0));
       for (int n = 0; n < nb; ++n, ++done) {
         const float4 now = next;  // factor of K, -, factor of V, whether V had other than numbers
         const int s_now = s0;
         if (n + 1 < nb) {
           s0 = k.v.slot0(b0 + n + 1, BN);
-          next = __ldg(reinterpret_cast<const float4*>(info + 2 * (size_t)unit_of(k, s0)));
+          next = *reinterpret_cast<const float4*>(info + 2 * (size_t)unit_of(k, s0));
         }
         const float f = fmaxf(back * now.x, 1.175494351e-38f);  // (-inf times 0 would be NaN)
         const bool edge = s_now + BN - 1 > p0 || (s_now <= p1 - a.window && s_now + BN > a.sinks);
@@ -607,9 +612,20 @@ cudaError_t launch(const RowsAttnArgs& a, const RowsBatch& b, int sms, int* laun
   const RowsPlan plan = rows_plan(a, b, kTcTileRows, T::BN, sms, kTcLeastShare, 2, &P);
   P.a.info = static_cast<char*>(a.planes) + (size_t)plan.units * 2 * T::kTile;
   rows_planes_kernel<KIND, HD><<<2 * plan.units, kPlaneThreads, 0, st>>>(P);
-  rows_tc_kernel<KIND, HD><<<plan.ctas, kTcThreads, T::kSmem, st>>>(P);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(plan.ctas);
+  cfg.blockDim = dim3(kTcThreads);
+  cfg.dynamicSmemBytes = T::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, rows_tc_kernel<KIND, HD>, P);
   *launches += 2;
-  const cudaError_t e = cudaGetLastError();
   return e != cudaSuccess ? e : rows_join(P, plan, kTcTileRows, T::BN, HD, launches, st);
 }
 
