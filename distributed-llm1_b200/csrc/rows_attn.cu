@@ -29,7 +29,8 @@
 // Up to 8 rows (WR = 0: decode steps) the products' 16 rows would be half empty. There o is
 // computed transposed, V^T (p^T): the 8 rows are the products' narrow side, what a thread holds of
 // row g of the scores is what the second operand wants, and scaling, cutting and accumulating p
-// and o take half the instructions and registers, so that two CTAs share an SM.
+// and o take half the instructions and registers, so that two CTAs share an SM. In the scores the second
+// terms of q take rows 8 to 15: one product instead of two.
 #include "rows_attn.cuh"
 
 #include <algorithm>
@@ -77,8 +78,9 @@ struct Tile {
   static constexpr int kChunks = kRowBytes / 16;
   static constexpr int kRows = BN * kRowBytes, kTileBytes = kRows + BN * kPairBytes;  // one of K, V
   static constexpr int kCtas = kNarrow && kQ4 ? 2 : 1;  // per SM
-  static constexpr int kQRows = kNarrow ? 16 : RT;
-  static constexpr int kQBytes = kQ4 ? (kNarrow ? HD * 32 : 0) : kQRows * HD * (kF32 ? 4 : 6);  // (wide 4-bit tiles: registers)
+  static constexpr int kQRows = kNarrow && !kF32 ? 16 : RT;
+  // (wide 4-bit tiles keep q in registers)
+  static constexpr int kQBytes = kQ4 ? (kNarrow ? HD * 32 : 0) : kQRows * HD * (kF32 ? 4 : kNarrow ? 4 : 6);
   static constexpr int kPad = HD + 4;
   static constexpr int kMergeBytes = WS * RT * (kPad + 2) * 4;
   static constexpr int kFit = ((kCtas == 2 ? 112 : 225) * 1024 - kQBytes) / (2 * kTileBytes);
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
 
   // ---- the q tile, scaled by log2(e) / sqrt(hd) so that the softmax is in powers of two
   uint32_t qf[Q4 && !N8 ? HD / 16 : 1][2][4];  // 4-bit rows: A fragments of two fp16 terms
-  uint2* qs = reinterpret_cast<uint2*>(sQ) + lane;  // of a narrow tile (rows 8 to 15 are zero): [k step][term][lane]
+  uint4* qs = reinterpret_cast<uint4*>(sQ) + lane;  // of a narrow tile: [k step][lane]
   float qsum_a[Q4 ? NG : 1], qsum_b[Q4 ? NG : 1], back_a = 1.f, back_b = 1.f;
   if constexpr (Q4) {
     // lane t of a row holds dims 8t .. 8t + 7 of every group: a u32 of codes
@@ -267,14 +269,13 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
         split2_f16(xa[i][d + u] * ia, xa[i][d + u + 4] * ia, f[0][2 * u], f[1][2 * u]);
         split2_f16(xb[i][d + u] * ib, xb[i][d + u + 4] * ib, f[0][2 * u + 1], f[1][2 * u + 1]);
       }
+      if constexpr (N8) {
+        if (warp == ks % 8) qs[ks * 32] = make_uint4(f[0][0], f[1][0], f[0][2], f[1][2]);  // (all warps have it)
+      } else {
 #pragma unroll
-      for (int term = 0; term < 2; ++term) {
-        if constexpr (N8) {
-          if (warp == ks % 8) qs[(ks * 2 + term) * 32] = make_uint2(f[term][0], f[term][2]);  // (all warps have it)
-        } else {
+        for (int term = 0; term < 2; ++term)
 #pragma unroll
           for (int e = 0; e < 4; ++e) qf[ks][term][e] = f[term][e];
-        }
       }
     }
   } else {
@@ -293,6 +294,14 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
         split3(f.x, f.y, h[0], m[0], l[0]);
         split3(f.z, f.w, h[1], m[1], l[1]);
         unsigned char* p = sQ + row * HD * 2 + (((d >> 3) ^ (row & 7)) << 4) + (d & 4) * 2;
+        if constexpr (N8) {  // rows 8 to 15: the second terms, and nothing beside the third ones
+          if (row < RT) {
+            *reinterpret_cast<uint2*>(p) = make_uint2(h[0], h[1]);
+            *reinterpret_cast<uint2*>(p + RT * HD * 2) = make_uint2(m[0], m[1]);
+          }
+          *reinterpret_cast<uint2*>(p + T::kQRows * HD * 2) = make_uint2(l[0], l[1]);
+          continue;
+        }
         *reinterpret_cast<uint2*>(p) = make_uint2(h[0], h[1]);
         *reinterpret_cast<uint2*>(p + T::kQRows * HD * 2) = make_uint2(m[0], m[1]);
         *reinterpret_cast<uint2*>(p + 2 * T::kQRows * HD * 2) = make_uint2(l[0], l[1]);
@@ -350,15 +359,15 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
     if constexpr (Q4) {
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
-        uint32_t q[2][2][4];  // [k step][term]
+        uint32_t q[2][2][4];  // [k step][term]; a narrow tile has the second term in rows 8 to 15 of the first
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < 2; ++u) {
           if constexpr (N8) {
-            const uint2 f = qs[(gr * 4 + u) * 32];
-            q[u / 2][u % 2][0] = f.x, q[u / 2][u % 2][1] = 0u, q[u / 2][u % 2][2] = f.y, q[u / 2][u % 2][3] = 0u;
+            const uint4 f = qs[(gr * 2 + u) * 32];
+            q[u][0][0] = f.x, q[u][0][1] = f.y, q[u][0][2] = f.z, q[u][0][3] = f.w;
           } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) q[u / 2][u % 2][e] = qf[gr * 2 + u / 2][u % 2][e];
+            for (int e = 0; e < 8; ++e) q[u][e / 4][e % 4] = qf[gr * 2 + u][e / 4][e % 4];
           }
         }
 #pragma unroll
@@ -369,10 +378,13 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
           const uint32_t p1 = *reinterpret_cast<const uint32_t*>(sK + T::kRows + slot_at(i, 1) * T::kPairBytes + gr * 4);
           float c[4] = {0.f, 0.f, 0.f, 0.f};
           const uint32_t n0 = codes_f16(w), n1 = codes_f16(w >> 4), n2 = codes_f16(w >> 8), n3 = codes_f16(w >> 12);
-          mma_f16(c, q[0][1], n0, n1);
-          mma_f16(c, q[1][1], n2, n3);
+          if constexpr (!N8) {
+            mma_f16(c, q[0][1], n0, n1);
+            mma_f16(c, q[1][1], n2, n3);
+          }
           mma_f16(c, q[0][0], n0, n1);
           mma_f16(c, q[1][0], n2, n3);
+          if constexpr (N8) c[0] += c[2], c[1] += c[3];
           // c is (q . (code - 8)) / back, and the sums of q are divided alike
           const float sc0 = bf16_lo(p0), sc1 = bf16_lo(p1);
           const float mn0 = fmaf(8.f, sc0, bf16_hi(p0)), mn1 = fmaf(8.f, sc1, bf16_hi(p1));
@@ -396,10 +408,10 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
       for (int ks = 0; ks < HD / 8; ++ks) {
         uint32_t qh[4], ql[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 4; e += N8 ? 2 : 1) {
           const int row = wr * 16 + g + (e & 1) * 8, ch = ks * 2 + (e >> 1);
-          if (N8 && (e & 1)) qh[e] = ql[e] = 0u;
-          else split_tf32(*reinterpret_cast<const float*>(sQ + row * HD * 4 + ((ch ^ (row & 7)) << 4) + t * 4), qh[e], ql[e]);
+          split_tf32(*reinterpret_cast<const float*>(sQ + row * HD * 4 + ((ch ^ (row & 7)) << 4) + t * 4), qh[e], ql[e]);
+          if constexpr (N8) qh[e + 1] = ql[e];  // a narrow tile: the second terms in rows 8 to 15
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -409,16 +421,21 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
           for (int e = 0; e < 2; ++e)
             split_tf32(*reinterpret_cast<const float*>(sK + row * T::kRowBytes + (((ks * 2 + e) ^ (row & 7)) << 4) + t * 4),
                        kh[e], kl[e]);
-          mma_tf32(s0_[nt], ql, kl[0], kl[1]);
           mma_tf32(sh[nt], qh, kh[0], kh[1]);
           mma_tf32(s1[nt], qh, kl[0], kl[1]);
-          mma_tf32(s2[nt], ql, kh[0], kh[1]);
+          if constexpr (!N8) {
+            mma_tf32(s0_[nt], ql, kl[0], kl[1]);
+            mma_tf32(s2[nt], ql, kh[0], kh[1]);
+          }
         }
       }
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sh[i][e] += s0_[i][e] + (s1[i][e] + s2[i][e]);
+        for (int e = 0; e < (N8 ? 2 : 4); ++e) {
+          if constexpr (N8) sh[i][e] += s1[i][e + 2] + (s1[i][e] + sh[i][e + 2]);
+          else sh[i][e] += s0_[i][e] + (s1[i][e] + s2[i][e]);
+        }
     } else {
       float ss[NT][4];
 #pragma unroll
@@ -432,9 +449,9 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
       for (int ks = 0; ks < HD / 16; ++ks) {
         uint32_t qh[4], qm[4], ql[4];
         const uint32_t at = qa + (((2 * ks + (lane >> 4)) ^ (arow & 7)) << 4);
-        ldsm4(qh, at);
-        ldsm4(qm, at + T::kQRows * HD * 2);
-        ldsm4(ql, at + 2 * T::kQRows * HD * 2);
+        ldsm4(qh, at);  // a narrow tile: with the second terms in rows 8 to 15
+        ldsm4(ql, at + (N8 ? 1 : 2) * T::kQRows * HD * 2);
+        if constexpr (!N8) ldsm4(qm, at + T::kQRows * HD * 2);
 #pragma unroll
         for (int np = 0; np < NT / 2; ++np) {
           const int row = wslot + np * 16 + krow;
@@ -442,8 +459,10 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
           ldsm4(k4, smem_addr(sK) + row * T::kRowBytes + (((2 * ks + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
           mma_bf16(sh[2 * np], qh, k4[0], k4[1]);
           mma_bf16(sh[2 * np + 1], qh, k4[2], k4[3]);
-          mma_bf16(ss[2 * np], qm, k4[0], k4[1]);
-          mma_bf16(ss[2 * np + 1], qm, k4[2], k4[3]);
+          if constexpr (!N8) {
+            mma_bf16(ss[2 * np], qm, k4[0], k4[1]);
+            mma_bf16(ss[2 * np + 1], qm, k4[2], k4[3]);
+          }
           mma_bf16(ss[2 * np], ql, k4[0], k4[1]);
           mma_bf16(ss[2 * np + 1], ql, k4[2], k4[3]);
         }
@@ -451,7 +470,10 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sh[i][e] += ss[i][e];
+        for (int e = 0; e < (N8 ? 2 : 4); ++e) {
+          if constexpr (N8) sh[i][e] += sh[i][e + 2] + ss[i][e];
+          else sh[i][e] += ss[i][e];
+        }
     }
 
     // ---- mask: only blocks that some row sees a part of have anything to hide
@@ -550,12 +572,10 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
         const uint32_t d0 = pack_bf16(mid[0] - bf16_lo(b0), mid[1] - bf16_hi(b0));
         const uint32_t d1 = pack_bf16(mid[2] - bf16_lo(b1), mid[3] - bf16_hi(b1));
         if constexpr (N8) {
-          const uint32_t bb4[4] = {b0, 0u, b1, 0u}, dd4[4] = {d0, 0u, d1, 0u};
-          mma_bf16(cm, bb4, l[0], l[2]);
-          mma_bf16(cm, dd4, m[0], m[2]);
-          mma_bf16(cm, dd4, h[0], h[2]);
-          mma_bf16(cm, bb4, m[0], m[2]);
-          mma_bf16(cm, bb4, h[0], h[2]);
+          const uint32_t bd4[4] = {b0, d0, b1, d1};  // rows 8 to 15: the second terms
+          mma_bf16(cm, bd4, l[0], l[2]);
+          mma_bf16(cm, bd4, m[0], m[2]);
+          mma_bf16(cm, bd4, h[0], h[2]);
         } else {
           mma_bf16(cm, l, b0, b1);
           mma_bf16(cm, m, d0, d1);
@@ -564,8 +584,9 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
           mma_bf16(cm, h, b0, b1);
         }
       }
+      if constexpr (N8) cm[0] += cm[2], cm[1] += cm[3];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < (N8 ? 2 : 4); ++e)
         om[e] = nan_bits[e] ? __uint_as_float(nan_bits[e]) : fmaf(om[e], second(e) ? fb : fa, cm[e]);
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
