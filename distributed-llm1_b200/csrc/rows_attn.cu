@@ -16,7 +16,8 @@
 // over 8000 slots the outputs were off by 8e-6, and are by 7e-7.) Codes are exact in any 16-bit type, and the other operand runs as two fp16 terms (22 bits)
 // of fp32 values brought into fp16's range by a power of two: a row of q by one next to its
 // largest element, p scale by one next to the block's largest scale. A pair of codes becomes
-// fp16 as (nibbles | bits of 1024) - 1032. (The nibbles alone, read as fp16, are code * 2^-24,
+// fp16 as (nibbles | bits of 1024) - 1032; the odd nibbles of a byte stay where they are, as 16 times their
+// codes, and what they meet is a sixteenth. (The nibbles alone, read as fp16, are code * 2^-24,
 // but the tensor core aligns such subnormal products by their exponents, 10 bits above their
 // leading ones, and the sums lose as many: 4e-6 over 9 slots.) p meets the middles in bf16
 // terms, three of p and two of them.
@@ -52,12 +53,19 @@ DLLM_DEV void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Nibbles 0 and 4 of u, less 8, as packed fp16.
+// Nibbles 0 and 4 of u, less 8, as packed fp16, and 16 times nibbles 1 and 5, less 8.
 DLLM_DEV uint32_t codes_f16(uint32_t u) {
   uint32_t r;
   asm("{\n\t.reg .b32 t;\n\tlop3.b32 t, %1, 0x000f000f, 0x64006400, 0xea;\n\tsub.rn.f16x2 %0, t, %2;\n\t}"
       : "=r"(r)
       : "r"(u), "r"(0x64086408u));
+  return r;
+}
+DLLM_DEV uint32_t codes16_f16(uint32_t u) {
+  uint32_t r;
+  asm("{\n\t.reg .b32 t;\n\tlop3.b32 t, %1, 0x00f000f0, 0x64006400, 0xea;\n\tsub.rn.f16x2 %0, t, %2;\n\t}"
+      : "=r"(r)
+      : "r"(u), "r"(0x64806480u));
   return r;
 }
 DLLM_DEV void cp8_zfill(uint32_t dst, const void* src, bool real) {
@@ -252,12 +260,12 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
         qsum_b[i] += __shfl_xor_sync(0xffffffffu, qsum_b[i], w);
       }
     }
-    // 2^e next to the largest element: the row divided by it lies in [-2, 2]. The exponent is
-    // kept where 2^e and its inverse are normal numbers.
-    auto power = [](float m) { return min(max((int)(__float_as_uint(m) >> 23) & 0xff, 1), 253); };
+    // 2^e next to the largest element: the row divided by it, times 16, lies in [-32, 32] (dims that meet
+    // 16 times their codes lack the 16). The exponent is kept where the factors are normal numbers.
+    auto power = [](float m) { return min(max((int)(__float_as_uint(m) >> 23) & 0xff, 5), 253); };
     const int ea = power(ma), eb = power(mb);
-    const float ia = power_of_two(254 - ea), ib = power_of_two(254 - eb);
-    back_a = power_of_two(ea), back_b = power_of_two(eb);
+    const float ia = power_of_two(258 - ea), ib = power_of_two(258 - eb);
+    back_a = power_of_two(ea - 4), back_b = power_of_two(eb - 4);
 #pragma unroll
     for (int i = 0; i < NG; ++i) qsum_a[i] *= ia, qsum_b[i] *= ib;
 #pragma unroll
@@ -266,8 +274,9 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
       uint32_t f[2][4];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {  // dims d + u and d + u + 4: the two halves of a nibble pair
-        split2_f16(xa[i][d + u] * ia, xa[i][d + u + 4] * ia, f[0][2 * u], f[1][2 * u]);
-        split2_f16(xb[i][d + u] * ib, xb[i][d + u + 4] * ib, f[0][2 * u + 1], f[1][2 * u + 1]);
+        const float ja = u ? ia * 0.0625f : ia, jb = u ? ib * 0.0625f : ib;
+        split2_f16(xa[i][d + u] * ja, xa[i][d + u + 4] * ja, f[0][2 * u], f[1][2 * u]);
+        split2_f16(xb[i][d + u] * jb, xb[i][d + u + 4] * jb, f[0][2 * u + 1], f[1][2 * u + 1]);
       }
       if constexpr (N8) {
         if (warp == ks % 8) qs[ks * 32] = make_uint4(f[0][0], f[1][0], f[0][2], f[1][2]);  // (all warps have it)
@@ -309,8 +318,8 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
     }
   }
 
-  // 4-bit rows: o of a group is in units of `unit` (a power of two, the same in the whole warp),
-  // and om is the middles' share, by group
+  // 4-bit rows: o of a group is in units of `unit` (a power of two, the same in the whole warp; dims of
+  // odd nibbles of a byte: a sixteenth of it), and om is the middles' share, by group
   constexpr int NO = N8 ? HD / 16 : HD / 8;
   float o[NO][4], om[4] = {0.f, 0.f, 0.f, 0.f}, unit[Q4 ? NG : 1];
 #pragma unroll
@@ -377,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
           const uint32_t p0 = *reinterpret_cast<const uint32_t*>(sK + T::kRows + slot_at(i, 0) * T::kPairBytes + gr * 4);
           const uint32_t p1 = *reinterpret_cast<const uint32_t*>(sK + T::kRows + slot_at(i, 1) * T::kPairBytes + gr * 4);
           float c[4] = {0.f, 0.f, 0.f, 0.f};
-          const uint32_t n0 = codes_f16(w), n1 = codes_f16(w >> 4), n2 = codes_f16(w >> 8), n3 = codes_f16(w >> 12);
+          const uint32_t n0 = codes_f16(w), n1 = codes16_f16(w), n2 = codes_f16(w >> 8), n3 = codes16_f16(w >> 8);
           if constexpr (!N8) {
             mma_f16(c, q[0][1], n0, n1);
             mma_f16(c, q[1][1], n2, n3);
@@ -632,11 +641,12 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
 #pragma unroll
           for (int i = 0; i < NC; ++i) {
             if constexpr (N8) {
-              const uint32_t v[4] = {codes_f16(w0 >> (8 * i)), codes_f16(w0 >> (8 * i + 4)), codes_f16(w1 >> (8 * i)), codes_f16(w1 >> (8 * i + 4))};
+              const uint32_t v[4] = {codes_f16(w0 >> (8 * i)), codes16_f16(w0 >> (8 * i)), codes_f16(w1 >> (8 * i)), codes16_f16(w1 >> (8 * i))};
               mma_f16(c[i], v, l[0], l[2]);
               mma_f16(c[i], v, h[0], h[2]);
             } else {
-              const uint32_t b0 = codes_f16(w0 >> (4 * i)), b1 = codes_f16(w1 >> (4 * i));
+              const uint32_t u0 = w0 >> (i / 2 * 8), u1 = w1 >> (i / 2 * 8);
+              const uint32_t b0 = i % 2 ? codes16_f16(u0) : codes_f16(u0), b1 = i % 2 ? codes16_f16(u1) : codes_f16(u1);
               mma_f16(c[i], l, b0, b1);
               mma_f16(c[i], h, b0, b1);
             }
@@ -834,9 +844,9 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
         const int d = gr * kGroup4 + 8 * (g & 3) + 4 * (g >> 2);
         const float(&x)[4] = o[gr * 2];
         const float(&y)[4] = o[gr * 2 + 1];
-        const float u = unit[gr];
-        *reinterpret_cast<float4*>(oc + d) = make_float4(fmaf(x[0], u, m0), fmaf(x[2], u, m0), fmaf(y[0], u, m0), fmaf(y[2], u, m0));
-        *reinterpret_cast<float4*>(od + d) = make_float4(fmaf(x[1], u, m1), fmaf(x[3], u, m1), fmaf(y[1], u, m1), fmaf(y[3], u, m1));
+        const float u = unit[gr], v = u * 0.0625f;
+        *reinterpret_cast<float4*>(oc + d) = make_float4(fmaf(x[0], u, m0), fmaf(x[2], v, m0), fmaf(y[0], u, m0), fmaf(y[2], v, m0));
+        *reinterpret_cast<float4*>(od + d) = make_float4(fmaf(x[1], u, m1), fmaf(x[3], v, m1), fmaf(y[1], u, m1), fmaf(y[3], v, m1));
       }
     } else {
 #pragma unroll
@@ -852,8 +862,9 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
       if constexpr (Q4) {
         const int gr = i / 4, d = gr * kGroup4 + (t & 1) * 16 + (t >> 1) * 4 + i % 4, from = (lane & ~3) | gr >> 1;
         const float m0 = __shfl_sync(0xffffffffu, om[gr & 1], from), m1 = __shfl_sync(0xffffffffu, om[2 + (gr & 1)], from);
-        oa[d] = fmaf(o[i][0], unit[gr], m0), oa[d + 8] = fmaf(o[i][1], unit[gr], m0);
-        ob[d] = fmaf(o[i][2], unit[gr], m1), ob[d + 8] = fmaf(o[i][3], unit[gr], m1);
+        const float u = i % 2 ? unit[gr] * 0.0625f : unit[gr];
+        oa[d] = fmaf(o[i][0], u, m0), oa[d + 8] = fmaf(o[i][1], u, m0);
+        ob[d] = fmaf(o[i][2], u, m1), ob[d + 8] = fmaf(o[i][3], u, m1);
       } else {
         *reinterpret_cast<float2*>(oa + i * 8 + 2 * t) = make_float2(o[i][0], o[i][1]);
         *reinterpret_cast<float2*>(ob + i * 8 + 2 * t) = make_float2(o[i][2], o[i][3]);
