@@ -288,7 +288,8 @@ class Stage:
     def window_attention(self, L: int, rows: RowBatch, qBuf: GpuBuffer, out: GpuBuffer | None = None, window: int = 0,
                          sinks: int = 0) -> GpuBuffer:
         """Every row of a batch, at slot p = T0 + j, over its sequence's slots s <= p with
-        s > p - window or s < sinks (window 0: all). The rows' own K/V come before, by append_rows."""
+        s > p - window or s < sinks (window 0: all). The rows' own K/V come before, by append_rows.
+        Without `out` the result is a new buffer, for which a stream under capture has no room."""
         return _rows_attention(self.lib.dllm_stage_window_attention, self, L, rows, qBuf, out, window, sinks, "window_attention")
 
     def close(self):

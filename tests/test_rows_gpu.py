@@ -581,3 +581,107 @@ def test_a_conversation(dllm):
             stage.set_t0(s, len(held[s][0]))
             cache.set_t0(s, len(held[s][0]))
     ctx.close()
+
+
+# ---- where a rule or a limit changes hands ---------------------------------------------------------
+@pytest.mark.parametrize("scale", [1.0, 1.5, 2.0 ** -100, 2.0 ** -130, 2.0 ** 100, 1.9921875])
+def test_cache4_codes_next_to_a_half(dllm, scale):
+    """Values at, just below and just above the middle between two codes: the code is that of the
+    quotient in fp32, ties to even, whatever the scale (a product with its inverse would be off, or
+    infinite for the smallest)."""
+    ctx = make_ctx(dllm, 4, 2, 64, max_pos=64)
+    cache, rows = dllm.Cache4(ctx, 0, 1), ctx.rowBatch([6])
+    half = np.float32(scale) * (np.arange(15, dtype=np.float32) + np.float32(0.5))
+    up, down = np.nextafter(half, np.float32(np.inf)), np.nextafter(half, np.float32(0))
+    group = lambda x: np.concatenate([x, [0, 15 * scale], np.float32(scale) * np.arange(15)]).astype(np.float32)  # noqa: E731
+    x = np.stack([group(g) for g in (half, up, down, -half + 15 * np.float32(scale))] * 6).reshape(6, 2, 64)
+    z = x.reshape(6, 2, 2, 32)
+    # the smallest value is 0 in each group, and fifteen scales are 15 * scale exactly
+    want = (np.rint(z / np.float32(scale)).clip(0, 15) * np.float64(np.float32(scale))).astype(np.float32).reshape(x.shape)
+    k, v = ctx.createF32(x.size), ctx.createF32(x.size)
+    cache.append(0, rows, f32(ctx, x), f32(ctx, x[::-1]))
+    cache.read_rows(0, rows, k, v)
+    assert np.array_equal(ctx.readF32(k, k.n).reshape(x.shape), want)
+    assert np.array_equal(ctx.readF32(v, v.n).reshape(x.shape), want[::-1])
+    ctx.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("m", [7, 8, 9, 16, 17, 32, 33, 64, 65, 128, 129, 256, 257])
+def test_window_attention_around_tile_sizes(dllm, kind, hd, m):
+    R = Rows(dllm, 2, 2, hd, kind, [210], [m])
+    check_attention(R)
+    check_attention(R, 100, 3)
+    R.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_window_attention_mixed_lengths(dllm, kind):
+    """Short, middling and long rows in one batch, out of order and with an idle sequence between."""
+    R = Rows(dllm, 10, 2, 64, kind, [700, 0, 1500, 31, 40, 64, 2000], [1, 150, 7, 0, 13, 64, 300], seqs=[5, 2, 0, 1, 6, 3, 8])
+    check_attention(R)
+    check_attention(R, 333, 40)
+    R.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_long_chunks_in_graphs(dllm, kind):
+    """A long chunk captured and replayed with other inputs; a longer one cannot be captured before
+    its scratch is there, and the first graph keeps its own when it is."""
+    torch = torch_()
+    R = Rows(dllm, 6, 2, 128, kind, [100, 20], [90, 1], max_pos=4000)
+    ctx, rng = R.ctx, np.random.default_rng(0)
+    q, out = ctx.createF32(91 * 768), ctx.createF32(91 * 768)
+    inputs = [rng.standard_normal(91 * 768).astype(np.float32) for _ in range(3)]
+    want = []
+    for x in inputs:
+        ctx.writeF32(q, x)
+        R.attend(q, 80, 2, out=out)
+        want.append(ctx.readF32(out, out.n))
+    many = ctx.rowBatch([3000], [0])
+    big, far = ctx.createF32(3000 * 768), ctx.createF32(3000 * 768)
+    ctx.synchronize()
+    stream = torch.cuda.Stream()
+    ctx.set_stream(stream.cuda_stream)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        R.attend(q, 80, 2, out=out)
+        with pytest.raises(dllm.DllmError):
+            R.attend(big, rows=many, out=far)
+    replay = lambda x: (ctx.writeF32(q, x), g.replay(), ctx.readF32(out, out.n))[2]  # noqa: E731
+    for round_ in range(2):
+        for x, w in zip(inputs, want):
+            with torch.cuda.stream(stream):
+                assert np.array_equal(replay(x), w)
+        if round_ == 0:  # the longer chunk, outside: more scratch, and slots behind those of the graph
+            R.cache.set_t0(0, 190)
+            R.append(ctx.rowBatch([2810], [0]), *(f32(ctx, np.zeros(2810 * 256)) for _ in range(2)))
+            R.cache.set_t0(0, 0)
+            R.attend(big, rows=many, out=far)
+            ctx.synchronize()
+    ctx.set_stream(None)
+    del g
+    R.close()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "4"])
+@pytest.mark.parametrize("m", [1, 9, 70])
+def test_rows_of_a_cache_beyond_32_bits(dllm, kind, m):
+    """The last slots of the last of 9 sequences of 2^20 slots: their offsets, in elements or bytes, do
+    not fit 32 bits."""
+    torch = torch_()
+    far, kvh, hd, seen = 1 << 20, 8, 128, 300
+    ctx = make_ctx(dllm, 8, kvh, hd, max_pos=far, max_seqs=9, kv_dtype="bf16", kv_page_size=256)
+    R = object.__new__(Rows)
+    R.ctx, R.kind, R.nq, R.kvh, R.hd, R.layer = ctx, kind, 8, kvh, hd, 0
+    R.cache = dllm.Cache4(ctx, 0, 1) if kind == "4" else dllm.Stage(ctx, 0, 1)
+    rng = np.random.default_rng(m)
+    kv = [rng.standard_normal((seen, kvh, hd)).astype(np.float32) for _ in range(2)]
+    R.cache.set_t0(8, far - seen)
+    R.append(ctx.rowBatch([seen], [8]), *(f32(ctx, x) for x in kv))
+    R.cache.set_t0(8, far - m)
+    R.rows, R.lens, R.counts = ctx.rowBatch([m], [8]), [seen - m], [m]
+    R.values = [[torch.from_numpy(R.held(x)).cuda() for x in kv]]
+    check_attention(R, window=200)  # the slots before the last 300 are outside of it
+    R.close()
