@@ -38,6 +38,31 @@ DLLM_DEV unsigned long long global_timer_ns() {
   return t;
 }
 
+// ---- kernels that start while the one before them ends ------------------------------
+// The next such kernel on the stream may start; this one goes on when the grid before it has
+// ended and its stores are visible. Called before the first access of global memory. (Five rows stored
+// in 4 bits and read back: 11.3 us with plain launches, 9.2 so.)
+DLLM_DEV void launch_next_and_wait() {
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// A launch that need not wait for the end of the kernel before: the kernel does, by
+// launch_next_and_wait or where it comes to need it.
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 // ---- bf16 bit helpers (weights.js:153-164: f32 bits = bf16 bits << 16) --------
 DLLM_DEV float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
 DLLM_DEV float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }

@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(kThreads)
     rows_append_kernel(const __grid_constant__ RowsBatch b, unsigned total, RowPages p, const float* k, const float* v,
                        void* kc, void* vc, uint32_t* ks, uint32_t* vs) {
   constexpr int C = HD / 8;
+  launch_next_and_wait();
   const unsigned i = blockIdx.x * kThreads + threadIdx.x, at = min(i, total - 1);  // whole warps take part in the shuffles
   const size_t src = first4(at);
   const float4 *k4 = reinterpret_cast<const float4*>(k) + src, *v4 = reinterpret_cast<const float4*>(v) + src;
@@ -138,6 +139,7 @@ __global__ void __launch_bounds__(kThreads)
     rows_read4_kernel(const __grid_constant__ RowsBatch b, unsigned total, RowPages p, const uint32_t* kc,
                       const uint32_t* vc, const uint32_t* ks, const uint32_t* vs, float* k, float* v) {
   constexpr int C = HD / 8;
+  launch_next_and_wait();
   const unsigned i = blockIdx.x * kThreads + threadIdx.x, at = min(i, total - 1);
   const size_t src = cache_row<HD>(b, p, at), dst = first4(at);
   const unsigned j = at % 4, group = at % C / 4;
@@ -166,9 +168,8 @@ template <int KIND>
 cudaError_t append(const RowsBatch& b, int n, const RowPages& p, int hd, const float* k, const float* v, void* kc, void* vc,
                    uint32_t* ks, uint32_t* vs, cudaStream_t st) {
   const unsigned units = units_of(n, p.kvh, hd), grid = grid_of(units);
-  if (hd == 64) rows_append_kernel<KIND, 64><<<grid, kThreads, 0, st>>>(b, units, p, k, v, kc, vc, ks, vs);
-  else rows_append_kernel<KIND, 128><<<grid, kThreads, 0, st>>>(b, units, p, k, v, kc, vc, ks, vs);
-  return cudaGetLastError();
+  const auto kernel = hd == 64 ? rows_append_kernel<KIND, 64> : rows_append_kernel<KIND, 128>;
+  return launch_early(kernel, grid, kThreads, 0, st, b, units, p, k, v, kc, vc, ks, vs);
 }
 
 }  // namespace
@@ -184,9 +185,8 @@ cudaError_t op_rows_read4(const RowsBatch& b, int n, const RowPages& p, int hd, 
                           const uint32_t* ks, const uint32_t* vs, float* k, float* v, cudaStream_t st) {
   const unsigned units = units_of(n, p.kvh, hd), grid = grid_of(units);
   const uint32_t *kw = static_cast<const uint32_t*>(kc), *vw = static_cast<const uint32_t*>(vc);
-  if (hd == 64) rows_read4_kernel<64><<<grid, kThreads, 0, st>>>(b, units, p, kw, vw, ks, vs, k, v);
-  else rows_read4_kernel<128><<<grid, kThreads, 0, st>>>(b, units, p, kw, vw, ks, vs, k, v);
-  return cudaGetLastError();
+  const auto kernel = hd == 64 ? rows_read4_kernel<64> : rows_read4_kernel<128>;
+  return launch_early(kernel, grid, kThreads, 0, st, b, units, p, kw, vw, ks, vs, k, v);
 }
 
 }  // namespace dllm

@@ -186,6 +186,7 @@ __global__ void __launch_bounds__(kNormRopeThreads) norm_rope_kernel(const NormR
   const int h_first = (blockIdx.y << log2_side) + (slot & ((1 << log2_side) - 1)), h_step = gridDim.y << log2_side;
   const int row = blockIdx.x * (slots >> log2_side) + (slot >> log2_side);
   if (row >= a.n) return;  // a head's threads leave together
+  launch_next_and_wait();
   const unsigned group = (lanes == 32 ? 0xffffffffu : (1u << (lanes & 31)) - 1) << (threadIdx.x % 32 - lane);
   // float offsets of this thread's packs within a head
   int o1[U], o2[U];
@@ -259,8 +260,7 @@ cudaError_t launch_norm_rope(const NormRopeArgs& n, int sms, cudaStream_t st) {
   const int rows = slots >> log2_side, chunks = (heads + (1 << log2_side) - 1) >> log2_side;
   const int ctas = (a.n + rows - 1) / rows;
   const dim3 grid(ctas, (long long)ctas * chunks <= 8ll * sms ? chunks : 1);  // as above
-  norm_rope_kernel<HD, VEC, INTER><<<grid, kNormRopeThreads, 0, st>>>(n, log2_side);
-  return cudaGetLastError();
+  return launch_early(norm_rope_kernel<HD, VEC, INTER>, grid, kNormRopeThreads, 0, st, n, log2_side);
 }
 
 template <int HD>

@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
   constexpr int NG = HD / kGroup4;  // 4-bit rows: groups
   extern __shared__ __align__(1024) unsigned char smem[];
   const RowsAttnArgs& a = P.a;
-  asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled; it waits for this grid's end
+  launch_next_and_wait();
   const int window = a.window, sinks = a.sinks;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int wr = N8 ? 0 : warp % (N8 ? 1 : WR), ws = N8 ? warp : warp / (N8 ? 1 : WR);
@@ -905,7 +905,7 @@ __global__ void __launch_bounds__(kThreads) rows_join_kernel(const __grid_consta
   const int live = k.R - k.r0 - row0;  // rows from row0 on
   // the tile is the first segment of every CTA but the first one, and of that one if it began there
   const bool later = P.begin_tile[c0] != P.split_tile[split];
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the segments' grid has ended and its stores are visible
+  launch_next_and_wait();
   float m[J], l[J], acc[J][V];
 #pragma unroll
   for (int j = 0; j < J; ++j) {
@@ -1011,9 +1011,8 @@ cudaError_t launch(const RowsAttnArgs& a, const RowsBatch& b, int sms, int* laun
   using T = Tile<KIND, HD, WR>;
   RowsKernelArgs P;
   const RowsPlan plan = rows_plan(a, b, T::RT, T::BN, sms * T::kCtas, 1, 2, &P);
-  rows_attn_kernel<KIND, HD, WR><<<plan.ctas, kThreads, T::kSmem, st>>>(P);
+  const cudaError_t e = launch_early(rows_attn_kernel<KIND, HD, WR>, plan.ctas, kThreads, T::kSmem, st, P);
   *launches += 1;
-  const cudaError_t e = cudaGetLastError();
   return e != cudaSuccess ? e : rows_join(P, plan, T::RT, T::BN, HD, launches, st);
 }
 
@@ -1135,16 +1134,7 @@ RowsPlan rows_plan(const RowsAttnArgs& a, const RowsBatch& b, int rt, int bn, in
 
 template <int HD, int W, int J>
 cudaError_t launch_join(const RowsKernelArgs& P, int splits, int rt, int bn, cudaStream_t st) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(splits * (rt / (8 / W * J)));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, rows_join_kernel<HD, W, J>, P, rt, bn);
+  return launch_early(rows_join_kernel<HD, W, J>, splits * (rt / (8 / W * J)), kThreads, 0, st, P, rt, bn);
 }
 template <int HD>
 cudaError_t join_hd(const RowsKernelArgs& P, const RowsPlan& plan, int rt, int bn, cudaStream_t st) {

@@ -614,17 +614,7 @@ cudaError_t launch(const RowsAttnArgs& a, const RowsBatch& b, int sms, int* laun
   rows_planes_kernel<KIND, HD><<<2 * plan.units, kPlaneThreads, 0, st>>>(P);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(plan.ctas);
-  cfg.blockDim = dim3(kTcThreads);
-  cfg.dynamicSmemBytes = T::kSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, rows_tc_kernel<KIND, HD>, P);
+  e = launch_early(rows_tc_kernel<KIND, HD>, plan.ctas, kTcThreads, T::kSmem, st, P);
   *launches += 2;
   return e != cudaSuccess ? e : rows_join(P, plan, kTcTileRows, T::BN, HD, launches, st);
 }
