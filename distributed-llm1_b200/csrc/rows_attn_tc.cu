@@ -33,7 +33,9 @@ namespace dllm {
 namespace {
 
 // ---- K and V as fp16 planes ------------------------------------------------------------------
-constexpr int kPlaneThreads = 256;
+constexpr int kPlaneEach = 2;  // units of 8 dims per thread (8 and 256 threads per block: 15 us for 400 blocks, 10 so)
+template <int KIND, int HD>
+constexpr int kPlaneThreads = TcTile<KIND, HD>::BN * (HD / 8) / kPlaneEach;
 
 // Eight values of one row, from 8 dims on.
 template <int KIND, int HD>
@@ -55,10 +57,10 @@ DLLM_DEV void load8(const void* rows, const uint32_t* pairs, size_t row, int c, 
 
 // Grid: (KV head, block, K or V) of every sequence in turn.
 template <int KIND, int HD>
-__global__ void __launch_bounds__(kPlaneThreads) rows_planes_kernel(const __grid_constant__ RowsKernelArgs P) {
+__global__ void __launch_bounds__(kPlaneThreads<KIND, HD>) rows_planes_kernel(const __grid_constant__ RowsKernelArgs P) {
   using T = TcTile<KIND, HD>;
-  constexpr int C = HD / 8, kEach = T::BN * C / kPlaneThreads;
-  __shared__ float smax[kPlaneThreads / 32];
+  constexpr int C = HD / 8, kEach = kPlaneEach, kThreads = kPlaneThreads<KIND, HD>;
+  __shared__ float smax[kThreads / 32];
   __shared__ int sbad;
   const RowsAttnArgs& a = P.a;
   asm volatile("griddepcontrol.launch_dependents;");  // the main kernel may start; it waits for this grid's end
@@ -73,7 +75,7 @@ __global__ void __launch_bounds__(kPlaneThreads) rows_planes_kernel(const __grid
   bool bad = false;
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
-    const int j = tid + e * kPlaneThreads, slot = s0 + j / C;
+    const int j = tid + e * kThreads, slot = s0 + j / C;
 #pragma unroll
     for (int u = 0; u < 8; ++u) x[e][u] = 0.f;
     if (slot < end) load8<KIND, HD>(rows, pairs, a.pages.row(P.seq[i], slot, head), j % C, x[e]);
@@ -94,14 +96,14 @@ __global__ void __launch_bounds__(kPlaneThreads) rows_planes_kernel(const __grid
   __syncthreads();
   if (bad) sbad = 1;
 #pragma unroll
-  for (int w = 0; w < kPlaneThreads / 32; ++w) m = fmaxf(m, smax[w]);
+  for (int w = 0; w < kThreads / 32; ++w) m = fmaxf(m, smax[w]);
   // in steps of 2^8, so that neighbouring blocks hardly ever differ
   const int ex = max((int)(__float_as_uint(m) >> 23) | 7, 15);
   const float up = power_of_two(268 - ex);
   unsigned char* image = static_cast<unsigned char*>(a.planes) + (size_t)blockIdx.x * T::kTile;
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
-    const int j = tid + e * kPlaneThreads, row = j / C, c = j % C;
+    const int j = tid + e * kThreads, row = j / C, c = j % C;
     uint32_t h[4], l[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) split2_f16(x[e][2 * u] * up, x[e][2 * u + 1] * up, h[u], l[u]);
@@ -611,7 +613,7 @@ cudaError_t launch(const RowsAttnArgs& a, const RowsBatch& b, int sms, int* laun
   RowsKernelArgs P;
   const RowsPlan plan = rows_plan(a, b, kTcTileRows, T::BN, sms, kTcLeastShare, 2, &P);
   P.a.info = static_cast<char*>(a.planes) + (size_t)plan.units * 2 * T::kTile;
-  rows_planes_kernel<KIND, HD><<<2 * plan.units, kPlaneThreads, 0, st>>>(P);
+  rows_planes_kernel<KIND, HD><<<2 * plan.units, kPlaneThreads<KIND, HD>, 0, st>>>(P);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   e = launch_early(rows_tc_kernel<KIND, HD>, plan.ctas, kTcThreads, T::kSmem, st, P);
