@@ -90,10 +90,11 @@ struct dllm_ctx {
   float* tree_part = nullptr;
   // partial results of split attention of rows, sized for any call; allocated with the first batch
   float* rows_part = nullptr;
-  // fp16 K and V blocks of long chunks. Grown by replacement: captured graphs may still refer to the
-  // earlier ones, which stay until the ctx goes.
+  // fp16 K and V blocks of long chunks. Grown by replacement: earlier ones that captured graphs refer
+  // to stay until the ctx goes.
   std::vector<void*> rows_planes;
   size_t rows_planes_bytes = 0;
+  bool rows_planes_captured = false;  // of the latest
   // token picks: per-row keys, then arrival counters (zero between calls)
   unsigned long long* pick_best = nullptr;
   // freed buffers kept for reuse, by size in bytes
@@ -881,15 +882,36 @@ int rows_attention(dllm_ctx* c, const char* what, dllm::RowsAttnArgs& a, const d
   const size_t need = dllm::rows_attn_planes_bytes(a, b, kind, f.head_dim);
   if (need > c->rows_planes_bytes) {
     if (int rc = refuse_capture(c, "attention of a longer chunk than any call before")) return rc;
-    const size_t bytes = std::max(need, std::min(2 * c->rows_planes_bytes, (size_t)1 << 30));
+    // twice as much as before, so that a growing conversation does not come here with every chunk, up to
+    // what any sequence could need
+    dllm::RowsBatch whole;
+    whole.n_seqs = 1, whole.seq[0] = whole.row0[0] = whole.t0[0] = 0, whole.m[0] = f.max_pos;
+    dllm::RowsAttnArgs all = a;
+    all.window = 0x7fffffff;
+    const size_t most = std::max((size_t)1 << 30, dllm::rows_attn_planes_bytes(all, whole, kind, f.head_dim));
+    size_t bytes = std::max(need, std::min(2 * c->rows_planes_bytes, most));
+    if (!c->rows_planes.empty() && !c->rows_planes_captured) {
+      dev_free(c->rows_planes.back());  // (waits for the GPU)
+      c->rows_planes.pop_back();
+      c->rows_planes_bytes = 0;
+    }
     void* p = nullptr;
-    const cudaError_t e = cudaMalloc(&p, bytes);
+    cudaError_t e = cudaMalloc(&p, bytes);
+    if (e != cudaSuccess && bytes > need) {
+      cudaGetLastError();
+      e = cudaMalloc(&p, bytes = need);
+    }
     if (e != cudaSuccess) {
       cudaGetLastError();
       return set_err(c, DLLM_ENOMEM, "%s: scratch of %zu bytes: %s", what, bytes, cudaGetErrorString(e));
     }
     c->rows_planes.push_back(p);
-    c->rows_planes_bytes = bytes;
+    c->rows_planes_bytes = bytes, c->rows_planes_captured = false;
+  }
+  if (need && !c->rows_planes_captured) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    CK(c, cudaStreamIsCapturing(c->stream, &st));
+    c->rows_planes_captured = st != cudaStreamCaptureStatusNone;
   }
   a.planes = c->rows_planes.empty() ? nullptr : c->rows_planes.back();
   a.planes_bytes = c->rows_planes_bytes;

@@ -685,3 +685,29 @@ def test_rows_of_a_cache_beyond_32_bits(dllm, kind, m):
     R.values = [[torch.from_numpy(R.held(x)).cuda() for x in kv]]
     check_attention(R, window=200)  # the slots before the last 300 are outside of it
     R.close()
+
+
+@pytest.mark.parametrize("kind", ["f32", "4"])
+def test_scratch_of_a_growing_conversation(dllm, kind):
+    """Chunk after chunk the scratch grows by doubling and the one before is given back, so that in the
+    end no more than twice the last chunk's share is held."""
+    torch = torch_()
+    far, chunk = 6000, 200
+    ctx = make_ctx(dllm, 8, 8, 128, max_pos=far, max_seqs=1, kv_dtype="f32")
+    cache = dllm.Cache4(ctx, 0, 1) if kind == "4" else dllm.Stage(ctx, 0, 1)
+    rows, q, out = ctx.rowBatch([chunk]), ctx.createF32(chunk * 1024), ctx.createF32(chunk * 1024)
+    k = ctx.createF32(chunk * 1024)
+    fn = cache.attention if kind == "4" else cache.window_attention
+    append = cache.append if kind == "4" else cache.append_rows
+    ctx.synchronize()
+    before, held = torch.cuda.mem_get_info()[0], []
+    for t in range(0, far, chunk):
+        cache.set_t0(0, t)
+        append(0, rows, k, k)
+        fn(0, rows, q, out)
+        held.append(before - torch.cuda.mem_get_info()[0])
+    share = 8 * 2 * far * 128 * 4  # 4 bytes per K or V value
+    assert share / 2 <= held[-1] <= 2 * share + (64 << 20), (held[-1], share)
+    assert len(set(held)) <= 8
+    assert (ctx.readF32(out, out.n) == 0).all()
+    ctx.close()
