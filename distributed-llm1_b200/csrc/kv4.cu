@@ -11,8 +11,8 @@
 //
 // Memory-bound: 4 bytes in and 5 bits out per value. A thread takes 8 dims of K and of V (four
 // 16-byte loads under way, one word of codes each); the four threads of a group exchange
-// their extremes in two shuffles. 8185 rows of 4 KV heads of 128: stored and read back in 20.6
-// us, 77 MB at 3.8 TB/s (a copy moves 6.6): two launches of 10 us, of which each spends 3 on
+// their extremes in two shuffles. 8185 rows of 4 KV heads of 128: stored and read back in 17.1
+// us, 77 MB at 4.5 TB/s (a copy moves 6.6): two launches of 9 us, of which each spends 3 on
 // one chain of page table, loads and stores. Sixteen dims per thread were slower (31.7 against 27.6
 // us for the pair, before the sectors below were filled).
 

@@ -171,7 +171,7 @@ cudaError_t rope_hd(const RopeAtArgs& a, int sms, cudaStream_t st) {
 // head's HD / 8 threads (a warp, where pairs go one by one) hold it in registers, add their
 // squares in fp32 by shuffles, and turn it. Bound by memory like the rotation alone: the norm
 // adds 4 flops per element and one chain of shuffles, and saves a whole pass over q and k.
-// 6007 rows of 32 heads of 128: 37 us, 197 MB at 5.3 TB/s (a copy moves 6.6). The next head's
+// 6007 rows of 32 heads of 128: 35 us, 197 MB at 5.6 TB/s (a copy moves 6.6). The next head's
 // loads ahead of this one's sum, or the heads of a row over several CTAs, were slower (41, 43):
 // more registers and angles taken twice. The weights are loaded before the sum, so that one row
 // waits for memory once (7.1 -> 6.3 us; CTAs of 256 threads then cost long batches 2 us).

@@ -35,8 +35,8 @@
 // the second terms of q take rows 8 to 15: one product instead of two. A warp copies the slots that it
 // works on itself, without barriers in the loop.
 //
-// What bounds it. 24 sequences of 4000 slots, 2 KV heads of 128, fp32: 44 us, 3.4 TB/s; 64 of 8000 in
-// 4 bits: 62 us, 2 TB/s, where a warp spends 1200 instructions per 32 slots, about as many each on
+// What bounds it. 24 sequences of 4000 slots, 2 KV heads of 128, fp32: 41 us, 3.7 TB/s; 64 of 8000 in
+// 4 bits: 61 us, 2 TB/s, where a warp spends 1200 instructions per 32 slots, about as many each on
 // the integer and the floating-point pipe (unpacking codes, cutting p, scales), and 70 MMAs.
 #include "rows_attn.cuh"
 
@@ -851,8 +851,10 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
           const float(&x)[4] = o[gr * 2];
           const float(&y)[4] = o[gr * 2 + 1];
           const float u = unit[gr], v = u * 0.0625f;
-          *reinterpret_cast<float4*>(oc + d) = make_float4(fmaf(x[0], u, m0), fmaf(x[2], v, m0), fmaf(y[0], u, m0), fmaf(y[2], v, m0));
-          *reinterpret_cast<float4*>(od + d) = make_float4(fmaf(x[1], u, m1), fmaf(x[3], v, m1), fmaf(y[1], u, m1), fmaf(y[3], v, m1));
+          *reinterpret_cast<float4*>(oc + d) =
+              make_float4(fmaf(x[0], u, m0), fmaf(x[2], v, m0), fmaf(y[0], u, m0), fmaf(y[2], v, m0));
+          *reinterpret_cast<float4*>(od + d) =
+              make_float4(fmaf(x[1], u, m1), fmaf(x[3], v, m1), fmaf(y[1], u, m1), fmaf(y[3], v, m1));
         }
       } else {
 #pragma unroll

@@ -24,6 +24,9 @@
 // registers. With two planes S takes q_high (K_high | K_low) as one MMA of N = 128, and
 // q_low K_high goes to the K_low half; the softmax adds the halves.
 // Tensor memory: S and P of both tiles 2 x 128 columns, O 2 x 128.
+// What bounds it: the products and, between them, the softmax. A chunk of 2048 rows of 28 heads of 128
+// under a 4096-token window, bf16: 216 us in the main kernel, 557 TFLOP/s of the floor's one product
+// per operand, tensor pipe 62 % busy; over 8148 4-bit slots 480 us, 436 TFLOP/s, 67 %.
 // The main kernel starts while the planes are written (its CTAs set up and bring q), and waits for
 // that grid's end before it reads them (a prompt of 1501 rows: 47 -> 43 us with its launches).
 #include "rows_attn_tc.cuh"
@@ -424,8 +427,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
         auto most = [&](const uint32_t(&u)[32]) {
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
-            x = max3(x, __uint_as_float(u[e]), __uint_as_float(u[e + 1])), x1 = max3(x1, __uint_as_float(u[e + 2]), __uint_as_float(u[e + 3]));
-            x2 = max3(x2, __uint_as_float(u[e + 4]), __uint_as_float(u[e + 5])), x3 = max3(x3, __uint_as_float(u[e + 6]), __uint_as_float(u[e + 7]));
+            x = max3(x, __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
+            x1 = max3(x1, __uint_as_float(u[e + 2]), __uint_as_float(u[e + 3]));
+            x2 = max3(x2, __uint_as_float(u[e + 4]), __uint_as_float(u[e + 5]));
+            x3 = max3(x3, __uint_as_float(u[e + 6]), __uint_as_float(u[e + 7]));
           }
         };
         // bit e: column c + e is visible (no branches: they would part the rows of a warp)
