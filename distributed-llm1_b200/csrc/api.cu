@@ -90,11 +90,14 @@ struct dllm_ctx {
   float* tree_part = nullptr;
   // partial results of split attention of rows, sized for any call; allocated with the first batch
   float* rows_part = nullptr;
-  // fp16 K and V blocks of long chunks. Grown by replacement: earlier ones that captured graphs refer
-  // to stay until the ctx goes.
-  std::vector<void*> rows_planes;
-  size_t rows_planes_bytes = 0;
-  bool rows_planes_captured = false;  // of the latest
+  // fp16 K and V blocks of long chunks, in the last of these. Grown by replacement: earlier ones that
+  // captured graphs refer to stay until the ctx goes, and serve again when there is no memory for more.
+  struct RowsPlanes {
+    void* ptr;
+    size_t bytes;
+    bool captured;
+  };
+  std::vector<RowsPlanes> rows_planes;
   // token picks: per-row keys, then arrival counters (zero between calls)
   unsigned long long* pick_best = nullptr;
   // freed buffers kept for reuse, by size in bytes
@@ -880,7 +883,7 @@ int rows_attention(dllm_ctx* c, const char* what, dllm::RowsAttnArgs& a, const d
   a.part_o = c->rows_part;
   a.part_ml = c->rows_part + dllm::rows_attn_part_rows(c->sms) * f.head_dim;
   const size_t need = dllm::rows_attn_planes_bytes(a, b, kind, f.head_dim);
-  if (need > c->rows_planes_bytes) {
+  if (c->rows_planes.empty() ? need > 0 : need > c->rows_planes.back().bytes) {
     if (int rc = refuse_capture(c, "attention of a longer chunk than any call before")) return rc;
     // twice as much as before, so that a growing conversation does not come here with every chunk, up to
     // what any sequence could need
@@ -889,11 +892,11 @@ int rows_attention(dllm_ctx* c, const char* what, dllm::RowsAttnArgs& a, const d
     dllm::RowsAttnArgs all = a;
     all.window = 0x7fffffff;
     const size_t most = std::max((size_t)1 << 30, dllm::rows_attn_planes_bytes(all, whole, kind, f.head_dim));
-    size_t bytes = std::max(need, std::min(2 * c->rows_planes_bytes, most));
-    if (!c->rows_planes.empty() && !c->rows_planes_captured) {
-      dev_free(c->rows_planes.back());  // (waits for the GPU)
+    const size_t before = c->rows_planes.empty() ? 0 : c->rows_planes.back().bytes;
+    size_t bytes = std::max(need, std::min(2 * before, most));
+    if (before && !c->rows_planes.back().captured) {
+      dev_free(c->rows_planes.back().ptr);  // (waits for the GPU)
       c->rows_planes.pop_back();
-      c->rows_planes_bytes = 0;
     }
     void* p = nullptr;
     cudaError_t e = cudaMalloc(&p, bytes);
@@ -905,16 +908,18 @@ int rows_attention(dllm_ctx* c, const char* what, dllm::RowsAttnArgs& a, const d
       cudaGetLastError();
       return set_err(c, DLLM_ENOMEM, "%s: scratch of %zu bytes: %s", what, bytes, cudaGetErrorString(e));
     }
-    c->rows_planes.push_back(p);
-    c->rows_planes_bytes = bytes, c->rows_planes_captured = false;
+    c->rows_planes.push_back({p, bytes, false});
   }
-  if (need && !c->rows_planes_captured) {
-    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-    CK(c, cudaStreamIsCapturing(c->stream, &st));
-    c->rows_planes_captured = st != cudaStreamCaptureStatusNone;
+  if (need) {
+    dllm_ctx::RowsPlanes& planes = c->rows_planes.back();
+    if (!planes.captured) {
+      cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+      CK(c, cudaStreamIsCapturing(c->stream, &st));
+      planes.captured = st != cudaStreamCaptureStatusNone;
+    }
+    a.planes = planes.ptr;
+    a.planes_bytes = planes.bytes;
   }
-  a.planes = c->rows_planes.empty() ? nullptr : c->rows_planes.back();
-  a.planes_bytes = c->rows_planes_bytes;
   int launches = 0;
   const cudaError_t e = dllm::op_rows_attention(a, b, kind, f.head_dim, c->sms, &launches, c->stream);
   c->launches += launches;
@@ -1065,7 +1070,7 @@ void ctx_free(dllm_ctx* c) {
   dev_free(c->tc_scratch);
   dev_free(c->tree_part);
   dev_free(c->rows_part);
-  for (void* p : c->rows_planes) dev_free(p);
+  for (const auto& p : c->rows_planes) dev_free(p.ptr);
   dev_free(c->pick_best);
   for (auto& kv : c->buf_cache) cudaFree(kv.second);
   c->buf_cache.clear();

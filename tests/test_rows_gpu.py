@@ -711,3 +711,56 @@ def test_scratch_of_a_growing_conversation(dllm, kind):
     assert len(set(held)) <= 8
     assert (ctx.readF32(out, out.n) == 0).all()
     ctx.close()
+
+
+def test_captured_scratch_outlives_a_failed_growth(dllm):
+    """A chunk captured, a longer one outside, a still longer one that finds no memory, then any chunk:
+    the scratch that the graph refers to is still its own."""
+    torch = torch_()
+    R = Rows(dllm, 8, 8, 128, "f32", [1000], [90], max_pos=70000)
+    ctx, rng = R.ctx, np.random.default_rng(0)
+    q, out, other = (ctx.createF32(90 * 1024) for _ in range(3))
+    inputs = [rng.standard_normal(90 * 1024).astype(np.float32) for _ in range(2)]
+    want = []
+    for x in inputs:
+        ctx.writeF32(q, x)
+        R.attend(q, out=out)
+        want.append(ctx.readF32(out, out.n))
+    ctx.synchronize()
+    stream = torch.cuda.Stream()
+    ctx.set_stream(stream.cuda_stream)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        R.attend(q, out=out)
+
+    def chunk_at(t0):
+        R.cache.set_t0(0, t0)
+        R.attend(q, out=other)
+        ctx.synchronize()
+
+    def check_replays():
+        for x, w in zip(inputs, want):
+            ctx.writeF32(q, x)
+            with torch.cuda.stream(stream):
+                g.replay()
+            assert np.array_equal(ctx.readF32(out, out.n), w)
+    chunk_at(3000)
+    check_replays()
+    held = []  # most of the card: less is left than the chunk at 60000 needs (8 x 2 x 60090 x 128 values of 4 bytes, 492 MB)
+    for size in (16 << 30, 1 << 30, 64 << 20):
+        while torch.cuda.mem_get_info()[0] > size + (200 << 20):
+            held.append(torch.empty(size, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(dllm.DllmError) as e:
+        chunk_at(60000)
+    assert e.value.status == dllm._lib.DLLM_ENOMEM
+    free = torch.cuda.mem_get_info()[0]
+    chunk_at(200)
+    assert torch.cuda.mem_get_info()[0] <= free  # nothing was given back
+    check_replays()
+    held.clear()
+    torch.cuda.empty_cache()
+    chunk_at(60000)
+    check_replays()
+    ctx.set_stream(None)
+    del g
+    R.close()
