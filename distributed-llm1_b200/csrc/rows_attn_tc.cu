@@ -503,8 +503,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
           tmem_ld_wait();
 #pragma unroll
           for (int e = 0; e < kStep; ++e) {
-            y[e] = fmaf(__uint_as_float(ua[e]), f, shift);
-            if constexpr (T::kPlanes == 2) y[e] = fmaf(__uint_as_float(ua[16 + e]), f, y[e]);
+            // the same sum as above: f is a power of two, so the largest score's p is 2^8 at any size of it
+            float u = __uint_as_float(ua[e]);
+            if constexpr (T::kPlanes == 2) u += __uint_as_float(ua[16 + e]);
+            y[e] = fmaf(u, f, shift);
           }
           if (i < 3) fetch(i + 1);
           if (__builtin_expect(edge, 0)) {

@@ -764,3 +764,35 @@ def test_captured_scratch_outlives_a_failed_growth(dllm):
     ctx.set_stream(None)
     del g
     R.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m", [1, 20, 90, 300])
+@pytest.mark.parametrize("size", [2.0 ** 16, 2.0 ** 40, 2.0 ** 100])
+def test_window_attention_of_huge_scores(dllm, kind, m, size):
+    """Scores far beyond a softmax's range, equal or further apart than that: the largest share the row,
+    and nothing overflows."""
+    torch = torch_()
+
+    def edit(_, kv):  # 4-bit codes with nothing to round
+        kv[0][:] = np.random.default_rng(1).integers(0, 16, kv[0].shape)
+        kv[0][..., ::32], kv[0][..., 1::32] = 0, 15
+    R = Rows(dllm, 8, 2, 128, kind, [500], [m], edit=edit)
+    # elements of one size: a score is a whole multiple of it, so two are equal or size * log2(e) / sqrt(128) >=
+    # 2^13 apart, while fp32 takes at most 22 steps of 2^-23 of 128 * 15 * size * 0.13 from them, a hundredth
+    # of that: p is 0 but for the slots with the largest score, and the row a mean of these slots' V in some
+    # proportion (their scores are equal but for that rounding, which is more than 1)
+    q = np.random.default_rng(2).choice([-size, size], (m, 8, 128)).astype(np.float32)
+    k, v = R.values[0]
+    slot, at = torch.arange(500, 500 + m, device="cuda")[:, None], torch.arange(500 + m, device="cuda")
+    for window, sinks in ((0, 0), (70, 6)):
+        out = R.attend(f32(R.ctx, q), window, sinks)
+        got = torch.from_numpy(R.ctx.readF32(out, out.n).reshape(m, 8, 128)).cuda().double()
+        see = (at <= slot) & ((at > slot - window) | (at < sinks) if window else at >= 0)
+        for h in range(8):
+            z = torch.where(see, torch.from_numpy(q[:, h]).cuda().double() @ k[:, h // 4].T, -math.inf)
+            best, vv = (z == z.amax(-1, keepdim=True))[..., None], v[None, :, h // 4]
+            low, high = torch.where(best, vv, math.inf).amin(1), torch.where(best, vv, -math.inf).amax(1)
+            room = vv.abs().max() * 2.0 ** -18  # V is to 22 bits; a few sums and a quotient
+            assert ((got[:, h] >= low - room) & (got[:, h] <= high + room)).all(), (window, h)
+    R.close()
