@@ -475,14 +475,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
         }
         x = fmaxf(max3(x, x1, x2), x3) * f;
         // p is 2^(x - m + 8) with scores x up to m + 7: m is the row's maximum at a time, and moves (with
-        // l and o) only when a score exceeds that.
-        if (__any_sync(0xffffffffu, x > m + 7.f)) {
+        // l and o) only when a score exceeds that. (m + 7 could round up, and p then leave fp16's range.)
+        if (__any_sync(0xffffffffu, x - m > 7.f)) {
           const float to = fmaxf(m, x), g = to == -INFINITY ? 1.f : ex2(m - to);
           m = to, l *= g;
 #pragma unroll
           for (int d = 0; d < HD; ++d) o[d] *= g;
         }
-        const float shift = 8.f - (m == -INFINITY ? 0.f : m);
+        const float base = m == -INFINITY ? 0.f : m;
+        const float shift = 8.f - base + base > 8.f ? -base : 8.f - base;  // (8 - m may round to 16 - m)
         // ---- p over the scores, 32 columns of tensor memory at a time (32 scores, or 16 and their
         // second parts): while the exponentials of some are under way, the next ones land. A loop, not
         // unrolled: the code of both groups has to stay in the instruction cache. (And no decision inside:

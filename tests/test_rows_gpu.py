@@ -796,3 +796,43 @@ def test_window_attention_of_huge_scores(dllm, kind, m, size):
             room = vv.abs().max() * 2.0 ** -18  # V is to 22 bits; a few sums and a quotient
             assert ((got[:, h] >= low - room) & (got[:, h] <= high + room)).all(), (window, h)
     R.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m", [1, 5, 20, 90, 300])
+@pytest.mark.parametrize("step", [4.0, 8.0, 9.0])
+def test_large_scores_that_grow_by_little(dllm, kind, m, step):
+    """Scores of 2^22 to 2^29 where each block of slots exceeds the one before by a step or two of fp32, or
+    less: whatever the rounding leaves of their differences, a row is a mean of V."""
+    torch = torch_()
+
+    def edit(_, kv):
+        kv[0][:] = 0
+        kv[0][..., 0] = 1
+        kv[0][..., 32] = np.arange(len(kv[0]))[:, None] // 64
+    R = Rows(dllm, 8, 2, 128, kind, [3000], [m], edit=edit)
+    unit = math.sqrt(128) / math.log2(math.e)  # of a score in powers of two
+    for base in [2.0 ** (22 + i / 2) for i in range(14)]:
+        for sign in (1, -1):
+            q = np.zeros((m, 8, 128), np.float32)
+            q[..., 0], q[..., 32] = sign * base * unit * (1 + np.arange(8) / 16), step * unit
+            out = R.attend(f32(R.ctx, q))
+            got = R.ctx.readF32(out, out.n).reshape(m, 8, 128)
+            v = R.values[0][1]
+            low, high = (torch.repeat_interleave(f(0), 4, 0).cpu().numpy() for f in (v.amin, v.amax))
+            assert ((got >= low - 1e-4) & (got <= high + 1e-4)).all(), (base, sign)
+    R.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m", [90, 300])
+def test_scores_where_eight_rounds_away(dllm, kind, m):
+    """Maxima between 2^27 and 2^28, where 8 is half a step of fp32."""
+    R = Rows(dllm, 8, 2, 128, kind, [300], [m])
+    rng = np.random.default_rng(4)
+    for size in (2.0 ** 23, 2.0 ** 24, 2.0 ** 25, 2.0 ** 26):
+        q = (rng.standard_normal((m, 8, 128)) * size).astype(np.float32)
+        out = R.attend(f32(R.ctx, q))
+        got, high = R.ctx.readF32(out, out.n), float(R.values[0][1].abs().max())
+        assert (np.abs(got) <= high * (1 + 1e-5)).all(), size
+    R.close()
