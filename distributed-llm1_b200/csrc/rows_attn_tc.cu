@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
           for (int d = 0; d < HD; ++d) o[d] *= g;
         }
         const float base = m == -INFINITY ? 0.f : m;
-        const float shift = 8.f - base + base > 8.f ? -base : 8.f - base;  // (8 - m may round to 16 - m)
+        const float shift = 8.f - base + base > 15.f ? -base : 8.f - base;  // (8 - m may round to 16 - m)
         // ---- p over the scores, 32 columns of tensor memory at a time (32 scores, or 16 and their
         // second parts): while the exponentials of some are under way, the next ones land. A loop, not
         // unrolled: the code of both groups has to stay in the instruction cache. (And no decision inside:
