@@ -1024,12 +1024,10 @@ cudaError_t launch(const RowsAttnArgs& a, const RowsBatch& b, int sms, int* laun
 // slow type here: 121 us for 28 rows, 203 against 133 for 35.
 bool is_long(const RowsAttnArgs& a, int m, int kind) { return m * (a.nq / a.pages.kvh) > (kind == kKvF32 ? 32 : 64); }
 
-// Scratch of one sequence's fp16 blocks: the blocks and their factors.
+// (KV head, block) pairs of one sequence.
 size_t planes_units(const RowsAttnArgs& a, const RowsBatch& b, int i, int kind) {
   return (size_t)a.pages.kvh * RowsView(b.t0[i], b.t0[i] + b.m[i] - 1, a.window, a.sinks, tc_block(kind)).nb;
 }
-constexpr size_t unit_bytes(int hd) { return (size_t)2 * 128 * 2 * hd + 16; }
-
 void add(RowsBatch& to, const RowsBatch& b, int i) {
   const int k = to.n_seqs++;
   to.seq[k] = b.seq[i], to.row0[k] = b.row0[i], to.m[k] = b.m[i], to.t0[k] = b.t0[i];
@@ -1062,8 +1060,8 @@ cudaError_t launch_kind(const RowsAttnArgs& a, const RowsBatch& b, int sms, int*
   for (int i = 0; e == cudaSuccess && i < b.n_seqs; ++i) {
     if (!is_long(a, b.m[i], KIND)) continue;
     const size_t u = planes_units(a, b, i, KIND);
-    if (u * unit_bytes(HD) > a.planes_bytes) return cudaErrorInvalidValue;
-    if ((units + u) * unit_bytes(HD) > a.planes_bytes) {
+    if (u * tc_unit_bytes(HD) > a.planes_bytes) return cudaErrorInvalidValue;
+    if ((units + u) * tc_unit_bytes(HD) > a.planes_bytes) {
       e = launch_rows_tc(a, many, KIND, HD, sms, launches, st);
       many.n_seqs = 0, units = 0;
     }
@@ -1157,7 +1155,7 @@ size_t rows_attn_planes_bytes(const RowsAttnArgs& a, const RowsBatch& b, int kin
   size_t all = 0, most = 0;
   for (int i = 0; i < b.n_seqs; ++i) {
     if (!is_long(a, b.m[i], kind)) continue;
-    const size_t n = planes_units(a, b, i, kind) * unit_bytes(hd);
+    const size_t n = planes_units(a, b, i, kind) * tc_unit_bytes(hd);
     all += n, most = std::max(most, n);
   }
   return std::max(most, std::min(all, (size_t)1 << 30));

@@ -58,7 +58,8 @@ struct RowsAttnArgs {
   int* err;
   void* planes;              // scratch for the K and V blocks of long chunks in fp16 (rows_attn_tc.cu)
   size_t planes_bytes;
-  void* info;                // in it: the blocks' factors (set by op_rows_attention)
+  unsigned char* exps;       // in it: exponents of the powers of two per slot (set by op_rows_attention),
+  uint16_t* info;            // and the blocks' exponents and flags
   float* part_o;             // [rows][hd] partial outputs of sequences that are split
   float* part_ml;            // [rows][2]
 };

@@ -5,8 +5,11 @@
 // rows_planes_kernel brings the K and V rows that a sequence's rows see into fp16 once, before
 // the many tiles that read them: per (KV head, block of slots) one power of two takes the
 // largest value below 2^15, and a value becomes one fp16 (bf16 caches: 8 significant bits fit)
-// or two (fp32 and 4-bit caches: 22 bits). What falls below fp16's range is 2^-32 of the
-// block's largest value at most. A block is written as the image that shared memory needs:
+// or two (fp32 and 4-bit caches), which keep 22 bits of the largest value of every slot. Where
+// some slot of a block lies too far below another for that ("wide" blocks), each slot has a power of
+// two of its own: a large value in a slot that a row does not see takes no bits from those that it sees.
+// The softmax then multiplies the scores by K's powers, and brings V's into p, relative to the largest
+// of the slots that the row sees. A block is written as the image that shared memory needs:
 // 128 rows (128 slots, or 64 slots and their second terms) in swizzled boxes of 64 dims, so
 // the main kernel fetches it with one bulk copy and knows no page table.
 //
@@ -40,6 +43,10 @@ constexpr int kPlaneEach = 2;  // units of 8 dims per thread (8 and 256 threads 
 template <int KIND, int HD>
 constexpr int kPlaneThreads = TcTile<KIND, HD>::BN * (HD / 8) / kPlaneEach;
 
+// What the main kernel is told of a block's K or V, 16 bits: the exponent of its power of two, whether it
+// had values that are no numbers, whether it has powers per slot.
+constexpr uint32_t kTcBad = 1u << 8, kTcWide = 1u << 9;
+
 // Eight values of one row, from 8 dims on.
 template <int KIND, int HD>
 DLLM_DEV void load8(const void* rows, const uint32_t* pairs, size_t row, int c, float (&x)[8]) {
@@ -60,10 +67,10 @@ DLLM_DEV void load8(const void* rows, const uint32_t* pairs, size_t row, int c, 
 
 // Grid: (KV head, block, K or V) of every sequence in turn.
 template <int KIND, int HD>
-__global__ void __launch_bounds__(kPlaneThreads<KIND, HD>) rows_planes_kernel(const __grid_constant__ RowsKernelArgs P) {
+__global__ void __launch_bounds__(kPlaneThreads<KIND, HD>, 2048 / kPlaneThreads<KIND, HD>) rows_planes_kernel(const __grid_constant__ RowsKernelArgs P) {
   using T = TcTile<KIND, HD>;
   constexpr int C = HD / 8, kEach = kPlaneEach, kThreads = kPlaneThreads<KIND, HD>;
-  __shared__ float smax[kThreads / 32];
+  __shared__ uint32_t smost[kThreads / 32], sleast[kThreads / 32];
   __shared__ int sbad;
   const RowsAttnArgs& a = P.a;
   asm volatile("griddepcontrol.launch_dependents;");  // the main kernel may start; it waits for this grid's end
@@ -74,7 +81,8 @@ __global__ void __launch_bounds__(kPlaneThreads<KIND, HD>) rows_planes_kernel(co
   const void* rows = which ? a.vc : a.kc;
   const uint32_t* pairs = which ? a.vs : a.ks;
   if (tid == 0) sbad = 0;
-  float x[kEach][8], m = 0.f;
+  float x[kEach][8];
+  uint32_t m[kEach];
   bool bad = false;
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
@@ -83,42 +91,53 @@ __global__ void __launch_bounds__(kPlaneThreads<KIND, HD>) rows_planes_kernel(co
     for (int u = 0; u < 8; ++u) x[e][u] = 0.f;
     if (slot < end) load8<KIND, HD>(rows, pairs, a.pages.row(P.seq[i], slot, head), j % C, x[e]);
   }
+  // the largest magnitude of each slot (C lanes side by side), and of the block's slots the most and
+  // the least that is not zero: positive numbers in the order of their bits
+  uint32_t most = 0u, least = ~0u;
 #pragma unroll
-  for (int e = 0; e < kEach; ++e)
+  for (int e = 0; e < kEach; ++e) {
+    m[e] = 0u;
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const bool fine = is_finite(x[e][u]);
-      m = fmaxf(m, fine ? fabsf(x[e][u]) : 0.f);
+      m[e] = max(m[e], fine ? __float_as_uint(fabsf(x[e][u])) : 0u);
       bad |= !fine;
       // 0 x NaN would reach rows that do not see the slot; the main kernel adds such values of V
       // to the rows that do
       if (which && !fine) x[e][u] = 0.f;
     }
-  m = warp_max(m);
-  if (tid % 32 == 0) smax[tid / 32] = m;
+#pragma unroll
+    for (int d = C / 2; d > 0; d >>= 1) m[e] = max(m[e], __shfl_xor_sync(0xffffffffu, m[e], d));
+    most = max(most, m[e]), least = min(least, m[e] ? m[e] : ~0u);
+  }
+  most = __reduce_max_sync(0xffffffffu, most), least = __reduce_min_sync(0xffffffffu, least);
+  if (tid % 32 == 0) smost[tid / 32] = most, sleast[tid / 32] = least;
   __syncthreads();
   if (bad) sbad = 1;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) m = fmaxf(m, smax[w]);
-  // in steps of 2^8, so that neighbouring blocks hardly ever differ
-  const int ex = max((int)(__float_as_uint(m) >> 23) | 7, 15);
-  const float up = power_of_two(268 - ex);
+  const bool has = tid % 32 < kThreads / 32;
+  most = __reduce_max_sync(0xffffffffu, has ? smost[tid % 32] : 0u);
+  least = __reduce_min_sync(0xffffffffu, has ? sleast[tid % 32] : ~0u);
+  // The block's power of two goes in steps of 2^8, so that neighbouring blocks hardly ever differ. With it,
+  // the largest value of a slot lies above 2^-3 if its exponent is ex - 17 or more, and what two fp16 terms
+  // lose, 2^-25, is 2^-22 of it.
+  const int ex = max((int)(most >> 23) | 7, 15);
+  const bool wide = (int)(least >> 23) < ex - 17;
   unsigned char* image = static_cast<unsigned char*>(a.planes) + (size_t)blockIdx.x * T::kTile;
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
     const int j = tid + e * kThreads, row = j / C, c = j % C;
+    const int own = wide ? max((int)(m[e] >> 23), 15) : ex;
+    const float up = power_of_two(268 - own);
     uint32_t h[4], l[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) split2_f16(x[e][2 * u] * up, x[e][2 * u + 1] * up, h[u], l[u]);
     unsigned char* p = image + (c / 8) * T::kBox + row * 128 + (((c & 7) ^ (row & 7)) << 4);
     *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
     if constexpr (T::kPlanes == 2) *reinterpret_cast<uint4*>(p + T::BN * 128) = make_uint4(l[0], l[1], l[2], l[3]);
+    if (wide && c == 0) a.exps[(size_t)blockIdx.x * kTcExps + row] = (unsigned char)own;
   }
   __syncthreads();
-  if (tid == 0) {
-    float2* info = static_cast<float2*>(a.info) + blockIdx.x;
-    *info = make_float2(power_of_two(ex - 14), sbad ? 1.f : 0.f);
-  }
+  if (tid == 0) a.info[blockIdx.x] = (uint16_t)((uint32_t)ex | (sbad ? kTcBad : 0u) | (wide ? kTcWide : 0u));
 }
 
 // ---- the main kernel ---------------------------------------------------------------------------
@@ -354,10 +373,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
     const int w = warp >> 2, me = tid & 127;
     const uint32_t lanes = tmem + (uint32_t)w * 128 + ((uint32_t)((warp & 3) * 32) << 16);
     unsigned char* tile = sQ + w * 2 * T::kTile;
-    int done = 0, all = 0;  // blocks of this tile's, and of the CTA
+    int done = 0;  // blocks of this tile's (of the first tile's: of the CTA)
     rows_segments(P, kTcTileRows, BN, [&](const RowsTile& k, int b0, int b1, bool first_segment) {
-      const int nb = b1 - b0, r0 = k.r0 + w * 128, all0 = all;
-      all += nb;
+      const int nb = b1 - b0, r0 = k.r0 + w * 128;
       if (r0 >= k.R) return;
       // ---- q: rows scaled so that the softmax is in powers of two, each divided by a power of two
       // next to its largest element, as two fp16 terms. Rows behind the last one are zero.
@@ -405,22 +423,58 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
       const float back = sh.back[w * 128 + me];
       // the rows of this tile see slots up to p0 at least, and from p1 - window on
       const int p0 = k.t0 + r0 / k.G, p1 = k.t0 + (min(r0 + 128, k.R) - 1) / k.G;
-      const float2* info = static_cast<const float2*>(a.info);
+      const uint32_t* info = reinterpret_cast<const uint32_t*>(a.info);  // K's low, V's high
       int s0 = k.v.slot0(b0, BN);
-      float4 next = *reinterpret_cast<const float4*>(info + 2 * (size_t)unit_of(k, s0));
+      uint32_t next = info[unit_of(k, s0)];
       for (int n = 0; n < nb; ++n, ++done) {
-        const float4 now = next;  // factor of K, -, factor of V, whether V had other than numbers
+        const uint32_t now = next;
         const int s_now = s0;
         if (n + 1 < nb) {
           s0 = k.v.slot0(b0 + n + 1, BN);
-          next = *reinterpret_cast<const float4*>(info + 2 * (size_t)unit_of(k, s0));
+          next = info[unit_of(k, s0)];
         }
-        const float f = fmaxf(back * now.x, 1.175494351e-38f);  // (-inf times 0 would be NaN)
+        float f = fmaxf(back * power_of_two((int)(now & 255u) - 14), 1.175494351e-38f);  // (-inf times 0 would be NaN)
         const bool edge = s_now + BN - 1 > p0 || (s_now <= p1 - a.window && s_now + BN > a.sinks);
         // column c of the block is visible where c <= last and (c >= first or c < sink)
         const int last = slot - s_now, first = last >= a.window ? last - a.window + 1 : 0, sink = a.sinks - s_now;
         wait_phase(&sh.s_full[w], (uint32_t)done & 1u, &sh.abort);
         tc_fence_after();
+        // ---- wide blocks, 8 columns at a time: what the MMA left of them (two parts of it where K is two
+        // planes), and the powers of their slots
+        auto exps = [&](int v) {
+          return reinterpret_cast<const uint2*>(a.exps + (2 * (size_t)unit_of(k, s_now) + v) * kTcExps);
+        };
+        auto exp_at = [](uint2 x, int e) { return (int)((e < 4 ? x.x : x.y) >> (e % 4 * 8) & 255u); };
+        auto fetch8 = [&](int c, uint32_t(&u)[8], uint32_t(&z)[8]) {
+          tmem_ld8(lanes + (uint32_t)c, u);
+          if constexpr (T::kPlanes == 2) tmem_ld8(lanes + (uint32_t)(64 + c), z);
+          tmem_ld_wait();
+        };
+        auto put8 = [&](int c, const uint32_t(&u)[8]) {
+          tmem_st8(lanes + (uint32_t)c, u);
+          if constexpr (T::kPlanes == 2) {
+            const uint32_t zero[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+            tmem_st8(lanes + (uint32_t)(64 + c), zero);
+          }
+        };
+        if (__builtin_expect((now & kTcWide) != 0u, 0)) {  // the scores themselves over it
+          const uint2* own = exps(0);
+#pragma unroll 1
+          for (int c = 0; c < BN; c += 8) {
+            uint32_t u[8], z[8];
+            const uint2 ex = own[c / 8];
+            fetch8(c, u, z);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float y = __uint_as_float(u[e]);
+              if constexpr (T::kPlanes == 2) y += __uint_as_float(z[e]);
+              u[e] = __float_as_uint(y * fmaxf(back * power_of_two(exp_at(ex, e) - 14), 1.175494351e-38f));
+            }
+            put8(c, u);
+          }
+          tmem_st_wait();
+          f = 1.f;
+        }
         // ---- the largest score; hidden ones are at -inf here and below
         uint32_t ua[32], ub[32];
         float x = -INFINITY, x1 = x, x2 = x, x3 = x;
@@ -484,6 +538,45 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
         }
         const float base = m == -INFINITY ? 0.f : m;
         const float shift = 8.f - base + base > 15.f ? -base : 8.f - base;  // (8 - m may round to 16 - m)
+        // V's factor; a row that sees nothing of the block keeps the unit of its o.
+        float fv = x == -INFINITY ? unit : power_of_two((int)(now >> 16 & 255u) - 14);
+        // In a wide block it is the largest of the slots that the row sees: p takes the others' powers
+        // relative to it, in its exponent, after its sum.
+        if (__builtin_expect((now >> 16 & kTcWide) != 0u, 0)) {
+          const uint2* own = exps(1);
+          int top = 15;
+#pragma unroll 1
+          for (int c = 0; c < BN; c += 8) {
+            uint32_t u[8], z[8];
+            const uint2 ex = own[c / 8];
+            const uint32_t see = visible(c);
+            fetch8(c, u, z);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float y = __uint_as_float(u[e]);
+              if constexpr (T::kPlanes == 2) y += __uint_as_float(z[e]);
+              y = fmaf(y, f, shift);
+              if (see >> e & 1) top = max(top, exp_at(ex, e));
+              l += see >> e & 1 ? ex2(y) : 0.f;
+            }
+          }
+#pragma unroll 1
+          for (int c = 0; c < BN; c += 8) {
+            uint32_t u[8], z[8];
+            const uint2 ex = own[c / 8];
+            fetch8(c, u, z);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float y = __uint_as_float(u[e]);
+              if constexpr (T::kPlanes == 2) y += __uint_as_float(z[e]);
+              u[e] = __float_as_uint(fmaf(y, f, (float)(exp_at(ex, e) - top)));
+            }
+            put8(c, u);
+          }
+          tmem_st_wait();
+          f = 1.f;
+          if (x != -INFINITY) fv = power_of_two(top - 14);
+        }
         // ---- p over the scores, 32 columns of tensor memory at a time (32 scores, or 16 and their
         // second parts): while the exponentials of some are under way, the next ones land. A loop, not
         // unrolled: the code of both groups has to stay in the instruction cache. (And no decision inside:
@@ -529,21 +622,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
             sum += (s[0] + s[1]) + (s[2] + s[3]);
           }
         }
-        l += sum;
+        l += now >> 16 & kTcWide ? 0.f : sum;
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(w ? &sh.p1_ready : &sh.pv_ready[(all0 + n) % T::kTurns]);
+        mbar_arrive(w ? &sh.p1_ready : &sh.pv_ready[done % T::kTurns]);
         // o is in units of `unit`, a power of two that only grows
         float lift = 1.f, drop = 1.f;
-        if (now.z != unit) {
-          const float to = fmaxf(now.z, unit);
-          lift = unit / to, drop = now.z / to, unit = to;
+        if (fv != unit) {
+          const float to = fmaxf(fv, unit);
+          lift = unit / to, drop = fv / to, unit = to;
         }
+        const bool drops = __any_sync(0xffffffffu, drop != 1.f);
         wait_phase(&sh.o_full[w], (uint32_t)done & 1u, &sh.abort);
         tc_fence_after();
         const uint32_t from = lanes + 256u;
         auto take = [&](int d, uint32_t(&v)[32]) {
-          if (__builtin_expect(drop != 1.f, 0)) {
+          if (__builtin_expect(drops, 0)) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * drop);
           }
@@ -561,7 +655,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
           take(d + 32, ub);
         }
         tc_fence_before();
-        if (now.w != 0.f) {
+        if (now >> 16 & kTcBad) {
 #pragma unroll 1
           for (int c = 0; c < BN; ++c) {
             if (!(c <= last && (c >= first || c < sink))) continue;
@@ -620,7 +714,8 @@ cudaError_t launch(const RowsAttnArgs& a, const RowsBatch& b, int sms, int* laun
   using T = TcTile<KIND, HD>;
   RowsKernelArgs P;
   const RowsPlan plan = rows_plan(a, b, kTcTileRows, T::BN, sms, kTcLeastShare, 2, &P);
-  P.a.info = static_cast<char*>(a.planes) + (size_t)plan.units * 2 * T::kTile;
+  P.a.exps = static_cast<unsigned char*>(a.planes) + (size_t)plan.units * 2 * T::kTile;
+  P.a.info = reinterpret_cast<uint16_t*>(P.a.exps + (size_t)plan.units * 2 * kTcExps);
   rows_planes_kernel<KIND, HD><<<2 * plan.units, kPlaneThreads<KIND, HD>, 0, st>>>(P);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;

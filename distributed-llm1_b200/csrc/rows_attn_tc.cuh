@@ -26,10 +26,13 @@ struct TcTile {
   static_assert(kSmem + 2048 <= 227 * 1024, "shared memory");
 };
 inline int tc_block(int kind) { return kind == kKvBf16 ? 128 : 64; }
+constexpr int kTcExps = 128;  // bytes of a K or V block's powers per slot
+// Scratch of a (KV head, block) pair: K and V as fp16 planes; behind those of all pairs the powers per slot,
+// then 4 bytes each of what the main kernel is told of them.
+constexpr size_t tc_unit_bytes(int hd) { return (size_t)2 * 128 * 2 * hd + 2 * kTcExps + 4; }
 
 cudaError_t configure_rows_attn_tc();
-// Long chunks of a batch; a.planes holds their (KV head, block) pairs, 2 x 256 x head-size bytes
-// each, and 16 bytes each behind.
+// Long chunks of a batch; a.planes has room for their (KV head, block) pairs.
 cudaError_t launch_rows_tc(const RowsAttnArgs& a, const RowsBatch& b, int kind, int hd, int sms, int* launches,
                            cudaStream_t st);
 

@@ -836,3 +836,51 @@ def test_scores_where_eight_rounds_away(dllm, kind, m):
         got, high = R.ctx.readF32(out, out.n), float(R.values[0][1].abs().max())
         assert (np.abs(got) <= high * (1 + 1e-5)).all(), size
     R.close()
+
+
+def check_unequal(dllm, kind, m, edit, hd=64, t0=200, window=70, sinks=6):
+    """Attention where some slots hold far larger numbers than others: each row within the bound of what it
+    sees, and where no row sees such a slot, as near as ever on average."""
+    R = Rows(dllm, 8, 2, hd, kind, [t0], [m], edit=edit)
+    q = np.random.default_rng(3).standard_normal((m, 8, hd)).astype(np.float32)
+    out = R.attend(f32(R.ctx, q), window, sinks)
+    got = R.ctx.readF32(out, out.n).reshape(m, 8, hd).astype(np.float64)
+    want, vmax, amax = attend64(R, q, window, sinks)
+    err, bound = np.abs(got - want), attention_bound(R, vmax, amax)
+    assert np.isfinite(got).all()
+    assert (err <= bound).all(), f"worst {float((err / bound).max())} of the bound"
+    small = vmax.max(1) < 100
+    assert np.linalg.norm((got - want)[small]) <= 4e-6 * np.linalg.norm(want[small])
+    R.close()
+
+
+def large_slots(value, m, t0=200):
+    """Slots that no row sees, one that only the last row sees and one that the later half does."""
+    def edit(_, kv):
+        for s in (6, 9, 64, 129) + ((t0 + m // 2, t0 + m - 1) if m > 1 else ()):
+            kv[0][s] *= np.float32(value)
+            kv[1][s] *= np.float32(value)
+    return edit
+
+
+def spread_slots(_, kv):
+    """K of each slot by a power of two down to 2^-60, V by one from 2^-60 to 2^60."""
+    rng = np.random.default_rng(9)
+    n = len(kv[0])
+    kv[0] *= np.ldexp(np.float32(1), rng.integers(-60, 1, (n, 1, 1))).astype(np.float32)
+    kv[1] *= np.ldexp(np.float32(1), rng.integers(-60, 61, (n, 1, 1))).astype(np.float32)
+
+
+@pytest.mark.parametrize("kind,m", [("bf16", 1), ("bf16", 8), ("f32", 1), ("f32", 8), ("f32", 20)] +
+                         [(k, m) for k in KINDS for m in (90, 300)])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("value", [2.0 ** 12, 2.0 ** 20, 2.0 ** 36, 1e30])
+def test_large_hidden_values_do_not_leak(dllm, kind, m, hd, value):
+    check_unequal(dllm, kind, m, large_slots(value, m), hd)
+
+
+@pytest.mark.parametrize("kind,m", [("bf16", 1), ("bf16", 8), ("f32", 1), ("f32", 8), ("f32", 20)] +
+                         [(k, m) for k in KINDS for m in (90, 300)])
+@pytest.mark.parametrize("window,sinks", [(70, 6), (0, 0), (150, 0), (1, 0)])
+def test_slots_of_very_unequal_sizes(dllm, kind, m, window, sinks):
+    check_unequal(dllm, kind, m, spread_slots, 64 if m % 4 else 128, 333, window, sinks)
