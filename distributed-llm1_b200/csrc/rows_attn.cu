@@ -41,6 +41,7 @@
 #include "rows_attn.cuh"
 
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
 #include "mma_sync.cuh"
@@ -602,77 +603,139 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
 #pragma unroll
         for (int e = 0; e < (N8 ? 2 : 4); ++e)
           om[e] = nan_bits[e] ? __uint_as_float(nan_bits[e]) : fmaf(om[e], second(e) ? fb : fa, cm[e]);
-#pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-          // Column c of tile i of a group is its dim 8 (c & 3) + 4 (c >> 2) + i: lane (g, t) holds the
-          // four nibbles of column g in one half of a word, of two slots side by side in a register. (Narrow:
-          // tiles i and i + 1 are the halves of a product's 16 rows.)
-          constexpr int NC = N8 ? 2 : 4;
-          float c[NC][4];
-#pragma unroll
-          for (int i = 0; i < NC; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) c[i][e] = 0.f;
-          float sc[NK][4], most = 0.f;
-#pragma unroll
-          for (int j = 0; j < NK; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              sc[j][e] = bf16_lo(*reinterpret_cast<const uint32_t*>(pairs + (wslot + j * 16 + t + 4 * e) * T::kPairBytes + gr * 4));
-              most = fmaxf(most, sc[j][e]);
-            }
-          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-          // scale * up lies below 2^15; the exponent moves in steps of 8, so that it hardly ever does.
-          // (A scale is below 2^109, so both factors are normal numbers.)
-          const int ex = max((int)(__float_as_uint(most) >> 23) | 7, 15);
-          const float up = power_of_two(268 - ex), back = power_of_two(ex - 14);
-#pragma unroll
-          for (int j = 0; j < NK; ++j) {
-            const int row = wslot + j * 16 + t;
-            uint32_t w[4], h[4], l[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              sc[j][e] *= up;
-              w[e] = *reinterpret_cast<const uint16_t*>(sV + at4<HD, true>(row + 4 * e, gr) + (g & 3) * 4 + (g >> 2) * 2);
-            }
-            split2_f16(sh[2 * j][0] * sc[j][0], sh[2 * j][1] * sc[j][1], h[0], l[0]);
-            split2_f16(sh[2 * j + 1][0] * sc[j][2], sh[2 * j + 1][1] * sc[j][3], h[2], l[2]);
-            if constexpr (!N8) {
-              split2_f16(sh[2 * j][2] * sc[j][0], sh[2 * j][3] * sc[j][1], h[1], l[1]);
-              split2_f16(sh[2 * j + 1][2] * sc[j][2], sh[2 * j + 1][3] * sc[j][3], h[3], l[3]);
-            }
-            const uint32_t w0 = w[0] | w[1] << 16, w1 = w[2] | w[3] << 16;
-#pragma unroll
-            for (int i = 0; i < NC; ++i) {
-              if constexpr (N8) {
-                const uint32_t u0 = w0 >> (8 * i), u1 = w1 >> (8 * i);
-                const uint32_t v[4] = {codes_f16(u0), codes16_f16(u0), codes_f16(u1), codes16_f16(u1)};
-                mma_f16(c[i], v, l[0], l[2]);
-                mma_f16(c[i], v, h[0], h[2]);
-              } else {
-                const uint32_t u0 = w0 >> (i / 2 * 8), u1 = w1 >> (i / 2 * 8);
-                const uint32_t b0 = i % 2 ? codes16_f16(u0) : codes_f16(u0), b1 = i % 2 ? codes16_f16(u1) : codes_f16(u1);
-                mma_f16(c[i], l, b0, b1);
-                mma_f16(c[i], h, b0, b1);
-              }
-            }
+        // Where rows see only a part of the block, a hidden slot's scale may be far larger than theirs, and with
+        // one factor for all it would leave p times theirs few bits, or none. So where the scales of a group are more
+        // than 2^10 to 2^17 apart (two fp16 terms lose 2^-25, 2^-22 of what 2^-17 of the largest leaves), each row
+        // goes by the scales that it sees (PART). That code is a copy of its own: 64 sequences of 8000 slots take
+        // 67.8 us with their launches, 66.7 without any of this, 68.6 with the copy for every block that rows
+        // see a part of, 71 with these decisions in one loop, 70.7 with the block's slots in turns of like scales.
+        auto p_at = [&](int j, int e, int row) { return sh[2 * j + e / 2][e % 2 + 2 * row]; };
+        auto scale_at = [&](int j, int e, int gr) {
+          return bf16_lo(*reinterpret_cast<const uint32_t*>(pairs + (wslot + j * 16 + t + 4 * e) * T::kPairBytes + gr * 4));
+        };
+        auto power = [](float m) { return max((int)(__float_as_uint(m) >> 23) | 7, 15); };
+        auto most_of_row = [](float m) {
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          return fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        };
+        bool uneven = false;
+        if (edge) {
+          const uint32_t* own = reinterpret_cast<const uint32_t*>(pairs + (wslot + lane % SN) * T::kPairBytes);  // a lane per slot
+#pragma unroll 1
+          for (int gr = 0; gr < NG; ++gr) {
+            const uint32_t x = own[gr] & 0x7fffu;  // the scale's bits: its exponent from bit 7 on
+            const uint32_t most = __reduce_max_sync(0xffffffffu, x) >> 7, least = __reduce_min_sync(0xffffffffu, x ? x : 0x7fffu) >> 7;
+            uneven |= least + 17u < (most | 7u);
           }
-          float ga = fa, gb = fb;
-          if (back != unit[gr]) {
-            const float now = fmaxf(back, unit[gr]), lift = unit[gr] / now, drop = back / now;
-            ga *= lift, gb *= lift;
-            unit[gr] = now;
+        }
+        auto add_codes = [&](auto part) {
+          constexpr bool PART = decltype(part)::value;
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr) {
+            // Column c of tile i of a group is its dim 8 (c & 3) + 4 (c >> 2) + i: lane (g, t) holds the
+            // four nibbles of column g in one half of a word, of two slots side by side in a register. (Narrow:
+            // tiles i and i + 1 are the halves of a product's 16 rows.)
+            constexpr int NC = N8 ? 2 : 4;
+            float c[NC][4];
 #pragma unroll
             for (int i = 0; i < NC; ++i)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) c[i][e] *= drop;
+              for (int e = 0; e < 4; ++e) c[i][e] = 0.f;
+            float sc[NK][4], most = 0.f;
+#pragma unroll
+            for (int j = 0; j < NK; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                sc[j][e] = scale_at(j, e, gr);
+                if constexpr (N8 && PART) sc[j][e] = p_at(j, e, 0) != 0.f ? sc[j][e] : 0.f;
+              }
+#pragma unroll
+            for (int j = 0; j < NK; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) most = fmaxf(most, sc[j][e]);
+            float most_b = most;
+            if constexpr (!N8 && PART) {
+              most = most_b = 0.f;
+#pragma unroll
+              for (int j = 0; j < NK; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  if (p_at(j, e, 0) != 0.f) most = fmaxf(most, sc[j][e]);
+                  if (p_at(j, e, 1) != 0.f) most_b = fmaxf(most_b, sc[j][e]);
+                }
+            }
+            most = most_of_row(most);
+            if constexpr (!N8 && PART) most_b = most_of_row(most_b);
+            else most_b = most;
+            // scale * up lies below 2^15; the exponent moves in steps of 8, so that it hardly ever does.
+            // (A scale is below 2^109, so both factors are normal numbers.)
+            const int ex = power(most), ex_b = N8 ? ex : power(most_b);
+            const float up = power_of_two(268 - ex), up_b = power_of_two(268 - ex_b), back = power_of_two(ex - 14);
+#pragma unroll
+            for (int j = 0; j < NK; ++j) {
+              const int row = wslot + j * 16 + t;
+              uint32_t w[4], h[4], l[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                w[e] = *reinterpret_cast<const uint16_t*>(sV + at4<HD, true>(row + 4 * e, gr) + (g & 3) * 4 + (g >> 2) * 2);
+              }
+              float y[4];  // (a scale above the row's own limit is of a hidden slot: cut, so that it times 0 is 0)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y[e] = p_at(j, e, 0) * (N8 || !PART ? sc[j][e] * up : fminf(sc[j][e] * up, 0x1p15f));
+              split2_f16(y[0], y[1], h[0], l[0]), split2_f16(y[2], y[3], h[2], l[2]);
+              if constexpr (!N8) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = p_at(j, e, 1) * (PART ? fminf(sc[j][e] * up_b, 0x1p15f) : sc[j][e] * up);
+                split2_f16(y[0], y[1], h[1], l[1]), split2_f16(y[2], y[3], h[3], l[3]);
+              }
+              const uint32_t w0 = w[0] | w[1] << 16, w1 = w[2] | w[3] << 16;
+#pragma unroll
+              for (int i = 0; i < NC; ++i) {
+                if constexpr (N8) {
+                  const uint32_t u0 = w0 >> (8 * i), u1 = w1 >> (8 * i);
+                  const uint32_t v[4] = {codes_f16(u0), codes16_f16(u0), codes_f16(u1), codes16_f16(u1)};
+                  mma_f16(c[i], v, l[0], l[2]);
+                  mma_f16(c[i], v, h[0], h[2]);
+                } else {
+                  const uint32_t u0 = w0 >> (i / 2 * 8), u1 = w1 >> (i / 2 * 8);
+                  const uint32_t b0 = i % 2 ? codes16_f16(u0) : codes_f16(u0), b1 = i % 2 ? codes16_f16(u1) : codes_f16(u1);
+                  mma_f16(c[i], l, b0, b1);
+                  mma_f16(c[i], h, b0, b1);
+                }
+              }
+            }
+            // o goes by the largest of its rows' units, but by 2^30 at most: what others hold stays far above
+            // fp32's smallest number, whatever one row sees.
+            float ga = fa, gb = fb;
+            if (PART || back != unit[gr]) {
+              float top = back, drop_c = back, drop_d = back;
+              if constexpr (PART) {
+                const float back_b = power_of_two(ex_b - 14);
+                top = fmaxf(back, back_b), drop_d = back_b;
+#pragma unroll
+                for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+                if constexpr (N8) {  // from row g to the rows of o
+                  drop_c = __shfl_sync(0xffffffffu, back, 8 * t);
+                  drop_d = __shfl_sync(0xffffffffu, back, 8 * t + 4);
+                }
+              }
+              const float now = fminf(fmaxf(top, unit[gr]), 0x1p30f), lift = unit[gr] / now;
+              drop_c /= now, drop_d /= now;
+              ga *= lift, gb *= lift;
+              unit[gr] = now;
+#pragma unroll
+              for (int i = 0; i < NC; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[i][e] *= second(e) ? drop_d : drop_c;
+            }
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[gr * NC + i][e] = fmaf(o[gr * NC + i][e], second(e) ? gb : ga, c[i][e]);
           }
-#pragma unroll
-          for (int i = 0; i < NC; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[gr * NC + i][e] = fmaf(o[gr * NC + i][e], second(e) ? gb : ga, c[i][e]);
-        }
+        };
+        if (uneven) add_codes(std::true_type{});
+        else add_codes(std::false_type{});
       } else {
         // A row of V that some rows do not see may hold infinities or NaN, and 0 x NaN would reach
         // the rows that must not see it: such values are taken out of the tile and added to the

@@ -857,7 +857,7 @@ def check_unequal(dllm, kind, m, edit, hd=64, t0=200, window=70, sinks=6):
 def large_slots(value, m, t0=200):
     """Slots that no row sees, one that only the last row sees and one that the later half does."""
     def edit(_, kv):
-        for s in (6, 9, 64, 129) + ((t0 + m // 2, t0 + m - 1) if m > 1 else ()):
+        for s in {6, 9, 64, 129} | ({t0 + m // 2, t0 + m - 1} if m > 1 else set()):
             kv[0][s] *= np.float32(value)
             kv[1][s] *= np.float32(value)
     return edit
@@ -884,3 +884,28 @@ def test_large_hidden_values_do_not_leak(dllm, kind, m, hd, value):
 @pytest.mark.parametrize("window,sinks", [(70, 6), (0, 0), (150, 0), (1, 0)])
 def test_slots_of_very_unequal_sizes(dllm, kind, m, window, sinks):
     check_unequal(dllm, kind, m, spread_slots, 64 if m % 4 else 128, 333, window, sinks)
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 8, 16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("value", [2.0 ** 12, 2.0 ** 20, 2.0 ** 40, 1e30, 2.0 ** 106])
+def test_large_hidden_codes_do_not_leak(dllm, m, hd, value):
+    """The scales of hidden slots of a 4-bit cache, in tiles of 8, 16 and 32 rows."""
+    check_unequal(dllm, "4", m, large_slots(value, m), hd)
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 8, 16])
+@pytest.mark.parametrize("window,sinks", [(70, 6), (0, 0), (150, 0), (1, 0)])
+def test_codes_of_very_unequal_scales(dllm, m, window, sinks):
+    check_unequal(dllm, "4", m, spread_slots, 64 if m % 4 else 128, 333, window, sinks)
+
+
+@pytest.mark.parametrize("m", [1, 3, 8])
+def test_scales_from_the_smallest_to_the_largest(dllm, m):
+    """Rows that see scales of 2^-60 beside slots that they do not see of 2^106, and the other way round."""
+    def edit(_, kv):
+        kv[1] *= np.float32(2.0 ** -60)
+        kv[1][::2] *= np.float32(2.0 ** 60)
+        kv[1][64:128] *= np.float32(2.0 ** 106)
+        kv[1][200:, :, 32:] *= np.float32(2.0 ** 100)
+    check_unequal(dllm, "4", m, edit, 64, 200, 70, 6)
