@@ -6,8 +6,9 @@
 //   c = (x - m) / s to the nearest whole number, ties to even
 // (x - m, largest - m and the quotients are rounded to fp32). Rounding m down and s up keeps
 // every value inside [m, m + 15 s], so each is off by at most s / 2 (and the fp32 rounding).
-// A group with a NaN, an infinity, or a range of 2^112 or more (no scale that kernels multiply
-// freely) has m = NaN: all its values read NaN.
+// A group with a NaN, a number beyond the largest bf16 one (3.39e38: no m below it, or no middle near
+// it), an infinity among them, or a range of 2^112 or more (no scale that kernels multiply freely) has
+// m = NaN: all its values read NaN.
 //
 // Memory-bound: 4 bytes in and 5 bits out per value. A thread takes 8 dims of K and of V (four
 // 16-byte loads under way, one word of codes each); the four threads of a group exchange
@@ -23,11 +24,11 @@ namespace {
 
 constexpr int kThreads = 256;
 
-DLLM_DEV float bf16_down(float x) {  // the largest finite bf16 that is not above x (x finite)
+constexpr float kBf16Most = 0x1.fep127f;
+DLLM_DEV float bf16_down(float x) {  // the largest bf16 that is not above x (|x| <= kBf16Most)
   uint32_t u = __float_as_uint(x);
   if (x < 0.f) u += 0xffffu;
-  u &= 0xffff0000u;
-  return __uint_as_float(u == 0xff800000u ? 0xff7f0000u : u);
+  return __uint_as_float(u & 0xffff0000u);
 }
 DLLM_DEV float bf16_up(float x) {  // the smallest bf16 that is not below x (x >= 0, far from the largest)
   return __uint_as_float((__float_as_uint(x) + 0xffffu) & 0xffff0000u);
@@ -48,7 +49,7 @@ DLLM_DEV uint32_t encode(const float (&x)[8], uint32_t& pair) {
   float lo = x[0], hi = x[0];
   bool fine = true;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]), fine = fine && is_finite(x[e]);
+  for (int e = 0; e < 8; ++e) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]), fine = fine && fabsf(x[e]) <= kBf16Most;
 #pragma unroll
   for (int w = 1; w < 4; w <<= 1) {
     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, w));

@@ -460,8 +460,8 @@ int dllm_stage_window_attention(dllm_stage* st, int layer, const dllm_rows* rows
  * share a minimum m and a scale s in bf16 (5 bits per value in all): a value is m + c s,
  *   m = the smallest of the 32 rounded down, s = fp32((largest - m) / 15) rounded up,
  *   c = (x - m) / s to the nearest of 0..15 (ties to even)
- * so that it is off by s / 2 at most. 32 values with a NaN, an infinity or a range of 2^112
- * and more among them all read NaN. */
+ * so that it is off by s / 2 at most. 32 values with a NaN, a number beyond bf16's largest (3.39e38;
+ * infinities are) or a range of 2^112 and more among them all read NaN. */
 typedef struct dllm_kv4 dllm_kv4;
 int dllm_kv4_create(dllm_ctx* ctx, int start, int end, dllm_kv4** out);
 void dllm_kv4_destroy(dllm_kv4* kv);

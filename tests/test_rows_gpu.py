@@ -909,3 +909,35 @@ def test_scales_from_the_smallest_to_the_largest(dllm, m):
         kv[1][64:128] *= np.float32(2.0 ** 106)
         kv[1][200:, :, 32:] *= np.float32(2.0 ** 100)
     check_unequal(dllm, "4", m, edit, 64, 200, 70, 6)
+
+
+@pytest.mark.parametrize("m", [1, 3, 8, 90])
+@pytest.mark.parametrize("value", [-3.4028235e38, 3.4028235e38, -3.397e38, -3.38953139e38, 3.38953139e38])
+def test_codes_of_the_largest_numbers(dllm, m, value):
+    """32 values beyond the largest bf16 number read NaN, by read_rows and by attention alike, and change
+    nothing where they are hidden; the largest number itself is kept."""
+    value = np.float32(value)
+    fits = abs(float(value)) <= float.fromhex("0x1.fep127")
+
+    def edit(_, kv):
+        for x in kv:
+            x[40, :, :32] = x[210 + m - 1, :, :32] = value
+            x[41, :, 32] = np.float32(-3.4028235e38)  # among ordinary values: a range beyond 2^112 besides
+    R = Rows(dllm, 4, 2, 64, "4", [210], [m], edit=edit)
+    R.cache.set_t0(0, 0)
+    got = R.ctx.readF32(R.cache.read_rows(0, R.ctx.rowBatch([210 + m]))[1], (210 + m) * 128).reshape(-1, 2, 2, 32)
+    R.cache.set_t0(0, 210)
+    assert np.isnan(got[41, :, 1]).all()
+    assert (got[[40, -1], :, 0] == value).all() if fits else np.isnan(got[[40, -1], :, 0]).all()
+    got[[40, -1], :, 0] = got[41, :, 1] = 0
+    assert np.isfinite(got).all()
+    # the last row, which sees its own slot, aside
+    R.values = [[torch_().nan_to_num(x, 0.0, 0.0, 0.0) for x in R.values[0]]]
+    q = np.random.default_rng(3).standard_normal((m, 4, 64)).astype(np.float32)
+    out = R.attend(f32(R.ctx, q), 100, 6)
+    got = R.ctx.readF32(out, out.n).reshape(m, 4, 64)
+    want, vmax, amax = attend64(R, q, 100, 6)
+    assert (np.abs(got - want) <= attention_bound(R, vmax, amax))[:-1].all()
+    if not fits:
+        assert np.isnan(got[-1, :, :32]).all()
+    R.close()
