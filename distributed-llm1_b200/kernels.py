@@ -10,6 +10,7 @@ reference does; every op runs a hand-written sm_100a kernel from libdllm.so.
 from __future__ import annotations
 
 import ctypes as C
+import operator
 
 import numpy as np
 
@@ -97,6 +98,17 @@ def int32s(values, what: str) -> np.ndarray:
     if b is None or (a != b).any():
         raise _lib.DllmError(_lib.DLLM_EINVAL, f"{what}: need 32-bit integers")
     return b
+
+
+def int32(value, what: str) -> int:
+    """One integer of 32 bits: ctypes would cut others to some other number."""
+    try:
+        n = operator.index(value)
+    except TypeError:
+        n = 1 << 31
+    if not -1 << 31 <= n < 1 << 31:
+        raise _lib.DllmError(_lib.DLLM_EINVAL, f"{what}: need a 32-bit integer, not {value!r}")
+    return n
 
 
 class DraftTree:
@@ -360,6 +372,7 @@ class KernelContext:
                kBuf: GpuBuffer | None = None, qOut: GpuBuffer | None = None, kOut: GpuBuffer | None = None):
         """Row t of q [n, NQ*HD] and k [n, KVH*HD] at positions[t]; in place without outputs."""
         h, o = self._h, self._opt
+        n = int32(n, "ropeAt")
         self._check(self.lib.dllm_rope_at(self.handle, h(plan, RopePlan), h(positions), n, o(qBuf), o(kBuf), o(qOut),
                                           o(kOut)), "ropeAt")
         return qOut or qBuf, kOut or kBuf
@@ -370,6 +383,7 @@ class KernelContext:
         """Each head of q [n, NQ*HD] and k [n, KVH*HD] divided by its root mean square and scaled
         by its norm (bf16 [HD]), then turned as by ropeAt; in place without outputs."""
         h, o = self._h, self._opt
+        n = int32(n, "normRopeAt")
         self._check(self.lib.dllm_norm_rope_at(self.handle, h(plan, RopePlan), h(positions), n, o(qBuf), o(kBuf), o(qNorm),
                                                o(kNorm), o(qOut), o(kOut)), "normRopeAt")
         return qOut or qBuf, kOut or kBuf

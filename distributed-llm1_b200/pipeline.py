@@ -18,7 +18,7 @@ import numpy as np
 
 from . import _lib, frames
 from .constants import FRAME
-from .kernels import DraftTree, GpuBuffer, KernelContext, RowBatch, int32s
+from .kernels import DraftTree, GpuBuffer, KernelContext, RowBatch, int32, int32s
 
 
 # ---- assignLayers (pipeline.js:6-23) ---------------------------------------------------
@@ -173,13 +173,13 @@ class Stage:
 
     @T0.setter
     def T0(self, v: int):
-        self.k._check(self.lib.dllm_stage_set_t0(self.handle, 0, int(v)), "T0")
+        self.k._check(self.lib.dllm_stage_set_t0(self.handle, 0, int32(int(v), "T0")), "T0")
 
     def t0_of(self, seq: int) -> int:
-        return self.lib.dllm_stage_get_t0(self.handle, seq)
+        return self.lib.dllm_stage_get_t0(self.handle, int32(seq, "t0_of"))
 
     def set_t0(self, seq: int, v: int):
-        self.k._check(self.lib.dllm_stage_set_t0(self.handle, seq, int(v)), "set_t0")
+        self.k._check(self.lib.dllm_stage_set_t0(self.handle, int32(seq, "set_t0"), int32(int(v), "set_t0")), "set_t0")
 
     def reset(self):
         self.k._check(self.lib.dllm_stage_reset(self.handle), "reset")
@@ -232,7 +232,7 @@ class Stage:
 
     def set_page_table(self, seq: int, pages):
         p = np.ascontiguousarray(pages, dtype=np.int32)
-        self.k._check(self.lib.dllm_stage_set_page_table(self.handle, seq, _lib.ptr(p, C.c_int32), p.size),
+        self.k._check(self.lib.dllm_stage_set_page_table(self.handle, int32(seq, "set_page_table"), _lib.ptr(p, C.c_int32), p.size),
                       "set_page_table")
 
     # ---- drafted trees (include/dllm.h; no counterpart in the reference)
@@ -283,7 +283,8 @@ class Stage:
     def append_rows(self, L: int, rows: RowBatch, kBuf: GpuBuffer, vBuf: GpuBuffer):
         """K/V rows of a batch -> slots T0 + j of their sequences (T0 unchanged)."""
         h = self.k._h
-        self.k._check(self.lib.dllm_stage_append_rows(self.handle, L, h(rows, RowBatch), h(kBuf), h(vBuf)), "append_rows")
+        self.k._check(self.lib.dllm_stage_append_rows(self.handle, int32(L, "append_rows"), h(rows, RowBatch), h(kBuf), h(vBuf)),
+                      "append_rows")
 
     def window_attention(self, L: int, rows: RowBatch, qBuf: GpuBuffer, out: GpuBuffer | None = None, window: int = 0,
                          sinks: int = 0) -> GpuBuffer:
@@ -307,9 +308,9 @@ class Stage:
 def _rows_attention(fn, cache, L, rows, qBuf, out, window, sinks, what) -> GpuBuffer:
     k = cache.k
     r, q = k._h(rows, RowBatch), k._h(qBuf)
+    L, window, sinks = int32(L, what), int32(window, what), int32(sinks, what)
     if out is None:
         out = k.createF32(rows.n * k.NQ * k.HD, what + " out")
-    window, sinks = (int(x) for x in int32s([window, sinks], what))
     k._check(fn(cache.handle, L, r, q, k._h(out), window, sinks), what)
     return out
 
@@ -321,7 +322,7 @@ class Cache4:
     def __init__(self, kctx: KernelContext, start: int, end: int):
         self.k, self.lib, self.start, self.end, self.handle = kctx, kctx.lib, start, end, None
         h = C.c_void_p()
-        kctx._check(self.lib.dllm_kv4_create(kctx.handle, start, end, C.byref(h)), "Cache4")
+        kctx._check(self.lib.dllm_kv4_create(kctx.handle, int32(start, "Cache4"), int32(end, "Cache4"), C.byref(h)), "Cache4")
         self.handle = h.value
 
     @property
@@ -333,10 +334,10 @@ class Cache4:
         self.set_t0(0, v)
 
     def t0_of(self, seq: int) -> int:
-        return self.lib.dllm_kv4_get_t0(self.handle, seq)
+        return self.lib.dllm_kv4_get_t0(self.handle, int32(seq, "t0_of"))
 
     def set_t0(self, seq: int, v: int):
-        self.k._check(self.lib.dllm_kv4_set_t0(self.handle, seq, int(v)), "set_t0")
+        self.k._check(self.lib.dllm_kv4_set_t0(self.handle, int32(seq, "set_t0"), int32(int(v), "set_t0")), "set_t0")
 
     def reset(self):
         self.k._check(self.lib.dllm_kv4_reset(self.handle), "reset")
@@ -351,17 +352,19 @@ class Cache4:
 
     def set_page_table(self, seq: int, pages):
         p = int32s(pages, "set_page_table")
+        seq = int32(seq, "set_page_table")
         self.k._check(self.lib.dllm_kv4_set_page_table(self.handle, seq, _lib.ptr(p, C.c_int32), p.size), "set_page_table")
 
     def append(self, L: int, rows: RowBatch, kBuf: GpuBuffer, vBuf: GpuBuffer):
         """K/V rows of a batch -> slots T0 + j of their sequences, rounded to 4 bits (T0 unchanged)."""
         h = self.k._h
+        L = int32(L, "append")
         self.k._check(self.lib.dllm_kv4_append(self.handle, L, h(rows, RowBatch), h(kBuf), h(vBuf)), "append")
 
     def read_rows(self, L: int, rows: RowBatch, kOut: GpuBuffer | None = None, vOut: GpuBuffer | None = None):
         """The values that the slots T0 + j of a batch stand for, fp32 [n, KVH*HD]."""
         k = self.k
-        r, n = k._h(rows, RowBatch), rows.n * k.KVH * k.HD
+        L, r, n = int32(L, "read_rows"), k._h(rows, RowBatch), rows.n * k.KVH * k.HD
         if kOut is None and vOut is None:
             kOut, vOut = k.createF32(n, "k rows"), k.createF32(n, "v rows")
         k._check(self.lib.dllm_kv4_read_rows(self.handle, L, r, k._opt(kOut), k._opt(vOut)), "read_rows")

@@ -83,3 +83,33 @@ def test_null_arguments_are_refused(dllm):
     assert lib.dllm_kv4_attention(None, 0, None, None, None, 0, 0) == bad
     lib.dllm_rows_destroy(None)
     lib.dllm_kv4_destroy(None)
+
+
+@pytest.mark.parametrize("wrong", [2 ** 32, 2 ** 32 + 1, -2 ** 32, 2 ** 31, np.int64(2 ** 32), 0.5, "0", None])
+def test_layers_sequences_and_slots_are_32_bit_integers(dllm, wrong):
+    """ctypes cuts larger numbers to some other layer, sequence or slot."""
+    ctx, stage, cache = bare(dllm)
+    buf = kernels.GpuBuffer(ctx, 16, 2, "f32")
+    plan, rows = object.__new__(kernels.RopePlan), object.__new__(kernels.RowBatch)
+    plan.ctx = rows.ctx = ctx
+    rows.n = 1
+    plan.handle, rows.handle = 48, 64
+    try:
+        for call in (lambda: stage.append_rows(wrong, rows, buf, buf), lambda: stage.window_attention(wrong, rows, buf, buf),
+                     lambda: stage.window_attention(wrong, rows, buf), lambda: stage.t0_of(wrong), lambda: stage.set_t0(wrong, 0),
+                     lambda: stage.set_page_table(wrong, [0]), lambda: cache.append(wrong, rows, buf, buf),
+                     lambda: cache.attention(wrong, rows, buf), lambda: cache.read_rows(wrong, rows, buf),
+                     lambda: cache.read_rows(wrong, rows), lambda: cache.t0_of(wrong), lambda: cache.set_t0(wrong, 0),
+                     lambda: cache.set_page_table(wrong, [0]), lambda: dllm.Cache4(ctx, wrong, 1), lambda: dllm.Cache4(ctx, 0, wrong),
+                     lambda: ctx.normRopeAt(plan, buf, wrong, buf, None, buf), lambda: ctx.ropeAt(plan, buf, wrong, buf)):
+            with pytest.raises(dllm.DllmError):
+                call()
+        if isinstance(wrong, (int, np.integer)):  # T0 takes what int() takes, as it did
+            for cached in (stage, cache):
+                with pytest.raises(dllm.DllmError):
+                    cached.set_t0(0, wrong)
+                with pytest.raises(dllm.DllmError):
+                    cached.T0 = wrong
+    finally:  # the handles are made up
+        for x in (buf, plan, rows):
+            x.handle = None
