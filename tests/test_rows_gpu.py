@@ -941,3 +941,37 @@ def test_codes_of_the_largest_numbers(dllm, m, value):
     if not fits:
         assert np.isnan(got[-1, :, :32]).all()
     R.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_values_while_the_scratch_grows(dllm, kind):
+    """Chunk after chunk of a conversation of ordinary numbers: the outputs are the definition's whenever the
+    scratch has just been replaced, and in between."""
+    torch = torch_()
+    far, chunk, nq, kvh, hd = 3000, 200, 8, 4, 128
+    ctx = make_ctx(dllm, nq, kvh, hd, max_pos=far, max_seqs=1, kv_dtype="bf16" if kind == "bf16" else "f32")
+    R = object.__new__(Rows)
+    R.ctx, R.kind, R.nq, R.kvh, R.hd, R.layer = ctx, kind, nq, kvh, hd, 0
+    R.cache = dllm.Cache4(ctx, 0, 1) if kind == "4" else dllm.Stage(ctx, 0, 1)
+    rng, rows = np.random.default_rng(8), ctx.rowBatch([chunk])
+    R.rows, R.counts, R.values = rows, [chunk], [[torch.empty((0, kvh, hd), dtype=torch.float64, device="cuda")] * 2]
+    q, k, v = (ctx.createF32(chunk * h * hd) for h in (nq, kvh, kvh))
+    out, held = ctx.createF32(chunk * nq * hd), []
+    for t in range(0, far, chunk):
+        x = [rng.standard_normal((chunk, h, hd)).astype(np.float32) for h in (nq, kvh, kvh)]
+        for b, a in zip((q, k, v), x):
+            ctx.writeF32(b, a)
+        R.cache.set_t0(0, t)
+        R.append(rows, k, v)
+        R.lens = [t]
+        R.values = [[torch.cat([h, torch.from_numpy(R.held(a)).cuda()]) for h, a in zip(R.values[0], x[1:])]]
+        ctx.writeF32(out, np.full(out.n, np.nan))
+        free = torch.cuda.mem_get_info()[0]
+        R.attend(q, out=out)
+        held.append(torch.cuda.mem_get_info()[0] != free)
+        got = ctx.readF32(out, out.n).reshape(chunk, nq, hd)
+        want, vmax, amax = attend64(R, x[0], 0, 0)
+        assert (np.abs(got - want) <= attention_bound(R, vmax, amax)).all(), t
+        assert np.linalg.norm(got - want) <= 4e-6 * np.linalg.norm(want)
+    assert sum(held) >= 2  # it did grow
+    R.close()
