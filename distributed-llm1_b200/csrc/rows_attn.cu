@@ -35,9 +35,10 @@
 // the second terms of q take rows 8 to 15: one product instead of two. A warp copies the slots that it
 // works on itself, without barriers in the loop.
 //
-// What bounds it. 24 sequences of 4000 slots, 2 KV heads of 128, fp32: 41 us, 3.7 TB/s; 64 of 8000 in
-// 4 bits: 61 us, 2 TB/s, where a warp spends 1200 instructions per 32 slots, about as many each on
-// the integer and the floating-point pipe (unpacking codes, cutting p, scales), and 70 MMAs.
+// What bounds it. 24 sequences of 2000 to 4000 slots (3043 on average), 2 KV heads of 128, fp32: 41 us, 3.7
+// TB/s; 64 of 4000 to 8000 (6032 on average) in 4 bits: 63 us, 2 TB/s, where a warp spends 1200 instructions
+// per 32 slots, about as many each on the integer and the floating-point pipe (unpacking codes, cutting
+// p, scales), and 70 MMAs.
 #include "rows_attn.cuh"
 
 #include <algorithm>
@@ -59,7 +60,8 @@ DLLM_DEV void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Nibbles 0 and 4 of u, less 8, as packed fp16, and 16 times nibbles 1 and 5, less 8.
+// Nibbles 0 and 4 of u, less 8, as packed fp16, and 16 times nibbles 1 and 5, less 8. (Small whole numbers
+// as the low bits of a float whose unit they are, a well-known conversion.)
 DLLM_DEV uint32_t codes_f16(uint32_t u) {
   uint32_t r;
   asm("{\n\t.reg .b32 t;\n\tlop3.b32 t, %1, 0x000f000f, 0x64006400, 0xea;\n\tsub.rn.f16x2 %0, t, %2;\n\t}"
@@ -606,8 +608,8 @@ __global__ void __launch_bounds__(kThreads, Tile<KIND, HD, WR>::kCtas) rows_attn
         // Where rows see only a part of the block, a hidden slot's scale may be far larger than theirs, and with
         // one factor for all it would leave p times theirs few bits, or none. So where the scales of a group are more
         // than 2^10 to 2^17 apart (two fp16 terms lose 2^-25, 2^-22 of what 2^-17 of the largest leaves), each row
-        // goes by the scales that it sees (PART). That code is a copy of its own: 64 sequences of 8000 slots take
-        // 67.8 us with their launches, 66.7 without any of this, 68.6 with the copy for every block that rows
+        // goes by the scales that it sees (PART). That code is a copy of its own: 64 sequences of 4000 to 8000 slots
+        // take 67.8 us with their launches, 66.7 without any of this, 68.6 with the copy for every block that rows
         // see a part of, 71 with these decisions in one loop, 70.7 with the block's slots in turns of like scales.
         auto p_at = [&](int j, int e, int row) { return sh[2 * j + e / 2][e % 2 + 2 * row]; };
         auto scale_at = [&](int j, int e, int gr) {
@@ -1084,7 +1086,8 @@ cudaError_t launch(const RowsAttnArgs& a, const RowsBatch& b, int sms, int* laun
 // Rows of a sequence that share a KV head, from which on it is a long chunk (rows_attn_tc.cu). Eight
 // sequences of 8000 slots, 4 KV heads of 128, with 63 rows and with 70, here against there: bf16 87
 // and 134, 139 and 135 us; 4-bit 102 and 141, 171 and 141. An fp32 row costs the tensor cores'
-// slow type here: 121 us for 28 rows, 203 against 133 for 35.
+// slow type here: 121 us for 28 rows, 203 against 133 for 35. (One shape: heads of 64, other groups and short
+// contexts go by the same numbers, unmeasured.)
 bool is_long(const RowsAttnArgs& a, int m, int kind) { return m * (a.nq / a.pages.kvh) > (kind == kKvF32 ? 32 : 64); }
 
 // (KV head, block) pairs of one sequence.
@@ -1102,7 +1105,9 @@ cudaError_t launch_short(const RowsAttnArgs& a, const RowsBatch& b, int sms, int
   for (int i = 0; i < b.n_seqs; ++i) rows = std::max(rows, b.m[i] * (a.nq / a.pages.kvh));
   // Eight sequences of 8000 slots, 4 KV heads of 128: 7 rows, tiles of 8 against 16 (fp32, bf16, 4-bit):
   // 58, 36, 30 against 82, 40, 42 us; 14 rows, tiles of 16 against 32: 83, 42, 43 against 119,
-  // 52, 60. Tiles of 64 gained nothing over two of 32 (63 rows: 87, 102 against 88, 101).
+  // 52, 60. Tiles of 64 gained nothing over two of 32 (63 rows: 87, 102 against 88, 101). One width serves
+  // all of a call's short sequences: beside 31 of one row, one of two rows costs 65, 138, 71 us (bf16, fp32,
+  // 4-bit; 56, 97, 46 for 32 of one), one of four 87, 208, 105, and in calls of their own 70, 117, 64.
   if (rows <= 8) return launch<KIND, HD, 0>(a, b, sms, launches, st);
   if (rows <= 16) return launch<KIND, HD, 1>(a, b, sms, launches, st);
   return launch<KIND, HD, 2>(a, b, sms, launches, st);

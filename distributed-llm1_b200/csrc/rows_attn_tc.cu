@@ -28,8 +28,10 @@
 // q_low K_high goes to the K_low half; the softmax adds the halves.
 // Tensor memory: S and P of both tiles 2 x 128 columns, O 2 x 128.
 // What bounds it: the products and, between them, the softmax. A chunk of 2048 rows of 28 heads of 128
-// under a 4096-token window, bf16: 216 us in the main kernel, 557 TFLOP/s of the floor's one product
-// per operand, tensor pipe 62 % busy; over 8148 4-bit slots 480 us, 436 TFLOP/s, 67 %.
+// under a 4096-token window, bf16: 220 us in the main kernel, 546 TFLOP/s of the floor's one product
+// per operand, tensor pipe 66 % busy; over 8148 4-bit slots 484 us, 432 TFLOP/s, 70 %. (The code of wide
+// blocks, which no block of these needs, takes 2 % of the first by its mere presence. With every block wide the
+// two take 561 and 1004 us with their launches instead of 224 and 461.)
 // The main kernel starts while the planes are written (its CTAs set up and bring q), and waits for
 // that grid's end before it reads them (a prompt of 1501 rows: 47 -> 43 us with its launches).
 #include "rows_attn_tc.cuh"
@@ -39,7 +41,7 @@ namespace dllm {
 namespace {
 
 // ---- K and V as fp16 planes ------------------------------------------------------------------
-constexpr int kPlaneEach = 2;  // units of 8 dims per thread (8 and 256 threads per block: 15 us for 400 blocks, 10 so)
+constexpr int kPlaneEach = 2;  // units of 8 dims per thread (8 and 256 threads per block: 15 us for 400 blocks, 10 so; 11 with the slots' maxima)
 template <int KIND, int HD>
 constexpr int kPlaneThreads = TcTile<KIND, HD>::BN * (HD / 8) / kPlaneEach;
 
@@ -528,7 +530,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) rows_tc_kernel(const __grid_con
           }
         }
         x = fmaxf(max3(x, x1, x2), x3) * f;
-        // p is 2^(x - m + 8) with scores x up to m + 7: m is the row's maximum at a time, and moves (with
+        // p is 2^(x - m + 8) with scores x up to m + 7: m is the row's maximum at a time, and moves late (with
         // l and o) only when a score exceeds that. (m + 7 could round up, and p then leave fp16's range.)
         if (__any_sync(0xffffffffu, x - m > 7.f)) {
           const float to = fmaxf(m, x), g = to == -INFINITY ? 1.f : ex2(m - to);

@@ -20,9 +20,8 @@ struct TcTile {
   static constexpr int kTile = BOX * kBox;               // of a K or V block, and of one term of 128 rows of q
   static constexpr int kRing = HD == 64 ? 6 : 3;         // K and V blocks under way
   static constexpr int kTurns = (kRing + 1) / 2;
-  static constexpr int kOut = kTcTileRows * (HD + 6) * 4;  // the results, over q and the ring
   static constexpr int kSmem = (4 + kRing) * kTile;
-  static_assert(kOut <= (4 + kRing) * kTile, "results reuse the operands' memory");
+  static_assert(128 * HD * 4 <= 2 * kTile, "the results of 128 rows pass through the memory of their q");
   static_assert(kSmem + 2048 <= 227 * 1024, "shared memory");
 };
 inline int tc_block(int kind) { return kind == kKvBf16 ? 128 : 64; }

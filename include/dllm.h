@@ -450,8 +450,9 @@ void dllm_rows_destroy(dllm_rows* rows);
 int dllm_stage_append_rows(dllm_stage* st, int layer, const dllm_rows* rows, const dllm_buf* k, const dllm_buf* v);
 /* out[row] = attention of the row at slot p = T0 + j (q [n, NQ*HD], after RoPE) over its
  * sequence's slots s <= p with s > p - window or s < sinks; window 0: all of them. The rows'
- * own K/V are in the cache before. A non-finite K/V value reaches only the rows that see it
- * (there an infinity may come out as NaN). */
+ * own K/V are in the cache before. Fp32 arithmetic: products keep 22 bits of q, of p, and of the largest
+ * fp32 value of each K or V row. A K/V value reaches only the rows that see it, whatever its size (an
+ * infinity may come out as NaN there). */
 int dllm_stage_window_attention(dllm_stage* st, int layer, const dllm_rows* rows, const dllm_buf* q, dllm_buf* out,
                                 int window, int sinks);
 
